@@ -9,7 +9,8 @@ from . import _lib
 _lib.load()
 
 from . import ivf_pq  # noqa: E402
+from . import kv_cache  # noqa: E402
 from .refine import refine  # noqa: E402
 from .common import Resources  # noqa: E402
 
-__all__ = ["ivf_pq", "refine", "Resources"]
+__all__ = ["ivf_pq", "kv_cache", "refine", "Resources"]

@@ -191,6 +191,14 @@ SIGNATURES = {
                                         C.c_int],
     "cuvsRefine": [C.c_size_t, _P(DLManagedTensor), _P(DLManagedTensor), _P(DLManagedTensor), C.c_int,
                    _P(DLManagedTensor), _P(DLManagedTensor)],
+    "cuvsKvCacheAppend": [C.c_size_t, *[_P(DLManagedTensor)] * 9, C.c_bool, *[_P(DLManagedTensor)] * 2],
+    "cuvsKvCacheAttention": [C.c_size_t, *[_P(DLManagedTensor)] * 5, C.c_float, C.c_int64, FilterStruct,
+                             *[_P(DLManagedTensor)] * 3],
+    "cuvsKvCacheAttentionWorkspace": [C.c_size_t, *[_P(DLManagedTensor)] * 3, C.c_int64, _P(C.c_size_t)],
+    "cuvsKvCacheAttendCandidates": [C.c_size_t, *[_P(DLManagedTensor)] * 4, C.c_float, FilterStruct, *[_P(DLManagedTensor)] * 2],
+    "cuvsKvCacheMergeParts": [C.c_size_t, *[_P(DLManagedTensor)] * 4],
+    "cuvsB200KvCacheArrays": [C.c_size_t, C.c_void_p, C.c_int, C.c_void_p, C.c_int64, C.c_bool],
+    "cuvsB200KvCacheCheck": [C.c_int, C.c_int, C.c_void_p, C.c_int64],
     "cuvsIvfPqTransform": [C.c_size_t, _P(IndexStruct), _P(DLManagedTensor), _P(DLManagedTensor),
                            _P(DLManagedTensor)],
     "cuvsMultiGpuResourcesCreate": [_P(C.c_size_t)],
