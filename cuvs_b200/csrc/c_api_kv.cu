@@ -36,21 +36,24 @@ tensor describe(const DLManagedTensor* mt, const char* name)
   return t;
 }
 
-constexpr int64_t kWords = 11;
-
-tensor describe(const int64_t* w, const char* name)
+// From words: ndim | type code << 32 | bits << 40 (0: not given), address, device, shape, strides.
+tensor describe(const int64_t*& w, const int64_t* end, const char* name)
 {
   tensor t;
-  t.ndim = int(w[1] & 0xFF);
-  if (t.ndim == 0) { return t; }
-  CUVS_EXPECTS(t.ndim <= 4, "%s: 1 to 4 dimensions, not %d", name, t.ndim);
+  CUVS_EXPECTS(w < end, "the words do not describe the call");
+  const int64_t kind = *w++;
+  if (kind == 0) { return t; }
+  t.ndim = int(kind & 0xFF);
+  CUVS_EXPECTS(t.ndim >= 1 && t.ndim <= 4, "%s: 1 to 4 dimensions, not %d", name, t.ndim);
+  CUVS_EXPECTS(end - w >= 2 + 2 * t.ndim, "the words do not describe the call");
+  t.code        = int((kind >> 32) & 0xFF);
+  t.bits        = int((kind >> 40) & 0xFF);
   t.data        = reinterpret_cast<char*>(w[0]);
-  t.code        = int((w[1] >> 32) & 0xFF);
-  t.bits        = int((w[1] >> 40) & 0xFF);
-  t.device_type = int(w[2] & 0xFFFFFFFF);
-  t.device_id   = int(w[2] >> 32);
-  std::copy(w + 3, w + 7, t.shape);
-  std::copy(w + 7, w + 11, t.stride);
+  t.device_type = int(w[1] & 0xFFFFFFFF);
+  t.device_id   = int(w[1] >> 32);
+  std::copy(w + 2, w + 2 + t.ndim, t.shape);
+  std::copy(w + 2 + t.ndim, w + 2 + 2 * t.ndim, t.stride);
+  w += 2 + 2 * t.ndim;
   return t;
 }
 
@@ -394,6 +397,21 @@ kv::merge_args merge_of(int device, tensor* t)
   return a;
 }
 
+void workspace_of(resources& res, tensor* t, int64_t window, size_t* bytes)
+{
+  enum { KEYS, QUERIES, PAGES };
+  CUVS_EXPECTS(bytes != nullptr, "null output pointer");
+  kv::elem type;
+  tensor values          = t[KEYS];
+  const kv::cache_view c = cache_of(res.device, t[KEYS], values, {}, type);
+  rows_of(res.device, t[QUERIES], type, c, -1, -1, "queries");
+  uint32_t n, width;
+  int64_t stride;
+  pages_of(res.device, t[PAGES], n, width, stride);
+  CUVS_EXPECTS(window >= 0, "window must not be negative");
+  *bytes = kv::attention_workspace(res, type, n, query_heads_of(t[QUERIES], c), c.n_heads, c.dim, uint64_t(width) * c.page_size, window);
+}
+
 resources& single_device(cuvsResources_t res)
 {
   resources* r = res_of(res);
@@ -437,18 +455,8 @@ extern "C" cuvsError_t cuvsKvCacheAttentionWorkspace(cuvsResources_t res, DLMana
                                                      DLManagedTensor* pages, int64_t window, size_t* bytes)
 {
   return translate_exceptions([=] {
-    CUVS_EXPECTS(bytes != nullptr, "null output pointer");
-    resources& r = single_device(res);
-    tensor k = describe(keys, "keys"), q = describe(queries, "queries"), p = describe(pages, "pages");
-    kv::elem type;
-    tensor v               = k;
-    const kv::cache_view c = cache_of(r.device, k, v, {}, type);
-    rows_of(r.device, q, type, c, -1, -1, "queries");
-    uint32_t n, width;
-    int64_t stride;
-    pages_of(r.device, p, n, width, stride);
-    CUVS_EXPECTS(window >= 0, "window must not be negative");
-    *bytes = kv::attention_workspace(r, type, n, query_heads_of(q, c), c.n_heads, c.dim, uint64_t(width) * c.page_size, window);
+    tensor t[] = {describe(keys, "keys"), describe(queries, "queries"), describe(pages, "pages")};
+    workspace_of(single_device(res), t, window, bytes);
   });
 }
 
@@ -493,9 +501,10 @@ struct call {
       {"keys", "values", "queries", "candidates", "filter", "out", "lse"},
       {"parts", "parts_lse", "out", "lse"}};
     CUVS_EXPECTS(op >= 0 && op < 4 && words != nullptr, "unknown call %d", op);
-    CUVS_EXPECTS(n_words == n_tensors[op] * kWords + n_scalars[op], "%lld words do not describe call %d", (long long)n_words, op);
-    for (int i = 0; i < n_tensors[op]; i++) { t[i] = describe(words + i * kWords, names[op][i]); }
-    const int64_t* scalars = words + n_tensors[op] * kWords;
+    const int64_t* end = words + n_words;
+    for (int i = 0; i < n_tensors[op]; i++) { t[i] = describe(words, end, names[op][i]); }
+    CUVS_EXPECTS(end - words == n_scalars[op], "the words do not describe the call");
+    const int64_t* scalars = words;
     if (op == 0) { interleaved = scalars[0] != 0; }
     if (op == 1) { window = scalars[0]; }
     if (op == 1 || op == 2) {
@@ -526,6 +535,19 @@ extern "C" cuvsError_t cuvsB200KvCacheArrays(cuvsResources_t res, cudaStream_t s
       default: kv::merge_parts(r, merge_of(r.device, c.t));
     }
     if (sync) { r.sync(); }
+  });
+}
+
+extern "C" cuvsError_t cuvsB200KvCacheWorkspaceArrays(cuvsResources_t res, const int64_t* words, int64_t n_words, size_t* bytes)
+{
+  return translate_exceptions([=] {
+    CUVS_EXPECTS(words != nullptr, "null words");
+    const int64_t *at = words, *end = words + n_words;
+    tensor t[3];
+    static const char* const names[] = {"keys", "queries", "pages"};
+    for (int i = 0; i < 3; i++) { t[i] = describe(at, end, names[i]); }
+    CUVS_EXPECTS(end - at == 1, "the words do not describe the call");
+    workspace_of(single_device(res), t, *at, bytes);
   });
 }
 

@@ -1,5 +1,4 @@
-// Attention of one query head over rows that lie anywhere in the cache: those that a search named (`attend_candidates`), or all of a
-// sequence's (`attention`).
+// Attention of one query head over the rows of the cache that a search named.
 //
 // One block per (token, query head).  A warp takes 32 rows of the list at a time: every lane finds the place of one of them, then groups
 // of lanes -- as many as a row has 16-byte pieces -- read four rows each, keys and values together, and carry a softmax of their own
@@ -14,40 +13,9 @@ namespace {
 
 constexpr int kWarps = 8;
 
-struct named_rows {  // what a search found
-  const int64_t* ids;
-  uint32_t n;  // per list
-  __device__ void range(const cache_view&, uint32_t, uint32_t& first, uint32_t& end) const
-  {
-    first = 0;
-    end   = n;
-  }
-  __device__ int64_t slot(const cache_view& c, uint32_t token, uint64_t list, uint32_t i) const
-  {
-    const int64_t id = ids[list * n + i];
-    return id >= 0 && id < c.n_slots ? id : -1;
-  }
-};
-
-struct sequence_rows {  // the last `window` positions of a sequence
-  const int32_t* pages;
-  const int32_t* lengths;
-  uint32_t width;
-  int64_t stride;
-  int64_t window;
-  __device__ void range(const cache_view& c, uint32_t token, uint32_t& first, uint32_t& end) const
-  {
-    attended(lengths[token], window, width, c.page_size, first, end);
-  }
-  __device__ int64_t slot(const cache_view& c, uint32_t token, uint64_t, uint32_t i) const
-  {
-    return slot_of(pages + int64_t(token) * stride, width, int32_t(i), c.page_size, c.page_shift, c.n_pages);
-  }
-};
-
-template <typename T, int LANES, int PIECES, class Rows>
+template <typename T, int LANES, int PIECES>
 __global__ void __launch_bounds__(kWarps * 32)
-rows_kernel(cache_view c, Rows rows, rows_view queries, rows_view out, float* lse, uint32_t n_query_heads, float scale_log2)
+rows_kernel(cache_view c, const int64_t* __restrict__ candidates, uint32_t n_candidates, rows_view queries, rows_view out, float* lse, uint32_t n_query_heads, float scale_log2)
 {
   chain_begin();
   constexpr int E      = kPerPiece<T>;
@@ -75,13 +43,11 @@ rows_kernel(cache_view c, Rows rows, rows_view queries, rows_view out, float* ls
   }
   float top = -INFINITY, sum = 0.0f;
   float acc[PIECES][E] = {};
-  uint32_t first, end;
-  rows.range(c, token, first, end);
-  for (uint64_t base = uint64_t(first) + warp * 32u; base < end; base += kWarps * 32u) {
+  for (uint32_t base = warp * 32u; base < n_candidates; base += kWarps * 32u) {
     int64_t k_at = -1, v_at = 0;
-    if (base + lane < end) {
-      const int64_t slot = rows.slot(c, token, list, uint32_t(base) + lane);
-      if (slot >= 0 && slot_allowed(c, slot)) {
+    if (base + lane < n_candidates) {
+      const int64_t slot = candidates[list * n_candidates + base + lane];
+      if (slot >= 0 && slot < c.n_slots && slot_allowed(c, slot)) {
         int64_t page;
         uint32_t place;
         split_slot(c, slot, page, place);
@@ -195,55 +161,39 @@ rows_kernel(cache_view c, Rows rows, rows_view queries, rows_view out, float* ls
   if (threadIdx.x == 0) { lse[list] = (safe + log2f(total)) * kLn2; }
 }
 
-template <typename T, class Rows>
-void launch(resources& res, const cache_view& c, const Rows& rows, const rows_view& queries, const rows_view& out, float* lse, uint32_t n_tokens,
-            uint32_t n_query_heads, float scale)
+template <typename T>
+void launch(resources& res, const candidates_args& a)
 {
-  const uint32_t pieces = c.dim / kPerPiece<T>;
+  const uint32_t pieces = a.cache.dim / kPerPiece<T>;
   auto go               = [&](auto kernel) {
-    launch_chained(kernel, dim3(n_tokens * n_query_heads), kWarps * 32, 0, res.stream, c, rows, queries, out, lse, n_query_heads,
-                   scale * kLog2E);
+    launch_chained(kernel, dim3(a.n_tokens * a.n_query_heads), kWarps * 32, 0, res.stream, a.cache, a.candidates, a.n_candidates, a.queries,
+                   a.out, a.lse, a.n_query_heads, a.scale * kLog2E);
     CUDA_TRY(cudaGetLastError());
   };
   if (pieces <= 4) {
-    go(rows_kernel<T, 4, 1, Rows>);
+    go(rows_kernel<T, 4, 1>);
   } else if (pieces <= 8) {
-    go(rows_kernel<T, 8, 1, Rows>);
+    go(rows_kernel<T, 8, 1>);
   } else if (pieces <= 16) {
-    go(rows_kernel<T, 16, 1, Rows>);
+    go(rows_kernel<T, 16, 1>);
   } else if (pieces <= 32) {
-    go(rows_kernel<T, 32, 1, Rows>);
+    go(rows_kernel<T, 32, 1>);
   } else if constexpr (sizeof(T) == 4) {
-    go(rows_kernel<T, 32, 2, Rows>);
+    go(rows_kernel<T, 32, 2>);
   }
   res.launches++;
-}
-
-template <class Rows>
-void launch_any(resources& res, elem type, const cache_view& c, const Rows& rows, const rows_view& queries, const rows_view& out, float* lse,
-                uint32_t n_tokens, uint32_t n_query_heads, float scale)
-{
-  if (n_tokens == 0) { return; }
-  switch (type) {
-    case elem::f16: return launch<__half>(res, c, rows, queries, out, lse, n_tokens, n_query_heads, scale);
-    case elem::bf16: return launch<__nv_bfloat16>(res, c, rows, queries, out, lse, n_tokens, n_query_heads, scale);
-    default: return launch<float>(res, c, rows, queries, out, lse, n_tokens, n_query_heads, scale);
-  }
 }
 
 }  // namespace
 
 void attend_candidates(resources& res, const candidates_args& a)
 {
-  launch_any(res, a.type, a.cache, named_rows{a.candidates, a.n_candidates}, a.queries, a.out, a.lse, a.n_tokens, a.n_query_heads, a.scale);
-}
-
-size_t attention_workspace(const resources&, elem, uint32_t, uint32_t, uint32_t, uint32_t, uint64_t, int64_t) { return 0; }
-
-void attention(resources& res, const attention_args& a)
-{
-  launch_any(res, a.type, a.cache, sequence_rows{a.pages, a.lengths, a.table_width, a.table_stride, a.window}, a.queries, a.out, a.lse, a.n_sequences,
-             a.n_query_heads, a.scale);
+  if (a.n_tokens == 0) { return; }
+  switch (a.type) {
+    case elem::f16: return launch<__half>(res, a);
+    case elem::bf16: return launch<__nv_bfloat16>(res, a);
+    default: return launch<float>(res, a);
+  }
 }
 
 }  // namespace cuvs_b200::kv

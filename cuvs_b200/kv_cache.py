@@ -21,79 +21,76 @@ wait for it unless ``sync=False``, which is what a captured call needs.
 """
 from __future__ import annotations
 
-import ctypes as C
 import struct
+from array import array
+from ctypes import c_size_t
 
 import torch
 
 from . import _lib as L
-from .common import Resources, default_resources
+from .common import Resources, _default_resources, default_resources
 
 # ndim | dtype code << 32 | bits << 40 | lanes << 48
 _WORD = {t: (code << 32) | (bits << 40) | (1 << 48)
          for t, code, bits in ((torch.float16, 2, 16), (torch.bfloat16, 4, 16), (torch.float32, 2, 32), (torch.float64, 2, 64),
                                (torch.int32, 0, 32), (torch.int64, 0, 64), (torch.uint32, 1, 32), (torch.uint8, 1, 8))}
-_PAD = [(0,) * n for n in range(5)]
-_ABSENT = (0,) * 11
 _APPEND, _ATTENTION, _CANDIDATES, _MERGE = range(4)
+_f32 = struct.Struct("<f")
+_u32 = struct.Struct("<I")
 
 
-def _words(tensors, device, scalars):
-    """The words that describe a call's tensors (the order of the C interface) and its scalars."""
+def _words(tensors, scalars):
+    """The words that describe a call's tensors (the order of the C interface) and its scalars.  One array of integers for all of
+    them: a descriptor structure for each took longer than the kernels of a small call."""
     words = []
     for t in tensors:
         if t is None:
-            words += _ABSENT
+            words.append(0)
             continue
         word, n, at = _WORD.get(t.dtype), t.dim(), t.get_device()
         if word is None:
             raise ValueError(f"unsupported element type {t.dtype}")
         if not 1 <= n <= 4:
             raise ValueError(f"tensors have 1 to 4 dimensions, not {n}")
-        pad = _PAD[4 - n]
-        words += (t.data_ptr(), word | n, (L.kDLCUDA | (at << 32)) if at >= 0 else L.kDLCPU, *t.shape, *pad, *t.stride(), *pad)
+        words += (word | n, t.data_ptr(), (at << 32) | L.kDLCUDA if at >= 0 else L.kDLCPU, *t.shape, *t.stride())
     words += scalars
-    return (C.c_int64 * len(words))(*words)
+    return array("q", words)
 
 
 def _bits(scale):
-    return struct.unpack("<I", struct.pack("<f", scale))[0]
+    return _u32.unpack(_f32.pack(scale))[0]
 
 
-class _Call:
-    """Where a call's work goes and where its results are allocated: the tensors' device and the stream of the handle."""
-
-    __slots__ = ("res", "stream", "device", "_scope")
-
-    def __init__(self, tensor, resources):
-        if not isinstance(tensor, torch.Tensor) or not tensor.is_cuda:
-            raise ValueError("expected CUDA tensors")
-        self.device = tensor.get_device()
-        self._scope = None
+def _handle(tensor, resources):
+    """The handle for a call on this tensor's device, and its stream."""
+    device = tensor.get_device() if type(tensor) is torch.Tensor or isinstance(tensor, torch.Tensor) else -1
+    if device < 0:
+        raise ValueError("expected CUDA tensors")
+    if resources is None:
+        resources = _default_resources.get(device)
         if resources is None:
-            if torch.cuda.current_device() == self.device:
-                resources = default_resources(self.device)
-            else:
-                with torch.cuda.device(self.device):
-                    resources = default_resources(self.device)
-        self.res = resources
-        self.stream = resources.stream_at_call(self.device)
-        if resources._fixed_stream is not None:
-            # results belong to the stream that writes them
-            self._scope = torch.cuda.stream(torch.cuda.ExternalStream(self.stream, device=self.device))
+            with torch.cuda.device(device):
+                resources = default_resources(device)
+    return resources, resources.stream_at_call(device)
 
-    def __enter__(self):
-        if self._scope is not None:
-            self._scope.__enter__()
-        return self
 
-    def __exit__(self, *what):
-        if self._scope is not None:
-            self._scope.__exit__(*what)
+def _empty(shape, dtype, tensor, resources, stream):
+    """A result on the tensor's device that belongs to the stream which writes it."""
+    if resources._fixed_stream is None:
+        return torch.empty(shape, dtype=dtype, device=tensor.device)
+    with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=tensor.device)):
+        return torch.empty(shape, dtype=dtype, device=tensor.device)
 
-    def run(self, op, tensors, scalars, sync):
-        words = _words(tensors, self.device, scalars)
-        L.check(L.load().cuvsB200KvCacheArrays(self.res.handle, self.stream, op, words, len(words), bool(sync)))
+
+def _call(resources, stream, op, tensors, scalars, sync):
+    words = _words(tensors, scalars)
+    at, n = words.buffer_info()
+    if _arrays(resources.handle, stream, op, at, n, sync) != L.CUVS_SUCCESS:
+        L.check(L.CUVS_ERROR)
+
+
+_arrays = L.load().cuvsB200KvCacheArrays
+_workspace = L.load().cuvsB200KvCacheWorkspaceArrays
 
 
 def append(keys, values, new_keys, new_values, pages, positions, sequences=None, queries=None, frequencies=None, interleaved=False,
@@ -111,13 +108,13 @@ def append(keys, values, new_keys, new_values, pages, positions, sequences=None,
 
     A token whose position is negative (padding), whose sequence does not exist or whose page is not in the cache gets slot -1 and is not
     written; the query row of a token with a negative position is copied as it is.  Two tokens of a call must not have the same slot."""
-    with _Call(keys, resources) as call:
-        if slots is None:
-            slots = torch.empty((new_keys.shape[0],), dtype=torch.int64, device=keys.device)
-        if queries is not None and rotated is None:
-            rotated = queries.new_empty(queries.shape)
-        call.run(_APPEND, (keys, values, new_keys, new_values, pages, positions, sequences, queries, frequencies, slots, rotated),
-                 (int(bool(interleaved)),), sync)
+    resources, stream = _handle(keys, resources)
+    if slots is None:
+        slots = _empty(new_keys.shape[:1], torch.int64, keys, resources, stream)
+    if queries is not None and rotated is None:
+        rotated = _empty(queries.shape, queries.dtype, keys, resources, stream)
+    _call(resources, stream, _APPEND, (keys, values, new_keys, new_values, pages, positions, sequences, queries, frequencies, slots, rotated),
+          (1 if interleaved else 0,), sync)
     return slots, rotated
 
 
@@ -135,23 +132,32 @@ def attention(keys, values, queries, pages, lengths, scale=None, window=None, fi
     one is allocated for the call."""
     if window is not None and window <= 0:
         raise ValueError("window must be positive, or None")
-    if scale is None:
-        scale = queries.shape[-1] ** -0.5
-    with _Call(keys, resources) as call:
-        if out is None:
-            out = queries.new_empty(queries.shape)
-        if lse is None:
-            lse = torch.empty(queries.shape[:2], dtype=torch.float32, device=keys.device)
-        if workspace is None:
-            need = _attention_workspace(call, keys, queries, pages, window)
-            if need:
-                workspace = torch.empty((need,), dtype=torch.uint8, device=keys.device)
-        call.run(_ATTENTION, (keys, values, queries, pages, lengths, filter, out, lse, workspace), (window or 0, _bits(scale)), sync)
+    resources, stream = _handle(keys, resources)
+    shape = queries.shape
+    if out is None:
+        out = _empty(shape, queries.dtype, keys, resources, stream)
+    if lse is None:
+        lse = _empty(shape[:2], torch.float32, keys, resources, stream)
+    if workspace is None:
+        need = _attention_workspace(resources, keys, queries, pages, window)
+        if need:
+            workspace = _empty((need,), torch.uint8, keys, resources, stream)
+    _call(resources, stream, _ATTENTION, (keys, values, queries, pages, lengths, filter, out, lse, workspace),
+          (window or 0, _bits(shape[-1] ** -0.5 if scale is None else scale)), sync)
     return out, lse
 
 
-def _attention_workspace(call, keys, queries, pages, window):
-    return 0
+def attention_workspace(keys, queries, pages, window=None, resources: Resources | None = None):
+    """Bytes of workspace that :func:`attention` needs for tensors of these shapes."""
+    return _attention_workspace(_handle(keys, resources)[0], keys, queries, pages, window)
+
+
+def _attention_workspace(resources, keys, queries, pages, window):
+    need = c_size_t()
+    words = _words((keys, queries, pages), (window or 0,))
+    at, n = words.buffer_info()
+    L.check(_workspace(resources.handle, at, n, need))
+    return need.value
 
 
 def attend_candidates(keys, values, queries, candidates, scale=None, filter=None, out=None, lse=None,
@@ -159,14 +165,14 @@ def attend_candidates(keys, values, queries, candidates, scale=None, filter=None
     """Attention of every query head of a token to the slots that its list names: ``candidates``, int64 ``[n_tokens, n_query_heads, k]``, as
     searches over the keys return them.  Ids that are no slots (the search's "no such neighbour", -1) and slots that ``filter`` leaves out
     are skipped; a slot that is named twice counts twice.  Returns ``(out, lse)`` as :func:`attention` does."""
-    if scale is None:
-        scale = queries.shape[-1] ** -0.5
-    with _Call(keys, resources) as call:
-        if out is None:
-            out = queries.new_empty(queries.shape)
-        if lse is None:
-            lse = torch.empty(queries.shape[:2], dtype=torch.float32, device=keys.device)
-        call.run(_CANDIDATES, (keys, values, queries, candidates, filter, out, lse), (_bits(scale),), sync)
+    resources, stream = _handle(keys, resources)
+    shape = queries.shape
+    if out is None:
+        out = _empty(shape, queries.dtype, keys, resources, stream)
+    if lse is None:
+        lse = _empty(shape[:2], torch.float32, keys, resources, stream)
+    _call(resources, stream, _CANDIDATES, (keys, values, queries, candidates, filter, out, lse),
+          (_bits(shape[-1] ** -0.5 if scale is None else scale),), sync)
     return out, lse
 
 
@@ -174,10 +180,11 @@ def merge_parts(parts, parts_lse, out=None, lse=None, resources: Resources | Non
     """Joins parts of one softmax over disjoint sets of rows: ``parts`` ``[n_parts, n_tokens, n_heads, dim]`` and their ``parts_lse``, float32
     ``[n_parts, n_tokens, n_heads]``, both of any strides between rows (blocks gathered from several GPUs, say).  Returns ``(out, lse)``.  A
     part whose lse is -inf is not read."""
-    with _Call(parts, resources) as call:
-        if out is None:
-            out = parts.new_empty(parts.shape[1:])
-        if lse is None:
-            lse = torch.empty(parts.shape[1:3], dtype=torch.float32, device=parts.device)
-        call.run(_MERGE, (parts, parts_lse, out, lse), (), sync)
+    resources, stream = _handle(parts, resources)
+    shape = parts.shape
+    if out is None:
+        out = _empty(shape[1:], parts.dtype, parts, resources, stream)
+    if lse is None:
+        lse = _empty(shape[1:3], torch.float32, parts, resources, stream)
+    _call(resources, stream, _MERGE, (parts, parts_lse, out, lse), (), sync)
     return out, lse

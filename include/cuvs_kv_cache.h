@@ -67,13 +67,15 @@ CUVS_EXPORT cuvsError_t cuvsKvCacheAttendCandidates(cuvsResources_t res, DLManag
 CUVS_EXPORT cuvsError_t cuvsKvCacheMergeParts(cuvsResources_t res, DLManagedTensor* parts, DLManagedTensor* parts_lse,
                                               DLManagedTensor* out, DLManagedTensor* lse);
 
-/* The calls above on arrays that are described by words: op 0 append, 1 attention, 2 attend candidates, 3 merge parts; the
- * tensors in the order of the calls, 11 words each (address; ndim | type code << 32 | bits << 40 | lanes << 48; device type | device
- * id << 32; 4 of the shape; 4 strides in elements), all 0 where there is none, a filter as a u32 tensor in the place of its
- * argument; behind them the scalars: {interleaved}, {window, bits of the f32 scale}, {bits of the scale}, {}.  Sets the handle's stream;
- * waits for the work if `sync`. */
+/* The calls above on arrays that are described by words: op 0 append, 1 attention, 2 attend candidates, 3 merge parts.  The
+ * tensors come in the order of the calls, each as ndim | type code << 32 | bits << 40 | lanes << 48; address; device type | device
+ * id << 32; the shape; the strides in elements -- or as one word 0 where there is none -- with a filter as a u32 tensor in the place
+ * of its argument; behind them the scalars: {interleaved}, {window, bits of the f32 scale}, {bits of the scale}, {}.  Sets the
+ * handle's stream; waits for the work if `sync`. */
 CUVS_EXPORT cuvsError_t cuvsB200KvCacheArrays(cuvsResources_t res, cudaStream_t stream, int op, const int64_t* words, int64_t n_words,
                                               bool sync);
+/* cuvsKvCacheAttentionWorkspace on the words of keys, queries, pages and {window}. */
+CUVS_EXPORT cuvsError_t cuvsB200KvCacheWorkspaceArrays(cuvsResources_t res, const int64_t* words, int64_t n_words, size_t* bytes);
 /* The checks of such a call alone, for a handle of `device`: touches no GPU and reads no tensor. */
 CUVS_EXPORT cuvsError_t cuvsB200KvCacheCheck(int device, int op, const int64_t* words, int64_t n_words);
 

@@ -63,8 +63,9 @@ def described(op):
 def check(op, changes=None, scalars=None):
     tensors, usual = described(op)
     tensors.update(changes or {})
-    words = kv_cache._words(tensors.values(), DEVICE, usual if scalars is None else scalars)
-    L.check(L.load().cuvsB200KvCacheCheck(DEVICE, op, words, len(words)))
+    words = kv_cache._words(tensors.values(), usual if scalars is None else scalars)
+    at, n = words.buffer_info()
+    L.check(L.load().cuvsB200KvCacheCheck(DEVICE, op, at, n))
 
 
 OPS = [kv_cache._APPEND, kv_cache._ATTENTION, kv_cache._CANDIDATES, kv_cache._MERGE]
@@ -185,9 +186,9 @@ def test_python_refuses_what_it_cannot_describe():
     with pytest.raises(ValueError, match="window"):
         kv_cache.attention(cpu, cpu, cpu[0], None, None, window=0)
     with pytest.raises(ValueError, match="element type"):
-        kv_cache._words([torch.zeros(3, dtype=torch.bool)], 0, ())
+        kv_cache._words([torch.zeros(3, dtype=torch.bool)], ())
     with pytest.raises(ValueError, match="dimensions"):
-        kv_cache._words([torch.zeros((1, 1, 1, 1, 1))], 0, ())
+        kv_cache._words([torch.zeros((1, 1, 1, 1, 1))], ())
 
 
 PLACES = r"""
