@@ -1,6 +1,11 @@
 // Joining parts of one softmax: parts o_p of disjoint sets of rows, each with the logarithm lse_p of its denominator, give
 //   lse = log sum_p exp(lse_p),   o = sum_p exp(lse_p - lse) o_p.
 // A part that attended to nothing (lse_p = -inf) has weight 0 and is not read.
+//
+// What bounds it: HBM (every part is read once, the result written once).  A group of lanes has a row: its lanes take the weights of as
+// many parts as there are lanes, one each, then all of them go through the parts, eight loads of 16 bytes in flight each.  The first
+// form, in which every lane formed every weight and waited for one part's row after the other, moved 3.7 TB/s (8 parts of 4,096 x 32
+// rows of 128 bf16: 83 us).
 #include "kv_rows.cuh"
 
 namespace cuvs_b200::kv {
@@ -9,52 +14,90 @@ namespace {
 
 constexpr int kThreads = 256;
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) merge_kernel(merge_args a, uint32_t log_lanes, uint32_t pieces)
+template <typename T, int LANES>
+__global__ void __launch_bounds__(kThreads) merge_kernel(merge_args a, uint32_t pieces)
 {
   chain_begin();
-  constexpr int E       = kPerPiece<T>;
-  const uint32_t lane   = threadIdx.x & ((1u << log_lanes) - 1u);
-  const uint64_t r      = (uint64_t(blockIdx.x) * kThreads + threadIdx.x) >> log_lanes;
-  if (r >= uint64_t(a.n_tokens) * a.n_heads) { return; }
-  const int64_t token = int64_t(r / a.n_heads), head = int64_t(r - uint64_t(token) * a.n_heads);
-  const float* lse    = a.parts_lse + token * a.l_row + head * a.l_head;
-  float top           = -INFINITY;
-  for (uint32_t p = 0; p < a.n_parts; p++) { top = fmaxf(top, lse[p * a.l_part]); }
+  constexpr int E         = kPerPiece<T>;
+  constexpr int AHEAD     = 8;
+  const uint32_t lane     = threadIdx.x % LANES;
+  const uint64_t asked    = (uint64_t(blockIdx.x) * kThreads + threadIdx.x) / LANES;
+  const uint64_t n_rows   = uint64_t(a.n_tokens) * a.n_heads;
+  const uint64_t r        = min(asked, n_rows - 1);  // groups behind the last row take part in the shuffles
+  const uint32_t token    = uint32_t(r / a.n_heads), head = uint32_t(r - uint64_t(token) * a.n_heads);
+  const float* lse        = a.parts_lse + int64_t(token) * a.l_row + int64_t(head) * a.l_head;
+  const char* rows        = a.parts + (int64_t(token) * a.p_row + int64_t(head) * a.p_head) * int64_t(sizeof(T));
+  const int64_t part_size = a.p_part * int64_t(sizeof(T));
+
+  float first = -INFINITY;  // of the first LANES parts, kept
+  float top   = -INFINITY;
+  for (uint32_t p = lane; p < a.n_parts; p += LANES) {
+    const float x = lse[int64_t(p) * a.l_part];
+    if (p == lane) { first = x; }
+    top = fmaxf(top, x);
+  }
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1) { top = fmaxf(top, __shfl_xor_sync(kAllLanes, top, o)); }
   top         = finite_top(top);
   float total = 0.0f;
-  for (uint32_t p = 0; p < a.n_parts; p++) { total += expf(lse[p * a.l_part] - top); }
-  const float scale = total == 0.0f ? 0.0f : 1.0f / total;
-  for (uint32_t j = lane; j < pieces; j += 1u << log_lanes) {
-    float acc[E] = {};
-#pragma unroll 4
-    for (uint32_t p = 0; p < a.n_parts; p++) {
-      const float w = expf(lse[p * a.l_part] - top);
-      if (w == 0.0f) { continue; }
-      const uint4 v = reinterpret_cast<const uint4*>(a.parts + (p * a.p_part + token * a.p_row + head * a.p_head) * int64_t(sizeof(T)))[j];
-      float x[E];
-      piece_to_floats<T>(v, x);
+  for (uint32_t p = lane; p < a.n_parts; p += LANES) { total += expf((p == lane ? first : lse[int64_t(p) * a.l_part]) - top); }
 #pragma unroll
-      for (int e = 0; e < E; e++) { acc[e] = fmaf(w, x[e], acc[e]); }
+  for (int o = LANES / 2; o > 0; o >>= 1) { total += __shfl_xor_sync(kAllLanes, total, o); }
+  const float scale = total == 0.0f ? 0.0f : 1.0f / total;
+
+  for (uint32_t j0 = 0; j0 < pieces; j0 += LANES) {
+    const uint32_t j = j0 + lane;
+    float acc[E]     = {};
+    for (uint32_t p0 = 0; p0 < a.n_parts; p0 += LANES) {
+      float mine = 0.0f;
+      if (p0 + lane < a.n_parts) { mine = expf((p0 == 0 ? first : lse[int64_t(p0 + lane) * a.l_part]) - top); }
+#pragma unroll 1
+      for (uint32_t q0 = 0; q0 < LANES && p0 + q0 < a.n_parts; q0 += AHEAD) {
+        uint4 v[AHEAD];
+        float w[AHEAD];
+#pragma unroll
+        for (int q = 0; q < AHEAD; q++) {
+          w[q] = __shfl_sync(kAllLanes, mine, (q0 + q) % LANES, LANES);
+          if (q0 + q >= LANES) { w[q] = 0.0f; }
+          v[q] = make_uint4(0, 0, 0, 0);
+          if (w[q] != 0.0f && j < pieces) { v[q] = __ldg(reinterpret_cast<const uint4*>(rows + (p0 + q0 + q) * part_size) + j); }
+        }
+#pragma unroll
+        for (int q = 0; q < AHEAD; q++) {
+          float x[E];
+          piece_to_floats<T>(v[q], x);
+#pragma unroll
+          for (int e = 0; e < E; e++) { acc[e] = fmaf(w[q], x[e], acc[e]); }
+        }
+      }
     }
 #pragma unroll
     for (int e = 0; e < E; e++) { acc[e] *= scale; }
-    reinterpret_cast<uint4*>(a.out.data + (token * a.out.row + head * a.out.head) * int64_t(sizeof(T)))[j] = floats_to_piece<T>(acc);
+    if (asked < n_rows && j < pieces) {
+      reinterpret_cast<uint4*>(a.out.data + (int64_t(token) * a.out.row + int64_t(head) * a.out.head) * int64_t(sizeof(T)))[j] =
+        floats_to_piece<T>(acc);
+    }
   }
-  if (lane == 0) { a.lse[r] = top + logf(total); }
+  if (asked < n_rows && lane == 0) { a.lse[r] = top + logf(total); }
 }
 
 template <typename T>
 void launch(resources& res, const merge_args& a)
 {
   const uint32_t pieces = a.dim / kPerPiece<T>;
-  uint32_t log_lanes    = 0;
-  while (log_lanes < 5 && (1u << log_lanes) < pieces) { log_lanes++; }
-  const uint64_t rows = uint64_t(a.n_tokens) * a.n_heads;
-  launch_chained(merge_kernel<T>, dim3(uint32_t(ceildiv<uint64_t>(rows, kThreads >> log_lanes))), kThreads, 0, res.stream, a, log_lanes,
-                 pieces);
-  CUDA_TRY(cudaGetLastError());
-  res.launches++;
+  const uint64_t rows   = uint64_t(a.n_tokens) * a.n_heads;
+  auto go               = [&](auto kernel, uint32_t lanes) {
+    launch_chained(kernel, dim3(uint32_t(ceildiv<uint64_t>(rows, kThreads / lanes))), kThreads, 0, res.stream, a, pieces);
+    CUDA_TRY(cudaGetLastError());
+    res.launches++;
+  };
+  if (pieces <= 8) {
+    go(merge_kernel<T, 8>, 8);
+  } else if (pieces <= 16) {
+    go(merge_kernel<T, 16>, 16);
+  } else {
+    go(merge_kernel<T, 32>, 32);
+  }
 }
 
 }  // namespace

@@ -21,8 +21,8 @@ wait for it unless ``sync=False``, which is what a captured call needs.
 """
 from __future__ import annotations
 
+import functools
 import struct
-from array import array
 from ctypes import c_size_t
 
 import torch
@@ -40,21 +40,27 @@ _u32 = struct.Struct("<I")
 
 
 def _words(tensors, scalars):
-    """The words that describe a call's tensors (the order of the C interface) and its scalars.  One array of integers for all of
-    them: a descriptor structure for each took longer than the kernels of a small call."""
+    """The words that describe a call's tensors (the order of the C interface) and its scalars, and how many they are.  One array of
+    integers for all of them: a descriptor structure for each took longer than the kernels of a small call."""
     words = []
     for t in tensors:
         if t is None:
             words.append(0)
             continue
-        word, n, at = _WORD.get(t.dtype), t.dim(), t.get_device()
+        shape, word, at = t.shape, _WORD.get(t.dtype), t.get_device()
         if word is None:
             raise ValueError(f"unsupported element type {t.dtype}")
-        if not 1 <= n <= 4:
-            raise ValueError(f"tensors have 1 to 4 dimensions, not {n}")
-        words += (word | n, t.data_ptr(), (at << 32) | L.kDLCUDA if at >= 0 else L.kDLCPU, *t.shape, *t.stride())
+        if not 1 <= len(shape) <= 4:
+            raise ValueError(f"tensors have 1 to 4 dimensions, not {len(shape)}")
+        words += (word | len(shape), t.data_ptr(), (at << 32) | L.kDLCUDA if at >= 0 else L.kDLCPU, *shape, *t.stride())
     words += scalars
-    return array("q", words)
+    n = len(words)
+    return _packer(n).pack(*words), n
+
+
+@functools.lru_cache(maxsize=256)
+def _packer(n):
+    return struct.Struct(f"{n}q")
 
 
 def _bits(scale):
@@ -63,7 +69,7 @@ def _bits(scale):
 
 def _handle(tensor, resources):
     """The handle for a call on this tensor's device, and its stream."""
-    device = tensor.get_device() if type(tensor) is torch.Tensor or isinstance(tensor, torch.Tensor) else -1
+    device = tensor.get_device() if isinstance(tensor, torch.Tensor) else -1
     if device < 0:
         raise ValueError("expected CUDA tensors")
     if resources is None:
@@ -74,18 +80,17 @@ def _handle(tensor, resources):
     return resources, resources.stream_at_call(device)
 
 
-def _empty(shape, dtype, tensor, resources, stream):
+def _empty(dtype, tensor, resources, stream, *shape):
     """A result on the tensor's device that belongs to the stream which writes it."""
     if resources._fixed_stream is None:
-        return torch.empty(shape, dtype=dtype, device=tensor.device)
+        return torch.empty(*shape, dtype=dtype, device=tensor.device)
     with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=tensor.device)):
-        return torch.empty(shape, dtype=dtype, device=tensor.device)
+        return torch.empty(*shape, dtype=dtype, device=tensor.device)
 
 
 def _call(resources, stream, op, tensors, scalars, sync):
-    words = _words(tensors, scalars)
-    at, n = words.buffer_info()
-    if _arrays(resources.handle, stream, op, at, n, sync) != L.CUVS_SUCCESS:
+    words, n = _words(tensors, scalars)
+    if _arrays(resources.handle, stream, op, words, n, sync) != L.CUVS_SUCCESS:
         L.check(L.CUVS_ERROR)
 
 
@@ -110,9 +115,9 @@ def append(keys, values, new_keys, new_values, pages, positions, sequences=None,
     written; the query row of a token with a negative position is copied as it is.  Two tokens of a call must not have the same slot."""
     resources, stream = _handle(keys, resources)
     if slots is None:
-        slots = _empty(new_keys.shape[:1], torch.int64, keys, resources, stream)
+        slots = _empty(torch.int64, keys, resources, stream, new_keys.shape[0])
     if queries is not None and rotated is None:
-        rotated = _empty(queries.shape, queries.dtype, keys, resources, stream)
+        rotated = _empty(queries.dtype, keys, resources, stream, *queries.shape)
     _call(resources, stream, _APPEND, (keys, values, new_keys, new_values, pages, positions, sequences, queries, frequencies, slots, rotated),
           (1 if interleaved else 0,), sync)
     return slots, rotated
@@ -135,13 +140,13 @@ def attention(keys, values, queries, pages, lengths, scale=None, window=None, fi
     resources, stream = _handle(keys, resources)
     shape = queries.shape
     if out is None:
-        out = _empty(shape, queries.dtype, keys, resources, stream)
+        out = _empty(queries.dtype, keys, resources, stream, *shape)
     if lse is None:
-        lse = _empty(shape[:2], torch.float32, keys, resources, stream)
+        lse = _empty(torch.float32, keys, resources, stream, *shape[:2])
     if workspace is None:
         need = _attention_workspace(resources, keys, queries, pages, window)
         if need:
-            workspace = _empty((need,), torch.uint8, keys, resources, stream)
+            workspace = _empty(torch.uint8, keys, resources, stream, need)
     _call(resources, stream, _ATTENTION, (keys, values, queries, pages, lengths, filter, out, lse, workspace),
           (window or 0, _bits(shape[-1] ** -0.5 if scale is None else scale)), sync)
     return out, lse
@@ -153,11 +158,20 @@ def attention_workspace(keys, queries, pages, window=None, resources: Resources 
 
 
 def _attention_workspace(resources, keys, queries, pages, window):
-    need = c_size_t()
-    words = _words((keys, queries, pages), (window or 0,))
-    at, n = words.buffer_info()
-    L.check(_workspace(resources.handle, at, n, need))
-    return need.value
+    # a function of these alone; asking for it takes as long as a launch
+    what = (keys.get_device(), keys.dtype, *keys.shape[1:], *queries.shape[:2], *pages.shape, window)
+    need = _workspaces.get(what)
+    if need is None:
+        size = c_size_t()
+        L.check(_workspace(resources.handle, *_words((keys, queries, pages), (window or 0,)), size))
+        need = size.value
+        if len(_workspaces) >= 4096:
+            _workspaces.clear()
+        _workspaces[what] = need
+    return need
+
+
+_workspaces = {}
 
 
 def attend_candidates(keys, values, queries, candidates, scale=None, filter=None, out=None, lse=None,
@@ -168,9 +182,9 @@ def attend_candidates(keys, values, queries, candidates, scale=None, filter=None
     resources, stream = _handle(keys, resources)
     shape = queries.shape
     if out is None:
-        out = _empty(shape, queries.dtype, keys, resources, stream)
+        out = _empty(queries.dtype, keys, resources, stream, *shape)
     if lse is None:
-        lse = _empty(shape[:2], torch.float32, keys, resources, stream)
+        lse = _empty(torch.float32, keys, resources, stream, *shape[:2])
     _call(resources, stream, _CANDIDATES, (keys, values, queries, candidates, filter, out, lse),
           (_bits(shape[-1] ** -0.5 if scale is None else scale),), sync)
     return out, lse
@@ -183,8 +197,8 @@ def merge_parts(parts, parts_lse, out=None, lse=None, resources: Resources | Non
     resources, stream = _handle(parts, resources)
     shape = parts.shape
     if out is None:
-        out = _empty(shape[1:], parts.dtype, parts, resources, stream)
+        out = _empty(parts.dtype, parts, resources, stream, *shape[1:])
     if lse is None:
-        lse = _empty(shape[1:3], torch.float32, parts, resources, stream)
+        lse = _empty(torch.float32, parts, resources, stream, *shape[1:3])
     _call(resources, stream, _MERGE, (parts, parts_lse, out, lse), (), sync)
     return out, lse

@@ -64,8 +64,7 @@ def check(op, changes=None, scalars=None):
     tensors, usual = described(op)
     tensors.update(changes or {})
     words = kv_cache._words(tensors.values(), usual if scalars is None else scalars)
-    at, n = words.buffer_info()
-    L.check(L.load().cuvsB200KvCacheCheck(DEVICE, op, at, n))
+    L.check(L.load().cuvsB200KvCacheCheck(DEVICE, op, *words))
 
 
 OPS = [kv_cache._APPEND, kv_cache._ATTENTION, kv_cache._CANDIDATES, kv_cache._MERGE]
