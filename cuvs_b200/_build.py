@@ -30,8 +30,9 @@ UNITS = [("resources.cu", "resources.o", []), ("index.cu", "index.o", []),
          ("label_tc.cu", "label_tc.o", []),
          ("dynamic_batching.cu", "dynamic_batching.o", []), ("mg.cu", "mg.o", []),
          ("c_api_mg.cu", "c_api_mg.o", []), ("c_api_kv.cu", "c_api_kv.o", []),
-         ("kv_append.cu", "kv_append.o", []), ("kv_attention.cu", "kv_attention.o", []), ("kv_rows.cu", "kv_rows.o", []),
+         ("kv_append.cu", "kv_append.o", []), ("kv_rows.cu", "kv_rows.o", []),
          ("kv_merge.cu", "kv_merge.o", [])]
+UNITS += [("kv_attention.cu", f"kv_attention_{name}.o", [f"-DKV_TYPE={t}"]) for name, t in (("f16", "__half"), ("bf16", "__nv_bfloat16"))]
 UNITS += [("scan_inst.cu", f"scan_{b}.o", [f"-DPQ_BITS={b}"]) for b in (4, 5, 6, 7, 8)]
 
 

@@ -12,143 +12,89 @@ namespace cuvs_b200::kv {
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kWarps = 8;
 
 // A row is cut into 16-byte pieces.  Where the halves that pair up start on piece boundaries (PAIRED), a step is two pieces, j and
-// j + half; else it is one piece, whose pairs lie inside it (adjacent pairs) or anywhere in the row (then one thread's store must not
-// be another's load: ANYWHERE reads all of a row's elements in a warp before it writes any).
+// j + half; else it is one piece, whose pairs lie inside it (ADJACENT) or anywhere in the row (ANYWHERE: then one lane's store must not
+// be another's load, and a warp reads all of a row's elements before it writes any).
 enum { ADJACENT = 0, PAIRED = 1, ANYWHERE = 2 };
 
+// A warp has a token, or some of its rows: its lanes take the token's angles, then go through the rows, each lane at the same pieces of every
+// row, so that it holds their sines and cosines in registers; four rows of a lane are in flight at a time.
+//
+// What bounds it: HBM.  Blocks that went through the rows of eight tokens with the angles in shared memory waited for those (four lanes on
+// one bank) and moved 5.2 TB/s: 20,000 tokens of 32 + 2 x 8 heads of 128 f16 92 us.
 template <typename T, int MODE>
-__global__ void __launch_bounds__(kThreads)
-append_kernel(append_args a, uint32_t tokens_per_block, uint32_t log_lanes, uint32_t steps)
+__global__ void __launch_bounds__(kWarps * 32)
+append_kernel(append_args a, uint32_t log_lanes, uint32_t steps, uint32_t slices, uint32_t rows_of_slice)
 {
   chain_begin();
-  constexpr int E = kPerPiece<T>;
-  extern __shared__ __align__(16) char smem[];
-  float2* turn     = reinterpret_cast<float2*>(smem);                                                    // [tokens][pairs] cos, sin
-  int64_t* s_slot  = reinterpret_cast<int64_t*>(smem + size_t(tokens_per_block) * a.n_pairs * sizeof(float2));
-  int32_t* s_pos   = reinterpret_cast<int32_t*>(s_slot + tokens_per_block);
-  const uint32_t t0 = blockIdx.x * tokens_per_block;
-  const uint32_t n  = min(tokens_per_block, a.n_tokens - t0);
-  for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
-    const int32_t pos  = a.positions[t0 + i];
-    const int64_t seq  = a.sequences ? int64_t(a.sequences[t0 + i]) : int64_t(t0 + i);
-    int64_t slot       = -1;
-    if (seq >= 0 && seq < int64_t(a.n_sequences)) {
-      slot = slot_of(a.pages + seq * a.table_stride, a.table_width, pos, a.cache.page_size, a.cache.page_shift, a.cache.n_pages);
-    }
-    s_slot[i] = slot;
-    s_pos[i]  = pos;
-    if (blockIdx.y == 0) { a.slots[t0 + i] = slot; }
+  constexpr int E     = kPerPiece<T>;
+  constexpr int AHEAD = 4;
+  extern __shared__ __align__(16) float2 s_turn[];
+  const uint32_t lane  = threadIdx.x & 31u;
+  float2* turn         = s_turn + (threadIdx.x >> 5) * a.n_pairs;  // cos, sin
+  const uint64_t task  = uint64_t(blockIdx.x) * kWarps + (threadIdx.x >> 5);
+  const uint32_t token = uint32_t(task / slices), slice = uint32_t(task - uint64_t(token) * slices);
+  if (token >= a.n_tokens) { return; }
+
+  const int32_t pos = a.positions[token];
+  const int64_t seq = a.sequences ? int64_t(a.sequences[token]) : int64_t(token);
+  int64_t slot      = -1;
+  if (seq >= 0 && seq < int64_t(a.n_sequences)) {
+    slot = slot_of(a.pages + seq * a.table_stride, a.table_width, pos, a.cache.page_size, a.cache.page_shift, a.cache.n_pages);
   }
-  for (uint32_t i = threadIdx.x; i < n * a.n_pairs; i += kThreads) {
-    const uint32_t token = i / a.n_pairs, pair = i - token * a.n_pairs;
-    const int32_t pos    = a.positions[t0 + token];
-    const double f       = a.frequencies_f32 ? double(static_cast<const float*>(a.frequencies)[pair])
-                                             : static_cast<const double*>(a.frequencies)[pair];
+  if (slice == 0 && lane == 0) { a.slots[token] = slot; }
+  int64_t page;
+  uint32_t place;
+  split_slot(a.cache, max(slot, int64_t(0)), page, place);
+  for (uint32_t pair = lane; pair < a.n_pairs; pair += 32) {
+    const double f = a.frequencies_f32 ? double(static_cast<const float*>(a.frequencies)[pair]) : static_cast<const double*>(a.frequencies)[pair];
     const double half_turns = double(max(pos, 0)) * f * 0.31830988618379067154;  // 1 / pi
-    const double whole      = 2.0 * rint(0.5 * half_turns);
     float s, c;
-    sincospif(float(half_turns - whole), &s, &c);
-    turn[i] = make_float2(c, s);
+    sincospif(float(half_turns - 2.0 * rint(0.5 * half_turns)), &s, &c);
+    turn[pair] = make_float2(c, s);
   }
-  __syncthreads();
+  __syncwarp();
 
   const uint32_t heads  = a.cache.n_heads;
-  const uint32_t rows   = a.n_query_heads + 2 * heads;
-  const uint32_t lane   = threadIdx.x & ((1u << log_lanes) - 1u);
-  const uint32_t stride = uint32_t(kThreads) >> log_lanes;
-  const uint32_t end    = n * rows;
-  for (uint32_t r0 = blockIdx.y * stride; r0 < end; r0 += gridDim.y * stride) {
-    const uint32_t r = r0 + (threadIdx.x >> log_lanes);
-    const bool here  = r < end;
-    const uint32_t i = here ? r / rows : 0u;
-    uint32_t head    = here ? r - i * rows : 0u;
-    const char* from = nullptr;
-    char* to         = nullptr;
-    bool turned      = s_pos[i] >= 0;
-    const size_t t   = t0 + i;
-    if (here) {
-      const int64_t slot = s_slot[i];
-      if (head < a.n_query_heads) {
-        from = a.queries.data + (int64_t(t) * a.queries.row + head * a.queries.head) * sizeof(T);
-        to   = a.rotated.data + (int64_t(t) * a.rotated.row + head * a.rotated.head) * sizeof(T);
-      } else {
-        head -= a.n_query_heads;
-        const bool value = head >= heads;
-        if (value) { head -= heads; }
-        if (slot >= 0) {
-          int64_t page;
-          uint32_t place;
-          split_slot(a.cache, slot, page, place);
-          if (value) {
-            turned = false;
-            from   = a.values + (int64_t(t) * a.v_row + head * a.v_head) * sizeof(T);
-            to     = const_cast<char*>(a.cache.values) +
-                 (page * a.cache.v_page + place * a.cache.v_token + head * a.cache.v_head) * sizeof(T);
-          } else {
-            from = a.keys + (int64_t(t) * a.k_row + head * a.k_head) * sizeof(T);
-            to   = const_cast<char*>(a.cache.keys) +
-                 (page * a.cache.k_page + place * a.cache.k_token + head * a.cache.k_head) * sizeof(T);
-          }
-        }
-      }
+  const uint32_t begin  = slice * rows_of_slice;
+  const uint32_t end    = min(begin + rows_of_slice, a.n_query_heads + 2 * heads);
+  const uint32_t gl     = lane & ((1u << log_lanes) - 1u);
+  const uint32_t stride = 32u >> log_lanes;
+  // where a row comes from and goes to; whether it is turned (values are not, nor is what has no position)
+  auto row_at = [&](uint32_t r, const char*& from, char*& to) -> bool {
+    from = nullptr;
+    if (r >= end) { return false; }
+    if (r < a.n_query_heads) {
+      from = a.queries.data + (int64_t(token) * a.queries.row + int64_t(r) * a.queries.head) * int64_t(sizeof(T));
+      to   = a.rotated.data + (int64_t(token) * a.rotated.row + int64_t(r) * a.rotated.head) * int64_t(sizeof(T));
+      return pos >= 0;
     }
-    const float2* angles = turn + i * a.n_pairs;
-    if constexpr (MODE == PAIRED) {
-      const uint32_t half = a.n_pairs / E;
-      for (uint32_t j = lane; j < steps; j += 1u << log_lanes) {
-        if (from == nullptr) { continue; }
-        if (j < half) {
-          uint4 lo = reinterpret_cast<const uint4*>(from)[j], hi = reinterpret_cast<const uint4*>(from)[j + half];
-          if (turned) {
-            float x[E], y[E];
-            piece_to_floats<T>(lo, x);
-            piece_to_floats<T>(hi, y);
-#pragma unroll
-            for (int e = 0; e < E; e++) {
-              const float2 cs = angles[j * E + e];
-              const float u   = x[e] * cs.x - y[e] * cs.y;
-              y[e]            = y[e] * cs.x + x[e] * cs.y;
-              x[e]            = u;
-            }
-            lo = floats_to_piece<T>(x);
-            hi = floats_to_piece<T>(y);
-          }
-          reinterpret_cast<uint4*>(to)[j]        = lo;
-          reinterpret_cast<uint4*>(to)[j + half] = hi;
-        } else {
-          reinterpret_cast<uint4*>(to)[j + half] = reinterpret_cast<const uint4*>(from)[j + half];
-        }
-      }
-    } else if constexpr (MODE == ADJACENT) {
-      for (uint32_t j = lane; j < steps; j += 1u << log_lanes) {
-        if (from == nullptr) { continue; }
-        uint4 w = reinterpret_cast<const uint4*>(from)[j];
-        if (turned && j * E < 2 * a.n_pairs) {
-          float x[E];
-          piece_to_floats<T>(w, x);
-#pragma unroll
-          for (int e = 0; e < E; e += 2) {
-            const uint32_t pair = (j * E + e) / 2;
-            if (pair < a.n_pairs) {
-              const float2 cs = angles[pair];
-              const float u   = x[e] * cs.x - x[e + 1] * cs.y;
-              x[e + 1]        = x[e + 1] * cs.x + x[e] * cs.y;
-              x[e]            = u;
-            }
-          }
-          w = floats_to_piece<T>(x);
-        }
-        reinterpret_cast<uint4*>(to)[j] = w;
-      }
-    } else {
+    if (slot < 0) { return false; }
+    const uint32_t h = r - a.n_query_heads;
+    if (h < heads) {
+      from = a.keys + (int64_t(token) * a.k_row + int64_t(h) * a.k_head) * int64_t(sizeof(T));
+      to   = const_cast<char*>(a.cache.keys) +
+           (page * a.cache.k_page + int64_t(place) * a.cache.k_token + int64_t(h) * a.cache.k_head) * int64_t(sizeof(T));
+      return true;
+    }
+    from = a.values + (int64_t(token) * a.v_row + int64_t(h - heads) * a.v_head) * int64_t(sizeof(T));
+    to   = const_cast<char*>(a.cache.values) +
+         (page * a.cache.v_page + int64_t(place) * a.cache.v_token + int64_t(h - heads) * a.cache.v_head) * int64_t(sizeof(T));
+    return false;
+  };
+
+  if constexpr (MODE == ANYWHERE) {
+    for (uint32_t r0 = begin; r0 < end; r0 += stride) {
+      const char* from;
+      char* to;
+      const bool turned = row_at(r0 + (lane >> log_lanes), from, to);
       // at most two pieces per lane (log_lanes is 5 for rows of more than 16 pieces); kept until the whole warp has read
       uint4 kept[2];
 #pragma unroll
       for (int u = 0; u < 2; u++) {
-        const uint32_t j = lane + (uint32_t(u) << log_lanes);
+        const uint32_t j = gl + (uint32_t(u) << log_lanes);
         if (from == nullptr || j >= steps) { continue; }
         kept[u] = reinterpret_cast<const uint4*>(from)[j];
         if (turned && j * E < 2 * a.n_pairs) {
@@ -158,11 +104,11 @@ append_kernel(append_args a, uint32_t tokens_per_block, uint32_t log_lanes, uint
           for (int e = 0; e < E; e++) {
             const uint32_t column = j * E + e;
             if (column < a.n_pairs) {
-              const float2 cs = angles[column];
-              x[e] = x[e] * cs.x - to_float(reinterpret_cast<const T*>(from)[column + a.n_pairs]) * cs.y;
+              const float2 cs = turn[column];
+              x[e]            = x[e] * cs.x - to_float(reinterpret_cast<const T*>(from)[column + a.n_pairs]) * cs.y;
             } else if (column < 2 * a.n_pairs) {
-              const float2 cs = angles[column - a.n_pairs];
-              x[e] = x[e] * cs.x + to_float(reinterpret_cast<const T*>(from)[column - a.n_pairs]) * cs.y;
+              const float2 cs = turn[column - a.n_pairs];
+              x[e]            = x[e] * cs.x + to_float(reinterpret_cast<const T*>(from)[column - a.n_pairs]) * cs.y;
             }
           }
           kept[u] = floats_to_piece<T>(x);
@@ -171,8 +117,66 @@ append_kernel(append_args a, uint32_t tokens_per_block, uint32_t log_lanes, uint
       __syncwarp();
 #pragma unroll
       for (int u = 0; u < 2; u++) {
-        const uint32_t j = lane + (uint32_t(u) << log_lanes);
+        const uint32_t j = gl + (uint32_t(u) << log_lanes);
         if (from != nullptr && j < steps) { reinterpret_cast<uint4*>(to)[j] = kept[u]; }
+      }
+    }
+  } else {
+    const uint32_t half = a.n_pairs / E;  // PAIRED: in pieces
+    for (uint32_t j = gl; j < steps; j += 1u << log_lanes) {
+      constexpr int PAIRS = MODE == PAIRED ? E : E / 2;  // of a step
+      const uint32_t pair = j * PAIRS;
+      const bool two      = MODE == PAIRED && j < half;
+      const uint32_t at   = MODE == PAIRED && !two ? j + half : j;
+      float2 cs[PAIRS];
+#pragma unroll
+      for (int e = 0; e < PAIRS; e++) { cs[e] = pair + e < a.n_pairs ? turn[pair + e] : make_float2(1.0f, 0.0f); }
+      for (uint32_t r0 = begin + (lane >> log_lanes); r0 < end; r0 += AHEAD * stride) {
+        uint4 lo[AHEAD], hi[MODE == PAIRED ? AHEAD : 1];
+        char* to[AHEAD];
+        bool there[AHEAD], turned[AHEAD];
+#pragma unroll
+        for (int u = 0; u < AHEAD; u++) {
+          const char* from;
+          turned[u] = row_at(r0 + u * stride, from, to[u]);
+          there[u]  = from != nullptr;
+          lo[u]     = load_piece(from + at * 16, there[u]);
+          if constexpr (MODE == PAIRED) { hi[u] = load_piece(from + (j + half) * 16, there[u] && two); }
+        }
+#pragma unroll
+        for (int u = 0; u < AHEAD; u++) {
+          if (turned[u] && pair < a.n_pairs) {
+            float x[E];
+            piece_to_floats<T>(lo[u], x);
+            if constexpr (MODE == PAIRED) {
+              float y[E];
+              piece_to_floats<T>(hi[u], y);
+#pragma unroll
+              for (int e = 0; e < E; e++) {
+                const float v = x[e] * cs[e].x - y[e] * cs[e].y;
+                y[e]          = y[e] * cs[e].x + x[e] * cs[e].y;
+                x[e]          = v;
+              }
+              hi[u] = floats_to_piece<T>(y);
+            } else {
+#pragma unroll
+              for (int e = 0; e < E; e += 2) {
+                if (pair + e / 2 < a.n_pairs) {
+                  const float v = x[e] * cs[e / 2].x - x[e + 1] * cs[e / 2].y;
+                  x[e + 1]      = x[e + 1] * cs[e / 2].x + x[e] * cs[e / 2].y;
+                  x[e]          = v;
+                }
+              }
+            }
+            lo[u] = floats_to_piece<T>(x);
+          }
+          if (there[u]) {
+            reinterpret_cast<uint4*>(to[u])[at] = lo[u];
+            if constexpr (MODE == PAIRED) {
+              if (two) { reinterpret_cast<uint4*>(to[u])[j + half] = hi[u]; }
+            }
+          }
+        }
       }
     }
   }
@@ -187,14 +191,15 @@ void launch(resources& res, const append_args& a)
   const uint32_t steps  = mode == PAIRED ? pieces - a.n_pairs / E : pieces;
   uint32_t log_lanes    = 0;
   while (log_lanes < 5 && (1u << log_lanes) < steps) { log_lanes++; }
-  // Tokens per block: as many as leave every SM several blocks, eight at most.
-  uint32_t per_block = 1;
-  while (per_block < 8 && a.n_tokens / (2 * per_block) >= uint32_t(res.sm_count) * 8) { per_block *= 2; }
-  const size_t smem = size_t(per_block) * (a.n_pairs * sizeof(float2) + sizeof(int64_t) + sizeof(int32_t));
-  const dim3 grid(ceildiv(a.n_tokens, per_block), 1);
-  auto go = [&](auto kernel) {
-    launch_chained(kernel, grid, kThreads, smem, res.stream, a, per_block, log_lanes, steps);
-    CUDA_TRY(cudaGetLastError());
+  // A token's rows go to several warps where tokens are few: until there are 16 warps per SM, or a warp has one turn of rows.
+  const uint32_t rows = a.n_query_heads + 2 * a.cache.n_heads, turn = 32u >> log_lanes;
+  uint32_t slices     = 1;
+  while (uint64_t(a.n_tokens) * slices * 2 <= uint64_t(res.sm_count) * 16 && rows > turn * slices) { slices *= 2; }
+  const uint32_t rows_of_slice = round_up(ceildiv(rows, slices), turn);
+  const size_t smem            = size_t(kWarps) * a.n_pairs * sizeof(float2);
+  auto go                      = [&](auto kernel) {
+    launch_chained(kernel, dim3(uint32_t(ceildiv<uint64_t>(uint64_t(a.n_tokens) * slices, kWarps))), kWarps * 32, smem, res.stream, a, log_lanes,
+                   steps, slices, rows_of_slice);
   };
   if (mode == PAIRED) {
     go(append_kernel<T, PAIRED>);

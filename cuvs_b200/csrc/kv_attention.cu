@@ -5,7 +5,7 @@
 // What bounds it: the rows are read once, 4 operations for each 16-bit key and value and query head, so with 8 query heads to a key head HBM
 // at 6.5 TB/s asks for 52 TFLOP/s: more than the FP32 pipes have left beside the conversions, a fraction of what mma.sync has, which
 // takes its operands from registers without tensor memory's detour.  Everything here serves keeping loads in flight.
-#include "kv_units.cuh"
+#include "kv_attention.hpp"
 
 #include <algorithm>
 #include <type_traits>
@@ -79,35 +79,35 @@ struct halves<__nv_bfloat16> {
 };
 
 // D: columns of a row in shared memory (64, 128, 256; what is behind the row's end is 0).  NT: query heads of a unit, in eights.
-template <int D, int NT>
+template <int D, int NT, int WARPS>
 struct mma_shape {
   static constexpr int kRows     = 8 * NT;
-  static constexpr int kTile     = kWarps * 16;
+  static constexpr int kTile     = WARPS * 16;
   static constexpr int kStages   = D == 64 ? 4 : D == 128 ? 2 : 3;
   static constexpr bool kQInRegs = D * NT <= 256;
-  static constexpr int kResident = D == 256 ? 1 : NT == 4 ? 2 : 3;  // blocks of an SM
+  static constexpr int kResident = WARPS == kLarge || D == 256 ? 1 : NT == 4 ? 2 : 3;  // blocks of an SM
   static constexpr int kRowBytes = D * 2;
   static constexpr int kStage    = 2 * 16 * kRowBytes;                       // 16 keys, 16 values
   static constexpr int kAccRow   = D + 4;                                    // floats: lanes of a store on different banks
-  static constexpr int kBuffers  = kWarps * kStages * kStage;
-  static constexpr int kAcc      = kWarps * kRows * kAccRow * 4;
+  static constexpr int kBuffers  = WARPS * kStages * kStage;
+  static constexpr int kAcc      = WARPS * kRows * kAccRow * 4;
   static constexpr int kQBytes   = kQInRegs ? 0 : kRows * kRowBytes;
   static constexpr int kStatsAt  = kBuffers > kAcc ? kBuffers : kAcc;
-  static constexpr int kJoinedAt = kStatsAt + kWarps * kRows * 8;
+  static constexpr int kJoinedAt = kStatsAt + WARPS * kRows * 8;
   static constexpr int kQAt      = kJoinedAt + kRows * 8;
   static constexpr int kMaskAt   = kQAt + kQBytes;
-  static constexpr int kShared   = kMaskAt + kWarps * kStages * 4;
+  static constexpr int kShared   = kMaskAt + WARPS * kStages * 4;
 };
 
 // Warps work alone: each has every fourth 16 positions of a unit, copies their rows ahead into its own part of shared memory, and keeps
 // its own top, sum and weighted sum.  Scores are formed as keys x queries (S^T: 16 keys by 8 query heads) and outputs as values x weights
 // (O^T: 16 columns by 8 heads), so that 8 query heads fill a product.  A thread of quad g, place t has keys g and g + 8 of heads 2t and
 // 2t + 1; turning its weights as a matrix makes them the second operand of the second product.
-template <typename T, int D, int NT, bool WHOLE_PAGES>
-__global__ void __launch_bounds__(kThreads, mma_shape<D, NT>::kResident)
+template <typename T, int D, int NT, int WARPS, bool WHOLE_PAGES>
+__global__ void __launch_bounds__(WARPS * 32, mma_shape<D, NT, WARPS>::kResident)
 mma_kernel(cache_view c, work_view w, positions lists, rows_view queries, result_view result, float scale_log2, parts_view parts)
 {
-  using shape       = mma_shape<D, NT>;
+  using shape       = mma_shape<D, NT, WARPS>;
   constexpr int S   = shape::kStages;
   constexpr int PR  = D / 8;  // pieces of a row in shared memory
   extern __shared__ __align__(128) char smem[];
@@ -121,7 +121,7 @@ mma_kernel(cache_view c, work_view w, positions lists, rows_view queries, result
   const uint32_t pieces  = c.dim / 8;
   chain_begin();
 
-  each_unit<T, shape::kTile>(
+  each_unit<T, WARPS, shape::kTile>(
     c, w, lists, result, parts, state,
     [&](uint32_t sequence, uint32_t unit, const positions::list& l, uint32_t tile0, uint32_t tile1) {
       const uint32_t head = unit / w.n_blocks_of, of = unit - head * w.n_blocks_of;
@@ -129,7 +129,7 @@ mma_kernel(cache_view c, work_view w, positions lists, rows_view queries, result
       const uint32_t head0 = head * w.group + of * shape::kRows;
       const char* keys     = c.keys + int64_t(head) * c.k_head * 2;
       const char* values   = c.values + int64_t(head) * c.v_head * 2;
-      row_stream<16, positions> stream(c, lists, l, warp, tile0, tile1);
+      row_stream<WARPS, 16, positions> stream(c, lists, l, warp, tile0, tile1);
       auto copy_rows = [&](uint32_t tile) {
         const uint32_t stage = (tile - tile0) % S;
         int64_t page;
@@ -190,7 +190,7 @@ mma_kernel(cache_view c, work_view w, positions lists, rows_view queries, result
           }
         }
       } else {
-        for (uint32_t i = threadIdx.x; i < uint32_t(shape::kRows * PR); i += kThreads) {
+        for (uint32_t i = threadIdx.x; i < uint32_t(shape::kRows * PR); i += WARPS * 32) {
           const uint32_t r = i / PR, piece = i % PR;
           uint4 x          = make_uint4(0, 0, 0, 0);
           if (r < rows && piece < pieces) {
@@ -331,63 +331,50 @@ mma_kernel(cache_view c, work_view w, positions lists, rows_view queries, result
     });
 }
 
-uint32_t padded(uint32_t dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
-
 }  // namespace
 
-plan attention16_plan(const resources& res, uint64_t sequences, uint32_t n_heads, uint32_t group, uint32_t dim, uint64_t most)
+// One object per type: KV_TYPE is __half or __nv_bfloat16.
+template <>
+void attention16<KV_TYPE>(resources& res, const attention_args& a, const plan& p, const work_view& w, const positions& lists,
+                          const result_view& result, const parts_view& parts)
 {
-  const uint32_t d = padded(dim);
-  const uint32_t nt = group <= 8 ? 1 : group <= 16 || d == 256 ? 2 : 4;
-  plan p{};
-  p.rows     = 8 * nt;
-  p.tile     = kWarps * 16;
-  p.resident = d == 256 ? 1 : nt == 4 ? 2 : 3;
-  deal_out(res, p, sequences * n_heads * ceildiv(group, p.rows), ceildiv<uint64_t>(most, p.tile));
-  return p;
-}
-
-void attention16(resources& res, const attention_args& a, const plan& p, const work_view& w, const positions& lists, const result_view& result,
-                 const parts_view& parts)
-{
-  auto pages = [&](auto type, auto d, auto nt) {
-    using T          = decltype(type);
-    constexpr int D  = decltype(d)::value;
-    constexpr int NT = decltype(nt)::value;
-    auto go          = [&](auto kernel) {
-      launch_units(res, kernel, p.blocks, p.cluster, mma_shape<D, NT>::kShared, a.cache, w, lists, a.queries, result, a.scale * kLog2E, parts);
+  using T     = KV_TYPE;
+  auto launch = [&](auto d, auto nt, auto warps) {
+    constexpr int D = decltype(d)::value, NT = decltype(nt)::value, WARPS = decltype(warps)::value;
+    auto go = [&](auto kernel) {
+      launch_units(res, kernel, p.blocks, WARPS * 32, p.cluster, mma_shape<D, NT, WARPS>::kShared, a.cache, w, lists, a.queries, result,
+                   a.scale * kLog2E, parts);
     };
     if (a.cache.page_size % 16 == 0) {
-      go(mma_kernel<T, D, NT, true>);
+      go(mma_kernel<T, D, NT, WARPS, true>);
     } else {
-      go(mma_kernel<T, D, NT, false>);
+      go(mma_kernel<T, D, NT, WARPS, false>);
     }
   };
-  auto any = [&](auto type) {
-    using std::integral_constant;
-    const uint32_t d = padded(a.cache.dim), nt = p.rows / 8;
-    auto by_rows = [&](auto cols) {
-      if (nt == 1) {
-        pages(type, cols, integral_constant<int, 1>{});
-      } else if (nt == 2) {
-        pages(type, cols, integral_constant<int, 2>{});
-      } else if constexpr (decltype(cols)::value <= 128) {
-        pages(type, cols, integral_constant<int, 4>{});
+  using std::integral_constant;
+  auto by_rows = [&](auto cols) {
+    constexpr int D = decltype(cols)::value;
+    auto by_warps   = [&](auto nt) {
+      if constexpr (has_large(D, decltype(nt)::value)) {
+        if (p.warps == uint32_t(kLarge)) { return launch(cols, nt, integral_constant<int, kLarge>{}); }
       }
+      launch(cols, nt, integral_constant<int, kSmall>{});
     };
-    if (d == 64) {
-      by_rows(integral_constant<int, 64>{});
-    } else if (d == 128) {
-      by_rows(integral_constant<int, 128>{});
-    } else {
-      by_rows(integral_constant<int, 256>{});
+    if (p.rows == 8) {
+      by_warps(integral_constant<int, 1>{});
+    } else if (p.rows == 16) {
+      by_warps(integral_constant<int, 2>{});
+    } else if constexpr (D <= 128) {
+      by_warps(integral_constant<int, 4>{});
     }
-    if (p.join) { launch_join<decltype(type)>(res, p, w, parts, a.cache.dim, a.cache.n_heads, result); }
   };
-  if (a.type == elem::f16) {
-    any(__half{});
+  const uint32_t d = padded(a.cache.dim);
+  if (d == 64) {
+    by_rows(integral_constant<int, 64>{});
+  } else if (d == 128) {
+    by_rows(integral_constant<int, 128>{});
   } else {
-    any(__nv_bfloat16{});
+    by_rows(integral_constant<int, 256>{});
   }
 }
 

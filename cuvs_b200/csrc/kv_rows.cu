@@ -4,43 +4,38 @@
 // What bounds it: HBM, through the bytes in flight: rows of a few hundred bytes that lie anywhere.  Every warp copies its rows into its own
 // part of shared memory a stage ahead; a group of lanes -- as many as a row has 16-byte pieces -- then reads them as registers and carries a
 // softmax of its own (running top, sum of weights, weighted sum of values), joined at the end.
-#include "kv_units.cuh"
+#include "kv_attention.hpp"
 
 #include <algorithm>
 #include <type_traits>
 
 namespace cuvs_b200::kv {
 
-// kv_attention.cu: 16-bit rows of sequences
-plan attention16_plan(const resources& res, uint64_t sequences, uint32_t n_heads, uint32_t group, uint32_t dim, uint64_t most);
-void attention16(resources& res, const attention_args& a, const plan& p, const work_view& w, const positions& lists, const result_view& result,
-                 const parts_view& parts);
-
 namespace {
 
 // LANES lanes have a row, PIECES 16-byte pieces each; R query heads share its reading.
-template <typename T, int LANES, int PIECES, int R>
+template <typename T, int LANES, int PIECES, int R, int WARPS>
 struct rows_shape {
   static constexpr int kPitch    = LANES * PIECES * 16;                    // bytes of a row in shared memory
   static constexpr int kChunk    = kPitch <= 128 ? 32 : 4096 / kPitch;     // rows of a warp's stage
   static constexpr int kStages   = kPitch < 128 ? 4 : 2;
-  static constexpr int kTile     = kWarps * kChunk;
+  static constexpr int kTile     = WARPS * kChunk;
   static constexpr int kGroups   = 32 / LANES;
   static constexpr int kTurns    = kChunk / kGroups;                       // rows of a lane group in a stage
   static constexpr int kColumns  = LANES * PIECES * kPerPiece<T>;
   static constexpr int kStage    = 2 * kChunk * kPitch;
-  static constexpr int kStatsAt  = kWarps * kStages * kStage;
-  static constexpr int kJoinedAt = kStatsAt + kWarps * R * 8;
+  static constexpr int kStatsAt  = WARPS * kStages * kStage;
+  static constexpr int kJoinedAt = kStatsAt + WARPS * R * 8;
   static constexpr int kMaskAt   = kJoinedAt + R * 8;
-  static constexpr int kShared   = kMaskAt + kWarps * kStages * 4;
-  static_assert(kWarps * R * kColumns * 4 <= kStatsAt, "the warps' sums take the stages' place");
+  static constexpr int kShared   = kMaskAt + WARPS * kStages * 4;
+  static_assert(WARPS * R * kColumns * 4 <= kStatsAt, "the warps' sums take the stages' place");
 };
 
-template <typename T, int LANES, int PIECES, int R, class Lists>
-__global__ void __launch_bounds__(kThreads, 3)
+template <typename T, int LANES, int PIECES, int R, int WARPS, class Lists>
+__global__ void __launch_bounds__(WARPS * 32, WARPS == kSmall ? 3 : 1)
 rows_kernel(cache_view c, work_view w, Lists lists, rows_view queries, result_view result, float scale_log2, parts_view parts)
 {
-  using shape          = rows_shape<T, LANES, PIECES, R>;
+  using shape          = rows_shape<T, LANES, PIECES, R, WARPS>;
   constexpr int E      = kPerPiece<T>;
   constexpr int S      = shape::kStages;
   constexpr int CHUNK  = shape::kChunk;
@@ -57,7 +52,7 @@ rows_kernel(cache_view c, work_view w, Lists lists, rows_view queries, result_vi
   const uint32_t pieces  = c.dim / E;
   chain_begin();
 
-  each_unit<T, shape::kTile>(
+  each_unit<T, WARPS, shape::kTile>(
     c, w, lists, result, parts, state,
     [&](uint32_t sequence, uint32_t unit, const typename Lists::list& l, uint32_t tile0, uint32_t tile1) {
       const uint32_t head = unit / w.n_blocks_of, of = unit - head * w.n_blocks_of;
@@ -65,7 +60,7 @@ rows_kernel(cache_view c, work_view w, Lists lists, rows_view queries, result_vi
       const uint32_t head0 = head * w.group + of * R;
       const char* keys     = c.keys + int64_t(head) * c.k_head * int64_t(sizeof(T));
       const char* values   = c.values + int64_t(head) * c.v_head * int64_t(sizeof(T));
-      row_stream<CHUNK, Lists> stream(c, lists, l, warp, tile0, tile1);
+      row_stream<WARPS, CHUNK, Lists> stream(c, lists, l, warp, tile0, tile1);
       auto advance = [&](uint32_t tile) {
         if (tile < tile1) {
           const uint32_t stage = (tile - tile0) % S;
@@ -235,11 +230,11 @@ void by_pieces(uint32_t pieces, Fn&& fn)
   }
 }
 
-uint32_t rows_tile(uint32_t pieces)
+uint32_t chunk_of(uint32_t pieces)
 {
-  uint32_t tile = 0;
-  by_pieces(pieces, [&](auto lanes, auto n) { tile = rows_shape<float, decltype(lanes)::value, decltype(n)::value, 1>::kTile; });
-  return tile;
+  uint32_t chunk = 0;
+  by_pieces(pieces, [&](auto lanes, auto n) { chunk = rows_shape<float, decltype(lanes)::value, decltype(n)::value, 1, kSmall>::kChunk; });
+  return chunk;
 }
 
 plan attention_plan(const resources& res, elem type, uint64_t sequences, uint32_t n_heads, uint32_t group, uint32_t dim, uint64_t capacity,
@@ -247,29 +242,52 @@ plan attention_plan(const resources& res, elem type, uint64_t sequences, uint32_
 {
   // a window may begin anywhere in 16 positions
   const uint64_t most = window > 0 && uint64_t(window) < capacity ? std::min(capacity, uint64_t(window) + 15) : capacity;
-  if (type != elem::f32) { return attention16_plan(res, sequences, n_heads, group, dim, most); }
   plan p{};
-  p.rows     = dim > 128 ? std::min(group, 4u) : group > 4 ? 8 : group;
-  p.rows     = p.rows == 3 ? 4 : p.rows;
-  p.tile     = rows_tile(dim / 4);
-  p.resident = 3;
-  deal_out(res, p, sequences * n_heads * ceildiv(group, p.rows), ceildiv<uint64_t>(most, p.tile));
+  bool large = true;
+  if (type == elem::f32) {
+    p.rows     = dim > 128 ? std::min(group, 4u) : group > 4 ? 8 : group;
+    p.rows     = p.rows == 3 ? 4 : p.rows;
+    p.chunk    = chunk_of(dim / 4);
+    p.resident = 3;
+  } else {
+    const uint32_t d = padded(dim), eights = group <= 8 ? 1 : group <= 16 || d == 256 ? 2 : 4;
+    p.rows     = 8 * eights;
+    p.chunk    = 16;
+    p.resident = d == 256 ? 1 : eights == 4 ? 2 : 3;
+    large      = has_large(d, eights);
+  }
+  deal_out(res, p, sequences * n_heads * ceildiv(group, p.rows), most, large, true);
   return p;
+}
+
+template <typename T, int LANES, int PIECES, int R, class Lists, typename... Args>
+void launch_rows(resources& res, const plan& p, Args&&... args)
+{
+  if (p.warps == uint32_t(kLarge)) {
+    launch_units(res, rows_kernel<T, LANES, PIECES, R, kLarge, Lists>, p.blocks, kLarge * 32, p.cluster,
+                 rows_shape<T, LANES, PIECES, R, kLarge>::kShared, args...);
+  } else {
+    launch_units(res, rows_kernel<T, LANES, PIECES, R, kSmall, Lists>, p.blocks, kSmall * 32, p.cluster,
+                 rows_shape<T, LANES, PIECES, R, kSmall>::kShared, args...);
+  }
 }
 
 template <typename T>
 void launch_candidates(resources& res, const candidates_args& a)
 {
-  const uint32_t group = a.n_query_heads / a.cache.n_heads;
-  const work_view w{a.n_tokens, a.n_query_heads, group, group, 1};
+  const uint32_t group = a.n_query_heads / a.cache.n_heads, pieces = a.cache.dim / kPerPiece<T>;
   const named_slots lists{a.candidates, a.n_candidates};
   parts_view parts{};
-  parts.rows = 1;
-  by_pieces(a.cache.dim / kPerPiece<T>, [&](auto lanes, auto n) {
+  plan p{};
+  p.rows = parts.rows = 1;
+  p.chunk             = chunk_of(pieces);
+  p.resident          = 3;
+  deal_out(res, p, uint64_t(a.n_tokens) * a.n_query_heads, a.n_candidates, true, false);
+  const work_view w{a.n_tokens, a.n_query_heads, group, group, p.cluster};
+  by_pieces(pieces, [&](auto lanes, auto n) {
     constexpr int LANES = decltype(lanes)::value, PIECES = decltype(n)::value;
     if constexpr (sizeof(T) == 4 || PIECES == 1) {
-      launch_units(res, rows_kernel<T, LANES, PIECES, 1, named_slots>, a.n_tokens * a.n_query_heads, 1, rows_shape<T, LANES, PIECES, 1>::kShared,
-                   a.cache, w, lists, a.queries, result_view{a.out, a.lse}, a.scale * kLog2E, parts);
+      launch_rows<T, LANES, PIECES, 1, named_slots>(res, p, a.cache, w, lists, a.queries, result_view{a.out, a.lse}, a.scale * kLog2E, parts);
     }
   });
 }
@@ -296,13 +314,22 @@ void attention(resources& res, const attention_args& a)
   parts_view parts{};
   if (p.join) { parts = parts_at(a.workspace, p.blocks, p.rows, c.dim); }
   parts.rows = p.rows;
-  if (a.type != elem::f32) { return attention16(res, a, p, w, lists, result, parts); }
+  auto join  = [&](auto type) {
+    if (p.join) { launch_join<decltype(type)>(res, p, w, parts, c.dim, c.n_heads, result); }
+  };
+  if (a.type == elem::f16) {
+    attention16<__half>(res, a, p, w, lists, result, parts);
+    return join(__half{});
+  }
+  if (a.type == elem::bf16) {
+    attention16<__nv_bfloat16>(res, a, p, w, lists, result, parts);
+    return join(__nv_bfloat16{});
+  }
   by_pieces(c.dim / 4, [&](auto lanes, auto n) {
     constexpr int LANES = decltype(lanes)::value, PIECES = decltype(n)::value;
     auto go = [&](auto r) {
       constexpr int R = decltype(r)::value;
-      launch_units(res, rows_kernel<float, LANES, PIECES, R, positions>, p.blocks, p.cluster, rows_shape<float, LANES, PIECES, R>::kShared, c, w, lists,
-                   a.queries, result, a.scale * kLog2E, parts);
+      launch_rows<float, LANES, PIECES, R, positions>(res, p, c, w, lists, a.queries, result, a.scale * kLog2E, parts);
     };
     using std::integral_constant;
     if (p.rows == 1) {
@@ -315,7 +342,7 @@ void attention(resources& res, const attention_args& a)
       go(integral_constant<int, 8>{});
     }
   });
-  if (p.join) { launch_join<float>(res, p, w, parts, c.dim, c.n_heads, result); }
+  join(float{});
 }
 
 void attend_candidates(resources& res, const candidates_args& a)

@@ -101,9 +101,17 @@ __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x)
   return __float2bfloat16_rn(x);
 }
 
-__device__ __forceinline__ bool slot_allowed(const cache_view& c, int64_t slot)
+// A 16-byte load that is made or not without a branch, so that several of them are in flight together; 0 where it is not made.
+__device__ __forceinline__ uint4 load_piece(const void* from, bool there)
 {
-  return c.filter == nullptr || ((c.filter[slot >> 5] >> (uint32_t(slot) & 31u)) & 1u) != 0u;
+  uint4 v;
+  asm volatile(
+    "{\n .reg .pred p;\n setp.ne.u32 p, %5, 0;\n mov.u32 %0, 0;\n mov.u32 %1, 0;\n mov.u32 %2, 0;\n mov.u32 %3, 0;\n"
+    " @p ld.global.v4.u32 {%0, %1, %2, %3}, [%4];\n}"
+    : "=&r"(v.x), "=&r"(v.y), "=&r"(v.z), "=&r"(v.w)
+    : "l"(from), "r"(uint32_t(there))
+    : "memory");
+  return v;
 }
 
 // Page and place in it of a position below 2^31 (or of a slot below 2^32).

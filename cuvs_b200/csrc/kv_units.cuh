@@ -20,8 +20,9 @@
 
 namespace cuvs_b200::kv {
 
-constexpr int kWarps   = 4;
-constexpr int kThreads = kWarps * 32;
+// Warps of a block: small blocks, several to an SM, balance best; where units are fewer than SMs, one large block has an SM's warps for one
+// unit.
+constexpr int kSmall = 4, kLarge = 12;
 
 struct work_view {
   uint32_t n_sequences;
@@ -204,22 +205,22 @@ struct block_state {
 
 // Joins the warps: the block's sums become output rows (whole), a part in the workspace, or warp 0's sums (for the cluster).
 enum { TO_OUTPUT, TO_PART, TO_CLUSTER };
-template <typename T>
+template <typename T, int WARPS>
 __device__ __forceinline__ void join_warps(const cache_view& c, const work_view& w, const block_state& s, uint32_t rows, uint32_t sequence,
                                            uint32_t head0, const result_view& result, int to, const parts_view& parts, uint32_t part)
 {
   constexpr uint32_t E  = kPerPiece<T>;
   const uint32_t pieces = c.dim / E;
-  for (uint32_t i = threadIdx.x; i < rows * pieces; i += kThreads) {
+  for (uint32_t i = threadIdx.x; i < rows * pieces; i += WARPS * 32) {
     const uint32_t r = i / pieces, piece = i - r * pieces;
     float top = -INFINITY;
 #pragma unroll
-    for (int v = 0; v < kWarps; v++) { top = fmaxf(top, s.stats[v * parts.rows + r].x); }
+    for (int v = 0; v < WARPS; v++) { top = fmaxf(top, s.stats[v * parts.rows + r].x); }
     const float safe = finite_top(top);
     float sum        = 0.0f;
     float x[E]       = {};
 #pragma unroll
-    for (int v = 0; v < kWarps; v++) {
+    for (int v = 0; v < WARPS; v++) {
       const float2 st = s.stats[v * parts.rows + r];
       const float f   = exp2f(st.x - safe);
       sum             = fmaf(st.y, f, sum);
@@ -250,7 +251,7 @@ __device__ __forceinline__ void join_warps(const cache_view& c, const work_view&
 }
 
 // Joins the blocks of a cluster, whose sums lie in warp 0's place of each: every block writes a share of the output.
-template <typename T>
+template <typename T, int WARPS>
 __device__ __forceinline__ void join_cluster(const cache_view& c, const work_view& w, const block_state& s, uint32_t rows, uint32_t sequence,
                                              uint32_t head0, const result_view& result)
 {
@@ -258,7 +259,7 @@ __device__ __forceinline__ void join_cluster(const cache_view& c, const work_vie
   const uint32_t pieces = c.dim / E;
   auto cluster          = cooperative_groups::this_cluster();
   cluster.sync();
-  for (uint32_t i = cluster.block_rank() * kThreads + threadIdx.x; i < rows * pieces; i += w.cluster * kThreads) {
+  for (uint32_t i = cluster.block_rank() * (WARPS * 32) + threadIdx.x; i < rows * pieces; i += w.cluster * (WARPS * 32)) {
     const uint32_t r = i / pieces, piece = i - r * pieces;
     float top = -INFINITY;
     for (uint32_t v = 0; v < w.cluster; v++) { top = fmaxf(top, cluster.map_shared_rank(s.joined, v)[r].x); }
@@ -290,7 +291,7 @@ __device__ __forceinline__ void join_cluster(const cache_view& c, const work_vie
 }
 
 // Rows of sequences that attend to nothing: they have no tiles in any share.
-template <typename T, int TILE, class Lists>
+template <typename T, int WARPS, int TILE, class Lists>
 __device__ __forceinline__ void empty_rows(const cache_view& c, const work_view& w, const Lists& lists, const result_view& result)
 {
   constexpr uint32_t E   = kPerPiece<T>;
@@ -299,15 +300,15 @@ __device__ __forceinline__ void empty_rows(const cache_view& c, const work_view&
   for (uint32_t b = blockIdx.x; b < w.n_sequences; b += gridDim.x) {
     typename Lists::list l;
     if (lists.open(c, b, TILE, l) != 0u) { continue; }
-    for (uint32_t i = threadIdx.x; i < heads * (c.dim / E); i += kThreads) {
+    for (uint32_t i = threadIdx.x; i < heads * (c.dim / E); i += WARPS * 32) {
       store_piece<T>(result.out, b, i / (c.dim / E), i % (c.dim / E), nothing);
     }
-    for (uint32_t i = threadIdx.x; i < heads; i += kThreads) { result.lse[size_t(b) * heads + i] = -INFINITY; }
+    for (uint32_t i = threadIdx.x; i < heads; i += WARPS * 32) { result.lse[size_t(b) * heads + i] = -INFINITY; }
   }
 }
 
 // Goes through what the block has to do, unit by unit: body(sequence, unit, list, tile0, tile1) leaves its warps' state in shared memory.
-template <typename T, int TILE, class Lists, class Body>
+template <typename T, int WARPS, int TILE, class Lists, class Body>
 __device__ __forceinline__ void each_unit(const cache_view& c, const work_view& w, const Lists& lists, const result_view& result,
                                           const parts_view& parts, const block_state& s, Body&& body)
 {
@@ -353,12 +354,12 @@ __device__ __forceinline__ void each_unit(const cache_view& c, const work_view& 
     const uint32_t rows = min(parts.rows, w.group - of * parts.rows), head0 = head * w.group + of * parts.rows;
     __syncthreads();
     if (w.cluster > 1u) {
-      join_warps<T>(c, w, s, rows, sequence, head0, result, TO_CLUSTER, parts, 0);
-      join_cluster<T>(c, w, s, rows, sequence, head0, result);
+      join_warps<T, WARPS>(c, w, s, rows, sequence, head0, result, TO_CLUSTER, parts, 0);
+      join_cluster<T, WARPS>(c, w, s, rows, sequence, head0, result);
       return;
     }
     const bool whole = w.cluster == 1u || (at == begin && last == begin + n);
-    join_warps<T>(c, w, s, rows, sequence, head0, result, whole ? TO_OUTPUT : TO_PART, parts, 2 * blockIdx.x + (at == begin ? 1u : 0u));
+    join_warps<T, WARPS>(c, w, s, rows, sequence, head0, result, whole ? TO_OUTPUT : TO_PART, parts, 2 * blockIdx.x + (at == begin ? 1u : 0u));
     __syncthreads();
     if (at == begin && !whole) {
       unfinished = begin + n;
@@ -376,7 +377,7 @@ __device__ __forceinline__ void each_unit(const cache_view& c, const work_view& 
       parts.unit[1] = all.blocks;
     }
   }
-  empty_rows<T, TILE>(c, w, lists, result);
+  empty_rows<T, WARPS, TILE>(c, w, lists, result);
 }
 
 // ---- joining parts ------------------------------------------------------------------------------------------------------------
@@ -490,7 +491,7 @@ __device__ __forceinline__ void copies_wait()
 
 // A warp's way through its rows of a unit, ahead of the copies: what memory says about a row two tiles ahead, the word of the filter one tile
 // ahead.  Lane i (modulo CHUNK) looks after row i of the warp's CHUNK rows of a tile.
-template <int CHUNK, class Lists>
+template <int WARPS, int CHUNK, class Lists>
 struct row_stream {
   const cache_view& c;
   const Lists& lists;
@@ -501,7 +502,7 @@ struct row_stream {
 
   __device__ __forceinline__ row_stream(const cache_view& c_, const Lists& lists_, const typename Lists::list& l_, uint32_t warp, uint32_t tile0,
                                         uint32_t tile1_)
-    : c(c_), lists(lists_), l(l_), base(warp * CHUNK + (threadIdx.x & 31u) % CHUNK), tile_rows(kWarps * CHUNK), tile1(tile1_)
+    : c(c_), lists(lists_), l(l_), base(warp * CHUNK + (threadIdx.x & 31u) % CHUNK), tile_rows(WARPS * CHUNK), tile1(tile1_)
   {
     name_0 = name(tile0);
     name_1 = name(tile0 + 1);
@@ -532,7 +533,8 @@ struct row_stream {
 // ---- host ---------------------------------------------------------------------------------------------------------------------
 
 template <typename... Params, typename... Args>
-void launch_units(resources& res, void (*kernel)(Params...), uint32_t blocks, uint32_t cluster, size_t smem, Args&&... args)
+void launch_units(resources& res, void (*kernel)(Params...), uint32_t blocks, uint32_t threads, uint32_t cluster, size_t smem,
+                  Args&&... args)
 {
   if (smem > 48 * 1024) { ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem); }
   cudaLaunchAttribute attrs[2]{};
@@ -544,7 +546,7 @@ void launch_units(resources& res, void (*kernel)(Params...), uint32_t blocks, ui
   attrs[1].val.clusterDim.z                           = 1;
   cudaLaunchConfig_t config{};
   config.gridDim          = blocks;
-  config.blockDim         = kThreads;
+  config.blockDim         = threads;
   config.dynamicSmemBytes = smem;
   config.stream           = res.stream;
   config.attrs            = attrs;
@@ -556,24 +558,35 @@ void launch_units(resources& res, void (*kernel)(Params...), uint32_t blocks, ui
 // What a call launches, by type and sizes alone.
 struct plan {
   uint32_t rows;      // query heads of a unit
-  uint32_t tile;      // rows of the cache in a tile
-  uint32_t resident;  // blocks of an SM
+  uint32_t chunk;     // rows of the cache that a warp takes of a tile
+  uint32_t resident;  // small blocks of an SM
+  uint32_t warps;     // of a block
   uint32_t blocks;
   uint32_t cluster;   // 0: shares
   bool join;          // a unit may lie in several shares
 };
 
-inline void deal_out(const resources& res, plan& p, uint64_t units, uint64_t tiles)
+// `most`: rows of a unit, at most; `large`: whether there are large blocks; `shares`: whether there may be shares.
+inline void deal_out(const resources& res, plan& p, uint64_t units, uint64_t most, bool large, bool shares)
 {
-  const uint64_t resident = uint64_t(res.sm_count) * p.resident;
-  tiles                   = std::max<uint64_t>(tiles, 1);
-  uint32_t cluster        = 1;
-  while (cluster < 8 && cluster < tiles) { cluster *= 2; }
-  // One wave of clusters whose blocks have few tiles
-  if (units * cluster <= resident && ceildiv<uint64_t>(tiles, cluster) <= 4 + units * tiles / resident) {
-    p.blocks  = uint32_t(units * cluster);
-    p.cluster = cluster;
-    p.join    = false;
+  const uint64_t sms = uint64_t(res.sm_count), resident = sms * p.resident;
+  p.join = false;
+  if (units <= sms) {
+    p.warps              = large ? kLarge : kSmall;
+    const uint64_t tiles = ceildiv<uint64_t>(most, p.warps * p.chunk);
+    uint32_t cluster     = 1;
+    while (cluster < 8 && 2 * cluster * units <= sms && cluster < tiles) { cluster *= 2; }
+    if (!shares || ceildiv<uint64_t>(tiles, cluster) <= 4) {
+      p.blocks  = uint32_t(units * cluster);
+      p.cluster = cluster;
+      return;
+    }
+  }
+  const uint64_t tiles = std::max<uint64_t>(1, ceildiv<uint64_t>(most, kSmall * p.chunk));
+  p.warps              = kSmall;
+  if (!shares) {
+    p.blocks  = uint32_t(units);
+    p.cluster = 1;
   } else {
     p.blocks  = uint32_t(std::min(resident, units * tiles));
     p.cluster = 0;

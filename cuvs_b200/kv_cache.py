@@ -192,8 +192,8 @@ def attend_candidates(keys, values, queries, candidates, scale=None, filter=None
 
 def merge_parts(parts, parts_lse, out=None, lse=None, resources: Resources | None = None, sync: bool = True):
     """Joins parts of one softmax over disjoint sets of rows: ``parts`` ``[n_parts, n_tokens, n_heads, dim]`` and their ``parts_lse``, float32
-    ``[n_parts, n_tokens, n_heads]``, both of any strides between rows (blocks gathered from several GPUs, say).  Returns ``(out, lse)``.  A
-    part whose lse is -inf is not read."""
+    ``[n_parts, n_tokens, n_heads]``, both of any strides between rows (blocks gathered from several GPUs, say).  Returns ``(out, lse)``.  What
+    the row of a part holds whose lse is -inf does not count."""
     resources, stream = _handle(parts, resources)
     shape = parts.shape
     if out is None:

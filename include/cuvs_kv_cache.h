@@ -62,8 +62,8 @@ CUVS_EXPORT cuvsError_t cuvsKvCacheAttendCandidates(cuvsResources_t res, DLManag
                                                     cuvsFilter filter, DLManagedTensor* out, DLManagedTensor* lse);
 
 /* Joins parts of one softmax over disjoint sets of rows: parts [n_parts, n_tokens, n_heads, dim] (any 16-byte strides) and their
- * lse, f32 [n_parts, n_tokens, n_heads] (any strides), give out [n_tokens, n_heads, dim] and lse f32 [n_tokens, n_heads].  A part
- * whose lse is -inf is not read. */
+ * lse, f32 [n_parts, n_tokens, n_heads] (any strides), give out [n_tokens, n_heads, dim] and lse f32 [n_tokens, n_heads].  What the
+ * row of a part holds whose lse is -inf does not count. */
 CUVS_EXPORT cuvsError_t cuvsKvCacheMergeParts(cuvsResources_t res, DLManagedTensor* parts, DLManagedTensor* parts_lse,
                                               DLManagedTensor* out, DLManagedTensor* lse);
 
