@@ -198,6 +198,9 @@ SIGNATURES = {
     "cuvsKvCacheAttendCandidates": [C.c_size_t, *[_P(DLManagedTensor)] * 4, C.c_float, FilterStruct, *[_P(DLManagedTensor)] * 2],
     "cuvsKvCacheMergeParts": [C.c_size_t, *[_P(DLManagedTensor)] * 4],
     "cuvsB200KvCacheArrays": [C.c_size_t, C.c_void_p, C.c_int, C.c_void_p, C.c_int64, C.c_bool],
+    "cuvsB200SetTensorExchange": [C.c_void_p, C.c_void_p],
+    "cuvsB200KvCacheTensors": [C.c_size_t, C.c_void_p, C.c_int, *[C.py_object] * 11, C.c_int64, C.c_float, C.c_bool],
+    "cuvsB200KvCacheWait": [C.c_size_t, C.c_void_p],
     "cuvsB200KvCacheWorkspaceArrays": [C.c_size_t, C.c_void_p, C.c_int64, _P(C.c_size_t)],
     "cuvsB200KvCacheCheck": [C.c_int, C.c_int, C.c_void_p, C.c_int64],
     "cuvsIvfPqTransform": [C.c_size_t, _P(IndexStruct), _P(DLManagedTensor), _P(DLManagedTensor),

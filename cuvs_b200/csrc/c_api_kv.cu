@@ -3,10 +3,12 @@
 
 #include "c_api_util.hpp"
 #include "kv_cache.hpp"
+#include "tensor_exchange.hpp"
 
 #include <algorithm>
 #include <cmath>
 #include <cstring>
+#include <mutex>
 
 using namespace cuvs_b200;
 using namespace cuvs_b200::capi;
@@ -14,11 +16,9 @@ using kv::tensor;
 
 namespace {
 
-tensor describe(const DLManagedTensor* mt, const char* name)
+tensor describe(const DLTensor& d, const char* name)
 {
   tensor t;
-  if (mt == nullptr) { return t; }
-  const DLTensor& d = mt->dl_tensor;
   CUVS_EXPECTS(d.ndim >= 1 && d.ndim <= 4, "%s: 1 to 4 dimensions, not %d", name, int(d.ndim));
   CUVS_EXPECTS(d.dtype.lanes == 1, "More than 1 DLTensor lanes not supported");
   t.data        = static_cast<char*>(d.data) + d.byte_offset;
@@ -35,6 +35,7 @@ tensor describe(const DLManagedTensor* mt, const char* name)
   }
   return t;
 }
+tensor describe(const DLManagedTensor* mt, const char* name) { return mt == nullptr ? tensor{} : describe(mt->dl_tensor, name); }
 
 // From words: ndim | type code << 32 | bits << 40 (0: not given), address, device, shape, strides.
 tensor describe(const int64_t*& w, const int64_t* end, const char* name)
@@ -168,6 +169,20 @@ kv::cache_view cache_of(int device, tensor& keys, tensor& values, const tensor& 
     c.page_shift = 0;
     while ((1u << c.page_shift) < c.page_size) { c.page_shift++; }
   }
+  // the largest unit that all strides are multiples of; 16 bytes at least
+  const int64_t size     = keys.bits / 8;
+  const int64_t strides[] = {c.k_page * size, c.k_token * size, c.v_page * size, c.v_token * size};
+  c.unit_shift           = 4;
+  while (c.unit_shift < 16 && std::all_of(strides, strides + 4, [&](int64_t x) { return x % (int64_t(2) << c.unit_shift) == 0; })) { c.unit_shift++; }
+  for (int i = 0; i < 4; i += 2) {
+    const auto reach = [&](int64_t n, int64_t stride) { return unsigned(n > 0 ? n - 1 : 0) * (unsigned __int128)(stride >> c.unit_shift); };
+    CUVS_EXPECTS(reach(c.n_pages, strides[i]) + reach(c.page_size, strides[i + 1]) < ((unsigned __int128)1 << 32),
+                 "%s: too large for rows at multiples of %u bytes", i == 0 ? "keys" : "values", 1u << c.unit_shift);
+  }
+  c.k_page_units  = uint32_t(strides[0] >> c.unit_shift);
+  c.k_token_units = uint32_t(strides[1] >> c.unit_shift);
+  c.v_page_units  = uint32_t(strides[2] >> c.unit_shift);
+  c.v_token_units = uint32_t(strides[3] >> c.unit_shift);
   if (filter_given.given()) {
     tensor f = filter_given;
     check_place(device, f, 1, "filter");
@@ -319,23 +334,26 @@ kv::attention_args attention_of(int device, tensor* t, float scale, int64_t wind
   return a;
 }
 
-// With the workspace that the caller gave, or the handle's own.
-void attention_call(resources& res, kv::attention_args a)
+// With the workspace that the caller gave, or the handle's own for the stream.  False: the stream is being captured, and the call needs one
+// to itself.
+bool attention_call(resources& res, cudaStream_t stream, kv::attention_args a)
 {
   const size_t need = kv::attention_workspace(res, a.type, a.n_sequences, a.n_query_heads, a.cache.n_heads, a.cache.dim,
                                               uint64_t(a.table_width) * a.cache.page_size, a.window);
-  if (a.workspace != nullptr) {
+  std::unique_lock<std::mutex> held;
+  if (need > 0 && a.workspace != nullptr) {
     CUVS_EXPECTS(a.workspace_bytes >= need, "workspace: %zu bytes, but %zu are needed", a.workspace_bytes, need);
+    CUDA_TRY(cudaMemsetAsync(a.workspace, 0, kv::attention_workspace_zeroed(res), stream));
   } else if (need > 0) {
     cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
-    CUDA_TRY(cudaStreamIsCapturing(res.stream, &capturing));
-    CUVS_EXPECTS(capturing == cudaStreamCaptureStatusNone, "a call that is captured needs a workspace of its own");
-    res.ws.reserve(need);
-    a.workspace       = res.ws.base();
-    a.workspace_bytes = res.ws.capacity();
+    CUDA_TRY(cudaStreamIsCapturing(stream, &capturing));
+    if (capturing != cudaStreamCaptureStatusNone) { return false; }
+    held = res.stream_workspace(stream, need, kv::attention_workspace_zeroed(res), &a.workspace);
   }
-  kv::attention(res, a);
+  kv::attention(res, stream, a);
+  return true;
 }
+constexpr const char* kOwnWorkspace = "a call that is captured needs a workspace of its own";
 
 kv::candidates_args candidates_of(int device, tensor* t, float scale)
 {
@@ -433,7 +451,7 @@ extern "C" cuvsError_t cuvsKvCacheAppend(cuvsResources_t res, DLManagedTensor* k
                   describe(new_values, "new_values"), describe(pages, "pages"),       describe(positions, "positions"),
                   describe(sequences, "sequences"), describe(queries, "queries"),     describe(frequencies, "frequencies"),
                   describe(slots, "slots"),         describe(rotated, "rotated")};
-    kv::append(r, append_of(r.device, t, interleaved));
+    kv::append(r, r.stream, append_of(r.device, t, interleaved));
   });
 }
 
@@ -447,7 +465,7 @@ extern "C" cuvsError_t cuvsKvCacheAttention(cuvsResources_t res, DLManagedTensor
     tensor t[] = {describe(keys, "keys"),       describe(values, "values"), describe(queries, "queries"),
                   describe(pages, "pages"),     describe(lengths, "lengths"), filter_of(filter),
                   describe(out, "out"),         describe(lse, "lse"),       describe(workspace, "workspace")};
-    attention_call(r, attention_of(r.device, t, scale, window));
+    CUVS_EXPECTS(attention_call(r, r.stream, attention_of(r.device, t, scale, window)), kOwnWorkspace);
   });
 }
 
@@ -469,7 +487,7 @@ extern "C" cuvsError_t cuvsKvCacheAttendCandidates(cuvsResources_t res, DLManage
     device_scope on(r.device);
     tensor t[] = {describe(keys, "keys"), describe(values, "values"), describe(queries, "queries"), describe(candidates, "candidates"),
                   filter_of(filter),      describe(out, "out"),       describe(lse, "lse")};
-    kv::attend_candidates(r, candidates_of(r.device, t, scale));
+    kv::attend_candidates(r, r.stream, candidates_of(r.device, t, scale));
   });
 }
 
@@ -480,61 +498,113 @@ extern "C" cuvsError_t cuvsKvCacheMergeParts(cuvsResources_t res, DLManagedTenso
     resources& r = single_device(res);
     device_scope on(r.device);
     tensor t[] = {describe(parts, "parts"), describe(parts_lse, "parts_lse"), describe(out, "out"), describe(lse, "lse")};
-    kv::merge_parts(r, merge_of(r.device, t));
+    kv::merge_parts(r, r.stream, merge_of(r.device, t));
   });
 }
 
 namespace {
 
+constexpr int kMost = 11;  // tensors of a call
+const int n_tensors[]            = {11, 9, 7, 4};
+const int n_scalars[]            = {1, 2, 1, 0};
+const char* const names[][kMost] = {
+  {"keys", "values", "new_keys", "new_values", "pages", "positions", "sequences", "queries", "frequencies", "slots", "rotated"},
+  {"keys", "values", "queries", "pages", "lengths", "filter", "out", "lse", "workspace"},
+  {"keys", "values", "queries", "candidates", "filter", "out", "lse"},
+  {"parts", "parts_lse", "out", "lse"}};
+
 struct call {
-  tensor t[11];
+  tensor t[kMost];
   bool interleaved = false;
   float scale      = 0.0f;
   int64_t window   = 0;
+  call() = default;
   call(int op, const int64_t* words, int64_t n_words)
   {
-    static const int n_tensors[]         = {11, 9, 7, 4};
-    static const int n_scalars[]         = {1, 2, 1, 0};
-    static const char* const names[][11] = {
-      {"keys", "values", "new_keys", "new_values", "pages", "positions", "sequences", "queries", "frequencies", "slots", "rotated"},
-      {"keys", "values", "queries", "pages", "lengths", "filter", "out", "lse", "workspace"},
-      {"keys", "values", "queries", "candidates", "filter", "out", "lse"},
-      {"parts", "parts_lse", "out", "lse"}};
     CUVS_EXPECTS(op >= 0 && op < 4 && words != nullptr, "unknown call %d", op);
     const int64_t* end = words + n_words;
     for (int i = 0; i < n_tensors[op]; i++) { t[i] = describe(words, end, names[op][i]); }
     CUVS_EXPECTS(end - words == n_scalars[op], "the words do not describe the call");
-    const int64_t* scalars = words;
-    if (op == 0) { interleaved = scalars[0] != 0; }
-    if (op == 1) { window = scalars[0]; }
+    if (op == 0) { interleaved = words[0] != 0; }
+    if (op == 1) { window = words[0]; }
     if (op == 1 || op == 2) {
-      const uint32_t bits = uint32_t(scalars[op == 1 ? 1 : 0]);
+      const uint32_t bits = uint32_t(words[op == 1 ? 1 : 0]);
       std::memcpy(&scale, &bits, 4);
     }
   }
-};
-
-}  // namespace
-
-extern "C" cuvsError_t cuvsB200KvCacheArrays(cuvsResources_t res, cudaStream_t stream, int op, const int64_t* words, int64_t n_words, bool sync)
-{
-  return translate_exceptions([=] {
+  // False: it needs a workspace to itself.
+  bool run(cuvsResources_t res, cudaStream_t stream, int op, bool sync)
+  {
     resources& r = single_device(res);
-    call c(op, words, n_words);
     device_scope on(r.device);
-    r.stream = stream;
     if (sync) {
       cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
       CUDA_TRY(cudaStreamIsCapturing(stream, &capturing));
       CUVS_EXPECTS(capturing == cudaStreamCaptureStatusNone, "a call that is captured cannot wait for its work: pass sync=False");
     }
     switch (op) {
-      case 0: kv::append(r, append_of(r.device, c.t, c.interleaved)); break;
-      case 1: attention_call(r, attention_of(r.device, c.t, c.scale, c.window)); break;
-      case 2: kv::attend_candidates(r, candidates_of(r.device, c.t, c.scale)); break;
-      default: kv::merge_parts(r, merge_of(r.device, c.t));
+      case 0: kv::append(r, stream, append_of(r.device, t, interleaved)); break;
+      case 1:
+        if (!attention_call(r, stream, attention_of(r.device, t, scale, window))) { return false; }
+        break;
+      case 2: kv::attend_candidates(r, stream, candidates_of(r.device, t, scale)); break;
+      default: kv::merge_parts(r, stream, merge_of(r.device, t));
     }
-    if (sync) { r.sync(); }
+    __atomic_fetch_add(&r.launches, uint64_t(1), __ATOMIC_RELAXED);
+    return true;
+  }
+};
+
+const tensor_exchange* g_exchange = nullptr;  // set once, when the Python module is imported
+const void* g_none                = nullptr;
+
+}  // namespace
+
+extern "C" cuvsError_t cuvsB200KvCacheArrays(cuvsResources_t res, cudaStream_t stream, int op, const int64_t* words, int64_t n_words, bool sync)
+{
+  return translate_exceptions([=] {
+    CUVS_EXPECTS(call(op, words, n_words).run(res, stream, op, sync), kOwnWorkspace);
+    if (sync) { CUDA_TRY(cudaStreamSynchronize(stream)); }
+  });
+}
+
+extern "C" cuvsError_t cuvsB200SetTensorExchange(const void* table, const void* none)
+{
+  return translate_exceptions([=] {
+    const auto* x = static_cast<const tensor_exchange*>(table);
+    CUVS_EXPECTS(x != nullptr && x->major == 1 && x->from_python != nullptr, "no DLPack 1.x table of exchange functions");
+    g_exchange = x;
+    g_none     = none;
+  });
+}
+
+extern "C" int cuvsB200KvCacheTensors(cuvsResources_t res, cudaStream_t stream, int op, void* t0, void* t1, void* t2, void* t3, void* t4, void* t5,
+                                      void* t6, void* t7, void* t8, void* t9, void* t10, int64_t integer, float scale, bool sync)
+{
+  int status = CUVS_ERROR;
+  const auto raised = translate_exceptions([&] {
+    CUVS_EXPECTS(g_exchange != nullptr && op >= 0 && op < 4, "unknown call %d", op);
+    void* const objects[kMost] = {t0, t1, t2, t3, t4, t5, t6, t7, t8, t9, t10};
+    call c;
+    for (int i = 0; i < n_tensors[op]; i++) {
+      if (objects[i] == g_none) { continue; }
+      DLTensor d{};
+      CUVS_EXPECTS(g_exchange->from_python(objects[i], &d) == 0, "%s: cannot be described", names[op][i]);
+      c.t[i] = describe(d, names[op][i]);
+    }
+    c.interleaved = integer != 0;
+    c.window      = integer;
+    c.scale       = scale;
+    status        = c.run(res, stream, op, sync) ? CUVS_SUCCESS : 2;
+  });
+  return raised == CUVS_SUCCESS ? status : CUVS_ERROR;
+}
+
+extern "C" cuvsError_t cuvsB200KvCacheWait(cuvsResources_t res, cudaStream_t stream)
+{
+  return translate_exceptions([=] {
+    device_scope on(single_device(res).device);
+    CUDA_TRY(cudaStreamSynchronize(stream));
   });
 }
 

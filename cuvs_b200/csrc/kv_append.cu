@@ -183,7 +183,7 @@ append_kernel(append_args a, uint32_t log_lanes, uint32_t steps, uint32_t slices
 }
 
 template <typename T>
-void launch(resources& res, const append_args& a)
+void launch(resources& res, cudaStream_t stream, const append_args& a)
 {
   constexpr uint32_t E  = kPerPiece<T>;
   const uint32_t pieces = a.cache.dim / E;
@@ -198,7 +198,7 @@ void launch(resources& res, const append_args& a)
   const uint32_t rows_of_slice = round_up(ceildiv(rows, slices), turn);
   const size_t smem            = size_t(kWarps) * a.n_pairs * sizeof(float2);
   auto go                      = [&](auto kernel) {
-    launch_chained(kernel, dim3(uint32_t(ceildiv<uint64_t>(uint64_t(a.n_tokens) * slices, kWarps))), kWarps * 32, smem, res.stream, a, log_lanes,
+    launch_chained(kernel, dim3(uint32_t(ceildiv<uint64_t>(uint64_t(a.n_tokens) * slices, kWarps))), kWarps * 32, smem, stream, a, log_lanes,
                    steps, slices, rows_of_slice);
   };
   if (mode == PAIRED) {
@@ -208,18 +208,17 @@ void launch(resources& res, const append_args& a)
   } else {
     go(append_kernel<T, ANYWHERE>);
   }
-  res.launches++;
 }
 
 }  // namespace
 
-void append(resources& res, const append_args& a)
+void append(resources& res, cudaStream_t stream, const append_args& a)
 {
   if (a.n_tokens == 0) { return; }
   switch (a.type) {
-    case elem::f16: return launch<__half>(res, a);
-    case elem::bf16: return launch<__nv_bfloat16>(res, a);
-    default: return launch<float>(res, a);
+    case elem::f16: return launch<__half>(res, stream, a);
+    case elem::bf16: return launch<__nv_bfloat16>(res, stream, a);
+    default: return launch<float>(res, stream, a);
   }
 }
 

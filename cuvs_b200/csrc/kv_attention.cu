@@ -82,10 +82,10 @@ struct halves<__nv_bfloat16> {
 template <int D, int NT, int WARPS>
 struct mma_shape {
   static constexpr int kRows     = 8 * NT;
-  static constexpr int kTile     = WARPS * 16;
+  static constexpr int kChunk    = 16;
   static constexpr int kStages   = D == 64 ? 4 : D == 128 ? 2 : 3;
   static constexpr bool kQInRegs = D * NT <= 256;
-  static constexpr int kResident = WARPS == kLarge || D == 256 ? 1 : NT == 4 ? 2 : 3;  // blocks of an SM
+  static constexpr int kResident = WARPS > kSmall || D == 256 ? 1 : NT == 4 ? 2 : 3;  // blocks of an SM
   static constexpr int kRowBytes = D * 2;
   static constexpr int kStage    = 2 * 16 * kRowBytes;                       // 16 keys, 16 values
   static constexpr int kAccRow   = D + 4;                                    // floats: lanes of a store on different banks
@@ -119,230 +119,278 @@ mma_kernel(cache_view c, work_view w, positions lists, rows_view queries, result
   const uint32_t buffers = shared_address(smem) + warp * (S * shape::kStage);
   const uint32_t s_q     = shared_address(smem + shape::kQAt);
   const uint32_t pieces  = c.dim / 8;
+  // Copies: a lane has one piece of every ROWS-th row.  Pieces stand in a row's place by place ^ (row & 7), so that eight rows' pieces of one
+  // column lie on different banks; behind the row's end they are 0.
+  constexpr int ROWS          = 32 / PR;
+  const uint32_t copy_row     = lane / PR;
+  const uint32_t copy_swizzle = ((lane % PR) ^ copy_row) << 4;
+  const uint32_t copy_bytes   = lane % PR < pieces ? 16u : 0u;
+  const uint32_t copy_from    = lane % PR < pieces ? (lane % PR) * 16u : 0u;
+  const uint64_t k_rows_on    = uint64_t(c.k_token_units * ROWS) << c.unit_shift;
+  const uint64_t v_rows_on    = uint64_t(c.v_token_units * ROWS) << c.unit_shift;
   chain_begin();
 
-  each_unit<T, WARPS, shape::kTile>(
-    c, w, lists, result, parts, state,
-    [&](uint32_t sequence, uint32_t unit, const positions::list& l, uint32_t tile0, uint32_t tile1) {
-      const uint32_t head = unit / w.n_blocks_of, of = unit - head * w.n_blocks_of;
-      const uint32_t rows  = min(uint32_t(shape::kRows), w.group - of * shape::kRows);
-      const uint32_t head0 = head * w.group + of * shape::kRows;
-      const char* keys     = c.keys + int64_t(head) * c.k_head * 2;
-      const char* values   = c.values + int64_t(head) * c.v_head * 2;
-      row_stream<WARPS, 16, positions> stream(c, lists, l, warp, tile0, tile1);
-      auto copy_rows = [&](uint32_t tile) {
-        const uint32_t stage = (tile - tile0) % S;
-        int64_t page;
-        uint32_t place;
-        const uint32_t mask = __ballot_sync(kAllLanes, stream.next(tile, page, place)) & 0xFFFFu;
-        if (lane == 0) { s_mask[stage] = mask; }
-        if (mask != 0u) {
-          const uint32_t to = buffers + stage * shape::kStage;
-          int64_t k_at, v_at;
-          if constexpr (WHOLE_PAGES) {
-            // all 16 rows are in the page of any of them; the place of row 0, whichever lane asks
-            const int64_t p    = __shfl_sync(kAllLanes, int32_t(page), __ffs(int(mask)) - 1);
-            const int64_t from = int64_t(place) - int64_t(lane & 15u);
-            k_at               = p * c.k_page + from * c.k_token;
-            v_at               = p * c.v_page + from * c.v_token;
-          } else {
-            k_at = page * c.k_page + int64_t(place) * c.k_token;
-            v_at = page * c.v_page + int64_t(place) * c.v_token;
-          }
+  float acc[NT][D / 16][4], top[NT][2], sum[NT][2];
+
+  auto body = [&](uint32_t sequence, uint32_t unit, const positions::list& l, uint32_t chunk0, uint32_t end, uint32_t step) {
+    const uint32_t head = unit / w.n_blocks_of, of = unit - head * w.n_blocks_of;
+    const uint32_t rows  = min(uint32_t(shape::kRows), w.group - of * shape::kRows);
+    const uint32_t head0 = head * w.group + of * shape::kRows;
+    const char* keys     = c.keys + int64_t(head) * c.k_head * 2 + copy_from;
+    const char* values   = c.values + int64_t(head) * c.v_head * 2 + copy_from;
+    row_stream<16, positions> stream(c, lists, l, chunk0, end, step);
+    uint32_t filling = 0, emptying = 0;  // stages
+    auto copy_rows = [&](uint32_t chunk) {
+      uint32_t page, place;
+      const bool there    = stream.next(chunk, page, place);
+      const uint32_t mask = __ballot_sync(kAllLanes, there) & 0xFFFFu;
+      if (lane == 0) { s_mask[filling] = mask; }
+      if (mask == 0u) { return; }
+      const uint32_t to = buffers + filling * shape::kStage + copy_row * shape::kRowBytes;
+      uint32_t k_at, v_at;
+      const char *k_from, *v_from;
+      if constexpr (WHOLE_PAGES) {
+        // all 16 rows are in the page of any of them, whether they are to be read or not; `place` is that of the lane's own row
+        page   = __shfl_sync(kAllLanes, page, __ffs(int(mask)) - 1);
+        place  = place - (lane & 15u) + copy_row;
+        k_from = keys + (uint64_t(page * c.k_page_units + place * c.k_token_units) << c.unit_shift);
+        v_from = values + (uint64_t(page * c.v_page_units + place * c.v_token_units) << c.unit_shift);
+      } else {
+        k_at = there ? page * c.k_page_units + place * c.k_token_units : 0u;
+        v_at = there ? page * c.v_page_units + place * c.v_token_units : 0u;
+      }
 #pragma unroll
-          for (int i = 0; i < 16 * PR / 32; i++) {
-            const uint32_t piece = lane % PR, row = (lane + 32u * i) / PR;
-            int64_t k = k_at, v = v_at;
-            if constexpr (WHOLE_PAGES) {
-              k += row * c.k_token;
-              v += row * c.v_token;
-            } else {
-              k = __shfl_sync(kAllLanes, k_at, row);
-              v = __shfl_sync(kAllLanes, v_at, row);
-            }
-            const bool read   = ((mask >> row) & 1u) != 0u && piece < pieces;
-            const uint32_t at = to + row * shape::kRowBytes + ((piece ^ (row & 7u)) << 4);
-            copy_piece(at, read ? keys + k * 2 + piece * 16 : c.keys, read);
-            copy_piece(at + 16 * shape::kRowBytes, read ? values + v * 2 + piece * 16 : c.values, read);
+      for (int i = 0; i < 16 / ROWS; i++) {
+        const uint32_t at = to + i * (ROWS * shape::kRowBytes) + (copy_swizzle ^ ((i * ROWS & 7) << 4));
+        if constexpr (!WHOLE_PAGES) {
+          k_from = keys + (uint64_t(__shfl_sync(kAllLanes, k_at, copy_row + i * ROWS)) << c.unit_shift);
+          v_from = values + (uint64_t(__shfl_sync(kAllLanes, v_at, copy_row + i * ROWS)) << c.unit_shift);
+        }
+        const uint32_t bytes = ((mask >> (copy_row + i * ROWS)) & 1u) != 0u ? copy_bytes : 0u;
+        copy_piece(at, k_from, bytes);
+        copy_piece(at + 16 * shape::kRowBytes, v_from, bytes);
+        if constexpr (WHOLE_PAGES) {
+          k_from += k_rows_on;
+          v_from += v_rows_on;
+        }
+      }
+    };
+    auto advance = [&](uint32_t chunk) {
+      if (chunk < end) { copy_rows(chunk); }
+      copies_end_group();  // past the unit's end an empty one
+      filling = filling + 1 == S ? 0 : filling + 1;
+    };
+
+    // queries: the second operand of the first product
+    uint32_t q[shape::kQInRegs ? NT : 1][shape::kQInRegs ? D / 16 : 1][2];
+    if constexpr (shape::kQInRegs) {
+#pragma unroll
+      for (int n = 0; n < NT; n++) {
+        const uint32_t r    = n * 8 + g;
+        const char* row     = queries.data + (int64_t(sequence) * queries.row + int64_t(head0 + r) * queries.head) * 2;
+#pragma unroll
+        for (int k = 0; k < D / 16; k++) {
+#pragma unroll
+          for (int h = 0; h < 2; h++) {
+            const uint32_t column = k * 16 + h * 8 + 2 * t;
+            q[n][k][h]            = r < rows && column < c.dim ? *reinterpret_cast<const uint32_t*>(row + column * 2) : 0u;
           }
         }
-      };
-      // past the unit's end a group is empty, and so is its mask
-      auto advance = [&](uint32_t tile) {
-        if (tile < tile1) { copy_rows(tile); }
-        copies_end_group();
-      };
+      }
+    } else {
+      for (uint32_t i = threadIdx.x; i < uint32_t(shape::kRows * PR); i += WARPS * 32) {
+        const uint32_t r = i / PR, piece = i % PR;
+        uint4 x          = make_uint4(0, 0, 0, 0);
+        if (r < rows && piece < pieces) {
+          x = reinterpret_cast<const uint4*>(queries.data + (int64_t(sequence) * queries.row + int64_t(head0 + r) * queries.head) * 2)[piece];
+        }
+        *reinterpret_cast<uint4*>(smem + shape::kQAt + r * shape::kRowBytes + ((piece ^ (r & 7u)) << 4)) = x;
+      }
+      __syncthreads();
+    }
 
-      // queries: the second operand of the first product
-      uint32_t q[shape::kQInRegs ? NT : 1][shape::kQInRegs ? D / 16 : 1][2];
-      if constexpr (shape::kQInRegs) {
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+#pragma unroll
+      for (int d = 0; d < D / 16; d++) { acc[n][d][0] = acc[n][d][1] = acc[n][d][2] = acc[n][d][3] = 0.0f; }
+      top[n][0] = top[n][1] = -INFINITY;
+      sum[n][0] = sum[n][1] = 0.0f;
+    }
+
+#pragma unroll
+    for (int i = 0; i < S; i++) { advance(chunk0 + i * step); }
+
+    for (uint32_t chunk = chunk0; chunk < end; chunk += step) {
+      copies_wait<S - 1>();
+      __syncwarp();
+      const uint32_t stage = emptying;
+      emptying             = emptying + 1 == S ? 0 : emptying + 1;
+      const uint32_t mask  = s_mask[stage];
+      if (mask != 0u) {
+        const uint32_t k_rows = buffers + stage * shape::kStage, v_rows = k_rows + 16 * shape::kRowBytes;
+        float s[NT][4] = {};
+#pragma unroll
+        for (int k = 0; k < D / 16; k++) {
+          uint32_t a[4];
+          const uint32_t row = (lane & 7u) + (lane & 8u), piece = k * 2 + (lane >> 4);
+          load_matrices(a, k_rows + row * shape::kRowBytes + ((piece ^ (row & 7u)) << 4));
+          if constexpr (shape::kQInRegs) {
+#pragma unroll
+            for (int n = 0; n < NT; n++) { multiply_add<T>(s[n], a, q[n][k][0], q[n][k][1]); }
+          } else {
+            // two eights of heads at a time: matrices (heads 0-7, columns 0-7), (0-7, 8-15), (8-15, 0-7), (8-15, 8-15)
+#pragma unroll
+            for (int n = 0; n < NT; n += 2) {
+              uint32_t b[4];
+              const uint32_t r = n * 8 + (lane & 7u) + ((lane >> 4) << 3), p = k * 2 + ((lane >> 3) & 1u);
+              load_matrices(b, s_q + r * shape::kRowBytes + ((p ^ (r & 7u)) << 4));
+              multiply_add<T>(s[n], a, b[0], b[1]);
+              multiply_add<T>(s[n + 1], a, b[2], b[3]);
+            }
+          }
+        }
+        const bool k0 = ((mask >> g) & 1u) != 0u, k1 = ((mask >> (g + 8)) & 1u) != 0u;
+        float next[NT][2];
+        bool higher = false;
 #pragma unroll
         for (int n = 0; n < NT; n++) {
-          const uint32_t r    = n * 8 + g;
-          const char* row     = queries.data + (int64_t(sequence) * queries.row + int64_t(head0 + r) * queries.head) * 2;
+          s[n][0] = k0 ? s[n][0] * scale_log2 : -INFINITY;
+          s[n][1] = k0 ? s[n][1] * scale_log2 : -INFINITY;
+          s[n][2] = k1 ? s[n][2] * scale_log2 : -INFINITY;
+          s[n][3] = k1 ? s[n][3] * scale_log2 : -INFINITY;
 #pragma unroll
-          for (int k = 0; k < D / 16; k++) {
+          for (int h = 0; h < 2; h++) {
+            float m = fmaxf(s[n][h], s[n][h + 2]);
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-              const uint32_t column = k * 16 + h * 8 + 2 * t;
-              q[n][k][h]            = r < rows && column < c.dim ? *reinterpret_cast<const uint32_t*>(row + column * 2) : 0u;
-            }
+            for (int o = 4; o < 32; o <<= 1) { m = fmaxf(m, __shfl_xor_sync(kAllLanes, m, o)); }
+            next[n][h] = fmaxf(top[n][h], m);
+            higher     = higher || next[n][h] > top[n][h];
           }
         }
-      } else {
-        for (uint32_t i = threadIdx.x; i < uint32_t(shape::kRows * PR); i += WARPS * 32) {
-          const uint32_t r = i / PR, piece = i % PR;
-          uint4 x          = make_uint4(0, 0, 0, 0);
-          if (r < rows && piece < pieces) {
-            x = reinterpret_cast<const uint4*>(queries.data + (int64_t(sequence) * queries.row + int64_t(head0 + r) * queries.head) * 2)[piece];
-          }
-          *reinterpret_cast<uint4*>(smem + shape::kQAt + r * shape::kRowBytes + ((piece ^ (r & 7u)) << 4)) = x;
-        }
-        __syncthreads();
-      }
-
-      float acc[NT][D / 16][4] = {};
-      float top[NT][2], sum[NT][2];
-#pragma unroll
-      for (int n = 0; n < NT; n++) {
-        top[n][0] = top[n][1] = -INFINITY;
-        sum[n][0] = sum[n][1] = 0.0f;
-      }
-
-#pragma unroll
-      for (int i = 0; i < S; i++) { advance(tile0 + i); }
-
-      for (uint32_t tile = tile0; tile < tile1; tile++) {
-        copies_wait<S - 1>();
-        __syncwarp();
-        const uint32_t stage = (tile - tile0) % S;
-        const uint32_t mask  = s_mask[stage];
-        if (mask != 0u) {
-          const uint32_t k_rows = buffers + stage * shape::kStage, v_rows = k_rows + 16 * shape::kRowBytes;
-          float s[NT][4] = {};
-#pragma unroll
-          for (int k = 0; k < D / 16; k++) {
-            uint32_t a[4];
-            const uint32_t row = (lane & 7u) + (lane & 8u), piece = k * 2 + (lane >> 4);
-            load_matrices(a, k_rows + row * shape::kRowBytes + ((piece ^ (row & 7u)) << 4));
-            if constexpr (shape::kQInRegs) {
-#pragma unroll
-              for (int n = 0; n < NT; n++) { multiply_add<T>(s[n], a, q[n][k][0], q[n][k][1]); }
-            } else {
-              // two eights of heads at a time: matrices (heads 0-7, columns 0-7), (0-7, 8-15), (8-15, 0-7), (8-15, 8-15)
-#pragma unroll
-              for (int n = 0; n < NT; n += 2) {
-                uint32_t b[4];
-                const uint32_t r = n * 8 + (lane & 7u) + ((lane >> 4) << 3), p = k * 2 + ((lane >> 3) & 1u);
-                load_matrices(b, s_q + r * shape::kRowBytes + ((p ^ (r & 7u)) << 4));
-                multiply_add<T>(s[n], a, b[0], b[1]);
-                multiply_add<T>(s[n + 1], a, b[2], b[3]);
-              }
-            }
-          }
-          const bool k0 = ((mask >> g) & 1u) != 0u, k1 = ((mask >> (g + 8)) & 1u) != 0u;
-          float next[NT][2];
-          bool higher = false;
+        if (__any_sync(kAllLanes, higher)) {
 #pragma unroll
           for (int n = 0; n < NT; n++) {
-            s[n][0] = k0 ? s[n][0] * scale_log2 : -INFINITY;
-            s[n][1] = k0 ? s[n][1] * scale_log2 : -INFINITY;
-            s[n][2] = k1 ? s[n][2] * scale_log2 : -INFINITY;
-            s[n][3] = k1 ? s[n][3] * scale_log2 : -INFINITY;
+            float keep[2];
 #pragma unroll
             for (int h = 0; h < 2; h++) {
-              float m = fmaxf(s[n][h], s[n][h + 2]);
+              keep[h]   = power_of_2(top[n][h] - finite_top(next[n][h]));
+              top[n][h] = next[n][h];
+              sum[n][h] *= keep[h];
+            }
 #pragma unroll
-              for (int o = 4; o < 32; o <<= 1) { m = fmaxf(m, __shfl_xor_sync(kAllLanes, m, o)); }
-              next[n][h] = fmaxf(top[n][h], m);
-              higher     = higher || next[n][h] > top[n][h];
+            for (int d = 0; d < D / 16; d++) {
+              acc[n][d][0] *= keep[0];
+              acc[n][d][1] *= keep[1];
+              acc[n][d][2] *= keep[0];
+              acc[n][d][3] *= keep[1];
             }
           }
-          if (__any_sync(kAllLanes, higher)) {
+        }
+        uint32_t high[NT][2], low[NT][2];
 #pragma unroll
-            for (int n = 0; n < NT; n++) {
-              float keep[2];
+        for (int n = 0; n < NT; n++) {
+          float p[4];
 #pragma unroll
-              for (int h = 0; h < 2; h++) {
-                keep[h]   = exp2f(top[n][h] - finite_top(next[n][h]));
-                top[n][h] = next[n][h];
-                sum[n][h] *= keep[h];
-              }
-#pragma unroll
-              for (int d = 0; d < D / 16; d++) {
-                acc[n][d][0] *= keep[0];
-                acc[n][d][1] *= keep[1];
-                acc[n][d][2] *= keep[0];
-                acc[n][d][3] *= keep[1];
-              }
-            }
+          for (int e = 0; e < 4; e++) {
+            p[e] = power_of_2(s[n][e] - (finite_top(top[n][e & 1]) - halves<T>::kShift));
+            sum[n][e & 1] += p[e];
           }
-          uint32_t high[NT][2], low[NT][2];
+#pragma unroll
+          for (int h = 0; h < 2; h++) {
+            high[n][h]       = halves<T>::pack(p[2 * h] * halves<T>::kBelow, p[2 * h + 1] * halves<T>::kBelow);
+            const float2 was = halves<T>::unpack(high[n][h]);
+            low[n][h]        = turn_matrix(halves<T>::pack(p[2 * h] - was.x, p[2 * h + 1] - was.y));
+            high[n][h]       = turn_matrix(high[n][h]);
+          }
+        }
+#pragma unroll
+        for (int d = 0; d < D / 16; d++) {
+          uint32_t a[4];
+          const uint32_t row = (lane & 7u) + ((lane >> 4) << 3), piece = d * 2 + ((lane >> 3) & 1u);
+          load_matrices_turned(a, v_rows + row * shape::kRowBytes + ((piece ^ (row & 7u)) << 4));
 #pragma unroll
           for (int n = 0; n < NT; n++) {
-            float p[4];
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-              p[e] = exp2f(s[n][e] - (finite_top(top[n][e & 1]) - halves<T>::kShift));
-              sum[n][e & 1] += p[e];
-            }
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-              high[n][h]       = halves<T>::pack(p[2 * h] * halves<T>::kBelow, p[2 * h + 1] * halves<T>::kBelow);
-              const float2 was = halves<T>::unpack(high[n][h]);
-              low[n][h]        = turn_matrix(halves<T>::pack(p[2 * h] - was.x, p[2 * h + 1] - was.y));
-              high[n][h]       = turn_matrix(high[n][h]);
-            }
-          }
-#pragma unroll
-          for (int d = 0; d < D / 16; d++) {
-            uint32_t a[4];
-            const uint32_t row = (lane & 7u) + ((lane >> 4) << 3), piece = d * 2 + ((lane >> 3) & 1u);
-            load_matrices_turned(a, v_rows + row * shape::kRowBytes + ((piece ^ (row & 7u)) << 4));
-#pragma unroll
-            for (int n = 0; n < NT; n++) {
-              multiply_add<T>(acc[n][d], a, high[n][0], high[n][1]);
-              multiply_add<T>(acc[n][d], a, low[n][0], low[n][1]);
-            }
-          }
-        }
-        __syncwarp();
-        advance(tile + S);
-      }
-      copies_wait<0>();
-      __syncthreads();  // shared memory changes hands: from rows to sums
-      const float unshift = exp2f(-halves<T>::kShift);
-#pragma unroll
-      for (int n = 0; n < NT; n++) {
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-#pragma unroll
-          for (int o = 4; o < 32; o <<= 1) { sum[n][h] += __shfl_xor_sync(kAllLanes, sum[n][h], o); }
-          const uint32_t r = n * 8 + 2 * t + h;
-          if (g == 0) { state.stats[warp * shape::kRows + r] = make_float2(top[n][h], sum[n][h] * unshift); }
-          float* a = state.acc + (warp * shape::kRows + r) * shape::kAccRow + g;
-#pragma unroll
-          for (int d = 0; d < D / 16; d++) {
-            a[d * 16]     = acc[n][d][h] * unshift;
-            a[d * 16 + 8] = acc[n][d][h + 2] * unshift;
+            multiply_add<T>(acc[n][d], a, high[n][0], high[n][1]);
+            multiply_add<T>(acc[n][d], a, low[n][0], low[n][1]);
           }
         }
       }
-    });
+      __syncwarp();
+      advance(chunk + S * step);
+    }
+    copies_wait<0>();
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) { sum[n][h] += __shfl_xor_sync(kAllLanes, sum[n][h], o); }
+      }
+    }
+  };
+  const float unshift = power_of_2(-halves<T>::kShift);
+  auto to_shared      = [&] {
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        const uint32_t r = n * 8 + 2 * t + h;
+        if (g == 0) { state.stats[warp * shape::kRows + r] = make_float2(top[n][h], sum[n][h] * unshift); }
+        float* a = state.acc + (warp * shape::kRows + r) * shape::kAccRow + g;
+#pragma unroll
+        for (int d = 0; d < D / 16; d++) {
+          a[d * 16]     = acc[n][d][h] * unshift;
+          a[d * 16 + 8] = acc[n][d][h + 2] * unshift;
+        }
+      }
+    }
+  };
+  // A store of a warp is eight neighbouring columns of four rows.
+  auto to_rows = [&](uint32_t rows, uint32_t sequence, uint32_t head0, bool whole, uint32_t part) {
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        const uint32_t r = n * 8 + 2 * t + h;
+        if (r >= rows) { continue; }
+        if (whole) {
+          const float scale = sum[n][h] == 0.0f ? 0.0f : 1.0f / sum[n][h];
+          T* o = reinterpret_cast<T*>(result.out.data) + int64_t(sequence) * result.out.row + int64_t(head0 + r) * result.out.head + g;
+#pragma unroll
+          for (int d = 0; d < D / 16; d++) {
+            if (d * 16 + g < c.dim) { o[d * 16] = from_float<T>(acc[n][d][h] * scale); }
+            if (d * 16 + 8 + g < c.dim) { o[d * 16 + 8] = from_float<T>(acc[n][d][h + 2] * scale); }
+          }
+          if (g == 0) {
+            result.lse[size_t(sequence) * (w.group * c.n_heads) + head0 + r] = (finite_top(top[n][h]) - halves<T>::kShift + log2f(sum[n][h])) * kLn2;
+          }
+        } else {
+          float* a = parts.acc + (size_t(part) * parts.rows + r) * c.dim + g;
+#pragma unroll
+          for (int d = 0; d < D / 16; d++) {
+            if (d * 16 + g < c.dim) { a[d * 16] = acc[n][d][h] * unshift; }
+            if (d * 16 + 8 + g < c.dim) { a[d * 16 + 8] = acc[n][d][h + 2] * unshift; }
+          }
+          if (g == 0) { parts.stats[size_t(part) * parts.rows + r] = make_float2(top[n][h], sum[n][h] * unshift); }
+        }
+      }
+    }
+  };
+  each_unit<T, WARPS, shape::kChunk, 2>(c, w, lists, result, parts, state, body, to_shared, to_rows);
 }
 
 }  // namespace
 
 // One object per type: KV_TYPE is __half or __nv_bfloat16.
 template <>
-void attention16<KV_TYPE>(resources& res, const attention_args& a, const plan& p, const work_view& w, const positions& lists,
+void attention16<KV_TYPE>(cudaStream_t stream, const attention_args& a, const plan& p, const work_view& w, const positions& lists,
                           const result_view& result, const parts_view& parts)
 {
   using T     = KV_TYPE;
   auto launch = [&](auto d, auto nt, auto warps) {
     constexpr int D = decltype(d)::value, NT = decltype(nt)::value, WARPS = decltype(warps)::value;
     auto go = [&](auto kernel) {
-      launch_units(res, kernel, p.blocks, WARPS * 32, p.cluster, mma_shape<D, NT, WARPS>::kShared, a.cache, w, lists, a.queries, result,
+      launch_units(stream, kernel, p.blocks, WARPS * 32, p.cluster, mma_shape<D, NT, WARPS>::kShared, a.cache, w, lists, a.queries, result,
                    a.scale * kLog2E, parts);
     };
     if (a.cache.page_size % 16 == 0) {
@@ -355,8 +403,8 @@ void attention16<KV_TYPE>(resources& res, const attention_args& a, const plan& p
   auto by_rows = [&](auto cols) {
     constexpr int D = decltype(cols)::value;
     auto by_warps   = [&](auto nt) {
-      if constexpr (has_large(D, decltype(nt)::value)) {
-        if (p.warps == uint32_t(kLarge)) { return launch(cols, nt, integral_constant<int, kLarge>{}); }
+      if constexpr (mma_large_of(D, decltype(nt)::value) != 0) {
+        if (p.warps != uint32_t(kSmall)) { return launch(cols, nt, integral_constant<int, mma_large_of(D, decltype(nt)::value)>{}); }
       }
       launch(cols, nt, integral_constant<int, kSmall>{});
     };

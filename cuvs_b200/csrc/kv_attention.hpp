@@ -7,17 +7,17 @@ namespace cuvs_b200::kv {
 
 // Columns of a row in the kernels' shared memory.
 inline uint32_t padded(uint32_t dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
-// Whether the kernel for so many columns and eights of query heads fits the registers of a large block's threads.
-constexpr bool has_large(uint32_t columns, uint32_t eights) { return columns <= 128 && eights <= 2; }
+// Warps of the large block of the kernel for so many columns and eights of query heads; 0: its threads' registers leave no room for one.
+constexpr int mma_large_of(uint32_t columns, uint32_t eights) { return columns <= 128 && eights <= 2 ? 12 : 0; }
 
 template <typename T>
-void attention16(resources& res, const attention_args& a, const plan& p, const work_view& w, const positions& lists, const result_view& result,
+void attention16(cudaStream_t stream, const attention_args& a, const plan& p, const work_view& w, const positions& lists, const result_view& result,
                  const parts_view& parts);
 template <>
-void attention16<__half>(resources& res, const attention_args& a, const plan& p, const work_view& w, const positions& lists,
+void attention16<__half>(cudaStream_t stream, const attention_args& a, const plan& p, const work_view& w, const positions& lists,
                          const result_view& result, const parts_view& parts);
 template <>
-void attention16<__nv_bfloat16>(resources& res, const attention_args& a, const plan& p, const work_view& w, const positions& lists,
+void attention16<__nv_bfloat16>(cudaStream_t stream, const attention_args& a, const plan& p, const work_view& w, const positions& lists,
                                 const result_view& result, const parts_view& parts);
 
 }  // namespace cuvs_b200::kv

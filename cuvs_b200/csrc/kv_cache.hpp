@@ -5,6 +5,7 @@
 
 #include <cstdint>
 
+// These calls do not touch the handle beyond its device's properties: several threads may make them through one handle.
 namespace cuvs_b200::kv {
 
 enum class elem { f16, bf16, f32 };
@@ -29,6 +30,8 @@ struct cache_view {
   const char* values;
   int64_t k_page, k_token, k_head;
   int64_t v_page, v_token, v_head;
+  // For reading: the same strides of pages and tokens in units of 1 << unit_shift bytes, small enough that a row's place fits 32 bits.
+  uint32_t k_page_units, k_token_units, v_page_units, v_token_units, unit_shift;
   int64_t n_slots;
   int32_t n_pages;
   uint32_t page_size;
@@ -63,7 +66,7 @@ struct append_args {
   bool interleaved;
   int64_t* slots;  // [n_tokens]
 };
-void append(resources& res, const append_args& a);
+void append(resources& res, cudaStream_t stream, const append_args& a);
 
 struct attention_args {
   cache_view cache;
@@ -82,7 +85,9 @@ struct attention_args {
 // How many bytes of workspace attention() wants, by sizes alone.
 size_t attention_workspace(const resources& res, elem type, uint32_t n_sequences, uint32_t n_query_heads, uint32_t n_heads, uint32_t dim,
                            uint64_t capacity, int64_t window);
-void attention(resources& res, const attention_args& a);
+// Its first bytes, which have to be 0 and are left 0.
+size_t attention_workspace_zeroed(const resources& res);
+void attention(resources& res, cudaStream_t stream, const attention_args& a);
 
 struct candidates_args {
   cache_view cache;
@@ -93,7 +98,7 @@ struct candidates_args {
   float scale;
   float* lse;  // [n_tokens, n_query_heads]
 };
-void attend_candidates(resources& res, const candidates_args& a);
+void attend_candidates(resources& res, cudaStream_t stream, const candidates_args& a);
 
 struct merge_args {
   elem type;
@@ -105,6 +110,6 @@ struct merge_args {
   rows_view out;
   float* lse;  // [n_tokens, n_heads]
 };
-void merge_parts(resources& res, const merge_args& a);
+void merge_parts(resources& res, cudaStream_t stream, const merge_args& a);
 
 }  // namespace cuvs_b200::kv

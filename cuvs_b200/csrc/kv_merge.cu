@@ -80,15 +80,13 @@ __global__ void __launch_bounds__(kThreads, 4) merge_kernel(merge_args a, uint32
 }
 
 template <typename T>
-void launch(resources& res, const merge_args& a)
+void launch(resources& res, cudaStream_t stream, const merge_args& a)
 {
   const uint32_t pieces = a.dim / kPerPiece<T>;
   const uint64_t rows   = uint64_t(a.n_tokens) * a.n_heads;
   auto go               = [&](auto kernel, uint32_t lanes) {
-    launch_chained(kernel, dim3(uint32_t(ceildiv<uint64_t>(rows, kThreads / lanes))), kThreads, 0, res.stream, a, pieces);
-    CUDA_TRY(cudaGetLastError());
-    res.launches++;
-  };
+    launch_chained(kernel, dim3(uint32_t(ceildiv<uint64_t>(rows, kThreads / lanes))), kThreads, 0, stream, a, pieces);
+    };
   if (pieces <= 8) {
     go(merge_kernel<T, 8>, 8);
   } else if (pieces <= 16) {
@@ -100,13 +98,13 @@ void launch(resources& res, const merge_args& a)
 
 }  // namespace
 
-void merge_parts(resources& res, const merge_args& a)
+void merge_parts(resources& res, cudaStream_t stream, const merge_args& a)
 {
   if (a.n_tokens == 0 || a.n_heads == 0) { return; }
   switch (a.type) {
-    case elem::f16: return launch<__half>(res, a);
-    case elem::bf16: return launch<__nv_bfloat16>(res, a);
-    default: return launch<float>(res, a);
+    case elem::f16: return launch<__half>(res, stream, a);
+    case elem::bf16: return launch<__nv_bfloat16>(res, stream, a);
+    default: return launch<float>(res, stream, a);
   }
 }
 

@@ -13,13 +13,22 @@ namespace cuvs_b200::kv {
 
 namespace {
 
+// Rows of a chunk, by the 16-byte pieces that a row has room for in shared memory: 4 KB of keys for several query heads, 2 KB for one, which
+// leaves room for twice the warps.
+constexpr uint32_t chunk_of(uint32_t pieces, uint32_t heads)
+{
+  const uint32_t most = heads == 1 ? 16 : 32, rows = (heads == 1 ? 128 : 256) / pieces;
+  return rows < most ? rows : most;
+}
+constexpr uint32_t resident_of(uint32_t heads) { return heads == 1 ? 6 : 3; }   // small blocks of an SM
+constexpr int large_of(uint32_t heads) { return heads == 1 ? 24 : 12; }         // warps of a large block
+
 // LANES lanes have a row, PIECES 16-byte pieces each; R query heads share its reading.
 template <typename T, int LANES, int PIECES, int R, int WARPS>
 struct rows_shape {
   static constexpr int kPitch    = LANES * PIECES * 16;                    // bytes of a row in shared memory
-  static constexpr int kChunk    = kPitch <= 128 ? 32 : 4096 / kPitch;     // rows of a warp's stage
+  static constexpr int kChunk    = chunk_of(LANES * PIECES, R);            // rows of a warp's stage
   static constexpr int kStages   = kPitch < 128 ? 4 : 2;
-  static constexpr int kTile     = WARPS * kChunk;
   static constexpr int kGroups   = 32 / LANES;
   static constexpr int kTurns    = kChunk / kGroups;                       // rows of a lane group in a stage
   static constexpr int kColumns  = LANES * PIECES * kPerPiece<T>;
@@ -32,7 +41,7 @@ struct rows_shape {
 };
 
 template <typename T, int LANES, int PIECES, int R, int WARPS, class Lists>
-__global__ void __launch_bounds__(WARPS * 32, WARPS == kSmall ? 3 : 1)
+__global__ void __launch_bounds__(WARPS * 32, WARPS == kSmall ? resident_of(R) : 1)
 rows_kernel(cache_view c, work_view w, Lists lists, rows_view queries, result_view result, float scale_log2, parts_view parts)
 {
   using shape          = rows_shape<T, LANES, PIECES, R, WARPS>;
@@ -40,7 +49,7 @@ rows_kernel(cache_view c, work_view w, Lists lists, rows_view queries, result_vi
   constexpr int S      = shape::kStages;
   constexpr int CHUNK  = shape::kChunk;
   constexpr int PR     = LANES * PIECES;
-  constexpr int U      = 4;  // rows that a lane group takes at a time
+  constexpr int U      = shape::kTurns < 4 ? shape::kTurns : 4;  // rows that a lane group takes at a time
   extern __shared__ __align__(128) char smem[];
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
   const uint32_t group = lane / LANES, gl = lane % LANES;
@@ -50,166 +59,207 @@ rows_kernel(cache_view c, work_view w, Lists lists, rows_view queries, result_vi
   const char* stages     = smem + warp * (S * shape::kStage);
   const uint32_t buffers = shared_address(stages);
   const uint32_t pieces  = c.dim / E;
+  // Copies: a lane has one piece (of 64: two) of every ROWS-th row.
+  constexpr int ROWS           = LANES == 32 ? 1 : 32 / PR;
+  const uint32_t copy_row      = LANES == 32 ? 0u : lane / PR;
+  const uint32_t copy_piece_of = LANES == 32 ? lane : lane % PR;
   chain_begin();
 
-  each_unit<T, WARPS, shape::kTile>(
-    c, w, lists, result, parts, state,
-    [&](uint32_t sequence, uint32_t unit, const typename Lists::list& l, uint32_t tile0, uint32_t tile1) {
-      const uint32_t head = unit / w.n_blocks_of, of = unit - head * w.n_blocks_of;
-      const uint32_t rows  = min(uint32_t(R), w.group - of * R);
-      const uint32_t head0 = head * w.group + of * R;
-      const char* keys     = c.keys + int64_t(head) * c.k_head * int64_t(sizeof(T));
-      const char* values   = c.values + int64_t(head) * c.v_head * int64_t(sizeof(T));
-      row_stream<WARPS, CHUNK, Lists> stream(c, lists, l, warp, tile0, tile1);
-      auto advance = [&](uint32_t tile) {
-        if (tile < tile1) {
-          const uint32_t stage = (tile - tile0) % S;
-          int64_t page;
-          uint32_t place;
-          const bool there    = stream.next(tile, page, place);
-          const uint32_t mask = __ballot_sync(kAllLanes, there) & uint32_t((uint64_t(1) << CHUNK) - 1u);
-          if (lane == 0) { s_mask[stage] = mask; }
-          if (mask != 0u) {
-            const uint32_t to  = buffers + stage * shape::kStage;
-            const int64_t k_at = page * c.k_page + int64_t(place) * c.k_token;
-            const int64_t v_at = page * c.v_page + int64_t(place) * c.v_token;
+  float acc[R][PIECES][E], top[R], sum[R];
+
+  auto body = [&](uint32_t sequence, uint32_t unit, const typename Lists::list& l, uint32_t chunk0, uint32_t end, uint32_t step) {
+    const uint32_t head = unit / w.n_blocks_of, of = unit - head * w.n_blocks_of;
+    const uint32_t rows  = min(uint32_t(R), w.group - of * R);
+    const uint32_t head0 = head * w.group + of * R;
+    const char* keys     = c.keys + int64_t(head) * c.k_head * int64_t(sizeof(T));
+    const char* values   = c.values + int64_t(head) * c.v_head * int64_t(sizeof(T));
+    row_stream<CHUNK, Lists> stream(c, lists, l, chunk0, end, step);
+    uint32_t filling = 0, emptying = 0;  // stages
+    auto advance = [&](uint32_t chunk) {
+      if (chunk < end) {
+        uint32_t page, place;
+        const bool there    = stream.next(chunk, page, place);
+        const uint32_t mask = __ballot_sync(kAllLanes, there) & uint32_t((uint64_t(1) << CHUNK) - 1u);
+        if (lane == 0) { s_mask[filling] = mask; }
+        if (mask != 0u) {
+          const uint32_t to   = buffers + filling * shape::kStage + copy_row * shape::kPitch + copy_piece_of * 16;
+          const uint32_t k_at = there ? page * c.k_page_units + place * c.k_token_units : 0u;
+          const uint32_t v_at = there ? page * c.v_page_units + place * c.v_token_units : 0u;
 #pragma unroll
-            for (int i = 0; i < CHUNK * PR / 32; i++) {
-              const uint32_t piece = (lane + 32u * i) % PR, row = (lane + 32u * i) / PR;
-              const int64_t k   = __shfl_sync(kAllLanes, k_at, row);
-              const int64_t v   = __shfl_sync(kAllLanes, v_at, row);
-              const bool read   = ((mask >> row) & 1u) != 0u && piece < pieces;
-              const uint32_t at = to + row * shape::kPitch + piece * 16u;
-              copy_piece(at, read ? keys + k * int64_t(sizeof(T)) + piece * 16 : c.keys, read);
-              copy_piece(at + CHUNK * shape::kPitch, read ? values + v * int64_t(sizeof(T)) + piece * 16 : c.values, read);
+          for (int i = 0; i < CHUNK / ROWS; i++) {
+            const char* k_from = keys + (uint64_t(__shfl_sync(kAllLanes, k_at, copy_row + i * ROWS)) << c.unit_shift);
+            const char* v_from = values + (uint64_t(__shfl_sync(kAllLanes, v_at, copy_row + i * ROWS)) << c.unit_shift);
+            const bool read    = ((mask >> (copy_row + i * ROWS)) & 1u) != 0u;
+#pragma unroll
+            for (int p = 0; p < PIECES; p++) {
+              const uint32_t piece = copy_piece_of + p * 32, bytes = read && piece < pieces ? 16u : 0u;
+              const uint32_t at   = to + i * (ROWS * shape::kPitch) + p * 512;
+              copy_piece(at, k_from + (piece < pieces ? piece * 16 : 0), bytes);
+              copy_piece(at + CHUNK * shape::kPitch, v_from + (piece < pieces ? piece * 16 : 0), bytes);
             }
           }
-        }
-        copies_end_group();  // past the unit's end an empty one
-      };
-
-      float q[R][PIECES][E], acc[R][PIECES][E] = {}, top[R], sum[R];
-#pragma unroll
-      for (int r = 0; r < R; r++) {
-        top[r] = -INFINITY;
-        sum[r] = 0.0f;
-#pragma unroll
-        for (int p = 0; p < PIECES; p++) {
-          const uint32_t j = gl + p * LANES;
-          uint4 x          = make_uint4(0, 0, 0, 0);
-          if (uint32_t(r) < rows && j < pieces) {
-            x = reinterpret_cast<const uint4*>(queries.data + (int64_t(sequence) * queries.row + int64_t(head0 + r) * queries.head) *
-                                                                int64_t(sizeof(T)))[j];
-          }
-          piece_to_floats<T>(x, q[r][p]);
         }
       }
-#pragma unroll
-      for (int i = 0; i < S; i++) { advance(tile0 + i); }
+      copies_end_group();  // past the unit's end an empty one
+      filling = filling + 1 == S ? 0 : filling + 1;
+    };
 
-      for (uint32_t tile = tile0; tile < tile1; tile++) {
-        copies_wait<S - 1>();
-        __syncwarp();
-        const uint32_t stage = (tile - tile0) % S;
-        const uint32_t mask  = s_mask[stage];
-        if (mask != 0u) {
-          const char* k_rows = stages + stage * shape::kStage;
-          const char* v_rows = k_rows + CHUNK * shape::kPitch;
+    float q[R][PIECES][E];
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+      top[r] = -INFINITY;
+      sum[r] = 0.0f;
+#pragma unroll
+      for (int p = 0; p < PIECES; p++) {
+        const uint32_t j = gl + p * LANES;
+        uint4 x          = make_uint4(0, 0, 0, 0);
+        if (uint32_t(r) < rows && j < pieces) {
+          x = reinterpret_cast<const uint4*>(queries.data + (int64_t(sequence) * queries.row + int64_t(head0 + r) * queries.head) *
+                                                              int64_t(sizeof(T)))[j];
+        }
+        piece_to_floats<T>(x, q[r][p]);
+#pragma unroll
+        for (int e = 0; e < E; e++) { acc[r][p][e] = 0.0f; }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < S; i++) { advance(chunk0 + i * step); }
+
+    for (uint32_t chunk = chunk0; chunk < end; chunk += step) {
+      copies_wait<S - 1>();
+      __syncwarp();
+      const uint32_t stage = emptying;
+      emptying             = emptying + 1 == S ? 0 : emptying + 1;
+      const uint32_t mask  = s_mask[stage];
+      if (mask != 0u) {
+        const char* k_rows = stages + stage * shape::kStage;
+        const char* v_rows = k_rows + CHUNK * shape::kPitch;
 #pragma unroll 1
-          for (int u0 = 0; u0 < shape::kTurns; u0 += U) {
-            float score[R][U];
+        for (int u0 = 0; u0 < shape::kTurns; u0 += U) {
+          float score[R][U];
 #pragma unroll
-            for (int u = 0; u < U; u++) {
-              const uint32_t row = uint32_t(u0 + u) * shape::kGroups + group;
-              float x[PIECES][E];
+          for (int u = 0; u < U; u++) {
+            const uint32_t row = uint32_t(u0 + u) * shape::kGroups + group;
+            float x[PIECES][E];
 #pragma unroll
-              for (int p = 0; p < PIECES; p++) {
-                piece_to_floats<T>(*reinterpret_cast<const uint4*>(k_rows + row * shape::kPitch + (gl + p * LANES) * 16), x[p]);
-              }
-              const bool ok = ((mask >> row) & 1u) != 0u;
-#pragma unroll
-              for (int r = 0; r < R; r++) {
-                float s = 0.0f;
-#pragma unroll
-                for (int p = 0; p < PIECES; p++) {
-#pragma unroll
-                  for (int e = 0; e < E; e++) { s = fmaf(q[r][p][e], x[p][e], s); }
-                }
-#pragma unroll
-                for (int o = LANES / 2; o > 0; o >>= 1) { s += __shfl_xor_sync(kAllLanes, s, o); }
-                score[r][u] = ok ? s * scale_log2 : -INFINITY;
-              }
+            for (int p = 0; p < PIECES; p++) {
+              piece_to_floats<T>(*reinterpret_cast<const uint4*>(k_rows + row * shape::kPitch + (gl + p * LANES) * 16), x[p]);
             }
+            const bool ok = ((mask >> row) & 1u) != 0u;
 #pragma unroll
             for (int r = 0; r < R; r++) {
-              float next = top[r];
-#pragma unroll
-              for (int u = 0; u < U; u++) { next = fmaxf(next, score[r][u]); }
-              const float safe = finite_top(next);
-              const float keep = exp2f(top[r] - safe);
-              top[r]           = next;
-              sum[r] *= keep;
+              float s = 0.0f;
 #pragma unroll
               for (int p = 0; p < PIECES; p++) {
 #pragma unroll
-                for (int e = 0; e < E; e++) { acc[r][p][e] *= keep; }
+                for (int e = 0; e < E; e++) { s = fmaf(q[r][p][e], x[p][e], s); }
               }
 #pragma unroll
-              for (int u = 0; u < U; u++) {
-                score[r][u] = exp2f(score[r][u] - safe);
-                sum[r] += score[r][u];
-              }
+              for (int o = LANES / 2; o > 0; o >>= 1) { s += __shfl_xor_sync(kAllLanes, s, o); }
+              score[r][u] = ok ? s * scale_log2 : -INFINITY;
+            }
+          }
+#pragma unroll
+          for (int r = 0; r < R; r++) {
+            float next = top[r];
+#pragma unroll
+            for (int u = 0; u < U; u++) { next = fmaxf(next, score[r][u]); }
+            const float safe = finite_top(next);
+            const float keep = power_of_2(top[r] - safe);
+            top[r]           = next;
+            sum[r] *= keep;
+#pragma unroll
+            for (int p = 0; p < PIECES; p++) {
+#pragma unroll
+              for (int e = 0; e < E; e++) { acc[r][p][e] *= keep; }
             }
 #pragma unroll
             for (int u = 0; u < U; u++) {
-              const uint32_t row = uint32_t(u0 + u) * shape::kGroups + group;
+              score[r][u] = power_of_2(score[r][u] - safe);
+              sum[r] += score[r][u];
+            }
+          }
 #pragma unroll
-              for (int p = 0; p < PIECES; p++) {
-                float x[E];
-                piece_to_floats<T>(*reinterpret_cast<const uint4*>(v_rows + row * shape::kPitch + (gl + p * LANES) * 16), x);
+          for (int u = 0; u < U; u++) {
+            const uint32_t row = uint32_t(u0 + u) * shape::kGroups + group;
 #pragma unroll
-                for (int r = 0; r < R; r++) {
+            for (int p = 0; p < PIECES; p++) {
+              float x[E];
+              piece_to_floats<T>(*reinterpret_cast<const uint4*>(v_rows + row * shape::kPitch + (gl + p * LANES) * 16), x);
 #pragma unroll
-                  for (int e = 0; e < E; e++) { acc[r][p][e] = fmaf(score[r][u], x[e], acc[r][p][e]); }
-                }
+              for (int r = 0; r < R; r++) {
+#pragma unroll
+                for (int e = 0; e < E; e++) { acc[r][p][e] = fmaf(score[r][u], x[e], acc[r][p][e]); }
               }
             }
           }
         }
-        __syncwarp();
-        advance(tile + S);
       }
-      copies_wait<0>();
-      __syncthreads();  // shared memory changes hands: from rows to sums
+      __syncwarp();
+      advance(chunk + S * step);
+    }
+    copies_wait<0>();
+    // the warp's lane groups
 #pragma unroll
-      for (int r = 0; r < R; r++) {
+    for (int r = 0; r < R; r++) {
 #pragma unroll
-        for (int o = LANES; o < 32; o <<= 1) {
-          const float other = __shfl_xor_sync(kAllLanes, top[r], o);
-          const float next  = fmaxf(top[r], other);
-          const float safe  = finite_top(next);
-          const float own = exp2f(top[r] - safe), theirs = exp2f(other - safe);
-          sum[r] = sum[r] * own + __shfl_xor_sync(kAllLanes, sum[r], o) * theirs;
+      for (int o = LANES; o < 32; o <<= 1) {
+        const float other = __shfl_xor_sync(kAllLanes, top[r], o);
+        const float next  = fmaxf(top[r], other);
+        const float safe  = finite_top(next);
+        const float own = power_of_2(top[r] - safe), theirs = power_of_2(other - safe);
+        sum[r] = sum[r] * own + __shfl_xor_sync(kAllLanes, sum[r], o) * theirs;
 #pragma unroll
-          for (int p = 0; p < PIECES; p++) {
+        for (int p = 0; p < PIECES; p++) {
 #pragma unroll
-            for (int e = 0; e < E; e++) { acc[r][p][e] = acc[r][p][e] * own + __shfl_xor_sync(kAllLanes, acc[r][p][e], o) * theirs; }
-          }
-          top[r] = next;
+          for (int e = 0; e < E; e++) { acc[r][p][e] = acc[r][p][e] * own + __shfl_xor_sync(kAllLanes, acc[r][p][e], o) * theirs; }
         }
-        if (group == 0) {
-#pragma unroll
-          for (int p = 0; p < PIECES; p++) {
-#pragma unroll
-            for (int e = 0; e < E; e += 4) {
-              *reinterpret_cast<float4*>(state.acc + (warp * R + r) * shape::kColumns + (gl + p * LANES) * E + e) =
-                make_float4(acc[r][p][e], acc[r][p][e + 1], acc[r][p][e + 2], acc[r][p][e + 3]);
-            }
-          }
-        }
-        if (lane == 0) { state.stats[warp * R + r] = make_float2(top[r], sum[r]); }
+        top[r] = next;
       }
-    });
+    }
+  };
+  auto to_floats = [&](float* row, int r) {
+#pragma unroll
+    for (int p = 0; p < PIECES; p++) {
+#pragma unroll
+      for (int e = 0; e < E; e += 4) {
+        if (gl + p * LANES < pieces) {
+          *reinterpret_cast<float4*>(row + (gl + p * LANES) * E + e) = make_float4(acc[r][p][e], acc[r][p][e + 1], acc[r][p][e + 2], acc[r][p][e + 3]);
+        }
+      }
+    }
+  };
+  auto to_shared = [&] {
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+      if (group == 0) { to_floats(state.acc + (warp * R + r) * shape::kColumns, r); }
+      if (lane == 0) { state.stats[warp * R + r] = make_float2(top[r], sum[r]); }
+    }
+  };
+  auto to_rows = [&](uint32_t rows, uint32_t sequence, uint32_t head0, bool whole, uint32_t part) {
+    if (group != 0) { return; }
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+      if (uint32_t(r) >= rows) { continue; }
+      if (whole) {
+        const float scale = sum[r] == 0.0f ? 0.0f : 1.0f / sum[r];
+#pragma unroll
+        for (int p = 0; p < PIECES; p++) {
+          if (gl + p * LANES < pieces) {
+            float x[E];
+#pragma unroll
+            for (int e = 0; e < E; e++) { x[e] = acc[r][p][e] * scale; }
+            store_piece<T>(result.out, sequence, head0 + r, gl + p * LANES, x);
+          }
+        }
+        if (gl == 0) { result.lse[size_t(sequence) * (w.group * c.n_heads) + head0 + r] = (finite_top(top[r]) + log2f(sum[r])) * kLn2; }
+      } else {
+        to_floats(parts.acc + (size_t(part) * parts.rows + r) * c.dim, r);
+        if (gl == 0) { parts.stats[size_t(part) * parts.rows + r] = make_float2(top[r], sum[r]); }
+      }
+    }
+  };
+  each_unit<T, WARPS, CHUNK, R == 1 ? 1 : 2>(c, w, lists, result, parts, state, body, to_shared, to_rows);
 }
 
 // How rows of so many 16-byte pieces are read.
@@ -230,11 +280,11 @@ void by_pieces(uint32_t pieces, Fn&& fn)
   }
 }
 
-uint32_t chunk_of(uint32_t pieces)
+uint32_t room_of(uint32_t pieces)
 {
-  uint32_t chunk = 0;
-  by_pieces(pieces, [&](auto lanes, auto n) { chunk = rows_shape<float, decltype(lanes)::value, decltype(n)::value, 1, kSmall>::kChunk; });
-  return chunk;
+  uint32_t room = 0;
+  by_pieces(pieces, [&](auto lanes, auto n) { room = decltype(lanes)::value * decltype(n)::value; });
+  return room;
 }
 
 plan attention_plan(const resources& res, elem type, uint64_t sequences, uint32_t n_heads, uint32_t group, uint32_t dim, uint64_t capacity,
@@ -243,51 +293,53 @@ plan attention_plan(const resources& res, elem type, uint64_t sequences, uint32_
   // a window may begin anywhere in 16 positions
   const uint64_t most = window > 0 && uint64_t(window) < capacity ? std::min(capacity, uint64_t(window) + 15) : capacity;
   plan p{};
-  bool large = true;
   if (type == elem::f32) {
     p.rows     = dim > 128 ? std::min(group, 4u) : group > 4 ? 8 : group;
     p.rows     = p.rows == 3 ? 4 : p.rows;
-    p.chunk    = chunk_of(dim / 4);
-    p.resident = 3;
+    p.chunk    = chunk_of(room_of(dim / 4), p.rows);
+    p.resident = resident_of(p.rows);
+    p.large    = large_of(p.rows);
   } else {
     const uint32_t d = padded(dim), eights = group <= 8 ? 1 : group <= 16 || d == 256 ? 2 : 4;
     p.rows     = 8 * eights;
     p.chunk    = 16;
     p.resident = d == 256 ? 1 : eights == 4 ? 2 : 3;
-    large      = has_large(d, eights);
+    p.large    = mma_large_of(d, eights);
   }
-  deal_out(res, p, sequences * n_heads * ceildiv(group, p.rows), most, large, true);
+  deal_out(res, p, sequences * n_heads * ceildiv(group, p.rows), most, true);
   return p;
 }
 
 template <typename T, int LANES, int PIECES, int R, class Lists, typename... Args>
-void launch_rows(resources& res, const plan& p, Args&&... args)
+void launch_rows(cudaStream_t stream, const plan& p, Args&&... args)
 {
-  if (p.warps == uint32_t(kLarge)) {
-    launch_units(res, rows_kernel<T, LANES, PIECES, R, kLarge, Lists>, p.blocks, kLarge * 32, p.cluster,
-                 rows_shape<T, LANES, PIECES, R, kLarge>::kShared, args...);
+  constexpr int LARGE = large_of(R);
+  if (p.warps == uint32_t(LARGE)) {
+    launch_units(stream, rows_kernel<T, LANES, PIECES, R, LARGE, Lists>, p.blocks, LARGE * 32, p.cluster,
+                 rows_shape<T, LANES, PIECES, R, LARGE>::kShared, args...);
   } else {
-    launch_units(res, rows_kernel<T, LANES, PIECES, R, kSmall, Lists>, p.blocks, kSmall * 32, p.cluster,
+    launch_units(stream, rows_kernel<T, LANES, PIECES, R, kSmall, Lists>, p.blocks, kSmall * 32, p.cluster,
                  rows_shape<T, LANES, PIECES, R, kSmall>::kShared, args...);
   }
 }
 
 template <typename T>
-void launch_candidates(resources& res, const candidates_args& a)
+void launch_candidates(resources& res, cudaStream_t stream, const candidates_args& a)
 {
   const uint32_t group = a.n_query_heads / a.cache.n_heads, pieces = a.cache.dim / kPerPiece<T>;
   const named_slots lists{a.candidates, a.n_candidates};
   parts_view parts{};
   plan p{};
   p.rows = parts.rows = 1;
-  p.chunk             = chunk_of(pieces);
-  p.resident          = 3;
-  deal_out(res, p, uint64_t(a.n_tokens) * a.n_query_heads, a.n_candidates, true, false);
-  const work_view w{a.n_tokens, a.n_query_heads, group, group, p.cluster};
+  p.chunk             = chunk_of(room_of(pieces), 1);
+  p.resident          = resident_of(1);
+  p.large             = large_of(1);
+  deal_out(res, p, uint64_t(a.n_tokens) * a.n_query_heads, a.n_candidates, false);
+  const work_view w{a.n_tokens, a.n_query_heads, group, group, p.cluster, false};
   by_pieces(pieces, [&](auto lanes, auto n) {
     constexpr int LANES = decltype(lanes)::value, PIECES = decltype(n)::value;
     if constexpr (sizeof(T) == 4 || PIECES == 1) {
-      launch_rows<T, LANES, PIECES, 1, named_slots>(res, p, a.cache, w, lists, a.queries, result_view{a.out, a.lse}, a.scale * kLog2E, parts);
+      launch_rows<T, LANES, PIECES, 1, named_slots>(stream, p, a.cache, w, lists, a.queries, result_view{a.out, a.lse}, a.scale * kLog2E, parts);
     }
   });
 }
@@ -298,38 +350,34 @@ size_t attention_workspace(const resources& res, elem type, uint32_t n_sequences
                            uint64_t capacity, int64_t window)
 {
   const plan p = attention_plan(res, type, n_sequences, n_heads, n_query_heads / n_heads, dim, capacity, window);
-  return p.join ? part_bytes(p.blocks, p.rows, dim) : 0;
+  return p.parts ? arrived_bytes(res) + part_bytes(p.teams(), p.rows, dim) : 0;
 }
+size_t attention_workspace_zeroed(const resources& res) { return arrived_bytes(res); }
 
-void attention(resources& res, const attention_args& a)
+void attention(resources& res, cudaStream_t stream, const attention_args& a)
 {
   if (a.n_sequences == 0) { return; }
   const cache_view& c  = a.cache;
   const uint32_t group = a.n_query_heads / c.n_heads;
   const plan p         = attention_plan(res, a.type, a.n_sequences, c.n_heads, group, c.dim, uint64_t(a.table_width) * c.page_size, a.window);
   const uint32_t of    = ceildiv(group, p.rows);
-  const work_view w{a.n_sequences, c.n_heads * of, of, group, p.cluster};
+  const work_view w{a.n_sequences, c.n_heads * of, of, group, p.cluster, p.warp_teams};
   const positions lists{a.pages, a.lengths, a.table_stride, a.window, a.table_width};
   const result_view result{a.out, a.lse};
   parts_view parts{};
-  if (p.join) { parts = parts_at(a.workspace, p.blocks, p.rows, c.dim); }
-  parts.rows = p.rows;
-  auto join  = [&](auto type) {
-    if (p.join) { launch_join<decltype(type)>(res, p, w, parts, c.dim, c.n_heads, result); }
-  };
-  if (a.type == elem::f16) {
-    attention16<__half>(res, a, p, w, lists, result, parts);
-    return join(__half{});
+  parts.teams = p.teams();
+  parts.rows  = p.rows;
+  if (p.parts) {
+    parts.arrived = reinterpret_cast<uint32_t*>(a.workspace);
+    parts.acc     = reinterpret_cast<float*>(a.workspace + arrived_bytes(res));
+    parts.stats   = reinterpret_cast<float2*>(parts.acc + size_t(2) * parts.teams * p.rows * c.dim);
   }
-  if (a.type == elem::bf16) {
-    attention16<__nv_bfloat16>(res, a, p, w, lists, result, parts);
-    return join(__nv_bfloat16{});
-  }
+  if (a.type == elem::f16) { return attention16<__half>(stream, a, p, w, lists, result, parts); }
+  if (a.type == elem::bf16) { return attention16<__nv_bfloat16>(stream, a, p, w, lists, result, parts); }
   by_pieces(c.dim / 4, [&](auto lanes, auto n) {
     constexpr int LANES = decltype(lanes)::value, PIECES = decltype(n)::value;
     auto go = [&](auto r) {
-      constexpr int R = decltype(r)::value;
-      launch_rows<float, LANES, PIECES, R, positions>(res, p, c, w, lists, a.queries, result, a.scale * kLog2E, parts);
+      launch_rows<float, LANES, PIECES, decltype(r)::value, positions>(stream, p, c, w, lists, a.queries, result, a.scale * kLog2E, parts);
     };
     using std::integral_constant;
     if (p.rows == 1) {
@@ -342,16 +390,15 @@ void attention(resources& res, const attention_args& a)
       go(integral_constant<int, 8>{});
     }
   });
-  join(float{});
 }
 
-void attend_candidates(resources& res, const candidates_args& a)
+void attend_candidates(resources& res, cudaStream_t stream, const candidates_args& a)
 {
   if (a.n_tokens == 0) { return; }
   switch (a.type) {
-    case elem::f16: return launch_candidates<__half>(res, a);
-    case elem::bf16: return launch_candidates<__nv_bfloat16>(res, a);
-    default: return launch_candidates<float>(res, a);
+    case elem::f16: return launch_candidates<__half>(res, stream, a);
+    case elem::bf16: return launch_candidates<__nv_bfloat16>(res, stream, a);
+    default: return launch_candidates<float>(res, stream, a);
   }
 }
 

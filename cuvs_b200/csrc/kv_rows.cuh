@@ -131,7 +131,15 @@ __device__ __forceinline__ void split_slot(const cache_view& c, int64_t slot, in
   }
 }
 
-// exp2 of (score - top) where nothing is an answer too: top = -inf leaves every weight 0.
+// 2^x, to 2^-22 of its value; below 2^-126 it is 0.
+__device__ __forceinline__ float power_of_2(float x)
+{
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// 2^(score - top) where nothing is an answer too: top = -inf leaves every weight 0.
 __device__ __forceinline__ float finite_top(float top) { return top == -INFINITY ? 0.0f : top; }
 
 }  // namespace cuvs_b200::kv

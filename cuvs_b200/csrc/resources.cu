@@ -80,6 +80,22 @@ resources::~resources()
   }
 }
 
+std::unique_lock<std::mutex> resources::stream_workspace(cudaStream_t on, size_t bytes, size_t zeroed, char** at)
+{
+  std::unique_lock<std::mutex> held(stream_ws_lock);
+  if (stream_ws.size() >= 64 && stream_ws.find(on) == stream_ws.end()) {
+    CUDA_TRY(cudaDeviceSynchronize());
+    stream_ws.clear();
+  }
+  workspace& w = stream_ws[on];
+  if (w.capacity() < bytes) {
+    w.reserve(bytes);
+    CUDA_TRY(cudaMemsetAsync(w.base(), 0, zeroed, on));
+  }
+  *at = w.base();
+  return held;
+}
+
 void resources::adopt_tc_verdict()
 {
   if (!tc_redo_pending || *static_cast<volatile uint32_t*>(pinned + 12) != tc_redo_seq) { return; }

@@ -21,9 +21,9 @@ wait for it unless ``sync=False``, which is what a captured call needs.
 """
 from __future__ import annotations
 
+import ctypes as C
 import functools
 import struct
-from ctypes import c_size_t
 
 import torch
 
@@ -80,22 +80,67 @@ def _handle(tensor, resources):
     return resources, resources.stream_at_call(device)
 
 
+def _on(stream, tensor):
+    return torch.cuda.stream(torch.cuda.ExternalStream(stream, device=tensor.device))
+
+
+def _rows_like(rows, resources, stream):
+    """A result of the shape and type of these rows that belongs to the stream which writes it."""
+    if resources._fixed_stream is None:
+        return torch.empty_like(rows)
+    with _on(stream, rows):
+        return torch.empty_like(rows)
+
+
 def _empty(dtype, tensor, resources, stream, *shape):
-    """A result on the tensor's device that belongs to the stream which writes it."""
     if resources._fixed_stream is None:
         return torch.empty(*shape, dtype=dtype, device=tensor.device)
-    with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=tensor.device)):
+    with _on(stream, tensor):
         return torch.empty(*shape, dtype=dtype, device=tensor.device)
 
 
-def _call(resources, stream, op, tensors, scalars, sync):
-    words, n = _words(tensors, scalars)
-    if _arrays(resources.handle, stream, op, words, n, sync) != L.CUVS_SUCCESS:
-        L.check(L.CUVS_ERROR)
+def _call(resources, stream, op, tensors, integer, scale, sync):
+    """`tensors`: those of the call in the order of the C interface, filled up with None to eleven.  False: the call is being captured, and
+    needs a workspace to itself."""
+    for t in tensors:
+        if t is not None and type(t) is not torch.Tensor:
+            break
+    else:
+        if _tensors is not None:
+            status = _tensors(resources.handle, stream, op, *tensors, integer, scale, sync)
+            if status == L.CUVS_SUCCESS:
+                if sync:
+                    L.check(_wait(resources.handle, stream))
+                return True
+            if status == 2:
+                return False
+            L.check(L.CUVS_ERROR)
+    # subclasses of torch.Tensor, and what is no tensor at all
+    scalars = ((integer,), (integer, _bits(scale)), (_bits(scale),), ())[op]
+    L.check(_arrays(resources.handle, stream, op, *_words(tensors[:_COUNTS[op]], scalars), sync))
+    return True
 
 
+def _tensor_calls():
+    """The entry point that reads tensors in place, through torch's table of DLPack exchange functions: describing them in Python took as long
+    as everything else of a small call together.  None where torch has no such table."""
+    capsule = getattr(torch.Tensor, "__dlpack_c_exchange_api__", None)
+    if capsule is None:
+        return None
+    pointer = C.pythonapi.PyCapsule_GetPointer
+    pointer.restype, pointer.argtypes = C.c_void_p, [C.py_object, C.c_char_p]
+    if L.load().cuvsB200SetTensorExchange(pointer(capsule, b"dlpack_exchange_api"), id(None)) != L.CUVS_SUCCESS:
+        return None
+    call = C.PyDLL(L.LIB_PATH).cuvsB200KvCacheTensors  # keeps the interpreter's lock: it reads Python objects
+    call.restype, call.argtypes = C.c_int, L.SIGNATURES["cuvsB200KvCacheTensors"]
+    return call
+
+
+_COUNTS = (11, 9, 7, 4)
 _arrays = L.load().cuvsB200KvCacheArrays
 _workspace = L.load().cuvsB200KvCacheWorkspaceArrays
+_wait = L.load().cuvsB200KvCacheWait
+_tensors = _tensor_calls()
 
 
 def append(keys, values, new_keys, new_values, pages, positions, sequences=None, queries=None, frequencies=None, interleaved=False,
@@ -117,9 +162,9 @@ def append(keys, values, new_keys, new_values, pages, positions, sequences=None,
     if slots is None:
         slots = _empty(torch.int64, keys, resources, stream, new_keys.shape[0])
     if queries is not None and rotated is None:
-        rotated = _empty(queries.dtype, keys, resources, stream, *queries.shape)
+        rotated = _rows_like(queries, resources, stream)
     _call(resources, stream, _APPEND, (keys, values, new_keys, new_values, pages, positions, sequences, queries, frequencies, slots, rotated),
-          (1 if interleaved else 0,), sync)
+          1 if interleaved else 0, 0.0, sync)
     return slots, rotated
 
 
@@ -134,21 +179,24 @@ def attention(keys, values, queries, pages, lengths, scale=None, window=None, fi
     ``i`` may be attended only if bit ``i % 32`` of word ``i // 32`` is set, as in ``ivf_pq.search``.
 
     ``workspace``: uint8 tensor of at least ``attention_workspace(...)`` bytes that nothing else uses until the work is done; by default
-    one is allocated for the call."""
+    the handle's own for the stream, and one allocated for the call while it is captured."""
     if window is not None and window <= 0:
         raise ValueError("window must be positive, or None")
     resources, stream = _handle(keys, resources)
-    shape = queries.shape
+    if queries.dim() != 3:
+        raise ValueError(f"queries: 3 dimensions, not {queries.dim()}")
+    n, n_heads, dim = queries.shape
     if out is None:
-        out = _empty(queries.dtype, keys, resources, stream, *shape)
+        out = _rows_like(queries, resources, stream)
     if lse is None:
-        lse = _empty(torch.float32, keys, resources, stream, *shape[:2])
-    if workspace is None:
-        need = _attention_workspace(resources, keys, queries, pages, window)
-        if need:
-            workspace = _empty(torch.uint8, keys, resources, stream, need)
-    _call(resources, stream, _ATTENTION, (keys, values, queries, pages, lengths, filter, out, lse, workspace),
-          (window or 0, _bits(shape[-1] ** -0.5 if scale is None else scale)), sync)
+        lse = _empty(torch.float32, keys, resources, stream, n, n_heads)
+    scale, window = dim ** -0.5 if scale is None else scale, window or 0
+    if not _call(resources, stream, _ATTENTION, (keys, values, queries, pages, lengths, filter, out, lse, workspace, None, None), window, scale,
+                 sync):
+        # what is replayed needs a workspace to itself; else the handle has one for the stream
+        workspace = _empty(torch.uint8, keys, resources, stream, _attention_workspace(resources, keys, queries, pages, window))
+        _call(resources, stream, _ATTENTION, (keys, values, queries, pages, lengths, filter, out, lse, workspace, None, None), window, scale,
+              sync)
     return out, lse
 
 
@@ -158,20 +206,9 @@ def attention_workspace(keys, queries, pages, window=None, resources: Resources 
 
 
 def _attention_workspace(resources, keys, queries, pages, window):
-    # a function of these alone; asking for it takes as long as a launch
-    what = (keys.get_device(), keys.dtype, *keys.shape[1:], *queries.shape[:2], *pages.shape, window)
-    need = _workspaces.get(what)
-    if need is None:
-        size = c_size_t()
-        L.check(_workspace(resources.handle, *_words((keys, queries, pages), (window or 0,)), size))
-        need = size.value
-        if len(_workspaces) >= 4096:
-            _workspaces.clear()
-        _workspaces[what] = need
-    return need
-
-
-_workspaces = {}
+    size = C.c_size_t()
+    L.check(_workspace(resources.handle, *_words((keys, queries, pages), (window or 0,)), size))
+    return size.value
 
 
 def attend_candidates(keys, values, queries, candidates, scale=None, filter=None, out=None, lse=None,
@@ -180,13 +217,15 @@ def attend_candidates(keys, values, queries, candidates, scale=None, filter=None
     searches over the keys return them.  Ids that are no slots (the search's "no such neighbour", -1) and slots that ``filter`` leaves out
     are skipped; a slot that is named twice counts twice.  Returns ``(out, lse)`` as :func:`attention` does."""
     resources, stream = _handle(keys, resources)
-    shape = queries.shape
+    if queries.dim() != 3:
+        raise ValueError(f"queries: 3 dimensions, not {queries.dim()}")
+    n, n_heads, dim = queries.shape
     if out is None:
-        out = _empty(queries.dtype, keys, resources, stream, *shape)
+        out = _rows_like(queries, resources, stream)
     if lse is None:
-        lse = _empty(torch.float32, keys, resources, stream, *shape[:2])
-    _call(resources, stream, _CANDIDATES, (keys, values, queries, candidates, filter, out, lse),
-          (_bits(shape[-1] ** -0.5 if scale is None else scale),), sync)
+        lse = _empty(torch.float32, keys, resources, stream, n, n_heads)
+    _call(resources, stream, _CANDIDATES, (keys, values, queries, candidates, filter, out, lse, None, None, None, None), 0,
+          dim ** -0.5 if scale is None else scale, sync)
     return out, lse
 
 
@@ -195,10 +234,12 @@ def merge_parts(parts, parts_lse, out=None, lse=None, resources: Resources | Non
     ``[n_parts, n_tokens, n_heads]``, both of any strides between rows (blocks gathered from several GPUs, say).  Returns ``(out, lse)``.  What
     the row of a part holds whose lse is -inf does not count."""
     resources, stream = _handle(parts, resources)
-    shape = parts.shape
+    if parts.dim() != 4:
+        raise ValueError(f"parts: 4 dimensions, not {parts.dim()}")
+    n_parts, n, n_heads, dim = parts.shape
     if out is None:
-        out = _empty(parts.dtype, parts, resources, stream, *shape[1:])
+        out = _empty(parts.dtype, parts, resources, stream, n, n_heads, dim)
     if lse is None:
-        lse = _empty(torch.float32, parts, resources, stream, *shape[1:3])
-    _call(resources, stream, _MERGE, (parts, parts_lse, out, lse), (), sync)
+        lse = _empty(torch.float32, parts, resources, stream, n, n_heads)
+    _call(resources, stream, _MERGE, (parts, parts_lse, out, lse, None, None, None, None, None, None, None), 0, 0.0, sync)
     return out, lse

@@ -43,8 +43,8 @@ CUVS_EXPORT cuvsError_t cuvsKvCacheAppend(cuvsResources_t res, DLManagedTensor* 
  * all).  queries, out: [n_sequences, n_query_heads, dim]; lengths: i32 [n_sequences] (what exceeds the table's width is not there;
  * a negative length is 0); scores are scale * q.k; filter: NO_FILTER or BITSET over slots; lse: f32 [n_sequences, n_query_heads],
  * the natural logarithm of the softmax's denominator.  workspace: u8 [cuvsKvCacheAttentionWorkspace bytes] that no other call uses
- * until this one's work is done, or NULL: the handle's own, which a call on another stream, or a later call that needs a larger one,
- * must not overlap with (so a call that is captured is given its own). */
+ * until this one's work is done, or NULL: the handle's own for this stream (refused while the stream is being captured: what is replayed
+ * needs one to itself). */
 CUVS_EXPORT cuvsError_t cuvsKvCacheAttention(cuvsResources_t res, DLManagedTensor* keys, DLManagedTensor* values,
                                              DLManagedTensor* queries, DLManagedTensor* pages, DLManagedTensor* lengths, float scale,
                                              int64_t window, cuvsFilter filter, DLManagedTensor* out, DLManagedTensor* lse,
@@ -70,10 +70,17 @@ CUVS_EXPORT cuvsError_t cuvsKvCacheMergeParts(cuvsResources_t res, DLManagedTens
 /* The calls above on arrays that are described by words: op 0 append, 1 attention, 2 attend candidates, 3 merge parts.  The
  * tensors come in the order of the calls, each as ndim | type code << 32 | bits << 40 | lanes << 48; address; device type | device
  * id << 32; the shape; the strides in elements -- or as one word 0 where there is none -- with a filter as a u32 tensor in the place
- * of its argument; behind them the scalars: {interleaved}, {window, bits of the f32 scale}, {bits of the scale}, {}.  Sets the
- * handle's stream; waits for the work if `sync`. */
+ * of its argument; behind them the scalars: {interleaved}, {window, bits of the f32 scale}, {bits of the scale}, {}.  The
+ * work goes to `stream`, and is waited for if `sync`. */
 CUVS_EXPORT cuvsError_t cuvsB200KvCacheArrays(cuvsResources_t res, cudaStream_t stream, int op, const int64_t* words, int64_t n_words,
                                               bool sync);
+/* The same for a caller in Python: tensors as Python objects (of the type that the table of DLPack exchange functions is from, or none),
+ * read in place; the caller holds the interpreter's lock.  `integer`: interleaved, or the window.  Returns 2 where the call needs a workspace
+ * to itself: nothing was done then.  Does not wait: cuvsB200KvCacheWait does, without the lock. */
+CUVS_EXPORT cuvsError_t cuvsB200SetTensorExchange(const void* table, const void* none);
+CUVS_EXPORT int cuvsB200KvCacheTensors(cuvsResources_t res, cudaStream_t stream, int op, void* t0, void* t1, void* t2, void* t3, void* t4,
+                                       void* t5, void* t6, void* t7, void* t8, void* t9, void* t10, int64_t integer, float scale, bool sync);
+CUVS_EXPORT cuvsError_t cuvsB200KvCacheWait(cuvsResources_t res, cudaStream_t stream);
 /* cuvsKvCacheAttentionWorkspace on the words of keys, queries, pages and {window}. */
 CUVS_EXPORT cuvsError_t cuvsB200KvCacheWorkspaceArrays(cuvsResources_t res, const int64_t* words, int64_t n_words, size_t* bytes);
 /* The checks of such a call alone, for a handle of `device`: touches no GPU and reads no tensor. */

@@ -157,6 +157,33 @@ def test_attention(dtype, lengths, heads, group, dim, page_size, how, window, ke
     assert torch.equal(out, again) and torch.equal(lse, lse_again)       # no order of arrival in the result
 
 
+# Work that no single block or warp finishes: parts of one unit by the hundred (three levels of joins), of many units with one long one among
+# short and empty ones, of all units at once; several eights of heads.
+LONG = [([60000], 1, 4, 64, 16, None), ([30001], 2, 16, 128, 64, None), ([20000, 0, 17], 3, 1, 128, 20, None), ([9000], 4, 40, 64, 16, None),
+        ([1, 0, 40000, 5, 300, 0, 77] + [10] * 60, 4, 2, 64, 16, None), ([700 + 13 * i for i in range(40)], 4, 8, 128, 16, None),
+        ([3000] * 20, 8, 1, 40, 32, 2000), ([25000] * 3, 1, 5, 256, 32, None), ([1500] * 80, 2, 3, 96, 24, None)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("lengths,heads,group,dim,page_size,window", LONG)
+def test_attention_shared_by_many(dtype, lengths, heads, group, dim, page_size, window):
+    from cuvs_b200 import kv_cache
+    g = generator(dim + len(lengths))
+    n_pages = sum(-(-n // page_size) for n in lengths) + 1
+    keys, values = layout((n_pages, page_size, heads, dim), dtype, g, "heads")
+    queries = rows((len(lengths), heads * group, dim), dtype, g, 2.0)
+    pages, n = tables(lengths, page_size, n_pages, g), ints(lengths)
+    out, lse = kv_cache.attention(keys, values, queries, pages, n, window=window)
+    check(out, lse, want_attention(keys, values, queries, pages, n, window=window))
+    for _ in range(5):
+        again, lse_again = kv_cache.attention(keys, values, queries, pages, n, window=window)
+        assert torch.equal(out, again) and torch.equal(lse, lse_again)
+    need = kv_cache.attention_workspace(keys, queries, pages, window)
+    own = torch.full((need + 16,), 255, dtype=torch.uint8, device="cuda")       # what a workspace held before does not matter
+    again, lse_again = kv_cache.attention(keys, values, queries, pages, n, window=window, workspace=own[:need] if need else None)
+    assert torch.equal(out, again) and torch.equal(lse, lse_again) and (own[need:] == 255).all()
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("page_size", [16, 20])
 def test_what_may_not_be_attended_is_not_read(dtype, page_size):
