@@ -343,12 +343,11 @@ bool attention_call(resources& res, cudaStream_t stream, kv::attention_args a)
   std::unique_lock<std::mutex> held;
   if (need > 0 && a.workspace != nullptr) {
     CUVS_EXPECTS(a.workspace_bytes >= need, "workspace: %zu bytes, but %zu are needed", a.workspace_bytes, need);
-    CUDA_TRY(cudaMemsetAsync(a.workspace, 0, kv::attention_workspace_zeroed(res), stream));
   } else if (need > 0) {
     cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
     CUDA_TRY(cudaStreamIsCapturing(stream, &capturing));
     if (capturing != cudaStreamCaptureStatusNone) { return false; }
-    held = res.stream_workspace(stream, need, kv::attention_workspace_zeroed(res), &a.workspace);
+    held = res.stream_workspace(stream, need, &a.workspace);
   }
   kv::attention(res, stream, a);
   return true;

@@ -83,7 +83,7 @@ template <int D, int NT, int WARPS>
 struct mma_shape {
   static constexpr int kRows     = 8 * NT;
   static constexpr int kChunk    = 16;
-  static constexpr int kStages   = D == 64 ? 4 : D == 128 ? 2 : 3;
+  static constexpr int kStages   = D == 64 ? 4 : D == 256 && NT == 1 ? 3 : 2;
   static constexpr bool kQInRegs = D * NT <= 256;
   static constexpr int kResident = WARPS > kSmall || D == 256 ? 1 : NT == 4 ? 2 : 3;  // blocks of an SM
   static constexpr int kRowBytes = D * 2;
@@ -91,103 +91,111 @@ struct mma_shape {
   static constexpr int kAccRow   = D + 4;                                    // floats: lanes of a store on different banks
   static constexpr int kBuffers  = WARPS * kStages * kStage;
   static constexpr int kAcc      = WARPS * kRows * kAccRow * 4;
-  static constexpr int kQBytes   = kQInRegs ? 0 : kRows * kRowBytes;
+  static constexpr int kQBytes   = kQInRegs ? 0 : kRows * kRowBytes;       // of a warp
   static constexpr int kStatsAt  = kBuffers > kAcc ? kBuffers : kAcc;
   static constexpr int kJoinedAt = kStatsAt + WARPS * kRows * 8;
   static constexpr int kQAt      = kJoinedAt + kRows * 8;
-  static constexpr int kMaskAt   = kQAt + kQBytes;
-  static constexpr int kShared   = kMaskAt + WARPS * kStages * 4;
+  static constexpr int kMaskAt   = kQAt + WARPS * kQBytes;
+  static constexpr int kPortion  = (D / 16 * 4 + 4) * 32;                    // floats that a warp sends another: the sums of eight heads
+  static constexpr int kExchangeAt = kMaskAt + WARPS * 16;
+  static constexpr int kShared   = kExchangeAt + (WARPS == kSmall ? WARPS / 2 * kPortion * 4 : 0);
 };
 
-// Warps work alone: each has every fourth 16 positions of a unit, copies their rows ahead into its own part of shared memory, and keeps
-// its own top, sum and weighted sum.  Scores are formed as keys x queries (S^T: 16 keys by 8 query heads) and outputs as values x weights
-// (O^T: 16 columns by 8 heads), so that 8 query heads fill a product.  A thread of quad g, place t has keys g and g + 8 of heads 2t and
-// 2t + 1; turning its weights as a matrix makes them the second operand of the second product.
+// Warps work alone: each copies its rows ahead into its own part of shared memory, and keeps its own top, sum and weighted sum.  Scores are
+// formed as keys x queries (S^T: 16 keys by 8 query heads) and outputs as values x weights (O^T: 16 columns by 8 heads), so that 8 query heads fill
+// a product.  A thread of quad g, place t has keys g and g + 8 of heads 2t and 2t + 1; turning its weights as a matrix makes them the second
+// operand of the second product.
 template <typename T, int D, int NT, int WARPS, bool WHOLE_PAGES>
-__global__ void __launch_bounds__(WARPS * 32, mma_shape<D, NT, WARPS>::kResident)
-mma_kernel(cache_view c, work_view w, positions lists, rows_view queries, result_view result, float scale_log2, parts_view parts)
-{
-  using shape       = mma_shape<D, NT, WARPS>;
-  constexpr int S   = shape::kStages;
-  constexpr int PR  = D / 8;  // pieces of a row in shared memory
-  extern __shared__ __align__(128) char smem[];
-  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
-  const uint32_t g = lane >> 2, t = lane & 3u;
-  const block_state state{reinterpret_cast<float*>(smem), reinterpret_cast<float2*>(smem + shape::kStatsAt),
-                          reinterpret_cast<float2*>(smem + shape::kJoinedAt), shape::kAccRow};
-  uint32_t* s_mask       = reinterpret_cast<uint32_t*>(smem + shape::kMaskAt) + warp * S;
-  const uint32_t buffers = shared_address(smem) + warp * (S * shape::kStage);
-  const uint32_t s_q     = shared_address(smem + shape::kQAt);
-  const uint32_t pieces  = c.dim / 8;
+struct mma_hooks {
+  using shape                    = mma_shape<D, NT, WARPS>;
+  static constexpr int PR        = D / 8;   // pieces of a row in shared memory
+  static constexpr int ROWS      = 32 / PR; // a copy of a warp: one piece of every lane, so many rows
+  static constexpr int kPortion  = shape::kPortion;
+  static constexpr int kPortions = NT;
+
+  const cache_view& c;
+  const work_view& w;
+  const rows_view& queries;
+  const result_view& result;
+  const parts_view& parts;
+  const block_state& state;
+  char* smem;
+  float scale_log2;
+  uint32_t warp, lane, g, t;
+  uint32_t buffers, s_q;
   // Copies: a lane has one piece of every ROWS-th row.  Pieces stand in a row's place by place ^ (row & 7), so that eight rows' pieces of one
   // column lie on different banks; behind the row's end they are 0.
-  constexpr int ROWS          = 32 / PR;
-  const uint32_t copy_row     = lane / PR;
-  const uint32_t copy_swizzle = ((lane % PR) ^ copy_row) << 4;
-  const uint32_t copy_bytes   = lane % PR < pieces ? 16u : 0u;
-  const uint32_t copy_from    = lane % PR < pieces ? (lane % PR) * 16u : 0u;
-  const uint64_t k_rows_on    = uint64_t(c.k_token_units * ROWS) << c.unit_shift;
-  const uint64_t v_rows_on    = uint64_t(c.v_token_units * ROWS) << c.unit_shift;
-  chain_begin();
-
+  uint32_t copy_row, copy_swizzle, copy_bytes, copy_from;
+  const char *keys, *values;
   float acc[NT][D / 16][4], top[NT][2], sum[NT][2];
+  uint32_t q[shape::kQInRegs ? NT : 1][shape::kQInRegs ? D / 16 : 1][2];  // the second operand of the first product
 
-  auto body = [&](uint32_t sequence, uint32_t unit, const positions::list& l, uint32_t chunk0, uint32_t end, uint32_t step) {
-    const uint32_t head = unit / w.n_blocks_of, of = unit - head * w.n_blocks_of;
-    const uint32_t rows  = min(uint32_t(shape::kRows), w.group - of * shape::kRows);
-    const uint32_t head0 = head * w.group + of * shape::kRows;
-    const char* keys     = c.keys + int64_t(head) * c.k_head * 2 + copy_from;
-    const char* values   = c.values + int64_t(head) * c.v_head * 2 + copy_from;
-    row_stream<16, positions> stream(c, lists, l, chunk0, end, step);
-    uint32_t filling = 0, emptying = 0;  // stages
-    auto copy_rows = [&](uint32_t chunk) {
-      uint32_t page, place;
-      const bool there    = stream.next(chunk, page, place);
-      const uint32_t mask = __ballot_sync(kAllLanes, there) & 0xFFFFu;
-      if (lane == 0) { s_mask[filling] = mask; }
-      if (mask == 0u) { return; }
-      const uint32_t to = buffers + filling * shape::kStage + copy_row * shape::kRowBytes;
-      uint32_t k_at, v_at;
-      const char *k_from, *v_from;
-      if constexpr (WHOLE_PAGES) {
-        // all 16 rows are in the page of any of them, whether they are to be read or not; `place` is that of the lane's own row
-        page   = __shfl_sync(kAllLanes, page, __ffs(int(mask)) - 1);
-        place  = place - (lane & 15u) + copy_row;
-        k_from = keys + (uint64_t(page * c.k_page_units + place * c.k_token_units) << c.unit_shift);
-        v_from = values + (uint64_t(page * c.v_page_units + place * c.v_token_units) << c.unit_shift);
-      } else {
-        k_at = there ? page * c.k_page_units + place * c.k_token_units : 0u;
-        v_at = there ? page * c.v_page_units + place * c.v_token_units : 0u;
-      }
+  __device__ __forceinline__ mma_hooks(const cache_view& c_, const work_view& w_, const rows_view& queries_, const result_view& result_,
+                                       const parts_view& parts_, const block_state& state_, char* smem_, float scale_log2_)
+    : c(c_), w(w_), queries(queries_), result(result_), parts(parts_), state(state_), smem(smem_), scale_log2(scale_log2_),
+      warp(threadIdx.x >> 5), lane(threadIdx.x & 31u), g((threadIdx.x & 31u) >> 2), t(threadIdx.x & 3u)
+  {
+    buffers      = shared_address(smem) + warp * (shape::kStages * shape::kStage);
+    s_q          = shared_address(smem + shape::kQAt);
+    copy_row     = lane / PR;
+    copy_swizzle = ((lane % PR) ^ copy_row) << 4;
+    copy_bytes   = lane % PR < c.dim / 8 ? 16u : 0u;
+    copy_from    = lane % PR < c.dim / 8 ? (lane % PR) * 16u : 0u;
+  }
+
+  __device__ __forceinline__ void attach(uint32_t unit)
+  {
+    const uint32_t head = unit / w.n_blocks_of;
+    keys                = c.keys + int64_t(head) * c.k_head * 2 + copy_from;
+    values              = c.values + int64_t(head) * c.v_head * 2 + copy_from;
+  }
+
+  __device__ __forceinline__ uint32_t copy(uint32_t stage, uint32_t page, uint32_t place, bool there)
+  {
+    const uint32_t mask = __ballot_sync(kAllLanes, there) & 0xFFFFu;
+    if (mask == 0u) { return 0u; }
+    const uint32_t to = buffers + stage * shape::kStage + copy_row * shape::kRowBytes;
+    uint32_t k_at, v_at;
+    const char *k_from, *v_from;
+    if constexpr (WHOLE_PAGES) {
+      // all 16 rows are in the page of any of them, whether they are to be read or not; `place` is that of the lane's own row
+      page   = __shfl_sync(kAllLanes, page, __ffs(int(mask)) - 1);
+      place  = place - (lane & 15u) + copy_row;
+      k_from = keys + (uint64_t(page * c.k_page_units + place * c.k_token_units) << c.unit_shift);
+      v_from = values + (uint64_t(page * c.v_page_units + place * c.v_token_units) << c.unit_shift);
+    } else {
+      k_at = there ? page * c.k_page_units + place * c.k_token_units : 0u;
+      v_at = there ? page * c.v_page_units + place * c.v_token_units : 0u;
+    }
+    const uint64_t k_rows_on = uint64_t(c.k_token_units * ROWS) << c.unit_shift, v_rows_on = uint64_t(c.v_token_units * ROWS) << c.unit_shift;
 #pragma unroll
-      for (int i = 0; i < 16 / ROWS; i++) {
-        const uint32_t at = to + i * (ROWS * shape::kRowBytes) + (copy_swizzle ^ ((i * ROWS & 7) << 4));
-        if constexpr (!WHOLE_PAGES) {
-          k_from = keys + (uint64_t(__shfl_sync(kAllLanes, k_at, copy_row + i * ROWS)) << c.unit_shift);
-          v_from = values + (uint64_t(__shfl_sync(kAllLanes, v_at, copy_row + i * ROWS)) << c.unit_shift);
-        }
-        const uint32_t bytes = ((mask >> (copy_row + i * ROWS)) & 1u) != 0u ? copy_bytes : 0u;
-        copy_piece(at, k_from, bytes);
-        copy_piece(at + 16 * shape::kRowBytes, v_from, bytes);
-        if constexpr (WHOLE_PAGES) {
-          k_from += k_rows_on;
-          v_from += v_rows_on;
-        }
+    for (int i = 0; i < 16 / ROWS; i++) {
+      const uint32_t at = to + i * (ROWS * shape::kRowBytes) + (copy_swizzle ^ ((i * ROWS & 7) << 4));
+      if constexpr (!WHOLE_PAGES) {
+        k_from = keys + (uint64_t(__shfl_sync(kAllLanes, k_at, copy_row + i * ROWS)) << c.unit_shift);
+        v_from = values + (uint64_t(__shfl_sync(kAllLanes, v_at, copy_row + i * ROWS)) << c.unit_shift);
       }
-    };
-    auto advance = [&](uint32_t chunk) {
-      if (chunk < end) { copy_rows(chunk); }
-      copies_end_group();  // past the unit's end an empty one
-      filling = filling + 1 == S ? 0 : filling + 1;
-    };
+      const uint32_t bytes = ((mask >> (copy_row + i * ROWS)) & 1u) != 0u ? copy_bytes : 0u;
+      copy_piece(at, k_from, bytes);
+      copy_piece(at + 16 * shape::kRowBytes, v_from, bytes);
+      if constexpr (WHOLE_PAGES) {
+        k_from += k_rows_on;
+        v_from += v_rows_on;
+      }
+    }
+    return mask;
+  }
 
-    // queries: the second operand of the first product
-    uint32_t q[shape::kQInRegs ? NT : 1][shape::kQInRegs ? D / 16 : 1][2];
+  __device__ __forceinline__ void start(uint32_t sequence, uint32_t unit)
+  {
+    const uint32_t head = unit / w.n_blocks_of, of = unit - head * w.n_blocks_of;
+    const uint32_t rows = min(uint32_t(shape::kRows), w.group - of * shape::kRows), head0 = head * w.group + of * shape::kRows;
+    const char* first   = queries.data + (int64_t(sequence) * queries.row + int64_t(head0) * queries.head) * 2;
     if constexpr (shape::kQInRegs) {
 #pragma unroll
       for (int n = 0; n < NT; n++) {
-        const uint32_t r    = n * 8 + g;
-        const char* row     = queries.data + (int64_t(sequence) * queries.row + int64_t(head0 + r) * queries.head) * 2;
+        const uint32_t r = n * 8 + g;
+        const char* row  = first + int64_t(r) * queries.head * 2;
 #pragma unroll
         for (int k = 0; k < D / 16; k++) {
 #pragma unroll
@@ -198,17 +206,16 @@ mma_kernel(cache_view c, work_view w, positions lists, rows_view queries, result
         }
       }
     } else {
-      for (uint32_t i = threadIdx.x; i < uint32_t(shape::kRows * PR); i += WARPS * 32) {
+      // the warp's own copy: warps are not at the same piece at the same time
+      __syncwarp();
+      for (uint32_t i = lane; i < uint32_t(shape::kRows * PR); i += 32) {
         const uint32_t r = i / PR, piece = i % PR;
         uint4 x          = make_uint4(0, 0, 0, 0);
-        if (r < rows && piece < pieces) {
-          x = reinterpret_cast<const uint4*>(queries.data + (int64_t(sequence) * queries.row + int64_t(head0 + r) * queries.head) * 2)[piece];
-        }
-        *reinterpret_cast<uint4*>(smem + shape::kQAt + r * shape::kRowBytes + ((piece ^ (r & 7u)) << 4)) = x;
+        if (r < rows && piece < c.dim / 8) { x = reinterpret_cast<const uint4*>(first + int64_t(r) * queries.head * 2)[piece]; }
+        *reinterpret_cast<uint4*>(smem + shape::kQAt + warp * shape::kQBytes + r * shape::kRowBytes + ((piece ^ (r & 7u)) << 4)) = x;
       }
-      __syncthreads();
+      __syncwarp();
     }
-
 #pragma unroll
     for (int n = 0; n < NT; n++) {
 #pragma unroll
@@ -216,109 +223,101 @@ mma_kernel(cache_view c, work_view w, positions lists, rows_view queries, result
       top[n][0] = top[n][1] = -INFINITY;
       sum[n][0] = sum[n][1] = 0.0f;
     }
+  }
 
+  __device__ __forceinline__ void consume(uint32_t stage, uint32_t mask)
+  {
+    const uint32_t k_rows = buffers + stage * shape::kStage, v_rows = k_rows + 16 * shape::kRowBytes;
+    float s[NT][4] = {};
 #pragma unroll
-    for (int i = 0; i < S; i++) { advance(chunk0 + i * step); }
-
-    for (uint32_t chunk = chunk0; chunk < end; chunk += step) {
-      copies_wait<S - 1>();
-      __syncwarp();
-      const uint32_t stage = emptying;
-      emptying             = emptying + 1 == S ? 0 : emptying + 1;
-      const uint32_t mask  = s_mask[stage];
-      if (mask != 0u) {
-        const uint32_t k_rows = buffers + stage * shape::kStage, v_rows = k_rows + 16 * shape::kRowBytes;
-        float s[NT][4] = {};
+    for (int k = 0; k < D / 16; k++) {
+      uint32_t a[4];
+      const uint32_t row = (lane & 7u) + (lane & 8u), piece = k * 2 + (lane >> 4);
+      load_matrices(a, k_rows + row * shape::kRowBytes + ((piece ^ (row & 7u)) << 4));
+      if constexpr (shape::kQInRegs) {
 #pragma unroll
-        for (int k = 0; k < D / 16; k++) {
-          uint32_t a[4];
-          const uint32_t row = (lane & 7u) + (lane & 8u), piece = k * 2 + (lane >> 4);
-          load_matrices(a, k_rows + row * shape::kRowBytes + ((piece ^ (row & 7u)) << 4));
-          if constexpr (shape::kQInRegs) {
+        for (int n = 0; n < NT; n++) { multiply_add<T>(s[n], a, q[n][k][0], q[n][k][1]); }
+      } else {
+        // two eights of heads at a time: matrices (heads 0-7, columns 0-7), (0-7, 8-15), (8-15, 0-7), (8-15, 8-15)
 #pragma unroll
-            for (int n = 0; n < NT; n++) { multiply_add<T>(s[n], a, q[n][k][0], q[n][k][1]); }
-          } else {
-            // two eights of heads at a time: matrices (heads 0-7, columns 0-7), (0-7, 8-15), (8-15, 0-7), (8-15, 8-15)
-#pragma unroll
-            for (int n = 0; n < NT; n += 2) {
-              uint32_t b[4];
-              const uint32_t r = n * 8 + (lane & 7u) + ((lane >> 4) << 3), p = k * 2 + ((lane >> 3) & 1u);
-              load_matrices(b, s_q + r * shape::kRowBytes + ((p ^ (r & 7u)) << 4));
-              multiply_add<T>(s[n], a, b[0], b[1]);
-              multiply_add<T>(s[n + 1], a, b[2], b[3]);
-            }
-          }
+        for (int n = 0; n < NT; n += 2) {
+          uint32_t b[4];
+          const uint32_t r = n * 8 + (lane & 7u) + ((lane >> 4) << 3), p = k * 2 + ((lane >> 3) & 1u);
+          load_matrices(b, s_q + warp * shape::kQBytes + r * shape::kRowBytes + ((p ^ (r & 7u)) << 4));
+          multiply_add<T>(s[n], a, b[0], b[1]);
+          multiply_add<T>(s[n + 1], a, b[2], b[3]);
         }
-        const bool k0 = ((mask >> g) & 1u) != 0u, k1 = ((mask >> (g + 8)) & 1u) != 0u;
-        float next[NT][2];
-        bool higher = false;
+      }
+    }
+    const bool k0 = ((mask >> g) & 1u) != 0u, k1 = ((mask >> (g + 8)) & 1u) != 0u;
+    float next[NT][2];
+    bool higher = false;
 #pragma unroll
-        for (int n = 0; n < NT; n++) {
-          s[n][0] = k0 ? s[n][0] * scale_log2 : -INFINITY;
-          s[n][1] = k0 ? s[n][1] * scale_log2 : -INFINITY;
-          s[n][2] = k1 ? s[n][2] * scale_log2 : -INFINITY;
-          s[n][3] = k1 ? s[n][3] * scale_log2 : -INFINITY;
+    for (int n = 0; n < NT; n++) {
+      s[n][0] = k0 ? s[n][0] * scale_log2 : -INFINITY;
+      s[n][1] = k0 ? s[n][1] * scale_log2 : -INFINITY;
+      s[n][2] = k1 ? s[n][2] * scale_log2 : -INFINITY;
+      s[n][3] = k1 ? s[n][3] * scale_log2 : -INFINITY;
 #pragma unroll
-          for (int h = 0; h < 2; h++) {
-            float m = fmaxf(s[n][h], s[n][h + 2]);
+      for (int h = 0; h < 2; h++) {
+        float m = fmaxf(s[n][h], s[n][h + 2]);
 #pragma unroll
-            for (int o = 4; o < 32; o <<= 1) { m = fmaxf(m, __shfl_xor_sync(kAllLanes, m, o)); }
-            next[n][h] = fmaxf(top[n][h], m);
-            higher     = higher || next[n][h] > top[n][h];
-          }
-        }
-        if (__any_sync(kAllLanes, higher)) {
+        for (int o = 4; o < 32; o <<= 1) { m = fmaxf(m, __shfl_xor_sync(kAllLanes, m, o)); }
+        next[n][h] = fmaxf(top[n][h], m);
+        higher     = higher || next[n][h] > top[n][h];
+      }
+    }
+    if (__any_sync(kAllLanes, higher)) {
 #pragma unroll
-          for (int n = 0; n < NT; n++) {
-            float keep[2];
+      for (int n = 0; n < NT; n++) {
+        float keep[2];
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-              keep[h]   = power_of_2(top[n][h] - finite_top(next[n][h]));
-              top[n][h] = next[n][h];
-              sum[n][h] *= keep[h];
-            }
-#pragma unroll
-            for (int d = 0; d < D / 16; d++) {
-              acc[n][d][0] *= keep[0];
-              acc[n][d][1] *= keep[1];
-              acc[n][d][2] *= keep[0];
-              acc[n][d][3] *= keep[1];
-            }
-          }
-        }
-        uint32_t high[NT][2], low[NT][2];
-#pragma unroll
-        for (int n = 0; n < NT; n++) {
-          float p[4];
-#pragma unroll
-          for (int e = 0; e < 4; e++) {
-            p[e] = power_of_2(s[n][e] - (finite_top(top[n][e & 1]) - halves<T>::kShift));
-            sum[n][e & 1] += p[e];
-          }
-#pragma unroll
-          for (int h = 0; h < 2; h++) {
-            high[n][h]       = halves<T>::pack(p[2 * h] * halves<T>::kBelow, p[2 * h + 1] * halves<T>::kBelow);
-            const float2 was = halves<T>::unpack(high[n][h]);
-            low[n][h]        = turn_matrix(halves<T>::pack(p[2 * h] - was.x, p[2 * h + 1] - was.y));
-            high[n][h]       = turn_matrix(high[n][h]);
-          }
+        for (int h = 0; h < 2; h++) {
+          keep[h]   = power_of_2(top[n][h] - finite_top(next[n][h]));
+          top[n][h] = next[n][h];
+          sum[n][h] *= keep[h];
         }
 #pragma unroll
         for (int d = 0; d < D / 16; d++) {
-          uint32_t a[4];
-          const uint32_t row = (lane & 7u) + ((lane >> 4) << 3), piece = d * 2 + ((lane >> 3) & 1u);
-          load_matrices_turned(a, v_rows + row * shape::kRowBytes + ((piece ^ (row & 7u)) << 4));
-#pragma unroll
-          for (int n = 0; n < NT; n++) {
-            multiply_add<T>(acc[n][d], a, high[n][0], high[n][1]);
-            multiply_add<T>(acc[n][d], a, low[n][0], low[n][1]);
-          }
+          acc[n][d][0] *= keep[0];
+          acc[n][d][1] *= keep[1];
+          acc[n][d][2] *= keep[0];
+          acc[n][d][3] *= keep[1];
         }
       }
-      __syncwarp();
-      advance(chunk + S * step);
     }
-    copies_wait<0>();
+    uint32_t high[NT][2], low[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+      float p[4];
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        p[e] = power_of_2(s[n][e] - (finite_top(top[n][e & 1]) - halves<T>::kShift));
+        sum[n][e & 1] += p[e];
+      }
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        high[n][h]       = halves<T>::pack(p[2 * h] * halves<T>::kBelow, p[2 * h + 1] * halves<T>::kBelow);
+        const float2 was = halves<T>::unpack(high[n][h]);
+        low[n][h]        = turn_matrix(halves<T>::pack(p[2 * h] - was.x, p[2 * h + 1] - was.y));
+        high[n][h]       = turn_matrix(high[n][h]);
+      }
+    }
+#pragma unroll
+    for (int d = 0; d < D / 16; d++) {
+      uint32_t a[4];
+      const uint32_t row = (lane & 7u) + ((lane >> 4) << 3), piece = d * 2 + ((lane >> 3) & 1u);
+      load_matrices_turned(a, v_rows + row * shape::kRowBytes + ((piece ^ (row & 7u)) << 4));
+#pragma unroll
+      for (int n = 0; n < NT; n++) {
+        multiply_add<T>(acc[n][d], a, high[n][0], high[n][1]);
+        multiply_add<T>(acc[n][d], a, low[n][0], low[n][1]);
+      }
+    }
+  }
+
+  __device__ __forceinline__ void close()
+  {
 #pragma unroll
     for (int n = 0; n < NT; n++) {
 #pragma unroll
@@ -327,9 +326,42 @@ mma_kernel(cache_view c, work_view w, positions lists, rows_view queries, result
         for (int o = 4; o < 32; o <<= 1) { sum[n][h] += __shfl_xor_sync(kAllLanes, sum[n][h], o); }
       }
     }
-  };
-  const float unshift = power_of_2(-halves<T>::kShift);
-  auto to_shared      = [&] {
+  }
+
+  // a lane's own values to the same lane of another warp
+  __device__ __forceinline__ void send(int n, float* to) const
+  {
+    float4* at = reinterpret_cast<float4*>(to) + lane;
+    at[0]      = make_float4(top[n][0], top[n][1], sum[n][0], sum[n][1]);
+#pragma unroll
+    for (int d = 0; d < D / 16; d++) { at[32 * (d + 1)] = make_float4(acc[n][d][0], acc[n][d][1], acc[n][d][2], acc[n][d][3]); }
+  }
+  __device__ __forceinline__ void receive(int n, const float* from)
+  {
+    const float4* at   = reinterpret_cast<const float4*>(from) + lane;
+    const float4 stats = at[0];
+    float own[2], theirs[2];
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      const float other = h == 0 ? stats.x : stats.y, next = fmaxf(top[n][h], other), safe = finite_top(next);
+      own[h]    = power_of_2(top[n][h] - safe);
+      theirs[h] = power_of_2(other - safe);
+      sum[n][h] = sum[n][h] * own[h] + (h == 0 ? stats.z : stats.w) * theirs[h];
+      top[n][h] = next;
+    }
+#pragma unroll
+    for (int d = 0; d < D / 16; d++) {
+      const float4 y = at[32 * (d + 1)];
+      acc[n][d][0]   = acc[n][d][0] * own[0] + y.x * theirs[0];
+      acc[n][d][1]   = acc[n][d][1] * own[1] + y.y * theirs[1];
+      acc[n][d][2]   = acc[n][d][2] * own[0] + y.z * theirs[0];
+      acc[n][d][3]   = acc[n][d][3] * own[1] + y.w * theirs[1];
+    }
+  }
+
+  __device__ __forceinline__ void to_shared() const
+  {
+    const float unshift = power_of_2(-halves<T>::kShift);
 #pragma unroll
     for (int n = 0; n < NT; n++) {
 #pragma unroll
@@ -344,9 +376,12 @@ mma_kernel(cache_view c, work_view w, positions lists, rows_view queries, result
         }
       }
     }
-  };
+  }
+
   // A store of a warp is eight neighbouring columns of four rows.
-  auto to_rows = [&](uint32_t rows, uint32_t sequence, uint32_t head0, bool whole, uint32_t part) {
+  __device__ __forceinline__ void to_rows(uint32_t rows, uint32_t sequence, uint32_t head0, bool whole, uint32_t part) const
+  {
+    const float unshift = power_of_2(-halves<T>::kShift);
 #pragma unroll
     for (int n = 0; n < NT; n++) {
 #pragma unroll
@@ -375,8 +410,22 @@ mma_kernel(cache_view c, work_view w, positions lists, rows_view queries, result
         }
       }
     }
-  };
-  each_unit<T, WARPS, shape::kChunk, 2>(c, w, lists, result, parts, state, body, to_shared, to_rows);
+  }
+};
+
+template <typename T, int D, int NT, int WARPS, bool WHOLE_PAGES>
+__global__ void __launch_bounds__(WARPS * 32, mma_shape<D, NT, WARPS>::kResident)
+mma_kernel(cache_view c, work_view w, positions lists, rows_view queries, result_view result, float scale_log2, parts_view parts)
+{
+  using shape = mma_shape<D, NT, WARPS>;
+  extern __shared__ __align__(128) char smem[];
+  const block_state state{reinterpret_cast<float*>(smem), reinterpret_cast<float2*>(smem + shape::kStatsAt),
+                          reinterpret_cast<float2*>(smem + shape::kJoinedAt), shape::kAccRow};
+  uint32_t* s_mask = reinterpret_cast<uint32_t*>(smem + shape::kMaskAt) + (threadIdx.x >> 5) * shape::kStages;
+  chain_begin();
+  mma_hooks<T, D, NT, WARPS, WHOLE_PAGES> hooks(c, w, queries, result, parts, state, smem, scale_log2);
+  run_units<T, WARPS, shape::kChunk, shape::kStages>(c, w, lists, result, parts, state, reinterpret_cast<float*>(smem + shape::kExchangeAt), s_mask,
+                                                     hooks);
 }
 
 }  // namespace

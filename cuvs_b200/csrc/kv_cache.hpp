@@ -85,8 +85,6 @@ struct attention_args {
 // How many bytes of workspace attention() wants, by sizes alone.
 size_t attention_workspace(const resources& res, elem type, uint32_t n_sequences, uint32_t n_query_heads, uint32_t n_heads, uint32_t dim,
                            uint64_t capacity, int64_t window);
-// Its first bytes, which have to be 0 and are left 0.
-size_t attention_workspace_zeroed(const resources& res);
 void attention(resources& res, cudaStream_t stream, const attention_args& a);
 
 struct candidates_args {

@@ -20,15 +20,16 @@ constexpr uint32_t chunk_of(uint32_t pieces, uint32_t heads)
   const uint32_t most = heads == 1 ? 16 : 32, rows = (heads == 1 ? 128 : 256) / pieces;
   return rows < most ? rows : most;
 }
-constexpr uint32_t resident_of(uint32_t heads) { return heads == 1 ? 6 : 3; }   // small blocks of an SM
-constexpr int large_of(uint32_t heads) { return heads == 1 ? 24 : 12; }         // warps of a large block
+// Small blocks of an SM and warps of a large block: what registers leave room for (the way through shares takes some).
+constexpr uint32_t resident_of(uint32_t heads, bool shares) { return heads > 1 ? 3 : shares ? 4 : 6; }
+constexpr int large_of(uint32_t heads, bool shares) { return heads > 1 ? 12 : shares ? 16 : 24; }
 
 // LANES lanes have a row, PIECES 16-byte pieces each; R query heads share its reading.
-template <typename T, int LANES, int PIECES, int R, int WARPS>
+template <typename T, int LANES, int PIECES, int R, int WARPS, bool SHARES>
 struct rows_shape {
   static constexpr int kPitch    = LANES * PIECES * 16;                    // bytes of a row in shared memory
   static constexpr int kChunk    = chunk_of(LANES * PIECES, R);            // rows of a warp's stage
-  static constexpr int kStages   = kPitch < 128 ? 4 : 2;
+  static constexpr int kStages   = kPitch < 128 ? 4 : R == 1 && SHARES ? 3 : 2;
   static constexpr int kGroups   = 32 / LANES;
   static constexpr int kTurns    = kChunk / kGroups;                       // rows of a lane group in a stage
   static constexpr int kColumns  = LANES * PIECES * kPerPiece<T>;
@@ -36,75 +37,83 @@ struct rows_shape {
   static constexpr int kStatsAt  = WARPS * kStages * kStage;
   static constexpr int kJoinedAt = kStatsAt + WARPS * R * 8;
   static constexpr int kMaskAt   = kJoinedAt + R * 8;
-  static constexpr int kShared   = kMaskAt + WARPS * kStages * 4;
+  static constexpr int kPortion  = (2 + PIECES * kPerPiece<T>) * 32;         // floats that a warp sends another: the sums of a query head
+  static constexpr int kExchangeAt = kMaskAt + WARPS * 16;
+  static constexpr int kShared   = kExchangeAt + (WARPS == kSmall && SHARES ? WARPS / 2 * kPortion * 4 : 0);
   static_assert(WARPS * R * kColumns * 4 <= kStatsAt, "the warps' sums take the stages' place");
 };
 
-template <typename T, int LANES, int PIECES, int R, int WARPS, class Lists>
-__global__ void __launch_bounds__(WARPS * 32, WARPS == kSmall ? resident_of(R) : 1)
-rows_kernel(cache_view c, work_view w, Lists lists, rows_view queries, result_view result, float scale_log2, parts_view parts)
-{
-  using shape          = rows_shape<T, LANES, PIECES, R, WARPS>;
-  constexpr int E      = kPerPiece<T>;
-  constexpr int S      = shape::kStages;
-  constexpr int CHUNK  = shape::kChunk;
-  constexpr int PR     = LANES * PIECES;
-  constexpr int U      = shape::kTurns < 4 ? shape::kTurns : 4;  // rows that a lane group takes at a time
-  extern __shared__ __align__(128) char smem[];
-  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
-  const uint32_t group = lane / LANES, gl = lane % LANES;
-  const block_state state{reinterpret_cast<float*>(smem), reinterpret_cast<float2*>(smem + shape::kStatsAt),
-                          reinterpret_cast<float2*>(smem + shape::kJoinedAt), shape::kColumns};
-  uint32_t* s_mask       = reinterpret_cast<uint32_t*>(smem + shape::kMaskAt) + warp * S;
-  const char* stages     = smem + warp * (S * shape::kStage);
-  const uint32_t buffers = shared_address(stages);
-  const uint32_t pieces  = c.dim / E;
-  // Copies: a lane has one piece (of 64: two) of every ROWS-th row.
-  constexpr int ROWS           = LANES == 32 ? 1 : 32 / PR;
-  const uint32_t copy_row      = LANES == 32 ? 0u : lane / PR;
-  const uint32_t copy_piece_of = LANES == 32 ? lane : lane % PR;
-  chain_begin();
+template <typename T, int LANES, int PIECES, int R, int WARPS, bool SHARES>
+struct rows_hooks {
+  using shape                    = rows_shape<T, LANES, PIECES, R, WARPS, SHARES>;
+  static constexpr int E         = kPerPiece<T>;
+  static constexpr int CHUNK     = shape::kChunk;
+  static constexpr int U         = shape::kTurns < 4 ? shape::kTurns : 4;  // rows that a lane group takes at a time
+  static constexpr int ROWS      = LANES == 32 ? 1 : 32 / LANES;           // a copy of a warp: one piece of every lane (of 64: two), so many rows
 
-  float acc[R][PIECES][E], top[R], sum[R];
+  static constexpr int kPortion  = shape::kPortion;
+  static constexpr int kPortions = R;
 
-  auto body = [&](uint32_t sequence, uint32_t unit, const typename Lists::list& l, uint32_t chunk0, uint32_t end, uint32_t step) {
-    const uint32_t head = unit / w.n_blocks_of, of = unit - head * w.n_blocks_of;
-    const uint32_t rows  = min(uint32_t(R), w.group - of * R);
-    const uint32_t head0 = head * w.group + of * R;
-    const char* keys     = c.keys + int64_t(head) * c.k_head * int64_t(sizeof(T));
-    const char* values   = c.values + int64_t(head) * c.v_head * int64_t(sizeof(T));
-    row_stream<CHUNK, Lists> stream(c, lists, l, chunk0, end, step);
-    uint32_t filling = 0, emptying = 0;  // stages
-    auto advance = [&](uint32_t chunk) {
-      if (chunk < end) {
-        uint32_t page, place;
-        const bool there    = stream.next(chunk, page, place);
-        const uint32_t mask = __ballot_sync(kAllLanes, there) & uint32_t((uint64_t(1) << CHUNK) - 1u);
-        if (lane == 0) { s_mask[filling] = mask; }
-        if (mask != 0u) {
-          const uint32_t to   = buffers + filling * shape::kStage + copy_row * shape::kPitch + copy_piece_of * 16;
-          const uint32_t k_at = there ? page * c.k_page_units + place * c.k_token_units : 0u;
-          const uint32_t v_at = there ? page * c.v_page_units + place * c.v_token_units : 0u;
+  const cache_view& c;
+  const work_view& w;
+  const rows_view& queries;
+  const result_view& result;
+  const parts_view& parts;
+  const block_state& state;
+  float scale_log2;
+  uint32_t warp, lane, group, gl;
+  const char* stages;
+  uint32_t buffers, copy_row, copy_piece_of;
+  const char *keys, *values;
+  float q[R][PIECES][E], acc[R][PIECES][E], top[R], sum[R];
+
+  __device__ __forceinline__ rows_hooks(const cache_view& c_, const work_view& w_, const rows_view& queries_, const result_view& result_,
+                                        const parts_view& parts_, const block_state& state_, const char* smem, float scale_log2_)
+    : c(c_), w(w_), queries(queries_), result(result_), parts(parts_), state(state_), scale_log2(scale_log2_), warp(threadIdx.x >> 5),
+      lane(threadIdx.x & 31u), group((threadIdx.x & 31u) / LANES), gl((threadIdx.x & 31u) % LANES)
+  {
+    stages        = smem + warp * (shape::kStages * shape::kStage);
+    buffers       = shared_address(stages);
+    copy_row      = LANES == 32 ? 0u : lane / LANES;
+    copy_piece_of = LANES == 32 ? lane : lane % LANES;
+  }
+  __device__ __forceinline__ uint32_t pieces() const { return c.dim / E; }
+
+  __device__ __forceinline__ void attach(uint32_t unit)
+  {
+    const uint32_t head = unit / w.n_blocks_of;
+    keys                = c.keys + int64_t(head) * c.k_head * int64_t(sizeof(T));
+    values              = c.values + int64_t(head) * c.v_head * int64_t(sizeof(T));
+  }
+
+  __device__ __forceinline__ uint32_t copy(uint32_t stage, uint32_t page, uint32_t place, bool there)
+  {
+    const uint32_t mask = __ballot_sync(kAllLanes, there) & uint32_t((uint64_t(1) << CHUNK) - 1u);
+    if (mask == 0u) { return 0u; }
+    const uint32_t to   = buffers + stage * shape::kStage + copy_row * shape::kPitch + copy_piece_of * 16;
+    const uint32_t k_at = there ? page * c.k_page_units + place * c.k_token_units : 0u;
+    const uint32_t v_at = there ? page * c.v_page_units + place * c.v_token_units : 0u;
 #pragma unroll
-          for (int i = 0; i < CHUNK / ROWS; i++) {
-            const char* k_from = keys + (uint64_t(__shfl_sync(kAllLanes, k_at, copy_row + i * ROWS)) << c.unit_shift);
-            const char* v_from = values + (uint64_t(__shfl_sync(kAllLanes, v_at, copy_row + i * ROWS)) << c.unit_shift);
-            const bool read    = ((mask >> (copy_row + i * ROWS)) & 1u) != 0u;
+    for (int i = 0; i < CHUNK / ROWS; i++) {
+      const char* k_from = keys + (uint64_t(__shfl_sync(kAllLanes, k_at, copy_row + i * ROWS)) << c.unit_shift);
+      const char* v_from = values + (uint64_t(__shfl_sync(kAllLanes, v_at, copy_row + i * ROWS)) << c.unit_shift);
+      const bool read    = ((mask >> (copy_row + i * ROWS)) & 1u) != 0u;
 #pragma unroll
-            for (int p = 0; p < PIECES; p++) {
-              const uint32_t piece = copy_piece_of + p * 32, bytes = read && piece < pieces ? 16u : 0u;
-              const uint32_t at   = to + i * (ROWS * shape::kPitch) + p * 512;
-              copy_piece(at, k_from + (piece < pieces ? piece * 16 : 0), bytes);
-              copy_piece(at + CHUNK * shape::kPitch, v_from + (piece < pieces ? piece * 16 : 0), bytes);
-            }
-          }
-        }
+      for (int p = 0; p < PIECES; p++) {
+        const uint32_t piece = copy_piece_of + p * 32, bytes = read && piece < pieces() ? 16u : 0u;
+        const uint32_t at    = to + i * (ROWS * shape::kPitch) + p * 512;
+        copy_piece(at, k_from + (piece < pieces() ? piece * 16 : 0), bytes);
+        copy_piece(at + CHUNK * shape::kPitch, v_from + (piece < pieces() ? piece * 16 : 0), bytes);
       }
-      copies_end_group();  // past the unit's end an empty one
-      filling = filling + 1 == S ? 0 : filling + 1;
-    };
+    }
+    return mask;
+  }
 
-    float q[R][PIECES][E];
+  __device__ __forceinline__ void start(uint32_t sequence, uint32_t unit)
+  {
+    const uint32_t head = unit / w.n_blocks_of, of = unit - head * w.n_blocks_of;
+    const uint32_t rows = min(uint32_t(R), w.group - of * R), head0 = head * w.group + of * R;
+    const char* first   = queries.data + (int64_t(sequence) * queries.row + int64_t(head0) * queries.head) * int64_t(sizeof(T));
 #pragma unroll
     for (int r = 0; r < R; r++) {
       top[r] = -INFINITY;
@@ -113,93 +122,83 @@ rows_kernel(cache_view c, work_view w, Lists lists, rows_view queries, result_vi
       for (int p = 0; p < PIECES; p++) {
         const uint32_t j = gl + p * LANES;
         uint4 x          = make_uint4(0, 0, 0, 0);
-        if (uint32_t(r) < rows && j < pieces) {
-          x = reinterpret_cast<const uint4*>(queries.data + (int64_t(sequence) * queries.row + int64_t(head0 + r) * queries.head) *
-                                                              int64_t(sizeof(T)))[j];
-        }
+        if (uint32_t(r) < rows && j < pieces()) { x = reinterpret_cast<const uint4*>(first + int64_t(r) * queries.head * int64_t(sizeof(T)))[j]; }
         piece_to_floats<T>(x, q[r][p]);
 #pragma unroll
         for (int e = 0; e < E; e++) { acc[r][p][e] = 0.0f; }
       }
     }
-#pragma unroll
-    for (int i = 0; i < S; i++) { advance(chunk0 + i * step); }
+  }
 
-    for (uint32_t chunk = chunk0; chunk < end; chunk += step) {
-      copies_wait<S - 1>();
-      __syncwarp();
-      const uint32_t stage = emptying;
-      emptying             = emptying + 1 == S ? 0 : emptying + 1;
-      const uint32_t mask  = s_mask[stage];
-      if (mask != 0u) {
-        const char* k_rows = stages + stage * shape::kStage;
-        const char* v_rows = k_rows + CHUNK * shape::kPitch;
+  __device__ __forceinline__ void consume(uint32_t stage, uint32_t mask)
+  {
+    const char* k_rows = stages + stage * shape::kStage;
+      const char* v_rows = k_rows + CHUNK * shape::kPitch;
 #pragma unroll 1
-        for (int u0 = 0; u0 < shape::kTurns; u0 += U) {
-          float score[R][U];
+      for (int u0 = 0; u0 < shape::kTurns; u0 += U) {
+        float score[R][U];
 #pragma unroll
-          for (int u = 0; u < U; u++) {
-            const uint32_t row = uint32_t(u0 + u) * shape::kGroups + group;
-            float x[PIECES][E];
+        for (int u = 0; u < U; u++) {
+          const uint32_t row = uint32_t(u0 + u) * shape::kGroups + group;
+          float x[PIECES][E];
 #pragma unroll
-            for (int p = 0; p < PIECES; p++) {
-              piece_to_floats<T>(*reinterpret_cast<const uint4*>(k_rows + row * shape::kPitch + (gl + p * LANES) * 16), x[p]);
-            }
-            const bool ok = ((mask >> row) & 1u) != 0u;
-#pragma unroll
-            for (int r = 0; r < R; r++) {
-              float s = 0.0f;
-#pragma unroll
-              for (int p = 0; p < PIECES; p++) {
-#pragma unroll
-                for (int e = 0; e < E; e++) { s = fmaf(q[r][p][e], x[p][e], s); }
-              }
-#pragma unroll
-              for (int o = LANES / 2; o > 0; o >>= 1) { s += __shfl_xor_sync(kAllLanes, s, o); }
-              score[r][u] = ok ? s * scale_log2 : -INFINITY;
-            }
+          for (int p = 0; p < PIECES; p++) {
+            piece_to_floats<T>(*reinterpret_cast<const uint4*>(k_rows + row * shape::kPitch + (gl + p * LANES) * 16), x[p]);
           }
+          const bool ok = ((mask >> row) & 1u) != 0u;
 #pragma unroll
           for (int r = 0; r < R; r++) {
-            float next = top[r];
-#pragma unroll
-            for (int u = 0; u < U; u++) { next = fmaxf(next, score[r][u]); }
-            const float safe = finite_top(next);
-            const float keep = power_of_2(top[r] - safe);
-            top[r]           = next;
-            sum[r] *= keep;
+            float s = 0.0f;
 #pragma unroll
             for (int p = 0; p < PIECES; p++) {
 #pragma unroll
-              for (int e = 0; e < E; e++) { acc[r][p][e] *= keep; }
+              for (int e = 0; e < E; e++) { s = fmaf(q[r][p][e], x[p][e], s); }
             }
 #pragma unroll
-            for (int u = 0; u < U; u++) {
-              score[r][u] = power_of_2(score[r][u] - safe);
-              sum[r] += score[r][u];
-            }
+            for (int o = LANES / 2; o > 0; o >>= 1) { s += __shfl_xor_sync(kAllLanes, s, o); }
+            score[r][u] = ok ? s * scale_log2 : -INFINITY;
+          }
+        }
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+          float next = top[r];
+#pragma unroll
+          for (int u = 0; u < U; u++) { next = fmaxf(next, score[r][u]); }
+          const float safe = finite_top(next);
+          const float keep = power_of_2(top[r] - safe);
+          top[r]           = next;
+          sum[r] *= keep;
+#pragma unroll
+          for (int p = 0; p < PIECES; p++) {
+#pragma unroll
+            for (int e = 0; e < E; e++) { acc[r][p][e] *= keep; }
           }
 #pragma unroll
           for (int u = 0; u < U; u++) {
-            const uint32_t row = uint32_t(u0 + u) * shape::kGroups + group;
+            score[r][u] = power_of_2(score[r][u] - safe);
+            sum[r] += score[r][u];
+          }
+        }
 #pragma unroll
-            for (int p = 0; p < PIECES; p++) {
-              float x[E];
-              piece_to_floats<T>(*reinterpret_cast<const uint4*>(v_rows + row * shape::kPitch + (gl + p * LANES) * 16), x);
+        for (int u = 0; u < U; u++) {
+          const uint32_t row = uint32_t(u0 + u) * shape::kGroups + group;
 #pragma unroll
-              for (int r = 0; r < R; r++) {
+          for (int p = 0; p < PIECES; p++) {
+            float x[E];
+            piece_to_floats<T>(*reinterpret_cast<const uint4*>(v_rows + row * shape::kPitch + (gl + p * LANES) * 16), x);
 #pragma unroll
-                for (int e = 0; e < E; e++) { acc[r][p][e] = fmaf(score[r][u], x[e], acc[r][p][e]); }
-              }
+            for (int r = 0; r < R; r++) {
+#pragma unroll
+              for (int e = 0; e < E; e++) { acc[r][p][e] = fmaf(score[r][u], x[e], acc[r][p][e]); }
             }
           }
         }
       }
-      __syncwarp();
-      advance(chunk + S * step);
-    }
-    copies_wait<0>();
-    // the warp's lane groups
+  }
+
+  // the warp's lane groups
+  __device__ __forceinline__ void close()
+  {
 #pragma unroll
     for (int r = 0; r < R; r++) {
 #pragma unroll
@@ -217,26 +216,54 @@ rows_kernel(cache_view c, work_view w, Lists lists, rows_view queries, result_vi
         top[r] = next;
       }
     }
-  };
-  auto to_floats = [&](float* row, int r) {
+  }
+
+  // a lane's own values to the same lane of another warp
+  __device__ __forceinline__ void send(int r, float* to) const
+  {
+    to[lane]      = top[r];
+    to[lane + 32] = sum[r];
+#pragma unroll
+    for (int p = 0; p < PIECES; p++) {
+#pragma unroll
+      for (int e = 0; e < E; e++) { to[lane + 32 * (2 + p * E + e)] = acc[r][p][e]; }
+    }
+  }
+  __device__ __forceinline__ void receive(int r, const float* from)
+  {
+    const float other = from[lane], next = fmaxf(top[r], other), safe = finite_top(next);
+    const float own = power_of_2(top[r] - safe), theirs = power_of_2(other - safe);
+    sum[r] = sum[r] * own + from[lane + 32] * theirs;
+    top[r] = next;
+#pragma unroll
+    for (int p = 0; p < PIECES; p++) {
+#pragma unroll
+      for (int e = 0; e < E; e++) { acc[r][p][e] = acc[r][p][e] * own + from[lane + 32 * (2 + p * E + e)] * theirs; }
+    }
+  }
+
+  __device__ __forceinline__ void to_floats(float* row, int r) const
+  {
 #pragma unroll
     for (int p = 0; p < PIECES; p++) {
 #pragma unroll
       for (int e = 0; e < E; e += 4) {
-        if (gl + p * LANES < pieces) {
+        if (gl + p * LANES < pieces()) {
           *reinterpret_cast<float4*>(row + (gl + p * LANES) * E + e) = make_float4(acc[r][p][e], acc[r][p][e + 1], acc[r][p][e + 2], acc[r][p][e + 3]);
         }
       }
     }
-  };
-  auto to_shared = [&] {
+  }
+  __device__ __forceinline__ void to_shared() const
+  {
 #pragma unroll
     for (int r = 0; r < R; r++) {
       if (group == 0) { to_floats(state.acc + (warp * R + r) * shape::kColumns, r); }
       if (lane == 0) { state.stats[warp * R + r] = make_float2(top[r], sum[r]); }
     }
-  };
-  auto to_rows = [&](uint32_t rows, uint32_t sequence, uint32_t head0, bool whole, uint32_t part) {
+  }
+  __device__ __forceinline__ void to_rows(uint32_t rows, uint32_t sequence, uint32_t head0, bool whole, uint32_t part) const
+  {
     if (group != 0) { return; }
 #pragma unroll
     for (int r = 0; r < R; r++) {
@@ -245,7 +272,7 @@ rows_kernel(cache_view c, work_view w, Lists lists, rows_view queries, result_vi
         const float scale = sum[r] == 0.0f ? 0.0f : 1.0f / sum[r];
 #pragma unroll
         for (int p = 0; p < PIECES; p++) {
-          if (gl + p * LANES < pieces) {
+          if (gl + p * LANES < pieces()) {
             float x[E];
 #pragma unroll
             for (int e = 0; e < E; e++) { x[e] = acc[r][p][e] * scale; }
@@ -258,8 +285,22 @@ rows_kernel(cache_view c, work_view w, Lists lists, rows_view queries, result_vi
         if (gl == 0) { parts.stats[size_t(part) * parts.rows + r] = make_float2(top[r], sum[r]); }
       }
     }
-  };
-  each_unit<T, WARPS, CHUNK, R == 1 ? 1 : 2>(c, w, lists, result, parts, state, body, to_shared, to_rows);
+  }
+};
+
+template <typename T, int LANES, int PIECES, int R, int WARPS, class Lists>
+__global__ void __launch_bounds__(WARPS * 32, WARPS == kSmall ? resident_of(R, Lists::kShares) : 1)
+rows_kernel(cache_view c, work_view w, Lists lists, rows_view queries, result_view result, float scale_log2, parts_view parts)
+{
+  using shape = rows_shape<T, LANES, PIECES, R, WARPS, Lists::kShares>;
+  extern __shared__ __align__(128) char smem[];
+  const block_state state{reinterpret_cast<float*>(smem), reinterpret_cast<float2*>(smem + shape::kStatsAt),
+                          reinterpret_cast<float2*>(smem + shape::kJoinedAt), shape::kColumns};
+  uint32_t* s_mask = reinterpret_cast<uint32_t*>(smem + shape::kMaskAt) + (threadIdx.x >> 5) * shape::kStages;
+  chain_begin();
+  rows_hooks<T, LANES, PIECES, R, WARPS, Lists::kShares> hooks(c, w, queries, result, parts, state, smem, scale_log2);
+  run_units<T, WARPS, shape::kChunk, shape::kStages>(c, w, lists, result, parts, state, reinterpret_cast<float*>(smem + shape::kExchangeAt), s_mask,
+                                                     hooks);
 }
 
 // How rows of so many 16-byte pieces are read.
@@ -297,8 +338,8 @@ plan attention_plan(const resources& res, elem type, uint64_t sequences, uint32_
     p.rows     = dim > 128 ? std::min(group, 4u) : group > 4 ? 8 : group;
     p.rows     = p.rows == 3 ? 4 : p.rows;
     p.chunk    = chunk_of(room_of(dim / 4), p.rows);
-    p.resident = resident_of(p.rows);
-    p.large    = large_of(p.rows);
+    p.resident = resident_of(p.rows, true);
+    p.large    = large_of(p.rows, true);
   } else {
     const uint32_t d = padded(dim), eights = group <= 8 ? 1 : group <= 16 || d == 256 ? 2 : 4;
     p.rows     = 8 * eights;
@@ -313,13 +354,13 @@ plan attention_plan(const resources& res, elem type, uint64_t sequences, uint32_
 template <typename T, int LANES, int PIECES, int R, class Lists, typename... Args>
 void launch_rows(cudaStream_t stream, const plan& p, Args&&... args)
 {
-  constexpr int LARGE = large_of(R);
+  constexpr int LARGE = large_of(R, Lists::kShares);
   if (p.warps == uint32_t(LARGE)) {
     launch_units(stream, rows_kernel<T, LANES, PIECES, R, LARGE, Lists>, p.blocks, LARGE * 32, p.cluster,
-                 rows_shape<T, LANES, PIECES, R, LARGE>::kShared, args...);
+                 rows_shape<T, LANES, PIECES, R, LARGE, Lists::kShares>::kShared, args...);
   } else {
     launch_units(stream, rows_kernel<T, LANES, PIECES, R, kSmall, Lists>, p.blocks, kSmall * 32, p.cluster,
-                 rows_shape<T, LANES, PIECES, R, kSmall>::kShared, args...);
+                 rows_shape<T, LANES, PIECES, R, kSmall, Lists::kShares>::kShared, args...);
   }
 }
 
@@ -332,8 +373,8 @@ void launch_candidates(resources& res, cudaStream_t stream, const candidates_arg
   plan p{};
   p.rows = parts.rows = 1;
   p.chunk             = chunk_of(room_of(pieces), 1);
-  p.resident          = resident_of(1);
-  p.large             = large_of(1);
+  p.resident          = resident_of(1, false);
+  p.large             = large_of(1, false);
   deal_out(res, p, uint64_t(a.n_tokens) * a.n_query_heads, a.n_candidates, false);
   const work_view w{a.n_tokens, a.n_query_heads, group, group, p.cluster, false};
   by_pieces(pieces, [&](auto lanes, auto n) {
@@ -350,9 +391,8 @@ size_t attention_workspace(const resources& res, elem type, uint32_t n_sequences
                            uint64_t capacity, int64_t window)
 {
   const plan p = attention_plan(res, type, n_sequences, n_heads, n_query_heads / n_heads, dim, capacity, window);
-  return p.parts ? arrived_bytes(res) + part_bytes(p.teams(), p.rows, dim) : 0;
+  return p.parts ? part_bytes(p.shares(), p.rows, dim) : 0;
 }
-size_t attention_workspace_zeroed(const resources& res) { return arrived_bytes(res); }
 
 void attention(resources& res, cudaStream_t stream, const attention_args& a)
 {
@@ -365,15 +405,20 @@ void attention(resources& res, cudaStream_t stream, const attention_args& a)
   const positions lists{a.pages, a.lengths, a.table_stride, a.window, a.table_width};
   const result_view result{a.out, a.lse};
   parts_view parts{};
-  parts.teams = p.teams();
-  parts.rows  = p.rows;
-  if (p.parts) {
-    parts.arrived = reinterpret_cast<uint32_t*>(a.workspace);
-    parts.acc     = reinterpret_cast<float*>(a.workspace + arrived_bytes(res));
-    parts.stats   = reinterpret_cast<float2*>(parts.acc + size_t(2) * parts.teams * p.rows * c.dim);
+  if (p.parts) { parts = parts_at(a.workspace, p.shares(), p.rows, c.dim); }
+  parts.shares = p.shares();
+  parts.rows   = p.rows;
+  auto join    = [&](auto type) {
+    if (p.parts) { launch_join<decltype(type)>(res, stream, p, w, parts, c.dim, c.n_heads, result); }
+  };
+  if (a.type == elem::f16) {
+    attention16<__half>(stream, a, p, w, lists, result, parts);
+    return join(__half{});
   }
-  if (a.type == elem::f16) { return attention16<__half>(stream, a, p, w, lists, result, parts); }
-  if (a.type == elem::bf16) { return attention16<__nv_bfloat16>(stream, a, p, w, lists, result, parts); }
+  if (a.type == elem::bf16) {
+    attention16<__nv_bfloat16>(stream, a, p, w, lists, result, parts);
+    return join(__nv_bfloat16{});
+  }
   by_pieces(c.dim / 4, [&](auto lanes, auto n) {
     constexpr int LANES = decltype(lanes)::value, PIECES = decltype(n)::value;
     auto go = [&](auto r) {
@@ -390,6 +435,7 @@ void attention(resources& res, cudaStream_t stream, const attention_args& a)
       go(integral_constant<int, 8>{});
     }
   });
+  join(float{});
 }
 
 void attend_candidates(resources& res, cudaStream_t stream, const candidates_args& a)

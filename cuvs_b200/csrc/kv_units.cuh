@@ -3,15 +3,18 @@
 // A unit is a (sequence, key head, block of query heads) with its list of rows, cut into chunks of as many rows as a warp takes at a time.
 // Two ways to deal the chunks out:
 //
-// Shares.  All units' chunks stand in one row, and each of a fixed number of teams -- the resident blocks, or their warps -- takes an equal,
-// contiguous share of it, whatever the lengths are (they are known on the device alone: every warp finds its share from them itself).  A
-// unit that lies in one share is finished there; of a unit that several share, each team leaves a part (top, sum and weighted sum in 32
-// bits).  Parts are joined in a tree, eight neighbours at a time, by whichever of the eight comes last; the order of the sums does not
-// depend on who that is.  Warps as teams need no barrier and never wait for one another between units: for many units.  Blocks as teams
-// leave a quarter of the parts: for few and long ones.
+// Shares.  All units' chunks stand in one row, and each of the resident teams -- blocks, or their warps -- takes an equal, contiguous share of
+// it, whatever the lengths are (they are known on the device alone: every warp finds its share from them itself).  A unit that lies in one share
+// is finished there; of a unit that several share, each team leaves a part (top, sum and weighted sum in 32 bits), and a second kernel joins
+// the parts in the order of the shares.  A warp copies the first rows of the next unit while it finishes this one.  The warps of a block team
+// take a unit's chunks in turn and join through shared memory at its end; warps as teams need no barrier, but leave four times the parts: they
+// are for units that are many and short (256 requests of up to 1,024 tokens, 2,048 units: 134 us with blocks, 103 with warps; 32 of up to 16,384,
+// 256 units: 151 and 175).
 //
-// Clusters.  One cluster of blocks per unit, whose blocks take equal runs of its chunks and join their parts through each other's shared
-// memory: no workspace and the shortest way to the end, but no balance between units: for few units with few rows.
+// Clusters.  One cluster of blocks per unit, whose warps take its chunks in turn and join their parts through shared memory, their own and
+// each other's: no workspace, one launch and the shortest way to the end, but no balance between units: for few units with few rows.
+//
+// Nothing depends on the order in which blocks run.
 #pragma once
 
 #include "kv_rows.cuh"
@@ -24,8 +27,7 @@ namespace cuvs_b200::kv {
 
 // Warps of a block: small blocks, several to an SM, balance best; where units are fewer than SMs, one large block has an SM's warps for one
 // unit.
-constexpr int kSmall     = 4;
-constexpr int kMostTeams = 24;  // warps of an SM, at most, where they are teams
+constexpr int kSmall = 4;
 
 struct work_view {
   uint32_t n_sequences;
@@ -113,23 +115,24 @@ __device__ __forceinline__ uint64_t quotient(uint64_t a, uint32_t b)
   return a >> 32 == 0 ? uint64_t(uint32_t(a) / b) : a / b;  // the short division where it is enough
 }
 
-// `total` chunks of all units dealt out to `teams` (at most one per chunk): the first `longer` get `each` + 1, the others `each`.
+// `total` chunks of all units dealt out in `count` equal shares, each of kLeast chunks at least while there are fewer than all warps could take.
 struct share {
+  static constexpr uint32_t kLeast = 4;  // chunks
   uint64_t total, each;
-  uint32_t teams, longer;
+  uint32_t count, longer;  // the first `longer` get `each` + 1, the others `each`
   __device__ __forceinline__ share(uint64_t total_, uint32_t most)
-    : total(total_), each(0), teams(uint32_t(min(uint64_t(most), total_))), longer(0)
+    : total(total_), each(0), count(uint32_t(min(uint64_t(most), ceildiv<uint64_t>(total_, kLeast)))), longer(0)
   {
-    if (teams != 0u) {
-      each   = quotient(total, teams);
-      longer = uint32_t(total - each * teams);
+    if (count != 0u) {
+      each   = quotient(total, count);
+      longer = uint32_t(total - each * count);
     }
   }
-  __device__ __forceinline__ uint64_t start(uint32_t team) const { return team * each + min(team, longer); }
-  __device__ __forceinline__ uint32_t team_of(uint64_t chunk) const
+  __device__ __forceinline__ uint64_t start(uint32_t i) const { return i * each + min(i, longer); }
+  __device__ __forceinline__ uint32_t of(uint64_t chunk) const  // the share that has it
   {
-    const uint64_t edge = longer * (each + 1);  // `each` is below 2^32 as long as there are fewer than 2^32 chunks per team
-    return chunk < edge ? uint32_t(quotient(chunk, uint32_t(each + 1))) : longer + uint32_t(quotient(chunk - edge, uint32_t(each)));
+    const uint64_t middle = longer * (each + 1);
+    return chunk < middle ? uint32_t(quotient(chunk, uint32_t(each + 1))) : longer + uint32_t(quotient(chunk - middle, uint32_t(each)));
   }
 };
 
@@ -197,24 +200,28 @@ __device__ __forceinline__ uint32_t sequence_of(const cache_view& c, const work_
 
 // ---- parts --------------------------------------------------------------------------------------------------------------------
 
-constexpr uint32_t kFan    = 8;  // parts that are joined at a time
-constexpr uint32_t kLevels = 4;  // of the tree, at most: fewer than 4,096 teams
-
-// Two parts per team: 0 of a unit that a team before began, 1 of a unit that this team begins and a later one goes on with.
+// Two parts per share: 0 of a unit that a share before began, 1 of a unit that this share begins and a later one goes on with.
 struct parts_view {
-  uint32_t* arrived;  // [levels][2 teams] how many of a node's parts are there; 0 between calls
-  float* acc;         // [2 teams][rows][dim]
-  float2* stats;      // [2 teams][rows] top (of scores in powers of two), sum
-  uint32_t teams;
+  float* acc;     // [2 shares][rows][dim]
+  float2* stats;  // [2 shares][rows] top (of scores in powers of two), sum
+  uint4* begun;   // [shares] the unit that share i begins and does not end: sequence, unit, how many parts it has (0: there is none)
+  uint32_t shares;
   uint32_t rows;  // query heads of a unit, at most
 };
 
-// A workspace begins with `arrived`, as large as any call's, so that calls of different sizes can follow one another in it.
-inline size_t arrived_bytes(uint32_t teams) { return size_t(kLevels) * 2 * teams * sizeof(uint32_t); }
-inline size_t arrived_bytes(const resources& res) { return round_up<size_t>(arrived_bytes(uint32_t(res.sm_count) * kMostTeams), 256); }
-inline size_t part_bytes(uint32_t teams, uint32_t rows, uint32_t dim)
+inline size_t part_bytes(uint32_t shares, uint32_t rows, uint32_t dim)
 {
-  return size_t(2) * teams * rows * (dim * sizeof(float) + sizeof(float2));
+  return size_t(shares) * (sizeof(uint4) + 2 * rows * (dim * sizeof(float) + sizeof(float2)));
+}
+inline parts_view parts_at(char* workspace, uint32_t shares, uint32_t rows, uint32_t dim)
+{
+  parts_view p;
+  p.begun  = reinterpret_cast<uint4*>(workspace);
+  p.acc    = reinterpret_cast<float*>(p.begun + shares);
+  p.stats  = reinterpret_cast<float2*>(p.acc + size_t(2) * shares * rows * dim);
+  p.shares = shares;
+  p.rows   = rows;
+  return p;
 }
 
 struct result_view {
@@ -237,11 +244,10 @@ struct block_state {
   uint32_t acc_row;
 };
 
-// Joins the warps: the block's sums become output rows (whole), a part in the workspace, or warp 0's sums (for the cluster).
-enum { TO_OUTPUT, TO_PART, TO_CLUSTER };
+// Joins the warps: the block's sums become output rows, or warp 0's sums (for the cluster).
 template <typename T, int WARPS>
 __device__ __forceinline__ void join_warps(const cache_view& c, const work_view& w, const block_state& s, uint32_t rows, uint32_t sequence,
-                                           uint32_t head0, const result_view& result, int to, const parts_view& parts, uint32_t part)
+                                           uint32_t head0, const result_view& result, bool clustered, const parts_view& parts)
 {
   constexpr uint32_t E  = kPerPiece<T>;
   const uint32_t pieces = c.dim / E;
@@ -268,18 +274,17 @@ __device__ __forceinline__ void join_warps(const cache_view& c, const work_view&
         x[e + 3]       = fmaf(y.w, f, x[e + 3]);
       }
     }
-    if (to == TO_OUTPUT) {
+    if (!clustered) {
       const float scale = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
       for (uint32_t e = 0; e < E; e++) { x[e] *= scale; }
       store_piece<T>(result.out, sequence, head0 + r, piece, x);
       if (piece == 0) { result.lse[size_t(sequence) * (w.group * c.n_heads) + head0 + r] = (safe + log2f(sum)) * kLn2; }
     } else {
-      float* base = to == TO_PART ? parts.acc + (size_t(part) * parts.rows + r) * c.dim : s.acc + size_t(r) * s.acc_row;
-      float4* a   = reinterpret_cast<float4*>(base + piece * E);
+      float4* a = reinterpret_cast<float4*>(s.acc + size_t(r) * s.acc_row + piece * E);
 #pragma unroll
       for (uint32_t e = 0; e < E; e += 4) { a[e / 4] = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]); }
-      if (piece == 0) { (to == TO_PART ? parts.stats + size_t(part) * parts.rows : s.joined)[r] = make_float2(top, sum); }
+      if (piece == 0) { s.joined[r] = make_float2(top, sum); }
     }
   }
 }
@@ -341,187 +346,202 @@ __device__ __forceinline__ void empty_rows(const cache_view& c, const work_view&
   }
 }
 
-// Joins a unit's n parts, of which this team has just written number k: up the tree as long as the team is the last of its node to come.
-// Part 0 is the second of team `first`, part i the first of team first + i.  A node's joined part takes the place of its first one.
-template <typename T, int THREADS, uint32_t B>
-__device__ __forceinline__ void join_tree(const cache_view& c, const work_view& w, const parts_view& parts, uint32_t first, uint32_t n, uint32_t k,
-                                          uint32_t rows, uint32_t sequence, uint32_t head0, const result_view& result)
+// ---- joining parts ------------------------------------------------------------------------------------------------------------
+
+constexpr int kJoinWarps = 16, kJoinAlone = 16;
+
+// A row of a unit with n parts, of which this warp takes every `step`-th from `from` on: their top and sum, and the weighted sum in columns
+// 4 * lane and 128 + 4 * lane on.
+__device__ __forceinline__ void join_some(const parts_view& parts, uint32_t share, uint32_t n, uint32_t r, uint32_t dim, uint32_t from, uint32_t step,
+                                          float& top, float& sum, float (&x)[2][4])
 {
-  constexpr int E = 4;
-  const uint32_t thread = THREADS == 32 ? threadIdx.x & 31u : threadIdx.x;
-  auto place  = [&](uint32_t p) { return p == 0 ? 2 * first + 1 : 2 * (first + p); };
-  auto team_sync = [] {
-    if constexpr (THREADS == 32) {
-      __syncwarp();
-    } else {
-      __syncthreads();
-    }
-  };
-  __shared__ uint32_t s_last;  // of block teams
-  uint32_t step = 1;           // parts of a node's child
-  for (uint32_t level = 0; level < kLevels; level++, step *= kFan) {
-    const uint32_t node    = k / (step * kFan) * (step * kFan);  // its first part
-    const uint32_t members = min(kFan, (n - node + step - 1) / step);
-    const bool root        = node == 0 && n <= step * kFan;
-    if (members > 1) {
-      __threadfence();
-      team_sync();
-      uint32_t last = 0;
-      if (thread == 0) { last = atomicInc(parts.arrived + size_t(level) * 2 * parts.teams + place(node), members - 1) == members - 1; }
-      if constexpr (THREADS == 32) {
-        last = __shfl_sync(kAllLanes, last, 0);
-      } else {
-        if (thread == 0) { s_last = last; }
-        __syncthreads();
-        last = s_last;
-      }
-      if (last == 0u) { return; }
-      __threadfence();
-      // a row's pieces of four columns lie side by side in the team's threads; B for a thread at a time
-      const uint32_t pieces = c.dim / E, items = rows * pieces;
-      for (uint32_t i0 = thread; i0 < items; i0 += B * THREADS) {
-        float2 st[B][kFan];
-        float4 y[B][kFan];
+  const uint32_t lane = threadIdx.x & 31u;
+  auto place          = [&](uint32_t p) { return size_t(p == 0 ? 2 * share + 1 : 2 * (share + p)) * parts.rows + r; };
+  top                 = -INFINITY;
+  for (uint32_t p = from + lane * step; p < n; p += 32 * step) { top = fmaxf(top, parts.stats[place(p)].x); }
 #pragma unroll
-        for (uint32_t u = 0; u < B; u++) {
-          const uint32_t i = min(i0 + u * THREADS, items - 1), r = i / pieces, piece = i - r * pieces;
+  for (int o = 16; o > 0; o >>= 1) { top = fmaxf(top, __shfl_xor_sync(kAllLanes, top, o)); }
+  const float safe = finite_top(top);
+  sum              = 0.0f;
 #pragma unroll
-          for (uint32_t m = 0; m < kFan; m++) {
-            const size_t at = size_t(place(node + min(m, members - 1) * step)) * parts.rows + r;
-            st[u][m]        = __ldcg(parts.stats + at);
-            y[u][m]         = __ldcg(reinterpret_cast<const float4*>(parts.acc + at * c.dim) + piece);
-          }
-        }
+  for (int v = 0; v < 2; v++) { x[v][0] = x[v][1] = x[v][2] = x[v][3] = 0.0f; }
+  for (uint32_t p0 = from; p0 < n; p0 += 8 * step) {
+    float2 st[8];
+    uint4 y[2][8];
 #pragma unroll
-        for (uint32_t u = 0; u < B; u++) {
-          const uint32_t i = i0 + u * THREADS, r = i / pieces, piece = i - r * pieces;
-          if (i >= items) { continue; }
-          float top = -INFINITY, sum = 0.0f;
+    for (uint32_t i = 0; i < 8; i++) {
+      const uint32_t p = p0 + i * step;
+      const bool there = p < n;
+      const size_t at  = place(there ? p : 0u);
+      st[i]            = there ? parts.stats[at] : make_float2(-INFINITY, 0.0f);
 #pragma unroll
-          for (uint32_t m = 0; m < kFan; m++) { top = fmaxf(top, st[u][m].x); }  // (the last member again and again does no harm here)
-          const float safe = finite_top(top);
-          float x[E]       = {};
-#pragma unroll
-          for (uint32_t m = 0; m < kFan; m++) {
-            if (m < members) {
-              const float f = power_of_2(st[u][m].x - safe);
-              sum           = fmaf(st[u][m].y, f, sum);
-              x[0]          = fmaf(y[u][m].x, f, x[0]);
-              x[1]          = fmaf(y[u][m].y, f, x[1]);
-              x[2]          = fmaf(y[u][m].z, f, x[2]);
-              x[3]          = fmaf(y[u][m].w, f, x[3]);
-            }
-          }
-          if (root) {
-            const float scale = sum == 0.0f ? 0.0f : 1.0f / sum;
-            T* o = reinterpret_cast<T*>(result.out.data) + int64_t(sequence) * result.out.row + int64_t(head0 + r) * result.out.head + piece * E;
-            alignas(16) T z[E];
-#pragma unroll
-            for (int e = 0; e < E; e++) { z[e] = from_float<T>(x[e] * scale); }
-            if constexpr (sizeof(T) == 2) {
-              *reinterpret_cast<uint2*>(o) = *reinterpret_cast<const uint2*>(z);
-            } else {
-              *reinterpret_cast<uint4*>(o) = *reinterpret_cast<const uint4*>(z);
-            }
-            if (piece == 0) { result.lse[size_t(sequence) * (w.group * c.n_heads) + head0 + r] = (safe + log2f(sum)) * kLn2; }
-          } else {
-            // other threads of the team still read this row's old top and sum: both are written when all have read
-            const size_t at = size_t(place(node)) * parts.rows + r;
-            reinterpret_cast<float4*>(parts.acc + at * c.dim)[piece] = make_float4(x[0], x[1], x[2], x[3]);
-          }
-        }
-      }
-      if (!root) {
-        team_sync();
-        for (uint32_t r = thread; r < rows; r += THREADS) {
-          float top = -INFINITY, sum = 0.0f;
-          for (uint32_t m = 0; m < members; m++) { top = fmaxf(top, __ldcg(parts.stats + size_t(place(node + m * step)) * parts.rows + r).x); }
-          const float safe = finite_top(top);
-          for (uint32_t m = 0; m < members; m++) {
-            const float2 s = __ldcg(parts.stats + size_t(place(node + m * step)) * parts.rows + r);
-            sum            = fmaf(s.y, power_of_2(s.x - safe), sum);
-          }
-          parts.stats[size_t(place(node)) * parts.rows + r] = make_float2(top, sum);
-        }
+      for (int v = 0; v < 2; v++) {
+        const uint32_t column = 4 * lane + 128u * v;
+        y[v][i]               = load_piece(parts.acc + at * dim + column, there && column < dim);
       }
     }
-    if (root) { return; }
+#pragma unroll
+    for (uint32_t i = 0; i < 8; i++) {
+      const float f = power_of_2(st[i].x - safe);
+      sum           = fmaf(st[i].y, f, sum);
+#pragma unroll
+      for (int v = 0; v < 2; v++) {
+        x[v][0] = fmaf(__uint_as_float(y[v][i].x), f, x[v][0]);
+        x[v][1] = fmaf(__uint_as_float(y[v][i].y), f, x[v][1]);
+        x[v][2] = fmaf(__uint_as_float(y[v][i].z), f, x[v][2]);
+        x[v][3] = fmaf(__uint_as_float(y[v][i].w), f, x[v][3]);
+      }
+    }
   }
 }
 
-// Goes through what the team has to do, unit by unit.  body(sequence, unit, list, chunk, end, step): the warp's chunks of a unit, into its
-// registers; to_shared(): from there into the block's shared memory; to_rows(...): from there to output rows, or a part.
-template <typename T, int WARPS, int CHUNK, uint32_t B, class Lists, class Body, class ToShared, class ToRows>
-__device__ __forceinline__ void each_unit(const cache_view& c, const work_view& w, const Lists& lists, const result_view& result,
-                                          const parts_view& parts, const block_state& s, Body&& body, ToShared&& to_shared, ToRows&& to_rows)
+template <typename T>
+__device__ __forceinline__ void write_joined(const result_view& result, uint32_t sequence, uint32_t head, uint32_t heads, uint32_t dim, float top,
+                                             float sum, const float (&x)[2][4])
 {
-  const uint32_t warp = threadIdx.x >> 5;
-  typename Lists::list l;
-  auto heads_of = [&](uint32_t unit, uint32_t& rows, uint32_t& head0) {
-    const uint32_t head = unit / w.n_blocks_of, of = unit - head * w.n_blocks_of;
-    rows  = min(parts.rows, w.group - of * parts.rows);
-    head0 = head * w.group + of * parts.rows;
-  };
-  uint32_t rows, head0;
-  if (w.cluster != 0u) {
-    const uint32_t which = blockIdx.x / w.cluster, rank = blockIdx.x - which * w.cluster;
-    const uint32_t sequence = which / w.n_units, unit = which - sequence * w.n_units;
-    const uint32_t n = lists.open(c, sequence, CHUNK, l);
-    lists.select(c, w, sequence, unit, l);
-    body(sequence, unit, l, uint32_t(uint64_t(rank) * n / w.cluster) + warp, uint32_t(uint64_t(rank + 1) * n / w.cluster), WARPS);
-    heads_of(unit, rows, head0);
-    __syncthreads();  // shared memory changes hands: from rows to sums
-    to_shared();
-    __syncthreads();
-    join_warps<T, WARPS>(c, w, s, rows, sequence, head0, result, w.cluster > 1u ? TO_CLUSTER : TO_OUTPUT, parts, 0);
-    if (w.cluster > 1u) { join_cluster<T, WARPS>(c, w, s, rows, sequence, head0, result); }
-    return;
+  const uint32_t lane = threadIdx.x & 31u;
+  const float scale   = sum == 0.0f ? 0.0f : 1.0f / sum;
+  T* o                = reinterpret_cast<T*>(result.out.data) + int64_t(sequence) * result.out.row + int64_t(head) * result.out.head;
+#pragma unroll
+  for (int v = 0; v < 2; v++) {
+    const uint32_t column = 4 * lane + 128u * v;
+    if (column >= dim) { continue; }
+    alignas(16) T z[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) { z[e] = from_float<T>(x[v][e] * scale); }
+    if constexpr (sizeof(T) == 2) {
+      *reinterpret_cast<uint2*>(o + column) = *reinterpret_cast<const uint2*>(z);
+    } else {
+      *reinterpret_cast<uint4*>(o + column) = *reinterpret_cast<const uint4*>(z);
+    }
   }
-  if constexpr (Lists::kShares) {
-    const share all(all_chunks<CHUNK>(c, w, lists), parts.teams);
-    const uint32_t team = w.warp_teams ? blockIdx.x * WARPS + warp : blockIdx.x;
-    if (team < all.teams) {
-      uint64_t at = all.start(team), before;  // chunks: the next one, those before the sequence
-      const uint64_t stop = all.start(team + 1);
-      uint32_t sequence   = sequence_of<CHUNK>(c, w, lists, at, before);
-      uint32_t n          = sequence < w.n_sequences ? lists.open(c, sequence, CHUNK, l) : 0u;
-      while (at < stop) {
-        while (at >= before + uint64_t(n) * w.n_units) {  // on to the next sequence that has chunks
-          before += uint64_t(n) * w.n_units;
-          if (++sequence >= w.n_sequences) { break; }
-          n = lists.open(c, sequence, CHUNK, l);
-        }
-        if (sequence >= w.n_sequences) { break; }  // lengths that changed meanwhile
-        const uint32_t unit  = uint32_t(quotient(at - before, n));
-        const uint64_t begin = before + uint64_t(unit) * n, end = begin + n, last = min(stop, end);
-        lists.select(c, w, sequence, unit, l);
-        body(sequence, unit, l, uint32_t(at - begin) + (w.warp_teams ? 0u : warp), uint32_t(last - begin), w.warp_teams ? 1u : uint32_t(WARPS));
-        heads_of(unit, rows, head0);
-        const bool whole    = at == begin && last == end;
-        const uint32_t part = uint32_t(2 * team + (at == begin ? 1 : 0));
-        if (w.warp_teams) {
-          to_rows(rows, sequence, head0, whole, part);
-        } else {
-          __syncthreads();  // shared memory changes hands: from rows to sums
-          to_shared();
-          __syncthreads();
-          join_warps<T, WARPS>(c, w, s, rows, sequence, head0, result, whole ? TO_OUTPUT : TO_PART, parts, part);
-        }
-        if (!whole) {
-          const uint32_t first = all.team_of(begin), n_parts = all.team_of(end - 1) - first + 1u;
-          if (w.warp_teams) {
-            join_tree<T, 32, B>(c, w, parts, first, n_parts, team - first, rows, sequence, head0, result);
-          } else {
-            join_tree<T, WARPS * 32, B>(c, w, parts, first, n_parts, team - first, rows, sequence, head0, result);
-          }
-        }
-        if (!w.warp_teams) { __syncthreads(); }
-        at = last;
+  if (lane == 0) { result.lse[size_t(sequence) * heads + head] = (finite_top(top) + log2f(sum)) * kLn2; }
+}
+
+// Every warp looks at its (share, row) pairs: rows of a few parts are joined by the warp alone, those of many by the block's warps together.
+template <typename T>
+__global__ void __launch_bounds__(kJoinWarps * 32)
+join_kernel(work_view w, parts_view parts, uint32_t dim, uint32_t n_heads, result_view result)
+{
+  chain_begin();
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, heads = w.group * n_heads;
+  __shared__ uint32_t s_many[kJoinWarps], s_n;
+  __shared__ float4 s_x[kJoinWarps][64];
+  __shared__ float2 s_stats[kJoinWarps];
+  // neighbouring warps have different shares: the rows of a unit with many parts are those of different blocks
+  const uint32_t pairs = parts.shares * parts.rows, stride = gridDim.x * kJoinWarps;
+  auto row_of = [&](uint32_t pair, uint32_t& share, uint32_t& r, uint4& unit, uint32_t& head) -> bool {
+    r                = pair / parts.shares;
+    share            = pair - r * parts.shares;
+    unit             = parts.begun[share];
+    const uint32_t h = unit.y / w.n_blocks_of, of = unit.y - h * w.n_blocks_of;
+    head             = h * w.group + of * parts.rows + r;
+    return unit.z != 0u && of * parts.rows + r < w.group;
+  };
+  float top, sum, x[2][4];
+  for (uint32_t base = blockIdx.x * kJoinWarps; base < pairs; base += stride) {
+    if (threadIdx.x == 0) { s_n = 0u; }
+    __syncthreads();
+    uint32_t share, r, head;
+    uint4 unit;
+    if (base + warp < pairs && row_of(base + warp, share, r, unit, head)) {
+      if (unit.z <= uint32_t(kJoinAlone)) {
+        join_some(parts, share, unit.z, r, dim, 0u, 1u, top, sum, x);
+        write_joined<T>(result, unit.x, head, heads, dim, top, sum, x);
+      } else if (lane == 0) {
+        s_many[atomicAdd(&s_n, 1u)] = base + warp;
       }
     }
-    empty_rows<T, WARPS, CHUNK>(c, w, lists, result);
+    __syncthreads();
+    const uint32_t many = s_n;
+    for (uint32_t i = 0; i < many; i++) {
+      row_of(s_many[i], share, r, unit, head);
+      join_some(parts, share, unit.z, r, dim, warp, kJoinWarps, top, sum, x);
+      s_x[warp][lane]      = make_float4(x[0][0], x[0][1], x[0][2], x[0][3]);
+      s_x[warp][lane + 32] = make_float4(x[1][0], x[1][1], x[1][2], x[1][3]);
+      if (lane == 0) { s_stats[warp] = make_float2(top, sum); }
+      __syncthreads();
+      if (warp == 0) {
+        top = -INFINITY;
+#pragma unroll
+        for (int v = 0; v < kJoinWarps; v++) { top = fmaxf(top, s_stats[v].x); }
+        const float safe = finite_top(top);
+        sum              = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 4; e++) { x[0][e] = x[1][e] = 0.0f; }
+#pragma unroll
+        for (int v = 0; v < kJoinWarps; v++) {
+          const float f = power_of_2(s_stats[v].x - safe);
+          sum           = fmaf(s_stats[v].y, f, sum);
+#pragma unroll
+          for (int u = 0; u < 2; u++) {
+            const float4 y = s_x[v][lane + 32 * u];
+            x[u][0]        = fmaf(y.x, f, x[u][0]);
+            x[u][1]        = fmaf(y.y, f, x[u][1]);
+            x[u][2]        = fmaf(y.z, f, x[u][2]);
+            x[u][3]        = fmaf(y.w, f, x[u][3]);
+          }
+        }
+        write_joined<T>(result, unit.x, head, heads, dim, top, sum, x);
+      }
+      __syncthreads();
+    }
   }
 }
+
+// ---- pieces -------------------------------------------------------------------------------------------------------------------
+
+// What a share has of one unit: its chunks [chunk, end), which may be all of it.
+struct piece {
+  uint32_t sequence, unit, chunk, end;
+  uint32_t n_parts;  // of a unit that the piece begins and does not end
+  bool begins, whole;
+};
+
+// A team's way through its share, piece by piece; the warps of a block team all go it.
+template <int CHUNK, class Lists>
+struct walk {
+  const cache_view& c;
+  const work_view& w;
+  const Lists& lists;
+  typename Lists::list l;  // of the sequence that the walk is at
+  share all;
+  uint32_t mine;
+  uint64_t at, stop, before;
+  uint32_t sequence, n;
+
+  __device__ __forceinline__ walk(const cache_view& c_, const work_view& w_, const Lists& lists_, uint32_t most, uint32_t share)
+    : c(c_), w(w_), lists(lists_), all(all_chunks<CHUNK>(c_, w_, lists_), most), mine(share), at(0), stop(0), before(0), sequence(0), n(0)
+  {
+    if (mine >= all.count) { return; }
+    at       = all.start(mine);
+    stop     = all.start(mine + 1);
+    sequence = sequence_of<CHUNK>(c, w, lists, at, before);
+    n        = sequence < w.n_sequences ? lists.open(c, sequence, CHUNK, l) : 0u;
+  }
+  __device__ __forceinline__ bool next(piece& p)
+  {
+    if (at >= stop) { return false; }
+    while (at >= before + uint64_t(n) * w.n_units) {  // on to the next sequence that has chunks
+      before += uint64_t(n) * w.n_units;
+      if (++sequence >= w.n_sequences) {  // lengths that changed meanwhile
+        at = stop;
+        return false;
+      }
+      n = lists.open(c, sequence, CHUNK, l);
+    }
+    p.unit               = uint32_t(quotient(at - before, n));
+    const uint64_t begin = before + uint64_t(p.unit) * n, end = begin + n, last = min(stop, end);
+    p.sequence           = sequence;
+    p.chunk              = uint32_t(at - begin);
+    p.end                = uint32_t(last - begin);
+    p.begins             = at == begin;
+    p.whole              = p.begins && last == end;
+    if (p.begins && !p.whole) { p.n_parts = all.of(end - 1) - mine + 1u; }
+    at = last;
+    return true;
+  }
+};
 
 // ---- copies into shared memory ------------------------------------------------------------------------------------------------
 
@@ -539,36 +559,40 @@ __device__ __forceinline__ void copies_wait()
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// A warp's way through its chunks of a unit, ahead of the copies: what memory says about a row two chunks ahead, the word of the filter one
+// A warp's way through its chunks of a piece, ahead of the copies: what memory says about a row two chunks ahead, the word of the filter one
 // chunk ahead.  Lane i (modulo CHUNK) looks after row i of a chunk.
 template <int CHUNK, class Lists>
 struct row_stream {
   using name_type = typename Lists::name_type;
   const cache_view& c;
   const Lists& lists;
-  const typename Lists::list& l;
-  uint32_t end, step;  // chunks
+  typename Lists::list l;
+  uint32_t chunk, end, step;  // the next chunk to copy, the piece's end
   name_type name_0, name_1;
   uint32_t word_0;
 
-  __device__ __forceinline__ row_stream(const cache_view& c_, const Lists& lists_, const typename Lists::list& l_, uint32_t chunk, uint32_t end_,
-                                        uint32_t step_)
-    : c(c_), lists(lists_), l(l_), end(end_), step(step_)
+  __device__ __forceinline__ row_stream(const cache_view& c_, const Lists& lists_) : c(c_), lists(lists_), chunk(0), end(0), step(1) {}
+  __device__ __forceinline__ void attach(const typename Lists::list& l_, uint32_t chunk_, uint32_t end_, uint32_t step_)
   {
+    l      = l_;
+    chunk  = chunk_;
+    end    = end_;
+    step   = step_;
     name_0 = name(chunk);
     name_1 = name(chunk + step);
     word_0 = word(chunk, name_0);
   }
-  __device__ __forceinline__ uint32_t row(uint32_t chunk) const { return chunk * CHUNK + (threadIdx.x & 31u) % CHUNK; }
-  __device__ __forceinline__ name_type name(uint32_t chunk) const { return chunk < end ? lists.name(c, l, row(chunk)) : name_type(-1); }
-  __device__ __forceinline__ uint32_t word(uint32_t chunk, name_type name) const
+  __device__ __forceinline__ bool done() const { return chunk >= end; }
+  __device__ __forceinline__ uint32_t row(uint32_t at) const { return at * CHUNK + (threadIdx.x & 31u) % CHUNK; }
+  __device__ __forceinline__ name_type name(uint32_t at) const { return at < end ? lists.name(c, l, row(at)) : name_type(-1); }
+  __device__ __forceinline__ uint32_t word(uint32_t at, name_type name) const
   {
     if (c.filter == nullptr) { return 0u; }
     uint32_t page, place;
-    return lists.place(c, l, row(chunk), name, page, place) ? c.filter[(uint64_t(page) * c.page_size + place) >> 5] : 0u;
+    return lists.place(c, l, row(at), name, page, place) ? c.filter[(uint64_t(page) * c.page_size + place) >> 5] : 0u;
   }
-  // The place of this lane's row of `chunk` (false: it is not to be read), and on to the next.
-  __device__ __forceinline__ bool next(uint32_t chunk, uint32_t& page, uint32_t& place)
+  // The place of this lane's row of the next chunk (false: it is not to be read), and on to the one after.
+  __device__ __forceinline__ bool next(uint32_t& page, uint32_t& place)
   {
     const name_type name_2 = name(chunk + 2 * step);
     const uint32_t word_1  = word(chunk + step, name_1);
@@ -577,9 +601,154 @@ struct row_stream {
     name_0 = name_1;
     name_1 = name_2;
     word_0 = word_1;
+    chunk += step;
     return there;
   }
 };
+
+// ---- the way of a block -------------------------------------------------------------------------------------------------------
+
+constexpr uint32_t kEmpty = 0xFFFFFFFFu;  // in the place of a stage's mask: no chunk of any piece is there
+
+// Goes through everything the block has to do.  A warp's stages are filled a few chunks ahead, over the ends of pieces: the first chunks of the
+// next one come while the last ones of this are worked on and its sums are written.  `hooks`:
+//   attach(unit)                       where the rows to be copied next lie
+//   copy(stage, page, place, there)    copies of a chunk's rows; returns which of them are read
+//   start(sequence, unit)              queries; sums to zero
+//   consume(stage, mask)               the rows of a stage
+//   close()                            a warp's lanes have the warp's sums
+//   send(i, to), receive(i, from)      a warp's sums to another, the i-th of kPortions portions of kPortion floats
+//   to_rows(...)                       the warp's sums become output rows, or a part
+//   to_shared()                        the warp's sums into the block's state
+// `s_mask`: the warp's [STAGES]; `exchange`: room for half the warps' portions; the block's state may lie where the stages are.
+template <typename T, int WARPS, int CHUNK, int STAGES, class Lists, class Hooks>
+__device__ __forceinline__ void run_units(const cache_view& c, const work_view& w, const Lists& lists, const result_view& result,
+                                          const parts_view& parts, const block_state& state, float* exchange, uint32_t* s_mask, Hooks& hooks)
+{
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+  uint32_t filling = 0, emptying = 0;  // stages
+  row_stream<CHUNK, Lists> stream(c, lists);
+  auto fill = [&] {  // the next stage, with a chunk if the stream has one
+    uint32_t mask = kEmpty;
+    if (!stream.done()) {
+      uint32_t page, place;
+      const bool there = stream.next(page, place);
+      mask             = hooks.copy(filling, page, place, there);
+    }
+    if (lane == 0) { s_mask[filling] = mask; }
+    copies_end_group();
+    filling = filling + 1 == STAGES ? 0 : filling + 1;
+  };
+  auto heads_of = [&](uint32_t unit, uint32_t& rows, uint32_t& head0) {
+    const uint32_t head = unit / w.n_blocks_of, of = unit - head * w.n_blocks_of;
+    rows  = min(parts.rows, w.group - of * parts.rows);
+    head0 = head * w.group + of * parts.rows;
+  };
+  uint32_t rows, head0;
+
+  if (!Lists::kShares || w.cluster != 0u) {
+    typename Lists::list l;
+    const uint32_t which = blockIdx.x / w.cluster, rank = blockIdx.x - which * w.cluster;
+    const uint32_t sequence = which / w.n_units, unit = which - sequence * w.n_units;
+    const uint32_t n = lists.open(c, sequence, CHUNK, l);
+    lists.select(c, w, sequence, unit, l);
+    hooks.attach(unit);
+    stream.attach(l, uint32_t(uint64_t(rank) * n / w.cluster) + warp, uint32_t(uint64_t(rank + 1) * n / w.cluster), WARPS);
+    hooks.start(sequence, unit);
+#pragma unroll 1
+    for (int i = 0; i < STAGES; i++) { fill(); }
+    while (true) {
+      copies_wait<STAGES - 1>();
+      __syncwarp();
+      const uint32_t mask = s_mask[emptying];
+      if (mask == kEmpty) { break; }
+      if (mask != 0u) { hooks.consume(emptying, mask); }
+      __syncwarp();
+      emptying = emptying + 1 == STAGES ? 0 : emptying + 1;
+      fill();
+    }
+    copies_wait<0>();
+    hooks.close();
+    heads_of(unit, rows, head0);
+    __syncthreads();  // shared memory changes hands: from rows to sums
+    hooks.to_shared();
+    __syncthreads();
+    join_warps<T, WARPS>(c, w, state, rows, sequence, head0, result, w.cluster > 1u, parts);
+    if (w.cluster > 1u) { join_cluster<T, WARPS>(c, w, state, rows, sequence, head0, result); }
+    return;
+  }
+
+  if constexpr (Lists::kShares) {
+    // of warp teams, neighbouring shares are on different SMs: where there are fewer than warps, every SM has some
+    walk<CHUNK, Lists> path(c, w, lists, parts.shares, w.warp_teams ? warp * gridDim.x + blockIdx.x : blockIdx.x);
+    const uint32_t step = w.warp_teams ? 1u : uint32_t(WARPS), offset = w.warp_teams ? 0u : warp;
+    piece now, then;
+    auto turn_to = [&](const piece& p) {
+      hooks.attach(p.unit);
+      stream.attach(path.l, p.chunk + offset, p.end, step);
+    };
+    bool found = path.next(now), more = false;
+    uint4 begun = make_uint4(0, 0, 0, 0);
+    if (found) { turn_to(now); }
+    // `more`: the piece behind this one, once the stream has come to it
+    bool looked  = false;
+    auto fill_on = [&] {
+      if (stream.done() && !looked) {
+        looked = true;
+        more   = path.next(then);
+        if (more) { turn_to(then); }
+      }
+      fill();
+    };
+    if (found) {
+#pragma unroll 1
+      for (int i = 0; i < STAGES; i++) { fill_on(); }
+    }
+    while (found) {
+      hooks.start(now.sequence, now.unit);
+      uint32_t left = now.end > now.chunk + offset ? (now.end - now.chunk - offset + step - 1) / step : 0u;
+      while (left != 0u) {
+        copies_wait<STAGES - 1>();
+        __syncwarp();
+        const uint32_t mask = s_mask[emptying];
+        if (mask != kEmpty) {  // (a stage may be empty where a piece was shorter than the stages are many)
+          left--;
+          if (mask != 0u) { hooks.consume(emptying, mask); }
+        }
+        __syncwarp();
+        emptying = emptying + 1 == STAGES ? 0 : emptying + 1;
+        fill_on();
+      }
+      hooks.close();
+      heads_of(now.unit, rows, head0);
+      if (!w.warp_teams) {  // the upper half of the warps to the lower, until the first has all
+#pragma unroll
+        for (int half = WARPS / 2; half > 0; half /= 2) {
+#pragma unroll
+          for (int i = 0; i < Hooks::kPortions; i++) {
+            if (int(warp) >= half && int(warp) < 2 * half) { hooks.send(i, exchange + (warp - half) * Hooks::kPortion); }
+            __syncthreads();
+            if (int(warp) < half) { hooks.receive(i, exchange + warp * Hooks::kPortion); }
+            __syncthreads();
+          }
+        }
+      }
+      if (w.warp_teams || warp == 0) { hooks.to_rows(rows, now.sequence, head0, now.whole, 2 * path.mine + (now.begins ? 1u : 0u)); }
+      if (now.begins && !now.whole) { begun = make_uint4(now.sequence, now.unit, now.n_parts, 0); }
+      if (!looked) {
+        more = path.next(then);
+        if (more) { turn_to(then); }
+      }
+      found  = more;
+      now    = then;
+      looked = false;
+      more   = false;
+    }
+    copies_wait<0>();
+    if (parts.begun != nullptr && lane == 0 && (w.warp_teams || warp == 0)) { parts.begun[path.mine] = begun; }
+    empty_rows<T, WARPS, CHUNK>(c, w, lists, result);
+  }
+}
 
 // ---- host ---------------------------------------------------------------------------------------------------------------------
 
@@ -615,13 +784,13 @@ struct plan {
   uint32_t cluster;   // 0: shares
   bool warp_teams;
   bool parts;         // a unit may lie in several shares
-  uint32_t teams() const { return warp_teams ? blocks * warps : blocks; }
+  uint32_t shares() const { return warp_teams ? blocks * warps : blocks; }
 };
 
 // `most`: rows of a unit, at most; `shares`: whether there may be any.
 inline void deal_out(const resources& res, plan& p, uint64_t units, uint64_t most, bool shares)
 {
-  const uint64_t sms = uint64_t(res.sm_count), resident = std::min<uint64_t>(sms * p.resident, 4095 / kSmall);  // a tree holds 4,095 parts
+  const uint64_t sms = uint64_t(res.sm_count), resident = sms * p.resident;
   p.parts = p.warp_teams = false;
   if (units <= sms) {
     p.warps               = p.large ? p.large : kSmall;
@@ -640,11 +809,19 @@ inline void deal_out(const resources& res, plan& p, uint64_t units, uint64_t mos
     p.cluster = 1;
   } else {
     const uint64_t chunks = std::max<uint64_t>(1, ceildiv<uint64_t>(most, p.chunk));
-    p.warp_teams          = units >= 2 * resident;
-    p.blocks              = uint32_t(std::min(resident, ceildiv<uint64_t>(units * chunks, kSmall)));
+    p.blocks              = uint32_t(std::min(resident, units * ceildiv<uint64_t>(chunks, share::kLeast)));
     p.cluster             = 0;
-    p.parts               = chunks > 1 && p.teams() > 1;
+    p.warp_teams          = units >= 2 * resident;
+    p.parts               = chunks > 1;
   }
+}
+
+template <typename T>
+void launch_join(const resources& res, cudaStream_t stream, const plan& p, const work_view& w, const parts_view& parts, uint32_t dim,
+                 uint32_t n_heads, const result_view& result)
+{
+  const uint32_t blocks = std::min<uint32_t>(ceildiv<uint32_t>(parts.shares * parts.rows, kJoinWarps), uint32_t(res.sm_count) * 4);
+  launch_chained(join_kernel<T>, dim3(blocks), kJoinWarps * 32, 0, stream, w, parts, dim, n_heads, result);
 }
 
 }  // namespace cuvs_b200::kv

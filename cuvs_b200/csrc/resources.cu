@@ -80,7 +80,7 @@ resources::~resources()
   }
 }
 
-std::unique_lock<std::mutex> resources::stream_workspace(cudaStream_t on, size_t bytes, size_t zeroed, char** at)
+std::unique_lock<std::mutex> resources::stream_workspace(cudaStream_t on, size_t bytes, char** at)
 {
   std::unique_lock<std::mutex> held(stream_ws_lock);
   if (stream_ws.size() >= 64 && stream_ws.find(on) == stream_ws.end()) {
@@ -88,10 +88,7 @@ std::unique_lock<std::mutex> resources::stream_workspace(cudaStream_t on, size_t
     stream_ws.clear();
   }
   workspace& w = stream_ws[on];
-  if (w.capacity() < bytes) {
-    w.reserve(bytes);
-    CUDA_TRY(cudaMemsetAsync(w.base(), 0, zeroed, on));
-  }
+  w.reserve(bytes);
   *at = w.base();
   return held;
 }

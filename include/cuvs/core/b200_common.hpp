@@ -138,13 +138,12 @@ struct resources {
   int cc_major          = 0;
   workspace ws;       // search
   workspace scratch;  // extend and transform: some 2 GB at most (what their chunks need, and the labels of 2^26 rows)
-  // Workspaces of calls that work on one stream at a time (attention over a paged cache), one for each stream they were made on; a
-  // workspace that is made anew starts with zeros.
+  // Workspaces of calls that several threads may make through one handle (attention over a paged cache), one for each stream.
   std::map<cudaStream_t, workspace> stream_ws;
   std::mutex stream_ws_lock;
-  // The workspace of a stream, at least `bytes` large; its first `zeroed` bytes are 0 when it is new.  To be used while the lock is held:
-  // another thread's call may replace it afterwards (and waits for the GPU then).
-  std::unique_lock<std::mutex> stream_workspace(cudaStream_t on, size_t bytes, size_t zeroed, char** at);
+  // The workspace of a stream, at least `bytes` large.  The lock is held until the call's work has been enqueued: another thread's call on
+  // the stream comes before or behind all of it, and may replace the workspace afterwards (and waits for the GPU then).
+  std::unique_lock<std::mutex> stream_workspace(cudaStream_t on, size_t bytes, char** at);
   // small pinned host word for an occasional device->host scalar
   uint32_t* pinned = nullptr;
   // counters read by the benchmark ("how many kernels of ours ran")
