@@ -36,6 +36,7 @@ struct work_view {
   uint32_t group;        // query heads of one key head
   uint32_t cluster;      // blocks of a unit's cluster; 0: shares
   bool warp_teams;       // of shares: warps, else blocks
+  uint32_t cost;         // of a unit beside its rows (queries, joining, writing), in chunks: what it counts for where shares are dealt out
 };
 
 // ---- lists --------------------------------------------------------------------------------------------------------------------
@@ -146,12 +147,13 @@ __device__ __forceinline__ uint64_t chunks_at(const cache_view& c, const work_vi
   for (uint32_t i = 0; i < kAtOnce; i++) {
     typename Lists::list l;
     n[i] = first + i < w.n_sequences ? lists.open(c, first + i, CHUNK, l) : 0u;
+    if (n[i] != 0u) { n[i] += w.cost; }
     sum += n[i];
   }
   return sum;
 }
 
-// The number of all chunks; every warp sums it up for itself.
+// The number of all chunks, with the units' costs, which come before their chunks; every warp sums it up for itself.
 template <int CHUNK, class Lists>
 __device__ __forceinline__ uint64_t all_chunks(const cache_view& c, const work_view& w, const Lists& lists)
 {
@@ -358,11 +360,7 @@ __device__ __forceinline__ void join_some(const parts_view& parts, uint32_t shar
   const uint32_t lane = threadIdx.x & 31u;
   auto place          = [&](uint32_t p) { return size_t(p == 0 ? 2 * share + 1 : 2 * (share + p)) * parts.rows + r; };
   top                 = -INFINITY;
-  for (uint32_t p = from + lane * step; p < n; p += 32 * step) { top = fmaxf(top, parts.stats[place(p)].x); }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) { top = fmaxf(top, __shfl_xor_sync(kAllLanes, top, o)); }
-  const float safe = finite_top(top);
-  sum              = 0.0f;
+  sum                 = 0.0f;
 #pragma unroll
   for (int v = 0; v < 2; v++) { x[v][0] = x[v][1] = x[v][2] = x[v][3] = 0.0f; }
   for (uint32_t p0 = from; p0 < n; p0 += 8 * step) {
@@ -379,6 +377,17 @@ __device__ __forceinline__ void join_some(const parts_view& parts, uint32_t shar
         const uint32_t column = 4 * lane + 128u * v;
         y[v][i]               = load_piece(parts.acc + at * dim + column, there && column < dim);
       }
+    }
+    float next = top;
+#pragma unroll
+    for (uint32_t i = 0; i < 8; i++) { next = fmaxf(next, st[i].x); }
+    const float safe = finite_top(next), keep = power_of_2(top - safe);
+    top = next;
+    sum *= keep;
+#pragma unroll
+    for (int v = 0; v < 2; v++) {
+#pragma unroll
+      for (int e = 0; e < 4; e++) { x[v][e] *= keep; }
     }
 #pragma unroll
     for (uint32_t i = 0; i < 8; i++) {
@@ -517,29 +526,37 @@ struct walk {
     at       = all.start(mine);
     stop     = all.start(mine + 1);
     sequence = sequence_of<CHUNK>(c, w, lists, at, before);
-    n        = sequence < w.n_sequences ? lists.open(c, sequence, CHUNK, l) : 0u;
+    if (sequence < w.n_sequences) { open(); }
+  }
+  __device__ __forceinline__ void open()
+  {
+    n = lists.open(c, sequence, CHUNK, l);
+    if (n != 0u) { n += w.cost; }
   }
   __device__ __forceinline__ bool next(piece& p)
   {
-    if (at >= stop) { return false; }
-    while (at >= before + uint64_t(n) * w.n_units) {  // on to the next sequence that has chunks
-      before += uint64_t(n) * w.n_units;
-      if (++sequence >= w.n_sequences) {  // lengths that changed meanwhile
-        at = stop;
-        return false;
+    while (at < stop) {
+      while (at >= before + uint64_t(n) * w.n_units) {  // on to the next sequence that has chunks
+        before += uint64_t(n) * w.n_units;
+        if (++sequence >= w.n_sequences) {  // lengths that changed meanwhile
+          at = stop;
+          return false;
+        }
+        open();
       }
-      n = lists.open(c, sequence, CHUNK, l);
+      p.unit              = uint32_t(quotient(at - before, n));
+      const uint64_t unit = before + uint64_t(p.unit) * n, begin = unit + w.cost, end = unit + n, from = max(at, begin), to = min(stop, end);
+      at                  = to;
+      if (from >= to) { continue; }  // of the unit's cost alone
+      p.sequence = sequence;
+      p.chunk    = uint32_t(from - begin);
+      p.end      = uint32_t(to - begin);
+      p.begins   = from == begin;
+      p.whole    = p.begins && to == end;
+      if (p.begins && !p.whole) { p.n_parts = all.of(end - 1) - mine + 1u; }
+      return true;
     }
-    p.unit               = uint32_t(quotient(at - before, n));
-    const uint64_t begin = before + uint64_t(p.unit) * n, end = begin + n, last = min(stop, end);
-    p.sequence           = sequence;
-    p.chunk              = uint32_t(at - begin);
-    p.end                = uint32_t(last - begin);
-    p.begins             = at == begin;
-    p.whole              = p.begins && last == end;
-    if (p.begins && !p.whole) { p.n_parts = all.of(end - 1) - mine + 1u; }
-    at = last;
-    return true;
+    return false;
   }
 };
 
@@ -782,6 +799,7 @@ struct plan {
   uint32_t warps;     // of a block
   uint32_t blocks;
   uint32_t cluster;   // 0: shares
+  uint32_t cost;      // of a unit beside its rows, in chunks
   bool warp_teams;
   bool parts;         // a unit may lie in several shares
   uint32_t shares() const { return warp_teams ? blocks * warps : blocks; }
@@ -812,6 +830,7 @@ inline void deal_out(const resources& res, plan& p, uint64_t units, uint64_t mos
     p.blocks              = uint32_t(std::min(resident, units * ceildiv<uint64_t>(chunks, share::kLeast)));
     p.cluster             = 0;
     p.warp_teams          = units >= 2 * resident;
+    if (p.warp_teams) { p.cost /= 4; }
     p.parts               = chunks > 1;
   }
 }

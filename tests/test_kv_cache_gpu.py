@@ -157,11 +157,12 @@ def test_attention(dtype, lengths, heads, group, dim, page_size, how, window, ke
     assert torch.equal(out, again) and torch.equal(lse, lse_again)       # no order of arrival in the result
 
 
-# Work that no single block or warp finishes: parts of one unit by the hundred (three levels of joins), of many units with one long one among
-# short and empty ones, of all units at once; several eights of heads.
+# Work that no single block or warp finishes: parts of one unit by the hundred, of many units with one long one among short and empty ones, of
+# all units at once; several eights of heads; so many units that warps take them alone.
 LONG = [([60000], 1, 4, 64, 16, None), ([30001], 2, 16, 128, 64, None), ([20000, 0, 17], 3, 1, 128, 20, None), ([9000], 4, 40, 64, 16, None),
         ([1, 0, 40000, 5, 300, 0, 77] + [10] * 60, 4, 2, 64, 16, None), ([700 + 13 * i for i in range(40)], 4, 8, 128, 16, None),
-        ([3000] * 20, 8, 1, 40, 32, 2000), ([25000] * 3, 1, 5, 256, 32, None), ([1500] * 80, 2, 3, 96, 24, None)]
+        ([3000] * 20, 8, 1, 40, 32, 2000), ([25000] * 3, 1, 5, 256, 32, None), ([1500] * 80, 2, 3, 96, 24, None),
+        ([60] * 150 + [20000] + [130] * 60, 8, 1, 64, 16, None), ([300, 40, 0, 1, 90] * 100, 4, 9, 128, 16, 200), ([5000] + [200] * 180, 3, 4, 200, 48, None)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
