@@ -88,6 +88,7 @@ void check_place(int device, tensor& t, int ndim, const char* name)
     empty = empty || t.shape[i] == 0;
   }
   CUVS_EXPECTS(empty || t.data != nullptr, "%s: null tensor", name);
+  CUVS_EXPECTS(empty || t.bits < 8 || reinterpret_cast<uintptr_t>(t.data) % (t.bits / 8) == 0, "%s: not on a boundary of its elements", name);
   if (empty) {  // no element has a place: as if it were dense
     int64_t dense = 1;
     for (int i = ndim - 1; i >= 0; i--) {

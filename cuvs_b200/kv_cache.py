@@ -103,7 +103,7 @@ def _call(resources, stream, op, tensors, integer, scale, sync):
     """`tensors`: those of the call in the order of the C interface, filled up with None to eleven.  False: the call is being captured, and
     needs a workspace to itself."""
     for t in tensors:
-        if t is not None and type(t) is not torch.Tensor:
+        if t is not None and type(t) is not _Tensor:
             break
     else:
         if _tensors is not None:
@@ -115,7 +115,10 @@ def _call(resources, stream, op, tensors, integer, scale, sync):
             if status == 2:
                 return False
             L.check(L.CUVS_ERROR)
-    # subclasses of torch.Tensor, and what is no tensor at all
+    for t in tensors:
+        if t is not None and not isinstance(t, torch.Tensor):
+            raise TypeError(f"expected torch tensors, not {type(t).__name__}")
+    # subclasses of torch.Tensor
     scalars = ((integer,), (integer, _bits(scale)), (_bits(scale),), ())[op]
     L.check(_arrays(resources.handle, stream, op, *_words(tensors[:_COUNTS[op]], scalars), sync))
     return True
@@ -137,6 +140,7 @@ def _tensor_calls():
 
 
 _COUNTS = (11, 9, 7, 4)
+_Tensor = torch.Tensor
 _arrays = L.load().cuvsB200KvCacheArrays
 _workspace = L.load().cuvsB200KvCacheWorkspaceArrays
 _wait = L.load().cuvsB200KvCacheWait

@@ -138,6 +138,11 @@ def test_tensors_of_another_place_or_rank_are_refused(op):
     (A, "values", Described(H, (9, 16, 4, 64), (4096, 128, 64, 1)), "overlap"),
     (N, "candidates", Described(torch.int64, (3, 8, 20), (320, 40, 2)), "contiguous"),
     (T, "workspace", Described(torch.uint8, (1 << 20,), address=(1 << 40) + 8), "16-byte boundary"),
+    (T, "lengths", Described(torch.int32, (3,), address=(1 << 40) + 2), "boundary of its elements"),
+    (A, "frequencies", Described(torch.float64, (32,), address=(1 << 40) + 4), "boundary of its elements"),
+    (N, "candidates", Described(torch.int64, (3, 8, 20), address=(1 << 40) + 4), "boundary of its elements"),
+    # rows at odd multiples of 16 bytes, farther than 2^32 of them reach; at multiples of 2 KB they may
+    (T, "keys", Described(H, (1 << 20, 16, 4, 8), (1 << 20, 8, 128, 1)), "same shape"),
 ])
 def test_refused(op, name, tensor, message):
     with pytest.raises(L.CuvsError, match=message):
@@ -148,6 +153,18 @@ def test_long_and_ragged_rows_are_refused():
     for dim, message in ((264, "1 to 256"), (68, "16-byte"), (4, "16-byte")):
         with pytest.raises(L.CuvsError, match=message):
             check(M, {"parts": Described(H, (2, 3, 8, dim)), "out": Described(H, (3, 8, dim))})
+
+
+def test_caches_that_places_of_32_bits_cannot_reach_are_refused():
+    def with_pages(n, page):
+        t = Described(H, (n, 16, 4, 64), (page, 64, 1024, 1))
+        return {"keys": t, "values": t, "filter": None}
+    check(T, with_pages(1 << 20, 4096))                                     # 8 GB
+    check(T, with_pages(1 << 24, 8192))                                     # 256 GB, rows at multiples of 128 bytes
+    with pytest.raises(L.CuvsError, match="too large for rows at multiples of 16 bytes"):
+        check(T, with_pages(1 << 24, 8192 + 8))
+    with pytest.raises(L.CuvsError, match="too large for rows at multiples of 128 bytes"):
+        check(T, with_pages((1 << 31) - 1, 8192))
 
 
 def test_scalars_are_checked():
@@ -182,6 +199,8 @@ def test_python_refuses_what_it_cannot_describe():
         kv_cache.attention(cpu, cpu, cpu[0], torch.zeros((16, 1), dtype=torch.int32), torch.zeros(16, dtype=torch.int32))
     with pytest.raises(ValueError, match="CUDA"):
         kv_cache.merge_parts(cpu, cpu[..., 0].float())
+    with pytest.raises(TypeError, match="expected torch tensors, not ndarray"):
+        kv_cache._call(None, 0, M, (cpu.numpy(), None), 0, 0.0, False)
     with pytest.raises(ValueError, match="window"):
         kv_cache.attention(cpu, cpu, cpu[0], None, None, window=0)
     with pytest.raises(ValueError, match="element type"):

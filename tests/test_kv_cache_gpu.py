@@ -363,6 +363,75 @@ def test_captured_steps_follow_their_inputs():
     assert torch.equal(out[1], got[0][1])
 
 
+def test_shared_units_on_several_streams_and_in_graphs():
+    """Work that leaves parts in a workspace: calls on several streams and from several threads at once, two graphs that are replayed side by
+    side while calls go on, each with the lengths of the moment."""
+    import threading
+    from cuvs_b200 import kv_cache
+    g = generator(12)
+    n_pages = 6000
+    keys, values = layout((n_pages, 16, 2, 64), torch.bfloat16, g, "heads")
+    lengths = [40000, 20000, 7000, 30]
+    pages = tables(lengths, 16, n_pages, g)
+    queries = [rows((4, 8, 64), torch.bfloat16, g) for _ in range(4)]
+    assert kv_cache.attention_workspace(keys, queries[0], pages) > 0
+    n = ints(lengths)
+    want = [kv_cache.attention(keys, values, q, pages, n) for q in queries]
+    check(*want[0], want_attention(keys, values, queries[0], pages, n))
+    moment = [ints(lengths), ints(lengths)]
+    graphs, outs = [], []
+    for i in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(kv_cache.attention(keys, values, queries[i], pages, moment[i], sync=False))
+        graphs.append(graph)
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    torch.cuda.synchronize()
+    shorter = [39000, 1, 0, 30]
+    want_shorter = [kv_cache.attention(keys, values, q, pages, ints(shorter)) for q in queries[:2]]
+    torch.cuda.synchronize()
+    for turn in range(10):
+        for m in moment:
+            m.copy_(ints(lengths if turn % 2 else shorter))
+        torch.cuda.synchronize()
+        got = []
+        for graph, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                graph.replay()
+        for q, s in zip(queries, streams[2:] * 2):
+            with torch.cuda.stream(s):
+                got.append(kv_cache.attention(keys, values, q, pages, n, sync=False))
+        torch.cuda.synchronize()
+        for (a, b), (c, d) in zip(got, want):
+            assert torch.equal(a, c) and torch.equal(b, d)
+        for (a, b), (c, d) in zip(outs, want if turn % 2 else want_shorter):
+            assert torch.equal(a, c) and torch.equal(b, d)
+    wrong = []
+
+    def work(q, w):
+        for _ in range(30):
+            a, b = kv_cache.attention(keys, values, q, pages, n)        # all threads on the default stream, through one handle
+            if not (torch.equal(a, w[0]) and torch.equal(b, w[1])):
+                wrong.append(1)
+
+    threads = [threading.Thread(target=work, args=x) for x in zip(queries, want)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
+def test_parameters_and_other_subclasses():
+    from cuvs_b200 import kv_cache
+    g = generator(13)
+    keys, values = layout((9, 16, 2, 64), torch.float16, g, "tokens")
+    q, pages, n = rows((1, 4, 64), torch.float16, g), ints([[3, 1, 7]]), ints([44])
+    want = kv_cache.attention(keys, values, q, pages, n)
+    got = kv_cache.attention(torch.nn.Parameter(keys), values, torch.nn.Parameter(q), pages, n)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
 def test_offsets_that_pass_32_bits():
     """A cache of more than 2^32 elements: rows of its last pages."""
     from cuvs_b200 import kv_cache
