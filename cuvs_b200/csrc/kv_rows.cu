@@ -380,7 +380,7 @@ void launch_candidates(resources& res, cudaStream_t stream, const candidates_arg
   p.resident          = resident_of(1, false);
   p.large             = large_of(1, false);
   deal_out(res, p, uint64_t(a.n_tokens) * a.n_query_heads, a.n_candidates, false);
-  const work_view w{a.n_tokens, a.n_query_heads, group, group, p.cluster, false, 0};
+  const work_view w{a.n_tokens, a.n_query_heads, group, group, p.cluster, 0};
   by_pieces(pieces, [&](auto lanes, auto n) {
     constexpr int LANES = decltype(lanes)::value, PIECES = decltype(n)::value;
     if constexpr (sizeof(T) == 4 || PIECES == 1) {
@@ -395,7 +395,7 @@ size_t attention_workspace(const resources& res, elem type, uint32_t n_sequences
                            uint64_t capacity, int64_t window)
 {
   const plan p = attention_plan(res, type, n_sequences, n_heads, n_query_heads / n_heads, dim, capacity, window);
-  return p.parts ? part_bytes(p.shares(), p.rows, dim) : 0;
+  return p.parts ? part_bytes(p.blocks, p.rows, dim) : 0;
 }
 
 void attention(resources& res, cudaStream_t stream, const attention_args& a)
@@ -405,12 +405,12 @@ void attention(resources& res, cudaStream_t stream, const attention_args& a)
   const uint32_t group = a.n_query_heads / c.n_heads;
   const plan p         = attention_plan(res, a.type, a.n_sequences, c.n_heads, group, c.dim, uint64_t(a.table_width) * c.page_size, a.window);
   const uint32_t of    = ceildiv(group, p.rows);
-  const work_view w{a.n_sequences, c.n_heads * of, of, group, p.cluster, p.warp_teams, p.cost};
+  const work_view w{a.n_sequences, c.n_heads * of, of, group, p.cluster, p.cost};
   const positions lists{a.pages, a.lengths, a.table_stride, a.window, a.table_width};
   const result_view result{a.out, a.lse};
   parts_view parts{};
-  if (p.parts) { parts = parts_at(a.workspace, p.shares(), p.rows, c.dim); }
-  parts.shares = p.shares();
+  if (p.parts) { parts = parts_at(a.workspace, p.blocks, p.rows, c.dim); }
+  parts.shares = p.blocks;
   parts.rows   = p.rows;
   auto join    = [&](auto type) {
     if (p.parts) { launch_join<decltype(type)>(res, stream, p, w, parts, c.dim, c.n_heads, result); }

@@ -3,13 +3,15 @@
 // A unit is a (sequence, key head, block of query heads) with its list of rows, cut into chunks of as many rows as a warp takes at a time.
 // Two ways to deal the chunks out:
 //
-// Shares.  All units' chunks stand in one row, and each of the resident teams -- blocks, or their warps -- takes an equal, contiguous share of
-// it, whatever the lengths are (they are known on the device alone: every warp finds its share from them itself).  A unit that lies in one share
-// is finished there; of a unit that several share, each team leaves a part (top, sum and weighted sum in 32 bits), and a second kernel joins
-// the parts in the order of the shares.  A warp copies the first rows of the next unit while it finishes this one.  The warps of a block team
-// take a unit's chunks in turn and join through shared memory at its end; warps as teams need no barrier, but leave four times the parts: they
-// are for units that are many and short (256 requests of up to 1,024 tokens, 2,048 units: 134 us with blocks, 103 with warps; 32 of up to 16,384,
-// 256 units: 151 and 175).
+// Shares.  All units' chunks stand in one row, and each of the resident blocks takes an equal, contiguous share of it, whatever the lengths
+// are (they are known on the device alone: every warp finds its block's share from them itself).  What a unit costs beside its rows counts too.
+// A block's warps take a unit's chunks in turn, copy the first rows of the next unit while they finish this one, and join through shared
+// memory at its end.  A unit that lies in one share is finished there; of a unit that several share, each block leaves a part (top, sum and
+// weighted sum in 32 bits), and a second kernel joins the parts in the order of the shares.
+//   What else was tried: warps with shares of their own, which need no barrier but leave four times the parts (32 requests of up to 16,384 tokens
+// 170 us against 148, 256 of up to 1,024 87 against 80); parts joined in a tree by whichever block came last, without the second kernel (12 us at
+// the end of one long list); shares that get smaller in rounds, taken by whoever is done (four ends of pieces instead of one: 118 us
+// against 94 on one list of 250,000); shares of equal chunks whatever the units cost (16 requests of up to 2,000 tokens 32 us, 16 now).
 //
 // Clusters.  One cluster of blocks per unit, whose warps take its chunks in turn and join their parts through shared memory, their own and
 // each other's: no workspace, one launch and the shortest way to the end, but no balance between units: for few units with few rows.
@@ -35,7 +37,6 @@ struct work_view {
   uint32_t n_blocks_of;  // blocks of query heads of one key head
   uint32_t group;        // query heads of one key head
   uint32_t cluster;      // blocks of a unit's cluster; 0: shares
-  bool warp_teams;       // of shares: warps, else blocks
   uint32_t cost;         // of a unit beside its rows (queries, joining, writing), in chunks: what it counts for where shares are dealt out
 };
 
@@ -116,7 +117,7 @@ __device__ __forceinline__ uint64_t quotient(uint64_t a, uint32_t b)
   return a >> 32 == 0 ? uint64_t(uint32_t(a) / b) : a / b;  // the short division where it is enough
 }
 
-// `total` chunks of all units dealt out in `count` equal shares, each of kLeast chunks at least while there are fewer than all warps could take.
+// `total` chunks of all units dealt out in `count` equal shares: one for every block, or fewer of kLeast chunks each (one for each of its warps).
 struct share {
   static constexpr uint32_t kLeast = 4;  // chunks
   uint64_t total, each;
@@ -507,7 +508,7 @@ struct piece {
   bool begins, whole;
 };
 
-// A team's way through its share, piece by piece; the warps of a block team all go it.
+// A block's way through its share, piece by piece; all its warps go it.
 template <int CHUNK, class Lists>
 struct walk {
   const cache_view& c;
@@ -515,16 +516,15 @@ struct walk {
   const Lists& lists;
   typename Lists::list l;  // of the sequence that the walk is at
   share all;
-  uint32_t mine;
   uint64_t at, stop, before;
   uint32_t sequence, n;
 
-  __device__ __forceinline__ walk(const cache_view& c_, const work_view& w_, const Lists& lists_, uint32_t most, uint32_t share)
-    : c(c_), w(w_), lists(lists_), all(all_chunks<CHUNK>(c_, w_, lists_), most), mine(share), at(0), stop(0), before(0), sequence(0), n(0)
+  __device__ __forceinline__ walk(const cache_view& c_, const work_view& w_, const Lists& lists_, uint32_t most)
+    : c(c_), w(w_), lists(lists_), all(all_chunks<CHUNK>(c_, w_, lists_), most), at(0), stop(0), before(0), sequence(0), n(0)
   {
-    if (mine >= all.count) { return; }
-    at       = all.start(mine);
-    stop     = all.start(mine + 1);
+    if (blockIdx.x >= all.count) { return; }
+    at       = all.start(blockIdx.x);
+    stop     = all.start(blockIdx.x + 1);
     sequence = sequence_of<CHUNK>(c, w, lists, at, before);
     if (sequence < w.n_sequences) { open(); }
   }
@@ -553,7 +553,7 @@ struct walk {
       p.end      = uint32_t(to - begin);
       p.begins   = from == begin;
       p.whole    = p.begins && to == end;
-      if (p.begins && !p.whole) { p.n_parts = all.of(end - 1) - mine + 1u; }
+      if (p.begins && !p.whole) { p.n_parts = all.of(end - 1) - blockIdx.x + 1u; }
       return true;
     }
     return false;
@@ -696,13 +696,11 @@ __device__ __forceinline__ void run_units(const cache_view& c, const work_view& 
   }
 
   if constexpr (Lists::kShares) {
-    // of warp teams, neighbouring shares are on different SMs: where there are fewer than warps, every SM has some
-    walk<CHUNK, Lists> path(c, w, lists, parts.shares, w.warp_teams ? warp * gridDim.x + blockIdx.x : blockIdx.x);
-    const uint32_t step = w.warp_teams ? 1u : uint32_t(WARPS), offset = w.warp_teams ? 0u : warp;
+    walk<CHUNK, Lists> path(c, w, lists, parts.shares);
     piece now, then;
     auto turn_to = [&](const piece& p) {
       hooks.attach(p.unit);
-      stream.attach(path.l, p.chunk + offset, p.end, step);
+      stream.attach(path.l, p.chunk + warp, p.end, WARPS);
     };
     bool found = path.next(now), more = false;
     uint4 begun = make_uint4(0, 0, 0, 0);
@@ -723,7 +721,7 @@ __device__ __forceinline__ void run_units(const cache_view& c, const work_view& 
     }
     while (found) {
       hooks.start(now.sequence, now.unit);
-      uint32_t left = now.end > now.chunk + offset ? (now.end - now.chunk - offset + step - 1) / step : 0u;
+      uint32_t left = now.end > now.chunk + warp ? ceildiv<uint32_t>(now.end - now.chunk - warp, WARPS) : 0u;
       while (left != 0u) {
         copies_wait<STAGES - 1>();
         __syncwarp();
@@ -738,19 +736,18 @@ __device__ __forceinline__ void run_units(const cache_view& c, const work_view& 
       }
       hooks.close();
       heads_of(now.unit, rows, head0);
-      if (!w.warp_teams) {  // the upper half of the warps to the lower, until the first has all
+      // the upper half of the warps to the lower, until the first has all
 #pragma unroll
-        for (int half = WARPS / 2; half > 0; half /= 2) {
+      for (int half = WARPS / 2; half > 0; half /= 2) {
 #pragma unroll
-          for (int i = 0; i < Hooks::kPortions; i++) {
-            if (int(warp) >= half && int(warp) < 2 * half) { hooks.send(i, exchange + (warp - half) * Hooks::kPortion); }
-            __syncthreads();
-            if (int(warp) < half) { hooks.receive(i, exchange + warp * Hooks::kPortion); }
-            __syncthreads();
-          }
+        for (int i = 0; i < Hooks::kPortions; i++) {
+          if (int(warp) >= half && int(warp) < 2 * half) { hooks.send(i, exchange + (warp - half) * Hooks::kPortion); }
+          __syncthreads();
+          if (int(warp) < half) { hooks.receive(i, exchange + warp * Hooks::kPortion); }
+          __syncthreads();
         }
       }
-      if (w.warp_teams || warp == 0) { hooks.to_rows(rows, now.sequence, head0, now.whole, 2 * path.mine + (now.begins ? 1u : 0u)); }
+      if (warp == 0) { hooks.to_rows(rows, now.sequence, head0, now.whole, 2 * blockIdx.x + (now.begins ? 1u : 0u)); }
       if (now.begins && !now.whole) { begun = make_uint4(now.sequence, now.unit, now.n_parts, 0); }
       if (!looked) {
         more = path.next(then);
@@ -762,7 +759,7 @@ __device__ __forceinline__ void run_units(const cache_view& c, const work_view& 
       more   = false;
     }
     copies_wait<0>();
-    if (parts.begun != nullptr && lane == 0 && (w.warp_teams || warp == 0)) { parts.begun[path.mine] = begun; }
+    if (parts.begun != nullptr && threadIdx.x == 0) { parts.begun[blockIdx.x] = begun; }
     empty_rows<T, WARPS, CHUNK>(c, w, lists, result);
   }
 }
@@ -800,16 +797,15 @@ struct plan {
   uint32_t blocks;
   uint32_t cluster;   // 0: shares
   uint32_t cost;      // of a unit beside its rows, in chunks
-  bool warp_teams;
   bool parts;         // a unit may lie in several shares
-  uint32_t shares() const { return warp_teams ? blocks * warps : blocks; }
 };
 
-// `most`: rows of a unit, at most; `shares`: whether there may be any.
+// `most`: rows of a unit, at most; `shares`: whether there may be any.  Clusters where one wave of them has few chunks for a warp: one request of
+// 4,096 tokens and 8 key heads (3 each) 9.1 us, 11.9 in shares; two of up to 6,144 (4 each) 17.1 and 14.5.
 inline void deal_out(const resources& res, plan& p, uint64_t units, uint64_t most, bool shares)
 {
   const uint64_t sms = uint64_t(res.sm_count), resident = sms * p.resident;
-  p.parts = p.warp_teams = false;
+  p.parts = false;
   if (units <= sms) {
     p.warps               = p.large ? p.large : kSmall;
     const uint64_t chunks = ceildiv<uint64_t>(most, p.warps * p.chunk);
@@ -829,8 +825,6 @@ inline void deal_out(const resources& res, plan& p, uint64_t units, uint64_t mos
     const uint64_t chunks = std::max<uint64_t>(1, ceildiv<uint64_t>(most, p.chunk));
     p.blocks              = uint32_t(std::min(resident, units * ceildiv<uint64_t>(chunks, share::kLeast)));
     p.cluster             = 0;
-    p.warp_teams          = units >= 2 * resident;
-    if (p.warp_teams) { p.cost /= 4; }
     p.parts               = chunks > 1;
   }
 }

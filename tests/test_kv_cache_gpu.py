@@ -3,9 +3,9 @@
 Tolerances count roundings.  u = 2^-24 is half a step of 32 bits.  A score, scale * sum of dim products, is off by at most
 (dim + 4) u * scale * sum |q k|; a weight exp(score - top) by twice that (score and top), and by 2^-21 for the exponential and what goes
 into it; a sum of n weights or weighted values in 32 bits by at most n u of the sum of their magnitudes, where n counts the additions
-that follow one another: at most those of an eighth of the rows (a block has at least four warps or lane groups, which take turns of at most 32
-rows), plus 80 for those within a turn and between warps and blocks.  Both come in twice, in the sum of values and in the sum of weights.  The output is rounded once to its type: half a
-step, eps / 2 of its magnitude (and 2^-25 for fp16's smallest numbers).
+that follow one another: a unit's rows go to four warps at least, in turn, and one warp adds at most a quarter of them, plus those of its
+lanes, of the warps and of the parts (fewer than 592).  Both come in twice, in the sum of values and in the sum of weights.  The output is
+rounded once to its type: half a step, eps / 2 of its magnitude (and 2^-25 for fp16's smallest numbers).
 """
 import math
 
@@ -60,7 +60,7 @@ def attend(query, keys, values, scale, dtype):
     p = torch.exp(s - lse)
     out = p @ v
     weight = 2 * (dim + 4) * U * abs(scale) * (k.abs() @ q.abs()).max().item() + 2.0 ** -21
-    total = weight + (n / 8 + 80) * U
+    total = weight + (n / 4 + 592) * U
     return out, lse.item(), 2 * total * (p @ v.abs()).max().item() + half_step(out, dtype), total + 4 * U * (1 + abs(lse.item()))
 
 
@@ -158,7 +158,7 @@ def test_attention(dtype, lengths, heads, group, dim, page_size, how, window, ke
 
 
 # Work that no single block or warp finishes: parts of one unit by the hundred, of many units with one long one among short and empty ones, of
-# all units at once; several eights of heads; so many units that warps take them alone.
+# all units at once; several eights of heads; more units than blocks.
 LONG = [([60000], 1, 4, 64, 16, None), ([30001], 2, 16, 128, 64, None), ([20000, 0, 17], 3, 1, 128, 20, None), ([9000], 4, 40, 64, 16, None),
         ([1, 0, 40000, 5, 300, 0, 77] + [10] * 60, 4, 2, 64, 16, None), ([700 + 13 * i for i in range(40)], 4, 8, 128, 16, None),
         ([3000] * 20, 8, 1, 40, 32, 2000), ([25000] * 3, 1, 5, 256, 32, None), ([1500] * 80, 2, 3, 96, 24, None),
