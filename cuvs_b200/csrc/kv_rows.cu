@@ -14,11 +14,11 @@ namespace cuvs_b200::kv {
 namespace {
 
 // Rows of a chunk, by the 16-byte pieces that a row has room for in shared memory: 4 KB of keys for several query heads, 2 KB for one, which
-// leaves room for twice the warps.
+// leaves room for more warps; 16 at most (a chunk's mask has 16 bits).
 constexpr uint32_t chunk_of(uint32_t pieces, uint32_t heads)
 {
-  const uint32_t most = heads == 1 ? 16 : 32, rows = (heads == 1 ? 128 : 256) / pieces;
-  return rows < most ? rows : most;
+  const uint32_t rows = (heads == 1 ? 128 : 256) / pieces;
+  return rows < 16 ? rows : 16;
 }
 // Small blocks of an SM and warps of a large block: what registers leave room for (the way through shares takes some).
 constexpr uint32_t resident_of(uint32_t heads, bool shares) { return heads > 1 ? 3 : shares ? 4 : 6; }
@@ -40,6 +40,7 @@ struct rows_shape {
   static constexpr int kPortion  = (2 + PIECES * kPerPiece<T>) * 32;         // floats that a warp sends another: the sums of a query head
   static constexpr int kExchangeAt = kMaskAt + WARPS * 16;
   static constexpr int kShared   = kExchangeAt + (WARPS == kSmall && SHARES ? WARPS / 2 * kPortion * 4 : 0);
+  static_assert(kChunk <= 16, "masks of 16 bits");
   static_assert(WARPS * R * kColumns * 4 <= kStatsAt, "the warps' sums take the stages' place");
 };
 
@@ -88,7 +89,7 @@ struct rows_hooks {
 
   __device__ __forceinline__ uint32_t copy(uint32_t stage, uint32_t page, uint32_t place, bool there)
   {
-    const uint32_t mask = __ballot_sync(kAllLanes, there) & uint32_t((uint64_t(1) << CHUNK) - 1u);
+    const uint32_t mask = __ballot_sync(kAllLanes, there) & ((1u << CHUNK) - 1u);
     if (mask == 0u) { return 0u; }
     const uint32_t to   = buffers + stage * shape::kStage + copy_row * shape::kPitch + copy_piece_of * 16;
     const uint32_t k_at = there ? page * c.k_page_units + place * c.k_token_units : 0u;

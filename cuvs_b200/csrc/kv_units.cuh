@@ -526,7 +526,11 @@ struct walk {
     at       = all.start(blockIdx.x);
     stop     = all.start(blockIdx.x + 1);
     sequence = sequence_of<CHUNK>(c, w, lists, at, before);
-    if (sequence < w.n_sequences) { open(); }
+    if (sequence < w.n_sequences) {
+      open();
+    } else {  // lengths that changed meanwhile
+      at = stop;
+    }
   }
   __device__ __forceinline__ void open()
   {
@@ -538,7 +542,7 @@ struct walk {
     while (at < stop) {
       while (at >= before + uint64_t(n) * w.n_units) {  // on to the next sequence that has chunks
         before += uint64_t(n) * w.n_units;
-        if (++sequence >= w.n_sequences) {  // lengths that changed meanwhile
+        if (++sequence >= w.n_sequences) {
           at = stop;
           return false;
         }
@@ -553,7 +557,7 @@ struct walk {
       p.end      = uint32_t(to - begin);
       p.begins   = from == begin;
       p.whole    = p.begins && to == end;
-      if (p.begins && !p.whole) { p.n_parts = all.of(end - 1) - blockIdx.x + 1u; }
+      if (p.begins && !p.whole) { p.n_parts = min(all.of(end - 1), all.count - 1u) - blockIdx.x + 1u; }
       return true;
     }
     return false;
@@ -702,7 +706,7 @@ __device__ __forceinline__ void run_units(const cache_view& c, const work_view& 
       hooks.attach(p.unit);
       stream.attach(path.l, p.chunk + warp, p.end, WARPS);
     };
-    bool found = path.next(now), more = false;
+    bool found = __syncthreads_and(path.next(now)) != 0, more = false;
     uint4 begun = make_uint4(0, 0, 0, 0);
     if (found) { turn_to(now); }
     // `more`: the piece behind this one, once the stream has come to it
@@ -736,6 +740,10 @@ __device__ __forceinline__ void run_units(const cache_view& c, const work_view& 
       }
       hooks.close();
       heads_of(now.unit, rows, head0);
+      if (!looked) {
+        more = path.next(then);
+        if (more) { turn_to(then); }
+      }
       // the upper half of the warps to the lower, until the first has all
 #pragma unroll
       for (int half = WARPS / 2; half > 0; half /= 2) {
@@ -744,16 +752,14 @@ __device__ __forceinline__ void run_units(const cache_view& c, const work_view& 
           if (int(warp) >= half && int(warp) < 2 * half) { hooks.send(i, exchange + (warp - half) * Hooks::kPortion); }
           __syncthreads();
           if (int(warp) < half) { hooks.receive(i, exchange + warp * Hooks::kPortion); }
-          __syncthreads();
+          if (half > 1 || i + 1 < Hooks::kPortions) { __syncthreads(); }
         }
       }
+      // The warps found this out each for itself.  They go on together, or none does: lengths that somebody changes while the kernel runs must not
+      // leave one of them waiting for the others.
+      found = __syncthreads_and(more) != 0;
       if (warp == 0) { hooks.to_rows(rows, now.sequence, head0, now.whole, 2 * blockIdx.x + (now.begins ? 1u : 0u)); }
       if (now.begins && !now.whole) { begun = make_uint4(now.sequence, now.unit, now.n_parts, 0); }
-      if (!looked) {
-        more = path.next(then);
-        if (more) { turn_to(then); }
-      }
-      found  = more;
       now    = then;
       looked = false;
       more   = false;

@@ -136,6 +136,9 @@ SHAPES = [
     ([260] * 40, 3, 1, 8, 7, "tokens", None),
     ([2500], 8, 1, 160, 256, "heads", None),
     ([90, 11], 1, 128, 64, 16, "tokens", None),
+    ([400, 31, 32, 33], 2, 5, 16, 16, "heads", None),
+    ([1000], 1, 2, 32, 20, "tokens", 700),
+    ([64, 63], 1, 8, 24, 16, "both", None),
 ]
 
 
@@ -162,7 +165,8 @@ def test_attention(dtype, lengths, heads, group, dim, page_size, how, window, ke
 LONG = [([60000], 1, 4, 64, 16, None), ([30001], 2, 16, 128, 64, None), ([20000, 0, 17], 3, 1, 128, 20, None), ([9000], 4, 40, 64, 16, None),
         ([1, 0, 40000, 5, 300, 0, 77] + [10] * 60, 4, 2, 64, 16, None), ([700 + 13 * i for i in range(40)], 4, 8, 128, 16, None),
         ([3000] * 20, 8, 1, 40, 32, 2000), ([25000] * 3, 1, 5, 256, 32, None), ([1500] * 80, 2, 3, 96, 24, None),
-        ([60] * 150 + [20000] + [130] * 60, 8, 1, 64, 16, None), ([300, 40, 0, 1, 90] * 100, 4, 9, 128, 16, 200), ([5000] + [200] * 180, 3, 4, 200, 48, None)]
+        ([60] * 150 + [20000] + [130] * 60, 8, 1, 64, 16, None), ([300, 40, 0, 1, 90] * 100, 4, 9, 128, 16, 200), ([5000] + [200] * 180, 3, 4, 200, 48, None),
+        ([9000, 3], 1, 4, 32, 16, None), ([15000, 700, 31], 2, 2, 8, 20, None), ([300] * 200, 2, 8, 16, 16, None)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
