@@ -537,6 +537,7 @@ struct call {
   {
     resources& r = single_device(res);
     device_scope on(r.device);
+    r.stream = stream;  // what cuvsStreamSync waits for
     if (sync) {
       cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
       CUDA_TRY(cudaStreamIsCapturing(stream, &capturing));
@@ -550,7 +551,6 @@ struct call {
       case 2: kv::attend_candidates(r, stream, candidates_of(r.device, t, scale)); break;
       default: kv::merge_parts(r, stream, merge_of(r.device, t));
     }
-    __atomic_fetch_add(&r.launches, uint64_t(1), __ATOMIC_RELAXED);
     return true;
   }
 };

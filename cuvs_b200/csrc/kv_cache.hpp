@@ -5,8 +5,11 @@
 
 #include <cstdint>
 
-// These calls do not touch the handle beyond its device's properties: several threads may make them through one handle.
+// These calls go by the stream that they are given and touch nothing of the handle but its count of launches: several threads may make
+// them through one handle.
 namespace cuvs_b200::kv {
+
+inline void count_launches(resources& res, uint64_t n) { __atomic_fetch_add(&res.launches, n, __ATOMIC_RELAXED); }
 
 enum class elem { f16, bf16, f32 };
 

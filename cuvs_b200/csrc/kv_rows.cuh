@@ -1,5 +1,4 @@
-// Rows of a paged cache of keys and values on the device: 16-byte pieces as floats, places of slots, and the softmax of one query
-// head over rows that lie anywhere.
+// Rows of a paged cache of keys and values on the device: 16-byte pieces as floats, places of slots, powers of two.
 #pragma once
 
 #include "kv_cache.hpp"
