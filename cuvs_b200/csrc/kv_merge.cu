@@ -86,7 +86,8 @@ void launch(resources& res, cudaStream_t stream, const merge_args& a)
   const uint64_t rows   = uint64_t(a.n_tokens) * a.n_heads;
   auto go               = [&](auto kernel, uint32_t lanes) {
     launch_chained(kernel, dim3(uint32_t(ceildiv<uint64_t>(rows, kThreads / lanes))), kThreads, 0, stream, a, pieces);
-    };
+      count_launches(res, 1);
+  };
   if (pieces <= 8) {
     go(merge_kernel<T, 8>, 8);
   } else if (pieces <= 16) {

@@ -133,77 +133,96 @@ struct rows_hooks {
     }
   }
 
+  // A lane group's sums of U values over its lanes: halves of the lanes take halves of the values, so that lane gl ends with the sum of value
+  // own(gl) alone: 5 exchanges of four values over 16 lanes instead of 16.
+  __device__ __forceinline__ uint32_t own() const { return gl / (LANES / U); }
+  __device__ __forceinline__ float own_sum(float (&v)[U]) const
+  {
+#pragma unroll
+    for (int n = U, o = LANES / 2; n > 1; n /= 2, o /= 2) {
+      const bool upper = (gl & uint32_t(o)) != 0u;
+#pragma unroll
+      for (int i = 0; i < n / 2; i++) {
+        const float give = upper ? v[i] : v[i + n / 2];
+        v[i]             = (upper ? v[i + n / 2] : v[i]) + __shfl_xor_sync(kAllLanes, give, o);
+      }
+    }
+#pragma unroll
+    for (int o = LANES / U / 2; o > 0; o /= 2) { v[0] += __shfl_xor_sync(kAllLanes, v[0], o); }
+    return v[0];
+  }
+
   __device__ __forceinline__ void consume(uint32_t stage, uint32_t mask)
   {
     const char* k_rows = stages + stage * shape::kStage;
-      const char* v_rows = k_rows + CHUNK * shape::kPitch;
+    const char* v_rows = k_rows + CHUNK * shape::kPitch;
 #pragma unroll 1
-      for (int u0 = 0; u0 < shape::kTurns; u0 += U) {
-        float score[R][U];
+    for (int u0 = 0; u0 < shape::kTurns; u0 += U) {
+      float part[R][U];
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-          const uint32_t row = uint32_t(u0 + u) * shape::kGroups + group;
-          float x[PIECES][E];
+      for (int u = 0; u < U; u++) {
+        const uint32_t row = uint32_t(u0 + u) * shape::kGroups + group;
+        float x[PIECES][E];
 #pragma unroll
-          for (int p = 0; p < PIECES; p++) {
-            piece_to_floats<T>(*reinterpret_cast<const uint4*>(k_rows + row * shape::kPitch + (gl + p * LANES) * 16), x[p]);
-          }
-          const bool ok = ((mask >> row) & 1u) != 0u;
-#pragma unroll
-          for (int r = 0; r < R; r++) {
-            float s = 0.0f;
-#pragma unroll
-            for (int p = 0; p < PIECES; p++) {
-#pragma unroll
-              for (int e = 0; e < E; e++) { s = fmaf(q[r][p][e], x[p][e], s); }
-            }
-#pragma unroll
-            for (int o = LANES / 2; o > 0; o >>= 1) { s += __shfl_xor_sync(kAllLanes, s, o); }
-            score[r][u] = ok ? s * scale_log2 : -INFINITY;
-          }
+        for (int p = 0; p < PIECES; p++) {
+          piece_to_floats<T>(*reinterpret_cast<const uint4*>(k_rows + row * shape::kPitch + (gl + p * LANES) * 16), x[p]);
         }
 #pragma unroll
         for (int r = 0; r < R; r++) {
-          float next = top[r];
-#pragma unroll
-          for (int u = 0; u < U; u++) { next = fmaxf(next, score[r][u]); }
-          const float safe = finite_top(next);
-          const float keep = power_of_2(top[r] - safe);
-          top[r]           = next;
-          sum[r] *= keep;
+          float s = 0.0f;
 #pragma unroll
           for (int p = 0; p < PIECES; p++) {
 #pragma unroll
-            for (int e = 0; e < E; e++) { acc[r][p][e] *= keep; }
+            for (int e = 0; e < E; e++) { s = fmaf(q[r][p][e], x[p][e], s); }
           }
+          part[r][u] = s;
+        }
+      }
+      const bool ok = ((mask >> (uint32_t(u0 + own()) * shape::kGroups + group)) & 1u) != 0u;
 #pragma unroll
-          for (int u = 0; u < U; u++) {
-            score[r][u] = power_of_2(score[r][u] - safe);
-            sum[r] += score[r][u];
-          }
+      for (int r = 0; r < R; r++) {
+        const float s     = own_sum(part[r]);
+        const float score = ok ? s * scale_log2 : -INFINITY;
+        float next        = fmaxf(top[r], score);
+#pragma unroll
+        for (int o = LANES / 2; o >= LANES / U; o /= 2) { next = fmaxf(next, __shfl_xor_sync(kAllLanes, next, o)); }
+        const float safe = finite_top(next);
+        const float keep = power_of_2(top[r] - safe);
+        top[r]           = next;
+        const float weight = power_of_2(score - safe);
+        sum[r]             = sum[r] * keep + weight;  // of the lane's own rows, until close()
+#pragma unroll
+        for (int p = 0; p < PIECES; p++) {
+#pragma unroll
+          for (int e = 0; e < E; e++) { acc[r][p][e] *= keep; }
         }
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-          const uint32_t row = uint32_t(u0 + u) * shape::kGroups + group;
+        for (int u = 0; u < U; u++) { part[r][u] = __shfl_sync(kAllLanes, weight, u * (LANES / U), LANES); }
+      }
 #pragma unroll
-          for (int p = 0; p < PIECES; p++) {
-            float x[E];
-            piece_to_floats<T>(*reinterpret_cast<const uint4*>(v_rows + row * shape::kPitch + (gl + p * LANES) * 16), x);
+      for (int u = 0; u < U; u++) {
+        const uint32_t row = uint32_t(u0 + u) * shape::kGroups + group;
 #pragma unroll
-            for (int r = 0; r < R; r++) {
+        for (int p = 0; p < PIECES; p++) {
+          float x[E];
+          piece_to_floats<T>(*reinterpret_cast<const uint4*>(v_rows + row * shape::kPitch + (gl + p * LANES) * 16), x);
 #pragma unroll
-              for (int e = 0; e < E; e++) { acc[r][p][e] = fmaf(score[r][u], x[e], acc[r][p][e]); }
-            }
+          for (int r = 0; r < R; r++) {
+#pragma unroll
+            for (int e = 0; e < E; e++) { acc[r][p][e] = fmaf(part[r][u], x[e], acc[r][p][e]); }
           }
         }
       }
+    }
   }
 
-  // the warp's lane groups
+  // the lanes of a group, then the warp's lane groups
   __device__ __forceinline__ void close()
   {
 #pragma unroll
     for (int r = 0; r < R; r++) {
+#pragma unroll
+      for (int o = LANES / 2; o >= LANES / U; o /= 2) { sum[r] += __shfl_xor_sync(kAllLanes, sum[r], o); }
 #pragma unroll
       for (int o = LANES; o < 32; o <<= 1) {
         const float other = __shfl_xor_sync(kAllLanes, top[r], o);
