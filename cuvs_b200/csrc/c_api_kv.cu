@@ -161,15 +161,10 @@ kv::cache_view cache_of(int device, tensor& keys, tensor& values, const tensor& 
   c.v_token    = values.stride[1];
   c.v_head     = values.stride[2];
   c.n_pages    = int32_t(keys.shape[0]);
-  c.page_size  = uint32_t(keys.shape[1]);
+  c.page       = kv::divisor_of(uint32_t(keys.shape[1]));
   c.n_heads    = uint32_t(keys.shape[2]);
   c.dim        = uint32_t(keys.shape[3]);
   c.n_slots    = keys.shape[0] * keys.shape[1];
-  c.page_shift = -1;
-  if ((c.page_size & (c.page_size - 1)) == 0) {
-    c.page_shift = 0;
-    while ((1u << c.page_shift) < c.page_size) { c.page_shift++; }
-  }
   // the largest unit that all strides are multiples of; 16 bytes at least
   const int64_t size     = keys.bits / 8;
   const int64_t strides[] = {c.k_page * size, c.k_token * size, c.v_page * size, c.v_token * size};
@@ -177,7 +172,7 @@ kv::cache_view cache_of(int device, tensor& keys, tensor& values, const tensor& 
   while (c.unit_shift < 16 && std::all_of(strides, strides + 4, [&](int64_t x) { return x % (int64_t(2) << c.unit_shift) == 0; })) { c.unit_shift++; }
   for (int i = 0; i < 4; i += 2) {
     const auto reach = [&](int64_t n, int64_t stride) { return unsigned(n > 0 ? n - 1 : 0) * (unsigned __int128)(stride >> c.unit_shift); };
-    CUVS_EXPECTS(reach(c.n_pages, strides[i]) + reach(c.page_size, strides[i + 1]) < ((unsigned __int128)1 << 32),
+    CUVS_EXPECTS(reach(c.n_pages, strides[i]) + reach(c.page.size, strides[i + 1]) < ((unsigned __int128)1 << 32),
                  "%s: too large for rows at multiples of %u bytes", i == 0 ? "keys" : "values", 1u << c.unit_shift);
   }
   c.k_page_units  = uint32_t(strides[0] >> c.unit_shift);
@@ -340,7 +335,7 @@ kv::attention_args attention_of(int device, tensor* t, float scale, int64_t wind
 bool attention_call(resources& res, cudaStream_t stream, kv::attention_args a)
 {
   const size_t need = kv::attention_workspace(res, a.type, a.n_sequences, a.n_query_heads, a.cache.n_heads, a.cache.dim,
-                                              uint64_t(a.table_width) * a.cache.page_size, a.window);
+                                              uint64_t(a.table_width) * a.cache.page.size, a.window);
   std::unique_lock<std::mutex> held;
   if (need > 0 && a.workspace != nullptr) {
     CUVS_EXPECTS(a.workspace_bytes >= need, "workspace: %zu bytes, but %zu are needed", a.workspace_bytes, need);
@@ -427,7 +422,7 @@ void workspace_of(resources& res, tensor* t, int64_t window, size_t* bytes)
   int64_t stride;
   pages_of(res.device, t[PAGES], n, width, stride);
   CUVS_EXPECTS(window >= 0, "window must not be negative");
-  *bytes = kv::attention_workspace(res, type, n, query_heads_of(t[QUERIES], c), c.n_heads, c.dim, uint64_t(width) * c.page_size, window);
+  *bytes = kv::attention_workspace(res, type, n, query_heads_of(t[QUERIES], c), c.n_heads, c.dim, uint64_t(width) * c.page.size, window);
 }
 
 resources& single_device(cuvsResources_t res)

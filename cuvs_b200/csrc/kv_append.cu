@@ -42,11 +42,10 @@ append_kernel(append_args a, uint32_t log_lanes, uint32_t steps, uint32_t slices
   const int64_t seq = a.sequences ? int64_t(a.sequences[token]) : int64_t(token);
   int64_t slot      = -1;
   if (seq >= 0 && seq < int64_t(a.n_sequences)) {
-    slot = slot_of(a.pages + seq * a.table_stride, a.table_width, pos, a.cache.page_size, a.cache.page_shift, a.cache.n_pages);
+    slot = slot_of(a.pages + seq * a.table_stride, a.table_width, pos, a.cache.page, a.cache.n_pages);
   }
   if (slice == 0 && lane == 0) { a.slots[token] = slot; }
-  int64_t page;
-  uint32_t place;
+  uint32_t page, place;
   split_slot(a.cache, max(slot, int64_t(0)), page, place);
   for (uint32_t pair = lane; pair < a.n_pairs; pair += 32) {
     const double f = a.frequencies_f32 ? double(static_cast<const float*>(a.frequencies)[pair]) : static_cast<const double*>(a.frequencies)[pair];
@@ -76,12 +75,12 @@ append_kernel(append_args a, uint32_t log_lanes, uint32_t steps, uint32_t slices
     if (h < heads) {
       from = a.keys + (int64_t(token) * a.k_row + int64_t(h) * a.k_head) * int64_t(sizeof(T));
       to   = const_cast<char*>(a.cache.keys) +
-           (page * a.cache.k_page + int64_t(place) * a.cache.k_token + int64_t(h) * a.cache.k_head) * int64_t(sizeof(T));
+           (int64_t(page) * a.cache.k_page + int64_t(place) * a.cache.k_token + int64_t(h) * a.cache.k_head) * int64_t(sizeof(T));
       return true;
     }
     from = a.values + (int64_t(token) * a.v_row + int64_t(h - heads) * a.v_head) * int64_t(sizeof(T));
     to   = const_cast<char*>(a.cache.values) +
-         (page * a.cache.v_page + int64_t(place) * a.cache.v_token + int64_t(h - heads) * a.cache.v_head) * int64_t(sizeof(T));
+         (int64_t(page) * a.cache.v_page + int64_t(place) * a.cache.v_token + int64_t(h - heads) * a.cache.v_head) * int64_t(sizeof(T));
     return false;
   };
 

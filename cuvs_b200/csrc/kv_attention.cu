@@ -443,7 +443,7 @@ void attention16<KV_TYPE>(cudaStream_t stream, const attention_args& a, const pl
       launch_units(stream, kernel, p.blocks, WARPS * 32, p.cluster, mma_shape<D, NT, WARPS>::kShared, a.cache, w, lists, a.queries, result,
                    a.scale * kLog2E, parts);
     };
-    if (a.cache.page_size % 16 == 0) {
+    if (a.cache.page.size % 16 == 0) {
       go(mma_kernel<T, D, NT, WARPS, true>);
     } else {
       go(mma_kernel<T, D, NT, WARPS, false>);

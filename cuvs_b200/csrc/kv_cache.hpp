@@ -2,6 +2,7 @@
 #pragma once
 
 #include "common.hpp"
+#include "kv_place.hpp"
 
 #include <cstdint>
 
@@ -37,8 +38,7 @@ struct cache_view {
   uint32_t k_page_units, k_token_units, v_page_units, v_token_units, unit_shift;
   int64_t n_slots;
   int32_t n_pages;
-  uint32_t page_size;
-  int32_t page_shift;  // log2 of the page size, -1 where it is no power of two
+  page_divisor page;
   uint32_t n_heads;
   uint32_t dim;
   const uint32_t* filter;  // bit i: slot i may be attended; nullptr: all

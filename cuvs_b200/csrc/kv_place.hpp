@@ -7,11 +7,23 @@
 
 namespace cuvs_b200::kv {
 
-// Page column and place in the page of a position; `shift`: log2 of the page size, -1 where it is no power of two.
-CUVS_HD inline void split_place(uint32_t at, uint32_t page_size, int32_t shift, uint32_t& page, uint32_t& place)
+// Division of numbers below 2^31 by the page size as one product (Granlund and Montgomery, Division by invariant integers using
+// multiplication, 1994): with l = ceil(log2 size) and m = floor(2^(31 + l) / size) + 1, which is below 2^32, n / size = n m >> (31 + l).
+struct page_divisor {
+  uint32_t size, factor, shift;
+};
+inline page_divisor divisor_of(uint32_t size)
 {
-  page  = shift >= 0 ? at >> shift : at / page_size;
-  place = at - page * page_size;
+  uint32_t l = 0;
+  while ((uint64_t(1) << l) < size) { l++; }
+  return {size, uint32_t((uint64_t(1) << (31 + l)) / size + 1), 31 + l};
+}
+
+// Page column and place in the page of a position (below 2^31).
+CUVS_HD inline void split_place(uint32_t at, const page_divisor& by, uint32_t& page, uint32_t& place)
+{
+  page  = uint32_t(uint64_t(at) * by.factor >> by.shift);
+  place = at - page * by.size;
 }
 
 // The page of the cache in column `column` of a sequence's row of the table, -1 where there is none.
@@ -23,13 +35,13 @@ CUVS_HD inline int32_t page_of(const int32_t* row, uint32_t width, uint32_t colu
 }
 
 // The slot of position `at` of a sequence; -1: the position has none.
-CUVS_HD inline int64_t slot_of(const int32_t* row, uint32_t width, int32_t at, uint32_t page_size, int32_t shift, int32_t n_pages)
+CUVS_HD inline int64_t slot_of(const int32_t* row, uint32_t width, int32_t at, const page_divisor& by, int32_t n_pages)
 {
   if (at < 0) { return -1; }
   uint32_t column, place;
-  split_place(uint32_t(at), page_size, shift, column, place);
+  split_place(uint32_t(at), by, column, place);
   const int32_t page = page_of(row, width, column, n_pages);
-  return page < 0 ? -1 : int64_t(page) * page_size + place;
+  return page < 0 ? -1 : int64_t(page) * by.size + place;
 }
 
 // First and one past the last position that a token attends to: the last `window` (0: all) of `length`, as far as the table reaches.

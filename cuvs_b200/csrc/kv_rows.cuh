@@ -113,20 +113,14 @@ __device__ __forceinline__ uint4 load_piece(const void* from, bool there)
   return v;
 }
 
-// Page and place in it of a position below 2^31 (or of a slot below 2^32).
-__device__ __forceinline__ void split_place(const cache_view& c, uint32_t at, uint32_t& page, uint32_t& place)
+// Page and place in it of a slot.
+__device__ __forceinline__ void split_slot(const cache_view& c, int64_t slot, uint32_t& page, uint32_t& place)
 {
-  split_place(at, c.page_size, c.page_shift, page, place);
-}
-__device__ __forceinline__ void split_slot(const cache_view& c, int64_t slot, int64_t& page, uint32_t& place)
-{
-  if (uint64_t(slot) >> 32 == 0) {
-    uint32_t p;
-    split_place(c, uint32_t(slot), p, place);
-    page = p;
+  if (uint64_t(slot) >> 31 == 0) {
+    split_place(uint32_t(slot), c.page, page, place);
   } else {
-    page  = slot / int64_t(c.page_size);
-    place = uint32_t(slot - page * int64_t(c.page_size));
+    page  = uint32_t(slot / int64_t(c.page.size));
+    place = uint32_t(slot - int64_t(page) * int64_t(c.page.size));
   }
 }
 

@@ -59,7 +59,7 @@ struct positions {
   };
   __device__ __forceinline__ uint32_t open(const cache_view& c, uint32_t sequence, uint32_t chunk, list& l) const
   {
-    attended(lengths[sequence], window, width, c.page_size, l.first, l.end);
+    attended(lengths[sequence], window, width, c.page.size, l.first, l.end);
     l.table = pages + int64_t(sequence) * table_stride;
     l.base  = l.first & ~15u;
     return l.end > l.first ? (l.end - l.base + chunk - 1) / chunk : 0u;
@@ -71,14 +71,14 @@ struct positions {
     const uint32_t at = l.base + i;
     if (at < l.first || at >= l.end) { return -1; }
     uint32_t column, place;
-    split_place(at, c.page_size, c.page_shift, column, place);
+    split_place(at, c.page, column, place);
     return l.table[column];  // at < end: the column is inside the table
   }
   // Its page and place in it; false: it has none.
   __device__ __forceinline__ bool place(const cache_view& c, const list& l, uint32_t i, int32_t name, uint32_t& page, uint32_t& place) const
   {
     uint32_t column;
-    split_place(l.base + i, c.page_size, c.page_shift, column, place);
+    split_place(l.base + i, c.page, column, place);
     page = uint32_t(name);
     return name >= 0 && name < c.n_pages;
   }
@@ -103,9 +103,7 @@ struct named_slots {
   __device__ __forceinline__ bool place(const cache_view& c, const list&, uint32_t, int64_t name, uint32_t& page, uint32_t& place) const
   {
     const bool there = name >= 0 && name < c.n_slots;
-    int64_t p;
-    split_slot(c, there ? name : 0, p, place);
-    page = uint32_t(p);
+    split_slot(c, there ? name : 0, page, place);
     return there;
   }
 };
@@ -610,7 +608,7 @@ struct row_stream {
   {
     if (c.filter == nullptr) { return 0u; }
     uint32_t page, place;
-    return lists.place(c, l, row(at), name, page, place) ? c.filter[(uint64_t(page) * c.page_size + place) >> 5] : 0u;
+    return lists.place(c, l, row(at), name, page, place) ? c.filter[(uint64_t(page) * c.page.size + place) >> 5] : 0u;
   }
   // The place of this lane's row of the next chunk (false: it is not to be read), and on to the one after.
   __device__ __forceinline__ bool next(uint32_t& page, uint32_t& place)
@@ -618,7 +616,7 @@ struct row_stream {
     const name_type name_2 = name(chunk + 2 * step);
     const uint32_t word_1  = word(chunk + step, name_1);
     bool there             = lists.place(c, l, row(chunk), name_0, page, place);
-    if (c.filter != nullptr) { there = there && ((word_0 >> ((page * c.page_size + place) & 31u)) & 1u) != 0u; }
+    if (c.filter != nullptr) { there = there && ((word_0 >> ((page * c.page.size + place) & 31u)) & 1u) != 0u; }
     name_0 = name_1;
     name_1 = name_2;
     word_0 = word_1;

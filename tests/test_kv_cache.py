@@ -220,19 +220,33 @@ int main()
   // pages that are none (negative, behind the last), the last page, entries behind the table's end
   const int32_t row[] = {5, -1, 0, 8, 9, 2147483647, -2147483647 - 1, 3};
   for (uint32_t size : {1u, 3u, 16u, 20u, 64u}) {
-    int32_t shift = -1;
-    for (int s = 0; s < 31; s++) { if ((1u << s) == size) { shift = s; } }
+    const page_divisor by = divisor_of(size);
     for (int64_t at = -3; at < int64_t(size) * 10; at++) {
       const int64_t column = at < 0 ? 0 : at / size;
       const bool there     = at >= 0 && column < 8 && row[column] >= 0 && row[column] < 9;
-      assert(slot_of(row, 8, int32_t(at), size, shift, 9) == (there ? row[column] * int64_t(size) + at % size : -1));
-      assert(slot_of(row, 0, int32_t(at), size, shift, 9) == -1);
-      assert(slot_of(row, 8, int32_t(at), size, shift, 0) == -1);
+      assert(slot_of(row, 8, int32_t(at), by, 9) == (there ? row[column] * int64_t(size) + at % size : -1));
+      assert(slot_of(row, 0, int32_t(at), by, 9) == -1);
+      assert(slot_of(row, 8, int32_t(at), by, 0) == -1);
     }
   }
-  assert(slot_of(row, 8, 2147483647, 1u << 28, 28, 9) == 3ll * (1 << 28) + (1 << 28) - 1);   // slots behind 2^29
+  assert(slot_of(row, 8, 2147483647, divisor_of(1u << 28), 9) == 3ll * (1 << 28) + (1 << 28) - 1);   // slots behind 2^29
   const int32_t far[] = {2147483646};
-  assert(slot_of(far, 1, 63, 64, 6, 2147483647) == 2147483646ll * 64 + 63);                   // slots behind 2^32
+  assert(slot_of(far, 1, 63, divisor_of(64), 2147483647) == 2147483646ll * 64 + 63);                   // slots behind 2^32
+  // the product that stands for the division: around multiples of the size, up to the last position
+  for (uint32_t size : {1u, 2u, 3u, 5u, 7u, 20u, 24u, 100u, 641u, 65535u, 65536u, 65537u, 1000003u, (1u << 30) - 1, 1u << 30, (1u << 30) + 1, 2147483647u}) {
+    const page_divisor by = divisor_of(size);
+    for (uint64_t k = 0; k * size < (uint64_t(1) << 31) + size; k += 1 + (uint64_t(1) << 31) / size / 4096) {
+      for (int64_t at = int64_t(k * size) - 1; at <= int64_t(k * size) + 1; at++) {
+        if (at < 0 || at >= int64_t(1) << 31) { continue; }
+        uint32_t page, place;
+        split_place(uint32_t(at), by, page, place);
+        assert(page == uint32_t(at) / size && place == uint32_t(at) % size);
+      }
+    }
+    uint32_t page, place;
+    split_place(2147483647u, by, page, place);
+    assert(page == 2147483647u / size && place == 2147483647u % size);
+  }
   uint32_t first, end;
   attended(-5, 0, 4, 16, first, end);  assert(first == 0 && end == 0);
   attended(0, 7, 4, 16, first, end);   assert(first == 0 && end == 0);
