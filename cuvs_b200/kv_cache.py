@@ -104,24 +104,26 @@ def _call(resources, stream, op, tensors, integer, scale, sync):
     needs a workspace to itself."""
     for t in tensors:
         if t is not None and type(t) is not _Tensor:
-            break
-    else:
-        if _tensors is not None:
-            status = _tensors(resources.handle, stream, op, *tensors, integer, scale, sync)
-            if status == L.CUVS_SUCCESS:
-                if sync:
-                    L.check(_wait(resources.handle, stream))
-                return True
-            if status == 2:
-                return False
-            L.check(L.CUVS_ERROR)
-    for t in tensors:
-        if t is not None and not isinstance(t, torch.Tensor):
-            raise TypeError(f"expected torch tensors, not {type(t).__name__}")
-    # subclasses of torch.Tensor
-    scalars = ((integer,), (integer, _bits(scale)), (_bits(scale),), ())[op]
-    L.check(_arrays(resources.handle, stream, op, *_words(tensors[:_COUNTS[op]], scalars), sync))
+            return _call(resources, stream, op, tuple(_plain(t) for t in tensors), integer, scale, sync)
+    if _tensors is None:
+        scalars = ((integer,), (integer, _bits(scale)), (_bits(scale),), ())[op]
+        L.check(_arrays(resources.handle, stream, op, *_words(tensors[:_COUNTS[op]], scalars), sync))
+        return True
+    status = _tensors(resources.handle, stream, op, *tensors, integer, scale, sync)
+    if status == 2:
+        return False
+    if status != L.CUVS_SUCCESS:
+        L.check(L.CUVS_ERROR)
+    if sync:
+        L.check(_wait(resources.handle, stream))
     return True
+
+
+def _plain(t):
+    """Parameters and other subclasses as the tensors that they are."""
+    if t is not None and not isinstance(t, _Tensor):
+        raise TypeError(f"expected torch tensors, not {type(t).__name__}")
+    return t if t is None or type(t) is _Tensor else t.as_subclass(_Tensor)
 
 
 def _tensor_calls():

@@ -434,6 +434,9 @@ def test_parameters_and_other_subclasses():
     want = kv_cache.attention(keys, values, q, pages, n)
     got = kv_cache.attention(torch.nn.Parameter(keys), values, torch.nn.Parameter(q), pages, n)
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    # tensors that require gradients are read all the same; the results have none
+    got = kv_cache.attention(keys, values, q.clone().requires_grad_(), pages, n)
+    assert torch.equal(got[0], want[0]) and not got[0].requires_grad
 
 
 def test_offsets_that_pass_32_bits():
