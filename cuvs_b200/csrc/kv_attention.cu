@@ -51,32 +51,44 @@ __device__ __forceinline__ void multiply_add<__nv_bfloat16>(float (&c)[4], const
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// A weight goes into the product with the values as the sum of two 16-bit numbers, so that its rounding (2^-9 of bf16) is not added to
-// that of the output: twice the mma.sync of that product, which has them to spare.  The first is taken a little too small, so that the
-// second is never 0 where the weight is not: 0 times an infinite value would be no number.
+// A weight of 32 bits goes into the product with the values as the sum of 16-bit numbers, so that nothing is lost beside what the exponential
+// itself is off by: a row of the output is rounded once, at its end.  The products, twice or three times the mma.sync of one number, are to spare.
+// No summand is 0 where the weight is not: 0 times an infinite value would be no number.
 template <typename T>
-struct halves;
+struct summands;
 template <>
-struct halves<__half> {
-  static constexpr float kBelow = 0.999f;
-  static constexpr float kShift = 14.0f;  // weights are held times 2^14: small ones keep their digits above fp16's smallest numbers
-  static __device__ __forceinline__ uint32_t pack(float a, float b)
+struct summands<__half> {
+  // 11 bits, cut off, and the rest rounded to 11 bits: to 2^-22 of the weight.  Weights are held times 2^14, so that small ones keep their digits
+  // above fp16's smallest number: it is 2^-38 of the largest weight, and what is below counts for nothing.
+  static constexpr int kCount   = 2;
+  static constexpr float kScale = 16384.0f;
+  static constexpr float kLog2  = 14.0f;
+  static __device__ __forceinline__ void split(float a, float b, uint32_t (&part)[kCount])
   {
-    const __half2 t = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&t);
+    constexpr float kSmallest = 5.9604644775390625e-8f;  // 2^-24
+    asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(part[0]) : "f"(b), "f"(a));
+    const float2 high = __half22float2(*reinterpret_cast<const __half2*>(&part[0]));
+    const __half2 low = __floats2half2_rn(fmaxf(a - high.x, fminf(a, kSmallest)), fmaxf(b - high.y, fminf(b, kSmallest)));
+    part[1]           = *reinterpret_cast<const uint32_t*>(&low);
   }
-  static __device__ __forceinline__ float2 unpack(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
 };
 template <>
-struct halves<__nv_bfloat16> {
-  static constexpr float kBelow = 0.99f;
-  static constexpr float kShift = 0.0f;
-  static __device__ __forceinline__ uint32_t pack(float a, float b)
+struct summands<__nv_bfloat16> {
+  // Three times 8 bits, cut off: all of the weight.  (Two of them, rounded, left the weights of a batch of 32 requests 1.7e-5 off on average: 2^-16.)
+  static constexpr int kCount   = 3;
+  static constexpr float kScale = 1.0f;
+  static constexpr float kLog2  = 0.0f;
+  static __device__ __forceinline__ uint32_t upper(float a, float b) { return __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632); }
+  static __device__ __forceinline__ float cut(float a) { return __uint_as_float(__float_as_uint(a) & 0xFFFF0000u); }
+  static __device__ __forceinline__ void split(float a, float b, uint32_t (&part)[kCount])
   {
-    const __nv_bfloat162 t = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&t);
+    constexpr float kNothing = 7.52316384526264e-37f;  // 2^-120
+    const float a1 = fmaxf(a - cut(a), kNothing), b1 = fmaxf(b - cut(b), kNothing);
+    const float a2 = fmaxf(a1 - cut(a1), kNothing), b2 = fmaxf(b1 - cut(b1), kNothing);
+    part[0] = upper(a, b);
+    part[1] = upper(a1, b1);
+    part[2] = upper(a2, b2);
   }
-  static __device__ __forceinline__ float2 unpack(uint32_t v) { return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xFFFF0000u)); }
 };
 
 // D: columns of a row in shared memory (64, 128, 256; what is behind the row's end is 0).  NT: query heads of a unit, in eights.
@@ -287,21 +299,21 @@ struct mma_hooks {
         }
       }
     }
-    uint32_t high[NT][2], low[NT][2];
+    constexpr int N = summands<T>::kCount;
+    uint32_t part[NT][2][N];
 #pragma unroll
     for (int n = 0; n < NT; n++) {
       float p[4];
 #pragma unroll
       for (int e = 0; e < 4; e++) {
-        p[e] = power_of_2(s[n][e] - (finite_top(top[n][e & 1]) - halves<T>::kShift));
+        p[e] = power_of_2(s[n][e] - finite_top(top[n][e & 1])) * summands<T>::kScale;
         sum[n][e & 1] += p[e];
       }
 #pragma unroll
       for (int h = 0; h < 2; h++) {
-        high[n][h]       = halves<T>::pack(p[2 * h] * halves<T>::kBelow, p[2 * h + 1] * halves<T>::kBelow);
-        const float2 was = halves<T>::unpack(high[n][h]);
-        low[n][h]        = turn_matrix(halves<T>::pack(p[2 * h] - was.x, p[2 * h + 1] - was.y));
-        high[n][h]       = turn_matrix(high[n][h]);
+        summands<T>::split(p[2 * h], p[2 * h + 1], part[n][h]);
+#pragma unroll
+        for (int i = 0; i < N; i++) { part[n][h][i] = turn_matrix(part[n][h][i]); }
       }
     }
 #pragma unroll
@@ -311,8 +323,8 @@ struct mma_hooks {
       load_matrices_turned(a, v_rows + row * shape::kRowBytes + ((piece ^ (row & 7u)) << 4));
 #pragma unroll
       for (int n = 0; n < NT; n++) {
-        multiply_add<T>(acc[n][d], a, high[n][0], high[n][1]);
-        multiply_add<T>(acc[n][d], a, low[n][0], low[n][1]);
+#pragma unroll
+        for (int i = 0; i < N; i++) { multiply_add<T>(acc[n][d], a, part[n][0][i], part[n][1][i]); }
       }
     }
   }
@@ -362,7 +374,7 @@ struct mma_hooks {
 
   __device__ __forceinline__ void to_shared() const
   {
-    const float unshift = power_of_2(-halves<T>::kShift);
+    constexpr float unshift = 1.0f / summands<T>::kScale;
 #pragma unroll
     for (int n = 0; n < NT; n++) {
 #pragma unroll
@@ -382,7 +394,7 @@ struct mma_hooks {
   // A store of a warp is eight neighbouring columns of four rows.
   __device__ __forceinline__ void to_rows(uint32_t rows, uint32_t sequence, uint32_t head0, bool whole, uint32_t part) const
   {
-    const float unshift = power_of_2(-halves<T>::kShift);
+    constexpr float unshift = 1.0f / summands<T>::kScale;
 #pragma unroll
     for (int n = 0; n < NT; n++) {
 #pragma unroll
@@ -398,7 +410,7 @@ struct mma_hooks {
             if (d * 16 + 8 + g < c.dim) { o[d * 16 + 8] = from_float<T>(acc[n][d][h + 2] * scale); }
           }
           if (g == 0) {
-            result.lse[size_t(sequence) * (w.group * c.n_heads) + head0 + r] = (finite_top(top[n][h]) - halves<T>::kShift + log2f(sum[n][h])) * kLn2;
+            result.lse[size_t(sequence) * (w.group * c.n_heads) + head0 + r] = (finite_top(top[n][h]) - summands<T>::kLog2 + log2f(sum[n][h])) * kLn2;
           }
         } else {
           float* a = parts.acc + (size_t(part) * parts.rows + r) * c.dim + g;
