@@ -2,6 +2,7 @@
 from __future__ import annotations
 
 import ctypes as C
+import threading
 
 import numpy as np
 import torch
@@ -40,21 +41,30 @@ class Resources:
         L.check(self._lib.cuvsResourcesCreate(C.byref(h)))
         self.handle = h.value
         self._fixed_stream = stream
+        # `stream`: that of this thread's last call, if it was one that leaves the handle's own stream alone (the calls of kv_cache)
+        self._last = threading.local()
         if stream is not None:
             L.check(self._lib.cuvsStreamSet(self.handle, C.c_void_p(stream)))
 
     def use_current_stream(self):
+        self._last.stream = None
         if self._fixed_stream is None:
             L.check(self._lib.cuvsStreamSet(self.handle, _current_stream()))
 
     def stream_at_call(self, device: int) -> int:
         """The stream that a call made now uses: the fixed one, else torch's current one."""
+        self._last.stream = None
         if self._fixed_stream is not None:
             return self._fixed_stream
         return _raw_stream(device) if _raw_stream is not None else _current_stream()
 
     def sync(self):
-        L.check(self._lib.cuvsStreamSync(self.handle))
+        """Waits for the work of this thread's last call."""
+        stream = getattr(self._last, "stream", None)
+        if stream is None:
+            L.check(self._lib.cuvsStreamSync(self.handle))
+        else:
+            L.check(self._lib.cuvsB200KvCacheWait(self.handle, stream))
 
     def set_workspace_pool(self, nbytes: int):
         L.check(self._lib.cuvsResourcesSetWorkspacePool(self.handle, C.c_size_t(nbytes)))

@@ -527,12 +527,11 @@ struct call {
       std::memcpy(&scale, &bits, 4);
     }
   }
-  // False: it needs a workspace to itself.
+  // False: it needs a workspace to itself.  The handle's stream stays what it is: another thread may be in the middle of a search that reads it.
   bool run(cuvsResources_t res, cudaStream_t stream, int op, bool sync)
   {
     resources& r = single_device(res);
     device_scope on(r.device);
-    r.stream = stream;  // what cuvsStreamSync waits for
     if (sync) {
       cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
       CUDA_TRY(cudaStreamIsCapturing(stream, &capturing));

@@ -6,11 +6,11 @@
 
 #include <cstdint>
 
-// These calls go by the stream that they are given and touch nothing of the handle but its count of launches: several threads may make
-// them through one handle.
+// These calls go by the stream that they are given and touch nothing of the handle but its count of launches and, under a lock, its workspaces
+// of streams: several threads may make them through one handle, and one more may search through it meanwhile.
 namespace cuvs_b200::kv {
 
-inline void count_launches(resources& res, uint64_t n) { __atomic_fetch_add(&res.launches, n, __ATOMIC_RELAXED); }
+inline void count_launches(resources& res, uint64_t n) { res.launches += n; }
 
 enum class elem { f16, bf16, f32 };
 

@@ -109,6 +109,8 @@ def _call(resources, stream, op, tensors, integer, scale, sync):
     if _tensors is None:
         scalars = ((integer,), (integer, _bits(scale)), (_bits(scale),), ())[op]
         L.check(_arrays(resources.handle, stream, op, *_words(tensors[:_COUNTS[op]], scalars), sync))
+        if not sync:
+            resources._last.stream = stream
         return True
     status = _tensors(resources.handle, stream, op, *tensors, integer, scale, sync)
     if status == 2:
@@ -117,6 +119,8 @@ def _call(resources, stream, op, tensors, integer, scale, sync):
         L.check(L.CUVS_ERROR)
     if sync:
         L.check(_wait(resources.handle, stream))
+    else:
+        resources._last.stream = stream  # what resources.sync() waits for
     return True
 
 

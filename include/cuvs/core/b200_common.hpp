@@ -4,6 +4,7 @@
 
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
@@ -146,8 +147,8 @@ struct resources {
   std::unique_lock<std::mutex> stream_workspace(cudaStream_t on, size_t bytes, char** at);
   // small pinned host word for an occasional device->host scalar
   uint32_t* pinned = nullptr;
-  // counters read by the benchmark ("how many kernels of ours ran")
-  uint64_t launches = 0;
+  // counter read by the benchmark ("how many kernels of ours ran"); calls of several threads may add to it
+  std::atomic<uint64_t> launches{0};
 
   // Optional stage timing (off by default): five events per internal batch, resolved on demand.
   struct stage_events {

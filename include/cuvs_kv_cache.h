@@ -72,7 +72,7 @@ CUVS_EXPORT cuvsError_t cuvsKvCacheMergeParts(cuvsResources_t res, DLManagedTens
  * tensors come in the order of the calls, each as ndim | type code << 32 | bits << 40 | lanes << 48; address; device type | device
  * id << 32; the shape; the strides in elements -- or as one word 0 where there is none -- with a filter as a u32 tensor in the place
  * of its argument; behind them the scalars: {interleaved}, {window, bits of the f32 scale}, {bits of the scale}, {}.  The
- * work goes to `stream`, which becomes the handle's, and is waited for if `sync`. */
+ * work goes to `stream`, whatever the handle's own is, and is waited for if `sync`. */
 CUVS_EXPORT cuvsError_t cuvsB200KvCacheArrays(cuvsResources_t res, cudaStream_t stream, int op, const int64_t* words, int64_t n_words,
                                               bool sync);
 /* The same for a caller in Python: tensors as Python objects (of the type that the table of DLPack exchange functions is from, or none),

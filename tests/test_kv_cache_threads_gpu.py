@@ -1,0 +1,119 @@
+"""GPU tests of attention over a paged cache called from several threads and on several streams through one handle, beside searches."""
+import ctypes as C
+import threading
+
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+
+@pytest.fixture(autouse=True)
+def need_gpu():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+
+
+def generator(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def rows(shape, dtype, g, scale=1.0):
+    return (scale * torch.randn(shape, generator=g, device="cuda")).to(dtype)
+
+
+def ints(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+def shared(lengths, g, n_queries=1, heads=2, n_heads=8, dim=64, page_size=16, dtype=torch.float16):
+    """A cache with sequences whose units lie in several blocks' shares, so that the call needs a workspace; [queries], pages, lengths."""
+    from cuvs_b200 import kv_cache
+    used = [-(-n // page_size) for n in lengths]
+    keys, values = (rows((sum(used), page_size, heads, dim), dtype, g) for _ in range(2))
+    pages = torch.full((len(lengths), max(used)), -1, dtype=torch.int32, device="cuda")
+    order, at = torch.randperm(sum(used), generator=g, device="cuda").int(), 0
+    for i, n in enumerate(used):
+        pages[i, :n] = order[at:at + n]
+        at += n
+    queries = [rows((len(lengths), n_heads, dim), dtype, g) for _ in range(n_queries)]
+    assert kv_cache.attention_workspace(keys, queries[0], pages) > 0
+    return keys, values, queries, pages, ints(lengths)
+
+
+def handle_stream(resources):
+    from cuvs_b200 import _lib as L
+    at = C.c_void_p()
+    L.check(L.load().cuvsStreamGet(resources.handle, C.byref(at)))
+    return at.value or 0
+
+
+def test_calls_leave_the_stream_of_the_handle_alone():
+    """It belongs to the thread that searches through the handle; `sync` waits for the calls of the thread that asks all the same."""
+    from cuvs_b200 import Resources, kv_cache
+    g = generator(1)
+    keys, values, (q,), pages, n = shared([200_000, 100_000], g)
+    resources = Resources()
+    resources.use_current_stream()
+    before = handle_stream(resources)
+    side = torch.cuda.Stream()
+    want = kv_cache.attention(keys, values, q, pages, n)
+    slots = torch.randint(0, 1000, (2, 8, 20), generator=g, device="cuda")
+    torch.cuda.synchronize()
+    for sync in (True, False):
+        with torch.cuda.stream(side):
+            for _ in range(20):
+                got = kv_cache.attention(keys, values, q, pages, n, resources=resources, sync=sync)
+                kv_cache.attend_candidates(keys, values, q, slots, resources=resources, sync=sync)
+                kv_cache.merge_parts(torch.stack((got[0], got[0])), torch.stack((got[1], got[1])), resources=resources, sync=sync)
+                kv_cache.append(keys, values, keys[0, :2], values[0, :2], pages, ints([-1, -1]), resources=resources, sync=sync)
+            got = kv_cache.attention(keys, values, q, pages, n, resources=resources, sync=sync)
+        assert handle_stream(resources) == before
+        resources.sync()
+        assert side.query()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_a_search_and_attention_through_one_handle_at_once():
+    """One thread searches on its stream, others attend on theirs, all through the default handle of the device."""
+    from cuvs_b200 import ivf_pq, kv_cache
+    rng = np.random.default_rng(0)
+    data = torch.from_numpy(rng.standard_normal((20_000, 32), dtype=np.float32)).cuda()
+    asked = [torch.from_numpy(rng.standard_normal((m, 32), dtype=np.float32)).cuda() for m in (1, 100, 3000)]
+    index = ivf_pq.build(ivf_pq.IndexParams(n_lists=64, pq_dim=16, kmeans_n_iters=4), data)
+    params = ivf_pq.SearchParams(n_probes=16)
+    want_found = [ivf_pq.search(params, index, q, 10) for q in asked]
+    g = generator(2)
+    keys, values, queries, pages, n = shared([30_000, 4000, 70], g, n_queries=3)
+    want = [kv_cache.attention(keys, values, q, pages, n) for q in queries]
+    torch.cuda.synchronize()
+    wrong, done = [], threading.Event()
+
+    def search():
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for i in range(300):
+                    d, found = ivf_pq.search(params, index, asked[i % 3], 10)
+                    if not (torch.equal(d, want_found[i % 3][0]) and torch.equal(found, want_found[i % 3][1])):
+                        wrong.append(f"search {i}")
+        except Exception as e:
+            wrong.append(repr(e))
+        done.set()
+
+    def attend(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                while not done.is_set():
+                    out, lse = kv_cache.attention(keys, values, queries[i], pages, n)
+                    if not (torch.equal(out, want[i][0]) and torch.equal(lse, want[i][1])):
+                        wrong.append(f"attention of {i}")
+        except Exception as e:
+            wrong.append(repr(e))
+
+    threads = [threading.Thread(target=search)] + [threading.Thread(target=attend, args=(i,)) for i in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong, wrong[:5]
