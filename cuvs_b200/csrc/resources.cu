@@ -82,12 +82,15 @@ resources::~resources()
 
 std::unique_lock<std::mutex> resources::stream_workspace(cudaStream_t on, size_t bytes, char** at)
 {
+  unsigned long long id = 0;
+  CUDA_TRY(cudaStreamGetId(on, &id));
   std::unique_lock<std::mutex> held(stream_ws_lock);
-  if (stream_ws.size() >= 64 && stream_ws.find(on) == stream_ws.end()) {
+  if (stream_ws.size() >= 64 && stream_ws.find(id) == stream_ws.end()) {
     CUDA_TRY(cudaDeviceSynchronize());
     stream_ws.clear();
   }
-  workspace& w = stream_ws[on];
+  workspace& w = stream_ws[id];
+  if (w.capacity() != 0 && bytes > w.capacity()) { CUDA_TRY(cudaStreamSynchronize(on)); }
   w.reserve(bytes);
   *at = w.base();
   return held;

@@ -139,11 +139,12 @@ struct resources {
   int cc_major          = 0;
   workspace ws;       // search
   workspace scratch;  // extend and transform: some 2 GB at most (what their chunks need, and the labels of 2^26 rows)
-  // Workspaces of calls that several threads may make through one handle (attention over a paged cache), one for each stream.
-  std::map<cudaStream_t, workspace> stream_ws;
+  // Workspaces of calls that several threads may make through one handle (attention over a paged cache), one for each stream, by the streams'
+  // ids: a handle's value names another stream in every thread (cudaStreamPerThread), or a later one where one was destroyed with work in it.
+  std::map<unsigned long long, workspace> stream_ws;
   std::mutex stream_ws_lock;
   // The workspace of a stream, at least `bytes` large.  The lock is held until the call's work has been enqueued: another thread's call on
-  // the stream comes before or behind all of it, and may replace the workspace afterwards (and waits for the GPU then).
+  // the stream comes before or behind all of it, and may replace the workspace afterwards, once the stream's work is done.
   std::unique_lock<std::mutex> stream_workspace(cudaStream_t on, size_t bytes, char** at);
   // small pinned host word for an occasional device->host scalar
   uint32_t* pinned = nullptr;

@@ -117,3 +117,93 @@ def test_a_search_and_attention_through_one_handle_at_once():
     for t in threads:
         t.join()
     assert not wrong, wrong[:5]
+
+
+PER_THREAD = 2  # cudaStreamPerThread: one value for a stream of every thread
+
+
+def test_the_stream_of_each_thread():
+    """cudaStreamPerThread through one handle: every thread's stream has a workspace to itself."""
+    from cuvs_b200 import Resources, kv_cache
+    g = generator(3)
+    keys, values, queries, pages, n = shared([60_000, 9000, 20, 0, 30_000], g, n_queries=4, dim=128)
+    want = [kv_cache.attention(keys, values, q, pages, n) for q in queries]
+    resources = Resources(PER_THREAD)
+    places = [[(torch.empty_like(q), torch.empty(q.shape[:2], device="cuda")) for _ in range(10)] for q in queries]
+    torch.cuda.synchronize()
+    start, wrong = threading.Barrier(len(queries)), []
+
+    def work(i):
+        try:
+            start.wait(60)
+            for _ in range(20):
+                for out, lse in places[i]:
+                    kv_cache.attention(keys, values, queries[i], pages, n, out=out, lse=lse, resources=resources, sync=False)
+                resources.sync()
+                wrong.extend(i for out, lse in places[i] if not (torch.equal(out, want[i][0]) and torch.equal(lse, want[i][1])))
+        except Exception as e:
+            wrong.append(repr(e))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(queries))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong, wrong[:5]
+
+
+class NewStream:
+    """A stream of the runtime's own making, not one of torch's pool."""
+
+    def __init__(self):
+        at = C.c_uint64()
+        assert int(torch.cuda.cudart().cudaStreamCreate(C.addressof(at))) == 0
+        self.value = at.value
+
+    def current(self):
+        return torch.cuda.stream(torch.cuda.ExternalStream(self.value))
+
+    def destroy(self):
+        assert int(torch.cuda.cudart().cudaStreamDestroy(self.value)) == 0
+
+
+def test_streams_that_are_destroyed_with_work_in_them():
+    """The next stream may get the handle of one whose work goes on; more streams than the handle has workspaces for."""
+    from cuvs_b200 import kv_cache
+    g = generator(4)
+    keys, values, queries, pages, n = shared([60_000, 9000, 20, 30_000], g, n_queries=5)
+    want = [kv_cache.attention(keys, values, q, pages, n) for q in queries]
+    places = [(torch.empty_like(queries[0]), torch.empty(queries[0].shape[:2], device="cuda")) for _ in range(150)]
+    torch.cuda.synchronize()
+    alive = []
+    for i, (out, lse) in enumerate(places):
+        stream = NewStream()
+        with stream.current():
+            kv_cache.attention(keys, values, queries[i % 5], pages, n, out=out, lse=lse, sync=False)
+        if i % 2:
+            stream.destroy()
+        else:
+            alive.append(stream)
+    torch.cuda.synchronize()
+    for i, (out, lse) in enumerate(places):
+        assert torch.equal(out, want[i % 5][0]) and torch.equal(lse, want[i % 5][1]), i
+    for stream in alive:
+        stream.destroy()
+
+
+def test_a_workspace_that_grows_behind_queued_work():
+    from cuvs_b200 import Resources, kv_cache
+    g = generator(5)
+    small, large = shared([30_000], g), shared([60_000, 50_000, 40_000], g, heads=4, n_heads=16, dim=128)
+    need = [kv_cache.attention_workspace(c[0], c[2][0], c[3]) for c in (small, large)]
+    assert 0 < need[0] < need[1]
+    want = [kv_cache.attention(c[0], c[1], c[2][0], c[3], c[4]) for c in (small, large)]
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(5):
+        resources = Resources()
+        with torch.cuda.stream(side):
+            got = [kv_cache.attention(c[0], c[1], c[2][0], c[3], c[4], resources=resources, sync=False) for c in (small, small, small, large, small)]
+        resources.sync()
+        for a, w in zip(got, [want[0]] * 3 + [want[1], want[0]]):
+            assert torch.equal(a[0], w[0]) and torch.equal(a[1], w[1])
