@@ -549,17 +549,21 @@ struct call {
   }
 };
 
+constexpr int kNeedsWorkspace = 2;  // beside the values of cuvsError_t: nothing was done, the call needs a workspace to itself
+
 const tensor_exchange* g_exchange = nullptr;  // set once, when the Python module is imported
 const void* g_none                = nullptr;
 
 }  // namespace
 
-extern "C" cuvsError_t cuvsB200KvCacheArrays(cuvsResources_t res, cudaStream_t stream, int op, const int64_t* words, int64_t n_words, bool sync)
+extern "C" int cuvsB200KvCacheArrays(cuvsResources_t res, cudaStream_t stream, int op, const int64_t* words, int64_t n_words, bool sync)
 {
-  return translate_exceptions([=] {
-    CUVS_EXPECTS(call(op, words, n_words).run(res, stream, op, sync), kOwnWorkspace);
-    if (sync) { CUDA_TRY(cudaStreamSynchronize(stream)); }
+  int status = CUVS_ERROR;
+  const auto raised = translate_exceptions([&] {
+    status = call(op, words, n_words).run(res, stream, op, sync) ? CUVS_SUCCESS : kNeedsWorkspace;
+    if (sync && status == CUVS_SUCCESS) { CUDA_TRY(cudaStreamSynchronize(stream)); }
   });
+  return raised == CUVS_SUCCESS ? status : CUVS_ERROR;
 }
 
 extern "C" cuvsError_t cuvsB200SetTensorExchange(const void* table, const void* none)
@@ -589,7 +593,7 @@ extern "C" int cuvsB200KvCacheTensors(cuvsResources_t res, cudaStream_t stream, 
     c.interleaved = integer != 0;
     c.window      = integer;
     c.scale       = scale;
-    status        = c.run(res, stream, op, sync) ? CUVS_SUCCESS : 2;
+    status        = c.run(res, stream, op, sync) ? CUVS_SUCCESS : kNeedsWorkspace;
   });
   return raised == CUVS_SUCCESS ? status : CUVS_ERROR;
 }

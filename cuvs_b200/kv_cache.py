@@ -108,19 +108,17 @@ def _call(resources, stream, op, tensors, integer, scale, sync):
             return _call(resources, stream, op, tuple(_plain(t) for t in tensors), integer, scale, sync)
     if _tensors is None:
         scalars = ((integer,), (integer, _bits(scale)), (_bits(scale),), ())[op]
-        L.check(_arrays(resources.handle, stream, op, *_words(tensors[:_COUNTS[op]], scalars), sync))
-        if not sync:
-            resources._last.stream = stream
-        return True
-    status = _tensors(resources.handle, stream, op, *tensors, integer, scale, sync)
-    if status == 2:
+        status = _arrays(resources.handle, stream, op, *_words(tensors[:_COUNTS[op]], scalars), sync)
+    else:
+        status = _tensors(resources.handle, stream, op, *tensors, integer, scale, sync)
+    if status == _NEEDS_WORKSPACE:
         return False
     if status != L.CUVS_SUCCESS:
         L.check(L.CUVS_ERROR)
-    if sync:
-        L.check(_wait(resources.handle, stream))
-    else:
+    if not sync:
         resources._last.stream = stream  # what resources.sync() waits for
+    elif _tensors is not None:
+        L.check(_wait(resources.handle, stream))
     return True
 
 
@@ -147,6 +145,7 @@ def _tensor_calls():
 
 
 _COUNTS = (11, 9, 7, 4)
+_NEEDS_WORKSPACE = 2
 _Tensor = torch.Tensor
 _arrays = L.load().cuvsB200KvCacheArrays
 _workspace = L.load().cuvsB200KvCacheWorkspaceArrays

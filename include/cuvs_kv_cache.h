@@ -72,12 +72,12 @@ CUVS_EXPORT cuvsError_t cuvsKvCacheMergeParts(cuvsResources_t res, DLManagedTens
  * tensors come in the order of the calls, each as ndim | type code << 32 | bits << 40 | lanes << 48; address; device type | device
  * id << 32; the shape; the strides in elements -- or as one word 0 where there is none -- with a filter as a u32 tensor in the place
  * of its argument; behind them the scalars: {interleaved}, {window, bits of the f32 scale}, {bits of the scale}, {}.  The
- * work goes to `stream`, whatever the handle's own is, and is waited for if `sync`. */
-CUVS_EXPORT cuvsError_t cuvsB200KvCacheArrays(cuvsResources_t res, cudaStream_t stream, int op, const int64_t* words, int64_t n_words,
-                                              bool sync);
+ * work goes to `stream`, whatever the handle's own is, and is waited for if `sync`.  Returns a cuvsError_t, or 2 where the call needs a
+ * workspace to itself (attention that is captured): nothing was done then. */
+CUVS_EXPORT int cuvsB200KvCacheArrays(cuvsResources_t res, cudaStream_t stream, int op, const int64_t* words, int64_t n_words, bool sync);
 /* The same for a caller in Python: tensors as Python objects (of the type that the table of DLPack exchange functions is from, or none),
- * read in place; the caller holds the interpreter's lock.  `integer`: interleaved, or the window.  Returns 2 where the call needs a workspace
- * to itself: nothing was done then.  Does not wait: cuvsB200KvCacheWait does, without the lock. */
+ * read in place; the caller holds the interpreter's lock.  `integer`: interleaved, or the window.  Does not wait: cuvsB200KvCacheWait
+ * does, without the lock. */
 CUVS_EXPORT cuvsError_t cuvsB200SetTensorExchange(const void* table, const void* none);
 CUVS_EXPORT int cuvsB200KvCacheTensors(cuvsResources_t res, cudaStream_t stream, int op, void* t0, void* t1, void* t2, void* t3, void* t4,
                                        void* t5, void* t6, void* t7, void* t8, void* t9, void* t10, int64_t integer, float scale, bool sync);
