@@ -54,15 +54,18 @@ __device__ __forceinline__ void multiply_add<__nv_bfloat16>(float (&c)[4], const
 // A weight of 32 bits goes into the product with the values as the sum of 16-bit numbers, so that nothing is lost beside what the exponential
 // itself is off by: a row of the output is rounded once, at its end.  The products, twice or three times the mma.sync of one number, are to spare.
 // No summand is 0 where the weight is not: 0 times an infinite value would be no number.
+// `scale`: what weights are held times, `back` = 1 / scale, `to_room`: from there to what sums are left for others to join with.
 template <typename T>
 struct summands;
 template <>
 struct summands<__half> {
   // 11 bits, cut off, and the rest rounded to 11 bits: to 2^-22 of the weight.  Weights are held times 2^14, so that small ones keep their digits
   // above fp16's smallest number: it is 2^-38 of the largest weight, and what is below counts for nothing.
-  static constexpr int kCount   = 2;
-  static constexpr float kScale = 16384.0f;
-  static constexpr float kLog2  = 14.0f;
+  // (Sums of 2^31 values of 65,504 are far from the ends of 32 bits: no room is made for them.)
+  static constexpr int kCount = 2;
+  static __device__ __forceinline__ float scale(const work_view&) { return 16384.0f; }
+  static __device__ __forceinline__ float back(const work_view&) { return 1.0f / 16384.0f; }
+  static __device__ __forceinline__ float to_room(const work_view& w) { return w.room * (1.0f / 16384.0f); }
   static __device__ __forceinline__ void split(float a, float b, uint32_t (&part)[kCount])
   {
     constexpr float kSmallest = 5.9604644775390625e-8f;  // 2^-24
@@ -75,9 +78,10 @@ struct summands<__half> {
 template <>
 struct summands<__nv_bfloat16> {
   // Three times 8 bits, cut off: all of the weight.  (Two of them, rounded, left the weights of a batch of 32 requests 1.7e-5 off on average: 2^-16.)
-  static constexpr int kCount   = 3;
-  static constexpr float kScale = 1.0f;
-  static constexpr float kLog2  = 0.0f;
+  static constexpr int kCount = 3;
+  static __device__ __forceinline__ float scale(const work_view& w) { return w.room; }
+  static __device__ __forceinline__ float back(const work_view& w) { return w.back; }
+  static __device__ __forceinline__ float to_room(const work_view&) { return 1.0f; }
   static __device__ __forceinline__ uint32_t upper(float a, float b) { return __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632); }
   static __device__ __forceinline__ float cut(float a) { return __uint_as_float(__float_as_uint(a) & 0xFFFF0000u); }
   static __device__ __forceinline__ void split(float a, float b, uint32_t (&part)[kCount])
@@ -306,7 +310,7 @@ struct mma_hooks {
       float p[4];
 #pragma unroll
       for (int e = 0; e < 4; e++) {
-        p[e] = power_of_2(s[n][e] - finite_top(top[n][e & 1])) * summands<T>::kScale;
+        p[e] = power_of_2(s[n][e] - finite_top(top[n][e & 1])) * summands<T>::scale(w);
         sum[n][e & 1] += p[e];
       }
 #pragma unroll
@@ -374,18 +378,18 @@ struct mma_hooks {
 
   __device__ __forceinline__ void to_shared() const
   {
-    constexpr float unshift = 1.0f / summands<T>::kScale;
+    const float to_room = summands<T>::to_room(w);
 #pragma unroll
     for (int n = 0; n < NT; n++) {
 #pragma unroll
       for (int h = 0; h < 2; h++) {
         const uint32_t r = n * 8 + 2 * t + h;
-        if (g == 0) { state.stats[warp * shape::kRows + r] = make_float2(top[n][h], sum[n][h] * unshift); }
+        if (g == 0) { state.stats[warp * shape::kRows + r] = make_float2(top[n][h], sum[n][h] * to_room); }
         float* a = state.acc + (warp * shape::kRows + r) * shape::kAccRow + g;
 #pragma unroll
         for (int d = 0; d < D / 16; d++) {
-          a[d * 16]     = acc[n][d][h] * unshift;
-          a[d * 16 + 8] = acc[n][d][h + 2] * unshift;
+          a[d * 16]     = acc[n][d][h] * to_room;
+          a[d * 16 + 8] = acc[n][d][h + 2] * to_room;
         }
       }
     }
@@ -394,7 +398,7 @@ struct mma_hooks {
   // A store of a warp is eight neighbouring columns of four rows.
   __device__ __forceinline__ void to_rows(uint32_t rows, uint32_t sequence, uint32_t head0, bool whole, uint32_t part) const
   {
-    constexpr float unshift = 1.0f / summands<T>::kScale;
+    const float to_room = summands<T>::to_room(w);
 #pragma unroll
     for (int n = 0; n < NT; n++) {
 #pragma unroll
@@ -410,16 +414,16 @@ struct mma_hooks {
             if (d * 16 + 8 + g < c.dim) { o[d * 16 + 8] = from_float<T>(acc[n][d][h + 2] * scale); }
           }
           if (g == 0) {
-            result.lse[size_t(sequence) * (w.group * c.n_heads) + head0 + r] = (finite_top(top[n][h]) - summands<T>::kLog2 + log2f(sum[n][h])) * kLn2;
+            result.lse[size_t(sequence) * (w.group * c.n_heads) + head0 + r] = (finite_top(top[n][h]) + log2f(sum[n][h] * summands<T>::back(w))) * kLn2;
           }
         } else {
           float* a = parts.acc + (size_t(part) * parts.rows + r) * c.dim + g;
 #pragma unroll
           for (int d = 0; d < D / 16; d++) {
-            if (d * 16 + g < c.dim) { a[d * 16] = acc[n][d][h] * unshift; }
-            if (d * 16 + 8 + g < c.dim) { a[d * 16 + 8] = acc[n][d][h + 2] * unshift; }
+            if (d * 16 + g < c.dim) { a[d * 16] = acc[n][d][h] * to_room; }
+            if (d * 16 + 8 + g < c.dim) { a[d * 16 + 8] = acc[n][d][h + 2] * to_room; }
           }
-          if (g == 0) { parts.stats[size_t(part) * parts.rows + r] = make_float2(top[n][h], sum[n][h] * unshift); }
+          if (g == 0) { parts.stats[size_t(part) * parts.rows + r] = make_float2(top[n][h], sum[n][h] * to_room); }
         }
       }
     }

@@ -189,7 +189,7 @@ struct rows_hooks {
         const float safe = finite_top(next);
         const float keep = power_of_2(top[r] - safe);
         top[r]           = next;
-        const float weight = power_of_2(score - safe);
+        const float weight = power_of_2(score - safe) * w.room;
         sum[r]             = sum[r] * keep + weight;  // of the lane's own rows, until close()
 #pragma unroll
         for (int p = 0; p < PIECES; p++) {
@@ -301,7 +301,7 @@ struct rows_hooks {
             store_piece<T>(result.out, sequence, head0 + r, gl + p * LANES, x);
           }
         }
-        if (gl == 0) { result.lse[size_t(sequence) * (w.group * c.n_heads) + head0 + r] = (finite_top(top[r]) + log2f(sum[r])) * kLn2; }
+        if (gl == 0) { result.lse[size_t(sequence) * (w.group * c.n_heads) + head0 + r] = (finite_top(top[r]) + log2f(sum[r] * w.back)) * kLn2; }
       } else {
         to_floats(parts.acc + (size_t(part) * parts.rows + r) * c.dim, r);
         if (gl == 0) { parts.stats[size_t(part) * parts.rows + r] = make_float2(top[r], sum[r]); }
@@ -402,7 +402,8 @@ void launch_candidates(resources& res, cudaStream_t stream, const candidates_arg
   p.resident          = resident_of(1, false);
   p.large             = large_of(1, false);
   deal_out(res, p, uint64_t(a.n_tokens) * a.n_query_heads, a.n_candidates, false);
-  const work_view w{a.n_tokens, a.n_query_heads, group, group, p.cluster, 0};
+  work_view w{a.n_tokens, a.n_query_heads, group, group, p.cluster, 0};
+  make_room(w, a.n_candidates);
   by_pieces(pieces, [&](auto lanes, auto n) {
     constexpr int LANES = decltype(lanes)::value, PIECES = decltype(n)::value;
     if constexpr (sizeof(T) == 4 || PIECES == 1) {
@@ -427,7 +428,9 @@ void attention(resources& res, cudaStream_t stream, const attention_args& a)
   const uint32_t group = a.n_query_heads / c.n_heads;
   const plan p         = attention_plan(res, a.type, a.n_sequences, c.n_heads, group, c.dim, uint64_t(a.table_width) * c.page.size, a.window);
   const uint32_t of    = ceildiv(group, p.rows);
-  const work_view w{a.n_sequences, c.n_heads * of, of, group, p.cluster, p.cost};
+  const uint64_t longest = uint64_t(a.table_width) * c.page.size;
+  work_view w{a.n_sequences, c.n_heads * of, of, group, p.cluster, p.cost};
+  make_room(w, a.window > 0 ? std::min(longest, uint64_t(a.window)) : longest);
   const positions lists{a.pages, a.lengths, a.table_stride, a.window, a.table_width};
   const result_view result{a.out, a.lse};
   parts_view parts{};

@@ -24,6 +24,7 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <cmath>
 
 namespace cuvs_b200::kv {
 
@@ -38,7 +39,20 @@ struct work_view {
   uint32_t group;        // query heads of one key head
   uint32_t cluster;      // blocks of a unit's cluster; 0: shares
   uint32_t cost;         // of a unit beside its rows (queries, joining, writing), in chunks: what it counts for where shares are dealt out
+  // Weights are held times `room`, a power of two that keeps the sum of a whole list below 1: weighted sums, which are divided by it at their end,
+  // stay below the largest value then, and finite where the answer is (times 1, 1,500 rows of 3e38 gave infinity).  What that costs is at the
+  // other end of the range: values below 1e-25 in lists of 2^17 rows lose digits.  `back` = 1 / room.
+  float room, back;
 };
+
+// For lists of `rows` at most.
+inline void make_room(work_view& w, uint64_t rows)
+{
+  int bits = 1;
+  while (bits < 32 && (uint64_t(1) << (bits - 1)) < rows) { bits++; }
+  w.room = std::ldexp(1.0f, -bits);
+  w.back = std::ldexp(1.0f, bits);
+}
 
 // ---- lists --------------------------------------------------------------------------------------------------------------------
 
@@ -280,7 +294,7 @@ __device__ __forceinline__ void join_warps(const cache_view& c, const work_view&
 #pragma unroll
       for (uint32_t e = 0; e < E; e++) { x[e] *= scale; }
       store_piece<T>(result.out, sequence, head0 + r, piece, x);
-      if (piece == 0) { result.lse[size_t(sequence) * (w.group * c.n_heads) + head0 + r] = (safe + log2f(sum)) * kLn2; }
+      if (piece == 0) { result.lse[size_t(sequence) * (w.group * c.n_heads) + head0 + r] = (safe + log2f(sum * w.back)) * kLn2; }
     } else {
       float4* a = reinterpret_cast<float4*>(s.acc + size_t(r) * s.acc_row + piece * E);
 #pragma unroll
@@ -325,7 +339,7 @@ __device__ __forceinline__ void join_cluster(const cache_view& c, const work_vie
 #pragma unroll
     for (uint32_t e = 0; e < E; e++) { x[e] *= scale; }
     store_piece<T>(result.out, sequence, head0 + r, piece, x);
-    if (piece == 0) { result.lse[size_t(sequence) * (w.group * c.n_heads) + head0 + r] = (safe + log2f(sum)) * kLn2; }
+    if (piece == 0) { result.lse[size_t(sequence) * (w.group * c.n_heads) + head0 + r] = (safe + log2f(sum * w.back)) * kLn2; }
   }
   cluster.sync();  // no block leaves while others read its shared memory
 }
@@ -404,8 +418,8 @@ __device__ __forceinline__ void join_some(const parts_view& parts, uint32_t shar
 }
 
 template <typename T>
-__device__ __forceinline__ void write_joined(const result_view& result, uint32_t sequence, uint32_t head, uint32_t heads, uint32_t dim, float top,
-                                             float sum, const float (&x)[2][4])
+__device__ __forceinline__ void write_joined(const work_view& w, const result_view& result, uint32_t sequence, uint32_t head, uint32_t heads,
+                                             uint32_t dim, float top, float sum, const float (&x)[2][4])
 {
   const uint32_t lane = threadIdx.x & 31u;
   const float scale   = sum == 0.0f ? 0.0f : 1.0f / sum;
@@ -423,7 +437,7 @@ __device__ __forceinline__ void write_joined(const result_view& result, uint32_t
       *reinterpret_cast<uint4*>(o + column) = *reinterpret_cast<const uint4*>(z);
     }
   }
-  if (lane == 0) { result.lse[size_t(sequence) * heads + head] = (finite_top(top) + log2f(sum)) * kLn2; }
+  if (lane == 0) { result.lse[size_t(sequence) * heads + head] = (finite_top(top) + log2f(sum * w.back)) * kLn2; }
 }
 
 // Every warp looks at its (share, row) pairs: rows of a few parts are joined by the warp alone, those of many by the block's warps together.
@@ -455,7 +469,7 @@ join_kernel(work_view w, parts_view parts, uint32_t dim, uint32_t n_heads, resul
     if (base + warp < pairs && row_of(base + warp, share, r, unit, head)) {
       if (unit.z <= uint32_t(kJoinAlone)) {
         join_some(parts, share, unit.z, r, dim, 0u, 1u, top, sum, x);
-        write_joined<T>(result, unit.x, head, heads, dim, top, sum, x);
+        write_joined<T>(w, result, unit.x, head, heads, dim, top, sum, x);
       } else if (lane == 0) {
         s_many[atomicAdd(&s_n, 1u)] = base + warp;
       }
@@ -490,7 +504,7 @@ join_kernel(work_view w, parts_view parts, uint32_t dim, uint32_t n_heads, resul
             x[u][3]        = fmaf(y.w, f, x[u][3]);
           }
         }
-        write_joined<T>(result, unit.x, head, heads, dim, top, sum, x);
+        write_joined<T>(w, result, unit.x, head, heads, dim, top, sum, x);
       }
       __syncthreads();
     }

@@ -14,8 +14,8 @@ rows of ``dim`` elements contiguous and on 16-byte boundaries.  A token's slot i
 its key is put into an index.  ``pages`` (int32 ``[n_sequences, width]``) names the pages of each sequence in the order of its positions;
 an entry that is no page of the cache, such as -1, holds no tokens.  Query head ``i`` reads the rows of head
 ``i // (n_query_heads // n_heads)``.  Softmax and sums are held in 32 bits, outputs are rounded once; where nothing may be attended to, the
-output is 0 and its ``lse`` is -inf.  Weights below 2^-126 of the largest count as 0, in :func:`attention` over float16 those below 2^-38 (times
-an infinite value that is no number).
+output is 0 and its ``lse`` is -inf.  Weights below 2^-100 of the largest may count as 0, in :func:`attention` over float16 those below 2^-38
+(times an infinite value that is no number).
 
 These calls serve: they have no gradients.  They enqueue their work on the stream of ``resources`` (torch's current stream by default) and
 wait for it unless ``sync=False``, which is what a captured call needs.

@@ -60,7 +60,7 @@ def test_weights_keep_their_digits(dtype, dim, heads):
 @pytest.mark.parametrize("dtype", TYPES)
 def test_infinite_values_of_small_weights(dtype):
     """A row of infinite values makes the output infinite however small its weight is, as far as the weights reach: 2^-38 of the largest weight
-    for fp16 (exp(-26) is 2^-37.5), 2^-126 else (exp(-87) is 2^-125.5)."""
+    for fp16 (exp(-26) is 2^-37.5), 2^-126 else in lists as short as these (exp(-87) is 2^-125.5)."""
     from cuvs_b200 import kv_cache
     n = 27 if dtype == torch.float16 else 88
     keys = torch.zeros((n, 16, 1, 64), dtype=dtype, device="cuda")
@@ -75,3 +75,75 @@ def test_infinite_values_of_small_weights(dtype):
         want = values[:, 1].expand_as(out)
         assert torch.equal(out[..., 0::4], want[..., 0::4]) and torch.equal(out[..., 1::4], want[..., 1::4]) and torch.equal(out[..., 2::4], want[..., 2::4])
         assert ((out[..., 3::4] - 1).abs() <= torch.finfo(dtype).eps).all()
+
+
+WIDE = [torch.bfloat16, torch.float32]
+LARGEST = 3.0e38   # of 3.4e38
+
+
+def tables(lengths, page):
+    """Pages in order, one sequence behind the other, and how many they are."""
+    used = [-(-n // page) for n in lengths]
+    pages = torch.full((len(lengths), max(used)), -1, dtype=torch.int32, device="cuda")
+    at = 0
+    for i, n in enumerate(used):
+        pages[i, :n] = torch.arange(at, at + n)
+        at += n
+    return pages, at
+
+
+def near(out, want, n, dtype):
+    """Sums of n equal terms: n / 4 + 592 additions follow one another at most, in the sum of values and in that of weights."""
+    return ((out.double() - want.double()).abs() <= (2 * (n / 4 + 592) * U + torch.finfo(dtype).eps / 2) * want.double().abs()).all()
+
+
+@pytest.mark.parametrize("dtype", WIDE)
+@pytest.mark.parametrize("lengths,heads,group,dim,window", [
+    ([1500], 1, 4, 64, None), ([1, 700, 0, 20], 3, 1, 128, None), ([3000, 20, 0, 700] * 20, 2, 3, 64, None), ([60000], 1, 1, 64, None),
+    ([40000, 300], 2, 8, 128, 30000), ([5000] * 10, 2, 12, 256, None), ([900] * 300, 4, 1, 64, 700)])
+def test_values_next_to_the_largest(dtype, lengths, heads, group, dim, window):
+    """Rows of the same values have the same values as their mean, and finite ones."""
+    from cuvs_b200 import kv_cache
+    pages, n_pages = tables(lengths, 16)
+    keys = torch.zeros((n_pages, 16, heads, dim), dtype=dtype, device="cuda")
+    values = torch.full_like(keys, LARGEST)
+    values[..., 1::2] = -LARGEST
+    queries = torch.randn((len(lengths), heads * group, dim), generator=generator(1), device="cuda").to(dtype)
+    out, lse = kv_cache.attention(keys, values, queries, pages, ints(lengths), window=window)
+    for i, n in enumerate(lengths):
+        n = min(n, window or n)
+        assert near(out[i], values[0, 0, 0] if n else torch.zeros_like(out[i]), n, dtype), i
+        assert ((lse[i].double() - math.log(n)).abs() <= (n / 4 + 600) * U).all() if n else (lse[i] == -math.inf).all()
+
+
+@pytest.mark.parametrize("dtype", WIDE)
+@pytest.mark.parametrize("n,k", [(1, 700), (1, 20_000), (300, 40)])
+def test_values_next_to_the_largest_among_candidates(dtype, n, k):
+    from cuvs_b200 import kv_cache
+    g = generator(2)
+    keys = torch.zeros((50, 16, 2, 64), dtype=dtype, device="cuda")
+    values = torch.full_like(keys, -LARGEST)
+    candidates = torch.randint(0, 800, (n, 4, k), generator=g, device="cuda")
+    out, lse = kv_cache.attend_candidates(keys, values, torch.randn((n, 4, 64), generator=g, device="cuda").to(dtype), candidates)
+    assert near(out, values[0, 0, 0], k, dtype) and ((lse.double() - math.log(k)).abs() <= (k / 4 + 600) * U).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_small_values_keep_their_digits(dtype):
+    """The other end: the smallest normal numbers of fp16; 1e-25, which leaves room for 24 digits and lists of 2^15 rows above 2^-126."""
+    from cuvs_b200 import kv_cache
+    g = generator(3)
+    lengths = [20_000, 300, 5]
+    pages, n_pages = tables(lengths, 16)
+    small = 6.2e-5 if dtype == torch.float16 else 1e-25
+    keys = torch.zeros((n_pages, 16, 2, 64), dtype=dtype, device="cuda")
+    values = (small * (1 + torch.rand((n_pages, 16, 2, 64), generator=g, device="cuda"))).to(dtype)
+    queries = torch.randn((3, 4, 64), generator=g, device="cuda").to(dtype)
+    out, _ = kv_cache.attention(keys, values, queries, pages, ints(lengths))
+    at = 0
+    for i, n in enumerate(lengths):
+        used = -(-n // 16)
+        mean = values[at:at + used].reshape(-1, 2, 64)[:n].double().mean(0).repeat_interleave(2, 0)
+        at += used
+        tol = (2 * (n / 4 + 592) * U + torch.finfo(dtype).eps / 2) * mean + (2.0 ** -25 if dtype == torch.float16 else 0.0)
+        assert ((out[i].double() - mean).abs() <= tol).all(), i
