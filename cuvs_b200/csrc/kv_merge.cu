@@ -1,6 +1,7 @@
 // Joining parts of one softmax: parts o_p of disjoint sets of rows, each with the logarithm lse_p of its denominator, give
 //   lse = log sum_p exp(lse_p),   o = sum_p exp(lse_p - lse) o_p.
-// A part that attended to nothing (lse_p = -inf) has weight 0, and what its row holds does not count.
+// A part that attended to nothing (lse_p = -inf) has weight 0, and what its row holds does not count.  Weights are divided by their sum before rows
+// are multiplied by them: sums of values next to the largest stay finite.
 //
 // What bounds it: HBM (every part is read once, the result written once), through the bytes in flight.  A group of lanes has a row.  It
 // asks for the first eight parts' pieces at once and, while they come, for the lse; its lanes take the weights of as many parts as there
@@ -59,7 +60,7 @@ __global__ void __launch_bounds__(kThreads, 4) merge_kernel(merge_args a, uint32
     float mine       = 0.0f;
     for (uint32_t p0 = 0; p0 < a.n_parts; p0 += AHEAD) {
       if (j0 != 0 || p0 != 0) { ask(j, p0); }
-      if (p0 % LANES == 0) { mine = p0 + lane < a.n_parts ? expf((p0 == 0 ? first : lse[int64_t(p0 + lane) * a.l_part]) - top) : 0.0f; }
+      if (p0 % LANES == 0) { mine = p0 + lane < a.n_parts ? expf((p0 == 0 ? first : lse[int64_t(p0 + lane) * a.l_part]) - top) * scale : 0.0f; }
 #pragma unroll
       for (int q = 0; q < AHEAD; q++) {
         const float w = __shfl_sync(kAllLanes, mine, (p0 + q) % LANES, LANES);
@@ -69,8 +70,6 @@ __global__ void __launch_bounds__(kThreads, 4) merge_kernel(merge_args a, uint32
         for (int e = 0; e < E; e++) { acc[e] = w != 0.0f ? fmaf(w, x[e], acc[e]) : acc[e]; }
       }
     }
-#pragma unroll
-    for (int e = 0; e < E; e++) { acc[e] *= scale; }
     if (asked < n_rows && j < pieces) {
       reinterpret_cast<uint4*>(a.out.data + (int64_t(token) * a.out.row + int64_t(head) * a.out.head) * int64_t(sizeof(T)))[j] =
         floats_to_piece<T>(acc);

@@ -147,3 +147,20 @@ def test_small_values_keep_their_digits(dtype):
         at += used
         tol = (2 * (n / 4 + 592) * U + torch.finfo(dtype).eps / 2) * mean + (2.0 ** -25 if dtype == torch.float16 else 0.0)
         assert ((out[i].double() - mean).abs() <= tol).all(), i
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n_parts,dim", [(2, 128), (9, 64), (40, 256), (7, 24)])
+def test_parts_next_to_the_largest(dtype, n_parts, dim):
+    from cuvs_b200 import kv_cache
+    parts = torch.full((n_parts, 5, 3, dim), 65000.0 if dtype == torch.float16 else LARGEST, dtype=dtype, device="cuda")
+    parts[..., 1::2] *= -1
+    lse = torch.full((n_parts, 5, 3), 4.0, device="cuda")
+    lse[1:, 0] = -math.inf
+    out, joined = kv_cache.merge_parts(parts, lse)
+    # weights and their sum: n_parts additions each, 2^-22 for the exponentials, a few roundings
+    tol = (2 * n_parts + 16) * U + torch.finfo(dtype).eps / 2
+    assert ((out.double() - parts[0].double()).abs() <= tol * parts[0].double().abs()).all()
+    want = torch.full((5, 3), 4.0 + math.log(n_parts), device="cuda").double()
+    want[0] = 4.0
+    assert ((joined.double() - want).abs() <= (n_parts + 16) * U * want).all()
