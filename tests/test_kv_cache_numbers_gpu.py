@@ -164,3 +164,28 @@ def test_parts_next_to_the_largest(dtype, n_parts, dim):
     want = torch.full((5, 3), 4.0 + math.log(n_parts), device="cuda").double()
     want[0] = 4.0
     assert ((joined.double() - want).abs() <= (n_parts + 16) * U * want).all()
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_sine_and_cosine(interleaved):
+    """Rows of (1, 0) pairs are turned into the cosine and the sine themselves.  A step of values below 1 is u at most: the 32-bit functions are
+    within one of them, and turning them by the angle's last digits rounds once more, by half a step.  Errors spread evenly within that
+    have a root mean square of sqrt(1/3 + 1/12) u = 0.65 u, were all values above 1/2; a third of them is not."""
+    from cuvs_b200 import kv_cache
+    g = generator(4)
+    n, dim, half = 4000, 128, 64
+    nothing = torch.zeros((n, 1, dim), device="cuda")
+    keys, values = torch.zeros((2, 4, 16, 1, dim), device="cuda")
+    positions = torch.cat((torch.arange(100, device="cuda"), torch.randint(0, 1_000_000, (n - 100,), generator=g, device="cuda"))).int()
+    f = torch.tensor([10000.0 ** (-i / half) for i in range(half)], dtype=torch.float64, device="cuda")
+    queries = nothing.clone()
+    queries[..., slice(0, dim, 2) if interleaved else slice(0, half)] = 1
+    _, turned = kv_cache.append(keys, values, nothing, nothing, torch.full((n, 1), -1, dtype=torch.int32, device="cuda"), positions, queries=queries,
+                                frequencies=f, interleaved=interleaved)
+    pairs = turned[:, 0].view(n, half, 2) if interleaved else turned[:, 0].view(n, 2, half).transpose(1, 2)
+    angle = positions.double()[:, None] * f
+    for got, want in ((pairs[..., 0], angle.cos()), (pairs[..., 1], angle.sin())):
+        off = (got.double() - want).abs()
+        # the product of position and frequency is rounded to 2^-53 of an angle of up to 2^20
+        assert (off <= 1.5 * U + 2.0 ** -33).all(), off.max().item() / U
+        assert off.square().mean().sqrt() <= 0.65 * U
