@@ -1,13 +1,18 @@
 """Attention over a paged cache of keys and values, next to the search over its keys.
 
 A decoder keeps the keys and values of its tokens in pages and reaches back over a context that is too long to be read in full by a
-search over the keys.  A step then is::
+search over the keys.  A step of several sequences, one token each, then is::
 
     slots, q = kv_cache.append(keys, values, new_keys, new_values, pages, positions, queries=queries, frequencies=frequencies)
-    _, candidates = ivf_pq.search(params, index_of_head, q[:, head], k)         # an index whose source ids are slots
     near = kv_cache.attention(keys, values, q, pages, lengths, window=window)
-    far = kv_cache.attend_candidates(keys, values, q, candidates)               # [n_tokens, n_query_heads, k]
+    # index[i][h]: over the keys of sequence i and key head h before the window, in float32, whose source ids are slots
+    own = q.float().unflatten(1, (n_heads, -1))
+    candidates = torch.stack([torch.cat([ivf_pq.search(params, index[i][h], own[i, h], k)[1] for h in range(n_heads)])
+                              for i in range(len(own))])
+    far = kv_cache.attend_candidates(keys, values, q, candidates)               # [n_sequences, n_query_heads, k]
     out, lse = kv_cache.merge_parts(torch.stack((near[0], far[0])), torch.stack((near[1], far[1])))
+
+An index that several sequences share would name slots of all of them for each: :func:`attend_candidates` attends to whatever a list names.
 
 ``keys`` and ``values`` are ``[n_pages, page_size, n_heads, dim]`` tensors of float16, bfloat16 or float32, of any strides that leave the
 rows of ``dim`` elements contiguous and on 16-byte boundaries.  A token's slot is ``page * page_size + place``, and is the id under which
@@ -224,7 +229,7 @@ def _attention_workspace(resources, keys, queries, pages, window):
 def attend_candidates(keys, values, queries, candidates, scale=None, filter=None, out=None, lse=None,
                       resources: Resources | None = None, sync: bool = True):
     """Attention of every query head of a token to the slots that its list names: ``candidates``, int64 ``[n_tokens, n_query_heads, k]``, as
-    searches over the keys return them.  Ids that are no slots (the search's "no such neighbour", -1) and slots that ``filter`` leaves out
+    searches over the keys of the token's sequence return them (whose slots they are is not looked at).  Ids that are no slots (the search's "no such neighbour", -1) and slots that ``filter`` leaves out
     are skipped; a slot that is named twice counts twice.  Returns ``(out, lse)`` as :func:`attention` does."""
     resources, stream = _handle(keys, resources)
     if queries.dim() != 3:
@@ -242,7 +247,7 @@ def attend_candidates(keys, values, queries, candidates, scale=None, filter=None
 def merge_parts(parts, parts_lse, out=None, lse=None, resources: Resources | None = None, sync: bool = True):
     """Joins parts of one softmax over disjoint sets of rows: ``parts`` ``[n_parts, n_tokens, n_heads, dim]`` and their ``parts_lse``, float32
     ``[n_parts, n_tokens, n_heads]``, both of any strides between rows (blocks gathered from several GPUs, say).  Returns ``(out, lse)``.  What
-    the row of a part holds whose lse is -inf does not count."""
+    the row of a part holds whose lse is -inf does not count.  Parts have been rounded to their type before, the joined rows are once more."""
     resources, stream = _handle(parts, resources)
     if parts.dim() != 4:
         raise ValueError(f"parts: 4 dimensions, not {parts.dim()}")
