@@ -373,7 +373,7 @@ plan attention_plan(const resources& res, elem type, uint64_t sequences, uint32_
     p.large    = mma_large_of(d, eights);
     p.cost     = 8 * eights * (d == 256 ? 2 : 1);
   }
-  deal_out(res, p, sequences * n_heads * ceildiv(group, p.rows), most, true);
+  deal_out(uint32_t(res.sm_count), res.clusters_at_once, p, sequences * n_heads * ceildiv(group, p.rows), most, true);
   return p;
 }
 
@@ -401,7 +401,7 @@ void launch_candidates(resources& res, cudaStream_t stream, const candidates_arg
   p.chunk             = chunk_of(room_of(pieces), 1);
   p.resident          = resident_of(1, false);
   p.large             = large_of(1, false);
-  deal_out(res, p, uint64_t(a.n_tokens) * a.n_query_heads, a.n_candidates, false);
+  deal_out(uint32_t(res.sm_count), res.clusters_at_once, p, uint64_t(a.n_tokens) * a.n_query_heads, a.n_candidates, false);
   work_view w{a.n_tokens, a.n_query_heads, group, group, p.cluster, 0};
   make_room(w, a.n_candidates);
   by_pieces(pieces, [&](auto lanes, auto n) {

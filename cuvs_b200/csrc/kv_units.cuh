@@ -19,6 +19,7 @@
 // Nothing depends on the order in which blocks run.
 #pragma once
 
+#include "kv_plan.hpp"
 #include "kv_rows.cuh"
 
 #include <cooperative_groups.h>
@@ -27,10 +28,6 @@
 #include <cmath>
 
 namespace cuvs_b200::kv {
-
-// Warps of a block: small blocks, several to an SM, balance best; where units are fewer than SMs, one large block has an SM's warps for one
-// unit.
-constexpr int kSmall = 4;
 
 struct work_view {
   uint32_t n_sequences;
@@ -131,7 +128,7 @@ __device__ __forceinline__ uint64_t quotient(uint64_t a, uint32_t b)
 
 // `total` chunks of all units dealt out in `count` equal shares: one for every block, or fewer of kLeast chunks each (one for each of its warps).
 struct share {
-  static constexpr uint32_t kLeast = 4;  // chunks
+  static constexpr uint32_t kLeast = kLeastShare;
   uint64_t total, each;
   uint32_t count, longer;  // the first `longer` get `each` + 1, the others `each`
   __device__ __forceinline__ share(uint64_t total_, uint32_t most)
@@ -803,48 +800,6 @@ void launch_units(cudaStream_t stream, void (*kernel)(Params...), uint32_t block
   config.attrs            = attrs;
   config.numAttrs         = cluster > 1 ? 2 : 1;
   CUDA_TRY(cudaLaunchKernelEx(&config, kernel, std::forward<Args>(args)...));
-}
-
-// What a call launches, by type and sizes alone.
-struct plan {
-  uint32_t rows;      // query heads of a unit
-  uint32_t chunk;     // rows of the cache that a warp takes at a time
-  uint32_t resident;  // small blocks of an SM
-  uint32_t large;     // warps of a large block; 0: there is none
-  uint32_t warps;     // of a block
-  uint32_t blocks;
-  uint32_t cluster;   // 0: shares
-  uint32_t cost;      // of a unit beside its rows, in chunks
-  bool parts;         // a unit may lie in several shares
-};
-
-// `most`: rows of a unit, at most; `shares`: whether there may be any.  Clusters where one wave of them has few chunks for a warp: one request of
-// 4,096 tokens and 8 key heads (3 each) 9.1 us, 11.9 in shares; two of up to 6,144 (4 each) 17.1 and 14.5.
-inline void deal_out(const resources& res, plan& p, uint64_t units, uint64_t most, bool shares)
-{
-  const uint64_t sms = uint64_t(res.sm_count), resident = sms * p.resident;
-  p.parts = false;
-  if (units <= sms) {
-    p.warps               = p.large ? p.large : kSmall;
-    const uint64_t chunks = ceildiv<uint64_t>(most, p.warps * p.chunk);
-    uint32_t cluster      = 1;
-    while (cluster < 8 && 2 * cluster * units <= sms && cluster < chunks) { cluster *= 2; }
-    if (!shares || ceildiv<uint64_t>(chunks, cluster) <= 4) {
-      p.blocks  = uint32_t(units * cluster);
-      p.cluster = cluster;
-      return;
-    }
-  }
-  p.warps = kSmall;
-  if (!shares) {
-    p.blocks  = uint32_t(units);
-    p.cluster = 1;
-  } else {
-    const uint64_t chunks = std::max<uint64_t>(1, ceildiv<uint64_t>(most, p.chunk));
-    p.blocks              = uint32_t(std::min(resident, units * ceildiv<uint64_t>(chunks, share::kLeast)));
-    p.cluster             = 0;
-    p.parts               = chunks > 1;
-  }
 }
 
 template <typename T>

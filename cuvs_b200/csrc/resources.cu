@@ -52,6 +52,32 @@ void ensure_dynamic_smem(const void* kernel, size_t bytes)
   }
 }
 
+namespace {
+// A kernel whose block has an SM's shared memory to itself; it is only asked about, not launched.
+__global__ void whole_sm_kernel() {}
+
+void ask_for_clusters(uint32_t (&at_once)[4], size_t whole_sm)
+{
+  ensure_dynamic_smem(reinterpret_cast<const void*>(whole_sm_kernel), whole_sm);
+  for (int log = 0; log < 4; log++) {
+    cudaLaunchAttribute attr{};
+    attr.id               = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = 1u << log;
+    attr.val.clusterDim.y = 1;
+    attr.val.clusterDim.z = 1;
+    cudaLaunchConfig_t config{};
+    config.gridDim          = 1u << log;
+    config.blockDim         = 128;
+    config.dynamicSmemBytes = whole_sm;
+    config.attrs            = &attr;
+    config.numAttrs         = 1;
+    int n                   = 0;
+    CUDA_TRY(cudaOccupancyMaxActiveClusters(&n, whole_sm_kernel, &config));
+    at_once[log] = uint32_t(n);
+  }
+}
+}  // namespace
+
 resources::resources()
 {
   CUDA_TRY(cudaGetDevice(&device));
@@ -60,6 +86,7 @@ resources::resources()
   sm_count   = prop.multiProcessorCount;
   smem_optin = static_cast<int>(prop.sharedMemPerBlockOptin);
   cc_major   = prop.major;
+  ask_for_clusters(clusters_at_once, size_t(smem_optin));
   CUDA_TRY(cudaMallocHost(&pinned, 64));
   pinned[12] = 0;
   pinned[13] = 0;

@@ -137,6 +137,7 @@ struct resources {
   int sm_count          = 0;
   int smem_optin        = 0;        // max dynamic shared memory per block (opt-in)
   int cc_major          = 0;
+  uint32_t clusters_at_once[4] = {};  // thread-block clusters of 1, 2, 4, 8 blocks that the GPU holds, with a block to an SM
   workspace ws;       // search
   workspace scratch;  // extend and transform: some 2 GB at most (what their chunks need, and the labels of 2^26 rows)
   // Workspaces of calls that several threads may make through one handle (attention over a paged cache), one for each stream, by the streams'

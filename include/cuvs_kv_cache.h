@@ -14,7 +14,7 @@
  * head i / (n_query_heads / n_heads).  Scores, softmax and sums are held in 32 bits; outputs are rounded once.  Where nothing may be
  * attended to, the output row is 0 and its lse -inf.  Weights below 2^-100 of the largest may count as 0, in attention over f16 those
  * below 2^-38 (times an infinite value that is no number).  The calls only enqueue work on the handle's stream and can be captured.
- * Results do not depend on anything but the arguments and the GPU's number of SMs.
+ * Results do not depend on anything but the arguments, the GPU's number of SMs and the clusters of thread blocks that it holds at once.
  */
 #ifndef CUVS_B200_KV_CACHE_H_
 #define CUVS_B200_KV_CACHE_H_
