@@ -107,6 +107,18 @@ resources::~resources()
   }
 }
 
+namespace {
+// While it lives, this thread may allocate although a stream is being captured, by itself or by another thread: the work that what it allocates
+// is for is not captured.
+struct capture_elsewhere {
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  capture_elsewhere() { CUDA_TRY(cudaThreadExchangeStreamCaptureMode(&mode)); }
+  ~capture_elsewhere() { cudaThreadExchangeStreamCaptureMode(&mode); }
+  capture_elsewhere(const capture_elsewhere&)            = delete;
+  capture_elsewhere& operator=(const capture_elsewhere&) = delete;
+};
+}  // namespace
+
 std::unique_lock<std::mutex> resources::stream_workspace(cudaStream_t on, size_t bytes, char** at)
 {
   unsigned long long id = 0;
@@ -117,8 +129,11 @@ std::unique_lock<std::mutex> resources::stream_workspace(cudaStream_t on, size_t
     stream_ws.clear();
   }
   workspace& w = stream_ws[id];
-  if (w.capacity() != 0 && bytes > w.capacity()) { CUDA_TRY(cudaStreamSynchronize(on)); }
-  w.reserve(bytes);
+  if (bytes > w.capacity()) {
+    capture_elsewhere scope;
+    if (w.capacity() != 0) { CUDA_TRY(cudaStreamSynchronize(on)); }
+    w.reserve(bytes);
+  }
   *at = w.base();
   return held;
 }

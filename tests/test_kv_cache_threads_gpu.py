@@ -207,3 +207,41 @@ def test_a_workspace_that_grows_behind_queued_work():
         resources.sync()
         for a, w in zip(got, [want[0]] * 3 + [want[1], want[0]]):
             assert torch.equal(a[0], w[0]) and torch.equal(a[1], w[1])
+
+
+@pytest.mark.parametrize("elsewhere", [False, True])
+def test_calls_on_other_streams_while_a_graph_is_captured(elsewhere):
+    """A call that is not captured may need a workspace of its stream just then: neither it nor the capture fails, whether the capturing
+    thread makes it or another one."""
+    from cuvs_b200 import Resources, kv_cache
+    g = generator(6)
+    small, large = shared([30_000], g), shared([60_000, 50_000, 40_000], g, heads=4, n_heads=16, dim=128)
+    want = [kv_cache.attention(c[0], c[1], c[2][0], c[3], c[4]) for c in (small, large)]
+    places = [(torch.empty_like(w[0]), torch.empty_like(w[1])) for w in want]
+    resources, side, raised = Resources(), torch.cuda.Stream(), []
+    torch.cuda.synchronize()
+
+    def calls():
+        try:
+            with torch.cuda.stream(side):
+                for c, (out, lse) in zip((small, large), places):        # the second one wants more
+                    kv_cache.attention(c[0], c[1], c[2][0], c[3], c[4], out=out, lse=lse, resources=resources, sync=False)
+        except Exception as e:
+            raised.append(repr(e))
+
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        first = kv_cache.attention(small[0], small[1], small[2][0], small[3], small[4], sync=False)
+        if elsewhere:
+            thread = threading.Thread(target=calls)
+            thread.start()
+            thread.join()
+        else:
+            calls()
+        second = kv_cache.attention(large[0], large[1], large[2][0], large[3], large[4], sync=False)
+    assert not raised, raised
+    graph.replay()
+    torch.cuda.synchronize()
+    for got in (places, (first, second)):
+        for a, w in zip(got, want):
+            assert torch.equal(a[0], w[0]) and torch.equal(a[1], w[1])
