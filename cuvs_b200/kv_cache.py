@@ -29,6 +29,7 @@ from __future__ import annotations
 
 import ctypes as C
 import functools
+import operator
 import struct
 
 import torch
@@ -84,6 +85,15 @@ def _handle(tensor, resources):
             with torch.cuda.device(device):
                 resources = default_resources(device)
     return resources, resources.stream_at_call(device)
+
+
+def _window(window):
+    """The window as a number of 64 bits; 0: none.  Positions are below 2^31."""
+    if window is None:
+        return 0
+    if window <= 0:
+        raise ValueError("window must be positive, or None")
+    return min(operator.index(window), 1 << 31)
 
 
 def _on(stream, tensor):
@@ -195,8 +205,7 @@ def attention(keys, values, queries, pages, lengths, scale=None, window=None, fi
 
     ``workspace``: uint8 tensor of at least ``attention_workspace(...)`` bytes that nothing else uses until the work is done; by default
     the handle's own for the stream, and one allocated for the call while it is captured."""
-    if window is not None and window <= 0:
-        raise ValueError("window must be positive, or None")
+    window = _window(window)
     resources, stream = _handle(keys, resources)
     if queries.dim() != 3:
         raise ValueError(f"queries: 3 dimensions, not {queries.dim()}")
@@ -205,7 +214,8 @@ def attention(keys, values, queries, pages, lengths, scale=None, window=None, fi
         out = _rows_like(queries, resources, stream)
     if lse is None:
         lse = _empty(torch.float32, keys, resources, stream, n, n_heads)
-    scale, window = dim ** -0.5 if scale is None else scale, window or 0
+    if scale is None:
+        scale = dim ** -0.5
     if not _call(resources, stream, _ATTENTION, (keys, values, queries, pages, lengths, filter, out, lse, workspace, None, None), window, scale,
                  sync):
         # what is replayed needs a workspace to itself; else the handle has one for the stream
@@ -217,12 +227,12 @@ def attention(keys, values, queries, pages, lengths, scale=None, window=None, fi
 
 def attention_workspace(keys, queries, pages, window=None, resources: Resources | None = None):
     """Bytes of workspace that :func:`attention` needs for tensors of these shapes."""
-    return _attention_workspace(_handle(keys, resources)[0], keys, queries, pages, window)
+    return _attention_workspace(_handle(keys, resources)[0], keys, queries, pages, _window(window or None))
 
 
 def _attention_workspace(resources, keys, queries, pages, window):
     size = C.c_size_t()
-    L.check(_workspace(resources.handle, *_words((keys, queries, pages), (window or 0,)), size))
+    L.check(_workspace(resources.handle, *_words((keys, queries, pages), (window,)), size))
     return size.value
 
 
