@@ -5,7 +5,7 @@
 // What bounds it: the rows are read once, 4 operations for each 16-bit key and value and query head, so with 8 query heads to a key head HBM
 // at 6.5 TB/s asks for 52 TFLOP/s: more than the FP32 pipes have left beside the conversions, a fraction of what mma.sync has, which
 // takes its operands from registers without tensor memory's detour.  Everything here serves keeping loads in flight.  32 requests of up to 16,384
-// tokens, 8 key heads of 8, 128 columns bf16: 148 us for 894 MB (6.05 TB/s); one of 250,000 tokens, 4 key heads of 7: 88 us for 512 MB.
+// tokens, 8 key heads of 8, 128 columns bf16: 149 us with the join for 894 MB (6.0 TB/s); one of 250,000 tokens, 4 key heads of 7: 90 us for 512 MB.
 #include "kv_attention.hpp"
 
 #include <algorithm>

@@ -4,8 +4,8 @@
 // What bounds it: HBM, through the bytes in flight: rows of a few hundred bytes that lie anywhere.  Every warp copies its rows into its own
 // part of shared memory a stage ahead; a group of lanes -- as many as a row has 16-byte pieces -- then reads them as registers and carries a
 // softmax of its own (running top, sum of weights, weighted sum of values), joined at the end.  64 tokens x 32 heads x 1,000 candidates of 128
-// bf16: 163 us, 5.8 TB/s of what random rows bring from DRAM (loaded into registers four rows at a time: 187); 32-bit rows of one head, 64
-// columns, with a window and a filter: 26 us for 116 MB, bound by instructions (loaded into registers: 45).
+// bf16: 163-166 us for the 0.99 GB that random rows bring from DRAM (6.0 TB/s; loaded into registers four rows at a time: 187); 32-bit rows of
+// one head, 64 columns, with a window and a filter: 26 us with the join for 116 MB, bound by instructions (loaded into registers: 45).
 #include "kv_attention.hpp"
 
 #include <algorithm>
@@ -353,8 +353,10 @@ uint32_t room_of(uint32_t pieces)
 plan attention_plan(const resources& res, elem type, uint64_t sequences, uint32_t n_heads, uint32_t group, uint32_t dim, uint64_t capacity,
                     int64_t window)
 {
-  // The cost of a unit is what the end of one piece and the start of the next take a block, 2.5 us for eight heads, against the 0.35 us of a chunk:
-  // with shares of equal chunks those with many short units were done last (16 requests of up to 2,000 tokens, 128 units: 32 us, 16 with it).
+  // The cost of a unit is what the end of one piece and the start of the next take a block: 2.5 us for eight heads of 16 bits, against the 0.35 us of
+  // a chunk.  With shares of equal chunks those with many short units were done last (16 requests of up to 2,000 tokens, 128 units: 32 us, 16
+  // with it).  32-bit rows of one to eight heads: 0, 4, 8, 16 chunks are 55, 44, 42, 42 us for one head (64 requests of up to 1,000 tokens, 8 key
+  // heads), 79, 55, 46, 48 for four, 47, 35, 30, 30 for eight (2 key heads).
   // A window may begin anywhere in 16 positions.
   const uint64_t most = window > 0 && uint64_t(window) < capacity ? std::min(capacity, uint64_t(window) + 15) : capacity;
   plan p{};
