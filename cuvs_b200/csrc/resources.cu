@@ -53,6 +53,16 @@ void ensure_dynamic_smem(const void* kernel, size_t bytes)
 }
 
 namespace {
+// While it lives, this thread may allocate although a stream is being captured, by itself or by another thread: the work that what it allocates
+// is for is not captured.
+struct capture_elsewhere {
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  capture_elsewhere() { CUDA_TRY(cudaThreadExchangeStreamCaptureMode(&mode)); }
+  ~capture_elsewhere() { cudaThreadExchangeStreamCaptureMode(&mode); }
+  capture_elsewhere(const capture_elsewhere&)            = delete;
+  capture_elsewhere& operator=(const capture_elsewhere&) = delete;
+};
+
 // A kernel whose block has an SM's shared memory to itself; it is only asked about, not launched.
 __global__ void whole_sm_kernel() {}
 
@@ -80,6 +90,7 @@ void ask_for_clusters(uint32_t (&at_once)[4], size_t whole_sm)
 
 resources::resources()
 {
+  capture_elsewhere scope;  // the first call on a device may be one that is captured
   CUDA_TRY(cudaGetDevice(&device));
   cudaDeviceProp prop{};
   CUDA_TRY(cudaGetDeviceProperties(&prop, device));
@@ -106,18 +117,6 @@ resources::~resources()
     cudaFreeHost(pinned);
   }
 }
-
-namespace {
-// While it lives, this thread may allocate although a stream is being captured, by itself or by another thread: the work that what it allocates
-// is for is not captured.
-struct capture_elsewhere {
-  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
-  capture_elsewhere() { CUDA_TRY(cudaThreadExchangeStreamCaptureMode(&mode)); }
-  ~capture_elsewhere() { cudaThreadExchangeStreamCaptureMode(&mode); }
-  capture_elsewhere(const capture_elsewhere&)            = delete;
-  capture_elsewhere& operator=(const capture_elsewhere&) = delete;
-};
-}  // namespace
 
 std::unique_lock<std::mutex> resources::stream_workspace(cudaStream_t on, size_t bytes, char** at)
 {

@@ -13,7 +13,7 @@ U = 2.0 ** -24
 
 
 def blocks():
-    """INTEGRATION.md's two: the prompts and their indexes, a step.  And the step of the module's own text."""
+    """The guide's two: the prompts and their indexes, a step.  And the step of the module's own text."""
     from cuvs_b200 import kv_cache
     with open(os.path.join(ROOT, "INTEGRATION.md")) as f:
         text = f.read()

@@ -245,3 +245,38 @@ def test_calls_on_other_streams_while_a_graph_is_captured(elsewhere):
     for got in (places, (first, second)):
         for a, w in zip(got, want):
             assert torch.equal(a[0], w[0]) and torch.equal(a[1], w[1])
+
+
+FIRST = """
+import torch
+from cuvs_b200 import kv_cache
+k, v = (torch.randn((4000, 16, 2, 64), device="cuda").bfloat16() for _ in range(2))
+q, new = torch.randn((1, 8, 64), device="cuda").bfloat16(), torch.randn((1, 2, 64), device="cuda").bfloat16()
+pages = torch.arange(4000, dtype=torch.int32, device="cuda")[None]
+n, place = (torch.tensor([x], dtype=torch.int32, device="cuda") for x in (60_000, 61_000))
+slots = torch.arange(1000, device="cuda").expand(1, 8, 1000).contiguous()
+torch.cuda.synchronize()
+
+def step():
+    at, _ = kv_cache.append(k, v, new, new, pages, place, sync=False)
+    near = kv_cache.attention(k, v, q, pages, n, sync=False)
+    far = kv_cache.attend_candidates(k, v, q, slots, sync=False)
+    return (at, *kv_cache.merge_parts(torch.stack((near[0], far[0])), torch.stack((near[1], far[1])), sync=False))
+
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = step()
+graph.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(got, step()))
+print("ok")
+"""
+
+
+def test_the_first_call_of_a_process_may_be_captured():
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, "-c", FIRST], cwd=root, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and done.stdout == "ok\n", done.stdout + done.stderr
