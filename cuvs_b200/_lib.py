@@ -200,6 +200,15 @@ SIGNATURES = {
     "cuvsB200KvCacheArrays": [C.c_size_t, C.c_void_p, C.c_int, C.c_void_p, C.c_int64, C.c_bool],
     "cuvsB200SetTensorExchange": [C.c_void_p, C.c_void_p],
     "cuvsB200KvCacheTensors": [C.c_size_t, C.c_void_p, C.c_int, *[C.py_object] * 11, C.c_int64, C.c_float, C.c_bool],
+    "cuvsKvCacheAppendTurned": [C.c_size_t, *[_P(DLManagedTensor)] * 9, C.c_bool, *[_P(DLManagedTensor)] * 4],
+    "cuvsKvCacheDraftTree": [C.c_size_t, *[_P(DLManagedTensor)] * 4],
+    "cuvsKvCacheAttendTree": [C.c_size_t, *[_P(DLManagedTensor)] * 7, C.c_float, C.c_int64, C.c_float, _P(DLManagedTensor), FilterStruct,
+                              *[_P(DLManagedTensor)] * 3],
+    "cuvsKvCacheAttendTreeWorkspace": [C.c_size_t, *[_P(DLManagedTensor)] * 3, C.c_int64, _P(C.c_size_t)],
+    "cuvsKvCacheKeepPath": [C.c_size_t, *[_P(DLManagedTensor)] * 6],
+    "cuvsKvCacheCopyPages": [C.c_size_t, *[_P(DLManagedTensor)] * 4],
+    "cuvsB200KvCacheMoreTensors": [C.c_size_t, C.c_void_p, C.c_int, *[C.py_object] * 13, C.c_int64, C.c_float, C.c_float, C.c_bool],
+    "cuvsB200KvCacheTreeWorkspaceArrays": [C.c_size_t, C.c_void_p, C.c_int64, _P(C.c_size_t)],
     "cuvsB200KvCacheWait": [C.c_size_t, C.c_void_p],
     "cuvsB200KvCacheWorkspaceArrays": [C.c_size_t, C.c_void_p, C.c_int64, _P(C.c_size_t)],
     "cuvsB200KvCacheCheck": [C.c_int, C.c_int, C.c_void_p, C.c_int64],

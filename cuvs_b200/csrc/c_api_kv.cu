@@ -246,9 +246,34 @@ void pages_of(int device, tensor& t, uint32_t& n_sequences, uint32_t& width, int
   stride      = t.stride[0];
 }
 
-kv::append_args append_of(int device, tensor* t, bool interleaved)
+void workspace_given(int device, tensor& t, char*& at, size_t& bytes)
 {
-  enum { KEYS, VALUES, NEW_KEYS, NEW_VALUES, PAGES, POSITIONS, SEQUENCES, QUERIES, FREQUENCIES, SLOTS, ROTATED };
+  check_place(device, t, 1, "workspace");
+  check_type(t, kDLUInt, 8, "workspace");
+  CUVS_EXPECTS(t.shape[0] <= 1 || t.stride[0] == 1, "workspace: must be contiguous");
+  CUVS_EXPECTS(reinterpret_cast<uintptr_t>(t.data) % 16 == 0, "workspace: must start on a 16-byte boundary");
+  at    = t.data;
+  bytes = size_t(t.shape[0]);
+}
+
+// The workspace that the caller gave, or the handle's own for the stream (`held` while the work is enqueued).  False: the stream is being
+// captured, and the call needs one to itself.
+bool workspace_for(resources& res, cudaStream_t stream, size_t need, char*& at, size_t bytes, std::unique_lock<std::mutex>& held)
+{
+  if (need > 0 && at != nullptr) {
+    CUVS_EXPECTS(bytes >= need, "workspace: %zu bytes, but %zu are needed", bytes, need);
+  } else if (need > 0) {
+    cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+    CUDA_TRY(cudaStreamIsCapturing(stream, &capturing));
+    if (capturing != cudaStreamCaptureStatusNone) { return false; }
+    held = res.stream_workspace(stream, need, &at);
+  }
+  return true;
+}
+
+kv::append_args append_of(int device, tensor* t, bool interleaved, bool turned)
+{
+  enum { KEYS, VALUES, NEW_KEYS, NEW_VALUES, PAGES, POSITIONS, SEQUENCES, QUERIES, FREQUENCIES, SLOTS, ROTATED, TURNS, AXES };
   kv::append_args a{};
   a.cache = cache_of(device, t[KEYS], t[VALUES], {}, a.type);
   check_distinct(t[KEYS], "keys");
@@ -297,6 +322,188 @@ kv::append_args append_of(int device, tensor* t, bool interleaved)
   check_type(t[SLOTS], kDLInt, 64, "slots");
   CUVS_EXPECTS(t[SLOTS].shape[0] == n && (n <= 1 || t[SLOTS].stride[0] == 1), "slots: a contiguous one for each token");
   a.slots = reinterpret_cast<int64_t*>(t[SLOTS].data);
+  if (!turned) { return a; }
+  tensor& by = t[TURNS];
+  CUVS_EXPECTS(by.given(), "turns: null tensor");
+  CUVS_EXPECTS(a.frequencies != nullptr, "turns go with frequencies");
+  if (by.ndim == 1) {  // one axis
+    by.ndim      = 2;
+    by.shape[1]  = 1;
+    by.stride[1] = 0;
+  }
+  check_place(device, by, 2, "turns");
+  check_type(by, kDLInt, 32, "turns");
+  CUVS_EXPECTS(by.shape[0] == n, "turns: one row for each token");
+  CUVS_EXPECTS(by.shape[1] >= 1 && by.shape[1] < 65536, "turns: 1 to 65535 axes, not %lld", (long long)by.shape[1]);
+  CUVS_EXPECTS(by.shape[1] == 1 || by.stride[1] == 1, "turns: the positions of a token must be contiguous");
+  a.turns        = reinterpret_cast<const int32_t*>(by.data);
+  a.turns_stride = by.stride[0];
+  a.n_axes       = uint32_t(by.shape[1]);
+  if (t[AXES].given()) {
+    a.axes = ints_of(device, t[AXES], "axes", a.n_pairs, "pair of columns");
+  } else {
+    CUVS_EXPECTS(a.n_axes == 1, "axes: null tensor, but turns by %u axes", a.n_axes);
+  }
+  return a;
+}
+
+// Rows of one step's drafted tokens, [n_sequences, n_drafted, n_heads, dim]
+kv::drafted_rows_view drafted_rows_of(int device, tensor& t, kv::elem type, const kv::cache_view& c, const char* name)
+{
+  check_rows(device, t, 4, type, name);
+  CUVS_EXPECTS(t.shape[3] == int64_t(c.dim), "%s: rows of %u elements, not %lld", name, c.dim, (long long)t.shape[3]);
+  return {t.data, t.stride[0], t.stride[1], t.stride[2]};
+}
+
+constexpr int64_t kMostDrafted = 1024;
+
+void check_drafted(int64_t n)
+{
+  CUVS_EXPECTS(n >= 1 && n <= kMostDrafted, "1 to %lld drafted tokens of a sequence, not %lld", (long long)kMostDrafted, (long long)n);
+}
+
+// [n, m] integers of the drafted tokens (or of paths), those of a sequence contiguous; sequences may share them (stride 0)
+const int32_t* per_sequence(int device, tensor& t, const char* name, int64_t n, int64_t m, int64_t& stride)
+{
+  check_place(device, t, 2, name);
+  check_type(t, kDLInt, 32, name);
+  CUVS_EXPECTS(t.shape[0] == n && (m < 0 || t.shape[1] == m), "%s: expected shape [%lld, %lld]", name, (long long)n,
+               (long long)(m < 0 ? t.shape[1] : m));
+  CUVS_EXPECTS(t.shape[1] <= 1 || t.stride[1] == 1, "%s: those of a sequence must be contiguous", name);
+  stride = t.stride[0];
+  return reinterpret_cast<const int32_t*>(t.data);
+}
+
+kv::draft_tree_args draft_tree_of(int device, tensor* t)
+{
+  enum { PARENTS, LENGTHS, MASK, POSITIONS };
+  kv::draft_tree_args a{};
+  CUVS_EXPECTS(t[PARENTS].given(), "parents: null tensor");
+  const int64_t n = t[PARENTS].shape[0], m = t[PARENTS].shape[1];
+  a.parents       = per_sequence(device, t[PARENTS], "parents", n, -1, a.parents_stride);
+  check_drafted(m);
+  CUVS_EXPECTS(n < (int64_t(1) << 31), "parents: too many sequences");
+  a.lengths       = ints_of(device, t[LENGTHS], "lengths", n, "sequence");
+  const int64_t w = (m + 31) / 32;
+  tensor& mask    = t[MASK];
+  check_place(device, mask, 3, "mask");
+  check_type(mask, kDLUInt, 32, "mask");
+  CUVS_EXPECTS(mask.shape[0] == n && mask.shape[1] == m && mask.shape[2] == w, "mask: expected shape [%lld, %lld, %lld]", (long long)n,
+               (long long)m, (long long)w);
+  CUVS_EXPECTS((w <= 1 || mask.stride[2] == 1) && (m <= 1 || mask.stride[1] == w) && (n <= 1 || mask.stride[0] == m * w), "mask: must be contiguous");
+  int64_t stride;
+  a.positions = const_cast<int32_t*>(per_sequence(device, t[POSITIONS], "positions", n, m, stride));
+  CUVS_EXPECTS(n <= 1 || stride == m, "positions: must be contiguous");
+  a.mask        = reinterpret_cast<uint32_t*>(mask.data);
+  a.n_sequences = uint32_t(n);
+  a.n_drafted   = uint32_t(m);
+  return a;
+}
+
+kv::attend_tree_args attend_tree_of(int device, tensor* t, float scale, int64_t window, float cap)
+{
+  enum { KEYS, VALUES, QUERIES, PAGES, LENGTHS, POSITIONS, MASK, SLOPES, FILTER, OUT, LSE, WORKSPACE };
+  kv::attend_tree_args a{};
+  a.cache   = cache_of(device, t[KEYS], t[VALUES], t[FILTER], a.type);
+  a.queries = drafted_rows_of(device, t[QUERIES], a.type, a.cache, "queries");
+  const int64_t n = t[QUERIES].shape[0], m = t[QUERIES].shape[1], h = t[QUERIES].shape[2];
+  check_drafted(m);
+  CUVS_EXPECTS(h >= 1 && h % a.cache.n_heads == 0 && h < 65536, "queries: their %lld heads are no multiple of the cache's %u", (long long)h,
+               a.cache.n_heads);
+  CUVS_EXPECTS(n < (int64_t(1) << 31) && n * m * h < (int64_t(1) << 31), "queries: too many rows");
+  a.n_sequences   = uint32_t(n);
+  a.n_drafted     = uint32_t(m);
+  a.n_query_heads = uint32_t(h);
+  uint32_t rows;
+  pages_of(device, t[PAGES], rows, a.table_width, a.table_stride);
+  CUVS_EXPECTS(int64_t(rows) == n, "pages: a row for each of the %lld sequences, not %u", (long long)n, rows);
+  a.pages     = reinterpret_cast<const int32_t*>(t[PAGES].data);
+  a.lengths   = ints_of(device, t[LENGTHS], "lengths", n, "sequence");
+  a.positions = per_sequence(device, t[POSITIONS], "positions", n, m, a.positions_stride);
+  tensor& mask = t[MASK];
+  check_place(device, mask, 3, "mask");
+  check_type(mask, kDLUInt, 32, "mask");
+  CUVS_EXPECTS(mask.shape[0] == n && mask.shape[1] == m && mask.shape[2] >= (m + 31) / 32,
+               "mask: expected shape [%lld, %lld, %lld]", (long long)n, (long long)m, (long long)((m + 31) / 32));
+  CUVS_EXPECTS(mask.shape[2] <= 1 || mask.stride[2] == 1, "mask: the words of a token must be contiguous");
+  a.mask          = reinterpret_cast<const uint32_t*>(mask.data);
+  a.mask_sequence = mask.stride[0];
+  a.mask_token    = mask.stride[1];
+  if (t[SLOPES].given()) {
+    check_place(device, t[SLOPES], 1, "slopes");
+    check_type(t[SLOPES], kDLFloat, 32, "slopes");
+    CUVS_EXPECTS(t[SLOPES].shape[0] == h && (h <= 1 || t[SLOPES].stride[0] == 1), "slopes: a contiguous one for each of the %lld query heads",
+                 (long long)h);
+    a.slopes = reinterpret_cast<const float*>(t[SLOPES].data);
+  }
+  CUVS_EXPECTS(std::isfinite(scale), "scale must be finite");
+  CUVS_EXPECTS(cap == 0.0f || (cap >= 0.99e-30f && cap <= 1.01e30f), "cap must be 0 (none) or between 1e-30 and 1e30");
+  CUVS_EXPECTS(window >= 0, "window must not be negative");
+  a.scale  = scale;
+  a.cap    = cap;
+  a.window = window;
+  a.out    = drafted_rows_of(device, t[OUT], a.type, a.cache, "out");
+  CUVS_EXPECTS(std::equal(t[OUT].shape, t[OUT].shape + 4, t[QUERIES].shape), "out: the shape of the queries");
+  check_distinct(t[OUT], "out");
+  tensor& l = t[LSE];
+  check_place(device, l, 3, "lse");
+  check_type(l, kDLFloat, 32, "lse");
+  CUVS_EXPECTS(std::equal(l.shape, l.shape + 3, t[QUERIES].shape), "lse: expected shape [%lld, %lld, %lld]", (long long)n, (long long)m, (long long)h);
+  CUVS_EXPECTS((h <= 1 || l.stride[2] == 1) && (m <= 1 || l.stride[1] == h) && (n <= 1 || l.stride[0] == m * h), "lse: must be contiguous");
+  a.lse = reinterpret_cast<float*>(l.data);
+  if (t[WORKSPACE].given()) { workspace_given(device, t[WORKSPACE], a.workspace, a.workspace_bytes); }
+  return a;
+}
+
+bool attend_tree_call(resources& res, cudaStream_t stream, kv::attend_tree_args a)
+{
+  const size_t need = kv::attend_tree_workspace(res, a.type, a.n_sequences, a.n_drafted, a.n_query_heads, a.cache.n_heads, a.cache.dim,
+                                                uint64_t(a.table_width) * a.cache.page.size, a.window);
+  std::unique_lock<std::mutex> held;
+  if (!workspace_for(res, stream, need, a.workspace, a.workspace_bytes, held)) { return false; }
+  kv::attend_tree(res, stream, a);
+  return true;
+}
+
+kv::keep_path_args keep_path_of(int device, tensor* t)
+{
+  enum { KEYS, VALUES, PAGES, LENGTHS, PATHS, KEPT };
+  kv::keep_path_args a{};
+  kv::elem type;
+  a.cache = cache_of(device, t[KEYS], t[VALUES], {}, type);
+  check_distinct(t[KEYS], "keys");
+  check_distinct(t[VALUES], "values");
+  a.row_bytes = a.cache.dim * uint32_t(t[KEYS].bits / 8);
+  pages_of(device, t[PAGES], a.n_sequences, a.table_width, a.table_stride);
+  a.pages   = reinterpret_cast<const int32_t*>(t[PAGES].data);
+  a.lengths = ints_of(device, t[LENGTHS], "lengths", a.n_sequences, "sequence");
+  a.paths   = per_sequence(device, t[PATHS], "paths", a.n_sequences, -1, a.paths_stride);
+  CUVS_EXPECTS(t[PATHS].shape[1] <= kMostDrafted, "paths: at most %lld entries, not %lld", (long long)kMostDrafted, (long long)t[PATHS].shape[1]);
+  a.n_entries = uint32_t(t[PATHS].shape[1]);
+  a.kept      = const_cast<int32_t*>(ints_of(device, t[KEPT], "kept", a.n_sequences, "sequence"));
+  // blocks of a sequence read its length while one of them writes the new one
+  const int64_t n = a.n_sequences;
+  CUVS_EXPECTS(n == 0 || a.kept + n <= a.lengths || a.lengths + n <= a.kept, "kept: must not be the lengths' own memory");
+  CUVS_EXPECTS(uint64_t(n) * 2 * a.cache.n_heads * (a.row_bytes / 16) < (uint64_t(1) << 37), "pages: too many sequences");
+  return a;
+}
+
+kv::copy_pages_args copy_pages_of(int device, tensor* t)
+{
+  enum { KEYS, VALUES, SOURCES, TARGETS };
+  kv::copy_pages_args a{};
+  kv::elem type;
+  a.cache = cache_of(device, t[KEYS], t[VALUES], {}, type);
+  check_distinct(t[KEYS], "keys");
+  check_distinct(t[VALUES], "values");
+  a.row_bytes = a.cache.dim * uint32_t(t[KEYS].bits / 8);
+  a.sources   = ints_of(device, t[SOURCES], "sources", -1, "");
+  const int64_t n = t[SOURCES].shape[0];
+  a.targets   = ints_of(device, t[TARGETS], "targets", n, "source");
+  // pieces of 16 bytes are counted in 31 bits, blocks in 31
+  CUVS_EXPECTS(2 * uint64_t(a.cache.n_heads) * a.cache.page.size * (a.row_bytes / 16) < (uint64_t(1) << 31), "keys: pages too large to be copied");
+  CUVS_EXPECTS(n < (int64_t(1) << 31), "sources: too many");
+  a.n_pairs = uint32_t(n);
   return a;
 }
 
@@ -319,32 +526,16 @@ kv::attention_args attention_of(int device, tensor* t, float scale, int64_t wind
   a.out    = rows_of(device, t[OUT], a.type, a.cache, n, a.n_query_heads, "out");
   check_distinct(t[OUT], "out");
   a.lse = lse_of(device, t[LSE], n, a.n_query_heads);
-  if (t[WORKSPACE].given()) {
-    check_place(device, t[WORKSPACE], 1, "workspace");
-    check_type(t[WORKSPACE], kDLUInt, 8, "workspace");
-    CUVS_EXPECTS(t[WORKSPACE].shape[0] <= 1 || t[WORKSPACE].stride[0] == 1, "workspace: must be contiguous");
-    CUVS_EXPECTS(reinterpret_cast<uintptr_t>(t[WORKSPACE].data) % 16 == 0, "workspace: must start on a 16-byte boundary");
-    a.workspace       = t[WORKSPACE].data;
-    a.workspace_bytes = size_t(t[WORKSPACE].shape[0]);
-  }
+  if (t[WORKSPACE].given()) { workspace_given(device, t[WORKSPACE], a.workspace, a.workspace_bytes); }
   return a;
 }
 
-// With the workspace that the caller gave, or the handle's own for the stream.  False: the stream is being captured, and the call needs one
-// to itself.
 bool attention_call(resources& res, cudaStream_t stream, kv::attention_args a)
 {
   const size_t need = kv::attention_workspace(res, a.type, a.n_sequences, a.n_query_heads, a.cache.n_heads, a.cache.dim,
                                               uint64_t(a.table_width) * a.cache.page.size, a.window);
   std::unique_lock<std::mutex> held;
-  if (need > 0 && a.workspace != nullptr) {
-    CUVS_EXPECTS(a.workspace_bytes >= need, "workspace: %zu bytes, but %zu are needed", a.workspace_bytes, need);
-  } else if (need > 0) {
-    cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
-    CUDA_TRY(cudaStreamIsCapturing(stream, &capturing));
-    if (capturing != cudaStreamCaptureStatusNone) { return false; }
-    held = res.stream_workspace(stream, need, &a.workspace);
-  }
+  if (!workspace_for(res, stream, need, a.workspace, a.workspace_bytes, held)) { return false; }
   kv::attention(res, stream, a);
   return true;
 }
@@ -425,6 +616,25 @@ void workspace_of(resources& res, tensor* t, int64_t window, size_t* bytes)
   *bytes = kv::attention_workspace(res, type, n, query_heads_of(t[QUERIES], c), c.n_heads, c.dim, uint64_t(width) * c.page.size, window);
 }
 
+void tree_workspace_of(resources& res, tensor* t, int64_t window, size_t* bytes)
+{
+  enum { KEYS, QUERIES, PAGES };
+  CUVS_EXPECTS(bytes != nullptr, "null output pointer");
+  kv::elem type;
+  tensor values          = t[KEYS];
+  const kv::cache_view c = cache_of(res.device, t[KEYS], values, {}, type);
+  drafted_rows_of(res.device, t[QUERIES], type, c, "queries");
+  const int64_t n = t[QUERIES].shape[0], m = t[QUERIES].shape[1], h = t[QUERIES].shape[2];
+  check_drafted(m);
+  CUVS_EXPECTS(h >= 1 && h % c.n_heads == 0 && h < 65536 && n < (int64_t(1) << 31) && n * m * h < (int64_t(1) << 31),
+               "queries: too many rows, or heads that are no multiple of the cache's");
+  uint32_t rows, width;
+  int64_t stride;
+  pages_of(res.device, t[PAGES], rows, width, stride);
+  CUVS_EXPECTS(window >= 0, "window must not be negative");
+  *bytes = kv::attend_tree_workspace(res, type, uint32_t(n), uint32_t(m), uint32_t(h), c.n_heads, c.dim, uint64_t(width) * c.page.size, window);
+}
+
 resources& single_device(cuvsResources_t res)
 {
   resources* r = res_of(res);
@@ -446,7 +656,7 @@ extern "C" cuvsError_t cuvsKvCacheAppend(cuvsResources_t res, DLManagedTensor* k
                   describe(new_values, "new_values"), describe(pages, "pages"),       describe(positions, "positions"),
                   describe(sequences, "sequences"), describe(queries, "queries"),     describe(frequencies, "frequencies"),
                   describe(slots, "slots"),         describe(rotated, "rotated")};
-    kv::append(r, r.stream, append_of(r.device, t, interleaved));
+    kv::append(r, r.stream, append_of(r.device, t, interleaved, false));
   });
 }
 
@@ -497,34 +707,130 @@ extern "C" cuvsError_t cuvsKvCacheMergeParts(cuvsResources_t res, DLManagedTenso
   });
 }
 
+extern "C" cuvsError_t cuvsKvCacheAppendTurned(cuvsResources_t res, DLManagedTensor* keys, DLManagedTensor* values, DLManagedTensor* new_keys,
+                                               DLManagedTensor* new_values, DLManagedTensor* pages, DLManagedTensor* positions,
+                                               DLManagedTensor* sequences, DLManagedTensor* queries, DLManagedTensor* frequencies,
+                                               bool interleaved, DLManagedTensor* slots, DLManagedTensor* rotated, DLManagedTensor* turns,
+                                               DLManagedTensor* axes)
+{
+  return translate_exceptions([=] {
+    resources& r = single_device(res);
+    device_scope on(r.device);
+    tensor t[] = {describe(keys, "keys"),           describe(values, "values"),       describe(new_keys, "new_keys"),
+                  describe(new_values, "new_values"), describe(pages, "pages"),       describe(positions, "positions"),
+                  describe(sequences, "sequences"), describe(queries, "queries"),     describe(frequencies, "frequencies"),
+                  describe(slots, "slots"),         describe(rotated, "rotated"),     describe(turns, "turns"),
+                  describe(axes, "axes")};
+    kv::append(r, r.stream, append_of(r.device, t, interleaved, true));
+  });
+}
+
+extern "C" cuvsError_t cuvsKvCacheDraftTree(cuvsResources_t res, DLManagedTensor* parents, DLManagedTensor* lengths, DLManagedTensor* mask,
+                                            DLManagedTensor* positions)
+{
+  return translate_exceptions([=] {
+    resources& r = single_device(res);
+    device_scope on(r.device);
+    tensor t[] = {describe(parents, "parents"), describe(lengths, "lengths"), describe(mask, "mask"), describe(positions, "positions")};
+    kv::draft_tree(r, r.stream, draft_tree_of(r.device, t));
+  });
+}
+
+extern "C" cuvsError_t cuvsKvCacheAttendTree(cuvsResources_t res, DLManagedTensor* keys, DLManagedTensor* values, DLManagedTensor* queries,
+                                             DLManagedTensor* pages, DLManagedTensor* lengths, DLManagedTensor* positions, DLManagedTensor* mask,
+                                             float scale, int64_t window, float cap, DLManagedTensor* slopes, cuvsFilter filter,
+                                             DLManagedTensor* out, DLManagedTensor* lse, DLManagedTensor* workspace)
+{
+  return translate_exceptions([=] {
+    resources& r = single_device(res);
+    device_scope on(r.device);
+    tensor t[] = {describe(keys, "keys"),           describe(values, "values"), describe(queries, "queries"), describe(pages, "pages"),
+                  describe(lengths, "lengths"),     describe(positions, "positions"), describe(mask, "mask"), describe(slopes, "slopes"),
+                  filter_of(filter),                describe(out, "out"),       describe(lse, "lse"),         describe(workspace, "workspace")};
+    CUVS_EXPECTS(attend_tree_call(r, r.stream, attend_tree_of(r.device, t, scale, window, cap)), kOwnWorkspace);
+  });
+}
+
+extern "C" cuvsError_t cuvsKvCacheAttendTreeWorkspace(cuvsResources_t res, DLManagedTensor* keys, DLManagedTensor* queries,
+                                                      DLManagedTensor* pages, int64_t window, size_t* bytes)
+{
+  return translate_exceptions([=] {
+    tensor t[] = {describe(keys, "keys"), describe(queries, "queries"), describe(pages, "pages")};
+    tree_workspace_of(single_device(res), t, window, bytes);
+  });
+}
+
+extern "C" cuvsError_t cuvsKvCacheKeepPath(cuvsResources_t res, DLManagedTensor* keys, DLManagedTensor* values, DLManagedTensor* pages,
+                                           DLManagedTensor* lengths, DLManagedTensor* paths, DLManagedTensor* kept)
+{
+  return translate_exceptions([=] {
+    resources& r = single_device(res);
+    device_scope on(r.device);
+    tensor t[] = {describe(keys, "keys"),       describe(values, "values"), describe(pages, "pages"),
+                  describe(lengths, "lengths"), describe(paths, "paths"),   describe(kept, "kept")};
+    kv::keep_path(r, r.stream, keep_path_of(r.device, t));
+  });
+}
+
+extern "C" cuvsError_t cuvsKvCacheCopyPages(cuvsResources_t res, DLManagedTensor* keys, DLManagedTensor* values, DLManagedTensor* sources,
+                                            DLManagedTensor* targets)
+{
+  return translate_exceptions([=] {
+    resources& r = single_device(res);
+    device_scope on(r.device);
+    tensor t[] = {describe(keys, "keys"), describe(values, "values"), describe(sources, "sources"), describe(targets, "targets")};
+    kv::copy_pages(r, r.stream, copy_pages_of(r.device, t));
+  });
+}
+
 namespace {
 
-constexpr int kMost = 11;  // tensors of a call
-const int n_tensors[]            = {11, 9, 7, 4};
-const int n_scalars[]            = {1, 2, 1, 0};
+enum { APPEND, ATTENTION, CANDIDATES, MERGE, APPEND_TURNED, DRAFT_TREE, ATTEND_TREE, KEEP_PATH, COPY_PAGES, kCalls };
+constexpr int kMost = 13;  // tensors of a call
+const int n_tensors[]            = {11, 9, 7, 4, 13, 4, 12, 6, 4};
+const int n_scalars[]            = {1, 2, 1, 0, 1, 0, 3, 0, 0};
 const char* const names[][kMost] = {
   {"keys", "values", "new_keys", "new_values", "pages", "positions", "sequences", "queries", "frequencies", "slots", "rotated"},
   {"keys", "values", "queries", "pages", "lengths", "filter", "out", "lse", "workspace"},
   {"keys", "values", "queries", "candidates", "filter", "out", "lse"},
-  {"parts", "parts_lse", "out", "lse"}};
+  {"parts", "parts_lse", "out", "lse"},
+  {"keys", "values", "new_keys", "new_values", "pages", "positions", "sequences", "queries", "frequencies", "slots", "rotated", "turns", "axes"},
+  {"parents", "lengths", "mask", "positions"},
+  {"keys", "values", "queries", "pages", "lengths", "positions", "mask", "slopes", "filter", "out", "lse", "workspace"},
+  {"keys", "values", "pages", "lengths", "paths", "kept"},
+  {"keys", "values", "sources", "targets"}};
+
+float float_of(int64_t word)
+{
+  const uint32_t bits = uint32_t(word);
+  float x;
+  std::memcpy(&x, &bits, 4);
+  return x;
+}
 
 struct call {
   tensor t[kMost];
   bool interleaved = false;
   float scale      = 0.0f;
+  float cap        = 0.0f;
   int64_t window   = 0;
   call() = default;
   call(int op, const int64_t* words, int64_t n_words)
   {
-    CUVS_EXPECTS(op >= 0 && op < 4 && words != nullptr, "unknown call %d", op);
+    CUVS_EXPECTS(op >= 0 && op < kCalls && words != nullptr, "unknown call %d", op);
     const int64_t* end = words + n_words;
     for (int i = 0; i < n_tensors[op]; i++) { t[i] = describe(words, end, names[op][i]); }
     CUVS_EXPECTS(end - words == n_scalars[op], "the words do not describe the call");
-    if (op == 0) { interleaved = words[0] != 0; }
-    if (op == 1) { window = words[0]; }
-    if (op == 1 || op == 2) {
-      const uint32_t bits = uint32_t(words[op == 1 ? 1 : 0]);
-      std::memcpy(&scale, &bits, 4);
+    switch (op) {
+      case APPEND:
+      case APPEND_TURNED: interleaved = words[0] != 0; break;
+      case ATTEND_TREE: cap = float_of(words[2]); [[fallthrough]];
+      case ATTENTION:
+        window = words[0];
+        scale  = float_of(words[1]);
+        break;
+      case CANDIDATES: scale = float_of(words[0]); break;
+      default: break;
     }
   }
   // False: it needs a workspace to itself.  The handle's stream stays what it is: another thread may be in the middle of a search that reads it.
@@ -538,12 +844,15 @@ struct call {
       CUVS_EXPECTS(capturing == cudaStreamCaptureStatusNone, "a call that is captured cannot wait for its work: pass sync=False");
     }
     switch (op) {
-      case 0: kv::append(r, stream, append_of(r.device, t, interleaved)); break;
-      case 1:
-        if (!attention_call(r, stream, attention_of(r.device, t, scale, window))) { return false; }
-        break;
-      case 2: kv::attend_candidates(r, stream, candidates_of(r.device, t, scale)); break;
-      default: kv::merge_parts(r, stream, merge_of(r.device, t));
+      case APPEND:
+      case APPEND_TURNED: kv::append(r, stream, append_of(r.device, t, interleaved, op == APPEND_TURNED)); break;
+      case ATTENTION: return attention_call(r, stream, attention_of(r.device, t, scale, window));
+      case CANDIDATES: kv::attend_candidates(r, stream, candidates_of(r.device, t, scale)); break;
+      case MERGE: kv::merge_parts(r, stream, merge_of(r.device, t)); break;
+      case DRAFT_TREE: kv::draft_tree(r, stream, draft_tree_of(r.device, t)); break;
+      case ATTEND_TREE: return attend_tree_call(r, stream, attend_tree_of(r.device, t, scale, window, cap));
+      case KEEP_PATH: kv::keep_path(r, stream, keep_path_of(r.device, t)); break;
+      default: kv::copy_pages(r, stream, copy_pages_of(r.device, t));
     }
     return true;
   }
@@ -579,10 +888,19 @@ extern "C" cuvsError_t cuvsB200SetTensorExchange(const void* table, const void* 
 extern "C" int cuvsB200KvCacheTensors(cuvsResources_t res, cudaStream_t stream, int op, void* t0, void* t1, void* t2, void* t3, void* t4, void* t5,
                                       void* t6, void* t7, void* t8, void* t9, void* t10, int64_t integer, float scale, bool sync)
 {
+  void* const none = const_cast<void*>(g_none);
+  if (op > MERGE) { op = -1; }  // those have more tensors
+  return cuvsB200KvCacheMoreTensors(res, stream, op, t0, t1, t2, t3, t4, t5, t6, t7, t8, t9, t10, none, none, integer, scale, 0.0f, sync);
+}
+
+extern "C" int cuvsB200KvCacheMoreTensors(cuvsResources_t res, cudaStream_t stream, int op, void* t0, void* t1, void* t2, void* t3, void* t4,
+                                          void* t5, void* t6, void* t7, void* t8, void* t9, void* t10, void* t11, void* t12, int64_t integer,
+                                          float scale, float cap, bool sync)
+{
   int status = CUVS_ERROR;
   const auto raised = translate_exceptions([&] {
-    CUVS_EXPECTS(g_exchange != nullptr && op >= 0 && op < 4, "unknown call %d", op);
-    void* const objects[kMost] = {t0, t1, t2, t3, t4, t5, t6, t7, t8, t9, t10};
+    CUVS_EXPECTS(g_exchange != nullptr && op >= 0 && op < kCalls, "unknown call %d", op);
+    void* const objects[kMost] = {t0, t1, t2, t3, t4, t5, t6, t7, t8, t9, t10, t11, t12};
     call c;
     for (int i = 0; i < n_tensors[op]; i++) {
       if (objects[i] == g_none) { continue; }
@@ -593,6 +911,7 @@ extern "C" int cuvsB200KvCacheTensors(cuvsResources_t res, cudaStream_t stream, 
     c.interleaved = integer != 0;
     c.window      = integer;
     c.scale       = scale;
+    c.cap         = cap;
     status        = c.run(res, stream, op, sync) ? CUVS_SUCCESS : kNeedsWorkspace;
   });
   return raised == CUVS_SUCCESS ? status : CUVS_ERROR;
@@ -606,17 +925,30 @@ extern "C" cuvsError_t cuvsB200KvCacheWait(cuvsResources_t res, cudaStream_t str
   });
 }
 
+namespace {
+
+void workspace_by_words(cuvsResources_t res, const int64_t* words, int64_t n_words, size_t* bytes,
+                        void (*of)(resources&, tensor*, int64_t, size_t*))
+{
+  CUVS_EXPECTS(words != nullptr, "null words");
+  const int64_t *at = words, *end = words + n_words;
+  tensor t[3];
+  static const char* const names[] = {"keys", "queries", "pages"};
+  for (int i = 0; i < 3; i++) { t[i] = describe(at, end, names[i]); }
+  CUVS_EXPECTS(end - at == 1, "the words do not describe the call");
+  of(single_device(res), t, *at, bytes);
+}
+
+}  // namespace
+
 extern "C" cuvsError_t cuvsB200KvCacheWorkspaceArrays(cuvsResources_t res, const int64_t* words, int64_t n_words, size_t* bytes)
 {
-  return translate_exceptions([=] {
-    CUVS_EXPECTS(words != nullptr, "null words");
-    const int64_t *at = words, *end = words + n_words;
-    tensor t[3];
-    static const char* const names[] = {"keys", "queries", "pages"};
-    for (int i = 0; i < 3; i++) { t[i] = describe(at, end, names[i]); }
-    CUVS_EXPECTS(end - at == 1, "the words do not describe the call");
-    workspace_of(single_device(res), t, *at, bytes);
-  });
+  return translate_exceptions([=] { workspace_by_words(res, words, n_words, bytes, workspace_of); });
+}
+
+extern "C" cuvsError_t cuvsB200KvCacheTreeWorkspaceArrays(cuvsResources_t res, const int64_t* words, int64_t n_words, size_t* bytes)
+{
+  return translate_exceptions([=] { workspace_by_words(res, words, n_words, bytes, tree_workspace_of); });
 }
 
 extern "C" cuvsError_t cuvsB200KvCacheCheck(int device, int op, const int64_t* words, int64_t n_words)
@@ -624,10 +956,15 @@ extern "C" cuvsError_t cuvsB200KvCacheCheck(int device, int op, const int64_t* w
   return translate_exceptions([=] {
     call c(op, words, n_words);
     switch (op) {
-      case 0: append_of(device, c.t, c.interleaved); break;
-      case 1: attention_of(device, c.t, c.scale, c.window); break;
-      case 2: candidates_of(device, c.t, c.scale); break;
-      default: merge_of(device, c.t);
+      case APPEND:
+      case APPEND_TURNED: append_of(device, c.t, c.interleaved, op == APPEND_TURNED); break;
+      case ATTENTION: attention_of(device, c.t, c.scale, c.window); break;
+      case CANDIDATES: candidates_of(device, c.t, c.scale); break;
+      case MERGE: merge_of(device, c.t); break;
+      case DRAFT_TREE: draft_tree_of(device, c.t); break;
+      case ATTEND_TREE: attend_tree_of(device, c.t, c.scale, c.window, c.cap); break;
+      case KEEP_PATH: keep_path_of(device, c.t); break;
+      default: copy_pages_of(device, c.t);
     }
   });
 }

@@ -4,7 +4,8 @@
 // Pairs of columns (x1, x2) become (x1 cos a - x2 sin a, x2 cos a + x1 sin a), a = position * frequency.  The angle is formed and reduced
 // to half a turn in 64 bits -- a position of a million times a frequency of one leaves 32 bits no digits for the sine.  Sine and cosine are
 // taken of its first 32 bits and turned by the rest (to first order: it is below 2^-25), so that they are as exact as the functions are, once
-// per token and pair for all of its heads.
+// per token and pair for all of its heads.  With `turns` the angle is turns[token, axis of the pair] * frequency: tokens of images and videos have
+// several positions, drafted ones another than their place.
 #include "kv_rows.cuh"
 
 #include <algorithm>
@@ -51,7 +52,12 @@ append_kernel(append_args a, uint32_t log_lanes, uint32_t steps, uint32_t slices
   split_slot(a.cache, max(slot, int64_t(0)), page, place);
   for (uint32_t pair = lane; pair < a.n_pairs; pair += 32) {
     const double f = a.frequencies_f32 ? double(static_cast<const float*>(a.frequencies)[pair]) : static_cast<const double*>(a.frequencies)[pair];
-    const double half_turns = double(max(pos, 0)) * f * 0.31830988618379067154;  // 1 / pi
+    int32_t by     = max(pos, 0);
+    if (a.turns != nullptr) {
+      const int32_t axis = a.axes != nullptr ? a.axes[pair] : 0;
+      by                 = axis >= 0 && uint32_t(axis) < a.n_axes ? a.turns[int64_t(token) * a.turns_stride + axis] : 0;
+    }
+    const double half_turns = double(by) * f * 0.31830988618379067154;  // 1 / pi
     const double angle = half_turns - 2.0 * rint(0.5 * half_turns);
     const float near   = float(angle), rest = float(angle - double(near)) * 3.14159265f;
     float s, c;

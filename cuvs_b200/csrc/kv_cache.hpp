@@ -68,6 +68,11 @@ struct append_args {
   uint32_t n_pairs;
   bool interleaved;
   int64_t* slots;  // [n_tokens]
+  // What tokens are turned by where that is not their positions: [n_tokens, n_axes], and the axis of each pair (nullptr: the first).
+  const int32_t* turns;
+  int64_t turns_stride;
+  uint32_t n_axes;
+  const int32_t* axes;
 };
 void append(resources& res, cudaStream_t stream, const append_args& a);
 
@@ -89,6 +94,67 @@ struct attention_args {
 size_t attention_workspace(const resources& res, elem type, uint32_t n_sequences, uint32_t n_query_heads, uint32_t n_heads, uint32_t dim,
                            uint64_t capacity, int64_t window);
 void attention(resources& res, cudaStream_t stream, const attention_args& a);
+
+// [n_sequences, n_drafted, n_query_heads, dim] rows at any 16-byte strides
+struct drafted_rows_view {
+  char* data;
+  int64_t sequence, token, head;
+};
+
+struct draft_tree_args {
+  uint32_t n_sequences, n_drafted;
+  const int32_t* parents;  // [n_sequences, n_drafted]
+  int64_t parents_stride;
+  const int32_t* lengths;  // [n_sequences]
+  uint32_t* mask;          // [n_sequences, n_drafted, ceil(n_drafted / 32)]
+  int32_t* positions;      // [n_sequences, n_drafted]
+};
+void draft_tree(resources& res, cudaStream_t stream, const draft_tree_args& a);
+
+struct attend_tree_args {
+  cache_view cache;
+  elem type;
+  uint32_t n_sequences, n_drafted, n_query_heads, table_width;
+  int64_t table_stride;
+  drafted_rows_view queries, out;
+  const int32_t* pages;    // [n_sequences, table_width]
+  const int32_t* lengths;  // [n_sequences], without the drafted tokens
+  const int32_t* positions;  // [n_sequences, n_drafted]
+  int64_t positions_stride;
+  const uint32_t* mask;    // [n_sequences, n_drafted, words]
+  int64_t mask_sequence, mask_token;
+  const float* slopes;     // [n_query_heads], nullptr: none
+  float scale, cap;        // cap 0: none
+  int64_t window;          // 0: none
+  float* lse;              // [n_sequences, n_drafted, n_query_heads]
+  char* workspace;
+  size_t workspace_bytes;
+};
+// How many bytes of workspace attend_tree() wants, by sizes alone.
+size_t attend_tree_workspace(const resources& res, elem type, uint32_t n_sequences, uint32_t n_drafted, uint32_t n_query_heads, uint32_t n_heads,
+                             uint32_t dim, uint64_t capacity, int64_t window);
+void attend_tree(resources& res, cudaStream_t stream, const attend_tree_args& a);
+
+struct keep_path_args {
+  cache_view cache;
+  uint32_t row_bytes;
+  uint32_t n_sequences, n_entries, table_width;
+  int64_t table_stride, paths_stride;
+  const int32_t* pages;    // [n_sequences, table_width]
+  const int32_t* lengths;  // [n_sequences]
+  const int32_t* paths;    // [n_sequences, n_entries]
+  int32_t* kept;           // [n_sequences]
+};
+void keep_path(resources& res, cudaStream_t stream, const keep_path_args& a);
+
+struct copy_pages_args {
+  cache_view cache;
+  uint32_t row_bytes;
+  uint32_t n_pairs;
+  const int32_t* sources;  // [n_pairs]
+  const int32_t* targets;
+};
+void copy_pages(resources& res, cudaStream_t stream, const copy_pages_args& a);
 
 struct candidates_args {
   cache_view cache;

@@ -56,7 +56,8 @@ inline void make_room(work_view& w, uint64_t rows)
 // All positions of a sequence, or its last ones.  A list begins at a multiple of 16 positions, so that 16 rows lie in one page where pages
 // are multiples of 16.
 struct positions {
-  static constexpr bool kShares = true;
+  static constexpr bool kShares    = true;
+  static constexpr uint32_t kLeast = kLeastShare;  // chunks of a share, at least: one for each warp of a block
   using name_type               = int32_t;
   const int32_t* pages;
   const int32_t* lengths;
@@ -126,13 +127,12 @@ __device__ __forceinline__ uint64_t quotient(uint64_t a, uint32_t b)
   return a >> 32 == 0 ? uint64_t(uint32_t(a) / b) : a / b;  // the short division where it is enough
 }
 
-// `total` chunks of all units dealt out in `count` equal shares: one for every block, or fewer of kLeast chunks each (one for each of its warps).
+// `total` chunks of all units dealt out in `count` equal shares: one for every block, or fewer of `least` chunks each.
 struct share {
-  static constexpr uint32_t kLeast = kLeastShare;
   uint64_t total, each;
   uint32_t count, longer;  // the first `longer` get `each` + 1, the others `each`
-  __device__ __forceinline__ share(uint64_t total_, uint32_t most)
-    : total(total_), each(0), count(uint32_t(min(uint64_t(most), ceildiv<uint64_t>(total_, kLeast)))), longer(0)
+  __device__ __forceinline__ share(uint64_t total_, uint32_t most, uint32_t least)
+    : total(total_), each(0), count(uint32_t(min(uint64_t(most), ceildiv<uint64_t>(total_, least)))), longer(0)
   {
     if (count != 0u) {
       each   = quotient(total, count);
@@ -526,14 +526,14 @@ struct walk {
   typename Lists::list l;  // of the sequence that the walk is at
   share all;
   uint64_t at, stop, before;
-  uint32_t sequence, n;
+  uint32_t sequence, n, which;  // `which`: the share
 
-  __device__ __forceinline__ walk(const cache_view& c_, const work_view& w_, const Lists& lists_, uint32_t most)
-    : c(c_), w(w_), lists(lists_), all(all_chunks<CHUNK>(c_, w_, lists_), most), at(0), stop(0), before(0), sequence(0), n(0)
+  __device__ __forceinline__ walk(const cache_view& c_, const work_view& w_, const Lists& lists_, uint32_t most, uint32_t which_)
+    : c(c_), w(w_), lists(lists_), all(all_chunks<CHUNK>(c_, w_, lists_), most, Lists::kLeast), at(0), stop(0), before(0), sequence(0), n(0), which(which_)
   {
-    if (blockIdx.x >= all.count) { return; }
-    at       = all.start(blockIdx.x);
-    stop     = all.start(blockIdx.x + 1);
+    if (which >= all.count) { return; }
+    at       = all.start(which);
+    stop     = all.start(which + 1);
     sequence = sequence_of<CHUNK>(c, w, lists, at, before);
     if (sequence < w.n_sequences) {
       open();
@@ -566,7 +566,7 @@ struct walk {
       p.end      = uint32_t(to - begin);
       p.begins   = from == begin;
       p.whole    = p.begins && to == end;
-      if (p.begins && !p.whole) { p.n_parts = min(all.of(end - 1), all.count - 1u) - blockIdx.x + 1u; }
+      if (p.begins && !p.whole) { p.n_parts = min(all.of(end - 1), all.count - 1u) - which + 1u; }
       return true;
     }
     return false;
@@ -709,7 +709,7 @@ __device__ __forceinline__ void run_units(const cache_view& c, const work_view& 
   }
 
   if constexpr (Lists::kShares) {
-    walk<CHUNK, Lists> path(c, w, lists, parts.shares);
+    walk<CHUNK, Lists> path(c, w, lists, parts.shares, blockIdx.x);
     piece now, then;
     auto turn_to = [&](const piece& p) {
       hooks.attach(p.unit);

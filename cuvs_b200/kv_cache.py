@@ -22,6 +22,20 @@ an entry that is no page of the cache, such as -1, holds no tokens.  Query head 
 output is 0 and its ``lse`` is -inf.  Weights below 2^-100 of the largest may count as 0, in :func:`attention` over float16 those below 2^-38
 (times an infinite value that is no number).
 
+A decoder that drafts several tokens per sequence, a tree of them, and keeps the path that it accepts has as its step::
+
+    mask, positions = kv_cache.draft_tree(parents, lengths)                     # [n_sequences, n_drafted]; lengths: without the drafted tokens
+    places = lengths[:, None] + torch.arange(n_drafted, dtype=torch.int32, device="cuda")
+    slots, q = kv_cache.append(keys, values, new_keys.flatten(0, 1), new_values.flatten(0, 1), pages,
+                               torch.where(positions >= 0, places, -1).flatten(), sequences=sequences, queries=queries.flatten(0, 1),
+                               frequencies=frequencies, turns=positions.flatten())
+    out, lse = kv_cache.attend_tree(keys, values, q.view(queries.shape), pages, lengths, positions, mask)
+    lengths = kv_cache.keep_path(keys, values, pages, lengths, paths)           # paths: which of the drafted tokens stay, in order
+
+The drafted token ``j`` of a sequence is stored behind the sequence's own tokens, at place ``lengths[i] + j``, whatever its depth in the tree: its
+position, by which it is turned, is that of its depth.  Where a sequence goes on in several ways they have its full pages in common, and
+:func:`copy_pages` copies the last one.
+
 These calls serve: they have no gradients.  They enqueue their work on the stream of ``resources`` (torch's current stream by default) and
 wait for it unless ``sync=False``, which is what a captured call needs.
 """
@@ -41,7 +55,7 @@ from .common import Resources, _default_resources, default_resources
 _WORD = {t: (code << 32) | (bits << 40) | (1 << 48)
          for t, code, bits in ((torch.float16, 2, 16), (torch.bfloat16, 4, 16), (torch.float32, 2, 32), (torch.float64, 2, 64),
                                (torch.int32, 0, 32), (torch.int64, 0, 64), (torch.uint32, 1, 32), (torch.uint8, 1, 8))}
-_APPEND, _ATTENTION, _CANDIDATES, _MERGE = range(4)
+_APPEND, _ATTENTION, _CANDIDATES, _MERGE, _APPEND_TURNED, _DRAFT_TREE, _ATTEND_TREE, _KEEP_PATH, _COPY_PAGES = range(9)
 _f32 = struct.Struct("<f")
 _u32 = struct.Struct("<I")
 
@@ -115,17 +129,19 @@ def _empty(dtype, tensor, resources, stream, *shape):
         return torch.empty(*shape, dtype=dtype, device=tensor.device)
 
 
-def _call(resources, stream, op, tensors, integer, scale, sync):
-    """`tensors`: those of the call in the order of the C interface, filled up with None to eleven.  False: the call is being captured, and
-    needs a workspace to itself."""
+def _call(resources, stream, op, tensors, integer, scale, sync, cap=0.0):
+    """`tensors`: those of the call in the order of the C interface, filled up with None to eleven, from the fifth call on to thirteen.  False:
+    the call is being captured, and needs a workspace to itself."""
     for t in tensors:
         if t is not None and type(t) is not _Tensor:
-            return _call(resources, stream, op, tuple(_plain(t) for t in tensors), integer, scale, sync)
+            return _call(resources, stream, op, tuple(_plain(t) for t in tensors), integer, scale, sync, cap)
     if _tensors is None:
-        scalars = ((integer,), (integer, _bits(scale)), (_bits(scale),), ())[op]
+        scalars = ((integer,), (integer, _bits(scale)), (_bits(scale),), (), (integer,), (), (integer, _bits(scale), _bits(cap)), (), ())[op]
         status = _arrays(resources.handle, stream, op, *_words(tensors[:_COUNTS[op]], scalars), sync)
-    else:
+    elif op < _APPEND_TURNED:
         status = _tensors(resources.handle, stream, op, *tensors, integer, scale, sync)
+    else:
+        status = _more_tensors(resources.handle, stream, op, *tensors, integer, scale, cap, sync)
     if status == _NEEDS_WORKSPACE:
         return False
     if status != L.CUVS_SUCCESS:
@@ -145,31 +161,35 @@ def _plain(t):
 
 
 def _tensor_calls():
-    """The entry point that reads tensors in place, through torch's table of DLPack exchange functions: describing them in Python took as long
+    """The entry points that read tensors in place, through torch's table of DLPack exchange functions: describing them in Python took as long
     as everything else of a small call together.  None where torch has no such table."""
     capsule = getattr(torch.Tensor, "__dlpack_c_exchange_api__", None)
     if capsule is None:
-        return None
+        return None, None
     pointer = C.pythonapi.PyCapsule_GetPointer
     pointer.restype, pointer.argtypes = C.c_void_p, [C.py_object, C.c_char_p]
     if L.load().cuvsB200SetTensorExchange(pointer(capsule, b"dlpack_exchange_api"), id(None)) != L.CUVS_SUCCESS:
-        return None
-    call = C.PyDLL(L.LIB_PATH).cuvsB200KvCacheTensors  # keeps the interpreter's lock: it reads Python objects
-    call.restype, call.argtypes = C.c_int, L.SIGNATURES["cuvsB200KvCacheTensors"]
-    return call
+        return None, None
+    lib, calls = C.PyDLL(L.LIB_PATH), []  # keeps the interpreter's lock: it reads Python objects
+    for name in ("cuvsB200KvCacheTensors", "cuvsB200KvCacheMoreTensors"):
+        call = getattr(lib, name)
+        call.restype, call.argtypes = C.c_int, L.SIGNATURES[name]
+        calls.append(call)
+    return calls
 
 
-_COUNTS = (11, 9, 7, 4)
+_COUNTS = (11, 9, 7, 4, 13, 4, 12, 6, 4)
 _NEEDS_WORKSPACE = 2
 _Tensor = torch.Tensor
 _arrays = L.load().cuvsB200KvCacheArrays
 _workspace = L.load().cuvsB200KvCacheWorkspaceArrays
+_tree_workspace = L.load().cuvsB200KvCacheTreeWorkspaceArrays
 _wait = L.load().cuvsB200KvCacheWait
-_tensors = _tensor_calls()
+_tensors, _more_tensors = _tensor_calls()
 
 
 def append(keys, values, new_keys, new_values, pages, positions, sequences=None, queries=None, frequencies=None, interleaved=False,
-           slots=None, rotated=None, resources: Resources | None = None, sync: bool = True):
+           slots=None, rotated=None, resources: Resources | None = None, sync: bool = True, *, turns=None, axes=None):
     """Writes the rows of new tokens to their places in the cache and returns ``(slots, rotated)``: the tokens' slots (int64), and their
     turned queries (None without ``queries``).
 
@@ -181,6 +201,11 @@ def append(keys, values, new_keys, new_values, pages, positions, sequences=None,
     ``interleaved`` ``(2i, 2i + 1)`` -- of keys and queries are turned by ``position * frequencies[i]`` radians; columns behind them stay.
     Angles are formed in 64 bits.
 
+    ``turns`` (int32 ``[n_tokens]`` or ``[n_tokens, n_axes]``) turns keys and queries by other positions than those that say where the tokens go:
+    pair ``i`` of token ``t`` by ``turns[t, axes[i]] * frequencies[i]`` radians, either way round; ``axes``: int32 ``[n_pairs]``, not needed where there is one axis;
+    a pair whose axis is none of them stays.  (Tokens of images and videos have a time, a row and a column; a drafted token's position is
+    its depth in the tree, not its place.)
+
     A token whose position is negative (padding), whose sequence does not exist or whose page is not in the cache gets slot -1 and is not
     written; the query row of a token with a negative position is copied as it is.  Two tokens of a call must not have the same slot."""
     resources, stream = _handle(keys, resources)
@@ -188,8 +213,13 @@ def append(keys, values, new_keys, new_values, pages, positions, sequences=None,
         slots = _empty(torch.int64, keys, resources, stream, new_keys.shape[0])
     if queries is not None and rotated is None:
         rotated = _rows_like(queries, resources, stream)
-    _call(resources, stream, _APPEND, (keys, values, new_keys, new_values, pages, positions, sequences, queries, frequencies, slots, rotated),
-          1 if interleaved else 0, 0.0, sync)
+    tensors = (keys, values, new_keys, new_values, pages, positions, sequences, queries, frequencies, slots, rotated)
+    if turns is not None:
+        _call(resources, stream, _APPEND_TURNED, (*tensors, turns, axes), 1 if interleaved else 0, 0.0, sync)
+    elif axes is not None:
+        raise ValueError("axes go with turns")
+    else:
+        _call(resources, stream, _APPEND, tensors, 1 if interleaved else 0, 0.0, sync)
     return slots, rotated
 
 
@@ -268,3 +298,95 @@ def merge_parts(parts, parts_lse, out=None, lse=None, resources: Resources | Non
         lse = _empty(torch.float32, parts, resources, stream, n, n_heads)
     _call(resources, stream, _MERGE, (parts, parts_lse, out, lse, None, None, None, None, None, None, None), 0, 0.0, sync)
     return out, lse
+
+
+def draft_tree(parents, lengths, mask=None, positions=None, resources: Resources | None = None, sync: bool = True):
+    """Who reaches whom in the trees of a step's drafted tokens.  ``parents``: int32 ``[n_sequences, n_drafted]`` (at most 1024; sequences may
+    share a row, as ``expand`` makes it), the index of the token that each one follows, in whatever order they stand, or -1: it follows the
+    sequence itself; any other value, and what follows it, is no token.  ``lengths``: int32 ``[n_sequences]``, the sequences' tokens without them.
+
+    Returns ``(mask, positions)``: uint32 ``[n_sequences, n_drafted, ceil(n_drafted / 32)]``, in whose row ``j`` bit ``k % 32`` of word ``k // 32`` says that
+    ``k`` is ``j`` or one of its ancestors, and int32 ``[n_sequences, n_drafted]``, the length plus the number of ancestors; 0 and -1 for what is no token.
+    They hold for all layers of a step."""
+    resources, stream = _handle(parents, resources)
+    if parents.dim() != 2:
+        raise ValueError(f"parents: 2 dimensions, not {parents.dim()}")
+    n, m = parents.shape
+    if mask is None:
+        mask = _empty(torch.uint32, parents, resources, stream, n, m, (m + 31) // 32)
+    if positions is None:
+        positions = _empty(torch.int32, parents, resources, stream, n, m)
+    _call(resources, stream, _DRAFT_TREE, (parents, lengths, mask, positions, *(None,) * 9), 0, 0.0, sync)
+    return mask, positions
+
+
+def attend_tree(keys, values, queries, pages, lengths, positions, mask, scale=None, window=None, cap=None, slopes=None, filter=None, out=None,
+                lse=None, workspace=None, resources: Resources | None = None, sync: bool = True):
+    """Attention of the drafted tokens of each sequence, ``queries`` ``[n_sequences, n_drafted, n_query_heads, dim]``, to the sequence's positions
+    ``0 .. lengths[i] - 1`` and to those of its drafted tokens that ``mask`` names.  Returns ``(out, lse)``: of the queries' shape, and float32
+    ``[n_sequences, n_drafted, n_query_heads]``.
+
+    ``lengths``: int32 ``[n_sequences]``, without the drafted tokens, of which number ``k`` is stored at place ``lengths[i] + k``; ``positions`` (int32
+    ``[n_sequences, n_drafted]``) and ``mask`` (uint32 ``[n_sequences, n_drafted, words]``) as :func:`draft_tree` returns them, or any others, sequences may share
+    them; a token whose position is below its sequence's length is none: it attends to nothing, and none to it.
+
+    Scores are ``s = scale * q.k`` (``dim ** -0.5``), with ``cap`` then ``cap * tanh(s / cap)``, with ``slopes`` (float32 ``[n_query_heads]``) then less ``slope *
+    distance`` of the two positions.  ``window``: only what is less than so many positions before the token's own; ``filter``, ``workspace`` as in
+    :func:`attention`.  Of 16-bit rows, weights below 2^-30 of the largest may count as 0."""
+    window = _window(window)
+    resources, stream = _handle(keys, resources)
+    if queries.dim() != 4:
+        raise ValueError(f"queries: 4 dimensions, not {queries.dim()}")
+    if cap is not None and not 1e-30 <= cap <= 1e30:
+        raise ValueError("cap must be between 1e-30 and 1e30, or None")
+    n, m, n_heads, dim = queries.shape
+    if out is None:
+        out = _empty(queries.dtype, keys, resources, stream, n, m, n_heads, dim)
+    if lse is None:
+        lse = _empty(torch.float32, keys, resources, stream, n, m, n_heads)
+    scale, cap = dim ** -0.5 if scale is None else scale, cap or 0.0
+    tensors = (keys, values, queries, pages, lengths, positions, mask, slopes, filter, out, lse)
+    if not _call(resources, stream, _ATTEND_TREE, (*tensors, workspace, None), window, scale, sync, cap):
+        # what is replayed needs a workspace to itself; else the handle has one for the stream
+        workspace = _empty(torch.uint8, keys, resources, stream, _attend_tree_workspace(resources, keys, queries, pages, window))
+        _call(resources, stream, _ATTEND_TREE, (*tensors, workspace, None), window, scale, sync, cap)
+    return out, lse
+
+
+def attend_tree_workspace(keys, queries, pages, window=None, resources: Resources | None = None):
+    """Bytes of workspace that :func:`attend_tree` needs for tensors of these shapes."""
+    return _attend_tree_workspace(_handle(keys, resources)[0], keys, queries, pages, _window(window or None))
+
+
+def _attend_tree_workspace(resources, keys, queries, pages, window):
+    size = C.c_size_t()
+    L.check(_tree_workspace(resources.handle, *_words((keys, queries, pages), (window,)), size))
+    return size.value
+
+
+def keep_path(keys, values, pages, lengths, paths, kept=None, resources: Resources | None = None, sync: bool = True):
+    """Moves the rows of the drafted tokens that stay up to their sequences' ends, and returns the sequences' new lengths, int32 ``[n_sequences]``.
+
+    ``paths``: int32 ``[n_sequences, n_entries]``, which of the drafted tokens stay, in ascending order; a path ends at its first entry that is not
+    greater than the one before it, such as -1.  The row at place ``lengths[i] + paths[i, m]`` goes to place ``lengths[i] + m`` where the cache has both;
+    it has been turned by its position before, which stays the same where a path goes from parent to child.  ``kept`` receives the new lengths, in memory of
+    its own.  Pages that are written belong to one sequence alone."""
+    resources, stream = _handle(keys, resources)
+    if kept is None:
+        kept = _empty(torch.int32, keys, resources, stream, lengths.shape[0])
+    _call(resources, stream, _KEEP_PATH, (keys, values, pages, lengths, paths, kept, *(None,) * 7), 0, 0.0, sync)
+    return kept
+
+
+def copy_pages(keys, values, sources, targets, resources: Resources | None = None, sync: bool = True):
+    """Copies the pages ``sources[m]`` of keys and values to the pages ``targets[m]``, int32 ``[n_pairs]`` each.  A pair with a number that is no page of the
+    cache is skipped; no page may be the target of two pairs, or a target and a source.
+
+    Where a sequence goes on in several ways, the new ones have its full pages in common, and a copy of the last::
+
+        last = pages[sources, lengths[sources] // page_size]
+        kv_cache.copy_pages(keys, values, last, free)
+        pages[targets] = pages[sources]
+        pages[targets, lengths[sources] // page_size] = free"""
+    resources, stream = _handle(keys, resources)
+    _call(resources, stream, _COPY_PAGES, (keys, values, sources, targets, *(None,) * 9), 0, 0.0, sync)

@@ -68,10 +68,58 @@ CUVS_EXPORT cuvsError_t cuvsKvCacheAttendCandidates(cuvsResources_t res, DLManag
 CUVS_EXPORT cuvsError_t cuvsKvCacheMergeParts(cuvsResources_t res, DLManagedTensor* parts, DLManagedTensor* parts_lse,
                                               DLManagedTensor* out, DLManagedTensor* lse);
 
-/* The calls above on arrays that are described by words: op 0 append, 1 attention, 2 attend candidates, 3 merge parts.  The
- * tensors come in the order of the calls, each as ndim | type code << 32 | bits << 40 | lanes << 48; address; device type | device
+/* ---- steps of several drafted tokens per sequence ----
+ * A decoder that drafts a tree of tokens for each sequence checks all of them in one step: draft tree, append turned, attend tree, and, once it
+ * is known which of them stay, keep path.  Drafted token j of a sequence is stored at place lengths[i] + j, behind the sequence's own tokens,
+ * whatever its depth in the tree. */
+
+/* cuvsKvCacheAppend with turns other than the tokens' positions: i32 [n_tokens] or [n_tokens, n_axes] (those of a token contiguous); axes: i32
+ * [n_pairs], by which of its token's turns a pair is turned (a pair whose axis is none of them stays), or NULL with one axis. */
+CUVS_EXPORT cuvsError_t cuvsKvCacheAppendTurned(cuvsResources_t res, DLManagedTensor* keys, DLManagedTensor* values,
+                                                DLManagedTensor* new_keys, DLManagedTensor* new_values, DLManagedTensor* pages,
+                                                DLManagedTensor* positions, DLManagedTensor* sequences, DLManagedTensor* queries,
+                                                DLManagedTensor* frequencies, bool interleaved, DLManagedTensor* slots,
+                                                DLManagedTensor* rotated, DLManagedTensor* turns, DLManagedTensor* axes);
+
+/* What the trees' parents say: parents i32 [n_sequences, n_drafted] (1 to 1024; sequences may share one row, stride 0), the index of the
+ * token that each one follows, or -1: it follows the sequence itself; any other value, and what follows it: no token.  lengths: i32
+ * [n_sequences] (negative: 0).  mask: u32 [n_sequences, n_drafted, ceil(n_drafted / 32)], bit k % 32 of word k / 32 of token j is set if k is j
+ * or one of its ancestors; positions: i32 [n_sequences, n_drafted], the length plus the number of its ancestors; of no token: 0 and -1. */
+CUVS_EXPORT cuvsError_t cuvsKvCacheDraftTree(cuvsResources_t res, DLManagedTensor* parents, DLManagedTensor* lengths, DLManagedTensor* mask,
+                                             DLManagedTensor* positions);
+
+/* Attention of each sequence's drafted tokens to its tokens and to those of the drafted ones that the mask names.  queries, out: [n_sequences,
+ * n_drafted, n_query_heads, dim]; lengths: i32 [n_sequences], without the drafted tokens (negative: 0); positions, mask: as
+ * cuvsKvCacheDraftTree leaves them, or others (strides of sequences and of the mask's tokens may be 0).  Token j attends to the positions
+ * 0 .. lengths[i] - 1 and to the drafted tokens k whose bits its row of the mask has, each at its position, as far as that is less than `window`
+ * before its own (window > 0; 0: all), in the cache and let through by the filter.  A token whose position is below its sequence's length is
+ * none: it attends to nothing, and none to it.  Scores are s = scale * q.k, with cap > 0 then cap * tanh(s / cap), with slopes (f32
+ * [n_query_heads]) then less slope * distance of the positions.  lse: f32 [n_sequences, n_drafted, n_query_heads].  In attention to 16-bit rows
+ * weights below 2^-30 of the largest may count as 0.  Workspace as in cuvsKvCacheAttention. */
+CUVS_EXPORT cuvsError_t cuvsKvCacheAttendTree(cuvsResources_t res, DLManagedTensor* keys, DLManagedTensor* values, DLManagedTensor* queries,
+                                              DLManagedTensor* pages, DLManagedTensor* lengths, DLManagedTensor* positions,
+                                              DLManagedTensor* mask, float scale, int64_t window, float cap, DLManagedTensor* slopes,
+                                              cuvsFilter filter, DLManagedTensor* out, DLManagedTensor* lse, DLManagedTensor* workspace);
+CUVS_EXPORT cuvsError_t cuvsKvCacheAttendTreeWorkspace(cuvsResources_t res, DLManagedTensor* keys, DLManagedTensor* queries,
+                                                       DLManagedTensor* pages, int64_t window, size_t* bytes);
+
+/* Moves the rows of the drafted tokens that stay up to their sequences' ends: paths i32 [n_sequences, n_entries] (at most 1024) names them in
+ * ascending order, and ends at the first entry that is not greater than the one before it (-1, say).  The row at place lengths[i] + path[m] goes to
+ * place lengths[i] + m, where both have slots; kept: i32 [n_sequences], receives lengths[i] + the number of entries (not the lengths' own
+ * memory).  No two sequences may have the pages that this writes in common. */
+CUVS_EXPORT cuvsError_t cuvsKvCacheKeepPath(cuvsResources_t res, DLManagedTensor* keys, DLManagedTensor* values, DLManagedTensor* pages,
+                                            DLManagedTensor* lengths, DLManagedTensor* paths, DLManagedTensor* kept);
+
+/* Copies pages sources[m] to pages targets[m], i32 [n_pairs] each: for a sequence that goes on in several ways, whose last page is not full.  A
+ * pair with a number that is no page is skipped.  No page may be the target of two pairs, or a target and a source. */
+CUVS_EXPORT cuvsError_t cuvsKvCacheCopyPages(cuvsResources_t res, DLManagedTensor* keys, DLManagedTensor* values, DLManagedTensor* sources,
+                                             DLManagedTensor* targets);
+
+/* The calls above on arrays that are described by words: op 0 append, 1 attention, 2 attend candidates, 3 merge parts, 4 append turned, 5
+ * draft tree, 6 attend tree, 7 keep path, 8 copy pages.  The tensors come in the order of the calls, each as ndim | type code << 32 | bits << 40 | lanes << 48; address; device type | device
  * id << 32; the shape; the strides in elements -- or as one word 0 where there is none -- with a filter as a u32 tensor in the place
- * of its argument; behind them the scalars: {interleaved}, {window, bits of the f32 scale}, {bits of the scale}, {}.  The
+ * of its argument; behind them the scalars: {interleaved}, {window, bits of the f32 scale}, {bits of the scale}, {}, {interleaved}, {},
+ * {window, bits of the scale, bits of the f32 cap}, {}, {}.  The
  * work goes to `stream`, whatever the handle's own is, and is waited for if `sync`.  Returns a cuvsError_t, or 2 where the call needs a
  * workspace to itself (attention that is captured): nothing was done then. */
 CUVS_EXPORT int cuvsB200KvCacheArrays(cuvsResources_t res, cudaStream_t stream, int op, const int64_t* words, int64_t n_words, bool sync);
@@ -81,9 +129,15 @@ CUVS_EXPORT int cuvsB200KvCacheArrays(cuvsResources_t res, cudaStream_t stream, 
 CUVS_EXPORT cuvsError_t cuvsB200SetTensorExchange(const void* table, const void* none);
 CUVS_EXPORT int cuvsB200KvCacheTensors(cuvsResources_t res, cudaStream_t stream, int op, void* t0, void* t1, void* t2, void* t3, void* t4,
                                        void* t5, void* t6, void* t7, void* t8, void* t9, void* t10, int64_t integer, float scale, bool sync);
+/* The same for all calls (those above: the first four). */
+CUVS_EXPORT int cuvsB200KvCacheMoreTensors(cuvsResources_t res, cudaStream_t stream, int op, void* t0, void* t1, void* t2, void* t3, void* t4,
+                                           void* t5, void* t6, void* t7, void* t8, void* t9, void* t10, void* t11, void* t12, int64_t integer,
+                                           float scale, float cap, bool sync);
 CUVS_EXPORT cuvsError_t cuvsB200KvCacheWait(cuvsResources_t res, cudaStream_t stream);
 /* cuvsKvCacheAttentionWorkspace on the words of keys, queries, pages and {window}. */
 CUVS_EXPORT cuvsError_t cuvsB200KvCacheWorkspaceArrays(cuvsResources_t res, const int64_t* words, int64_t n_words, size_t* bytes);
+/* cuvsKvCacheAttendTreeWorkspace on such words. */
+CUVS_EXPORT cuvsError_t cuvsB200KvCacheTreeWorkspaceArrays(cuvsResources_t res, const int64_t* words, int64_t n_words, size_t* bytes);
 /* The checks of such a call alone, for a handle of `device`: touches no GPU and reads no tensor. */
 CUVS_EXPORT cuvsError_t cuvsB200KvCacheCheck(int device, int op, const int64_t* words, int64_t n_words);
 
