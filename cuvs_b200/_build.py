@@ -33,6 +33,7 @@ UNITS = [("resources.cu", "resources.o", []), ("index.cu", "index.o", []),
          ("kv_append.cu", "kv_append.o", []), ("kv_rows.cu", "kv_rows.o", []),
          ("kv_merge.cu", "kv_merge.o", []), ("kv_pages.cu", "kv_pages.o", []), ("kv_tree_rows.cu", "kv_tree_rows.o", [])]
 UNITS += [("kv_attention.cu", f"kv_attention_{name}.o", [f"-DKV_TYPE={t}"]) for name, t in (("f16", "__half"), ("bf16", "__nv_bfloat16"))]
+UNITS += [("kv_tree_tc.cu", f"kv_tree_tc_{name}.o", [f"-DKV_TYPE={t}"]) for name, t in (("f16", "__half"), ("bf16", "__nv_bfloat16"))]
 UNITS += [("scan_inst.cu", f"scan_{b}.o", [f"-DPQ_BITS={b}"]) for b in (4, 5, 6, 7, 8)]
 
 

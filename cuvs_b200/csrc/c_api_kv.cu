@@ -635,6 +635,17 @@ void tree_workspace_of(resources& res, tensor* t, int64_t window, size_t* bytes)
   *bytes = kv::attend_tree_workspace(res, type, uint32_t(n), uint32_t(m), uint32_t(h), c.n_heads, c.dim, uint64_t(width) * c.page.size, window);
 }
 
+void wait_for(resources& res, cudaStream_t stream)
+{
+  device_scope on(res.device);
+  CUDA_TRY(cudaStreamSynchronize(stream));
+  // a kernel of this handle that gave up on a wait inside it (its waits have limits)
+  volatile uint32_t* timeouts = res.pinned + 14;
+  const bool timed_out        = *timeouts != 0u;
+  if (timed_out) { *timeouts = 0u; }
+  CUVS_EXPECTS(!timed_out, "attention to drafted tokens gave up on a wait: its results are not complete");
+}
+
 resources& single_device(cuvsResources_t res)
 {
   resources* r = res_of(res);
@@ -870,7 +881,7 @@ extern "C" int cuvsB200KvCacheArrays(cuvsResources_t res, cudaStream_t stream, i
   int status = CUVS_ERROR;
   const auto raised = translate_exceptions([&] {
     status = call(op, words, n_words).run(res, stream, op, sync) ? CUVS_SUCCESS : kNeedsWorkspace;
-    if (sync && status == CUVS_SUCCESS) { CUDA_TRY(cudaStreamSynchronize(stream)); }
+    if (sync && status == CUVS_SUCCESS) { wait_for(single_device(res), stream); }
   });
   return raised == CUVS_SUCCESS ? status : CUVS_ERROR;
 }
@@ -920,8 +931,7 @@ extern "C" int cuvsB200KvCacheMoreTensors(cuvsResources_t res, cudaStream_t stre
 extern "C" cuvsError_t cuvsB200KvCacheWait(cuvsResources_t res, cudaStream_t stream)
 {
   return translate_exceptions([=] {
-    device_scope on(single_device(res).device);
-    CUDA_TRY(cudaStreamSynchronize(stream));
+    wait_for(single_device(res), stream);
   });
 }
 

@@ -294,6 +294,28 @@ inline tree_plan deal_out_tree(uint32_t blocks, uint32_t rows, uint32_t tile, ui
   return p;
 }
 
+constexpr uint32_t tree_columns(uint32_t dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
+
+// Everything that a kernel for rows of one type is called with.
+struct tree_call {
+  cache_view c;
+  work_view w;
+  drafted_lists lists;
+  tree_view t;
+  tree_parts parts;
+  tree_plan plan;
+  const int32_t* pages;
+  int64_t table_stride;
+  float shift;         // weights are held times 2^shift
+  uint32_t* timeouts;  // calls whose waits took too long, counted
+};
+template <typename T>
+void attend_tree16(cudaStream_t stream, const tree_call& call);
+template <>
+void attend_tree16<__half>(cudaStream_t stream, const tree_call& call);
+template <>
+void attend_tree16<__nv_bfloat16>(cudaStream_t stream, const tree_call& call);
+
 template <typename T>
 void launch_tree_join(cudaStream_t stream, const tree_plan& p, uint64_t units, const tree_view& t, const tree_parts& parts, uint32_t dim,
                       uint32_t n_heads, float shift)

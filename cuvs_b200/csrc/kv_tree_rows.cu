@@ -246,15 +246,14 @@ tree_rows_kernel(cache_view c, work_view w, drafted_lists lists, tree_view t, tr
   empty_tree_rows<T>(c, w.n_sequences, lists, t, threadIdx.x, kThreads);
 }
 
-constexpr uint32_t padded_columns(uint32_t dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
-
-tree_plan plan_of(const resources& res, elem, uint64_t sequences, uint32_t n_drafted, uint32_t n_heads, uint32_t group, uint32_t dim,
+tree_plan plan_of(const resources& res, elem type, uint64_t sequences, uint32_t n_drafted, uint32_t n_heads, uint32_t group, uint32_t dim,
                   uint64_t capacity, int64_t window)
 {
-  const uint32_t n_rows = n_drafted * group;
+  const uint32_t n_rows = n_drafted * group, sms = uint32_t(res.sm_count);
   // the keys of the longest list: a window may begin anywhere in 16 positions
   const uint64_t most = window > 0 && uint64_t(window) < capacity ? std::min(capacity, uint64_t(window) + n_drafted + 15) : capacity;
-  return deal_out_tree(uint32_t(res.sm_count), n_rows <= 16 ? 16 : 64, dim <= 128 ? 64 : 32, 2, sequences * n_heads, n_rows, most);
+  if (type == elem::f32) { return deal_out_tree(sms, n_rows <= 16 ? 16 : 64, dim <= 128 ? 64 : 32, 2, sequences * n_heads, n_rows, most); }
+  return deal_out_tree(sms, dim <= 128 && n_rows > 128 ? 256 : 128, dim <= 128 ? 128 : 64, 1, sequences * n_heads, n_rows, most);
 }
 
 }  // namespace
@@ -274,7 +273,13 @@ void attend_tree(resources& res, cudaStream_t stream, const attend_tree_args& a)
   const uint32_t group    = a.n_query_heads / c.n_heads;
   const uint64_t capacity = uint64_t(a.table_width) * c.page.size, units = uint64_t(a.n_sequences) * c.n_heads;
   const tree_plan p       = plan_of(res, a.type, a.n_sequences, a.n_drafted, c.n_heads, group, c.dim, capacity, a.window);
-  tree_view t{};
+  tree_call call{};
+  call.c             = c;
+  call.plan          = p;
+  call.pages         = a.pages;
+  call.table_stride  = a.table_stride;
+  call.timeouts      = res.pinned + 14;
+  tree_view& t       = call.t;
   t.n_drafted        = a.n_drafted;
   t.group            = group;
   t.n_rows           = a.n_drafted * group;
@@ -293,46 +298,50 @@ void attend_tree(resources& res, cudaStream_t stream, const attend_tree_args& a)
   t.scale_log2       = a.scale * kLog2E;
   t.scale_cap        = a.cap != 0.0f ? a.scale / a.cap : 0.0f;
   t.cap_log2         = a.cap * kLog2E;
-  const drafted_lists lists{a.lengths, a.window, a.table_width, a.n_drafted};
-  work_view w{a.n_sequences, c.n_heads, 1, group, 0, p.cost};
-  make_room(w, capacity);
-  const float shift = std::log2(w.room);
-  tree_parts parts{};
-  if (p.parts) { parts = tree_parts_at(a.workspace, p.shares, p.blocks_of, p.rows, c.dim); }
-  parts.shares    = p.shares;
-  parts.blocks_of = p.blocks_of;
-  parts.rows      = p.rows;
+  call.lists         = {a.lengths, a.window, a.table_width, a.n_drafted};
+  call.w             = {a.n_sequences, c.n_heads, 1, group, 0, p.cost};
+  make_room(call.w, capacity);
+  // room for the sum of a whole list, and for weights above 1 where a top may be behind; the weights of 16-bit floats have their own (kv_tree_tc.cuh)
+  call.shift = a.type == elem::f32 ? std::log2(call.w.room) : a.type == elem::bf16 ? std::log2(call.w.room) - 4.0f : 11.0f;
+  if (p.parts) { call.parts = tree_parts_at(a.workspace, p.shares, p.blocks_of, p.rows, c.dim); }
+  call.parts.shares    = p.shares;
+  call.parts.blocks_of = p.blocks_of;
+  call.parts.rows      = p.rows;
   count_launches(res, p.parts ? 2 : 1);
 
-  auto go = [&](auto type, auto columns, auto bm) {
-    using T = decltype(type);
+  auto join = [&](auto type) {
+    if (p.parts) { launch_tree_join<decltype(type)>(stream, p, units, t, call.parts, c.dim, c.n_heads, call.shift); }
+  };
+  if (a.type == elem::f16) {
+    attend_tree16<__half>(stream, call);
+    return join(__half{});
+  }
+  if (a.type == elem::bf16) {
+    attend_tree16<__nv_bfloat16>(stream, call);
+    return join(__nv_bfloat16{});
+  }
+  auto go = [&](auto columns, auto bm) {
     constexpr int D = decltype(columns)::value, BM = decltype(bm)::value;
-    auto kernel = tree_rows_kernel<T, D, BM>;
+    auto kernel = tree_rows_kernel<float, D, BM>;
     constexpr size_t smem = tree_shape<D, BM>::kShared;
-    if (smem > 48 * 1024) { ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem); }
-    launch_chained(kernel, dim3(p.shares * p.blocks_of), kThreads, smem, stream, c, w, lists, t, parts, a.pages, a.table_stride, shift);
-    if (p.parts) { launch_tree_join<T>(stream, p, units, t, parts, c.dim, c.n_heads, shift); }
+    ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem);
+    launch_chained(kernel, dim3(p.shares * p.blocks_of), kThreads, smem, stream, c, call.w, call.lists, t, call.parts, a.pages, a.table_stride,
+                   call.shift);
   };
   using std::integral_constant;
-  auto by_rows = [&](auto type, auto columns) {
+  auto by_rows = [&](auto columns) {
     if (p.rows == 16) {
-      go(type, columns, integral_constant<int, 16>{});
+      go(columns, integral_constant<int, 16>{});
     } else {
-      go(type, columns, integral_constant<int, 64>{});
+      go(columns, integral_constant<int, 64>{});
     }
   };
-  auto by_columns = [&](auto type) {
-    switch (padded_columns(c.dim)) {
-      case 64: return by_rows(type, integral_constant<int, 64>{});
-      case 128: return by_rows(type, integral_constant<int, 128>{});
-      default: return by_rows(type, integral_constant<int, 256>{});
-    }
-  };
-  switch (a.type) {
-    case elem::f16: return by_columns(__half{});
-    case elem::bf16: return by_columns(__nv_bfloat16{});
-    default: return by_columns(float{});
+  switch (tree_columns(c.dim)) {
+    case 64: by_rows(integral_constant<int, 64>{}); break;
+    case 128: by_rows(integral_constant<int, 128>{}); break;
+    default: by_rows(integral_constant<int, 256>{});
   }
+  join(float{});
 }
 
 }  // namespace cuvs_b200::kv

@@ -101,6 +101,7 @@ resources::resources()
   CUDA_TRY(cudaMallocHost(&pinned, 64));
   pinned[12] = 0;
   pinned[13] = 0;
+  pinned[14] = 0;
   CUDA_TRY(cudaMalloc(&redo_counts, N_REDO_COUNTS * sizeof(*redo_counts)));
   CUDA_TRY(cudaMemset(redo_counts, 0, N_REDO_COUNTS * sizeof(*redo_counts)));
 }
