@@ -441,7 +441,7 @@ kv::attend_tree_args attend_tree_of(int device, tensor* t, float scale, int64_t 
   CUVS_EXPECTS(window >= 0, "window must not be negative");
   a.scale  = scale;
   a.cap    = cap;
-  a.window = window;
+  a.window = std::min(window, int64_t(1) << 31);  // (no two positions are further apart)
   a.out    = drafted_rows_of(device, t[OUT], a.type, a.cache, "out");
   CUVS_EXPECTS(std::equal(t[OUT].shape, t[OUT].shape + 4, t[QUERIES].shape), "out: the shape of the queries");
   check_distinct(t[OUT], "out");

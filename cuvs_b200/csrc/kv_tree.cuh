@@ -30,7 +30,11 @@ struct tree_view {
   float* lse;
   float scale_log2;  // scores in powers of two: scale * log2(e)
   float scale_cap, cap_log2;  // scale / cap, cap * log2(e); cap_log2 = 0: no cap
+  float cap_near[5];          // cap_log2 tanh(y) = y (cap_near[0] + cap_near[1] y^2 + ..) for |y| below kTanhNear
 };
+// tanh(y) / y by least squares at Chebyshev's points of y^2: to 2^-27.
+constexpr float kTanhNear = 0.4f;
+constexpr float kTanh[5]  = {1.0f, -0.333333283662796f, 0.13332538306713104f, -0.0537162646651268f, 0.019272800534963608f};
 
 // The keys of a sequence and its drafted tokens, as far as any of them may be seen.  What is in the list of positions of one token is in this one: the
 // window is that of a token at position `length`, and those after it see no key before its first.
@@ -100,8 +104,10 @@ __device__ __forceinline__ uint32_t seen_keys(const tree_view& t, const drafted_
 struct tree_parts {
   float4* acc;
   float2* stats;  // [parts][rows] top (of scores in powers of two), sum
-  uint4* begun;   // [shares] sequence, key head, how many parts (0: there is none)
+  uint4* begun;   // [entries] sequence, key head, how many parts (0: there is none), the share that has the first
+  uint32_t entries;  // one for each unit, or, where these are more than the shares, for the one unit that a share begins and does not end
   uint32_t shares, blocks_of, rows, quads;
+  bool by_unit;
   __device__ __forceinline__ size_t part(uint32_t share, uint32_t block, uint32_t slot) const
   {
     return (size_t(share) * blocks_of + block) * 2 + slot;
@@ -111,9 +117,11 @@ inline size_t tree_part_bytes(uint32_t shares, uint32_t blocks_of, uint32_t rows
 {
   return size_t(shares) * (sizeof(uint4) + size_t(blocks_of) * 2 * rows * (ceildiv(dim, 4u) * sizeof(float4) + sizeof(float2)));
 }
-inline tree_parts tree_parts_at(char* workspace, uint32_t shares, uint32_t blocks_of, uint32_t rows, uint32_t dim)
+inline tree_parts tree_parts_at(char* workspace, uint32_t shares, uint32_t blocks_of, uint32_t rows, uint32_t dim, uint64_t units)
 {
   tree_parts p;
+  p.by_unit   = units <= shares;
+  p.entries   = p.by_unit ? uint32_t(units) : shares;
   p.shares    = shares;
   p.blocks_of = blocks_of;
   p.rows      = rows;
@@ -152,19 +160,31 @@ __device__ __forceinline__ void store_quad(T* to, float4 x)
 // What sequences have no keys at all: they are in no share.  By `threads` threads of each block.
 template <typename T>
 __device__ __forceinline__ void empty_tree_rows(const cache_view& c, uint32_t n_sequences, const drafted_lists& lists, const tree_view& t,
-                                                uint32_t thread, uint32_t threads)
+                                                const tree_parts& parts, uint32_t thread, uint32_t threads)
 {
   for (uint32_t b = blockIdx.x; b < n_sequences; b += gridDim.x) {
     drafted_lists::list l;
     if (lists.open(c, b, 16, l) != 0u) { continue; }
     const uint32_t quads = c.dim / 4;
     for (uint32_t h = 0; h < c.n_heads; h++) {
+      if (parts.begun != nullptr && parts.by_unit && thread == 0) { parts.begun[b * c.n_heads + h] = make_uint4(0, 0, 0, 0); }
       for (uint32_t i = thread; i < t.n_rows * quads; i += threads) {
         const uint32_t r = i / quads;
         store_quad<T>(out_row<T>(t, b, h, r) + (i - r * quads) * 4, make_float4(0.0f, 0.0f, 0.0f, 0.0f));
       }
       for (uint32_t r = thread; r < t.n_rows; r += threads) { *lse_at(t, b, h, c.n_heads, r) = -INFINITY; }
     }
+  }
+}
+
+// What the join finds of a piece that begins its unit; `last`: of the share's last such unit, if entries are those of shares.
+__device__ __forceinline__ void note_begun(const tree_parts& parts, const piece& p, uint32_t n_heads, uint32_t which, uint4& last)
+{
+  const uint4 entry = make_uint4(p.sequence, p.unit, p.whole ? 0u : p.n_parts, which);
+  if (parts.begun != nullptr && parts.by_unit) {
+    parts.begun[p.sequence * n_heads + p.unit] = entry;
+  } else {
+    last = entry;
   }
 }
 
@@ -180,11 +200,11 @@ tree_join_kernel(tree_view t, tree_parts parts, uint32_t dim, uint32_t n_heads, 
 {
   chain_begin();
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
-  const uint32_t groups = ceildiv(parts.rows, 32u);
-  const uint32_t share = blockIdx.x / (groups * parts.blocks_of), rest = blockIdx.x - share * (groups * parts.blocks_of);
+  const uint32_t groups = ceildiv(min(parts.rows, t.n_rows), 32u);
+  const uint32_t entry = blockIdx.x / (groups * parts.blocks_of), rest = blockIdx.x - entry * (groups * parts.blocks_of);
   const uint32_t block = rest / groups, r = (rest - block * groups) * 32 + lane;
-  const uint4 unit = parts.begun[share];
-  const uint32_t n = unit.z, row = block * parts.rows + r;
+  const uint4 unit = parts.begun[entry];
+  const uint32_t n = unit.z, share = unit.w, row = block * parts.rows + r;
   if (n == 0u || block * parts.rows + (r - lane) >= t.n_rows) { return; }
   const bool there = r < parts.rows && row < t.n_rows;
   const uint32_t rr = min(r, parts.rows - 1u);
@@ -320,7 +340,7 @@ template <typename T>
 void launch_tree_join(cudaStream_t stream, const tree_plan& p, uint64_t units, const tree_view& t, const tree_parts& parts, uint32_t dim,
                       uint32_t n_heads, float shift)
 {
-  const uint32_t items = p.shares * p.blocks_of * ceildiv(p.rows, 32u), quads = ceildiv(dim, 4u);
+  const uint32_t items = parts.entries * p.blocks_of * ceildiv(std::min(p.rows, t.n_rows), 32u), quads = ceildiv(dim, 4u);
   // Many parts of few units: warps share them.
   if (uint64_t(p.shares) > 8 * units) {
     launch_chained(tree_join_kernel<T, true>, dim3(items, quads), kTreeJoinWarps * 32, 0, stream, t, parts, dim, n_heads, shift);

@@ -10,6 +10,9 @@ namespace {
 
 constexpr int kThreads = 256;
 
+// Blocks of an SM: what shared memory and registers leave room for.  They hide each other's loads.
+constexpr int tree_resident(int columns, int rows) { return columns == 64 ? (rows == 16 ? 4 : 3) : columns == 128 ? (rows == 16 ? 2 : 1) : rows == 16 ? 2 : 1; }
+
 // D: columns of a row in shared memory; BM: rows of a block.  Threads stand in 16 x 16: thread (y, x) has BM / 16 rows, their scores with every 16th key
 // and their weighted sums in every 16th four columns.
 template <int D, int BM>
@@ -26,10 +29,12 @@ struct tree_shape {
   static constexpr int kValidAt = kSeenAt + BM * (kTile / 32);
   static constexpr int kPlaceAt = kValidAt + 4;
   static constexpr int kShared = (kPlaceAt + 3 * kTile) * 4;
+  static constexpr int kResident = tree_resident(D, BM);
+  static_assert(kResident * (kShared + 1024) <= 233472, "");
 };
 
 template <typename T, int D, int BM>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kThreads, tree_shape<D, BM>::kResident)
 tree_rows_kernel(cache_view c, work_view w, drafted_lists lists, tree_view t, tree_parts parts, const int32_t* pages, int64_t table_stride, float shift)
 {
   using shape = tree_shape<D, BM>;
@@ -240,10 +245,10 @@ tree_rows_kernel(cache_view c, work_view w, drafted_lists lists, tree_view t, tr
         }
       }
     }
-    if (now.begins && !now.whole) { begun = make_uint4(now.sequence, now.unit, now.n_parts, 0); }
+    if (now.begins && threadIdx.x == 0) { note_begun(parts, now, c.n_heads, which, begun); }
   }
-  if (parts.begun != nullptr && block == 0 && threadIdx.x == 0) { parts.begun[which] = begun; }
-  empty_tree_rows<T>(c, w.n_sequences, lists, t, threadIdx.x, kThreads);
+  if (parts.begun != nullptr && !parts.by_unit && block == 0 && threadIdx.x == 0) { parts.begun[which] = begun; }
+  empty_tree_rows<T>(c, w.n_sequences, lists, t, parts, threadIdx.x, kThreads);
 }
 
 tree_plan plan_of(const resources& res, elem type, uint64_t sequences, uint32_t n_drafted, uint32_t n_heads, uint32_t group, uint32_t dim,
@@ -252,8 +257,11 @@ tree_plan plan_of(const resources& res, elem type, uint64_t sequences, uint32_t 
   const uint32_t n_rows = n_drafted * group, sms = uint32_t(res.sm_count);
   // the keys of the longest list: a window may begin anywhere in 16 positions
   const uint64_t most = window > 0 && uint64_t(window) < capacity ? std::min(capacity, uint64_t(window) + n_drafted + 15) : capacity;
-  if (type == elem::f32) { return deal_out_tree(sms, n_rows <= 16 ? 16 : 64, dim <= 128 ? 64 : 32, 2, sequences * n_heads, n_rows, most); }
-  return deal_out_tree(sms, dim <= 128 && n_rows > 128 ? 256 : 128, dim <= 128 ? 128 : 64, 1, sequences * n_heads, n_rows, most);
+  if (type == elem::f32) {
+    const int rows = n_rows <= 16 ? 16 : 64;
+    return deal_out_tree(sms * tree_resident(int(tree_columns(dim)), rows), n_rows <= 16 ? 16 : 64, dim <= 128 ? 64 : 32, 2, sequences * n_heads, n_rows, most);
+  }
+  return deal_out_tree(sms, dim <= 128 && n_rows > 128 ? 256 : 128, 64, 2, sequences * n_heads, n_rows, most);
 }
 
 }  // namespace
@@ -298,12 +306,13 @@ void attend_tree(resources& res, cudaStream_t stream, const attend_tree_args& a)
   t.scale_log2       = a.scale * kLog2E;
   t.scale_cap        = a.cap != 0.0f ? a.scale / a.cap : 0.0f;
   t.cap_log2         = a.cap * kLog2E;
+  for (int i = 0; i < 5; i++) { t.cap_near[i] = t.cap_log2 * kTanh[i]; }
   call.lists         = {a.lengths, a.window, a.table_width, a.n_drafted};
   call.w             = {a.n_sequences, c.n_heads, 1, group, 0, p.cost};
   make_room(call.w, capacity);
   // room for the sum of a whole list, and for weights above 1 where a top may be behind; the weights of 16-bit floats have their own (kv_tree_tc.cuh)
   call.shift = a.type == elem::f32 ? std::log2(call.w.room) : a.type == elem::bf16 ? std::log2(call.w.room) - 4.0f : 11.0f;
-  if (p.parts) { call.parts = tree_parts_at(a.workspace, p.shares, p.blocks_of, p.rows, c.dim); }
+  if (p.parts) { call.parts = tree_parts_at(a.workspace, p.shares, p.blocks_of, p.rows, c.dim, units); }
   call.parts.shares    = p.shares;
   call.parts.blocks_of = p.blocks_of;
   call.parts.rows      = p.rows;

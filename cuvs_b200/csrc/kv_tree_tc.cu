@@ -19,29 +19,30 @@ namespace cuvs_b200::kv {
 namespace {
 
 constexpr int kThreads    = 512;  // two softmax groups, four warps that copy, one that multiplies, one that finds the way
-constexpr int kInfos      = 8;    // tiles whose descriptions are kept
+constexpr int kInfos      = 16;   // tiles whose descriptions are kept: more than can be between copying keys and the softmax
 constexpr int kPieces     = 2;
-constexpr int kReaders    = 13;   // warps that read a piece's description
+constexpr int kReaders    = 14;   // warps that read a piece's description
+constexpr uint32_t kTile  = 64;   // keys
+constexpr int kMostStages = 10;
 constexpr uint32_t kLimit = kSpinLimit;
 
 template <int D>
 struct tc_shape {
-  static constexpr bool kTwo      = D <= 128;
-  static constexpr int kTile      = kTwo ? 128 : 64;
+  static constexpr bool kTwo      = D <= 128;          // two streams with sums of their own
   static constexpr int kRows      = kTwo ? 256 : 128;  // of a block, at most
-  static constexpr int kPanel     = kTile * 128;       // bytes of 64 columns of a tile
+  static constexpr int kPanel     = int(kTile) * 128;  // bytes of 64 columns of a tile
   static constexpr int kTileBytes = kPanel * (D / 64);
   static constexpr int kQPanel    = 128 * 128;
   static constexpr int kQBytes    = kQPanel * (D / 64);
   static constexpr int kExchange  = kQBytes;  // where two groups exchange sums: behind the first 128 rows
   static constexpr int kQRegion   = !kTwo ? kQBytes : 2 * kQBytes > kQBytes + 32768 ? 2 * kQBytes : kQBytes + 32768;
   static constexpr int kMisc      = 3072;
-  static constexpr int kStages    = (232448 - kQRegion - kMisc) / kTileBytes < 10 ? (232448 - kQRegion - kMisc) / kTileBytes : 10;
-  static constexpr int kBehind    = kStages - 2;  // tiles in flight: one more would wait for what waits for it
+  static constexpr int kFit       = (232448 - kQRegion - kMisc) / kTileBytes;
+  static constexpr int kStages    = kFit < kMostStages ? kFit : kMostStages;
   static constexpr int kRingAt    = kQRegion;
   static constexpr int kMiscAt    = kRingAt + kStages * kTileBytes;
   static constexpr int kShared    = kMiscAt + kMisc;
-  static constexpr int kSumsAt    = 256;               // first column of the sums in tensor memory
+  static constexpr int kSumsAt    = 256;               // first column of the sums in tensor memory, behind two tiles of scores of each stream
   static_assert(kStages >= 4 && kShared <= 232448, "");
 };
 
@@ -54,11 +55,12 @@ struct tree_piece {
 };
 
 struct tc_shared {
-  uint64_t full[10], empty[10];
-  uint64_t q_full, q_empty, s_full[2], p_full[2], o_full[2], pv_done, exchanged, drained;
+  uint64_t full[kMostStages], empty[kMostStages];
+  uint64_t q_full, q_empty, s_full[4], p_full[4], pv_done[2], o_full[2], exchanged, drained[2], turn[2][4];
   uint64_t piece_full[kPieces], piece_empty[kPieces];
   tree_piece pieces[kPieces];
-  uint32_t valid[kInfos][4], bad[kInfos][4];
+  uint4 valid[kInfos];  // of the four warps that copy: which keys are there
+  uint4 bad[kInfos];    // whether values are no numbers
   float2 stats[2][128];
   uint32_t tmem, failed;
 };
@@ -107,23 +109,30 @@ struct piece_reader {
   }
 };
 
-// Of a piece's 2 n tiles in the order in which they are copied and wanted -- K0 K1 V0 K2 V1 .. -- the place of tile j's values.
-__device__ __forceinline__ uint32_t values_at(uint32_t j, uint32_t n) { return j + 1 < n ? 2 * j + 2 : 2 * n - 1; }
-
-// Whether all rows that are there see all keys of the tile that are there.
-template <int TILE>
+// Whether a tile has keys that not all rows see.
 __device__ __forceinline__ bool is_mixed(const tree_view& t, const tree_piece& p, uint32_t base)
 {
-  return int64_t(base) + TILE > int64_t(p.length) || (t.window > 0 && int64_t(base) <= int64_t(p.latest) - t.window);
+  return int64_t(base) + kTile > int64_t(p.length) || (t.window > 0 && int64_t(base) <= int64_t(p.latest) - t.window);
 }
+
+// Tiles whose scores are wanted ahead: two of each stream.
+__device__ __forceinline__ uint32_t lead_of(bool alternate) { return alternate ? 4u : 2u; }
 
 // ---- copying ------------------------------------------------------------------------------------------------------------------
 
+// This thread's arrival, once its copies so far are there.
+__device__ __forceinline__ void arrive_behind_copies(uint64_t& bar)
+{
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&bar)) : "memory");
+}
+
+// The warps that copy never wait for their own copies: a tile's barrier counts them as they arrive, and the warp that multiplies orders them before what
+// the tensor core reads.  (A proxy fence by the warps that copy waited for all of their copies in flight: 2.5 us a tile.)
 template <typename T, int D>
-__device__ __forceinline__ void copy_role(const tc_args& a, tc_shared& sh, char* smem, const waiter& wait, uint32_t which, uint32_t block)
+__device__ __forceinline__ void copy_role(const tc_args& a, tc_shared& sh, char* smem, const waiter& wait, uint32_t block)
 {
   using shape                = tc_shape<D>;
-  constexpr uint32_t TILE    = shape::kTile, ROWS = TILE / 4, PR = D / 8, AT_ONCE = 32 / PR > 0 ? 32 / PR : 1, NB = shape::kStages, BEHIND = shape::kBehind;
+  constexpr uint32_t ROWS = kTile / 4, PR = D / 8, AT_ONCE = 32 / PR, NB = shape::kStages;
   const cache_view& c        = a.c;
   const tree_view& t         = a.t;
   const uint32_t warp        = (threadIdx.x >> 5) & 3u, lane = threadIdx.x & 31u;
@@ -133,99 +142,99 @@ __device__ __forceinline__ void copy_role(const tc_args& a, tc_shared& sh, char*
   const uint32_t row0        = block * shape::kRows, rows = min(uint32_t(shape::kRows), t.n_rows - row0);
   const uint32_t column_from = piece < pieces ? piece * 16 : 0u;
   const uint32_t column_to   = (piece >> 3) * shape::kPanel;
-  uint32_t it = 0, sent = 0, tiles = 0, q_turn = 0;
-  uint64_t scan = 0;  // 4 bits for each place of the ring: 1 + which info, if the values there have to be looked at
-  auto send = [&](uint32_t i) {
-    const uint32_t slot = i % NB, info = uint32_t(scan >> (4 * slot)) & 15u;
-    if (info != 0u) {
+  const bool alternate       = shape::kTwo && rows <= 128;
+  const uint32_t lead        = lead_of(alternate);
+  // tiles begin at multiples of 16 positions
+  const bool together        = c.page.size % ROWS == 0;
+  const uint64_t k_on = uint64_t(c.k_token_units * AT_ONCE) << c.unit_shift, v_on = uint64_t(c.v_token_units * AT_ONCE) << c.unit_shift;
+  uint32_t it = 0, tiles = 0, q_turn = 0;
+  // The rows of one tile, of which this lane knows the place of one.  `on`: bytes from a lane's row to its next in a page; `look`: values that are to be looked at, for info `info`.
+  auto copy = [&](const char* from, uint32_t at, uint32_t there, uint64_t on, bool look, uint32_t info) -> bool {
+    const uint32_t slot = it % NB;
+    if (it >= NB && !wait(sh.empty[slot], it / NB - 1)) { return false; }
+    const uint32_t to = ring + slot * shape::kTileBytes + column_to;
+    if (together && there == 0xFFFFu) {
+      // all of the warp's rows are there and in one page, one behind the other
+      const char* row_from    = from + (uint64_t(__shfl_sync(kAllLanes, at, sub)) << c.unit_shift);
+      const uint32_t to_piece = to + (warp * ROWS + sub) * 128, bytes = piece < pieces ? 16u : 0u;
+#pragma unroll
+      for (uint32_t i = 0; i < ROWS / AT_ONCE; i++) {
+        if (piece < wide) { copy_piece(to_piece + i * (AT_ONCE * 128) + (((piece ^ sub ^ (i * AT_ONCE)) & 7u) << 4), row_from, bytes); }
+        row_from += on;
+      }
+    } else {
+#pragma unroll
+      for (uint32_t i = 0; i < ROWS / AT_ONCE; i++) {
+        const uint32_t r = i * AT_ONCE + sub, row = warp * ROWS + r;
+        const uint32_t place = __shfl_sync(kAllLanes, at, r);
+        const uint32_t bytes = piece < pieces && ((there >> r) & 1u) != 0u ? 16u : 0u;
+        if (piece < wide) { copy_piece(to + row * 128 + (((piece & 7u) ^ (row & 7u)) << 4), from + (uint64_t(place) << c.unit_shift), bytes); }
+      }
+    }
+    if (look) {
+      copies_end_group();
+      copies_wait<0>();
       bool bad = false;
-      for (uint32_t r = sub; r < ROWS; r += AT_ONCE) {
-        if (piece >= wide || sub >= AT_ONCE) { break; }
+      for (uint32_t r = sub; r < ROWS && piece < wide; r += AT_ONCE) {
         const uint32_t row = warp * ROWS + r;
         const uint4 x = *reinterpret_cast<const uint4*>(smem + shape::kRingAt + slot * shape::kTileBytes + column_to + row * 128 +
                                                         (((piece & 7u) ^ (row & 7u)) << 4));
         constexpr uint32_t kAll = std::is_same<T, __half>::value ? 0x7C00u : 0x7F80u;
         const uint32_t words[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-          bad = bad || (words[e] & kAll) == kAll || ((words[e] >> 16) & kAll) == kAll;
-        }
+        for (int e = 0; e < 4; e++) { bad = bad || (words[e] & kAll) == kAll || ((words[e] >> 16) & kAll) == kAll; }
       }
-      if (__any_sync(kAllLanes, bad) && lane == 0) { sh.bad[info - 1][warp] = 1u; }
-      scan &= ~(uint64_t(15) << (4 * slot));
+      if (__any_sync(kAllLanes, bad) && lane == 0) { reinterpret_cast<uint32_t*>(&sh.bad[info])[warp] = 1u; }
+      __syncwarp();
     }
-    fence_async_smem();
-    arrive_warp(sh.full[slot]);
-  };
-  auto flush = [&] {
-    copies_wait<0>();
-    for (; sent < it; sent++) { send(sent); }
-  };
-  // The rows of one tile, of which this lane knows the place of one.
-  auto copy = [&](const char* from, uint32_t at, uint32_t there) -> bool {
-    if (it >= NB && !wait(sh.empty[it % NB], it / NB - 1)) { return false; }
-    const uint32_t to = ring + (it % NB) * shape::kTileBytes + column_to;
-#pragma unroll
-    for (uint32_t i = 0; i < ROWS / AT_ONCE; i++) {
-      const uint32_t r = i * AT_ONCE + sub, row = warp * ROWS + r;
-      const uint32_t place = __shfl_sync(kAllLanes, at, r);
-      const uint32_t bytes = piece < pieces && ((there >> r) & 1u) != 0u ? 16u : 0u;
-      if (piece < wide) { copy_piece(to + row * 128 + (((piece & 7u) ^ (row & 7u)) << 4), from + (uint64_t(place) << c.unit_shift), bytes); }
-    }
-    copies_end_group();
+    arrive_behind_copies(sh.full[slot]);
+    arrive_warp(sh.full[slot]);  // what the warp wrote itself
     it++;
-    copies_wait<BEHIND>();
-    if (it > BEHIND && sent < it - BEHIND) { send(sent++); }
     return true;
   };
 
   piece_reader reader;
   tree_piece p;
   while (reader.next(sh, wait, p)) {
-    const uint32_t n        = p.end - p.chunk;
-    const int32_t* table    = a.pages + int64_t(p.sequence) * a.table_stride;
+    const uint32_t n         = p.end - p.chunk;
+    const int32_t* table     = a.pages + int64_t(p.sequence) * a.table_stride;
     const int32_t* positions = t.positions + int64_t(p.sequence) * t.positions_stride;
-    const char* keys        = c.keys + int64_t(p.head) * c.k_head * 2 + column_from;
-    const char* values      = c.values + int64_t(p.head) * c.v_head * 2 + column_from;
-    // queries: they may be replaced once the last scores of the piece before are there
-    if (q_turn > 0) {
-      flush();
-      if (!wait(sh.q_empty, q_turn - 1)) { break; }
-    }
-    const uint32_t q_rows = rows <= 128 ? 128 : 256;
-    for (uint32_t r0 = warp * 32; r0 < q_rows; r0 += 128) {
-      const uint32_t mine = r0 + lane, r = row0 + min(mine, rows - 1u), token = r / t.group, g = r - token * t.group;
-      const char* from = t.queries.data + (int64_t(p.sequence) * t.queries.sequence + int64_t(token) * t.queries.token +
-                                           int64_t(p.head * t.group + g) * t.queries.head) * 2;
-      for (uint32_t i = 0; i < 32; i += AT_ONCE) {
-        const uint32_t row  = r0 + i + sub;
-        const uint64_t at   = __shfl_sync(kAllLanes, reinterpret_cast<uint64_t>(from), (i + sub) & 31u);
-        const uint32_t to   = q_at + (row >> 7) * shape::kQBytes + (piece >> 3) * shape::kQPanel + (row & 127u) * 128 + (((piece & 7u) ^ (row & 7u)) << 4);
-        if (piece < wide) { copy_piece(to, reinterpret_cast<const char*>(at) + column_from, piece < pieces && row < rows ? 16u : 0u); }
-      }
-    }
-    copies_end_group();
-    copies_wait<0>();
-    fence_async_smem();
-    arrive_warp(sh.q_full);
-    q_turn++;
-
+    const char* keys         = c.keys + int64_t(p.head) * c.k_head * 2 + column_from;
+    const char* values       = c.values + int64_t(p.head) * c.v_head * 2 + column_from;
     // what the table says about this lane's key of a tile, asked for a tile ahead
     const uint32_t own_row = warp * ROWS + lane % ROWS;
     auto name = [&](uint32_t tile) -> int32_t {
-      const uint32_t at = p.base + tile * TILE + own_row;
+      const uint32_t at = p.base + tile * kTile + own_row;
       if (tile >= p.end || at < p.first || at >= p.last) { return -1; }
       uint32_t column, place;
       split_place(at, c.page, column, place);
       return table[column];  // at < last: the column is inside the table
     };
     int32_t next = name(p.chunk);
-    uint32_t v_at = 0, v_there = 0;  // of the tile before
+    // queries: they may be replaced once the last scores of the piece before are there
+    if (q_turn > 0 && !wait(sh.q_empty, q_turn - 1)) { break; }
+    const uint32_t q_rows = rows <= 128 ? 128 : 256;
+    for (uint32_t r0 = warp * 32; r0 < q_rows; r0 += 128) {
+      const uint32_t mine = r0 + lane, r = row0 + min(mine, rows - 1u), token = r / t.group, g = r - token * t.group;
+      const char* from = t.queries.data + (int64_t(p.sequence) * t.queries.sequence + int64_t(token) * t.queries.token +
+                                           int64_t(p.head * t.group + g) * t.queries.head) * 2;
+#pragma unroll 4
+      for (uint32_t i = 0; i < 32; i += AT_ONCE) {
+        const uint32_t row  = r0 + i + sub;
+        const uint64_t at   = __shfl_sync(kAllLanes, reinterpret_cast<uint64_t>(from), i + sub);
+        const uint32_t to   = q_at + (row >> 7) * shape::kQBytes + (piece >> 3) * shape::kQPanel + (row & 127u) * 128 + (((piece & 7u) ^ (row & 7u)) << 4);
+        if (piece < wide) { copy_piece(to, reinterpret_cast<const char*>(at) + column_from, piece < pieces && row < rows ? 16u : 0u); }
+      }
+    }
+    arrive_behind_copies(sh.q_full);
+    q_turn++;
+
+    // Keys come `lead` - 1 tiles before their values, whose places have been found with theirs.
+    uint32_t v_at[4] = {0, 0, 0, 0}, v_there[4] = {0, 0, 0, 0};
     bool ok = true;
-    for (uint32_t j = 0; j <= n && ok; j++) {
-      uint32_t k_at = 0, this_v_at = 0, this_there = 0;
+    for (uint32_t j = 0; j < n + lead - 1 && ok; j++) {
       if (j < n) {
-        const uint32_t base = p.base + (p.chunk + j) * TILE, at = base + own_row;
+        const uint32_t base = p.base + (p.chunk + j) * kTile, at = base + own_row;
         const int32_t page  = next;
         next                = name(p.chunk + j + 1);
         uint32_t column, place;
@@ -239,157 +248,189 @@ __device__ __forceinline__ void copy_role(const tc_args& a, tc_shared& sh, char*
           const int32_t of = positions[at - p.length];
           there            = of >= 0 && uint32_t(of) >= p.length;
         }
-        k_at       = there ? uint32_t(page) * c.k_page_units + place * c.k_token_units : 0u;
-        this_v_at  = there ? uint32_t(page) * c.v_page_units + place * c.v_token_units : 0u;
-        this_there = __ballot_sync(kAllLanes, there);
-        const uint32_t info = tiles % kInfos;
+        const uint32_t k_at = there ? uint32_t(page) * c.k_page_units + place * c.k_token_units : 0u;
+        const uint32_t rows_there = __ballot_sync(kAllLanes, there) & 0xFFFFu;
+        v_at[0]    = there ? uint32_t(page) * c.v_page_units + place * c.v_token_units : 0u;
+        v_there[0] = rows_there;
+        const uint32_t info = tiles++ % kInfos;
         if (lane == 0) {
-          sh.valid[info][warp] = ROWS == 32 ? this_there : this_there & 0xFFFFu;
-          sh.bad[info][warp]   = 0u;
+          reinterpret_cast<uint32_t*>(&sh.valid[info])[warp] = rows_there;
+          reinterpret_cast<uint32_t*>(&sh.bad[info])[warp]   = 0u;
         }
-        tiles++;
-        ok = copy(keys, k_at, this_there);
+        __syncwarp();
+        ok = copy(keys, k_at, rows_there, k_on, false, 0);
       }
-      // tile j's keys come before tile j - 1's values, which have been named together
-      if (j > 0 && ok) {
-        const uint32_t base = p.base + (p.chunk + j - 1) * TILE;
-        if (is_mixed<TILE>(t, p, base)) {
-          const uint32_t info = (tiles - (j < n ? 2 : 1)) % kInfos;
-          scan |= uint64_t(info + 1) << (4 * (it % NB));
-        }
-        ok = copy(values, v_at, v_there);
+      if (j + 1 >= lead && ok) {
+        const uint32_t of = j + 1 - lead;
+        ok = copy(values, alternate ? v_at[3] : v_at[1], alternate ? v_there[3] : v_there[1], v_on, is_mixed(t, p, p.base + (p.chunk + of) * kTile),
+                  (tiles - min(j + 1, n) + of) % kInfos);
       }
-      v_at    = this_v_at;
-      v_there = this_there;
+#pragma unroll
+      for (int i = 3; i > 0; i--) {
+        v_at[i]    = v_at[i - 1];
+        v_there[i] = v_there[i - 1];
+      }
     }
     if (!ok) { break; }
   }
-  flush();
+  copies_end_group();
+  copies_wait<0>();
 }
 
 // ---- multiplying --------------------------------------------------------------------------------------------------------------
 
+// One warp for each stream: what a warp has to wait for and to look up between its products would leave the tensor core idle (with one warp for
+// both streams 3,000 clocks for 64 keys of 2 x 128 rows, of which the products are 1,800).
 template <typename T, int D>
-__device__ __forceinline__ void multiply_role(const tc_args& a, tc_shared& sh, char* smem, const waiter& wait, uint32_t block)
+__device__ __forceinline__ void multiply_role(const tc_args& a, tc_shared& sh, char* smem, const waiter& wait, uint32_t block, uint32_t stream)
 {
   using shape              = tc_shape<D>;
-  constexpr uint32_t TILE  = shape::kTile, NB = shape::kStages;
+  constexpr uint32_t NB    = shape::kStages;
   constexpr uint32_t kType = std::is_same<T, __half>::value ? 0u : 1u;
-  const uint32_t tmem      = sh.tmem;
   const uint32_t rows      = min(uint32_t(shape::kRows), a.t.n_rows - block * shape::kRows);
   const bool both          = shape::kTwo && rows > 128;  // two blocks of rows on the same tiles
+  const bool alternate     = shape::kTwo && !both;
+  const uint32_t lead      = lead_of(alternate);
   const uint32_t steps     = (a.c.dim + 15) / 16;
-  const uint32_t qk        = (1u << 4) | (kType << 7) | (kType << 10) | ((TILE >> 3) << 17) | ((128u >> 4) << 24);
+  const uint32_t qk        = (1u << 4) | (kType << 7) | (kType << 10) | ((kTile >> 3) << 17) | ((128u >> 4) << 24);
   const uint32_t pv        = (1u << 4) | (kType << 7) | (kType << 10) | (1u << 16) | (((steps * 16) >> 3) << 17) | ((128u >> 4) << 24);
-  const uint32_t q_at = smem_u32(smem), ring = smem_u32(smem + shape::kRingAt);
-  auto scores_at = [&](uint32_t s) { return tmem + s * TILE; };
-  auto sums_at   = [&](uint32_t s) { return tmem + shape::kSumsAt + (shape::kTwo ? s * 128 : 0); };
-  auto scores = [&](uint32_t slot, uint32_t s) {
-    const uint32_t from = ring + slot * shape::kTileBytes, q = q_at + (both ? s * shape::kQBytes : 0u);
-    if (elect_one()) {
-      for (uint32_t k = 0; k < steps; k++) {
-        const uint32_t panel = k >> 2, in = (k & 3u) * 32;
-        tc_mma_f16(scores_at(s), make_desc_sw128(q + panel * shape::kQPanel + in), make_desc_sw128(from + panel * shape::kPanel + in), qk, k != 0u);
-      }
-      tc_commit(smem_u32(&sh.s_full[s]));
-    }
-    __syncwarp();
-  };
-  auto sums = [&](uint32_t slot, uint32_t s, bool add) {
-    const uint32_t from = ring + slot * shape::kTileBytes;
-    if (elect_one()) {
-#pragma unroll 1
-      for (uint32_t part = 0; part < 2; part++) {
-        for (uint32_t k = 0; k < TILE / 16; k++) {
-          tc_mma_f16_ts(sums_at(s), scores_at(s) + part * (TILE / 2) + k * 8, make_desc_sw128_rows(from + k * 2048, shape::kPanel), pv,
-                        add || (part | k) != 0u);
-        }
-      }
-    }
-    __syncwarp();
-  };
-  auto commit = [&](uint64_t& bar) {
-    if (elect_one()) { tc_commit(smem_u32(&bar)); }
-    __syncwarp();
-  };
+  const uint32_t tmem      = __shfl_sync(kAllLanes, sh.tmem, 0);
+  const uint32_t scores_at = tmem + stream * (2 * kTile), sums_at = tmem + shape::kSumsAt + stream * 128;
+  const uint32_t q_lo      = desc_sw128_lo(smem_u32(smem)) + (both ? stream * (shape::kQBytes >> 4) : 0u);
+  const uint32_t ring_lo   = desc_sw128_lo(smem_u32(smem + shape::kRingAt));
+  const uint32_t v_lo      = (smem_u32(smem + shape::kRingAt) >> 4) | (uint32_t(shape::kPanel >> 4) << 16);
 
   piece_reader reader;
   tree_piece p;
-  uint32_t it = 0, tiles = 0, q_turn = 0, p_turn[2] = {0, 0};
-  auto next_full = [&](uint32_t& slot) {
-    slot          = it % NB;
-    const bool ok = wait(sh.full[slot], it / NB);
-    it++;
-    return ok;
-  };
+  uint32_t items = 0, tiles = 0, q_turn = 0, p_turn = 0;  // p_turn: a bit for each buffer
   while (reader.next(sh, wait, p)) {
-    const uint32_t n = p.end - p.chunk;
-    uint32_t slot;
+    const uint32_t n   = p.end - p.chunk;
+    const uint32_t own = alternate ? (n + 1 - stream) / 2 : n;  // tiles of this stream
     if (!wait(sh.q_full, q_turn++)) { break; }
-    tc_fence_after();
-    bool ok = true;
-    // the first scores
-    for (uint32_t s = 0; s < (both || n < 2 ? 1u : 2u) && ok; s++) {
-      ok = next_full(slot);
-      if (!ok) { break; }
-      scores(slot, s);
-      if (both) { scores(slot, 1); }
-      commit(sh.empty[slot]);
+    // The tile of a place in the ring.  (A stream that passes over the other's tiles has seen one of its own that came at most nine places before:
+    // copies arrive in their order, so the barrier is at most one phase behind.)
+    auto arrived = [&](uint32_t item, uint32_t& slot) {
+      slot          = item % NB;
+      const bool ok = wait(sh.full[slot], item / NB);
+      fence_async_smem();  // what was copied, before what the tensor core reads
+      return ok;
+    };
+    auto scores = [&](uint32_t i) {
+      const uint32_t j = alternate ? 2 * i + stream : i;
+      uint32_t slot;
+      if (!arrived(items + (j < lead ? j : 2 * j + 1 - lead), slot)) { return false; }
+      const uint32_t from = ring_lo + slot * (shape::kTileBytes >> 4), to = scores_at + (i & 1u) * kTile;
+      if (elect_one()) {
+        tc_mma_f16_lo<false>(to, q_lo, from, qk);
+#pragma unroll
+        for (uint32_t k = 1; k < D / 16; k++) {
+          if (k < steps) {
+            tc_mma_f16_lo<true>(to, q_lo + ((k >> 2) * shape::kQPanel + (k & 3u) * 32) / 16, from + ((k >> 2) * shape::kPanel + (k & 3u) * 32) / 16, qk);
+          }
+        }
+        tc_commit(smem_u32(&sh.s_full[stream * 2 + (i & 1u)]));
+        tc_commit(smem_u32(&sh.empty[slot]));
+        if (i + 1 == own) { tc_commit(smem_u32(&sh.q_empty)); }
+      }
+      __syncwarp();
+      return true;
+    };
+    if (own == 0) {  // nothing for this stream, but the queries may be replaced
+      if (elect_one()) { tc_commit(smem_u32(&sh.q_empty)); }
+      __syncwarp();
     }
-    if (n == 1 || (n == 2 && !both)) { commit(sh.q_empty); }
-    for (uint32_t j = 0; j < n && ok; j++) {
-      uint32_t k_slot = 0, v_slot = 0;
-      const bool more = j + (both ? 1 : 2) < n;
-      if (both) {
-        // the next tile's keys stand before this one's values in the ring
-        if (more && !next_full(k_slot)) { ok = false; break; }
-        if (!next_full(v_slot)) { ok = false; break; }
-      } else if (!next_full(v_slot)) {
-        ok = false;
-        break;
-      }
-      const uint32_t info = (tiles + j) % kInfos;
-      for (uint32_t s = both ? 0u : (j & 1u); s < (both ? 2u : (j & 1u) + 1u); s++) {
-        if (!wait(sh.p_full[s], p_turn[s]++)) { ok = false; break; }
-        tc_fence_after();
-        // where values are no numbers the threads of the rows have added them up themselves
-        const volatile uint32_t* b = sh.bad[info];
-        if ((b[0] | b[1] | b[2] | b[3]) == 0u) { sums(v_slot, s, shape::kTwo && !both ? j > 1 : j > 0); }
-        if constexpr (!shape::kTwo) { commit(sh.pv_done); }
-        if (both) {
-          if (more) { scores(k_slot, s); }
-          if (j + 1 == n) { commit(sh.o_full[s]); }
-        } else if constexpr (shape::kTwo) {
-          if (!more) { commit(sh.o_full[s]); }
-        } else {
-          if (j + 1 == n) { commit(sh.o_full[0]); }
+    bool ok = own < 1 || scores(0);
+    ok      = ok && (own < 2 || scores(1));
+    for (uint32_t i = 0; i < own && ok; i++) {
+      const uint32_t j = alternate ? 2 * i + stream : i, buffer = i & 1u;
+      uint32_t slot;
+      if (!arrived(items + min(n, j + lead) + j, slot)) { ok = false; break; }
+      // where values are no numbers the threads of the rows add them up themselves
+      const uint4 bad = sh.bad[(tiles + j) % kInfos];
+      const bool good = (bad.x | bad.y | bad.z | bad.w) == 0u;
+      if (!wait(sh.p_full[stream * 2 + buffer], p_turn >> buffer)) { ok = false; break; }
+      p_turn ^= 1u << buffer;
+      tc_fence_after();
+      if (elect_one()) {
+        if (good) {
+          // 32 keys of weights stand where their scores stood: 16 columns of the first numbers, 16 of the second
+          const uint32_t from = v_lo + slot * (shape::kTileBytes >> 4), w = scores_at + buffer * kTile;
+#pragma unroll
+          for (uint32_t k = 0; k < kTile / 16; k++) {
+            const uint32_t at = w + (k >> 1) * 32 + (k & 1u) * 8;
+            tc_mma_f16_ts(sums_at, at, from + k * (2048 >> 4), pv, k != 0u || i > 0);
+            tc_mma_f16_ts(sums_at, at + 16, from + k * (2048 >> 4), pv, true);
+          }
         }
+        tc_commit(smem_u32(&sh.pv_done[stream]));
+        tc_commit(smem_u32(&sh.empty[slot]));
+        if (i + 1 == own) { tc_commit(smem_u32(&sh.o_full[stream])); }
       }
-      if (!ok) { break; }
-      commit(sh.empty[v_slot]);
-      if (more) {
-        if (!both) {
-          if (!next_full(k_slot)) { ok = false; break; }
-          scores(k_slot, j & 1u);
-        }
-        commit(sh.empty[k_slot]);
-        if (j + (both ? 2 : 3) == n) { commit(sh.q_empty); }
-      }
+      __syncwarp();
+      if (i + 2 < own) { ok = scores(i + 2); }
     }
     if (!ok) { break; }
     tiles += n;
+    items += 2 * n;
   }
-  commit(sh.drained);
-  wait(sh.drained, 0);
+  if (elect_one()) { tc_commit(smem_u32(&sh.drained[stream])); }
+  __syncwarp();
+  wait(sh.drained[stream], 0);
 }
 
 // ---- softmax ------------------------------------------------------------------------------------------------------------------
+
+// 32 scores from key `at` on, in powers of two: scaled, capped, less what their distance costs.  They stand at `scores` in tensor memory.
+__device__ __forceinline__ void shape_scores(const tree_view& t, const tree_piece& p, const int32_t* positions, int32_t own, float slope, uint32_t at,
+                                             bool mixed, uint32_t scores, uint32_t (&x)[32])
+{
+  if (t.cap_log2 != 0.0f) {
+    const two by(t.scale_cap, t.scale_cap);
+    float most = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 32; k += 2) {
+      const two y = mul2(two(__uint_as_float(x[k]), __uint_as_float(x[k + 1])), by);
+      float u, v;
+      y.get(u, v);
+      most = fmaxf(most, fmaxf(fabsf(u), fabsf(v)));
+      tanh_near(y, t.cap_near).get(u, v);
+      x[k]     = __float_as_uint(u);
+      x[k + 1] = __float_as_uint(v);
+    }
+    if (__any_sync(kAllLanes, !(most < kTanhNear))) {  // seldom: once more, the long way
+      uint32_t y[32];
+      tmem_ld32(scores, y);
+#pragma unroll
+      for (int k = 0; k < 32; k++) {
+        const float z = __uint_as_float(y[k]) * t.scale_cap;
+        x[k]          = fabsf(z) < kTanhNear ? x[k] : __float_as_uint(tanh_far(z) * t.cap_log2);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 32; k++) { x[k] = __float_as_uint(__uint_as_float(x[k]) * t.scale_log2); }
+  }
+  if (t.slopes != nullptr) {
+    const float from = float(int64_t(at) - own);
+    if (!mixed) {
+#pragma unroll
+      for (int k = 0; k < 32; k++) { x[k] = __float_as_uint(fmaf(slope, from + float(k), __uint_as_float(x[k]))); }
+    } else {
+#pragma unroll
+      for (int k = 0; k < 32; k++) {
+        const int64_t drafted = int64_t(at) + k - int64_t(p.length);
+        const float distance  = drafted >= 0 && drafted < int64_t(t.n_drafted) ? float(int64_t(positions[drafted]) - own) : from + float(k);
+        x[k]                  = __float_as_uint(fmaf(slope, distance, __uint_as_float(x[k])));
+      }
+    }
+  }
+}
 
 template <typename T, int D, bool SHAPED>
 __device__ __forceinline__ void softmax_role(const tc_args& a, tc_shared& sh, char* smem, const waiter& wait, uint32_t which, uint32_t block)
 {
   using shape             = tc_shape<D>;
-  constexpr uint32_t TILE = shape::kTile, NB = shape::kStages, GROUPS = TILE / 32;
+  constexpr uint32_t NB = shape::kStages;
   const tree_view& t      = a.t;
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, stream = warp >> 2, quarter = warp & 3u;
   const uint32_t row0 = block * shape::kRows, rows = min(uint32_t(shape::kRows), t.n_rows - row0);
@@ -398,13 +439,17 @@ __device__ __forceinline__ void softmax_role(const tc_args& a, tc_shared& sh, ch
   const uint32_t in    = quarter * 32 + lane, r = both ? stream * 128 + in : in;
   const bool exists    = r < rows;
   const uint32_t row   = row0 + min(r, rows - 1u), token = row / t.group, g = row - token * t.group;
+  const int64_t out_at = int64_t(token) * t.out.token + int64_t(g) * t.out.head;  // of this row, in its sequence and key head
   const bool alive     = __any_sync(kAllLanes, exists);
   const uint32_t lanes = quarter << 21;  // this warp's lanes of tensor memory
-  const uint32_t sums  = sh.tmem + lanes + shape::kSumsAt + (shape::kTwo ? stream * 128 : 0);
+  const uint32_t lead  = lead_of(alternate);
+  const uint32_t sh_tmem = sh.tmem;
+  const uint32_t sums  = sh_tmem + lanes + shape::kSumsAt + (shape::kTwo ? stream * 128 : 0);
   const uint32_t width = (a.c.dim + 31) / 32;  // columns of the sums, in 32
   piece_reader reader;
   tree_piece p;
-  uint32_t s_turn[2] = {0, 0}, o_turn = 0, x_turn = 0, tiles = 0, items = 0, pv_turn = 0;
+  const bool in_turns = both && 128 + quarter * 32 < rows;  // both streams' warps of this quarter have rows
+  uint32_t e_turn = 0, s_turn = 0, o_turn = 0, x_turn = 0, tiles = 0, items = 0, pv_turn = 0;  // s_turn: a bit for each buffer
 
   while (reader.next(sh, wait, p)) {
     const uint32_t n = p.end - p.chunk;
@@ -417,98 +462,51 @@ __device__ __forceinline__ void softmax_role(const tc_args& a, tc_shared& sh, ch
     if (SHAPED && t.slopes != nullptr) { slope = t.slopes[p.head * t.group + g] * kLog2E; }
     float top = -INFINITY, sum = 0.0f;
     drafted_lists::list l{p.length, p.first, p.last, p.base};
+    // tiles that not all rows see whole: from `tail_from` on, and up to `edge_to`
+    const int32_t tail_from = int32_t((int64_t(p.length) - int64_t(p.base)) >> 6);
+    const int32_t edge_to   = t.window > 0 ? int32_t((int64_t(p.latest) - t.window - int64_t(p.base)) >> 6) : -1;
     uint32_t done = 0;  // tiles of this stream
     bool ok = true;
     for (uint32_t j = alternate ? stream : 0u; j < n; j += alternate ? 2u : 1u, done++) {
-      const uint32_t buffer = shape::kTwo ? stream : (j & 1u);
-      const uint32_t scores = sh.tmem + lanes + buffer * TILE;
-      if (!wait(sh.s_full[buffer], s_turn[buffer]++)) { ok = false; break; }
+      const uint32_t buffer = stream * 2 + (done & 1u);
+      const uint32_t scores = sh_tmem + lanes + buffer * kTile;
+      if (!wait(sh.s_full[buffer], s_turn >> (done & 1u))) { ok = false; break; }
+      s_turn ^= 1u << (done & 1u);
       tc_fence_after();
       if (!alive) {
         arrive_warp(sh.p_full[buffer]);
         continue;
       }
-      uint32_t raw[GROUPS][32];
-#pragma unroll
-      for (uint32_t i = 0; i < GROUPS; i++) { tmem_ld32_async(scores + i * 32, raw[i]); }
-      const uint32_t base = p.base + (p.chunk + j) * TILE, info = (tiles + j) % kInfos;
-      const bool mixed    = is_mixed<int(TILE)>(t, p, base);
-      uint32_t seen[GROUPS];
-#pragma unroll
-      for (uint32_t i = 0; i < GROUPS; i++) {
-        if constexpr (TILE == 128) {
-          seen[i] = sh.valid[info][i];
-        } else {
-          seen[i] = sh.valid[info][2 * i] | (sh.valid[info][2 * i + 1] << 16);
-        }
-        if (!is_token) { seen[i] = 0u; }
-        if (mixed && is_token) { seen[i] &= seen_keys(t, l, positions, own, mask, base + i * 32); }
-      }
-      float s[GROUPS][32];
-#pragma unroll
-      for (uint32_t i = 0; i < GROUPS; i++) {
-        tmem_ld_wait(raw[i]);
-#pragma unroll
-        for (int k = 0; k < 32; k++) { s[i][k] = __uint_as_float(raw[i][k]); }
-      }
+      uint32_t x[2][32];
+      tmem_ld32_async(scores, x[0]);
+      tmem_ld32_async(scores + 32, x[1]);
+      const uint32_t info = (tiles + j) % kInfos, base = p.base + (p.chunk + j) * kTile;
+      const bool mixed    = int32_t(p.chunk + j) >= tail_from || int32_t(p.chunk + j) <= edge_to;
+      const uint4 valid   = sh.valid[info];
+      const bool whole    = (valid.x & valid.y & valid.z & valid.w) == 0xFFFFu && !mixed;
+      tmem_ld_wait(x[0]);
+      tmem_ld_wait(x[1]);
       if constexpr (SHAPED) {
-        if (t.cap_log2 != 0.0f) {
 #pragma unroll
-          for (uint32_t i = 0; i < GROUPS; i++) {
-            float most = 0.0f;
-#pragma unroll
-            for (int k = 0; k < 32; k++) {
-              s[i][k] *= t.scale_cap;
-              most = fmaxf(most, fabsf(s[i][k]));
-            }
-            if (__any_sync(kAllLanes, !(most < 0.6f))) {
-#pragma unroll
-              for (int k = 0; k < 32; k++) { s[i][k] = tanh_any(s[i][k]) * t.cap_log2; }
-            } else {
-#pragma unroll
-              for (int k = 0; k < 32; k++) { s[i][k] = tanh_near(s[i][k]) * t.cap_log2; }
-            }
-          }
-        } else {
-#pragma unroll
-          for (uint32_t i = 0; i < GROUPS; i++) {
-#pragma unroll
-            for (int k = 0; k < 32; k++) { s[i][k] *= t.scale_log2; }
-          }
-        }
-        if (t.slopes != nullptr) {
-          const float from = float(int64_t(base) - own);
-#pragma unroll
-          for (uint32_t i = 0; i < GROUPS; i++) {
-#pragma unroll
-            for (int k = 0; k < 32; k++) {
-              float distance = from + float(int(i) * 32 + k);
-              if (mixed) {
-                const int64_t drafted = int64_t(base) + int(i * 32 + k) - int64_t(p.length);
-                if (drafted >= 0 && drafted < int64_t(t.n_drafted)) { distance = float(int64_t(positions[drafted]) - own); }
-              }
-              s[i][k] = fmaf(slope, distance, s[i][k]);
-            }
-          }
-        }
+        for (uint32_t i = 0; i < 2; i++) { shape_scores(t, p, positions, own, slope, base + i * 32, mixed, scores + i * 32, x[i]); }
       }
-      bool whole = true;
+      if (!whole) {
 #pragma unroll
-      for (uint32_t i = 0; i < GROUPS; i++) { whole = whole && seen[i] == 0xFFFFFFFFu; }
-      if (!__all_sync(kAllLanes, whole)) {
+        for (uint32_t i = 0; i < 2; i++) {
+          uint32_t seen = i == 0 ? valid.x | valid.y << 16 : valid.z | valid.w << 16;
+          if (mixed) { seen &= seen_keys(t, l, positions, own, mask, base + i * 32); }
 #pragma unroll
-        for (uint32_t i = 0; i < GROUPS; i++) {
-#pragma unroll
-          for (int k = 0; k < 32; k++) { s[i][k] = ((seen[i] >> k) & 1u) != 0u ? s[i][k] : -INFINITY; }
+          for (int k = 0; k < 32; k++) { x[i][k] = ((seen >> k) & 1u) != 0u ? x[i][k] : 0xFF800000u; }
         }
+        __syncwarp();
       }
       float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (uint32_t i = 0; i < GROUPS; i++) {
+      for (uint32_t i = 0; i < 2; i++) {
 #pragma unroll
         for (int k = 0; k < 32; k += 4) {
 #pragma unroll
-          for (int e = 0; e < 4; e++) { most[e] = fmaxf(most[e], s[i][k + e]); }
+          for (int e = 0; e < 4; e++) { most[e] = fmaxf(most[e], __uint_as_float(x[i][k + e])); }
         }
       }
       float highest = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
@@ -518,52 +516,60 @@ __device__ __forceinline__ void softmax_role(const tc_args& a, tc_shared& sh, ch
         const float next = highest > top + kAhead ? highest : top;
         const float keep = top == -INFINITY ? 1.0f : power_of_2(top - next);
         if (done > 0 && __any_sync(kAllLanes, keep != 1.0f)) {
-          if constexpr (!shape::kTwo) {  // the tile before may still be added up
-            if (!wait(sh.pv_done, pv_turn + j - 1)) { ok = false; break; }
-            tc_fence_after();
-          }
+          // The tile before may still be added up.  (The one before that is: this tile's scores took the place of its weights.  So the barrier is at
+          // most one phase behind.)
+          if (!wait(sh.pv_done[stream], pv_turn + done - 1)) { ok = false; break; }
+          tc_fence_after();
+#pragma unroll 1
           for (uint32_t i = 0; i < width; i++) {
             uint32_t o[32];
             tmem_ld32(sums + i * 32, o);
-            uint32_t x[2][16];
 #pragma unroll
-            for (int k = 0; k < 32; k++) { x[k / 16][k % 16] = __float_as_uint(__uint_as_float(o[k]) * keep); }
-            tmem_st16(sums + i * 32, x[0]);
-            tmem_st16(sums + i * 32 + 16, x[1]);
+            for (int k = 0; k < 32; k++) { o[k] = __float_as_uint(__uint_as_float(o[k]) * keep); }
+            tmem_st32(sums + i * 32, o);
           }
           tmem_st_wait();
         }
         sum *= keep;
         top = next;
       }
-      const float from = a.shift - finite_top(top);
-      float part[4]    = {0.0f, 0.0f, 0.0f, 0.0f};
+      // Exponentials are what the two streams' warps of a scheduler share: they take turns at them, and do the rest meanwhile.
+      if (in_turns) {
+        if (!wait(sh.turn[stream][quarter], e_turn + 1 - stream)) { ok = false; break; }
+        e_turn++;
+      }
+      const float from = a.shift - finite_top(top), by = SHAPED ? 1.0f : t.scale_log2;
+      const two from2(from, from), by2(by, by);
+      two part[2] = {two(0.0f, 0.0f), two(0.0f, 0.0f)};
 #pragma unroll
-      for (uint32_t i = 0; i < GROUPS; i++) {
-        uint32_t high[16], low[16];
+      for (uint32_t i = 0; i < 2; i++) {
+        uint32_t pairs[32];
 #pragma unroll
         for (int k = 0; k < 32; k += 2) {
-          const float x = power_of_2(SHAPED ? s[i][k] + from : fmaf(s[i][k], t.scale_log2, from));
-          const float y = power_of_2(SHAPED ? s[i][k + 1] + from : fmaf(s[i][k + 1], t.scale_log2, from));
-          part[k & 2] += x;
-          part[(k & 2) + 1] += y;
-          weight_pair<T>::split(x, y, high[k / 2], low[k / 2]);
+          float u, v;
+          fma2(two(__uint_as_float(x[i][k]), __uint_as_float(x[i][k + 1])), by2, from2).get(u, v);
+          u = power_of_2(u);
+          v = power_of_2(v);
+          part[(k / 2) % 2] = add2(part[(k / 2) % 2], two(u, v));
+          weight_pair<T>::split(u, v, pairs[k / 2], pairs[16 + k / 2]);
         }
-        tmem_st16(scores + i * 16, high);
-        tmem_st16(scores + TILE / 2 + i * 16, low);
+        tmem_st32(scores + i * 32, pairs);
       }
-      sum += (part[0] + part[1]) + (part[2] + part[3]);
+      if (in_turns) { arrive_warp(sh.turn[1 - stream][quarter]); }
       tmem_st_wait();
+      {
+        float u, v;
+        add2(part[0], part[1]).get(u, v);
+        sum += u + v;
+      }
       if (mixed) {
         // Values that are no numbers must not reach rows that do not see them, as 0 times them would: each row adds up what it sees.
-        const uint32_t at = items + values_at(j, n), slot = at % NB;
+        const uint32_t at = items + min(n, j + lead) + j, slot = at % NB;  // in the order in which tiles are copied
         if (!wait(sh.full[slot], at / NB)) { ok = false; break; }
-        const volatile uint32_t* b = sh.bad[info];
-        if ((b[0] | b[1] | b[2] | b[3]) != 0u) {
-          if constexpr (!shape::kTwo) {
-            if (j > 0 && !wait(sh.pv_done, pv_turn + j - 1)) { ok = false; break; }
-            tc_fence_after();
-          }
+        const uint4 bad = sh.bad[info];
+        if ((bad.x | bad.y | bad.z | bad.w) != 0u) {
+          if (done > 0 && !wait(sh.pv_done[stream], pv_turn + done - 1)) { ok = false; break; }
+          tc_fence_after();
           const char* v = smem + shape::kRingAt + slot * shape::kTileBytes;
 #pragma unroll 1
           for (uint32_t i = 0; i < width; i++) {
@@ -575,13 +581,12 @@ __device__ __forceinline__ void softmax_role(const tc_args& a, tc_shared& sh, ch
               for (int k = 0; k < 32; k++) { o[k] = 0u; }
             }
 #pragma unroll 1
-            for (uint32_t k0 = 0; k0 < TILE; k0 += 32) {
-              uint32_t high[16], low[16];
-              tmem_ld16(scores + k0 / 2, high);
-              tmem_ld16(scores + TILE / 2 + k0 / 2, low);
+            for (uint32_t k0 = 0; k0 < kTile; k0 += 32) {
+              uint32_t pairs[32];
+              tmem_ld32(scores + k0, pairs);
 #pragma unroll
               for (uint32_t k = 0; k < 32; k++) {
-                const float2 pair = weight_pair<T>::join(high[k / 2], low[k / 2]);
+                const float2 pair = weight_pair<T>::join(pairs[k / 2], pairs[16 + k / 2]);
                 const float x     = (k & 1u) != 0u ? pair.y : pair.x;
                 if (x == 0.0f) { continue; }
                 const uint32_t key = k0 + k;
@@ -597,11 +602,7 @@ __device__ __forceinline__ void softmax_role(const tc_args& a, tc_shared& sh, ch
               }
               __syncwarp();
             }
-            uint32_t x[2][16];
-#pragma unroll
-            for (int k = 0; k < 32; k++) { x[k / 16][k % 16] = o[k]; }
-            tmem_st16(sums + i * 32, x[0]);
-            tmem_st16(sums + i * 32 + 16, x[1]);
+            tmem_st32(sums + i * 32, o);
           }
           tmem_st_wait();
         }
@@ -610,21 +611,27 @@ __device__ __forceinline__ void softmax_role(const tc_args& a, tc_shared& sh, ch
       arrive_warp(sh.p_full[buffer]);
     }
     if (!ok) { return; }
+    if (!is_token) {  // whatever stands in the sums of a row that is none
+      top = -INFINITY;
+      sum = 0.0f;
+    }
     tiles += n;
     items += 2 * n;
-    pv_turn += n;
-    if (done > 0 || (!alternate && n > 0)) {
-      if (!wait(sh.o_full[shape::kTwo ? stream : 0], o_turn++)) { return; }
+    pv_turn += done;
+    if (done > 0) {
+      if (!wait(sh.o_full[stream], o_turn++)) { return; }
       tc_fence_after();
     }
 
     const size_t part_of = a.parts.part(which, block, p.begins ? 1u : 0u);
+    T* const out         = reinterpret_cast<T*>(t.out.data) + int64_t(p.sequence) * t.out.sequence + out_at + int64_t(p.head * t.group) * t.out.head;
+    float4* const part   = a.parts.acc + part_of * a.parts.quads * a.parts.rows + r;
     auto write = [&](uint32_t quad, const float4& x, float scale) {  // four columns of this row
       if (!exists || quad * 4 >= a.c.dim) { return; }
       if (p.whole) {
-        store_quad<T>(out_row<T>(t, p.sequence, p.head, row) + quad * 4, make_float4(x.x * scale, x.y * scale, x.z * scale, x.w * scale));
+        store_quad<T>(out + quad * 4, make_float4(x.x * scale, x.y * scale, x.z * scale, x.w * scale));
       } else {
-        a.parts.acc[(part_of * a.parts.quads + quad) * a.parts.rows + r] = x;
+        part[quad * a.parts.rows] = x;
       }
     };
     auto finish = [&](float top_, float sum_) {
@@ -653,13 +660,13 @@ __device__ __forceinline__ void softmax_role(const tc_args& a, tc_shared& sh, ch
     } else {
       // Each of the two groups has the sums of every other tile; one finishes the first half of the columns, the other one the second.
       float4* room = reinterpret_cast<float4*>(smem + shape::kExchange);
-      constexpr uint32_t HALF = D / 64;  // 32 columns at a time
+      constexpr uint32_t SIDE = D / 64;  // 32 columns at a time
       sh.stats[stream][in] = make_float2(top, sum);
       float2 other;
       float own_keep = 0.0f, other_keep = 0.0f, joined_top = 0.0f, joined_sum = 0.0f, scale = 0.0f;
 #pragma unroll 1
-      for (uint32_t i = 0; i < HALF; i++) {
-        const uint32_t theirs = (1u - stream) * HALF + i, ours = stream * HALF + i;
+      for (uint32_t i = 0; i < SIDE; i++) {
+        const uint32_t theirs = (1u - stream) * SIDE + i, ours = stream * SIDE + i;
         uint32_t o[32];
         if (alive) {
           if (theirs < width) {
@@ -721,12 +728,10 @@ __device__ __forceinline__ void softmax_role(const tc_args& a, tc_shared& sh, ch
 
 // ---- the way ------------------------------------------------------------------------------------------------------------------
 
-template <int D>
 __device__ __forceinline__ void way_role(const tc_args& a, tc_shared& sh, const waiter& wait, uint32_t which, uint32_t block)
 {
-  constexpr int TILE  = tc_shape<D>::kTile;
   const uint32_t lane = threadIdx.x & 31u;
-  walk<TILE, drafted_lists> path(a.c, a.w, a.lists, a.parts.shares, which);
+  walk<int(kTile), drafted_lists> path(a.c, a.w, a.lists, a.parts.shares, which);
   piece now;
   uint4 begun = make_uint4(0, 0, 0, 0);
   uint32_t i  = 0;
@@ -745,14 +750,14 @@ __device__ __forceinline__ void way_role(const tc_args& a, tc_shared& sh, const 
       p.sequence = kNoMore;
       if (more) {
         p = {now.sequence, now.unit, now.chunk, now.end, path.l.length, path.l.first, path.l.end, path.l.base, latest, now.begins, now.whole};
-        if (now.begins && !now.whole) { begun = make_uint4(now.sequence, now.unit, now.n_parts, 0); }
+        if (now.begins) { note_begun(a.parts, now, a.c.n_heads, which, begun); }
       }
       sh.pieces[i % kPieces] = p;
     }
     arrive_warp(sh.piece_full[i % kPieces]);
     i++;
   }
-  if (a.parts.begun != nullptr && block == 0 && lane == 0) { a.parts.begun[which] = begun; }
+  if (a.parts.begun != nullptr && !a.parts.by_unit && block == 0 && lane == 0) { a.parts.begun[which] = begun; }
 }
 
 template <typename T, int D, bool SHAPED>
@@ -766,24 +771,30 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sh.tmem)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
+  const uint32_t which = blockIdx.x / a.t.n_blocks_of, block = blockIdx.x - which * a.t.n_blocks_of;
   if (threadIdx.x == 32) {
+    const bool both = shape::kTwo && a.t.n_rows - block * shape::kRows > 128;
     for (int i = 0; i < shape::kStages; i++) {
-      mbar_init(smem_u32(&sh.full[i]), 4);
-      mbar_init(smem_u32(&sh.empty[i]), 1);
+      mbar_init(smem_u32(&sh.full[i]), 128 + 4);
+      mbar_init(smem_u32(&sh.empty[i]), both ? 2 : 1);
     }
-    mbar_init(smem_u32(&sh.q_full), 4);
-    mbar_init(smem_u32(&sh.q_empty), 1);
-    for (int i = 0; i < 2; i++) {
+    mbar_init(smem_u32(&sh.q_full), 128);
+    mbar_init(smem_u32(&sh.q_empty), shape::kTwo ? 2 : 1);
+    for (int i = 0; i < 4; i++) {
       mbar_init(smem_u32(&sh.s_full[i]), 1);
       mbar_init(smem_u32(&sh.p_full[i]), 4);
-      mbar_init(smem_u32(&sh.o_full[i]), 1);
     }
-    mbar_init(smem_u32(&sh.pv_done), 1);
+    mbar_init(smem_u32(&sh.pv_done[0]), 1);
+    mbar_init(smem_u32(&sh.pv_done[1]), 1);
+    mbar_init(smem_u32(&sh.o_full[0]), 1);
+    mbar_init(smem_u32(&sh.o_full[1]), 1);
+    for (int i = 0; i < 8; i++) { mbar_init(smem_u32(&sh.turn[i / 4][i % 4]), 1); }
     mbar_init(smem_u32(&sh.exchanged), 8);
-    mbar_init(smem_u32(&sh.drained), 1);
+    mbar_init(smem_u32(&sh.drained[0]), 1);
+    mbar_init(smem_u32(&sh.drained[1]), 1);
     for (int i = 0; i < kPieces; i++) {
       mbar_init(smem_u32(&sh.piece_full[i]), 1);
-      mbar_init(smem_u32(&sh.piece_empty[i]), kReaders);
+      mbar_init(smem_u32(&sh.piece_empty[i]), shape::kTwo ? kReaders : kReaders - 1);
     }
     sh.failed = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -792,21 +803,22 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t which = blockIdx.x / a.t.n_blocks_of, block = blockIdx.x - which * a.t.n_blocks_of;
   const waiter wait{sh};
   if (warp < 8) {
-    registers_up<184>();
+    registers_up<168>();
     softmax_role<T, D, SHAPED>(a, sh, smem, wait, which, block);
   } else {
-    registers_down<72>();
+    registers_down<88>();  // 256 threads of 168 and 256 of 88: what the block was launched with
     if (warp < 12) {
-      copy_role<T, D>(a, sh, smem, wait, which, block);
+      copy_role<T, D>(a, sh, smem, wait, block);
     } else if (warp == 12) {
-      multiply_role<T, D>(a, sh, smem, wait, block);
+      multiply_role<T, D>(a, sh, smem, wait, block, 0);
     } else if (warp == 13) {
-      way_role<D>(a, sh, wait, which, block);
+      way_role(a, sh, wait, which, block);
+    } else if (warp == 14) {
+      if constexpr (shape::kTwo) { multiply_role<T, D>(a, sh, smem, wait, block, 1); }
     } else {
-      empty_tree_rows<T>(a.c, a.w.n_sequences, a.lists, a.t, threadIdx.x - 14 * 32, 64);
+      empty_tree_rows<T>(a.c, a.w.n_sequences, a.lists, a.t, a.parts, threadIdx.x - 15 * 32, 32);
     }
   }
   tc_fence_before();

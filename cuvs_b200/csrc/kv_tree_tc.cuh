@@ -6,48 +6,39 @@
 
 namespace cuvs_b200::kv {
 
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16])
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32])
 {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
-                 "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+  asm volatile(
+    "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+    "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+    "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]),
+    "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
+    "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+    : "memory");
+}
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8])
+{
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
                : "r"(taddr)
                : "memory");
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
   asm volatile("" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]));
-  asm volatile("" : "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]));
-}
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16])
-{
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::"r"(r[0]),
-               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]),
-               "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
-               : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// A row-block of weights in tensor memory times values: A [128 rows x 16 keys] from tensor memory.
-__device__ __forceinline__ void tc_mma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate)
+// A step of 16 keys: weights [128 rows x 16 keys] from tensor memory, and values by the low word of the descriptor of a tile whose rows are the
+// product's depth: 64 columns of 128 bytes, 128-byte swizzle, 8 rows 1024 bytes apart; bits 16 on of the word: the way to the next 64 columns.
+__device__ __forceinline__ void tc_mma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint32_t lo_b, uint32_t idesc, bool add)
 {
+  constexpr uint32_t kHi = (1024u >> 4) | (1u << 14) | (2u << 29);
   asm volatile(
-    "{\n\t.reg .pred p;\n\t"
-    "setp.ne.b32 p, %4, 0;\n\t"
-    "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-    ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+    "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
+    "setp.ne.b32 p, %5, 0;\n\t"
+    "mov.b64 b, {%2, %4};\n\t"
+    "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}"
+    ::"r"(tmem_d), "r"(tmem_a), "r"(lo_b), "r"(idesc), "r"(kHi), "r"(uint32_t(add))
     : "memory");
-}
-
-// Shared-memory descriptor of a tile whose rows are the product's depth (keys): 64 columns of 128 bytes, 128-byte swizzle, 8 rows 1024 bytes apart,
-// the next 64 columns `panel` bytes on.
-__device__ __forceinline__ uint64_t make_desc_sw128_rows(uint32_t saddr, uint32_t panel)
-{
-  uint64_t d = 0;
-  d |= uint64_t((saddr & 0x3FFFFu) >> 4);
-  d |= uint64_t(panel >> 4) << 16;
-  d |= uint64_t(1024 >> 4) << 32;
-  d |= uint64_t(1) << 46;
-  d |= uint64_t(2) << 61;
-  return d;
 }
 
 template <int N>
@@ -59,6 +50,32 @@ template <int N>
 __device__ __forceinline__ void registers_down()
 {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
+// Two 32-bit numbers in one operation.
+struct two {
+  uint64_t v;
+  __device__ __forceinline__ two() {}
+  __device__ __forceinline__ two(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
+  __device__ __forceinline__ void get(float& a, float& b) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+};
+__device__ __forceinline__ two fma2(two a, two b, two c)
+{
+  two d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return d;
+}
+__device__ __forceinline__ two mul2(two a, two b)
+{
+  two d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+  return d;
+}
+__device__ __forceinline__ two add2(two a, two b)
+{
+  two d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+  return d;
 }
 
 // A weight of 32 bits as the sum of two 16-bit numbers, so that a row of the output is off by little more than its own rounding: what one number
@@ -74,10 +91,13 @@ struct weight_pair<__half> {
   // their digits above fp16's smallest number, 2^-24: it is 2^-35 of the largest weight, or 2^-31 where the top is behind.
   static __device__ __forceinline__ void split(float a, float b, uint32_t& high, uint32_t& low)
   {
-    asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(high) : "f"(b), "f"(a));
+    // of a little less than the weight: the rest is more than 0
+    float x, y, u, v;
+    mul2(two(a, b), two(1.0f - 1.1920928955078125e-7f, 1.0f - 1.1920928955078125e-7f)).get(x, y);
+    asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(high) : "f"(y), "f"(x));
     const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&high));
-    const __half2 rest = __floats2half2_rn(a - h.x, b - h.y);
-    low                = __vmaxu2(*reinterpret_cast<const uint32_t*>(&rest), __vminu2(high, 0x00010001u));
+    add2(two(a, b), two(-h.x, -h.y)).get(u, v);
+    asm("cvt.rn.f16x2.f32 %0, %2, %1;" : "=r"(low) : "f"(u), "f"(v));
   }
   static __device__ __forceinline__ float2 join(uint32_t high, uint32_t low)
   {
@@ -90,11 +110,12 @@ struct weight_pair<__nv_bfloat16> {
   // 8 bits, cut off, and the rest rounded to 8 bits: to 2^-17 of the weight.  (The rest comes times 1 + 2^-22 of the weight: more than nothing.)
   static __device__ __forceinline__ void split(float a, float b, uint32_t& high, uint32_t& low)
   {
-    high                   = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
-    const float x          = fmaf(a, 1.0f + 2.384185791015625e-7f, -__uint_as_float(__float_as_uint(a) & 0xFFFF0000u));
-    const float y          = fmaf(b, 1.0f + 2.384185791015625e-7f, -__uint_as_float(__float_as_uint(b) & 0xFFFF0000u));
-    const __nv_bfloat162 l = __floats2bfloat162_rn(x, y);
-    low                    = *reinterpret_cast<const uint32_t*>(&l);
+    constexpr float kMore = 1.0f + 2.384185791015625e-7f;
+    high = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
+    const float x = __uint_as_float(__float_as_uint(a) & 0xFFFF0000u), y = __uint_as_float(__float_as_uint(b) & 0xFFFF0000u);
+    float u, v;
+    fma2(two(a, b), two(kMore, kMore), two(-x, -y)).get(u, v);
+    asm("cvt.rn.bf16x2.f32 %0, %2, %1;" : "=r"(low) : "f"(u), "f"(v));
   }
   static __device__ __forceinline__ float2 join(uint32_t high, uint32_t low)
   {
@@ -102,23 +123,22 @@ struct weight_pair<__nv_bfloat16> {
   }
 };
 
-// tanh for scores that are capped: below 0.6 an odd polynomial (least squares at Chebyshev's points; to 2^-26 of the value), else by an exponential (to 2^-22).
-__device__ __forceinline__ float tanh_near(float y)
+// cap tanh(y) for scores that are capped: below kTanhNear y times a polynomial of y^2 (tree_view::cap_near), else by an exponential (to 2^-22).
+__device__ __forceinline__ two tanh_near(two y, const float (&c)[5])
 {
-  const float z = y * y;
-  float p       = fmaf(z, -0.006276390049606562f, 0.021116215735673904f);
-  p             = fmaf(z, p, -0.053875137120485306f);
-  p             = fmaf(z, p, 0.13332924246788025f);
-  p             = fmaf(z, p, -0.3333333134651184f);
-  return fmaf(y * z, p, y);
+  const two z = mul2(y, y);
+  two p       = fma2(z, two(c[4], c[4]), two(c[3], c[3]));
+  p           = fma2(z, p, two(c[2], c[2]));
+  p           = fma2(z, p, two(c[1], c[1]));
+  p           = fma2(z, p, two(c[0], c[0]));
+  return mul2(y, p);
 }
-__device__ __forceinline__ float tanh_any(float y)
+__device__ __forceinline__ float tanh_far(float y)
 {
   const float e = power_of_2(2.8853900817779268f * fabsf(y));  // 2 log2(e)
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(e + 1.0f));
-  const float t = copysignf(fmaf(-2.0f, r, 1.0f), y);
-  return fabsf(y) < 0.6f ? tanh_near(y) : t;
+  return copysignf(fmaf(-2.0f, r, 1.0f), y);
 }
 
 }  // namespace cuvs_b200::kv
