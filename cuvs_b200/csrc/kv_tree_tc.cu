@@ -23,7 +23,7 @@ constexpr int kInfos      = 16;   // tiles whose descriptions are kept: more tha
 constexpr int kPieces     = 2;
 constexpr int kReaders    = 14;   // warps that read a piece's description
 constexpr uint32_t kTile  = 64;   // keys
-constexpr int kMostStages = 10;
+constexpr int kMostStages = 8;    // of keys, and of values
 constexpr uint32_t kLimit = kSpinLimit;
 
 template <int D>
@@ -38,12 +38,14 @@ struct tc_shape {
   static constexpr int kQRegion   = !kTwo ? kQBytes : 2 * kQBytes > kQBytes + 32768 ? 2 * kQBytes : kQBytes + 32768;
   static constexpr int kMisc      = 3072;
   static constexpr int kFit       = (232448 - kQRegion - kMisc) / kTileBytes;
-  static constexpr int kStages    = kFit < kMostStages ? kFit : kMostStages;
-  static constexpr int kRingAt    = kQRegion;
-  static constexpr int kMiscAt    = kRingAt + kStages * kTileBytes;
+  static constexpr int kKeys      = kFit / 2 < kMostStages ? kFit / 2 : kMostStages;  // tiles of keys in flight, and of values
+  static constexpr int kValues    = kFit - kKeys < kMostStages ? kFit - kKeys : kMostStages;
+  static constexpr int kKeysAt    = kQRegion;
+  static constexpr int kValuesAt  = kKeysAt + kKeys * kTileBytes;
+  static constexpr int kMiscAt    = kValuesAt + kValues * kTileBytes;
   static constexpr int kShared    = kMiscAt + kMisc;
   static constexpr int kSumsAt    = 256;               // first column of the sums in tensor memory, behind two tiles of scores of each stream
-  static_assert(kStages >= 4 && kShared <= 232448, "");
+  static_assert(kKeys >= 2 && kValues >= 2 && kShared <= 232448, "");
 };
 
 // A piece of a unit as the way through the share found it.
@@ -55,12 +57,12 @@ struct tree_piece {
 };
 
 struct tc_shared {
-  uint64_t full[kMostStages], empty[kMostStages];
+  uint64_t k_full[kMostStages], k_empty[kMostStages], v_full[kMostStages], v_empty[kMostStages];
   uint64_t q_full, q_empty, s_full[4], p_full[4], pv_done[2], o_full[2], exchanged, drained[2], turn[2][4];
   uint64_t piece_full[kPieces], piece_empty[kPieces];
   tree_piece pieces[kPieces];
-  uint4 valid[kInfos];  // of the four warps that copy: which keys are there
-  uint4 bad[kInfos];    // whether values are no numbers
+  uint2 valid[kInfos];  // of the two warps that copy keys: which are there
+  uint2 bad[kInfos];    // of the two that copy values: whether any is no number
   float2 stats[2][128];
   uint32_t tmem, failed;
 };
@@ -115,9 +117,6 @@ __device__ __forceinline__ bool is_mixed(const tree_view& t, const tree_piece& p
   return int64_t(base) + kTile > int64_t(p.length) || (t.window > 0 && int64_t(base) <= int64_t(p.latest) - t.window);
 }
 
-// Tiles whose scores are wanted ahead: two of each stream.
-__device__ __forceinline__ uint32_t lead_of(bool alternate) { return alternate ? 4u : 2u; }
-
 // ---- copying ------------------------------------------------------------------------------------------------------------------
 
 // This thread's arrival, once its copies so far are there.
@@ -126,72 +125,30 @@ __device__ __forceinline__ void arrive_behind_copies(uint64_t& bar)
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&bar)) : "memory");
 }
 
-// The warps that copy never wait for their own copies: a tile's barrier counts them as they arrive, and the warp that multiplies orders them before what
-// the tensor core reads.  (A proxy fence by the warps that copy waited for all of their copies in flight: 2.5 us a tile.)
+// Two warps copy keys, two values, half of a tile's rows each.  They never wait for their own copies: a tile's barrier counts them as they arrive, and the
+// warp that multiplies orders them before what the tensor core reads.  (A proxy fence by the warps that copy waited for all of their copies in
+// flight: 2.5 us a tile.)
 template <typename T, int D>
 __device__ __forceinline__ void copy_role(const tc_args& a, tc_shared& sh, char* smem, const waiter& wait, uint32_t block)
 {
   using shape                = tc_shape<D>;
-  constexpr uint32_t ROWS = kTile / 4, PR = D / 8, AT_ONCE = 32 / PR, NB = shape::kStages;
+  constexpr uint32_t PR = D / 8, AT_ONCE = 32 / PR;  // pieces of a row, rows of a copy
   const cache_view& c        = a.c;
   const tree_view& t         = a.t;
-  const uint32_t warp        = (threadIdx.x >> 5) & 3u, lane = threadIdx.x & 31u;
+  const uint32_t warp        = (threadIdx.x >> 5) & 3u, lane = threadIdx.x & 31u, half = warp & 1u;
+  const bool of_values       = warp >= 2;
   const uint32_t piece       = lane % PR, sub = lane / PR;
   const uint32_t pieces      = c.dim / 8, wide = (pieces + 1) & ~1u;  // products take 16 columns at a time: those behind the row's end are 0
-  const uint32_t ring        = smem_u32(smem + shape::kRingAt), q_at = smem_u32(smem);
   const uint32_t row0        = block * shape::kRows, rows = min(uint32_t(shape::kRows), t.n_rows - row0);
   const uint32_t column_from = piece < pieces ? piece * 16 : 0u;
-  const uint32_t column_to   = (piece >> 3) * shape::kPanel;
-  const bool alternate       = shape::kTwo && rows <= 128;
-  const uint32_t lead        = lead_of(alternate);
-  // tiles begin at multiples of 16 positions
-  const bool together        = c.page.size % ROWS == 0;
-  const uint64_t k_on = uint64_t(c.k_token_units * AT_ONCE) << c.unit_shift, v_on = uint64_t(c.v_token_units * AT_ONCE) << c.unit_shift;
-  uint32_t it = 0, tiles = 0, q_turn = 0;
-  // The rows of one tile, of which this lane knows the place of one.  `on`: bytes from a lane's row to its next in a page; `look`: values that are to be looked at, for info `info`.
-  auto copy = [&](const char* from, uint32_t at, uint32_t there, uint64_t on, bool look, uint32_t info) -> bool {
-    const uint32_t slot = it % NB;
-    if (it >= NB && !wait(sh.empty[slot], it / NB - 1)) { return false; }
-    const uint32_t to = ring + slot * shape::kTileBytes + column_to;
-    if (together && there == 0xFFFFu) {
-      // all of the warp's rows are there and in one page, one behind the other
-      const char* row_from    = from + (uint64_t(__shfl_sync(kAllLanes, at, sub)) << c.unit_shift);
-      const uint32_t to_piece = to + (warp * ROWS + sub) * 128, bytes = piece < pieces ? 16u : 0u;
-#pragma unroll
-      for (uint32_t i = 0; i < ROWS / AT_ONCE; i++) {
-        if (piece < wide) { copy_piece(to_piece + i * (AT_ONCE * 128) + (((piece ^ sub ^ (i * AT_ONCE)) & 7u) << 4), row_from, bytes); }
-        row_from += on;
-      }
-    } else {
-#pragma unroll
-      for (uint32_t i = 0; i < ROWS / AT_ONCE; i++) {
-        const uint32_t r = i * AT_ONCE + sub, row = warp * ROWS + r;
-        const uint32_t place = __shfl_sync(kAllLanes, at, r);
-        const uint32_t bytes = piece < pieces && ((there >> r) & 1u) != 0u ? 16u : 0u;
-        if (piece < wide) { copy_piece(to + row * 128 + (((piece & 7u) ^ (row & 7u)) << 4), from + (uint64_t(place) << c.unit_shift), bytes); }
-      }
-    }
-    if (look) {
-      copies_end_group();
-      copies_wait<0>();
-      bool bad = false;
-      for (uint32_t r = sub; r < ROWS && piece < wide; r += AT_ONCE) {
-        const uint32_t row = warp * ROWS + r;
-        const uint4 x = *reinterpret_cast<const uint4*>(smem + shape::kRingAt + slot * shape::kTileBytes + column_to + row * 128 +
-                                                        (((piece & 7u) ^ (row & 7u)) << 4));
-        constexpr uint32_t kAll = std::is_same<T, __half>::value ? 0x7C00u : 0x7F80u;
-        const uint32_t words[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-        for (int e = 0; e < 4; e++) { bad = bad || (words[e] & kAll) == kAll || ((words[e] >> 16) & kAll) == kAll; }
-      }
-      if (__any_sync(kAllLanes, bad) && lane == 0) { reinterpret_cast<uint32_t*>(&sh.bad[info])[warp] = 1u; }
-      __syncwarp();
-    }
-    arrive_behind_copies(sh.full[slot]);
-    arrive_warp(sh.full[slot]);  // what the warp wrote itself
-    it++;
-    return true;
-  };
+  const uint32_t stages      = of_values ? shape::kValues : shape::kKeys;
+  const uint32_t ring_at     = (of_values ? shape::kValuesAt : shape::kKeysAt) + (piece >> 3) * shape::kPanel + half * (32 * 128);
+  const uint32_t ring = smem_u32(smem) + ring_at, q_at = smem_u32(smem);
+  uint64_t *full = of_values ? sh.v_full : sh.k_full, *empty = of_values ? sh.v_empty : sh.k_empty;
+  const uint32_t page_units = of_values ? c.v_page_units : c.k_page_units, token_units = of_values ? c.v_token_units : c.k_token_units;
+  const bool together = c.page.size % 16 == 0;  // (tiles begin at multiples of 16 positions)
+  const uint64_t on   = uint64_t(token_units * AT_ONCE) << c.unit_shift;
+  uint32_t tiles = 0, q_turn = 0, slot = 0, round = 0;
 
   piece_reader reader;
   tree_piece p;
@@ -199,10 +156,9 @@ __device__ __forceinline__ void copy_role(const tc_args& a, tc_shared& sh, char*
     const uint32_t n         = p.end - p.chunk;
     const int32_t* table     = a.pages + int64_t(p.sequence) * a.table_stride;
     const int32_t* positions = t.positions + int64_t(p.sequence) * t.positions_stride;
-    const char* keys         = c.keys + int64_t(p.head) * c.k_head * 2 + column_from;
-    const char* values       = c.values + int64_t(p.head) * c.v_head * 2 + column_from;
+    const char* from         = (of_values ? c.values + int64_t(p.head) * c.v_head * 2 : c.keys + int64_t(p.head) * c.k_head * 2) + column_from;
     // what the table says about this lane's key of a tile, asked for a tile ahead
-    const uint32_t own_row = warp * ROWS + lane % ROWS;
+    const uint32_t own_row = half * 32 + lane;
     auto name = [&](uint32_t tile) -> int32_t {
       const uint32_t at = p.base + tile * kTile + own_row;
       if (tile >= p.end || at < p.first || at >= p.last) { return -1; }
@@ -216,12 +172,12 @@ __device__ __forceinline__ void copy_role(const tc_args& a, tc_shared& sh, char*
     const uint32_t q_rows = rows <= 128 ? 128 : 256;
     for (uint32_t r0 = warp * 32; r0 < q_rows; r0 += 128) {
       const uint32_t mine = r0 + lane, r = row0 + min(mine, rows - 1u), token = r / t.group, g = r - token * t.group;
-      const char* from = t.queries.data + (int64_t(p.sequence) * t.queries.sequence + int64_t(token) * t.queries.token +
-                                           int64_t(p.head * t.group + g) * t.queries.head) * 2;
+      const char* q = t.queries.data + (int64_t(p.sequence) * t.queries.sequence + int64_t(token) * t.queries.token +
+                                        int64_t(p.head * t.group + g) * t.queries.head) * 2;
 #pragma unroll 4
       for (uint32_t i = 0; i < 32; i += AT_ONCE) {
         const uint32_t row  = r0 + i + sub;
-        const uint64_t at   = __shfl_sync(kAllLanes, reinterpret_cast<uint64_t>(from), i + sub);
+        const uint64_t at   = __shfl_sync(kAllLanes, reinterpret_cast<uint64_t>(q), i + sub);
         const uint32_t to   = q_at + (row >> 7) * shape::kQBytes + (piece >> 3) * shape::kQPanel + (row & 127u) * 128 + (((piece & 7u) ^ (row & 7u)) << 4);
         if (piece < wide) { copy_piece(to, reinterpret_cast<const char*>(at) + column_from, piece < pieces && row < rows ? 16u : 0u); }
       }
@@ -229,46 +185,71 @@ __device__ __forceinline__ void copy_role(const tc_args& a, tc_shared& sh, char*
     arrive_behind_copies(sh.q_full);
     q_turn++;
 
-    // Keys come `lead` - 1 tiles before their values, whose places have been found with theirs.
-    uint32_t v_at[4] = {0, 0, 0, 0}, v_there[4] = {0, 0, 0, 0};
     bool ok = true;
-    for (uint32_t j = 0; j < n + lead - 1 && ok; j++) {
-      if (j < n) {
-        const uint32_t base = p.base + (p.chunk + j) * kTile, at = base + own_row;
-        const int32_t page  = next;
-        next                = name(p.chunk + j + 1);
-        uint32_t column, place;
-        split_place(min(at, 0x7FFFFFFFu), c.page, column, place);
-        bool there = page >= 0 && page < c.n_pages;
-        if (there && c.filter != nullptr) {
-          const uint64_t slot = uint64_t(page) * c.page.size + place;
-          there               = ((c.filter[slot >> 5] >> (slot & 31u)) & 1u) != 0u;
-        }
-        if (there && at >= p.length) {
-          const int32_t of = positions[at - p.length];
-          there            = of >= 0 && uint32_t(of) >= p.length;
-        }
-        const uint32_t k_at = there ? uint32_t(page) * c.k_page_units + place * c.k_token_units : 0u;
-        const uint32_t rows_there = __ballot_sync(kAllLanes, there) & 0xFFFFu;
-        v_at[0]    = there ? uint32_t(page) * c.v_page_units + place * c.v_token_units : 0u;
-        v_there[0] = rows_there;
-        const uint32_t info = tiles++ % kInfos;
-        if (lane == 0) {
-          reinterpret_cast<uint32_t*>(&sh.valid[info])[warp] = rows_there;
-          reinterpret_cast<uint32_t*>(&sh.bad[info])[warp]   = 0u;
-        }
-        __syncwarp();
-        ok = copy(keys, k_at, rows_there, k_on, false, 0);
+    for (uint32_t j = 0; j < n; j++, tiles++) {
+      const uint32_t base = p.base + (p.chunk + j) * kTile, at = base + own_row;
+      const int32_t page  = next;
+      next                = name(p.chunk + j + 1);
+      uint32_t column, place;
+      split_place(min(at, 0x7FFFFFFFu), c.page, column, place);
+      bool there = page >= 0 && page < c.n_pages;
+      if (there && c.filter != nullptr) {
+        const uint64_t number = uint64_t(page) * c.page.size + place;
+        there                 = ((c.filter[number >> 5] >> (number & 31u)) & 1u) != 0u;
       }
-      if (j + 1 >= lead && ok) {
-        const uint32_t of = j + 1 - lead;
-        ok = copy(values, alternate ? v_at[3] : v_at[1], alternate ? v_there[3] : v_there[1], v_on, is_mixed(t, p, p.base + (p.chunk + of) * kTile),
-                  (tiles - min(j + 1, n) + of) % kInfos);
+      if (there && at >= p.length) {
+        const int32_t of = positions[at - p.length];
+        there            = of >= 0 && uint32_t(of) >= p.length;
       }
+      const uint32_t units = there ? uint32_t(page) * page_units + place * token_units : 0u;
+      const uint32_t rows_there = __ballot_sync(kAllLanes, there);
+      if (round > 0 && !wait(empty[slot], round - 1)) { ok = false; break; }
+      const uint32_t to = ring + slot * shape::kTileBytes;
+      if (together && rows_there == 0xFFFFFFFFu) {
+        // all of the warp's rows are there, 16 of them in a page one behind the other
+        const uint32_t bytes = piece < pieces ? 16u : 0u, to_piece = to + sub * 128;
 #pragma unroll
-      for (int i = 3; i > 0; i--) {
-        v_at[i]    = v_at[i - 1];
-        v_there[i] = v_there[i - 1];
+        for (uint32_t g = 0; g < 2; g++) {
+          const char* row = from + (uint64_t(__shfl_sync(kAllLanes, units, g * 16 + sub)) << c.unit_shift);
+#pragma unroll
+          for (uint32_t i = 0; i < 16; i += AT_ONCE) {
+            if (piece < wide) { copy_piece(to_piece + (g * 16 + i) * 128 + (((piece ^ sub ^ i) & 7u) << 4), row, bytes); }
+            row += on;
+          }
+        }
+      } else {
+#pragma unroll 4
+        for (uint32_t i = 0; i < 32; i += AT_ONCE) {
+          const uint32_t r     = i + sub;
+          const uint32_t where = __shfl_sync(kAllLanes, units, r);
+          const uint32_t bytes = piece < pieces && ((rows_there >> r) & 1u) != 0u ? 16u : 0u;
+          if (piece < wide) { copy_piece(to + r * 128 + (((piece ^ r) & 7u) << 4), from + (uint64_t(where) << c.unit_shift), bytes); }
+        }
+      }
+      const uint32_t info = tiles % kInfos;
+      if (of_values) {
+        bool bad = false;
+        if (is_mixed(t, p, base)) {  // values that some rows do not see
+          copies_end_group();
+          copies_wait<0>();
+          for (uint32_t r = sub; r < 32 && piece < wide; r += AT_ONCE) {
+            const uint4 x = *reinterpret_cast<const uint4*>(smem + ring_at + slot * shape::kTileBytes + r * 128 + (((piece ^ r) & 7u) << 4));
+            constexpr uint32_t kAll = std::is_same<T, __half>::value ? 0x7C00u : 0x7F80u;
+            const uint32_t words[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+            for (int e = 0; e < 4; e++) { bad = bad || (words[e] & kAll) == kAll || ((words[e] >> 16) & kAll) == kAll; }
+          }
+        }
+        const bool any = __any_sync(kAllLanes, bad);
+        if (lane == 0) { (half == 0 ? sh.bad[info].x : sh.bad[info].y) = any; }
+      } else if (lane == 0) {
+        (half == 0 ? sh.valid[info].x : sh.valid[info].y) = rows_there;
+      }
+      arrive_behind_copies(full[slot]);
+      arrive_warp(full[slot]);  // what the warp wrote itself
+      if (++slot == stages) {
+        slot = 0;
+        round++;
       }
     }
     if (!ok) { break; }
@@ -285,41 +266,38 @@ template <typename T, int D>
 __device__ __forceinline__ void multiply_role(const tc_args& a, tc_shared& sh, char* smem, const waiter& wait, uint32_t block, uint32_t stream)
 {
   using shape              = tc_shape<D>;
-  constexpr uint32_t NB    = shape::kStages;
   constexpr uint32_t kType = std::is_same<T, __half>::value ? 0u : 1u;
   const uint32_t rows      = min(uint32_t(shape::kRows), a.t.n_rows - block * shape::kRows);
   const bool both          = shape::kTwo && rows > 128;  // two blocks of rows on the same tiles
   const bool alternate     = shape::kTwo && !both;
-  const uint32_t lead      = lead_of(alternate);
   const uint32_t steps     = (a.c.dim + 15) / 16;
   const uint32_t qk        = (1u << 4) | (kType << 7) | (kType << 10) | ((kTile >> 3) << 17) | ((128u >> 4) << 24);
   const uint32_t pv        = (1u << 4) | (kType << 7) | (kType << 10) | (1u << 16) | (((steps * 16) >> 3) << 17) | ((128u >> 4) << 24);
   const uint32_t tmem      = __shfl_sync(kAllLanes, sh.tmem, 0);
   const uint32_t scores_at = tmem + stream * (2 * kTile), sums_at = tmem + shape::kSumsAt + stream * 128;
   const uint32_t q_lo      = desc_sw128_lo(smem_u32(smem)) + (both ? stream * (shape::kQBytes >> 4) : 0u);
-  const uint32_t ring_lo   = desc_sw128_lo(smem_u32(smem + shape::kRingAt));
-  const uint32_t v_lo      = (smem_u32(smem + shape::kRingAt) >> 4) | (uint32_t(shape::kPanel >> 4) << 16);
+  const uint32_t k_lo      = desc_sw128_lo(smem_u32(smem + shape::kKeysAt));
+  const uint32_t v_lo      = (smem_u32(smem + shape::kValuesAt) >> 4) | (uint32_t(shape::kPanel >> 4) << 16);
 
   piece_reader reader;
   tree_piece p;
-  uint32_t items = 0, tiles = 0, q_turn = 0, p_turn = 0;  // p_turn: a bit for each buffer
+  uint32_t tiles = 0, q_turn = 0, p_turn = 0;  // p_turn: a bit for each buffer
   while (reader.next(sh, wait, p)) {
     const uint32_t n   = p.end - p.chunk;
     const uint32_t own = alternate ? (n + 1 - stream) / 2 : n;  // tiles of this stream
     if (!wait(sh.q_full, q_turn++)) { break; }
-    // The tile of a place in the ring.  (A stream that passes over the other's tiles has seen one of its own that came at most nine places before:
-    // copies arrive in their order, so the barrier is at most one phase behind.)
-    auto arrived = [&](uint32_t item, uint32_t& slot) {
-      slot          = item % NB;
-      const bool ok = wait(sh.full[slot], item / NB);
+    // (A stream passes over the other's tiles.  Copies arrive in their order, so the barrier of a tile is at most one phase behind where the one before
+    // it has been seen.)
+    auto arrived = [&](const uint64_t& full, uint32_t round) {
+      const bool ok = wait(full, round);
       fence_async_smem();  // what was copied, before what the tensor core reads
       return ok;
     };
     auto scores = [&](uint32_t i) {
       const uint32_t j = alternate ? 2 * i + stream : i;
-      uint32_t slot;
-      if (!arrived(items + (j < lead ? j : 2 * j + 1 - lead), slot)) { return false; }
-      const uint32_t from = ring_lo + slot * (shape::kTileBytes >> 4), to = scores_at + (i & 1u) * kTile;
+      const uint32_t slot = (tiles + j) % shape::kKeys;
+      if (!arrived(sh.k_full[slot], (tiles + j) / shape::kKeys)) { return false; }
+      const uint32_t from = k_lo + slot * (shape::kTileBytes >> 4), to = scores_at + (i & 1u) * kTile;
       if (elect_one()) {
         tc_mma_f16_lo<false>(to, q_lo, from, qk);
 #pragma unroll
@@ -329,7 +307,7 @@ __device__ __forceinline__ void multiply_role(const tc_args& a, tc_shared& sh, c
           }
         }
         tc_commit(smem_u32(&sh.s_full[stream * 2 + (i & 1u)]));
-        tc_commit(smem_u32(&sh.empty[slot]));
+        tc_commit(smem_u32(&sh.k_empty[slot]));
         if (i + 1 == own) { tc_commit(smem_u32(&sh.q_empty)); }
       }
       __syncwarp();
@@ -343,11 +321,11 @@ __device__ __forceinline__ void multiply_role(const tc_args& a, tc_shared& sh, c
     ok      = ok && (own < 2 || scores(1));
     for (uint32_t i = 0; i < own && ok; i++) {
       const uint32_t j = alternate ? 2 * i + stream : i, buffer = i & 1u;
-      uint32_t slot;
-      if (!arrived(items + min(n, j + lead) + j, slot)) { ok = false; break; }
+      const uint32_t slot = (tiles + j) % shape::kValues;
+      if (!arrived(sh.v_full[slot], (tiles + j) / shape::kValues)) { ok = false; break; }
       // where values are no numbers the threads of the rows add them up themselves
-      const uint4 bad = sh.bad[(tiles + j) % kInfos];
-      const bool good = (bad.x | bad.y | bad.z | bad.w) == 0u;
+      const uint2 bad = sh.bad[(tiles + j) % kInfos];
+      const bool good = (bad.x | bad.y) == 0u;
       if (!wait(sh.p_full[stream * 2 + buffer], p_turn >> buffer)) { ok = false; break; }
       p_turn ^= 1u << buffer;
       tc_fence_after();
@@ -363,7 +341,7 @@ __device__ __forceinline__ void multiply_role(const tc_args& a, tc_shared& sh, c
           }
         }
         tc_commit(smem_u32(&sh.pv_done[stream]));
-        tc_commit(smem_u32(&sh.empty[slot]));
+        tc_commit(smem_u32(&sh.v_empty[slot]));
         if (i + 1 == own) { tc_commit(smem_u32(&sh.o_full[stream])); }
       }
       __syncwarp();
@@ -371,7 +349,6 @@ __device__ __forceinline__ void multiply_role(const tc_args& a, tc_shared& sh, c
     }
     if (!ok) { break; }
     tiles += n;
-    items += 2 * n;
   }
   if (elect_one()) { tc_commit(smem_u32(&sh.drained[stream])); }
   __syncwarp();
@@ -430,7 +407,6 @@ template <typename T, int D, bool SHAPED>
 __device__ __forceinline__ void softmax_role(const tc_args& a, tc_shared& sh, char* smem, const waiter& wait, uint32_t which, uint32_t block)
 {
   using shape             = tc_shape<D>;
-  constexpr uint32_t NB = shape::kStages;
   const tree_view& t      = a.t;
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, stream = warp >> 2, quarter = warp & 3u;
   const uint32_t row0 = block * shape::kRows, rows = min(uint32_t(shape::kRows), t.n_rows - row0);
@@ -442,14 +418,13 @@ __device__ __forceinline__ void softmax_role(const tc_args& a, tc_shared& sh, ch
   const int64_t out_at = int64_t(token) * t.out.token + int64_t(g) * t.out.head;  // of this row, in its sequence and key head
   const bool alive     = __any_sync(kAllLanes, exists);
   const uint32_t lanes = quarter << 21;  // this warp's lanes of tensor memory
-  const uint32_t lead  = lead_of(alternate);
   const uint32_t sh_tmem = sh.tmem;
   const uint32_t sums  = sh_tmem + lanes + shape::kSumsAt + (shape::kTwo ? stream * 128 : 0);
   const uint32_t width = (a.c.dim + 31) / 32;  // columns of the sums, in 32
   piece_reader reader;
   tree_piece p;
   const bool in_turns = both && 128 + quarter * 32 < rows;  // both streams' warps of this quarter have rows
-  uint32_t e_turn = 0, s_turn = 0, o_turn = 0, x_turn = 0, tiles = 0, items = 0, pv_turn = 0;  // s_turn: a bit for each buffer
+  uint32_t e_turn = 0, s_turn = 0, o_turn = 0, x_turn = 0, tiles = 0, pv_turn = 0;  // s_turn: a bit for each buffer
 
   while (reader.next(sh, wait, p)) {
     const uint32_t n = p.end - p.chunk;
@@ -482,8 +457,8 @@ __device__ __forceinline__ void softmax_role(const tc_args& a, tc_shared& sh, ch
       tmem_ld32_async(scores + 32, x[1]);
       const uint32_t info = (tiles + j) % kInfos, base = p.base + (p.chunk + j) * kTile;
       const bool mixed    = int32_t(p.chunk + j) >= tail_from || int32_t(p.chunk + j) <= edge_to;
-      const uint4 valid   = sh.valid[info];
-      const bool whole    = (valid.x & valid.y & valid.z & valid.w) == 0xFFFFu && !mixed;
+      const uint2 valid   = sh.valid[info];
+      const bool whole    = (valid.x & valid.y) == 0xFFFFFFFFu && !mixed;
       tmem_ld_wait(x[0]);
       tmem_ld_wait(x[1]);
       if constexpr (SHAPED) {
@@ -493,7 +468,7 @@ __device__ __forceinline__ void softmax_role(const tc_args& a, tc_shared& sh, ch
       if (!whole) {
 #pragma unroll
         for (uint32_t i = 0; i < 2; i++) {
-          uint32_t seen = i == 0 ? valid.x | valid.y << 16 : valid.z | valid.w << 16;
+          uint32_t seen = i == 0 ? valid.x : valid.y;
           if (mixed) { seen &= seen_keys(t, l, positions, own, mask, base + i * 32); }
 #pragma unroll
           for (int k = 0; k < 32; k++) { x[i][k] = ((seen >> k) & 1u) != 0u ? x[i][k] : 0xFF800000u; }
@@ -564,13 +539,13 @@ __device__ __forceinline__ void softmax_role(const tc_args& a, tc_shared& sh, ch
       }
       if (mixed) {
         // Values that are no numbers must not reach rows that do not see them, as 0 times them would: each row adds up what it sees.
-        const uint32_t at = items + min(n, j + lead) + j, slot = at % NB;  // in the order in which tiles are copied
-        if (!wait(sh.full[slot], at / NB)) { ok = false; break; }
-        const uint4 bad = sh.bad[info];
-        if ((bad.x | bad.y | bad.z | bad.w) != 0u) {
+        const uint32_t slot = (tiles + j) % shape::kValues;
+        if (!wait(sh.v_full[slot], (tiles + j) / shape::kValues)) { ok = false; break; }
+        const uint2 bad = sh.bad[info];
+        if ((bad.x | bad.y) != 0u) {
           if (done > 0 && !wait(sh.pv_done[stream], pv_turn + done - 1)) { ok = false; break; }
           tc_fence_after();
-          const char* v = smem + shape::kRingAt + slot * shape::kTileBytes;
+          const char* v = smem + shape::kValuesAt + slot * shape::kTileBytes;
 #pragma unroll 1
           for (uint32_t i = 0; i < width; i++) {
             uint32_t o[32];
@@ -616,7 +591,6 @@ __device__ __forceinline__ void softmax_role(const tc_args& a, tc_shared& sh, ch
       sum = 0.0f;
     }
     tiles += n;
-    items += 2 * n;
     pv_turn += done;
     if (done > 0) {
       if (!wait(sh.o_full[stream], o_turn++)) { return; }
@@ -774,9 +748,11 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
   const uint32_t which = blockIdx.x / a.t.n_blocks_of, block = blockIdx.x - which * a.t.n_blocks_of;
   if (threadIdx.x == 32) {
     const bool both = shape::kTwo && a.t.n_rows - block * shape::kRows > 128;
-    for (int i = 0; i < shape::kStages; i++) {
-      mbar_init(smem_u32(&sh.full[i]), 128 + 4);
-      mbar_init(smem_u32(&sh.empty[i]), both ? 2 : 1);
+    for (int i = 0; i < kMostStages; i++) {
+      mbar_init(smem_u32(&sh.k_full[i]), 64 + 2);
+      mbar_init(smem_u32(&sh.v_full[i]), 64 + 2);
+      mbar_init(smem_u32(&sh.k_empty[i]), both ? 2 : 1);
+      mbar_init(smem_u32(&sh.v_empty[i]), both ? 2 : 1);
     }
     mbar_init(smem_u32(&sh.q_full), 128);
     mbar_init(smem_u32(&sh.q_empty), shape::kTwo ? 2 : 1);
