@@ -300,8 +300,8 @@ struct tree_plan {
   uint32_t cost;       // of a unit beside its tiles, in tiles
   bool parts;          // a unit may lie in several shares
 };
-// `units` of `most` keys each, at most; `blocks`: thread blocks that the GPU holds at once.
-inline tree_plan deal_out_tree(uint32_t blocks, uint32_t rows, uint32_t tile, uint32_t cost, uint64_t units, uint32_t n_rows, uint64_t most)
+// `units` of `most` keys each, at most; `blocks`: thread blocks that the GPU holds at once; `least`: tiles of a share.
+inline tree_plan deal_out_tree(uint32_t blocks, uint32_t rows, uint32_t tile, uint32_t cost, uint32_t least, uint64_t units, uint32_t n_rows, uint64_t most)
 {
   tree_plan p;
   p.rows      = rows;
@@ -309,7 +309,7 @@ inline tree_plan deal_out_tree(uint32_t blocks, uint32_t rows, uint32_t tile, ui
   p.cost      = cost;
   p.blocks_of = ceildiv(n_rows, rows);
   const uint64_t tiles = std::max<uint64_t>(1, ceildiv<uint64_t>(most, tile));
-  p.shares = uint32_t(std::max<uint64_t>(1, std::min<uint64_t>(blocks / p.blocks_of, ceildiv<uint64_t>(units * (tiles + cost), drafted_lists::kLeast))));
+  p.shares = uint32_t(std::max<uint64_t>(1, std::min<uint64_t>(blocks / p.blocks_of, ceildiv<uint64_t>(units * (tiles + cost), least))));
   p.parts  = p.shares > 1 && tiles > 1;
   return p;
 }

@@ -11,12 +11,13 @@ namespace {
 constexpr int kThreads = 256;
 
 // Blocks of an SM: what shared memory and registers leave room for.  They hide each other's loads.
-constexpr int tree_resident(int columns, int rows) { return columns == 64 ? (rows == 16 ? 4 : 3) : columns == 128 ? (rows == 16 ? 2 : 1) : rows == 16 ? 2 : 1; }
+constexpr int tree_resident(int columns) { return columns == 64 ? 3 : 1; }
 
 // D: columns of a row in shared memory; BM: rows of a block.  Threads stand in 16 x 16: thread (y, x) has BM / 16 rows, their scores with every 16th key
 // and their weighted sums in every 16th four columns.
-template <int D, int BM>
+template <int D>
 struct tree_shape {
+  static constexpr int BM     = 64;
   static constexpr int kTile  = D <= 128 ? 64 : 32;
   static constexpr int kRows  = BM / 16;    // of a thread
   static constexpr int kKeys  = kTile / 16;
@@ -29,15 +30,17 @@ struct tree_shape {
   static constexpr int kValidAt = kSeenAt + BM * (kTile / 32);
   static constexpr int kPlaceAt = kValidAt + 4;
   static constexpr int kShared = (kPlaceAt + 3 * kTile) * 4;
-  static constexpr int kResident = tree_resident(D, BM);
+  static constexpr int kResident = tree_resident(D);
   static_assert(kResident * (kShared + 1024) <= 233472, "");
 };
 
-template <typename T, int D, int BM>
-__global__ void __launch_bounds__(kThreads, tree_shape<D, BM>::kResident)
+template <int D>
+__global__ void __launch_bounds__(kThreads, tree_shape<D>::kResident)
 tree_rows_kernel(cache_view c, work_view w, drafted_lists lists, tree_view t, tree_parts parts, const int32_t* pages, int64_t table_stride, float shift)
 {
-  using shape = tree_shape<D, BM>;
+  using T     = float;
+  using shape = tree_shape<D>;
+  constexpr int BM = shape::BM;
   constexpr int TILE = shape::kTile, ROWS = shape::kRows, KEYS = shape::kKeys, QUADS = shape::kQuads, PITCH = shape::kPitch, E = kPerPiece<T>;
   chain_begin();
   extern __shared__ __align__(16) float s_mem[];
@@ -251,6 +254,276 @@ tree_rows_kernel(cache_view c, work_view w, drafted_lists lists, tree_view t, tr
   empty_tree_rows<T>(c, w.n_sequences, lists, t, parts, threadIdx.x, kThreads);
 }
 
+// ---- few rows -----------------------------------------------------------------------------------------------------------------
+//
+// Where a unit has few rows the keys' and values' way through shared memory is what counts.  Warps work alone, each on chunks of 8 KB of keys and as
+// much of values that it copies a stage ahead.  Scores: a lane has a key (of rows of more than 64 columns some lanes share one), and reads each of its pieces
+// once for all rows, whose queries are broadcast.  Sums: a lane has columns, and reads each value once for all rows, whose weights are broadcast.
+//
+// What bounds it: HBM, with one multiply-add of every lane for each key, column and row beside it: 32 keys of 64 columns and 8 rows are 1,024 of a warp.
+
+constexpr int kFewWarps = 6;
+struct few_lists : drafted_lists {
+  static constexpr uint32_t kLeast = kFewWarps;  // a chunk for each warp
+};
+
+template <int D, int R>
+struct few_shape {
+  static constexpr int kKeys   = 2048 / D;   // of a chunk
+  static constexpr int kParts  = 32 / kKeys; // lanes of a key
+  static constexpr int kPitch  = D + 4 * kParts;  // floats: eight lanes' pieces on different banks
+  static constexpr int kStage  = 2 * kKeys * kPitch;
+  static constexpr int kOwn    = 2 * kStage + R * 32;  // of a warp: two stages, weights
+  static constexpr int kQAt    = kFewWarps * kOwn;
+  static constexpr int kShared = (kQAt + R * D) * 4;
+  static constexpr int kColumns = D / 32;    // of a lane
+  static_assert(kShared <= 232448 && R * (D + 2) <= kOwn, "");
+};
+
+template <int D, int R>
+__global__ void __launch_bounds__(kFewWarps * 32, 1)
+tree_few_kernel(cache_view c, work_view w, few_lists lists, tree_view t, tree_parts parts, const int32_t* pages, int64_t table_stride, float shift)
+{
+  using shape = few_shape<D, R>;
+  constexpr int KEYS = shape::kKeys, PARTS = shape::kParts, PITCH = shape::kPitch, COLUMNS = shape::kColumns, PIECES = D / 4;
+  chain_begin();
+  extern __shared__ __align__(16) float s_mem[];
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+  float* s_own = s_mem + warp * shape::kOwn;
+  float* s_p   = s_own + 2 * shape::kStage;
+  float* s_q   = s_mem + shape::kQAt;
+  const uint32_t which = blockIdx.x / t.n_blocks_of, block = blockIdx.x - which * t.n_blocks_of;
+  const uint32_t row0 = block * R, rows = min(uint32_t(R), t.n_rows - row0);
+  const uint32_t pieces = c.dim / 4, key_of = lane / PARTS, part_of = lane % PARTS;
+
+  walk<KEYS, few_lists> path(c, w, lists, parts.shares, which);
+  piece now;
+  uint4 begun = make_uint4(0, 0, 0, 0);
+  while (__syncthreads_and(path.next(now)) != 0) {
+    const drafted_lists::list l = path.l;
+    const uint32_t head         = now.unit;
+    const int32_t* table        = pages + int64_t(now.sequence) * table_stride;
+    const int32_t* positions    = t.positions + int64_t(now.sequence) * t.positions_stride;
+    const char* keys            = c.keys + int64_t(head) * c.k_head * 4;
+    const char* values          = c.values + int64_t(head) * c.v_head * 4;
+    for (uint32_t i = threadIdx.x; i < uint32_t(R * PIECES); i += kFewWarps * 32) {
+      const uint32_t r = i / PIECES, p = i - r * PIECES;
+      uint4 x = make_uint4(0, 0, 0, 0);
+      if (r < rows && p < pieces) {
+        const uint32_t token = (row0 + r) / t.group, g = row0 + r - token * t.group;
+        x = reinterpret_cast<const uint4*>(t.queries.data + (int64_t(now.sequence) * t.queries.sequence + int64_t(token) * t.queries.token +
+                                                             int64_t(head * t.group + g) * t.queries.head) * 4)[p];
+      }
+      reinterpret_cast<uint4*>(s_q)[i] = x;
+    }
+    // lane r looks after row r: its position, its slope, its row of the mask
+    const uint32_t my_row = row0 + min(lane, rows - 1u), my_token = my_row / t.group;
+    const int32_t my_at   = positions[my_token];
+    const bool my_is      = lane < rows && my_at >= 0 && uint32_t(my_at) >= l.length;
+    const float my_slope  = t.slopes != nullptr ? t.slopes[head * t.group + (my_row - my_token * t.group)] * kLog2E : 0.0f;
+    const uint32_t* my_mask = t.mask + int64_t(now.sequence) * t.mask_sequence + int64_t(my_token) * t.mask_token;
+    int32_t latest = 0;
+    if (t.window > 0) {
+      for (uint32_t i = lane; i < t.n_drafted; i += 32) { latest = max(latest, positions[i]); }
+      latest = __reduce_max_sync(kAllLanes, latest);
+    }
+    float top[R], sum[R], acc[R][COLUMNS];
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+      top[r] = -INFINITY;
+      sum[r] = 0.0f;
+#pragma unroll
+      for (int e = 0; e < COLUMNS; e++) { acc[r][e] = 0.0f; }
+    }
+    __syncthreads();
+
+    // what memory says about this lane's key of a chunk
+    auto look = [&](uint32_t chunk, uint32_t& k_at, uint32_t& v_at) -> bool {
+      const uint32_t at = l.base + chunk * KEYS + lane;
+      if (lane >= uint32_t(KEYS) || chunk >= now.end || at < l.first || at >= l.end) { return false; }
+      uint32_t column, place;
+      split_place(at, c.page, column, place);
+      const int32_t page = table[column];  // at < end: the column is inside the table
+      if (page < 0 || page >= c.n_pages) { return false; }
+      k_at = uint32_t(page) * c.k_page_units + place * c.k_token_units;
+      v_at = uint32_t(page) * c.v_page_units + place * c.v_token_units;
+      if (c.filter != nullptr) {
+        const uint64_t slot = uint64_t(page) * c.page.size + place;
+        if (((c.filter[slot >> 5] >> (slot & 31u)) & 1u) == 0u) { return false; }
+      }
+      if (at >= l.length) {
+        const int32_t of = positions[at - l.length];
+        return of >= 0 && uint32_t(of) >= l.length;
+      }
+      return true;
+    };
+    // copies of the rows that are there; the others are 0
+    auto copy = [&](uint32_t stage, bool there, uint32_t k_at, uint32_t v_at) -> uint32_t {
+      const uint32_t valid = __ballot_sync(kAllLanes, there);
+      const uint32_t to    = shared_address(s_own + stage * shape::kStage);
+#pragma unroll 4
+      for (uint32_t i = 0; i < uint32_t(KEYS * PIECES / 32); i++) {
+        const uint32_t index = i * 32 + lane, row = index / PIECES, p = index % PIECES;
+        const uint32_t bytes = p < pieces && ((valid >> row) & 1u) != 0u ? 16u : 0u, from = p < pieces ? p * 16 : 0u;
+        const uint32_t k = __shfl_sync(kAllLanes, k_at, row), v = __shfl_sync(kAllLanes, v_at, row);
+        copy_piece(to + (row * PITCH + p * 4) * 4, keys + (uint64_t(k) << c.unit_shift) + from, bytes);
+        copy_piece(to + ((KEYS + row) * PITCH + p * 4) * 4, values + (uint64_t(v) << c.unit_shift) + from, bytes);
+      }
+      copies_end_group();
+      return valid;
+    };
+    uint32_t k_at = 0, v_at = 0, chunk = now.chunk + warp;
+    bool there      = look(chunk, k_at, v_at);
+    uint32_t valid  = chunk < now.end ? copy(0, there, k_at, v_at) : 0u;
+    k_at = v_at     = 0;
+    there           = look(chunk + kFewWarps, k_at, v_at);
+    for (uint32_t stage = 0; chunk < now.end; chunk += kFewWarps, stage ^= 1u) {
+      const uint32_t next_valid = copy(stage ^ 1u, there, k_at, v_at);
+      k_at = v_at = 0;
+      there       = look(chunk + 2 * kFewWarps, k_at, v_at);
+      copies_wait<1>();
+      __syncwarp();
+      const float* s_k     = s_own + stage * shape::kStage;
+      const float* s_v     = s_k + KEYS * PITCH;
+      const uint32_t base  = l.base + chunk * KEYS;
+      const bool mixed     = int64_t(base) + KEYS > int64_t(l.length) || (t.window > 0 && int64_t(base) <= int64_t(latest) - t.window);
+      uint32_t seen        = my_is ? valid : 0u;
+      if (mixed && my_is) { seen &= seen_keys(t, l, positions, my_at, my_mask, base); }
+      float s[R];
+#pragma unroll
+      for (int r = 0; r < R; r++) { s[r] = 0.0f; }
+#pragma unroll 4
+      for (int d = 0; d < D; d += 4 * PARTS) {
+        const float4 k = *reinterpret_cast<const float4*>(s_k + key_of * PITCH + d + part_of * 4);
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+          const float4 q = *reinterpret_cast<const float4*>(s_q + r * D + d + part_of * 4);
+          s[r]           = fmaf(q.x, k.x, s[r]);
+          s[r]           = fmaf(q.y, k.y, s[r]);
+          s[r]           = fmaf(q.z, k.z, s[r]);
+          s[r]           = fmaf(q.w, k.w, s[r]);
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < R; r++) {
+#pragma unroll
+        for (int o = 1; o < PARTS; o *= 2) { s[r] += __shfl_xor_sync(kAllLanes, s[r], o); }
+      }
+      int32_t of = int32_t(base + key_of);  // the key's position
+      if (mixed && base + key_of >= l.length && base + key_of - l.length < t.n_drafted) { of = positions[base + key_of - l.length]; }
+#pragma unroll
+      for (int r = 0; r < R; r++) {
+        if (uint32_t(r) >= rows) { continue; }
+        float score = t.cap_log2 != 0.0f ? tanhf(s[r] * t.scale_cap) * t.cap_log2 : s[r] * t.scale_log2;
+        if (t.slopes != nullptr) {
+          score = fmaf(__shfl_sync(kAllLanes, my_slope, r), float(int64_t(of) - __shfl_sync(kAllLanes, my_at, r)), score);
+        }
+        const uint32_t sees = __shfl_sync(kAllLanes, seen, r);
+        score               = ((sees >> key_of) & 1u) != 0u ? score : -INFINITY;
+        float next          = score;
+#pragma unroll
+        for (int o = PARTS; o < 32; o *= 2) { next = fmaxf(next, __shfl_xor_sync(kAllLanes, next, o)); }
+        next             = fmaxf(next, top[r]);
+        const float safe = finite_top(next);
+        if (next != top[r]) {  // of the whole warp
+          const float keep = power_of_2(top[r] - safe);
+          top[r]           = next;
+          sum[r] *= keep;
+#pragma unroll
+          for (int e = 0; e < COLUMNS; e++) { acc[r][e] *= keep; }
+        }
+        const float p = power_of_2(score - safe + shift);
+        if (part_of == 0) {
+          sum[r] += p;  // of the lane's own keys, until the end
+          s_p[r * 32 + key_of] = p;
+        }
+      }
+      __syncwarp();
+#pragma unroll 2
+      for (int k = 0; k < KEYS; k += 4) {
+        float v[4][COLUMNS];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const float* row = s_v + (k + i) * PITCH;
+          if constexpr (COLUMNS == 2) {
+            const float2 x = *reinterpret_cast<const float2*>(row + lane * 2);
+            v[i][0] = x.x, v[i][1] = x.y;
+          } else {
+#pragma unroll
+            for (int e = 0; e < COLUMNS; e += 4) {
+              const float4 x = *reinterpret_cast<const float4*>(row + e * 32 + lane * 4);
+              v[i][e] = x.x, v[i][e + 1] = x.y, v[i][e + 2] = x.z, v[i][e + 3] = x.w;
+            }
+          }
+        }
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+          if (uint32_t(r) >= rows) { continue; }
+          const float4 p4  = *reinterpret_cast<const float4*>(s_p + r * 32 + k);
+          const float p[4] = {p4.x, p4.y, p4.z, p4.w};
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            if (mixed && p[i] == 0.0f) { continue; }  // what the row does not see may be infinite, or no number
+#pragma unroll
+            for (int e = 0; e < COLUMNS; e++) { acc[r][e] = fmaf(p[i], v[i][e], acc[r][e]); }
+          }
+        }
+      }
+      __syncwarp();
+      valid = next_valid;
+    }
+    copies_wait<0>();
+    __syncwarp();
+    // the warps' sums, in the place of their stages: top, sum, columns
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+#pragma unroll
+      for (int o = 16; o > 0; o /= 2) { sum[r] += __shfl_xor_sync(kAllLanes, sum[r], o); }
+      float* mine = s_own + r * (D + 2);
+      if (lane == 0) {
+        mine[0] = top[r];
+        mine[1] = sum[r];
+      }
+#pragma unroll
+      for (int e = 0; e < COLUMNS; e++) { mine[2 + (COLUMNS == 2 ? lane * 2 + e : (e / 4) * 128 + lane * 4 + e % 4)] = acc[r][e]; }
+    }
+    __syncthreads();
+    const size_t part = parts.part(which, block, now.begins ? 1u : 0u);
+    for (uint32_t i = threadIdx.x; i < rows * pieces; i += kFewWarps * 32) {
+      const uint32_t r = i / pieces, quad = i - r * pieces;
+      float most = -INFINITY;
+#pragma unroll
+      for (int v = 0; v < kFewWarps; v++) { most = fmaxf(most, s_mem[v * shape::kOwn + r * (D + 2)]); }
+      const float safe = finite_top(most);
+      float total = 0.0f, x[4] = {};
+#pragma unroll
+      for (int v = 0; v < kFewWarps; v++) {
+        const float* of = s_mem + v * shape::kOwn + r * (D + 2);
+        const float f   = power_of_2(of[0] - safe);
+        total           = fmaf(of[1], f, total);
+        if (of[0] == -INFINITY) { continue; }
+#pragma unroll
+        for (int e = 0; e < 4; e++) { x[e] = fmaf(of[2 + quad * 4 + e], f, x[e]); }
+      }
+      if (now.whole) {
+        const float scale = total == 0.0f ? 0.0f : 1.0f / total;
+        store_quad<float>(out_row<float>(t, now.sequence, head, row0 + r) + quad * 4, make_float4(x[0] * scale, x[1] * scale, x[2] * scale, x[3] * scale));
+        if (quad == 0) { *lse_at(t, now.sequence, head, c.n_heads, row0 + r) = (safe + log2f(total) - shift) * kLn2; }
+      } else {
+        parts.acc[(part * parts.quads + quad) * parts.rows + r] = make_float4(x[0], x[1], x[2], x[3]);
+        if (quad == 0) { parts.stats[part * parts.rows + r] = make_float2(most, total); }
+      }
+    }
+    if (now.begins && threadIdx.x == 0) { note_begun(parts, now, c.n_heads, which, begun); }
+  }
+  if (parts.begun != nullptr && !parts.by_unit && block == 0 && threadIdx.x == 0) { parts.begun[which] = begun; }
+  empty_tree_rows<float>(c, w.n_sequences, lists, t, parts, threadIdx.x, kFewWarps * 32);
+}
+
+// Rows of a block, by how many a unit has; more of few than of many: the kernel for few.
+constexpr uint32_t few_rows_of(uint32_t n_rows, uint32_t dim) { return n_rows <= 4 ? 4 : n_rows <= 8 || dim > 128 ? 8 : 16; }
+constexpr uint32_t kFew = 32;
+
 tree_plan plan_of(const resources& res, elem type, uint64_t sequences, uint32_t n_drafted, uint32_t n_heads, uint32_t group, uint32_t dim,
                   uint64_t capacity, int64_t window)
 {
@@ -258,10 +531,11 @@ tree_plan plan_of(const resources& res, elem type, uint64_t sequences, uint32_t 
   // the keys of the longest list: a window may begin anywhere in 16 positions
   const uint64_t most = window > 0 && uint64_t(window) < capacity ? std::min(capacity, uint64_t(window) + n_drafted + 15) : capacity;
   if (type == elem::f32) {
-    const int rows = n_rows <= 16 ? 16 : 64;
-    return deal_out_tree(sms * tree_resident(int(tree_columns(dim)), rows), n_rows <= 16 ? 16 : 64, dim <= 128 ? 64 : 32, 2, sequences * n_heads, n_rows, most);
+    const uint32_t columns = tree_columns(dim);
+    if (n_rows <= kFew) { return deal_out_tree(sms, few_rows_of(n_rows, dim), 2048 / columns, 12, few_lists::kLeast, sequences * n_heads, n_rows, most); }
+    return deal_out_tree(sms * tree_resident(int(columns)), 64, columns <= 128 ? 64 : 32, 2, drafted_lists::kLeast, sequences * n_heads, n_rows, most);
   }
-  return deal_out_tree(sms, dim <= 128 && n_rows > 128 ? 256 : 128, 64, 2, sequences * n_heads, n_rows, most);
+  return deal_out_tree(sms, dim <= 128 && n_rows > 128 ? 256 : 128, 64, 2, drafted_lists::kLeast, sequences * n_heads, n_rows, most);
 }
 
 }  // namespace
@@ -329,26 +603,22 @@ void attend_tree(resources& res, cudaStream_t stream, const attend_tree_args& a)
     attend_tree16<__nv_bfloat16>(stream, call);
     return join(__nv_bfloat16{});
   }
-  auto go = [&](auto columns, auto bm) {
-    constexpr int D = decltype(columns)::value, BM = decltype(bm)::value;
-    auto kernel = tree_rows_kernel<float, D, BM>;
-    constexpr size_t smem = tree_shape<D, BM>::kShared;
+  auto go = [&](auto kernel, const auto& lists, int threads, size_t smem) {
     ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem);
-    launch_chained(kernel, dim3(p.shares * p.blocks_of), kThreads, smem, stream, c, call.w, call.lists, t, call.parts, a.pages, a.table_stride,
-                   call.shift);
+    launch_chained(kernel, dim3(p.shares * p.blocks_of), threads, smem, stream, c, call.w, lists, t, call.parts, a.pages, a.table_stride, call.shift);
+  };
+  auto by_columns = [&](auto columns) {
+    constexpr int D = decltype(columns)::value;
+    if (t.n_rows > kFew) { return go(tree_rows_kernel<D>, call.lists, kThreads, tree_shape<D>::kShared); }
+    if (p.rows == 4) { return go(tree_few_kernel<D, 4>, few_lists{call.lists}, kFewWarps * 32, few_shape<D, 4>::kShared); }
+    if (p.rows == 8) { return go(tree_few_kernel<D, 8>, few_lists{call.lists}, kFewWarps * 32, few_shape<D, 8>::kShared); }
+    if constexpr (D <= 128) { go(tree_few_kernel<D, 16>, few_lists{call.lists}, kFewWarps * 32, few_shape<D, 16>::kShared); }
   };
   using std::integral_constant;
-  auto by_rows = [&](auto columns) {
-    if (p.rows == 16) {
-      go(columns, integral_constant<int, 16>{});
-    } else {
-      go(columns, integral_constant<int, 64>{});
-    }
-  };
   switch (tree_columns(c.dim)) {
-    case 64: by_rows(integral_constant<int, 64>{}); break;
-    case 128: by_rows(integral_constant<int, 128>{}); break;
-    default: by_rows(integral_constant<int, 256>{});
+    case 64: by_columns(integral_constant<int, 64>{}); break;
+    case 128: by_columns(integral_constant<int, 128>{}); break;
+    default: by_columns(integral_constant<int, 256>{});
   }
   join(float{});
 }
