@@ -16,6 +16,32 @@
 
 namespace cuvs_b200::kv {
 
+// Two 32-bit numbers in one operation.
+struct two {
+  uint64_t v;
+  __device__ __forceinline__ two() {}
+  __device__ __forceinline__ two(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
+  __device__ __forceinline__ void get(float& a, float& b) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+};
+__device__ __forceinline__ two fma2(two a, two b, two c)
+{
+  two d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return d;
+}
+__device__ __forceinline__ two mul2(two a, two b)
+{
+  two d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+  return d;
+}
+__device__ __forceinline__ two add2(two a, two b)
+{
+  two d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+  return d;
+}
+
 struct tree_view {
   uint32_t n_drafted, group, n_rows;  // n_rows = n_drafted * group, of a unit
   uint32_t n_blocks_of;               // row blocks of a unit

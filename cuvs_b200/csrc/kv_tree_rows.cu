@@ -256,36 +256,38 @@ tree_rows_kernel(cache_view c, work_view w, drafted_lists lists, tree_view t, tr
 
 // ---- few rows -----------------------------------------------------------------------------------------------------------------
 //
-// Where a unit has few rows the keys' and values' way through shared memory is what counts.  Warps work alone, each on chunks of 8 KB of keys and as
-// much of values that it copies a stage ahead.  Scores: a lane has a key (of rows of more than 64 columns some lanes share one), and reads each of its pieces
-// once for all rows, whose queries are broadcast.  Sums: a lane has columns, and reads each value once for all rows, whose weights are broadcast.
+// Where a unit has few rows the keys' and values' way through shared memory is what counts.  Warps work alone, each on chunks of 4 KB of keys and as
+// much of values that it copies a stage ahead.  Scores: some lanes share a key, and each of its pieces is read once for all rows, whose queries are
+// broadcast.  Sums: a lane has columns, and reads each value once for all rows, whose weights are broadcast.
 //
-// What bounds it: HBM, with one multiply-add of every lane for each key, column and row beside it: 32 keys of 64 columns and 8 rows are 1,024 of a warp.
+// What bounds it: the instructions' latency, with twelve warps of an SM (of six, whose chunks were twice as large: 92 us where twelve take less).
 
-constexpr int kFewWarps = 6;
+constexpr int kFewMost = 12;  // warps of a block, at most
 struct few_lists : drafted_lists {
-  static constexpr uint32_t kLeast = kFewWarps;  // a chunk for each warp
+  static constexpr uint32_t kLeast = kFewMost;  // a chunk for each warp
 };
 
 template <int D, int R>
 struct few_shape {
-  static constexpr int kKeys   = 2048 / D;   // of a chunk
+  static constexpr int kKeys   = 1024 / D;   // of a chunk
   static constexpr int kParts  = 32 / kKeys; // lanes of a key
   static constexpr int kPitch  = D + 4 * kParts;  // floats: eight lanes' pieces on different banks
   static constexpr int kStage  = 2 * kKeys * kPitch;
-  static constexpr int kOwn    = 2 * kStage + R * 32;  // of a warp: two stages, weights
-  static constexpr int kQAt    = kFewWarps * kOwn;
+  static constexpr int kOwn    = 2 * kStage + R * kKeys * 2;  // of a warp: two stages, weights (each twice)
+  static constexpr int kFit    = (232448 / 4 - R * D) / kOwn;
+  static constexpr int kWarps  = kFit < kFewMost ? kFit : kFewMost;
+  static constexpr int kQAt    = kWarps * kOwn;
   static constexpr int kShared = (kQAt + R * D) * 4;
   static constexpr int kColumns = D / 32;    // of a lane
   static_assert(kShared <= 232448 && R * (D + 2) <= kOwn, "");
 };
 
 template <int D, int R>
-__global__ void __launch_bounds__(kFewWarps * 32, 1)
+__global__ void __launch_bounds__(few_shape<D, R>::kWarps * 32, 1)
 tree_few_kernel(cache_view c, work_view w, few_lists lists, tree_view t, tree_parts parts, const int32_t* pages, int64_t table_stride, float shift)
 {
   using shape = few_shape<D, R>;
-  constexpr int KEYS = shape::kKeys, PARTS = shape::kParts, PITCH = shape::kPitch, COLUMNS = shape::kColumns, PIECES = D / 4;
+  constexpr int KEYS = shape::kKeys, PARTS = shape::kParts, PITCH = shape::kPitch, COLUMNS = shape::kColumns, PIECES = D / 4, WARPS = shape::kWarps;
   chain_begin();
   extern __shared__ __align__(16) float s_mem[];
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
@@ -306,7 +308,7 @@ tree_few_kernel(cache_view c, work_view w, few_lists lists, tree_view t, tree_pa
     const int32_t* positions    = t.positions + int64_t(now.sequence) * t.positions_stride;
     const char* keys            = c.keys + int64_t(head) * c.k_head * 4;
     const char* values          = c.values + int64_t(head) * c.v_head * 4;
-    for (uint32_t i = threadIdx.x; i < uint32_t(R * PIECES); i += kFewWarps * 32) {
+    for (uint32_t i = threadIdx.x; i < uint32_t(R * PIECES); i += WARPS * 32) {
       const uint32_t r = i / PIECES, p = i - r * PIECES;
       uint4 x = make_uint4(0, 0, 0, 0);
       if (r < rows && p < pieces) {
@@ -327,13 +329,14 @@ tree_few_kernel(cache_view c, work_view w, few_lists lists, tree_view t, tree_pa
       for (uint32_t i = lane; i < t.n_drafted; i += 32) { latest = max(latest, positions[i]); }
       latest = __reduce_max_sync(kAllLanes, latest);
     }
-    float top[R], sum[R], acc[R][COLUMNS];
+    float top[R], sum[R];
+    two acc[R][COLUMNS / 2];
 #pragma unroll
     for (int r = 0; r < R; r++) {
       top[r] = -INFINITY;
       sum[r] = 0.0f;
 #pragma unroll
-      for (int e = 0; e < COLUMNS; e++) { acc[r][e] = 0.0f; }
+      for (int e = 0; e < COLUMNS / 2; e++) { acc[r][e] = two(0.0f, 0.0f); }
     }
     __syncthreads();
 
@@ -376,11 +379,11 @@ tree_few_kernel(cache_view c, work_view w, few_lists lists, tree_view t, tree_pa
     bool there      = look(chunk, k_at, v_at);
     uint32_t valid  = chunk < now.end ? copy(0, there, k_at, v_at) : 0u;
     k_at = v_at     = 0;
-    there           = look(chunk + kFewWarps, k_at, v_at);
-    for (uint32_t stage = 0; chunk < now.end; chunk += kFewWarps, stage ^= 1u) {
+    there           = look(chunk + WARPS, k_at, v_at);
+    for (uint32_t stage = 0; chunk < now.end; chunk += WARPS, stage ^= 1u) {
       const uint32_t next_valid = copy(stage ^ 1u, there, k_at, v_at);
       k_at = v_at = 0;
-      there       = look(chunk + 2 * kFewWarps, k_at, v_at);
+      there       = look(chunk + 2 * WARPS, k_at, v_at);
       copies_wait<1>();
       __syncwarp();
       const float* s_k     = s_own + stage * shape::kStage;
@@ -390,82 +393,109 @@ tree_few_kernel(cache_view c, work_view w, few_lists lists, tree_view t, tree_pa
       uint32_t seen        = my_is ? valid : 0u;
       if (mixed && my_is) { seen &= seen_keys(t, l, positions, my_at, my_mask, base); }
       float s[R];
+      two s2[R];
 #pragma unroll
-      for (int r = 0; r < R; r++) { s[r] = 0.0f; }
+      for (int r = 0; r < R; r++) { s2[r] = two(0.0f, 0.0f); }
 #pragma unroll 4
       for (int d = 0; d < D; d += 4 * PARTS) {
         const float4 k = *reinterpret_cast<const float4*>(s_k + key_of * PITCH + d + part_of * 4);
 #pragma unroll
         for (int r = 0; r < R; r++) {
           const float4 q = *reinterpret_cast<const float4*>(s_q + r * D + d + part_of * 4);
-          s[r]           = fmaf(q.x, k.x, s[r]);
-          s[r]           = fmaf(q.y, k.y, s[r]);
-          s[r]           = fmaf(q.z, k.z, s[r]);
-          s[r]           = fmaf(q.w, k.w, s[r]);
+          s2[r]          = fma2(two(q.x, q.y), two(k.x, k.y), s2[r]);
+          s2[r]          = fma2(two(q.z, q.w), two(k.z, k.w), s2[r]);
         }
       }
 #pragma unroll
       for (int r = 0; r < R; r++) {
+        float u, v;
+        s2[r].get(u, v);
+        s[r] = u + v;
 #pragma unroll
         for (int o = 1; o < PARTS; o *= 2) { s[r] += __shfl_xor_sync(kAllLanes, s[r], o); }
       }
-      int32_t of = int32_t(base + key_of);  // the key's position
-      if (mixed && base + key_of >= l.length && base + key_of - l.length < t.n_drafted) { of = positions[base + key_of - l.length]; }
+      // (all rows side by side: those that are none see nothing)
+#pragma unroll
+      for (int r = 0; r < R; r++) { s[r] = t.cap_log2 != 0.0f ? tanhf(s[r] * t.scale_cap) * t.cap_log2 : s[r] * t.scale_log2; }
+      if (t.slopes != nullptr) {
+        int32_t of = int32_t(base + key_of);  // the key's position
+        if (mixed && base + key_of >= l.length && base + key_of - l.length < t.n_drafted) { of = positions[base + key_of - l.length]; }
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+          s[r] = fmaf(__shfl_sync(kAllLanes, my_slope, r), float(int64_t(of) - __shfl_sync(kAllLanes, my_at, r)), s[r]);
+        }
+      }
+      float next[R];
 #pragma unroll
       for (int r = 0; r < R; r++) {
-        if (uint32_t(r) >= rows) { continue; }
-        float score = t.cap_log2 != 0.0f ? tanhf(s[r] * t.scale_cap) * t.cap_log2 : s[r] * t.scale_log2;
-        if (t.slopes != nullptr) {
-          score = fmaf(__shfl_sync(kAllLanes, my_slope, r), float(int64_t(of) - __shfl_sync(kAllLanes, my_at, r)), score);
-        }
         const uint32_t sees = __shfl_sync(kAllLanes, seen, r);
-        score               = ((sees >> key_of) & 1u) != 0u ? score : -INFINITY;
-        float next          = score;
+        s[r]                = ((sees >> key_of) & 1u) != 0u ? s[r] : -INFINITY;
+        next[r]             = fmaxf(s[r], top[r]);
+      }
 #pragma unroll
-        for (int o = PARTS; o < 32; o *= 2) { next = fmaxf(next, __shfl_xor_sync(kAllLanes, next, o)); }
-        next             = fmaxf(next, top[r]);
-        const float safe = finite_top(next);
-        if (next != top[r]) {  // of the whole warp
-          const float keep = power_of_2(top[r] - safe);
-          top[r]           = next;
+      for (int o = PARTS; o < 32; o *= 2) {
+#pragma unroll
+        for (int r = 0; r < R; r++) { next[r] = fmaxf(next[r], __shfl_xor_sync(kAllLanes, next[r], o)); }
+      }
+      bool higher = false;
+#pragma unroll
+      for (int r = 0; r < R; r++) { higher = higher || next[r] != top[r]; }
+      if (higher) {  // of the whole warp
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+          const float keep = power_of_2(top[r] - finite_top(next[r]));
+          top[r]           = next[r];
           sum[r] *= keep;
 #pragma unroll
-          for (int e = 0; e < COLUMNS; e++) { acc[r][e] *= keep; }
+          for (int e = 0; e < COLUMNS / 2; e++) { acc[r][e] = mul2(acc[r][e], two(keep, keep)); }
         }
-        const float p = power_of_2(score - safe + shift);
+      }
+#pragma unroll
+      for (int r = 0; r < R; r++) {
+        const float p = power_of_2(s[r] - finite_top(top[r]) + shift);
         if (part_of == 0) {
           sum[r] += p;  // of the lane's own keys, until the end
-          s_p[r * 32 + key_of] = p;
+          reinterpret_cast<float2*>(s_p)[r * KEYS + key_of] = make_float2(p, p);
         }
       }
       __syncwarp();
 #pragma unroll 2
       for (int k = 0; k < KEYS; k += 4) {
-        float v[4][COLUMNS];
+        two v[4][COLUMNS / 2];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
           const float* row = s_v + (k + i) * PITCH;
           if constexpr (COLUMNS == 2) {
             const float2 x = *reinterpret_cast<const float2*>(row + lane * 2);
-            v[i][0] = x.x, v[i][1] = x.y;
+            v[i][0]        = two(x.x, x.y);
           } else {
 #pragma unroll
             for (int e = 0; e < COLUMNS; e += 4) {
-              const float4 x = *reinterpret_cast<const float4*>(row + e * 32 + lane * 4);
-              v[i][e] = x.x, v[i][e + 1] = x.y, v[i][e + 2] = x.z, v[i][e + 3] = x.w;
+              const float4 x  = *reinterpret_cast<const float4*>(row + e * 32 + lane * 4);
+              v[i][e / 2]     = two(x.x, x.y);
+              v[i][e / 2 + 1] = two(x.z, x.w);
             }
           }
         }
 #pragma unroll
         for (int r = 0; r < R; r++) {
-          if (uint32_t(r) >= rows) { continue; }
-          const float4 p4  = *reinterpret_cast<const float4*>(s_p + r * 32 + k);
-          const float p[4] = {p4.x, p4.y, p4.z, p4.w};
+          const float4* p4 = reinterpret_cast<const float4*>(s_p + (r * KEYS + k) * 2);
+          const float4 a = p4[0], b = p4[1];
+          const two p[4] = {two(a.x, a.y), two(a.z, a.w), two(b.x, b.y), two(b.z, b.w)};
+          if (!mixed) {
 #pragma unroll
-          for (int i = 0; i < 4; i++) {
-            if (mixed && p[i] == 0.0f) { continue; }  // what the row does not see may be infinite, or no number
+            for (int i = 0; i < 4; i++) {
 #pragma unroll
-            for (int e = 0; e < COLUMNS; e++) { acc[r][e] = fmaf(p[i], v[i][e], acc[r][e]); }
+              for (int e = 0; e < COLUMNS / 2; e++) { acc[r][e] = fma2(p[i], v[i][e], acc[r][e]); }
+            }
+          } else {  // what a row does not see may be infinite, or no number
+            const float weight[4] = {a.x, a.z, b.x, b.z};
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+              if (weight[i] == 0.0f) { continue; }
+#pragma unroll
+              for (int e = 0; e < COLUMNS / 2; e++) { acc[r][e] = fma2(p[i], v[i][e], acc[r][e]); }
+            }
           }
         }
       }
@@ -485,19 +515,25 @@ tree_few_kernel(cache_view c, work_view w, few_lists lists, tree_view t, tree_pa
         mine[1] = sum[r];
       }
 #pragma unroll
-      for (int e = 0; e < COLUMNS; e++) { mine[2 + (COLUMNS == 2 ? lane * 2 + e : (e / 4) * 128 + lane * 4 + e % 4)] = acc[r][e]; }
+      for (int e = 0; e < COLUMNS; e += 2) {
+        float u, v;
+        acc[r][e / 2].get(u, v);
+        float* at = mine + 2 + (COLUMNS == 2 ? lane * 2 : (e / 4) * 128 + lane * 4 + e % 4);
+        at[0]     = u;
+        at[1]     = v;
+      }
     }
     __syncthreads();
     const size_t part = parts.part(which, block, now.begins ? 1u : 0u);
-    for (uint32_t i = threadIdx.x; i < rows * pieces; i += kFewWarps * 32) {
+    for (uint32_t i = threadIdx.x; i < rows * pieces; i += WARPS * 32) {
       const uint32_t r = i / pieces, quad = i - r * pieces;
       float most = -INFINITY;
 #pragma unroll
-      for (int v = 0; v < kFewWarps; v++) { most = fmaxf(most, s_mem[v * shape::kOwn + r * (D + 2)]); }
+      for (int v = 0; v < WARPS; v++) { most = fmaxf(most, s_mem[v * shape::kOwn + r * (D + 2)]); }
       const float safe = finite_top(most);
       float total = 0.0f, x[4] = {};
 #pragma unroll
-      for (int v = 0; v < kFewWarps; v++) {
+      for (int v = 0; v < WARPS; v++) {
         const float* of = s_mem + v * shape::kOwn + r * (D + 2);
         const float f   = power_of_2(of[0] - safe);
         total           = fmaf(of[1], f, total);
@@ -517,7 +553,7 @@ tree_few_kernel(cache_view c, work_view w, few_lists lists, tree_view t, tree_pa
     if (now.begins && threadIdx.x == 0) { note_begun(parts, now, c.n_heads, which, begun); }
   }
   if (parts.begun != nullptr && !parts.by_unit && block == 0 && threadIdx.x == 0) { parts.begun[which] = begun; }
-  empty_tree_rows<float>(c, w.n_sequences, lists, t, parts, threadIdx.x, kFewWarps * 32);
+  empty_tree_rows<float>(c, w.n_sequences, lists, t, parts, threadIdx.x, WARPS * 32);
 }
 
 // Rows of a block, by how many a unit has; more of few than of many: the kernel for few.
@@ -532,7 +568,7 @@ tree_plan plan_of(const resources& res, elem type, uint64_t sequences, uint32_t 
   const uint64_t most = window > 0 && uint64_t(window) < capacity ? std::min(capacity, uint64_t(window) + n_drafted + 15) : capacity;
   if (type == elem::f32) {
     const uint32_t columns = tree_columns(dim);
-    if (n_rows <= kFew) { return deal_out_tree(sms, few_rows_of(n_rows, dim), 2048 / columns, 12, few_lists::kLeast, sequences * n_heads, n_rows, most); }
+    if (n_rows <= kFew) { return deal_out_tree(sms, few_rows_of(n_rows, dim), 1024 / columns, 24, few_lists::kLeast, sequences * n_heads, n_rows, most); }
     return deal_out_tree(sms * tree_resident(int(columns)), 64, columns <= 128 ? 64 : 32, 2, drafted_lists::kLeast, sequences * n_heads, n_rows, most);
   }
   return deal_out_tree(sms, dim <= 128 && n_rows > 128 ? 256 : 128, 64, 2, drafted_lists::kLeast, sequences * n_heads, n_rows, most);
@@ -610,9 +646,9 @@ void attend_tree(resources& res, cudaStream_t stream, const attend_tree_args& a)
   auto by_columns = [&](auto columns) {
     constexpr int D = decltype(columns)::value;
     if (t.n_rows > kFew) { return go(tree_rows_kernel<D>, call.lists, kThreads, tree_shape<D>::kShared); }
-    if (p.rows == 4) { return go(tree_few_kernel<D, 4>, few_lists{call.lists}, kFewWarps * 32, few_shape<D, 4>::kShared); }
-    if (p.rows == 8) { return go(tree_few_kernel<D, 8>, few_lists{call.lists}, kFewWarps * 32, few_shape<D, 8>::kShared); }
-    if constexpr (D <= 128) { go(tree_few_kernel<D, 16>, few_lists{call.lists}, kFewWarps * 32, few_shape<D, 16>::kShared); }
+    if (p.rows == 4) { return go(tree_few_kernel<D, 4>, few_lists{call.lists}, few_shape<D, 4>::kWarps * 32, few_shape<D, 4>::kShared); }
+    if (p.rows == 8) { return go(tree_few_kernel<D, 8>, few_lists{call.lists}, few_shape<D, 8>::kWarps * 32, few_shape<D, 8>::kShared); }
+    if constexpr (D <= 128) { go(tree_few_kernel<D, 16>, few_lists{call.lists}, few_shape<D, 16>::kWarps * 32, few_shape<D, 16>::kShared); }
   };
   using std::integral_constant;
   switch (tree_columns(c.dim)) {

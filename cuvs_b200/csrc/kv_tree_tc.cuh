@@ -52,32 +52,6 @@ __device__ __forceinline__ void registers_down()
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 
-// Two 32-bit numbers in one operation.
-struct two {
-  uint64_t v;
-  __device__ __forceinline__ two() {}
-  __device__ __forceinline__ two(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
-  __device__ __forceinline__ void get(float& a, float& b) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
-};
-__device__ __forceinline__ two fma2(two a, two b, two c)
-{
-  two d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-  return d;
-}
-__device__ __forceinline__ two mul2(two a, two b)
-{
-  two d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
-  return d;
-}
-__device__ __forceinline__ two add2(two a, two b)
-{
-  two d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
-  return d;
-}
-
 // A weight of 32 bits as the sum of two 16-bit numbers, so that a row of the output is off by little more than its own rounding: what one number
 // loses (2^-9 of each weight in bf16, 2^-12 in fp16) is as much as that.  The second number is never 0 where the first is not: 0 times an infinite value
 // would be no number.
