@@ -9,65 +9,71 @@ namespace {
 
 // ---- draft_tree ---------------------------------------------------------------------------------------------------------------
 //
-// A token reaches itself and what its parent reaches.  Every token looks 1, 2, 4, .. steps up: after k rounds `next` is the ancestor 2^k steps up
-// (or how the way ends) and the token's bits are those of the 2^k - 1 nearest ancestors and its own; a round adds the bits of `next` and takes
-// its `next`.  ceil(log2 n) rounds see a whole tree in whatever order its tokens stand, and a way that has not ended by then goes in a circle.
+// A token reaches itself and what its parent reaches.  Every token looks 1, 2, 4, .. steps up: after k rounds `up` is the ancestor 2^k steps up
+// (or how the way ends) and the token's bits are those of the 2^k - 1 nearest ancestors and its own; a round adds the bits of `up` and takes
+// its `up`.  ceil(log2 n) rounds see a whole tree in whatever order its tokens stand, and a way that has not ended by then goes in a circle.
 //
-// What bounds it: the latency of a launch and of the rounds, which one block makes per sequence in shared memory.
+// What bounds it: the latency of a launch and of the rounds, which one block makes per sequence in shared memory, a thread per token with the token's
+// words in registers.  (A thread per word, with their divisions: 64 trees of 255 tokens 10.7 us.)
 constexpr int32_t kNoToken = -2, kFollows = -1;
 
 __global__ void __launch_bounds__(1024) draft_tree_kernel(draft_tree_args a)
 {
   chain_begin();
-  constexpr uint32_t kMost = 32;  // words of a thread: 1,024 tokens of 32 words in 1,024 threads
+  constexpr uint32_t kMost = 32;  // words of 1,024 tokens
   extern __shared__ uint32_t s_words[];
-  const uint32_t n = a.n_drafted, words = (n + 31) / 32, sequence = blockIdx.x;
-  uint32_t* s_bits       = s_words;
-  int32_t* s_next        = reinterpret_cast<int32_t*>(s_words + n * words);
-  const int32_t* parents = a.parents + int64_t(sequence) * a.parents_stride;
-  const int64_t length   = max(a.lengths[sequence], 0);
-  for (uint32_t i = threadIdx.x; i < n; i += blockDim.x) {
-    const int32_t p = parents[i];
-    s_next[i]       = p >= kFollows && p < int32_t(n) ? p : kNoToken;
+  const uint32_t n = a.n_drafted, words = (n + 31) / 32, pitch = words | 1u, sequence = blockIdx.x, token = threadIdx.x;
+  int32_t* s_up        = reinterpret_cast<int32_t*>(s_words + n * pitch);
+  const bool exists    = token < n;
+  const int64_t length = max(a.lengths[sequence], 0);
+  const int32_t parent = exists ? a.parents[int64_t(sequence) * a.parents_stride + token] : kNoToken;
+  int32_t up           = parent >= kFollows && parent < int32_t(n) ? parent : kNoToken;
+  uint32_t bits[kMost];
+#pragma unroll
+  for (uint32_t word = 0; word < kMost; word++) {
+    if (word >= words) { break; }
+    bits[word] = word == token / 32 ? 1u << (token & 31u) : 0u;
+    if (exists) { s_words[token * pitch + word] = bits[word]; }
   }
-  for (uint32_t i = threadIdx.x; i < n * words; i += blockDim.x) {
-    const uint32_t token = i / words, word = i - token * words;
-    s_bits[i]            = word == token / 32 ? 1u << (token & 31u) : 0u;
-  }
+  if (exists) { s_up[token] = up; }
   __syncthreads();
   for (uint32_t reach = 1; reach < n; reach *= 2) {  // the way of a chain of n tokens ends n steps up
-    uint32_t bits[kMost];
-    int32_t next[kMost];
+    int32_t next = up;
+    if (up >= 0) {
 #pragma unroll
-    for (uint32_t u = 0; u < kMost; u++) {
-      const uint32_t i = threadIdx.x + u * blockDim.x;
-      if (i >= n * words) { break; }
-      const uint32_t token = i / words, word = i - token * words;
-      const int32_t up     = s_next[token];
-      bits[u]              = up >= 0 ? s_bits[up * words + word] : 0u;
-      next[u]              = word == 0 && up >= 0 ? s_next[up] : up;
+      for (uint32_t word = 0; word < kMost; word++) {
+        if (word >= words) { break; }
+        bits[word] |= s_words[up * pitch + word];
+      }
+      next = s_up[up];
     }
-    __syncthreads();
+    if (__syncthreads_or(up >= 0) == 0) { break; }  // all have read; all ways have ended
+    if (up >= 0) {
 #pragma unroll
-    for (uint32_t u = 0; u < kMost; u++) {
-      const uint32_t i = threadIdx.x + u * blockDim.x;
-      if (i >= n * words) { break; }
-      const uint32_t token = i / words;
-      s_bits[i] |= bits[u];
-      if (i == token * words) { s_next[token] = next[u]; }
+      for (uint32_t word = 0; word < kMost; word++) {
+        if (word >= words) { break; }
+        s_words[token * pitch + word] = bits[word];
+      }
+      up          = next;
+      s_up[token] = up;
     }
     __syncthreads();
   }
-  for (uint32_t token = threadIdx.x; token < n; token += blockDim.x) {
-    int64_t position = length - 1;
-    for (uint32_t word = 0; word < words; word++) { position += __popc(s_bits[token * words + word]); }
-    const bool there = s_next[token] == kFollows && position <= 0x7FFFFFFF;
-    if (!there) { s_next[token] = kNoToken; }
+  int64_t position = length - 1;
+#pragma unroll
+  for (uint32_t word = 0; word < kMost; word++) {
+    if (word >= words) { break; }
+    position += __popc(bits[word]);
+  }
+  const bool there = up == kFollows && position <= 0x7FFFFFFF;
+  if (exists) {
+    s_up[token] = there;
     a.positions[size_t(sequence) * n + token] = there ? int32_t(position) : -1;
   }
   __syncthreads();
   for (uint32_t i = threadIdx.x; i < n * words; i += blockDim.x) {
-    a.mask[size_t(sequence) * n * words + i] = s_next[i / words] == kFollows ? s_bits[i] : 0u;
+    const uint32_t of = i / words;
+    a.mask[size_t(sequence) * n * words + i] = s_up[of] != 0 ? s_words[of * pitch + (i - of * words)] : 0u;
   }
 }
 
@@ -194,9 +200,9 @@ void draft_tree(resources& res, cudaStream_t stream, const draft_tree_args& a)
 {
   if (a.n_sequences == 0 || a.n_drafted == 0) { return; }
   const uint32_t words = ceildiv(a.n_drafted, 32u);
-  const size_t smem    = (size_t(a.n_drafted) * words + a.n_drafted) * sizeof(uint32_t);
+  const size_t smem    = size_t(a.n_drafted) * ((words | 1u) + 1) * sizeof(uint32_t);
   if (smem > 48 * 1024) { ensure_dynamic_smem(reinterpret_cast<const void*>(draft_tree_kernel), smem); }
-  const uint32_t threads = std::min<uint32_t>(1024, std::max<uint32_t>(64, round_up(a.n_drafted * words, 32u)));
+  const uint32_t threads = round_up(a.n_drafted, 32u);
   launch_chained(draft_tree_kernel, dim3(a.n_sequences), threads, smem, stream, a);
   count_launches(res, 1);
 }
