@@ -58,7 +58,7 @@ struct tree_piece {
 
 struct tc_shared {
   uint64_t k_full[kMostStages], k_empty[kMostStages], v_full[kMostStages], v_empty[kMostStages];
-  uint64_t q_full, q_empty, s_full[4], p_full[4], pv_done[2], o_full[2], exchanged, drained[2], turn[2][4];
+  uint64_t q_full, q_empty, s_full[4], p_full[4], pv_done[2], o_full[2], exchanged, drained[2];
   uint64_t piece_full[kPieces], piece_empty[kPieces];
   tree_piece pieces[kPieces];
   uint2 valid[kInfos];  // of the two warps that copy keys: which are there
@@ -423,8 +423,7 @@ __device__ __forceinline__ void softmax_role(const tc_args& a, tc_shared& sh, ch
   const uint32_t width = (a.c.dim + 31) / 32;  // columns of the sums, in 32
   piece_reader reader;
   tree_piece p;
-  const bool in_turns = both && 128 + quarter * 32 < rows;  // both streams' warps of this quarter have rows
-  uint32_t e_turn = 0, s_turn = 0, o_turn = 0, x_turn = 0, tiles = 0, pv_turn = 0;  // s_turn: a bit for each buffer
+  uint32_t s_turn = 0, o_turn = 0, x_turn = 0, tiles = 0, pv_turn = 0;  // s_turn: a bit for each buffer
 
   while (reader.next(sh, wait, p)) {
     const uint32_t n = p.end - p.chunk;
@@ -508,11 +507,6 @@ __device__ __forceinline__ void softmax_role(const tc_args& a, tc_shared& sh, ch
         sum *= keep;
         top = next;
       }
-      // Exponentials are what the two streams' warps of a scheduler share: they take turns at them, and do the rest meanwhile.
-      if (in_turns) {
-        if (!wait(sh.turn[stream][quarter], e_turn + 1 - stream)) { ok = false; break; }
-        e_turn++;
-      }
       const float from = a.shift - finite_top(top), by = SHAPED ? 1.0f : t.scale_log2;
       const two from2(from, from), by2(by, by);
       two part[2] = {two(0.0f, 0.0f), two(0.0f, 0.0f)};
@@ -530,7 +524,6 @@ __device__ __forceinline__ void softmax_role(const tc_args& a, tc_shared& sh, ch
         }
         tmem_st32(scores + i * 32, pairs);
       }
-      if (in_turns) { arrive_warp(sh.turn[1 - stream][quarter]); }
       tmem_st_wait();
       {
         float u, v;
@@ -764,7 +757,6 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
     mbar_init(smem_u32(&sh.pv_done[1]), 1);
     mbar_init(smem_u32(&sh.o_full[0]), 1);
     mbar_init(smem_u32(&sh.o_full[1]), 1);
-    for (int i = 0; i < 8; i++) { mbar_init(smem_u32(&sh.turn[i / 4][i % 4]), 1); }
     mbar_init(smem_u32(&sh.exchanged), 8);
     mbar_init(smem_u32(&sh.drained[0]), 1);
     mbar_init(smem_u32(&sh.drained[1]), 1);
