@@ -229,8 +229,10 @@ tree_join_kernel(tree_view t, tree_parts parts, uint32_t dim, uint32_t n_heads, 
   const uint32_t groups = ceildiv(min(parts.rows, t.n_rows), 32u);
   const uint32_t entry = blockIdx.x / (groups * parts.blocks_of), rest = blockIdx.x - entry * (groups * parts.blocks_of);
   const uint32_t block = rest / groups, r = (rest - block * groups) * 32 + lane;
-  const uint4 unit = parts.begun[entry];
-  const uint32_t n = unit.z, share = unit.w, row = block * parts.rows + r;
+  uint4 unit = parts.begun[entry];
+  // (an entry that nothing has written, where lengths changed meanwhile, leads nowhere else)
+  if (parts.by_unit) { unit.x = entry / n_heads, unit.y = entry - unit.x * n_heads; }
+  const uint32_t share = unit.w, n = share < parts.shares ? min(unit.z, parts.shares - share) : 0u, row = block * parts.rows + r;
   if (n == 0u || block * parts.rows + (r - lane) >= t.n_rows) { return; }
   const bool there = r < parts.rows && row < t.n_rows;
   const uint32_t rr = min(r, parts.rows - 1u);

@@ -10,6 +10,30 @@ namespace {
 
 constexpr int kThreads = 256;
 
+// What a block's first warp finds of its share, for all of them: lengths that somebody changes meanwhile must not lead them apart.
+struct found_piece {
+  piece now;
+  drafted_lists::list l;
+  uint32_t more;
+};
+template <class Walk>
+__device__ __forceinline__ bool next_piece(Walk& path, found_piece& found, piece& now, drafted_lists::list& l)
+{
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    const bool more = path.next(now);
+    if (threadIdx.x == 0) {
+      found.more = more;
+      found.now  = now;
+      found.l    = path.l;
+    }
+  }
+  __syncthreads();
+  now = found.now;
+  l   = found.l;
+  return found.more != 0u;
+}
+
 // Blocks of an SM: what shared memory and registers leave room for.  They hide each other's loads.
 constexpr int tree_resident(int columns) { return columns == 64 ? 3 : 1; }
 
@@ -61,8 +85,9 @@ tree_rows_kernel(cache_view c, work_view w, drafted_lists lists, tree_view t, tr
   walk<TILE, drafted_lists> path(c, w, lists, parts.shares, which);
   piece now;
   uint4 begun = make_uint4(0, 0, 0, 0);
-  while (__syncthreads_and(path.next(now)) != 0) {
-    const drafted_lists::list l = path.l;
+  __shared__ found_piece s_found;
+  drafted_lists::list l;
+  while (next_piece(path, s_found, now, l)) {
     const uint32_t head         = now.unit;
     const int32_t* table        = pages + int64_t(now.sequence) * table_stride;
     const int32_t* positions    = t.positions + int64_t(now.sequence) * t.positions_stride;
@@ -274,12 +299,12 @@ struct few_shape {
   static constexpr int kPitch  = D + 4 * kParts;  // floats: eight lanes' pieces on different banks
   static constexpr int kStage  = 2 * kKeys * kPitch;
   static constexpr int kOwn    = 2 * kStage + R * kKeys * 2;  // of a warp: two stages, weights (each twice)
-  static constexpr int kFit    = (232448 / 4 - R * D) / kOwn;
+  static constexpr int kFit    = (232448 / 4 - 64 - R * D) / kOwn;  // (64: what found_piece takes)
   static constexpr int kWarps  = kFit < kFewMost ? kFit : kFewMost;
   static constexpr int kQAt    = kWarps * kOwn;
   static constexpr int kShared = (kQAt + R * D) * 4;
   static constexpr int kColumns = D / 32;    // of a lane
-  static_assert(kShared <= 232448 && R * (D + 2) <= kOwn, "");
+  static_assert(kShared + int(sizeof(found_piece)) <= 232448 && sizeof(found_piece) <= 256 && R * (D + 2) <= kOwn, "");
 };
 
 template <int D, int R>
@@ -301,8 +326,9 @@ tree_few_kernel(cache_view c, work_view w, few_lists lists, tree_view t, tree_pa
   walk<KEYS, few_lists> path(c, w, lists, parts.shares, which);
   piece now;
   uint4 begun = make_uint4(0, 0, 0, 0);
-  while (__syncthreads_and(path.next(now)) != 0) {
-    const drafted_lists::list l = path.l;
+  __shared__ found_piece s_found;
+  drafted_lists::list l;
+  while (next_piece(path, s_found, now, l)) {
     const uint32_t head         = now.unit;
     const int32_t* table        = pages + int64_t(now.sequence) * table_stride;
     const int32_t* positions    = t.positions + int64_t(now.sequence) * t.positions_stride;

@@ -1,14 +1,18 @@
 // Attention of drafted tokens to the 16-bit rows of their sequences in a paged cache, on tensor cores (the mathematics: kv_tree.cuh).
 //
-// A block has 128 query rows, or twice 128, and goes through its share's tiles of 128 keys (64 where rows have more than 128 columns).  One warp issues
+// A block has 128 query rows, or twice 128, and goes through its share's tiles of 64 keys.  A warp for each of two streams issues
 // tcgen05.mma: scores S = Q K^T into tensor memory; four warps of 32 rows each, a thread a row, read them, carry the softmax (top and sum in 32
-// bits) and write the weights back over them as two 16-bit numbers; the same warp issues O += P V with P from tensor memory.  Four more
-// warps copy rows of keys and values, 16 bytes at a time, into a ring of tiles, in the order in which they are wanted, and one finds the way through the
-// share.  Two streams of tiles keep the tensor core busy while one of them is at its softmax: the two halves of 256 rows on the same tiles, or even
-// and odd tiles of the same 128 rows, whose sums are joined at a unit's end.  Rows of more than 128 columns leave tensor memory room for one
-// sum only: there the scores of two tiles take turns.
+// bits) and write the weights back over them as two 16-bit numbers; the stream's warp issues O += P V with P from tensor memory.  Four more
+// warps copy rows of keys and values, 16 bytes at a time, into a ring of tiles for each, and one finds the way through the share.  The streams are the two
+// halves of 256 rows on the same tiles, or even and odd tiles of the same 128 rows, whose sums are joined at a unit's end.  Each has two tiles of scores,
+// so that the next ones are formed while the softmax is at the last.  Rows of more than 128 columns leave tensor memory room for one stream.
 //
 // Sums are brought to a new top only where it is 2^4 above the old one: a turn through tensor memory that few tiles need.
+//
+// What bounds it: of 256 rows the softmax, 2,300 clocks of 64 keys where the products are 1,800 (with pairs of weights half again those of one
+// number): one request of 250,001 + 64 tokens, 4 key heads of 7, fp16, 348 us (658 TFLOP/s of what is asked for, 1.5 TB/s); 16 requests
+// of up to 16,384 + 32 tokens, 8 key heads of 8, bf16, 211 us, with a cap 262.  Of 32 rows HBM and the blocks' starts: the same with 4 tokens of 4 heads
+// each 121 us (3.6 TB/s).
 #include "kv_tree_tc.cuh"
 
 #include <algorithm>
@@ -24,7 +28,8 @@ constexpr int kPieces     = 2;
 constexpr int kReaders    = 14;   // warps that read a piece's description
 constexpr uint32_t kTile  = 64;   // keys
 constexpr int kMostStages = 8;    // of keys, and of values
-constexpr uint32_t kLimit = kSpinLimit;
+constexpr uint32_t kLimit = kSpinLimit;       // of waits for a tile
+constexpr uint32_t kPatience = kSpinLimit * 32;  // of waits for a piece, which may be all of a sequence
 
 template <int D>
 struct tc_shape {
@@ -85,9 +90,9 @@ constexpr uint32_t kNoMore = 0xFFFFFFFFu;
 // Waits with a limit, after which the block gives up; a whole warp at a time.
 struct waiter {
   tc_shared& sh;
-  __device__ __forceinline__ bool operator()(const uint64_t& bar, uint32_t parity) const
+  __device__ __forceinline__ bool operator()(const uint64_t& bar, uint32_t parity, uint32_t limit = kLimit) const
   {
-    if (mbar_wait_warp(smem_u32(&bar), parity & 1u, kLimit)) { return true; }
+    if (mbar_wait_warp(smem_u32(&bar), parity & 1u, limit)) { return true; }
     *const_cast<volatile uint32_t*>(&sh.failed) = 1u;
     return false;
   }
@@ -103,7 +108,7 @@ struct piece_reader {
   uint32_t i = 0;
   __device__ __forceinline__ bool next(tc_shared& sh, const waiter& wait, tree_piece& p)
   {
-    if (!wait(sh.piece_full[i % kPieces], i / kPieces)) { return false; }
+    if (!wait(sh.piece_full[i % kPieces], i / kPieces, kPatience)) { return false; }
     p = sh.pieces[i % kPieces];
     arrive_warp(sh.piece_empty[i % kPieces]);
     i++;
@@ -711,7 +716,7 @@ __device__ __forceinline__ void way_role(const tc_args& a, tc_shared& sh, const 
       for (uint32_t k = lane; k < a.t.n_drafted; k += 32) { latest = max(latest, positions[k]); }
       latest = __reduce_max_sync(kAllLanes, latest);
     }
-    if (i >= kPieces && !wait(sh.piece_empty[i % kPieces], i / kPieces - 1)) { return; }
+    if (i >= kPieces && !wait(sh.piece_empty[i % kPieces], i / kPieces - 1, kPatience)) { return; }
     if (lane == 0) {
       tree_piece p{};
       p.sequence = kNoMore;
