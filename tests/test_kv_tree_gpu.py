@@ -543,3 +543,56 @@ def test_copies(dtype, heads_outside, heads, dim, page_size, n):
         t[targets[:n].long()] = t[sources[:n].long()]
     kv_cache.copy_pages(keys, values, sources, targets)
     assert torch.equal(keys, want[0]) and torch.equal(values, want[1])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,group,dim", [(2, 4, 128), (6, 1, 64), (40, 8, 64), (64, 4, 128), (9, 4, 256)])
+def test_scores_that_rise_and_fall(dtype, m, group, dim):
+    """A row's largest score so far grows with every tile of keys, by many powers of two; then all keys are far below it."""
+    for falls in (False, True):
+        step = Step(dtype, [1200, 700], m, 2, group, dim, 16)
+        slot = step.allowed()[1]
+        step.queries.abs_()
+        for i, n in enumerate((1200, 700)):
+            s = slot[i, :n + m]
+            rise = torch.linspace(0.0, 60.0 / dim ** 0.5, n + m, device="cuda").to(dtype)
+            rise = rise.flip(0) if falls else rise
+            step.keys[s // 16, s % 16] = (step.keys[s // 16, s % 16].float() * 0.1 + rise.float()[:, None, None]).to(dtype)
+        check(step)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,group", [(3, 4), (40, 8)])
+def test_slots_that_are_all_left_out(dtype, m, group):
+    step = Step(dtype, [500, 64], m, 2, group, 128, 16)
+    n_words = -(-step.keys.shape[0] * 16 // 32)
+    none = torch.zeros(n_words, dtype=torch.uint32, device="cuda")
+    out, lse = step.call(filter=none)
+    assert (out == 0).all() and (lse == -math.inf).all()
+    # all but the drafted tokens' own
+    bits = torch.zeros((n_words, 32), dtype=torch.int64, device="cuda")
+    slot = step.allowed()[1]
+    for i, n in enumerate((500, 64)):
+        s = slot[i, n:n + m]
+        bits[s // 32, s % 32] = 1
+    check(step, filter=(bits << torch.arange(32, device="cuda")).sum(1).to(torch.uint32))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,group", [(1024, 1), (300, 4), (1, 16)])
+def test_the_largest_trees(dtype, m, group):
+    check(Step(dtype, [150, 0], m, 1, group, 64, 16, spread=0.1))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_lengths_around_the_ends_of_tiles(dtype, dim):
+    lengths = [15, 16, 17, 31, 33, 47, 61, 62, 63, 64, 65, 66, 126, 127, 128, 129, 191, 192, 193, 255, 256, 257]
+    for m, group in ((1, 2), (2, 8), (33, 5)):
+        check(Step(dtype, lengths, m, 1, group, dim, 16 if m != 2 else 24))
+
+
+def test_groups_that_are_no_power_of_two_and_many_key_heads():
+    for dtype in DTYPES:
+        check(Step(dtype, [100, 40], 11, 13, 3, 64, 16))
+        check(Step(dtype, [100, 40], 3, 40, 11, 32, 10))
