@@ -582,9 +582,12 @@ tree_few_kernel(cache_view c, work_view w, few_lists lists, tree_view t, tree_pa
   empty_tree_rows<float>(c, w.n_sequences, lists, t, parts, threadIdx.x, WARPS * 32);
 }
 
-// Rows of a block, by how many a unit has; more of few than of many: the kernel for few.
+// Rows of a block of the kernel for few, by how many a unit has.
 constexpr uint32_t few_rows_of(uint32_t n_rows, uint32_t dim) { return n_rows <= 4 ? 4 : n_rows <= 8 || dim > 128 ? 8 : 16; }
-constexpr uint32_t kFew = 32;
+// Which kernel: 4 sequences of 20,000 tokens, 2 key heads, us by warps alone and in tiles of 64 rows: 64 columns 16 rows 46 and 78, 32 rows 68 and 79,
+// 40 rows 100 and 81; 128 columns 16 rows 83 and 157, 32 rows 146 and 157, 40 rows 213 and 173; 256 columns 32 rows 223 and 376, 48 rows 324 and
+// 381, 64 rows 423 and 382.
+constexpr bool is_few(uint32_t n_rows, uint32_t dim) { return n_rows <= (dim <= 128 ? 32u : 48u); }
 
 tree_plan plan_of(const resources& res, elem type, uint64_t sequences, uint32_t n_drafted, uint32_t n_heads, uint32_t group, uint32_t dim,
                   uint64_t capacity, int64_t window)
@@ -594,7 +597,7 @@ tree_plan plan_of(const resources& res, elem type, uint64_t sequences, uint32_t 
   const uint64_t most = window > 0 && uint64_t(window) < capacity ? std::min(capacity, uint64_t(window) + n_drafted + 15) : capacity;
   if (type == elem::f32) {
     const uint32_t columns = tree_columns(dim);
-    if (n_rows <= kFew) { return deal_out_tree(sms, few_rows_of(n_rows, dim), 1024 / columns, 24, few_lists::kLeast, sequences * n_heads, n_rows, most); }
+    if (is_few(n_rows, dim)) { return deal_out_tree(sms, few_rows_of(n_rows, dim), 1024 / columns, 24, few_lists::kLeast, sequences * n_heads, n_rows, most); }
     return deal_out_tree(sms * tree_resident(int(columns)), 64, columns <= 128 ? 64 : 32, 2, drafted_lists::kLeast, sequences * n_heads, n_rows, most);
   }
   return deal_out_tree(sms, dim <= 128 && n_rows > 128 ? 256 : 128, 64, 2, drafted_lists::kLeast, sequences * n_heads, n_rows, most);
@@ -671,7 +674,7 @@ void attend_tree(resources& res, cudaStream_t stream, const attend_tree_args& a)
   };
   auto by_columns = [&](auto columns) {
     constexpr int D = decltype(columns)::value;
-    if (t.n_rows > kFew) { return go(tree_rows_kernel<D>, call.lists, kThreads, tree_shape<D>::kShared); }
+    if (!is_few(t.n_rows, c.dim)) { return go(tree_rows_kernel<D>, call.lists, kThreads, tree_shape<D>::kShared); }
     if (p.rows == 4) { return go(tree_few_kernel<D, 4>, few_lists{call.lists}, few_shape<D, 4>::kWarps * 32, few_shape<D, 4>::kShared); }
     if (p.rows == 8) { return go(tree_few_kernel<D, 8>, few_lists{call.lists}, few_shape<D, 8>::kWarps * 32, few_shape<D, 8>::kShared); }
     if constexpr (D <= 128) { go(tree_few_kernel<D, 16>, few_lists{call.lists}, few_shape<D, 16>::kWarps * 32, few_shape<D, 16>::kShared); }
