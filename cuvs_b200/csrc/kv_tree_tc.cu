@@ -41,7 +41,7 @@ struct tc_shape {
   static constexpr int kQBytes    = kQPanel * (D / 64);
   static constexpr int kExchange  = kQBytes;  // where two groups exchange sums: behind the first 128 rows
   static constexpr int kQRegion   = !kTwo ? kQBytes : 2 * kQBytes > kQBytes + 32768 ? 2 * kQBytes : kQBytes + 32768;
-  static constexpr int kMisc      = 3072;
+  static constexpr int kMisc      = 3200;  // tc_shared
   static constexpr int kFit       = (232448 - kQRegion - kMisc) / kTileBytes;
   static constexpr int kKeys      = kFit / 2 < kMostStages ? kFit / 2 : kMostStages;  // tiles of keys in flight, and of values
   static constexpr int kValues    = kFit - kKeys < kMostStages ? kFit - kKeys : kMostStages;
@@ -71,7 +71,7 @@ struct tc_shared {
   float2 stats[2][128];
   uint32_t tmem, failed;
 };
-static_assert(sizeof(tc_shared) <= 3072, "");
+static_assert(sizeof(tc_shared) <= 3200, "");
 
 struct tc_args {
   cache_view c;
