@@ -34,11 +34,14 @@ __device__ __forceinline__ bool next_piece(Walk& path, found_piece& found, piece
   return found.more != 0u;
 }
 
-// Blocks of an SM: what shared memory and registers leave room for.  They hide each other's loads.
-constexpr int tree_resident(int columns) { return columns == 64 ? 3 : 1; }
+// Blocks of an SM: what shared memory leaves room for.
+constexpr int tree_resident(int columns) { return columns == 64 ? 2 : 1; }
 
 // D: columns of a row in shared memory; BM: rows of a block.  Threads stand in 16 x 16: thread (y, x) has BM / 16 rows, their scores with every 16th key
 // and their weighted sums in every 16th four columns.
+//
+// What bounds it: 32-bit multiply-adds, and the barriers between a tile's steps with few blocks of an SM.  One sequence of 20,000 + 64 tokens, 2 key heads of 4,
+// 128 columns: 210 us, 25 TFLOP/s (264 where a tile was loaded between barriers).
 template <int D>
 struct tree_shape {
   static constexpr int BM     = 64;
@@ -48,12 +51,12 @@ struct tree_shape {
   static constexpr int kQuads = D / 64;
   static constexpr int kPitch = D + 4;      // floats: 16 lanes' quads of different rows on different banks
   static constexpr int kKAt   = BM * kPitch;
-  static constexpr int kVAt   = kKAt + kTile * kPitch;
-  static constexpr int kPAt   = kVAt + kTile * kPitch;
+  static constexpr int kStage = 2 * kTile * kPitch;  // keys, values; two of them: a tile is copied while the one before it is worked on
+  static constexpr int kPAt   = kKAt + 2 * kStage;
   static constexpr int kSeenAt = kPAt + BM * (kTile + 4);
   static constexpr int kValidAt = kSeenAt + BM * (kTile / 32);
   static constexpr int kPlaceAt = kValidAt + 4;
-  static constexpr int kShared = (kPlaceAt + 3 * kTile) * 4;
+  static constexpr int kShared = (kPlaceAt + 2 * 3 * kTile) * 4;
   static constexpr int kResident = tree_resident(D);
   static_assert(kResident * (kShared + 1024) <= 233472, "");
 };
@@ -69,14 +72,11 @@ tree_rows_kernel(cache_view c, work_view w, drafted_lists lists, tree_view t, tr
   chain_begin();
   extern __shared__ __align__(16) float s_mem[];
   float* s_q        = s_mem;
-  float* s_k        = s_mem + shape::kKAt;
-  float* s_v        = s_mem + shape::kVAt;
   float* s_p        = s_mem + shape::kPAt;
   uint32_t* s_seen  = reinterpret_cast<uint32_t*>(s_mem + shape::kSeenAt);
-  uint32_t* s_valid = reinterpret_cast<uint32_t*>(s_mem + shape::kValidAt);
-  uint32_t* s_k_at  = reinterpret_cast<uint32_t*>(s_mem + shape::kPlaceAt);
-  uint32_t* s_v_at  = s_k_at + TILE;
-  int32_t* s_of     = reinterpret_cast<int32_t*>(s_v_at + TILE);  // the keys' positions
+  uint32_t* s_valid_of[2] = {reinterpret_cast<uint32_t*>(s_mem + shape::kValidAt), reinterpret_cast<uint32_t*>(s_mem + shape::kValidAt) + 2};
+  // of each stage: places of keys, of values, the keys' positions
+  auto places = [&](uint32_t stage) { return reinterpret_cast<uint32_t*>(s_mem + shape::kPlaceAt) + stage * (3 * TILE); };
   const uint32_t y = threadIdx.x / 16, x = threadIdx.x % 16;
   const uint32_t which = blockIdx.x / t.n_blocks_of, block = blockIdx.x - which * t.n_blocks_of;
   const uint32_t row0 = block * BM, rows = min(uint32_t(BM), t.n_rows - row0);
@@ -120,45 +120,58 @@ tree_rows_kernel(cache_view c, work_view w, drafted_lists lists, tree_view t, tr
       for (uint32_t i = 0; i < t.n_drafted; i++) { latest = max(latest, positions[i]); }
     }
 
-    for (uint32_t tile = now.chunk; tile < now.end; tile++) {
-      const uint32_t base = l.base + tile * TILE;
-      const bool mixed    = int64_t(base) + TILE > int64_t(l.length) || (t.window > 0 && int64_t(base) <= int64_t(latest) - t.window);
-      if (threadIdx.x < TILE) {
-        const uint32_t at = base + threadIdx.x;
-        bool there        = at >= l.first && at < l.end;
-        uint32_t column, place;
-        split_place(min(at, 0x7FFFFFFFu), c.page, column, place);
-        const int32_t page = there ? table[column] : -1;  // at < end: the column is inside the table
-        there              = there && page >= 0 && page < c.n_pages;
-        if (there && c.filter != nullptr) {
-          const uint64_t slot = uint64_t(page) * c.page.size + place;
-          there               = (c.filter[slot >> 5] >> (slot & 31u)) & 1u;
-        }
-        int32_t of = int32_t(at);
-        if (there && at >= l.length) {
-          of    = positions[at - l.length];
-          there = of >= 0 && uint32_t(of) >= l.length;
-        }
-        s_k_at[threadIdx.x] = there ? uint32_t(page) * c.k_page_units + place * c.k_token_units : 0u;
-        s_v_at[threadIdx.x] = there ? uint32_t(page) * c.v_page_units + place * c.v_token_units : 0u;
-        s_of[threadIdx.x]   = of;
-        const uint32_t word = __ballot_sync(kAllLanes, there);
-        if ((threadIdx.x & 31u) == 0) { s_valid[threadIdx.x / 32] = word; }
+    auto look = [&](uint32_t tile, uint32_t stage) {
+      if (threadIdx.x >= TILE) { return; }
+      const uint32_t at = l.base + tile * TILE + threadIdx.x;
+      bool there        = at >= l.first && at < l.end;
+      uint32_t column, place;
+      split_place(min(at, 0x7FFFFFFFu), c.page, column, place);
+      const int32_t page = there ? table[column] : -1;  // at < end: the column is inside the table
+      there              = there && page >= 0 && page < c.n_pages;
+      if (there && c.filter != nullptr) {
+        const uint64_t slot = uint64_t(page) * c.page.size + place;
+        there               = (c.filter[slot >> 5] >> (slot & 31u)) & 1u;
       }
-      __syncthreads();
+      int32_t of = int32_t(at);
+      if (there && at >= l.length) {
+        of    = positions[at - l.length];
+        there = of >= 0 && uint32_t(of) >= l.length;
+      }
+      uint32_t* at_stage               = places(stage) + threadIdx.x;
+      at_stage[0]                      = there ? uint32_t(page) * c.k_page_units + place * c.k_token_units : 0u;
+      at_stage[TILE]                   = there ? uint32_t(page) * c.v_page_units + place * c.v_token_units : 0u;
+      at_stage[2 * TILE]               = uint32_t(of);
+      const uint32_t word = __ballot_sync(kAllLanes, there);
+      if ((threadIdx.x & 31u) == 0) { s_valid_of[stage][threadIdx.x / 32] = word; }
+    };
+    // rows that are not there, and columns behind a row's end: 0
+    auto load = [&](uint32_t stage) {
+      const uint32_t to = shared_address(s_mem + shape::kKAt + stage * shape::kStage);
+      const char *keys = c.keys + int64_t(head) * c.k_head * 4, *values = c.values + int64_t(head) * c.v_head * 4;
+#pragma unroll 4
       for (uint32_t i = threadIdx.x; i < uint32_t(TILE * (D / E)); i += kThreads) {
         const uint32_t k = i / (D / E), p = i - k * (D / E);
-        const bool there = p < pieces && ((s_valid[k / 32] >> (k & 31u)) & 1u) != 0u;
-        const char* from = c.keys + int64_t(head) * c.k_head * int64_t(sizeof(T)) + (uint64_t(s_k_at[k]) << c.unit_shift) + (there ? p * 16 : 0);
-        float f[E];
-        piece_to_floats<T>(load_piece(from, there), f);
-#pragma unroll
-        for (int e = 0; e < E; e++) { s_k[k * PITCH + p * E + e] = f[e]; }
-        from = c.values + int64_t(head) * c.v_head * int64_t(sizeof(T)) + (uint64_t(s_v_at[k]) << c.unit_shift) + (there ? p * 16 : 0);
-        piece_to_floats<T>(load_piece(from, there), f);
-#pragma unroll
-        for (int e = 0; e < E; e++) { s_v[k * PITCH + p * E + e] = f[e]; }
+        const bool there = p < pieces && ((s_valid_of[stage][k / 32] >> (k & 31u)) & 1u) != 0u;
+        const uint32_t from = there ? p * 16 : 0u, bytes = there ? 16u : 0u;
+        copy_piece(to + (k * PITCH + p * E) * 4, keys + (uint64_t(places(stage)[k]) << c.unit_shift) + from, bytes);
+        copy_piece(to + ((TILE + k) * PITCH + p * E) * 4, values + (uint64_t(places(stage)[TILE + k]) << c.unit_shift) + from, bytes);
       }
+    };
+    look(now.chunk, 0);
+    __syncthreads();
+    load(0);
+    copies_end_group();
+    for (uint32_t tile = now.chunk; tile < now.end; tile++) {
+      const uint32_t stage = (tile - now.chunk) & 1u, base = l.base + tile * TILE;
+      const bool mixed     = int64_t(base) + TILE > int64_t(l.length) || (t.window > 0 && int64_t(base) <= int64_t(latest) - t.window);
+      if (tile + 1 < now.end) { look(tile + 1, stage ^ 1u); }
+      __syncthreads();
+      if (tile + 1 < now.end) { load(stage ^ 1u); }
+      copies_end_group();
+      const float* s_k        = s_mem + shape::kKAt + stage * shape::kStage;
+      const float* s_v        = s_k + TILE * PITCH;
+      const uint32_t* s_valid = s_valid_of[stage];
+      const int32_t* s_of     = reinterpret_cast<const int32_t*>(places(stage)) + 2 * TILE;
       for (uint32_t i = threadIdx.x; i < uint32_t(BM * (TILE / 32)); i += kThreads) {
         const uint32_t r = i / (TILE / 32), word = i - r * (TILE / 32);
         uint32_t seen = s_valid[word];
@@ -175,6 +188,7 @@ tree_rows_kernel(cache_view c, work_view w, drafted_lists lists, tree_view t, tr
         }
         s_seen[i] = seen;
       }
+      copies_wait<1>();
       __syncthreads();
 
       float s[ROWS][KEYS] = {};
@@ -204,8 +218,8 @@ tree_rows_kernel(cache_view c, work_view w, drafted_lists lists, tree_view t, tr
         for (int j = 0; j < KEYS; j++) {
           const uint32_t k = x + 16 * j;
           float score      = t.cap_log2 != 0.0f ? tanhf(s[i][j] * t.scale_cap) * t.cap_log2 : s[i][j] * t.scale_log2;
-          score            = fmaf(slope[i], float(int64_t(s_of[k]) - own[i]), score);
-          s[i][j]          = ((s_seen[r * (TILE / 32) + k / 32] >> (k & 31u)) & 1u) != 0u ? score : -INFINITY;
+          if (t.slopes != nullptr) { score = fmaf(slope[i], float(int64_t(s_of[k]) - own[i]), score); }
+          s[i][j] = ((s_seen[r * (TILE / 32) + k / 32] >> (k & 31u)) & 1u) != 0u ? score : -INFINITY;
           next             = fmaxf(next, s[i][j]);
         }
 #pragma unroll
@@ -285,7 +299,8 @@ tree_rows_kernel(cache_view c, work_view w, drafted_lists lists, tree_view t, tr
 // much of values that it copies a stage ahead.  Scores: some lanes share a key, and each of its pieces is read once for all rows, whose queries are
 // broadcast.  Sums: a lane has columns, and reads each value once for all rows, whose weights are broadcast.
 //
-// What bounds it: the instructions' latency, with twelve warps of an SM (of six, whose chunks were twice as large: 92 us where twelve take less).
+// What bounds it: the instructions' latency, with twelve warps of an SM (six, whose chunks were twice as large: 92 us for 9 sequences of
+// up to 9,000 + 5 tokens, 12 key heads of 64 columns, with a window, slopes and a filter; twelve 80, and 64 to 67 with the rows side by side; HBM asks for 18).
 
 constexpr int kFewMost = 12;  // warps of a block, at most
 struct few_lists : drafted_lists {
@@ -584,10 +599,9 @@ tree_few_kernel(cache_view c, work_view w, few_lists lists, tree_view t, tree_pa
 
 // Rows of a block of the kernel for few, by how many a unit has.
 constexpr uint32_t few_rows_of(uint32_t n_rows, uint32_t dim) { return n_rows <= 4 ? 4 : n_rows <= 8 || dim > 128 ? 8 : 16; }
-// Which kernel: 4 sequences of 20,000 tokens, 2 key heads, us by warps alone and in tiles of 64 rows: 64 columns 16 rows 46 and 78, 32 rows 68 and 79,
-// 40 rows 100 and 81; 128 columns 16 rows 83 and 157, 32 rows 146 and 157, 40 rows 213 and 173; 256 columns 32 rows 223 and 376, 48 rows 324 and
-// 381, 64 rows 423 and 382.
-constexpr bool is_few(uint32_t n_rows, uint32_t dim) { return n_rows <= (dim <= 128 ? 32u : 48u); }
+// Which kernel: 4 sequences of 20,000 tokens, 2 key heads, us by warps alone and in tiles of 64 rows: 64 columns 16 rows 46 and 67, 32 rows 68 and 68;
+// 128 columns 16 rows 83 and 117, 32 rows 145 and 117; 256 columns 32 rows 222 and 260, 40 rows 273 and 260.
+constexpr bool is_few(uint32_t n_rows, uint32_t dim) { return n_rows <= (dim <= 128 ? 16u : 32u); }
 
 tree_plan plan_of(const resources& res, elem type, uint64_t sequences, uint32_t n_drafted, uint32_t n_heads, uint32_t group, uint32_t dim,
                   uint64_t capacity, int64_t window)
