@@ -327,7 +327,13 @@ struct tree_plan {
   uint32_t tile;       // keys
   uint32_t cost;       // of a unit beside its tiles, in tiles
   bool parts;          // a unit may lie in several shares
+  bool sets_aside;     // sums in tensor memory may be longer than kChain tiles
 };
+// Tiles that a sum in tensor memory is carried over.  The tensor core cuts off what it adds to a sum, always towards 0: some 7e-7 of the sum for a tile
+// of 64 keys, so that fp16 outputs of 200,000 keys in one share were 1.6e-3 too small (half a step of theirs is 4.9e-4).  After so many tiles a
+// sum is set aside -- in the workspace, added in 32 bits, rounded, to those before it -- and begun anew.  With 32 tiles 2.3e-5 is lost, with 64 5.0e-5; one
+// request of 250,001 + 64 tokens takes 356 us with either, 340 without.
+constexpr uint32_t kChain = 32;
 // `units` of `most` keys each, at most; `blocks`: thread blocks that the GPU holds at once; `least`: tiles of a share.
 inline tree_plan deal_out_tree(uint32_t blocks, uint32_t rows, uint32_t tile, uint32_t cost, uint32_t least, uint64_t units, uint32_t n_rows, uint64_t most)
 {
@@ -339,6 +345,7 @@ inline tree_plan deal_out_tree(uint32_t blocks, uint32_t rows, uint32_t tile, ui
   const uint64_t tiles = std::max<uint64_t>(1, ceildiv<uint64_t>(most, tile));
   p.shares = uint32_t(std::max<uint64_t>(1, std::min<uint64_t>(blocks / p.blocks_of, ceildiv<uint64_t>(units * (tiles + cost), least))));
   p.parts  = p.shares > 1 && tiles > 1;
+  p.sets_aside = false;
   return p;
 }
 
@@ -354,6 +361,7 @@ struct tree_call {
   tree_plan plan;
   const int32_t* pages;
   int64_t table_stride;
+  float4* aside;       // of every thread block: sums that were set aside, [columns / 4][rows]
   float shift;         // weights are held times 2^shift
   uint32_t* timeouts;  // calls whose waits took too long, counted
 };

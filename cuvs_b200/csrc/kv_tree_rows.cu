@@ -614,7 +614,15 @@ tree_plan plan_of(const resources& res, elem type, uint64_t sequences, uint32_t 
     if (is_few(n_rows, dim)) { return deal_out_tree(sms, few_rows_of(n_rows, dim), 1024 / columns, 24, few_lists::kLeast, sequences * n_heads, n_rows, most); }
     return deal_out_tree(sms * tree_resident(int(columns)), 64, columns <= 128 ? 64 : 32, 2, drafted_lists::kLeast, sequences * n_heads, n_rows, most);
   }
-  return deal_out_tree(sms, dim <= 128 && n_rows > 128 ? 256 : 128, 64, 2, drafted_lists::kLeast, sequences * n_heads, n_rows, most);
+  tree_plan p  = deal_out_tree(sms, dim <= 128 && n_rows > 128 ? 256 : 128, 64, 2, drafted_lists::kLeast, sequences * n_heads, n_rows, most);
+  p.sets_aside = most > kChain / 2 * p.tile;  // (the second stream's first turn comes half way)
+  return p;
+}
+// Of a plan's parts, and of what its blocks set aside: rows of two streams of 128, one of more than 128 columns.
+size_t part_bytes_of(const tree_plan& p, uint32_t dim) { return p.parts ? tree_part_bytes(p.shares, p.blocks_of, p.rows, dim) : 0; }
+size_t aside_bytes_of(const tree_plan& p, uint32_t dim)
+{
+  return p.sets_aside ? size_t(p.shares) * p.blocks_of * (dim <= 128 ? 256 : 128) * dim * sizeof(float) : 0;
 }
 
 }  // namespace
@@ -624,7 +632,7 @@ size_t attend_tree_workspace(const resources& res, elem type, uint32_t n_sequenc
 {
   if (n_sequences == 0) { return 0; }
   const tree_plan p = plan_of(res, type, n_sequences, n_drafted, n_heads, n_query_heads / n_heads, dim, capacity, window);
-  return p.parts ? tree_part_bytes(p.shares, p.blocks_of, p.rows, dim) : 0;
+  return part_bytes_of(p, dim) + aside_bytes_of(p, dim);
 }
 
 void attend_tree(resources& res, cudaStream_t stream, const attend_tree_args& a)
@@ -669,6 +677,7 @@ void attend_tree(resources& res, cudaStream_t stream, const attend_tree_args& a)
   call.parts.shares    = p.shares;
   call.parts.blocks_of = p.blocks_of;
   call.parts.rows      = p.rows;
+  if (p.sets_aside) { call.aside = reinterpret_cast<float4*>(a.workspace + part_bytes_of(p, c.dim)); }
   count_launches(res, p.parts ? 2 : 1);
 
   auto join = [&](auto type) {

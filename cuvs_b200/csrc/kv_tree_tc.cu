@@ -81,6 +81,7 @@ struct tc_args {
   tree_parts parts;
   const int32_t* pages;
   int64_t table_stride;
+  float4* aside;
   float shift;
   uint32_t* timeouts;
 };
@@ -115,6 +116,9 @@ struct piece_reader {
     return p.sequence != kNoMore;
   }
 };
+
+// Whether tile `i` of a stream's piece begins sums in tensor memory; the two streams' turns do not come at the same time.
+__device__ __forceinline__ bool begins_sums(uint32_t i, uint32_t stream) { return i == 0u || (i + stream * (kChain / 2)) % kChain == 0u; }
 
 // Whether a tile has keys that not all rows see.
 __device__ __forceinline__ bool is_mixed(const tree_view& t, const tree_piece& p, uint32_t base)
@@ -334,6 +338,7 @@ __device__ __forceinline__ void multiply_role(const tc_args& a, tc_shared& sh, c
       if (!wait(sh.p_full[stream * 2 + buffer], p_turn >> buffer)) { ok = false; break; }
       p_turn ^= 1u << buffer;
       tc_fence_after();
+      const bool anew = begins_sums(i, stream);
       if (elect_one()) {
         if (good) {
           // 32 keys of weights stand where their scores stood: 16 columns of the first numbers, 16 of the second
@@ -341,7 +346,7 @@ __device__ __forceinline__ void multiply_role(const tc_args& a, tc_shared& sh, c
 #pragma unroll
           for (uint32_t k = 0; k < kTile / 16; k++) {
             const uint32_t at = w + (k >> 1) * 32 + (k & 1u) * 8;
-            tc_mma_f16_ts(sums_at, at, from + k * (2048 >> 4), pv, k != 0u || i > 0);
+            tc_mma_f16_ts(sums_at, at, from + k * (2048 >> 4), pv, k != 0u || !anew);
             tc_mma_f16_ts(sums_at, at + 16, from + k * (2048 >> 4), pv, true);
           }
         }
@@ -426,6 +431,39 @@ __device__ __forceinline__ void softmax_role(const tc_args& a, tc_shared& sh, ch
   const uint32_t sh_tmem = sh.tmem;
   const uint32_t sums  = sh_tmem + lanes + shape::kSumsAt + (shape::kTwo ? stream * 128 : 0);
   const uint32_t width = (a.c.dim + 31) / 32;  // columns of the sums, in 32
+  // After `done` tiles: adds the sums of this row and stream that were set aside to those in tensor memory, which are set aside in their turn, or put
+  // back at the piece's end.  (Their top stands where the piece's will.)
+  auto add_aside = [&](float top, uint32_t done, bool back) {
+    constexpr uint32_t kRows = shape::kTwo ? 256 : 128;
+    float4* const aside      = a.aside + size_t(blockIdx.x) * (a.c.dim / 4) * kRows + stream * 128 + in;
+    const bool some          = exists && done > kChain - stream * (kChain / 2);
+    const float keep         = some ? power_of_2(sh.stats[stream][in].x - finite_top(top)) : 0.0f;
+#pragma unroll 1
+    for (uint32_t i = 0; i < width; i++) {
+      float4 y[8];
+#pragma unroll
+      for (uint32_t q = 0; q < 8; q++) {
+        y[q] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (some && (i * 8 + q) * 4 < a.c.dim) { y[q] = aside[(i * 8 + q) * kRows]; }
+      }
+      uint32_t o[32];
+      tmem_ld32(sums + i * 32, o);
+#pragma unroll
+      for (uint32_t q = 0; q < 8; q++) {
+        y[q] = make_float4(fmaf(y[q].x, keep, __uint_as_float(o[4 * q])), fmaf(y[q].y, keep, __uint_as_float(o[4 * q + 1])),
+                           fmaf(y[q].z, keep, __uint_as_float(o[4 * q + 2])), fmaf(y[q].w, keep, __uint_as_float(o[4 * q + 3])));
+        if (!back && exists && (i * 8 + q) * 4 < a.c.dim) { aside[(i * 8 + q) * kRows] = y[q]; }
+        o[4 * q]     = __float_as_uint(y[q].x);
+        o[4 * q + 1] = __float_as_uint(y[q].y);
+        o[4 * q + 2] = __float_as_uint(y[q].z);
+        o[4 * q + 3] = __float_as_uint(y[q].w);
+      }
+      __syncwarp();
+      if (back) { tmem_st32(sums + i * 32, o); }
+    }
+    if (back) { tmem_st_wait(); }
+    sh.stats[stream][in].x = top;
+  };
   piece_reader reader;
   tree_piece p;
   uint32_t s_turn = 0, o_turn = 0, x_turn = 0, tiles = 0, pv_turn = 0;  // s_turn: a bit for each buffer
@@ -455,6 +493,13 @@ __device__ __forceinline__ void softmax_role(const tc_args& a, tc_shared& sh, ch
       if (!alive) {
         arrive_warp(sh.p_full[buffer]);
         continue;
+      }
+      const bool anew = begins_sums(done, stream);
+      if (anew && done > 0) {
+        // (Of the tile before the last one: this tile's scores took the place of its weights.  So the barrier is at most one phase behind.)
+        if (!wait(sh.pv_done[stream], pv_turn + done - 1)) { ok = false; break; }
+        tc_fence_after();
+        add_aside(top, done, false);
       }
       uint32_t x[2][32];
       tmem_ld32_async(scores, x[0]);
@@ -494,9 +539,8 @@ __device__ __forceinline__ void softmax_role(const tc_args& a, tc_shared& sh, ch
       if (__any_sync(kAllLanes, highest > top + kAhead)) {
         const float next = highest > top + kAhead ? highest : top;
         const float keep = top == -INFINITY ? 1.0f : power_of_2(top - next);
-        if (done > 0 && __any_sync(kAllLanes, keep != 1.0f)) {
-          // The tile before may still be added up.  (The one before that is: this tile's scores took the place of its weights.  So the barrier is at
-          // most one phase behind.)
+        if (!anew && __any_sync(kAllLanes, keep != 1.0f)) {
+          // the tile before may still be added up
           if (!wait(sh.pv_done[stream], pv_turn + done - 1)) { ok = false; break; }
           tc_fence_after();
 #pragma unroll 1
@@ -547,7 +591,7 @@ __device__ __forceinline__ void softmax_role(const tc_args& a, tc_shared& sh, ch
 #pragma unroll 1
           for (uint32_t i = 0; i < width; i++) {
             uint32_t o[32];
-            if (done > 0) {
+            if (!anew) {
               tmem_ld32(sums + i * 32, o);
             } else {
 #pragma unroll
@@ -593,6 +637,7 @@ __device__ __forceinline__ void softmax_role(const tc_args& a, tc_shared& sh, ch
     if (done > 0) {
       if (!wait(sh.o_full[stream], o_turn++)) { return; }
       tc_fence_after();
+      if (done > kChain - stream * (kChain / 2) && alive) { add_aside(top, done, true); }
     }
 
     const size_t part_of = a.parts.part(which, block, p.begins ? 1u : 0u);
@@ -808,7 +853,7 @@ template <>
 void attend_tree16<KV_TYPE>(cudaStream_t stream, const tree_call& call)
 {
   using T = KV_TYPE;
-  tc_args a{call.c, call.w, call.lists, call.t, call.parts, call.pages, call.table_stride, call.shift, call.timeouts};
+  tc_args a{call.c, call.w, call.lists, call.t, call.parts, call.pages, call.table_stride, call.aside, call.shift, call.timeouts};
   // a scale above 0 keeps the order of scores: they need not be touched before their largest is known
   const bool shaped = call.t.cap_log2 != 0.0f || call.t.slopes != nullptr || !(call.t.scale_log2 > 0.0f);
   auto go = [&](auto columns) {
