@@ -209,6 +209,7 @@ SIGNATURES = {
     "cuvsKvCacheCopyPages": [C.c_size_t, *[_P(DLManagedTensor)] * 4],
     "cuvsB200KvCacheMoreTensors": [C.c_size_t, C.c_void_p, C.c_int, *[C.py_object] * 13, C.c_int64, C.c_float, C.c_float, C.c_bool],
     "cuvsB200KvCacheTreeWorkspaceArrays": [C.c_size_t, C.c_void_p, C.c_int64, _P(C.c_size_t)],
+    "cuvsB200SetTreeWaitTest": [C.c_uint32, C.c_uint32],
     "cuvsB200KvCacheWait": [C.c_size_t, C.c_void_p],
     "cuvsB200KvCacheWorkspaceArrays": [C.c_size_t, C.c_void_p, C.c_int64, _P(C.c_size_t)],
     "cuvsB200KvCacheCheck": [C.c_int, C.c_int, C.c_void_p, C.c_int64],

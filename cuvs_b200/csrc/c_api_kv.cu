@@ -928,6 +928,15 @@ extern "C" int cuvsB200KvCacheMoreTensors(cuvsResources_t res, cudaStream_t stre
   return raised == CUVS_SUCCESS ? status : CUVS_ERROR;
 }
 
+extern "C" cuvsError_t cuvsB200SetTreeWaitTest(uint32_t limit, uint32_t skip_tile)
+{
+  return translate_exceptions([=] {
+    // a limit below 1000 iterations could run out on a healthy but busy GPU
+    CUVS_EXPECTS(limit == 0 || limit >= 1000, "limit must be 0 or at least 1000");
+    kv::set_tree_wait_test(limit, skip_tile);
+  });
+}
+
 extern "C" cuvsError_t cuvsB200KvCacheWait(cuvsResources_t res, cudaStream_t stream)
 {
   return translate_exceptions([=] {

@@ -134,6 +134,7 @@ struct attend_tree_args {
 size_t attend_tree_workspace(const resources& res, elem type, uint32_t n_sequences, uint32_t n_drafted, uint32_t n_query_heads, uint32_t n_heads,
                              uint32_t dim, uint64_t capacity, int64_t window);
 void attend_tree(resources& res, cudaStream_t stream, const attend_tree_args& a);
+void set_tree_wait_test(uint32_t limit /* 0: the usual one */, uint32_t skip_tile);
 
 struct keep_path_args {
   cache_view cache;

@@ -230,7 +230,7 @@ tree_join_kernel(tree_view t, tree_parts parts, uint32_t dim, uint32_t n_heads, 
   const uint32_t entry = blockIdx.x / (groups * parts.blocks_of), rest = blockIdx.x - entry * (groups * parts.blocks_of);
   const uint32_t block = rest / groups, r = (rest - block * groups) * 32 + lane;
   uint4 unit = parts.begun[entry];
-  // (an entry that nothing has written, where lengths changed meanwhile, leads nowhere else)
+  // (an entry that nothing has written, where lengths changed meanwhile or a block gave up, leads nowhere else; those of shares are always written)
   if (parts.by_unit) { unit.x = entry / n_heads, unit.y = entry - unit.x * n_heads; }
   const uint32_t share = unit.w, n = share < parts.shares ? min(unit.z, parts.shares - share) : 0u, row = block * parts.rows + r;
   if (n == 0u || block * parts.rows + (r - lane) >= t.n_rows) { return; }
@@ -364,6 +364,7 @@ struct tree_call {
   float4* aside;       // of every thread block: sums that were set aside, [columns / 4][rows]
   float shift;         // weights are held times 2^shift
   uint32_t* timeouts;  // calls whose waits took too long, counted
+  uint32_t limit, skip_tile;  // of waits; for tests of them
 };
 template <typename T>
 void attend_tree16(cudaStream_t stream, const tree_call& call);

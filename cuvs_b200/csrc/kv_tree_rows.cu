@@ -1,7 +1,9 @@
 // Attention of drafted tokens to the rows of their sequences in a paged cache, with 32-bit products (the mathematics: kv_tree.cuh).
 #include "kv_tree.cuh"
+#include "tc_ptx.cuh"
 
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 namespace cuvs_b200::kv {
@@ -625,7 +627,16 @@ size_t aside_bytes_of(const tree_plan& p, uint32_t dim)
   return p.sets_aside ? size_t(p.shares) * p.blocks_of * (dim <= 128 ? 256 : 128) * dim * sizeof(float) : 0;
 }
 
+// Waits of the kernel on tensor cores (tests make one run out).
+std::atomic<uint32_t> g_wait_limit{kSpinLimit}, g_skip_tile{0};
+
 }  // namespace
+
+void set_tree_wait_test(uint32_t limit, uint32_t skip_tile)
+{
+  g_wait_limit = limit != 0u ? limit : kSpinLimit;
+  g_skip_tile  = skip_tile;
+}
 
 size_t attend_tree_workspace(const resources& res, elem type, uint32_t n_sequences, uint32_t n_drafted, uint32_t n_query_heads, uint32_t n_heads,
                              uint32_t dim, uint64_t capacity, int64_t window)
@@ -648,6 +659,8 @@ void attend_tree(resources& res, cudaStream_t stream, const attend_tree_args& a)
   call.pages         = a.pages;
   call.table_stride  = a.table_stride;
   call.timeouts      = res.pinned + 14;
+  call.limit         = g_wait_limit;
+  call.skip_tile     = g_skip_tile;
   tree_view& t       = call.t;
   t.n_drafted        = a.n_drafted;
   t.group            = group;

@@ -28,8 +28,7 @@ constexpr int kPieces     = 2;
 constexpr int kReaders    = 14;   // warps that read a piece's description
 constexpr uint32_t kTile  = 64;   // keys
 constexpr int kMostStages = 8;    // of keys, and of values
-constexpr uint32_t kLimit = kSpinLimit;       // of waits for a tile
-constexpr uint32_t kPatience = kSpinLimit * 32;  // of waits for a piece, which may be all of a sequence
+constexpr uint32_t kPatience = 32;  // times the limit: for a piece, which may be all of a sequence
 
 template <int D>
 struct tc_shape {
@@ -84,6 +83,7 @@ struct tc_args {
   float4* aside;
   float shift;
   uint32_t* timeouts;
+  uint32_t limit, skip_tile;  // of waits; for tests: 1 + the tile of each block whose keys nobody is told of (0: none)
 };
 
 constexpr uint32_t kNoMore = 0xFFFFFFFFu;
@@ -91,11 +91,24 @@ constexpr uint32_t kNoMore = 0xFFFFFFFFu;
 // Waits with a limit, after which the block gives up; a whole warp at a time.
 struct waiter {
   tc_shared& sh;
-  __device__ __forceinline__ bool operator()(const uint64_t& bar, uint32_t parity, uint32_t limit = kLimit) const
+  uint32_t limit;
+  __device__ __forceinline__ bool give_up() const
   {
-    if (mbar_wait_warp(smem_u32(&bar), parity & 1u, limit)) { return true; }
     *const_cast<volatile uint32_t*>(&sh.failed) = 1u;
     return false;
+  }
+  __device__ __forceinline__ bool operator()(const uint64_t& bar, uint32_t parity) const
+  {
+    return mbar_wait_warp(smem_u32(&bar), parity & 1u, limit) || give_up();
+  }
+  // for a piece, or until another warp has given up
+  __device__ __forceinline__ bool patiently(const uint64_t& bar, uint32_t parity) const
+  {
+    for (uint32_t i = 0; i < kPatience; i++) {
+      if (mbar_wait_warp(smem_u32(&bar), parity & 1u, limit)) { return true; }
+      if (__any_sync(kAllLanes, *const_cast<volatile uint32_t*>(&sh.failed) != 0u)) { break; }
+    }
+    return give_up();
   }
 };
 
@@ -109,7 +122,7 @@ struct piece_reader {
   uint32_t i = 0;
   __device__ __forceinline__ bool next(tc_shared& sh, const waiter& wait, tree_piece& p)
   {
-    if (!wait(sh.piece_full[i % kPieces], i / kPieces, kPatience)) { return false; }
+    if (!wait.patiently(sh.piece_full[i % kPieces], i / kPieces)) { return false; }
     p = sh.pieces[i % kPieces];
     arrive_warp(sh.piece_empty[i % kPieces]);
     i++;
@@ -254,8 +267,10 @@ __device__ __forceinline__ void copy_role(const tc_args& a, tc_shared& sh, char*
       } else if (lane == 0) {
         (half == 0 ? sh.valid[info].x : sh.valid[info].y) = rows_there;
       }
-      arrive_behind_copies(full[slot]);
-      arrive_warp(full[slot]);  // what the warp wrote itself
+      if (of_values || tiles + 1 != a.skip_tile) {
+        arrive_behind_copies(full[slot]);
+        arrive_warp(full[slot]);  // what the warp wrote itself
+      }
       if (++slot == stages) {
         slot = 0;
         round++;
@@ -362,7 +377,8 @@ __device__ __forceinline__ void multiply_role(const tc_args& a, tc_shared& sh, c
   }
   if (elect_one()) { tc_commit(smem_u32(&sh.drained[stream])); }
   __syncwarp();
-  wait(sh.drained[stream], 0);
+  // (whatever the limit: nothing may be on its way into tensor memory that is given back)
+  if (!mbar_wait_warp(smem_u32(&sh.drained[stream]), 0u, kSpinLimit)) { wait.give_up(); }
 }
 
 // ---- softmax ------------------------------------------------------------------------------------------------------------------
@@ -761,7 +777,10 @@ __device__ __forceinline__ void way_role(const tc_args& a, tc_shared& sh, const 
       for (uint32_t k = lane; k < a.t.n_drafted; k += 32) { latest = max(latest, positions[k]); }
       latest = __reduce_max_sync(kAllLanes, latest);
     }
-    if (i >= kPieces && !wait(sh.piece_empty[i % kPieces], i / kPieces - 1, kPatience)) { return; }
+    if (i >= kPieces && !wait.patiently(sh.piece_empty[i % kPieces], i / kPieces - 1)) {
+      begun = make_uint4(0, 0, 0, 0);  // the join must find no entry that an earlier call has left
+      break;
+    }
     if (lane == 0) {
       tree_piece p{};
       p.sequence = kNoMore;
@@ -821,7 +840,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const waiter wait{sh};
+  const waiter wait{sh, a.limit};
   if (warp < 8) {
     registers_up<168>();
     softmax_role<T, D, SHAPED>(a, sh, smem, wait, which, block);
@@ -853,7 +872,7 @@ template <>
 void attend_tree16<KV_TYPE>(cudaStream_t stream, const tree_call& call)
 {
   using T = KV_TYPE;
-  tc_args a{call.c, call.w, call.lists, call.t, call.parts, call.pages, call.table_stride, call.aside, call.shift, call.timeouts};
+  tc_args a{call.c, call.w, call.lists, call.t, call.parts, call.pages, call.table_stride, call.aside, call.shift, call.timeouts, call.limit, call.skip_tile};
   // a scale above 0 keeps the order of scores: they need not be touched before their largest is known
   const bool shaped = call.t.cap_log2 != 0.0f || call.t.slopes != nullptr || !(call.t.scale_log2 > 0.0f);
   auto go = [&](auto columns) {

@@ -139,6 +139,9 @@ CUVS_EXPORT cuvsError_t cuvsB200KvCacheWait(cuvsResources_t res, cudaStream_t st
 CUVS_EXPORT cuvsError_t cuvsB200KvCacheWorkspaceArrays(cuvsResources_t res, const int64_t* words, int64_t n_words, size_t* bytes);
 /* cuvsKvCacheAttendTreeWorkspace on such words. */
 CUVS_EXPORT cuvsError_t cuvsB200KvCacheTreeWorkspaceArrays(cuvsResources_t res, const int64_t* words, int64_t n_words, size_t* bytes);
+/* For tests of waits that run out, process-wide: iterations (about a microsecond each) that a wait of attend tree on tensor cores may take, 0: the
+ * usual two seconds; 1 + the number of a tile in each block's way whose keys nobody is told of, so that the wait for it runs out, 0: none. */
+CUVS_EXPORT cuvsError_t cuvsB200SetTreeWaitTest(uint32_t limit, uint32_t skip_tile);
 /* The checks of such a call alone, for a handle of `device`: touches no GPU and reads no tensor. */
 CUVS_EXPORT cuvsError_t cuvsB200KvCacheCheck(int device, int op, const int64_t* words, int64_t n_words);
 

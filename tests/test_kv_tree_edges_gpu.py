@@ -4,8 +4,9 @@ import math
 import pytest
 import torch
 
+from cuvs_b200 import _lib as L
 from cuvs_b200 import kv_cache
-from test_kv_tree_gpu import U, generator, ints, needs_a_gpu  # noqa: F401
+from test_kv_tree_gpu import Step, U, generator, ints, needs_a_gpu  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -47,3 +48,46 @@ def test_sums_of_long_sequences_lose_nothing(dtype, n_sequences, m, group, dim):
     # roundings are spread evenly over half a step either way, those of different columns independently
     assert off.mean().abs() <= chain + 6 * half / math.sqrt(3 * dim)
     assert lse_off.abs().max() <= total + 4 * U * 14
+
+
+# ---- waits that run out -------------------------------------------------------------------------------------------------------
+
+@pytest.fixture
+def giving_up():
+    """Sets a limit of about a millisecond, and a tile of each block whose keys nobody is told of; what it yields does so, or ends it with 0."""
+    def wait_test(tile):
+        L.check(L.load().cuvsB200SetTreeWaitTest(1000 if tile else 0, tile))
+
+    yield wait_test
+    torch.cuda.synchronize()
+    wait_test(0)
+
+
+@pytest.mark.parametrize("dtype,dim", [(torch.float16, 64), (torch.bfloat16, 128), (torch.bfloat16, 256)])
+@pytest.mark.parametrize("lengths,m", [([(7 * i) % 700 for i in range(200)], 10),   # more units than blocks
+                                       ([(7 * i) % 700 for i in range(200)], 80),
+                                       ([40_000, 5, 9000], 10), ([40_000, 5, 9000], 80)])
+@pytest.mark.parametrize("tile", [1, 2, 5])
+def test_a_call_that_gives_up_writes_nothing_elsewhere(giving_up, dtype, dim, lengths, m, tile):
+    """What the workspace holds from before must not say where outputs go."""
+    step = Step(dtype, lengths, m, 2, 4, dim, 16)
+    want = step.call()
+    n = len(lengths)
+    frame, lse_frame = torch.full((n + 2, m, 8, dim), 7.0, dtype=dtype, device="cuda"), torch.full((n + 2, m, 8), 7.0, device="cuda")
+    out, lse = frame[1:-1], lse_frame[1:-1]
+    words = kv_cache.attend_tree_workspace(step.keys, step.queries, step.pages) // 4
+    # entries of units behind the last sequence, with parts
+    workspace = ints([n, 1, 1, 0]).repeat(words // 4 + 1)[:words].view(torch.uint8)
+    giving_up(tile)
+    with pytest.raises(L.CuvsError, match="gave up on a wait"):
+        step.call(out=out, lse=lse, workspace=workspace)
+    giving_up(0)
+    for t in (frame, lse_frame):
+        assert (t[0] == 7).all() and (t[-1] == 7).all()
+    got = step.call(out=out, lse=lse, workspace=workspace)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_limits_that_a_busy_gpu_would_reach_are_refused():
+    with pytest.raises(L.CuvsError, match="at least 1000"):
+        L.check(L.load().cuvsB200SetTreeWaitTest(999, 0))
