@@ -74,7 +74,11 @@ extern "C" cuvsError_t cuvsStreamGet(cuvsResources_t res, cudaStream_t* stream)
 }
 extern "C" cuvsError_t cuvsStreamSync(cuvsResources_t res)
 {
-  return translate_exceptions([=] { res_of(res)->sync(); });
+  return translate_exceptions([=] {
+    auto* r = res_of(res);
+    r->sync();
+    r->raise_reports(r->stream);
+  });
 }
 extern "C" cuvsError_t cuvsDeviceIdGet(cuvsResources_t res, int* device_id)
 {

@@ -461,6 +461,11 @@ bool attend_tree_call(resources& res, cudaStream_t stream, kv::attend_tree_args 
                                                 uint64_t(a.table_width) * a.cache.page.size, a.window);
   std::unique_lock<std::mutex> held;
   if (!workspace_for(res, stream, need, a.workspace, a.workspace_bytes, held)) { return false; }
+  if (a.type != kv::elem::f32) {  // on tensor cores, with waits inside the kernel
+    cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(stream, &capturing) != cudaSuccess) { cudaGetLastError(); }  // (the legacy stream, beside a capture)
+    a.report = res.report_word(stream, capturing != cudaStreamCaptureStatusNone);
+  }
   kv::attend_tree(res, stream, a);
   return true;
 }
@@ -639,11 +644,7 @@ void wait_for(resources& res, cudaStream_t stream)
 {
   device_scope on(res.device);
   CUDA_TRY(cudaStreamSynchronize(stream));
-  // a kernel of this handle that gave up on a wait inside it (its waits have limits)
-  volatile uint32_t* timeouts = res.pinned + 14;
-  const bool timed_out        = *timeouts != 0u;
-  if (timed_out) { *timeouts = 0u; }
-  CUVS_EXPECTS(!timed_out, "attention to drafted tokens gave up on a wait: its results are not complete");
+  res.raise_reports(stream);
 }
 
 resources& single_device(cuvsResources_t res)

@@ -129,6 +129,7 @@ struct attend_tree_args {
   float* lse;              // [n_sequences, n_drafted, n_query_heads]
   char* workspace;
   size_t workspace_bytes;
+  uint32_t* report;        // host word that is set where a wait inside the kernel runs out
 };
 // How many bytes of workspace attend_tree() wants, by sizes alone.
 size_t attend_tree_workspace(const resources& res, elem type, uint32_t n_sequences, uint32_t n_drafted, uint32_t n_query_heads, uint32_t n_heads,

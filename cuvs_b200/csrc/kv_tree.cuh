@@ -363,7 +363,7 @@ struct tree_call {
   int64_t table_stride;
   float4* aside;       // of every thread block: sums that were set aside, [columns / 4][rows]
   float shift;         // weights are held times 2^shift
-  uint32_t* timeouts;  // calls whose waits took too long, counted
+  uint32_t* report;    // host word that is set where a wait runs out
   uint32_t limit, skip_tile;  // of waits; for tests of them
 };
 template <typename T>

@@ -658,7 +658,7 @@ void attend_tree(resources& res, cudaStream_t stream, const attend_tree_args& a)
   call.plan          = p;
   call.pages         = a.pages;
   call.table_stride  = a.table_stride;
-  call.timeouts      = res.pinned + 14;
+  call.report        = a.report;
   call.limit         = g_wait_limit;
   call.skip_tile     = g_skip_tile;
   tree_view& t       = call.t;

@@ -82,7 +82,7 @@ struct tc_args {
   int64_t table_stride;
   float4* aside;
   float shift;
-  uint32_t* timeouts;
+  uint32_t* report;
   uint32_t limit, skip_tile;  // of waits; for tests: 1 + the tile of each block whose keys nobody is told of (0: none)
 };
 
@@ -862,7 +862,10 @@ __global__ void __launch_bounds__(kThreads, 1) tree_tc_kernel(const __grid_const
   __syncthreads();
   tc_fence_after();
   if (warp == 0) { asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(sh.tmem) : "memory"); }
-  if (threadIdx.x == 0 && sh.failed != 0u) { count_timeout(a.timeouts); }
+  if (threadIdx.x == 0 && sh.failed != 0u) {
+    *const_cast<volatile uint32_t*>(a.report) = 1u;
+    __threadfence_system();
+  }
 }
 
 }  // namespace
@@ -872,7 +875,7 @@ template <>
 void attend_tree16<KV_TYPE>(cudaStream_t stream, const tree_call& call)
 {
   using T = KV_TYPE;
-  tc_args a{call.c, call.w, call.lists, call.t, call.parts, call.pages, call.table_stride, call.aside, call.shift, call.timeouts, call.limit, call.skip_tile};
+  tc_args a{call.c, call.w, call.lists, call.t, call.parts, call.pages, call.table_stride, call.aside, call.shift, call.report, call.limit, call.skip_tile};
   // a scale above 0 keeps the order of scores: they need not be touched before their largest is known
   const bool shaped = call.t.cap_log2 != 0.0f || call.t.slopes != nullptr || !(call.t.scale_log2 > 0.0f);
   auto go = [&](auto columns) {

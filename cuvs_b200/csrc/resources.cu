@@ -2,6 +2,7 @@
 
 #include <nvtx3/nvToolsExt.h>
 
+#include <algorithm>
 #include <atomic>
 #include <mutex>
 
@@ -53,6 +54,8 @@ void ensure_dynamic_smem(const void* kernel, size_t bytes)
 }
 
 namespace {
+constexpr uint32_t kPinnedWords = 1024, kSharedReport = 14, kFirstReport = 16;
+
 // While it lives, this thread may allocate although a stream is being captured, by itself or by another thread: the work that what it allocates
 // is for is not captured.
 struct capture_elsewhere {
@@ -98,10 +101,8 @@ resources::resources()
   smem_optin = static_cast<int>(prop.sharedMemPerBlockOptin);
   cc_major   = prop.major;
   ask_for_clusters(clusters_at_once, size_t(smem_optin));
-  CUDA_TRY(cudaMallocHost(&pinned, 64));
-  pinned[12] = 0;
-  pinned[13] = 0;
-  pinned[14] = 0;
+  CUDA_TRY(cudaMallocHost(&pinned, kPinnedWords * sizeof(uint32_t)));
+  std::fill_n(pinned, kPinnedWords, 0u);
   CUDA_TRY(cudaMalloc(&redo_counts, N_REDO_COUNTS * sizeof(*redo_counts)));
   CUDA_TRY(cudaMemset(redo_counts, 0, N_REDO_COUNTS * sizeof(*redo_counts)));
 }
@@ -136,6 +137,37 @@ std::unique_lock<std::mutex> resources::stream_workspace(cudaStream_t on, size_t
   }
   *at = w.base();
   return held;
+}
+
+uint32_t* resources::report_word(cudaStream_t on, bool captured)
+{
+  std::lock_guard<std::mutex> held(report_lock);
+  has_reports = true;
+  if (captured) { return pinned + kSharedReport; }
+  unsigned long long id = 0;
+  CUDA_TRY(cudaStreamGetId(on, &id));
+  const auto at = report_of.find(id);
+  if (at != report_of.end()) { return pinned + at->second; }
+  const uint32_t next = kFirstReport + uint32_t(report_of.size());
+  if (next >= kPinnedWords) { return pinned + kSharedReport; }
+  report_of[id] = next;
+  return pinned + next;
+}
+
+void resources::raise_reports(cudaStream_t on)
+{
+  if (!has_reports) { return; }
+  bool own = false;
+  {
+    std::lock_guard<std::mutex> held(report_lock);
+    unsigned long long id = 0;
+    CUDA_TRY(cudaStreamGetId(on, &id));
+    const auto at = report_of.find(id);
+    own           = at != report_of.end() && __atomic_exchange_n(pinned + at->second, 0u, __ATOMIC_ACQ_REL) != 0u;
+  }
+  CUVS_EXPECTS(!own, "attention to drafted tokens gave up on a wait: the results of a call on this stream are not complete");
+  CUVS_EXPECTS(__atomic_exchange_n(pinned + kSharedReport, 0u, __ATOMIC_ACQ_REL) == 0u,
+               "attention to drafted tokens gave up on a wait: the results of a captured call (or one of many streams) are not complete");
 }
 
 void resources::adopt_tc_verdict()

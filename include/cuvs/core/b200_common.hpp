@@ -147,8 +147,16 @@ struct resources {
   // The workspace of a stream, at least `bytes` large.  The lock is held until the call's work has been enqueued: another thread's call on
   // the stream comes before or behind all of it, and may replace the workspace afterwards, once the stream's work is done.
   std::unique_lock<std::mutex> stream_workspace(cudaStream_t on, size_t bytes, char** at);
-  // small pinned host word for an occasional device->host scalar
+  // a page of pinned host memory: words for an occasional device->host scalar, and those by which kernels report
   uint32_t* pinned = nullptr;
+  // Reports of kernels that gave up on a wait: a word for each stream (by its id) that has had such a kernel, which any number of its blocks set.  What
+  // is captured may be replayed on any stream: it has one word of the handle, and so have the streams beyond the page's room.
+  std::map<unsigned long long, uint32_t> report_of;
+  std::mutex report_lock;
+  std::atomic<bool> has_reports{false};
+  uint32_t* report_word(cudaStream_t on, bool captured);
+  // After the stream has been waited for: raises an error if one of its kernels gave up since the last time, or a captured one.
+  void raise_reports(cudaStream_t on);
   // counter read by the benchmark ("how many kernels of ours ran"); calls of several threads may add to it
   std::atomic<uint64_t> launches{0};
 

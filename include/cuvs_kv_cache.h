@@ -96,7 +96,9 @@ CUVS_EXPORT cuvsError_t cuvsKvCacheDraftTree(cuvsResources_t res, DLManagedTenso
  * none: it attends to nothing, and none to it.  Scores are s = scale * q.k, with cap (0: none; 1e-30 to
  * 1e30) then cap * tanh(s / cap), with slopes (f32
  * [n_query_heads]) then less slope * distance of the positions.  lse: f32 [n_sequences, n_drafted, n_query_heads].  In attention to 16-bit rows
- * weights below 2^-30 of the largest may count as 0.  Workspace as in cuvsKvCacheAttention. */
+ * weights below 2^-30 of the largest may count as 0.  Workspace as in cuvsKvCacheAttention.  Attention to 16-bit rows waits inside its kernel, with
+ * limits of seconds: should one run out, the next wait for the stream through this handle (cuvsStreamSync) is an error, of a captured call the next
+ * wait for any stream. */
 CUVS_EXPORT cuvsError_t cuvsKvCacheAttendTree(cuvsResources_t res, DLManagedTensor* keys, DLManagedTensor* values, DLManagedTensor* queries,
                                               DLManagedTensor* pages, DLManagedTensor* lengths, DLManagedTensor* positions,
                                               DLManagedTensor* mask, float scale, int64_t window, float cap, DLManagedTensor* slopes,

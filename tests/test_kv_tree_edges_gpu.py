@@ -1,9 +1,12 @@
 """GPU tests of attention of drafted tokens at the ends of its ranges: very long sequences, values and scores that are no numbers."""
+import ctypes as C
 import math
+import threading
 
 import pytest
 import torch
 
+from cuvs_b200 import Resources
 from cuvs_b200 import _lib as L
 from cuvs_b200 import kv_cache
 from test_kv_tree_gpu import Step, U, generator, ints, needs_a_gpu  # noqa: F401
@@ -91,3 +94,138 @@ def test_a_call_that_gives_up_writes_nothing_elsewhere(giving_up, dtype, dim, le
 def test_limits_that_a_busy_gpu_would_reach_are_refused():
     with pytest.raises(L.CuvsError, match="at least 1000"):
         L.check(L.load().cuvsB200SetTreeWaitTest(999, 0))
+
+
+def small_step(seed=0, **options):
+    return Step(torch.float16, [3000, 100], 9, 2, 4, 64, 16, seed, **options)
+
+
+def test_who_gave_up_is_told(giving_up):
+    """Two streams of one handle: a call of one of them gives up, whoever waits first."""
+    step, resources = small_step(), Resources()
+    want = step.call()
+    one, other = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+
+    def on(stream, **options):
+        with torch.cuda.stream(stream):
+            return step.call(resources=resources, **options)
+
+    giving_up(1)
+    on(one, sync=False)
+    torch.cuda.synchronize()
+    giving_up(0)
+    assert all(torch.equal(a, b) for a, b in zip(on(other), want))
+    with torch.cuda.stream(other):
+        kv_cache.draft_tree(step.parents, step.lengths, resources=resources)
+    with pytest.raises(L.CuvsError, match="gave up on a wait: the results of a call on this stream"):
+        on(one)
+    assert all(torch.equal(a, b) for a, b in zip(on(one), want))
+    # another call that waits, and the handle's own wait
+    for wait in (lambda: kv_cache.draft_tree(step.parents, step.lengths, resources=resources), resources.sync):
+        giving_up(1)
+        on(one, sync=False)
+        torch.cuda.synchronize()
+        giving_up(0)
+        with torch.cuda.stream(one), pytest.raises(L.CuvsError, match="gave up on a wait"):
+            wait()
+    assert all(torch.equal(a, b) for a, b in zip(on(one), want))
+
+
+def test_threads_are_told_of_their_own_calls(giving_up):
+    """Three threads with a stream each, through one handle; the calls of all of them give up."""
+    steps, resources = [small_step(i) for i in range(3)], Resources()
+    torch.cuda.synchronize()
+    giving_up(1)
+    told, barrier = [None] * 3, threading.Barrier(3)
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            steps[i].call(resources=resources, sync=False)
+            torch.cuda.synchronize()
+            barrier.wait()
+            try:
+                kv_cache.draft_tree(steps[i].parents, steps[i].lengths, resources=resources)
+            except L.CuvsError as e:
+                told[i] = str(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert all(t is not None and "a call on this stream" in t for t in told)
+
+
+def test_a_c_caller_is_told(giving_up):
+    from cuvs_b200.common import DLTensorRef
+    step, resources, lib = small_step(heads_outside=False), Resources(), L.load()
+    want = step.call()
+    out, lse = torch.empty_like(want[0]), torch.empty_like(want[1])
+    refs = [DLTensorRef(t) for t in (step.keys, step.values, step.queries, step.pages, step.lengths, step.positions, step.mask, out, lse)]
+    resources.use_current_stream()
+
+    def call():
+        L.check(lib.cuvsKvCacheAttendTree(resources.handle, *(r.ref() for r in refs[:7]), 0.125, 0, 0.0, None, L.FilterStruct(0, 0), refs[7].ref(),
+                                          refs[8].ref(), None))
+
+    giving_up(1)
+    call()
+    torch.cuda.synchronize()
+    giving_up(0)
+    with pytest.raises(L.CuvsError, match="gave up on a wait"):
+        L.check(lib.cuvsStreamSync(resources.handle))
+    L.check(lib.cuvsStreamSync(resources.handle))
+    call()
+    L.check(lib.cuvsStreamSync(resources.handle))
+    assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
+
+
+def test_a_captured_call_that_gives_up(giving_up):
+    """It may be replayed on any stream: the next wait of the handle is told, and says what it was."""
+    step, resources = small_step(), Resources()
+    want = step.call(resources=resources)
+    graph = torch.cuda.CUDAGraph()
+    giving_up(1)
+    with torch.cuda.graph(graph):
+        step.call(resources=resources, sync=False)
+    giving_up(0)
+    assert all(torch.equal(a, b) for a, b in zip(step.call(resources=resources), want))
+    graph.replay()
+    torch.cuda.synchronize()
+    with pytest.raises(L.CuvsError, match="results of a captured call"):
+        step.call(resources=resources)
+    assert all(torch.equal(a, b) for a, b in zip(step.call(resources=resources), want))
+
+
+def test_more_streams_than_there_are_words(giving_up):
+    """A page has a word for each of 1,008 streams; those behind share one."""
+    from cuvs_b200.common import DLTensorRef
+    step, resources, lib = small_step(heads_outside=False), Resources(), L.load()
+    want = step.call()
+    out, lse = torch.empty_like(want[0]), torch.empty_like(want[1])
+    workspace = torch.empty(kv_cache.attend_tree_workspace(step.keys, step.queries, step.pages), dtype=torch.uint8, device="cuda")
+    refs = [DLTensorRef(t) for t in (step.keys, step.values, step.queries, step.pages, step.lengths, step.positions, step.mask, out, lse, workspace)]
+    torch.cuda.synchronize()
+    cudart = torch.cuda.cudart()
+
+    def call():
+        L.check(lib.cuvsKvCacheAttendTree(resources.handle, *(r.ref() for r in refs[:7]), 0.125, 0, 0.0, None, L.FilterStruct(0, 0), refs[7].ref(),
+                                          refs[8].ref(), refs[9].ref()))
+
+    for i in range(1050):
+        stream = C.c_uint64()
+        assert int(cudart.cudaStreamCreate(C.addressof(stream))) == 0
+        L.check(lib.cuvsStreamSet(resources.handle, stream.value))
+        for fails in ((True, False) if i in (0, 1007, 1008, 1049) else (False,)):
+            giving_up(1 if fails else 0)
+            call()
+            giving_up(0)
+            if fails:
+                with pytest.raises(L.CuvsError, match="gave up on a wait"):
+                    L.check(lib.cuvsStreamSync(resources.handle))
+            else:
+                L.check(lib.cuvsStreamSync(resources.handle))
+        L.check(lib.cuvsStreamSet(resources.handle, None))
+        assert int(cudart.cudaStreamDestroy(stream.value)) == 0
+    assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
