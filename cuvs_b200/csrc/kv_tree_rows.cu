@@ -274,6 +274,7 @@ tree_rows_kernel(cache_view c, work_view w, drafted_lists lists, tree_view t, tr
       for (int q = 0; q < QUADS; q++) {
         const uint32_t quad = x + 16 * q;
         if (quad * 4 >= c.dim) { continue; }
+        if (top[i] == -INFINITY) { acc[i][q][0] = acc[i][q][1] = acc[i][q][2] = acc[i][q][3] = 0.0f; }  // 0 times what is no number, of a row that saw nothing
         if (now.whole) {
           store_quad<T>(out_row<T>(t, now.sequence, head, row0 + r) + quad * 4,
                         make_float4(acc[i][q][0] * scale, acc[i][q][1] * scale, acc[i][q][2] * scale, acc[i][q][3] * scale));

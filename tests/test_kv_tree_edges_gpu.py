@@ -9,7 +9,7 @@ import torch
 from cuvs_b200 import Resources
 from cuvs_b200 import _lib as L
 from cuvs_b200 import kv_cache
-from test_kv_tree_gpu import Step, U, generator, ints, needs_a_gpu  # noqa: F401
+from test_kv_tree_gpu import DTYPES, Step, U, generator, ints, needs_a_gpu  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -229,3 +229,22 @@ def test_more_streams_than_there_are_words(giving_up):
         L.check(lib.cuvsStreamSet(resources.handle, None))
         assert int(cudart.cudaStreamDestroy(stream.value)) == 0
     assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
+
+
+# ---- what is no number --------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,group,dim", [(2, 2, 64), (9, 8, 64), (40, 8, 128), (9, 5, 256)])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_a_token_that_is_none_attends_to_nothing(dtype, m, group, dim, bad):
+    """Beside values of its sequence that are no numbers, in tiles that all other tokens see whole; in one share and in several."""
+    for lengths in ([300, 40, 300], [20_000], [130] * 300):
+        step = Step(dtype, lengths, m, 2, group, dim, 16, padding=1)
+        slot = step.allowed()[1][0]
+        assert lengths[0] >= 128  # place 70 lies in a tile before the drafted tokens
+        step.values[slot[70] // 16, slot[70] % 16] = bad
+        out, lse = step.call()
+        none = step.positions < 0
+        assert none.any() and (out[none] == 0).all() and (lse[none] == -math.inf).all()
+        assert not out[0][~none[0]].isfinite().any() and lse[~none].isfinite().all()
+        assert out[1:][~none[1:]].isfinite().all()
