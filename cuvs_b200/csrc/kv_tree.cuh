@@ -264,9 +264,10 @@ tree_join_kernel(tree_view t, tree_parts parts, uint32_t dim, uint32_t n_heads, 
       x.x *= keep, x.y *= keep, x.z *= keep, x.w *= keep;
 #pragma unroll
       for (int i = 0; i < AHEAD; i++) {
-        if (st[i].x == -INFINITY) { continue; }  // of a part that saw nothing
+        // (a part that saw nothing has a sum of 0, one whose scores are all no numbers has one that is none either)
         const float f = power_of_2(st[i].x - safe);
         sum           = fmaf(st[i].y, f, sum);
+        if (st[i].x == -INFINITY) { continue; }
         x.x           = fmaf(y[i].x, f, x.x);
         x.y           = fmaf(y[i].y, f, x.y);
         x.z           = fmaf(y[i].z, f, x.z);
@@ -304,10 +305,10 @@ tree_join_kernel(tree_view t, tree_parts parts, uint32_t dim, uint32_t n_heads, 
 #pragma unroll
     for (int v = 0; v < kTreeJoinWarps; v++) {
       const float2 st = s_stats[v][lane];
+      const float f = power_of_2(st.x - safe);
+      sum           = fmaf(st.y, f, sum);
       if (st.x == -INFINITY) { continue; }
-      const float f  = power_of_2(st.x - safe);
       const float4 y = s_x[v][lane];
-      sum            = fmaf(st.y, f, sum);
       x.x            = fmaf(y.x, f, x.x);
       x.y            = fmaf(y.y, f, x.y);
       x.z            = fmaf(y.z, f, x.z);

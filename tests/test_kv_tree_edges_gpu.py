@@ -248,3 +248,24 @@ def test_a_token_that_is_none_attends_to_nothing(dtype, m, group, dim, bad):
         assert none.any() and (out[none] == 0).all() and (lse[none] == -math.inf).all()
         assert not out[0][~none[0]].isfinite().any() and lse[~none].isfinite().all()
         assert out[1:][~none[1:]].isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,group,dim", [(2, 2, 64), (9, 8, 64), (40, 8, 128), (9, 5, 256)])
+@pytest.mark.parametrize("lengths", [[300, 40], [20_000, 300], [130] * 300])
+def test_scores_that_are_no_numbers(dtype, m, group, dim, lengths):
+    """Of a token's query, and of all keys that one share of many has: whoever has such a score has no answer, in as many parts as it comes."""
+    step = Step(dtype, lengths, m, 2, group, dim, 16)
+    want, want_lse = step.call()
+    step.queries[0, 1, 3 % (2 * group)] = math.nan
+    out, lse = step.call()
+    touched = torch.zeros_like(lse, dtype=torch.bool)
+    touched[0, 1, 3 % (2 * group)] = True
+    assert out[touched].isnan().all() and lse[touched].isnan().all()
+    assert torch.equal(out[~touched], want[~touched]) and torch.equal(lse[~touched], want_lse[~touched])
+    slot = step.allowed()[1][0, :lengths[0] * 3 // 4]
+    step.keys[slot // 16, slot % 16, 0] = math.nan  # of the first key head
+    out, lse = step.call()
+    touched[0, :, :group] = True
+    assert out[touched].isnan().all() and lse[touched].isnan().all()
+    assert torch.equal(out[~touched], want[~touched]) and torch.equal(lse[~touched], want_lse[~touched])
