@@ -44,8 +44,8 @@ __device__ __forceinline__ void registers_down()
 }
 
 // A weight of 32 bits as the sum of two 16-bit numbers, so that a row of the output is off by little more than its own rounding: what one number
-// loses (2^-9 of each weight in bf16, 2^-12 in fp16) is as much as that.  The second number is never 0 where the first is not: 0 times an infinite value
-// would be no number.
+// loses (2^-9 of each weight in bf16, 2^-12 in fp16) is as much as that.  Neither number is 0 where the weight is 2^-30 of the largest or more: 0 times an
+// infinite value would be no number.
 // kAhead: by how much (as a power of two) a running top may be behind before sums are brought back to it.
 constexpr float kAhead = 4.0f;
 template <typename T>
@@ -56,10 +56,11 @@ struct weight_pair<__half> {
   // their digits above fp16's smallest number, 2^-24: it is 2^-35 of the largest weight, or 2^-31 where the top is behind.
   static __device__ __forceinline__ void split(float a, float b, uint32_t& high, uint32_t& low)
   {
-    // of a little less than the weight: the rest is more than 0
+    // Of a little less than the weight, by a step of 32 bits and fp16's smallest number: the rest is not rounded to 0.  (Less than 0 is cut off to 0.)
+    constexpr float kLess = 1.0f - 1.1920928955078125e-7f, kSmallest = 5.9604644775390625e-8f;  // 1 - 2^-23, 2^-24
     float x, y, u, v;
-    mul2(two(a, b), two(1.0f - 1.1920928955078125e-7f, 1.0f - 1.1920928955078125e-7f)).get(x, y);
-    asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(high) : "f"(y), "f"(x));
+    fma2(two(a, b), two(kLess, kLess), two(-kSmallest, -kSmallest)).get(x, y);
+    asm("cvt.rz.relu.f16x2.f32 %0, %1, %2;" : "=r"(high) : "f"(y), "f"(x));
     const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&high));
     add2(two(a, b), two(-h.x, -h.y)).get(u, v);
     asm("cvt.rn.f16x2.f32 %0, %2, %1;" : "=r"(low) : "f"(u), "f"(v));

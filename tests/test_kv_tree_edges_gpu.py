@@ -269,3 +269,26 @@ def test_scores_that_are_no_numbers(dtype, m, group, dim, lengths):
     touched[0, :, :group] = True
     assert out[touched].isnan().all() and lse[touched].isnan().all()
     assert torch.equal(out[~touched], want[~touched]) and torch.equal(lse[~touched], want_lse[~touched])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,group,dim", [(1, 2, 64), (3, 8, 128), (20, 8, 64), (20, 8, 128), (3, 8, 256)])
+def test_an_infinite_value_of_a_small_weight(dtype, m, group, dim):
+    """Weights from 1 down to 2^-30 of the largest, in a tile that all rows see whole: the output is infinite, of the value's sign."""
+    n = 300
+    step = Step(dtype, [200] * n, m, 1, group, dim, 16)
+    slot = step.allowed()[1]
+    step.queries.zero_()
+    step.queries[..., 0] = 1.0
+    step.keys.zero_()
+    step.keys[..., 0] = -100.0
+    row = torch.arange(n, device="cuda")
+    first, small = slot[:, 5], slot[:, 70]
+    step.keys[first // 16, first % 16, 0, 0] = 0.0
+    weight = torch.linspace(0.0, 29.9 * math.log(2), n, device="cuda").to(dtype)
+    weight = torch.where(weight.float() > 29.95 * math.log(2), 29.9 * math.log(2) - 0.05, weight.float()).to(dtype)  # (rounded up)
+    step.keys[small // 16, small % 16, 0, 0] = -weight
+    step.values[small // 16, small % 16, 0, 3] = torch.where(row % 2 == 0, math.inf, -math.inf).to(dtype)
+    out, lse = step.call(scale=1.0)
+    want = torch.where(row % 2 == 0, math.inf, -math.inf)[:, None, None].expand(n, m, group)
+    assert torch.equal(out[..., 3].float(), want) and out[..., :3].isfinite().all() and out[..., 4:].isfinite().all() and lse.isfinite().all()
