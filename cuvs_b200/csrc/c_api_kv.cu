@@ -470,6 +470,17 @@ bool attend_tree_call(resources& res, cudaStream_t stream, kv::attend_tree_args 
   return true;
 }
 
+// Whether `n` integers share memory with a row of `t` (integers of 32 bits [rows, columns], those of a row contiguous).
+bool in_rows_of(const int32_t* at, int64_t n, const tensor& t)
+{
+  const int64_t rows = t.shape[0], columns = t.shape[1], bytes = 4 * columns, stride = 4 * t.stride[0];
+  if (n == 0 || rows == 0 || columns == 0) { return false; }
+  const int64_t from = reinterpret_cast<const char*>(at) - t.data, to = from + 4 * n;  // [from, to) against [row * stride, row * stride + bytes)
+  if (stride == 0) { return from < bytes && to > 0; }
+  const int64_t row = from < bytes ? 0 : (from - bytes) / stride + 1;  // the first that ends behind `from`
+  return row < rows && row * stride < to;
+}
+
 kv::keep_path_args keep_path_of(int device, tensor* t)
 {
   enum { KEYS, VALUES, PAGES, LENGTHS, PATHS, KEPT };
@@ -486,9 +497,10 @@ kv::keep_path_args keep_path_of(int device, tensor* t)
   CUVS_EXPECTS(t[PATHS].shape[1] <= kMostDrafted, "paths: at most %lld entries, not %lld", (long long)kMostDrafted, (long long)t[PATHS].shape[1]);
   a.n_entries = uint32_t(t[PATHS].shape[1]);
   a.kept      = const_cast<int32_t*>(ints_of(device, t[KEPT], "kept", a.n_sequences, "sequence"));
-  // blocks of a sequence read its length while one of them writes the new one
+  // blocks of a sequence read its length, its path and its pages while one of them writes the new length
   const int64_t n = a.n_sequences;
   CUVS_EXPECTS(n == 0 || a.kept + n <= a.lengths || a.lengths + n <= a.kept, "kept: must not be the lengths' own memory");
+  CUVS_EXPECTS(!in_rows_of(a.kept, n, t[PATHS]) && !in_rows_of(a.kept, n, t[PAGES]), "kept: must not be memory of the paths or the pages");
   CUVS_EXPECTS(uint64_t(n) * 2 * a.cache.n_heads * (a.row_bytes / 16) < (uint64_t(1) << 37), "pages: too many sequences");
   return a;
 }

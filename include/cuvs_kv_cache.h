@@ -108,8 +108,8 @@ CUVS_EXPORT cuvsError_t cuvsKvCacheAttendTreeWorkspace(cuvsResources_t res, DLMa
 
 /* Moves the rows of the drafted tokens that stay up to their sequences' ends: paths i32 [n_sequences, n_entries] (at most 1024) names them in
  * ascending order, and ends at the first entry that is not greater than the one before it (-1, say) or whose length no i32 holds.  The row at place lengths[i] + path[m] goes to
- * place lengths[i] + m, where both have slots; kept: i32 [n_sequences], receives lengths[i] + the number of entries (not the lengths' own
- * memory).  No two sequences may have the pages that this writes in common. */
+ * place lengths[i] + m, where both have slots; kept: i32 [n_sequences], receives lengths[i] + the number of entries (in memory
+ * of its own, not that of lengths, paths or pages).  No two sequences may have the pages that this writes in common. */
 CUVS_EXPORT cuvsError_t cuvsKvCacheKeepPath(cuvsResources_t res, DLManagedTensor* keys, DLManagedTensor* values, DLManagedTensor* pages,
                                             DLManagedTensor* lengths, DLManagedTensor* paths, DLManagedTensor* kept);
 
