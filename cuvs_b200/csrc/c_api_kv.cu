@@ -438,6 +438,9 @@ kv::attend_tree_args attend_tree_of(int device, tensor* t, float scale, int64_t 
   }
   CUVS_EXPECTS(std::isfinite(scale), "scale must be finite");
   CUVS_EXPECTS(cap == 0.0f || (cap >= 0.99e-30f && cap <= 1.01e30f), "cap must be 0 (none) or between 1e-30 and 1e30");
+  // scores are formed in powers of two and divided by the cap in one factor
+  CUVS_EXPECTS(std::isfinite(scale * 1.5f), "scale: too large");
+  CUVS_EXPECTS(cap == 0.0f || scale == 0.0f || std::isnormal(scale / cap), "scale / cap must lie in the range of 32-bit numbers");
   CUVS_EXPECTS(window >= 0, "window must not be negative");
   a.scale  = scale;
   a.cap    = cap;

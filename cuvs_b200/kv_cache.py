@@ -330,8 +330,8 @@ def attend_tree(keys, values, queries, pages, lengths, positions, mask, scale=No
     ``[n_sequences, n_drafted]``) and ``mask`` (uint32 ``[n_sequences, n_drafted, words]``) as :func:`draft_tree` returns them, or any others, sequences may share
     them; a token whose position is below its sequence's length is none: it attends to nothing, and none to it.
 
-    Scores are ``s = scale * q.k`` (``dim ** -0.5``), with ``cap`` (1e-30 to 1e30) then ``cap * tanh(s / cap)``, with ``slopes`` (float32 ``[n_query_heads]``) then less ``slope *
-    distance`` of the two positions.  ``window``: only what is less than so many positions before the token's own; ``filter``, ``workspace`` as in
+    Scores are ``s = scale * q.k`` (``dim ** -0.5``), with ``cap`` (1e-30 to 1e30, ``scale / cap`` in the range of 32-bit numbers) then ``cap *
+    tanh(s / cap)``, with ``slopes`` (float32 ``[n_query_heads]``) then less ``slope * distance`` of the two positions.  ``window``: only what is less than so many positions before the token's own; ``filter``, ``workspace`` as in
     :func:`attention`.  Of 16-bit rows, weights below 2^-30 of the largest may count as 0."""
     window = _window(window)
     resources, stream = _handle(keys, resources)

@@ -93,10 +93,9 @@ CUVS_EXPORT cuvsError_t cuvsKvCacheDraftTree(cuvsResources_t res, DLManagedTenso
  * cuvsKvCacheDraftTree leaves them, or others (strides of sequences and of the mask's tokens may be 0).  Token j attends to the positions
  * 0 .. lengths[i] - 1 and to the drafted tokens k whose bits its row of the mask has, each at its position, as far as that is less than `window`
  * before its own (window > 0; 0: all), in the cache and let through by the filter.  A token whose position is below its sequence's length is
- * none: it attends to nothing, and none to it.  Scores are s = scale * q.k, with cap (0: none; 1e-30 to
- * 1e30) then cap * tanh(s / cap), with slopes (f32
- * [n_query_heads]) then less slope * distance of the positions.  lse: f32 [n_sequences, n_drafted, n_query_heads].  In attention to 16-bit rows
- * weights below 2^-30 of the largest may count as 0.  Workspace as in cuvsKvCacheAttention.  Attention to 16-bit rows waits inside its kernel, with
+ * none: it attends to nothing, and none to it.  Scores are s = scale * q.k, with cap (0: none; 1e-30 to 1e30, scale / cap in the range of
+ * 32-bit numbers) then cap * tanh(s / cap), with slopes (f32 [n_query_heads]) then less slope * distance of the positions.  lse: f32
+ * [n_sequences, n_drafted, n_query_heads].  In attention to 16-bit rows weights below 2^-30 of the largest may count as 0.  Workspace as in cuvsKvCacheAttention.  Attention to 16-bit rows waits inside its kernel, with
  * limits of seconds: should one run out, the next wait for the stream through this handle (cuvsStreamSync) is an error, of a captured call the next
  * wait for any stream. */
 CUVS_EXPORT cuvsError_t cuvsKvCacheAttendTree(cuvsResources_t res, DLManagedTensor* keys, DLManagedTensor* values, DLManagedTensor* queries,
@@ -107,9 +106,9 @@ CUVS_EXPORT cuvsError_t cuvsKvCacheAttendTreeWorkspace(cuvsResources_t res, DLMa
                                                        DLManagedTensor* pages, int64_t window, size_t* bytes);
 
 /* Moves the rows of the drafted tokens that stay up to their sequences' ends: paths i32 [n_sequences, n_entries] (at most 1024) names them in
- * ascending order, and ends at the first entry that is not greater than the one before it (-1, say) or whose length no i32 holds.  The row at place lengths[i] + path[m] goes to
- * place lengths[i] + m, where both have slots; kept: i32 [n_sequences], receives lengths[i] + the number of entries (in memory
- * of its own, not that of lengths, paths or pages).  No two sequences may have the pages that this writes in common. */
+ * ascending order, and ends at the first entry that is not greater than the one before it (-1, say) or whose length no i32 holds.  The row
+ * at place lengths[i] + path[m] goes to place lengths[i] + m, where both have slots; kept: i32 [n_sequences], receives lengths[i] + the number of
+ * entries (in memory of its own, not that of lengths, paths or pages).  No two sequences may have the pages that this writes in common. */
 CUVS_EXPORT cuvsError_t cuvsKvCacheKeepPath(cuvsResources_t res, DLManagedTensor* keys, DLManagedTensor* values, DLManagedTensor* pages,
                                             DLManagedTensor* lengths, DLManagedTensor* paths, DLManagedTensor* kept);
 

@@ -1,8 +1,9 @@
-"""CPU tests: what keep_path writes must not be what it reads, as far as its checks can tell (no GPU)."""
+"""CPU tests of the checks of a step of drafted tokens (no GPU): what keep_path writes is not what it reads, scales and caps whose ratio is a number."""
 import pytest
 
 from cuvs_b200 import _lib as L
-from test_kv_tree import I, K, check
+from cuvs_b200 import kv_cache
+from test_kv_tree import I, K, T, check
 from test_kv_cache import Described
 
 BASE = 1 << 41
@@ -35,3 +36,25 @@ def test_kept_and_rows_that_sequences_share():
 
 def test_empty_paths_share_nothing():
     check(K, {"paths": Described(I, (3, 0), address=BASE), "kept": Described(I, (3,), address=BASE)})
+
+
+def scalars(scale, cap):
+    return 0, kv_cache._bits(scale), kv_cache._bits(cap)
+
+
+@pytest.mark.parametrize("scale,cap", [(1e9, 1e-30), (-1e9, 1e-30), (1e-10, 1e30), (1e-40, 1.0)])
+def test_scales_that_no_32_bit_number_divides_by_the_cap(scale, cap):
+    with pytest.raises(L.CuvsError, match="scale / cap"):
+        check(T, scalars=scalars(scale, cap))
+    check(T, scalars=scalars(scale, 0.0))
+
+
+def test_scales_at_the_ends_of_their_range():
+    for cap in (0.0, 1e-30, 50.0, 1e30):
+        check(T, scalars=scalars(0.0, cap))
+    for scale in (1e8, -1e8, 1e-7):
+        for cap in (1e-30, 1e30):
+            check(T, scalars=scalars(scale, cap))
+    for scale in (3e38, -3e38):
+        with pytest.raises(L.CuvsError, match="scale: too large"):
+            check(T, scalars=scalars(scale, 0.0))
