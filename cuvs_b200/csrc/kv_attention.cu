@@ -327,8 +327,14 @@ struct mma_hooks {
       load_matrices_turned(a, v_rows + row * shape::kRowBytes + ((piece ^ (row & 7u)) << 4));
 #pragma unroll
       for (int n = 0; n < NT; n++) {
+        // The tensor core cuts off what it adds to a sum, always towards 0: it gets the products of these keys alone, and what they come to is
+        // added in 32 bits, rounded.  (With a sum of all keys outputs of 300 sequences of 200,000 tokens were 2.9e-4 too small in fp16, 4.6e-4 in
+        // bf16.  It costs 8% where 16 query heads or more go with a key head, 0.5% where HBM is what counts.)
+        float t[4] = {};
 #pragma unroll
-        for (int i = 0; i < N; i++) { multiply_add<T>(acc[n][d], a, part[n][0][i], part[n][1][i]); }
+        for (int i = 0; i < N; i++) { multiply_add<T>(t, a, part[n][0][i], part[n][1][i]); }
+#pragma unroll
+        for (int e = 0; e < 4; e++) { acc[n][d][e] += t[e]; }
       }
     }
   }
