@@ -429,6 +429,47 @@ __device__ __forceinline__ void shape_scores(const tree_view& t, const tree_piec
   }
 }
 
+// Adds the sums of this thread's row and stream that were set aside (`some`: there are) to those in tensor memory, which are set aside in their turn, or
+// put back at the piece's end.
+template <uint32_t kRows>
+__device__ __forceinline__ void add_sums_aside(float4* aside, uint32_t sums, uint32_t dim, bool exists, bool some, float top, float& aside_top, bool back)
+{
+  const uint32_t width = (dim + 31) / 32;
+  const float keep     = some ? power_of_2(aside_top - finite_top(top)) : 0.0f;
+#pragma unroll 1
+  for (uint32_t i = 0; i < width; i++) {
+    float4 y[8];
+#pragma unroll
+    for (uint32_t q = 0; q < 8; q++) {
+      y[q] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (some && (i * 8 + q) * 4 < dim) { y[q] = aside[(i * 8 + q) * kRows]; }
+    }
+    uint32_t o[32];
+    tmem_ld32(sums + i * 32, o);
+#pragma unroll
+    for (uint32_t q = 0; q < 8; q++) {
+      y[q] = make_float4(fmaf(y[q].x, keep, __uint_as_float(o[4 * q])), fmaf(y[q].y, keep, __uint_as_float(o[4 * q + 1])),
+                         fmaf(y[q].z, keep, __uint_as_float(o[4 * q + 2])), fmaf(y[q].w, keep, __uint_as_float(o[4 * q + 3])));
+      if (!back && exists && (i * 8 + q) * 4 < dim) { aside[(i * 8 + q) * kRows] = y[q]; }
+      o[4 * q]     = __float_as_uint(y[q].x);
+      o[4 * q + 1] = __float_as_uint(y[q].y);
+      o[4 * q + 2] = __float_as_uint(y[q].z);
+      o[4 * q + 3] = __float_as_uint(y[q].w);
+    }
+    __syncwarp();
+    if (back) { tmem_st32(sums + i * 32, o); }
+  }
+  if (back) { tmem_st_wait(); }
+  aside_top = top;
+}
+// Out of the way of the loop over tiles, where that is short: 4 requests of 60,000 + 64 tokens, 4 key heads of 8, 64 columns fp16, 166 us, 190 inside it; but
+// capped scores (16 requests, 128 columns) 293, 286 inside.
+template <uint32_t kRows>
+__device__ __noinline__ void add_sums_aside_apart(float4* aside, uint32_t sums, uint32_t dim, bool exists, bool some, float top, float& aside_top, bool back)
+{
+  add_sums_aside<kRows>(aside, sums, dim, exists, some, top, aside_top, back);
+}
+
 template <typename T, int D, bool SHAPED>
 __device__ __forceinline__ void softmax_role(const tc_args& a, tc_shared& sh, char* smem, const waiter& wait, uint32_t which, uint32_t block)
 {
@@ -447,38 +488,16 @@ __device__ __forceinline__ void softmax_role(const tc_args& a, tc_shared& sh, ch
   const uint32_t sh_tmem = sh.tmem;
   const uint32_t sums  = sh_tmem + lanes + shape::kSumsAt + (shape::kTwo ? stream * 128 : 0);
   const uint32_t width = (a.c.dim + 31) / 32;  // columns of the sums, in 32
-  // After `done` tiles: adds the sums of this row and stream that were set aside to those in tensor memory, which are set aside in their turn, or put
-  // back at the piece's end.  (Their top stands where the piece's will.)
+  // (their top stands where the piece's will)
   auto add_aside = [&](float top, uint32_t done, bool back) {
     constexpr uint32_t kRows = shape::kTwo ? 256 : 128;
     float4* const aside      = a.aside + size_t(blockIdx.x) * (a.c.dim / 4) * kRows + stream * 128 + in;
     const bool some          = exists && done > kChain - stream * (kChain / 2);
-    const float keep         = some ? power_of_2(sh.stats[stream][in].x - finite_top(top)) : 0.0f;
-#pragma unroll 1
-    for (uint32_t i = 0; i < width; i++) {
-      float4 y[8];
-#pragma unroll
-      for (uint32_t q = 0; q < 8; q++) {
-        y[q] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (some && (i * 8 + q) * 4 < a.c.dim) { y[q] = aside[(i * 8 + q) * kRows]; }
-      }
-      uint32_t o[32];
-      tmem_ld32(sums + i * 32, o);
-#pragma unroll
-      for (uint32_t q = 0; q < 8; q++) {
-        y[q] = make_float4(fmaf(y[q].x, keep, __uint_as_float(o[4 * q])), fmaf(y[q].y, keep, __uint_as_float(o[4 * q + 1])),
-                           fmaf(y[q].z, keep, __uint_as_float(o[4 * q + 2])), fmaf(y[q].w, keep, __uint_as_float(o[4 * q + 3])));
-        if (!back && exists && (i * 8 + q) * 4 < a.c.dim) { aside[(i * 8 + q) * kRows] = y[q]; }
-        o[4 * q]     = __float_as_uint(y[q].x);
-        o[4 * q + 1] = __float_as_uint(y[q].y);
-        o[4 * q + 2] = __float_as_uint(y[q].z);
-        o[4 * q + 3] = __float_as_uint(y[q].w);
-      }
-      __syncwarp();
-      if (back) { tmem_st32(sums + i * 32, o); }
+    if constexpr (SHAPED) {
+      add_sums_aside<kRows>(aside, sums, a.c.dim, exists, some, top, sh.stats[stream][in].x, back);
+    } else {
+      add_sums_aside_apart<kRows>(aside, sums, a.c.dim, exists, some, top, sh.stats[stream][in].x, back);
     }
-    if (back) { tmem_st_wait(); }
-    sh.stats[stream][in].x = top;
   };
   piece_reader reader;
   tree_piece p;
