@@ -130,8 +130,11 @@ struct piece_reader {
   }
 };
 
-// Whether tile `i` of a stream's piece begins sums in tensor memory; the two streams' turns do not come at the same time.
-__device__ __forceinline__ bool begins_sums(uint32_t i, uint32_t stream) { return i == 0u || (i + stream * (kChain / 2)) % kChain == 0u; }
+// The tile of a stream's piece before which sums that have tile `i` are set aside; the two streams' turns do not come at the same time.
+__device__ __forceinline__ uint32_t sums_end(uint32_t i, uint32_t stream)
+{
+  return ((i + stream * (kChain / 2)) / kChain + 1) * kChain - stream * (kChain / 2);
+}
 
 // Whether a tile has keys that not all rows see.
 __device__ __forceinline__ bool is_mixed(const tree_view& t, const tree_piece& p, uint32_t base)
@@ -353,7 +356,7 @@ __device__ __forceinline__ void multiply_role(const tc_args& a, tc_shared& sh, c
       if (!wait(sh.p_full[stream * 2 + buffer], p_turn >> buffer)) { ok = false; break; }
       p_turn ^= 1u << buffer;
       tc_fence_after();
-      const bool anew = begins_sums(i, stream);
+      const bool anew = i == 0u || sums_end(i - 1, stream) == i;
       if (elect_one()) {
         if (good) {
           // 32 keys of weights stand where their scores stood: 16 columns of the first numbers, 16 of the second
@@ -462,8 +465,8 @@ __device__ __forceinline__ void add_sums_aside(float4* aside, uint32_t sums, uin
   if (back) { tmem_st_wait(); }
   aside_top = top;
 }
-// Out of the way of the loop over tiles, where that is short: 4 requests of 60,000 + 64 tokens, 4 key heads of 8, 64 columns fp16, 166 us, 190 inside it; but
-// capped scores (16 requests, 128 columns) 293, 286 inside.
+// Out of the way of the loop over tiles, where that is short: 4 requests of 60,000 + 64 tokens, 4 key heads of 8, 64 columns fp16, 166 us, 172 to 190 beside it;
+// where scores are capped (16 requests, 128 columns) 293 us, 268 beside it.
 template <uint32_t kRows>
 __device__ __noinline__ void add_sums_aside_apart(float4* aside, uint32_t sums, uint32_t dim, bool exists, bool some, float top, float& aside_top, bool back)
 {
@@ -519,148 +522,156 @@ __device__ __forceinline__ void softmax_role(const tc_args& a, tc_shared& sh, ch
     const int32_t edge_to   = t.window > 0 ? int32_t((int64_t(p.latest) - t.window - int64_t(p.base)) >> 6) : -1;
     uint32_t done = 0;  // tiles of this stream
     bool ok = true;
-    for (uint32_t j = alternate ? stream : 0u; j < n; j += alternate ? 2u : 1u, done++) {
-      const uint32_t buffer = stream * 2 + (done & 1u);
-      const uint32_t scores = sh_tmem + lanes + buffer * kTile;
-      if (!wait(sh.s_full[buffer], s_turn >> (done & 1u))) { ok = false; break; }
-      s_turn ^= 1u << (done & 1u);
-      tc_fence_after();
-      if (!alive) {
-        arrive_warp(sh.p_full[buffer]);
-        continue;
-      }
-      const bool anew = begins_sums(done, stream);
-      if (anew && done > 0) {
-        // (Of the tile before the last one: this tile's scores took the place of its weights.  So the barrier is at most one phase behind.)
-        if (!wait(sh.pv_done[stream], pv_turn + done - 1)) { ok = false; break; }
+    // From one turn at setting aside to the next: a test for it inside the loop over tiles cost capped scores 7%.
+    const uint32_t step = alternate ? 2u : 1u;
+    uint32_t j          = alternate ? stream : 0u;
+    while (true) {
+      const uint32_t begun = done, full = sums_end(done, stream);
+      for (; j < n && done < full; j += step, done++) {
+        const uint32_t buffer = stream * 2 + (done & 1u);
+        const uint32_t scores = sh_tmem + lanes + buffer * kTile;
+        if (!wait(sh.s_full[buffer], s_turn >> (done & 1u))) { ok = false; break; }
+        s_turn ^= 1u << (done & 1u);
         tc_fence_after();
-        add_aside(top, done, false);
-      }
-      uint32_t x[2][32];
-      tmem_ld32_async(scores, x[0]);
-      tmem_ld32_async(scores + 32, x[1]);
-      const uint32_t info = (tiles + j) % kInfos, base = p.base + (p.chunk + j) * kTile;
-      const bool mixed    = int32_t(p.chunk + j) >= tail_from || int32_t(p.chunk + j) <= edge_to;
-      const uint2 valid   = sh.valid[info];
-      const bool whole    = (valid.x & valid.y) == 0xFFFFFFFFu && !mixed;
-      tmem_ld_wait(x[0]);
-      tmem_ld_wait(x[1]);
-      if constexpr (SHAPED) {
+        if (!alive) {
+          arrive_warp(sh.p_full[buffer]);
+          continue;
+        }
+        uint32_t x[2][32];
+        tmem_ld32_async(scores, x[0]);
+        tmem_ld32_async(scores + 32, x[1]);
+        const uint32_t info = (tiles + j) % kInfos, base = p.base + (p.chunk + j) * kTile;
+        const bool mixed    = int32_t(p.chunk + j) >= tail_from || int32_t(p.chunk + j) <= edge_to;
+        const uint2 valid   = sh.valid[info];
+        const bool whole    = (valid.x & valid.y) == 0xFFFFFFFFu && !mixed;
+        tmem_ld_wait(x[0]);
+        tmem_ld_wait(x[1]);
+        if constexpr (SHAPED) {
 #pragma unroll
-        for (uint32_t i = 0; i < 2; i++) { shape_scores(t, p, positions, own, slope, base + i * 32, mixed, scores + i * 32, x[i]); }
-      }
-      if (!whole) {
+          for (uint32_t i = 0; i < 2; i++) { shape_scores(t, p, positions, own, slope, base + i * 32, mixed, scores + i * 32, x[i]); }
+        }
+        if (!whole) {
+#pragma unroll
+          for (uint32_t i = 0; i < 2; i++) {
+            uint32_t seen = i == 0 ? valid.x : valid.y;
+            if (mixed) { seen &= seen_keys(t, l, positions, own, mask, base + i * 32); }
+#pragma unroll
+            for (int k = 0; k < 32; k++) { x[i][k] = ((seen >> k) & 1u) != 0u ? x[i][k] : 0xFF800000u; }
+          }
+          __syncwarp();
+        }
+        float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
         for (uint32_t i = 0; i < 2; i++) {
-          uint32_t seen = i == 0 ? valid.x : valid.y;
-          if (mixed) { seen &= seen_keys(t, l, positions, own, mask, base + i * 32); }
 #pragma unroll
-          for (int k = 0; k < 32; k++) { x[i][k] = ((seen >> k) & 1u) != 0u ? x[i][k] : 0xFF800000u; }
-        }
-        __syncwarp();
-      }
-      float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          for (int k = 0; k < 32; k += 4) {
 #pragma unroll
-      for (uint32_t i = 0; i < 2; i++) {
-#pragma unroll
-        for (int k = 0; k < 32; k += 4) {
-#pragma unroll
-          for (int e = 0; e < 4; e++) { most[e] = fmaxf(most[e], __uint_as_float(x[i][k + e])); }
-        }
-      }
-      float highest = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
-      if constexpr (!SHAPED) { highest *= t.scale_log2; }  // (a scale above 0)
-      // (a top of -inf: nothing was seen, and the sums are 0)
-      if (__any_sync(kAllLanes, highest > top + kAhead)) {
-        const float next = highest > top + kAhead ? highest : top;
-        const float keep = top == -INFINITY ? 1.0f : power_of_2(top - next);
-        if (!anew && __any_sync(kAllLanes, keep != 1.0f)) {
-          // the tile before may still be added up
-          if (!wait(sh.pv_done[stream], pv_turn + done - 1)) { ok = false; break; }
-          tc_fence_after();
-#pragma unroll 1
-          for (uint32_t i = 0; i < width; i++) {
-            uint32_t o[32];
-            tmem_ld32(sums + i * 32, o);
-#pragma unroll
-            for (int k = 0; k < 32; k++) { o[k] = __float_as_uint(__uint_as_float(o[k]) * keep); }
-            tmem_st32(sums + i * 32, o);
+            for (int e = 0; e < 4; e++) { most[e] = fmaxf(most[e], __uint_as_float(x[i][k + e])); }
           }
-          tmem_st_wait();
         }
-        sum *= keep;
-        top = next;
-      }
-      const float from = a.shift - finite_top(top), by = SHAPED ? 1.0f : t.scale_log2;
-      const two from2(from, from), by2(by, by);
-      two part[2] = {two(0.0f, 0.0f), two(0.0f, 0.0f)};
-#pragma unroll
-      for (uint32_t i = 0; i < 2; i++) {
-        uint32_t pairs[32];
-#pragma unroll
-        for (int k = 0; k < 32; k += 2) {
-          float u, v;
-          fma2(two(__uint_as_float(x[i][k]), __uint_as_float(x[i][k + 1])), by2, from2).get(u, v);
-          u = power_of_2(u);
-          v = power_of_2(v);
-          part[(k / 2) % 2] = add2(part[(k / 2) % 2], two(u, v));
-          weight_pair<T>::split(u, v, pairs[k / 2], pairs[16 + k / 2]);
-        }
-        tmem_st32(scores + i * 32, pairs);
-      }
-      tmem_st_wait();
-      {
-        float u, v;
-        add2(part[0], part[1]).get(u, v);
-        sum += u + v;
-      }
-      if (mixed) {
-        // Values that are no numbers must not reach rows that do not see them, as 0 times them would: each row adds up what it sees.
-        const uint32_t slot = (tiles + j) % shape::kValues;
-        if (!wait(sh.v_full[slot], (tiles + j) / shape::kValues)) { ok = false; break; }
-        const uint2 bad = sh.bad[info];
-        if ((bad.x | bad.y) != 0u) {
-          if (done > 0 && !wait(sh.pv_done[stream], pv_turn + done - 1)) { ok = false; break; }
-          tc_fence_after();
-          const char* v = smem + shape::kValuesAt + slot * shape::kTileBytes;
+        float highest = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
+        if constexpr (!SHAPED) { highest *= t.scale_log2; }  // (a scale above 0)
+        // (a top of -inf: nothing was seen, and the sums are 0)
+        if (__any_sync(kAllLanes, highest > top + kAhead)) {
+          const float next = highest > top + kAhead ? highest : top;
+          const float keep = top == -INFINITY ? 1.0f : power_of_2(top - next);
+          if (done != begun && __any_sync(kAllLanes, keep != 1.0f)) {
+            // the tile before may still be added up
+            if (!wait(sh.pv_done[stream], pv_turn + done - 1)) { ok = false; break; }
+            tc_fence_after();
 #pragma unroll 1
-          for (uint32_t i = 0; i < width; i++) {
-            uint32_t o[32];
-            if (!anew) {
+            for (uint32_t i = 0; i < width; i++) {
+              uint32_t o[32];
               tmem_ld32(sums + i * 32, o);
-            } else {
 #pragma unroll
-              for (int k = 0; k < 32; k++) { o[k] = 0u; }
+              for (int k = 0; k < 32; k++) { o[k] = __float_as_uint(__uint_as_float(o[k]) * keep); }
+              tmem_st32(sums + i * 32, o);
             }
-#pragma unroll 1
-            for (uint32_t k0 = 0; k0 < kTile; k0 += 32) {
-              uint32_t pairs[32];
-              tmem_ld32(scores + k0, pairs);
-#pragma unroll
-              for (uint32_t k = 0; k < 32; k++) {
-                const float2 pair = weight_pair<T>::join(pairs[k / 2], pairs[16 + k / 2]);
-                const float x     = (k & 1u) != 0u ? pair.y : pair.x;
-                if (x == 0.0f) { continue; }
-                const uint32_t key = k0 + k;
-#pragma unroll
-                for (uint32_t q = 0; q < 4; q++) {
-                  const uint32_t column = i * 4 + q;  // in pieces
-                  if (column * 8 >= a.c.dim) { break; }
-                  float f[8];
-                  piece_to_floats<T>(*reinterpret_cast<const uint4*>(v + (column >> 3) * shape::kPanel + key * 128 + (((column & 7u) ^ (key & 7u)) << 4)), f);
-#pragma unroll
-                  for (int e = 0; e < 8; e++) { o[q * 8 + e] = __float_as_uint(fmaf(x, f[e], __uint_as_float(o[q * 8 + e]))); }
-                }
-              }
-              __syncwarp();
-            }
-            tmem_st32(sums + i * 32, o);
+            tmem_st_wait();
           }
-          tmem_st_wait();
+          sum *= keep;
+          top = next;
         }
+        const float from = a.shift - finite_top(top), by = SHAPED ? 1.0f : t.scale_log2;
+        const two from2(from, from), by2(by, by);
+        two part[2] = {two(0.0f, 0.0f), two(0.0f, 0.0f)};
+#pragma unroll
+        for (uint32_t i = 0; i < 2; i++) {
+          uint32_t pairs[32];
+#pragma unroll
+          for (int k = 0; k < 32; k += 2) {
+            float u, v;
+            fma2(two(__uint_as_float(x[i][k]), __uint_as_float(x[i][k + 1])), by2, from2).get(u, v);
+            u = power_of_2(u);
+            v = power_of_2(v);
+            part[(k / 2) % 2] = add2(part[(k / 2) % 2], two(u, v));
+            weight_pair<T>::split(u, v, pairs[k / 2], pairs[16 + k / 2]);
+          }
+          tmem_st32(scores + i * 32, pairs);
+        }
+        tmem_st_wait();
+        {
+          float u, v;
+          add2(part[0], part[1]).get(u, v);
+          sum += u + v;
+        }
+        if (mixed) {
+          // Values that are no numbers must not reach rows that do not see them, as 0 times them would: each row adds up what it sees.
+          const uint32_t slot = (tiles + j) % shape::kValues;
+          if (!wait(sh.v_full[slot], (tiles + j) / shape::kValues)) { ok = false; break; }
+          const uint2 bad = sh.bad[info];
+          if ((bad.x | bad.y) != 0u) {
+            if (done > 0 && !wait(sh.pv_done[stream], pv_turn + done - 1)) { ok = false; break; }
+            tc_fence_after();
+            const char* v = smem + shape::kValuesAt + slot * shape::kTileBytes;
+#pragma unroll 1
+            for (uint32_t i = 0; i < width; i++) {
+              uint32_t o[32];
+              if (done != begun) {
+                tmem_ld32(sums + i * 32, o);
+              } else {
+#pragma unroll
+                for (int k = 0; k < 32; k++) { o[k] = 0u; }
+              }
+#pragma unroll 1
+              for (uint32_t k0 = 0; k0 < kTile; k0 += 32) {
+                uint32_t pairs[32];
+                tmem_ld32(scores + k0, pairs);
+#pragma unroll
+                for (uint32_t k = 0; k < 32; k++) {
+                  const float2 pair = weight_pair<T>::join(pairs[k / 2], pairs[16 + k / 2]);
+                  const float x     = (k & 1u) != 0u ? pair.y : pair.x;
+                  if (x == 0.0f) { continue; }
+                  const uint32_t key = k0 + k;
+#pragma unroll
+                  for (uint32_t q = 0; q < 4; q++) {
+                    const uint32_t column = i * 4 + q;  // in pieces
+                    if (column * 8 >= a.c.dim) { break; }
+                    float f[8];
+                    piece_to_floats<T>(*reinterpret_cast<const uint4*>(v + (column >> 3) * shape::kPanel + key * 128 + (((column & 7u) ^ (key & 7u)) << 4)), f);
+#pragma unroll
+                    for (int e = 0; e < 8; e++) { o[q * 8 + e] = __float_as_uint(fmaf(x, f[e], __uint_as_float(o[q * 8 + e]))); }
+                  }
+                }
+                __syncwarp();
+              }
+              tmem_st32(sums + i * 32, o);
+            }
+            tmem_st_wait();
+          }
+        }
+        tc_fence_before();
+        arrive_warp(sh.p_full[buffer]);
       }
-      tc_fence_before();
-      arrive_warp(sh.p_full[buffer]);
+      if (!ok || j >= n) { break; }
+      if (alive) {
+        // (The scores of the next tile took the place of the weights of the last tile but one, which has been added up then: the barrier is at most one
+        // phase behind, and no further one ends before this warp has written its next weights.)
+        if (!wait(sh.s_full[stream * 2 + (done & 1u)], s_turn >> (done & 1u)) || !wait(sh.pv_done[stream], pv_turn + done - 1)) { ok = false; break; }
+        tc_fence_after();
+        add_aside(top, done, false);
+        tc_fence_before();
+      }
     }
     if (!ok) { return; }
     if (!is_token) {  // whatever stands in the sums of a row that is none
