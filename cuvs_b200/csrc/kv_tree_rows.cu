@@ -43,7 +43,7 @@ constexpr int tree_resident(int columns) { return columns == 64 ? 2 : 1; }
 // and their weighted sums in every 16th four columns.
 //
 // What bounds it: 32-bit multiply-adds, and the barriers between a tile's steps with few blocks of an SM.  One sequence of 20,000 + 64 tokens, 2 key heads of 4,
-// 128 columns: 210 us, 25 TFLOP/s (264 where a tile was loaded between barriers).
+// 128 columns: 188 us, 28 TFLOP/s (264 where a tile was loaded between barriers).
 template <int D>
 struct tree_shape {
   static constexpr int BM     = 64;
@@ -603,7 +603,9 @@ tree_few_kernel(cache_view c, work_view w, few_lists lists, tree_view t, tree_pa
 // Rows of a block of the kernel for few, by how many a unit has.
 constexpr uint32_t few_rows_of(uint32_t n_rows, uint32_t dim) { return n_rows <= 4 ? 4 : n_rows <= 8 || dim > 128 ? 8 : 16; }
 // Which kernel: 4 sequences of 20,000 tokens, 2 key heads, us by warps alone and in tiles of 64 rows: 64 columns 16 rows 46 and 67, 32 rows 68 and 68;
-// 128 columns 16 rows 83 and 117, 32 rows 145 and 117; 256 columns 32 rows 222 and 260, 40 rows 273 and 260.
+// 128 columns 16 rows 83 and 117, 32 rows 145 and 117; 256 columns 32 rows 222 and 260, 40 rows 273 and 260.  With a window of 4,000 (9 of 9,000, 12 heads)
+// 16 rows 155 and 251, 334 and 484, 256 columns 32 rows 1,014 and 1,096.  Of many short units (40 of 306 tokens, 8 heads) 16 rows 66 and 75, 119 and 138, 256
+// columns 24 rows 259 and 287 but 32 rows 338 and 291; 300 of 100 tokens 16 rows 120 and 113, 224 and 216, 256 columns 32 rows 603 and 470.
 constexpr bool is_few(uint32_t n_rows, uint32_t dim) { return n_rows <= (dim <= 128 ? 16u : 32u); }
 
 tree_plan plan_of(const resources& res, elem type, uint64_t sequences, uint32_t n_drafted, uint32_t n_heads, uint32_t group, uint32_t dim,

@@ -7,12 +7,15 @@
 // halves of 256 rows on the same tiles, or even and odd tiles of the same 128 rows, whose sums are joined at a unit's end.  Each has two tiles of scores,
 // so that the next ones are formed while the softmax is at the last.  Rows of more than 128 columns leave tensor memory room for one stream.
 //
-// Sums are brought to a new top only where it is 2^4 above the old one: a turn through tensor memory that few tiles need.
+// Sums are brought to a new top only where it is 2^4 above the old one: a turn through tensor memory that few tiles need.  Every 32 tiles of a stream
+// they are set aside, for the tensor core cuts off what it adds (kChain in kv_tree.cuh).
 //
 // What bounds it: of 256 rows the softmax, 2,300 clocks of 64 keys where the products are 1,800 (with pairs of weights half again those of one
-// number): one request of 250,001 + 64 tokens, 4 key heads of 7, fp16, 348 us (658 TFLOP/s of what is asked for, 1.5 TB/s); 16 requests
-// of up to 16,384 + 32 tokens, 8 key heads of 8, bf16, 211 us, with a cap 262.  Of 32 rows HBM and the blocks' starts: the same with 4 tokens of 4 heads
-// each 121 us (3.6 TB/s).
+// number).  From replayed graphs with pauses between, and from calls back to back for seconds, for which the power limit leaves lower clocks: one request
+// of 250,001 + 64 tokens, 4 key heads of 7, fp16, 354 and 418 us (648 and 549 TFLOP/s of what is asked for); 16 requests of up to 16,384 + 32
+// tokens, 8 key heads of 8, bf16, with a cap 264 and 287 us, without 209 and 238.  Of 16 rows HBM and the blocks' starts: the same with 4 tokens of 4 heads each
+// 121 us (3.8 TB/s).  Of more than 128 columns one stream, whose scores and weights nothing covers: 32 requests of up to 8,192 + 8 tokens, 2 key heads of
+// 8, bf16, 66 us with 192 columns, 74 with 256 (bytes alone: 26, 35).
 #include "kv_tree_tc.cuh"
 
 #include <algorithm>

@@ -25,10 +25,10 @@ output is 0 and its ``lse`` is -inf.  Weights below 2^-100 of the largest may co
 A decoder that drafts several tokens per sequence, a tree of them, and keeps the path that it accepts has as its step::
 
     mask, positions = kv_cache.draft_tree(parents, lengths)                     # [n_sequences, n_drafted]; lengths: without the drafted tokens
-    places = lengths[:, None] + torch.arange(n_drafted, dtype=torch.int32, device="cuda")
-    slots, q = kv_cache.append(keys, values, new_keys.flatten(0, 1), new_values.flatten(0, 1), pages,
-                               torch.where(positions >= 0, places, -1).flatten(), sequences=sequences, queries=queries.flatten(0, 1),
-                               frequencies=frequencies, turns=positions.flatten())
+    places = torch.where(positions >= 0, lengths[:, None] + torch.arange(n_drafted, dtype=torch.int32, device="cuda"), -1).flatten()
+    # these hold for all layers; for each of them
+    slots, q = kv_cache.append(keys, values, new_keys.flatten(0, 1), new_values.flatten(0, 1), pages, places, sequences=sequences,
+                               queries=queries.flatten(0, 1), frequencies=frequencies, turns=positions.flatten())
     out, lse = kv_cache.attend_tree(keys, values, q.view(queries.shape), pages, lengths, positions, mask)
     lengths = kv_cache.keep_path(keys, values, pages, lengths, paths)           # paths: which of the drafted tokens stay, in order
 
@@ -37,7 +37,8 @@ position, by which it is turned, is that of its depth.  Where a sequence goes on
 :func:`copy_pages` copies the last one.
 
 These calls serve: they have no gradients.  They enqueue their work on the stream of ``resources`` (torch's current stream by default) and
-wait for it unless ``sync=False``, which is what a captured call needs.
+wait for it unless ``sync=False``, which is what a captured call needs.  :func:`attend_tree` of 16-bit rows waits inside its kernel, with limits of seconds:
+should one run out, the next call that waits for that stream, or ``Resources.sync``, raises an error (of a captured call, the next on any stream).
 """
 from __future__ import annotations
 
