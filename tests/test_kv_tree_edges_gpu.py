@@ -9,7 +9,7 @@ import torch
 from cuvs_b200 import Resources
 from cuvs_b200 import _lib as L
 from cuvs_b200 import kv_cache
-from test_kv_tree_gpu import DTYPES, Step, U, generator, ints, needs_a_gpu  # noqa: F401
+from test_kv_tree_gpu import DTYPES, Step, U, check, generator, ints, needs_a_gpu  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -292,3 +292,69 @@ def test_an_infinite_value_of_a_small_weight(dtype, m, group, dim):
     out, lse = step.call(scale=1.0)
     want = torch.where(row % 2 == 0, math.inf, -math.inf)[:, None, None].expand(n, m, group)
     assert torch.equal(out[..., 3].float(), want) and out[..., :3].isfinite().all() and out[..., 4:].isfinite().all() and lse.isfinite().all()
+
+
+# ---- sums that are set aside --------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("m,group,dim", [(3, 4, 128), (20, 8, 64), (20, 8, 104), (9, 4, 256)])
+@pytest.mark.parametrize("rising", [False, True])
+def test_lengths_around_the_turns_at_setting_sums_aside(dtype, m, group, dim, rising):
+    """More units than blocks, of about 16, 32, 48, .. tiles; scores whose largest stays, or grows by many powers of two on the way."""
+    lengths = [64 * tiles + more for tiles in (15, 16, 17, 31, 32, 33, 47, 48, 64, 65, 96, 97) for more in (-m, -1, 0, 17)]
+    step = Step(dtype, lengths, m, 5, group, dim, 16, dim, padding=1)
+    if rising:
+        slot = step.allowed()[1]
+        step.queries.abs_()
+        for i, n in enumerate(lengths):
+            s = slot[i, :n + m]
+            rise = torch.linspace(0.0, 40.0 / dim ** 0.5, n + m, device="cuda")
+            step.keys[s // 16, s % 16] = (step.keys[s // 16, s % 16].float() * 0.1 + rise[:, None, None]).to(dtype)
+    check(step)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_values_that_are_no_numbers_beside_sums_that_were_set_aside(dtype):
+    """In the tiles around a turn, of a sequence's last tokens and of drafted ones that only some rows see."""
+    for m, group, dim in ((3, 4, 128), (20, 8, 64), (9, 4, 256)):
+        lengths = [64 * tiles - 20 for tiles in (17, 33, 49, 65)] * 20
+        step = Step(dtype, lengths, m, 3, group, dim, 16, padding=1, spread=0.1)
+        seen, slot, _ = step.allowed()
+        touched = torch.zeros_like(step.positions, dtype=torch.bool)
+        for i, n in enumerate(lengths):
+            if i % 3 == 0:
+                step.values[slot[i, n + 1] // 16, slot[i, n + 1] % 16] = math.inf
+                touched[i] = seen[i, :, n + 1]
+        exact, exact_lse, off, lse_off = step.exact()
+        out, lse = step.call()
+        none = step.positions < 0
+        clean = ~touched & ~none
+        assert touched.any() and clean.any() and (out[none] == 0).all() and not out[touched].isfinite().any()
+        assert ((out[clean].double() - exact[clean]).abs() <= off[clean]).all()
+        assert ((lse[~none].double() - exact_lse[~none]).abs() <= lse_off[~none]).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_sums_set_aside_in_calls_of_several_streams_and_graphs(dtype):
+    """Calls of one handle at a time on several streams, and captured ones, each with room of its own for what it sets aside."""
+    steps = [Step(dtype, [30_000 + 7000 * i] * 2, 40, 1, 8, 128, 16, i) for i in range(3)]
+    want = [s.call() for s in steps]
+    graphs = []
+    for s in steps:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = s.call(sync=False)
+        graphs.append((graph, got))
+    streams = [torch.cuda.Stream() for _ in range(6)]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        live = []
+        for i in range(3):
+            with torch.cuda.stream(streams[i]):
+                live.append(steps[i].call(sync=False))
+            with torch.cuda.stream(streams[3 + i]):
+                graphs[i][0].replay()
+        torch.cuda.synchronize()
+        for i in range(3):
+            assert all(torch.equal(a, b) for a, b in zip(live[i], want[i]))
+            assert all(torch.equal(a, b) for a, b in zip(graphs[i][1], want[i]))
