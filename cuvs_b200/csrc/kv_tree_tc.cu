@@ -450,6 +450,7 @@ __device__ __forceinline__ void add_sums_aside(float4* aside, uint32_t sums, uin
       y[q] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       if (some && (i * 8 + q) * 4 < dim) { y[q] = aside[(i * 8 + q) * kRows]; }
     }
+    __syncwarp();  // (rows that are none ask for nothing; a load from tensor memory is of the whole warp)
     uint32_t o[32];
     tmem_ld32(sums + i * 32, o);
 #pragma unroll
@@ -720,6 +721,7 @@ __device__ __forceinline__ void softmax_role(const tc_args& a, tc_shared& sh, ch
             if (top == -INFINITY) { x = make_float4(0.0f, 0.0f, 0.0f, 0.0f); }
             write(i * 8 + q, x, scale);
           }
+          __syncwarp();
         }
         finish(top, sum);
       }
